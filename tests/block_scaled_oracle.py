@@ -1,0 +1,91 @@
+"""The definition of 8-bit block-scaled rows and products in 64 bits, for the tests (any device)."""
+from __future__ import annotations
+
+import torch
+
+BLOCK = 128
+
+
+def random_matrix(n, k, seed, device="cpu", sizes=(0.02, 3.0)):
+    """Codes over the whole range of e4m3 (zeros and its subnormal numbers among them) and scales of different sizes."""
+    from torchinferno_b200.kernels.block_scaled import BlockScaledMatrix
+    g = torch.Generator().manual_seed(seed)
+    codes = (torch.randn(n, k, generator=g) * 60).clamp(-448, 448)
+    codes[torch.rand(n, k, generator=g) < 0.05] *= 1e-4
+    scales = torch.empty(-(-n // BLOCK), -(-k // BLOCK)).uniform_(*sizes, generator=g) / 60
+    return BlockScaledMatrix(codes.to(torch.float8_e4m3fn).to(device), scales.to(device))
+
+
+def matrix64(matrix):
+    n, k = matrix.shape
+    at_n, at_k = torch.arange(n, device=matrix.device) // BLOCK, torch.arange(k, device=matrix.device) // BLOCK
+    return matrix.codes.to(torch.float32).double() * matrix.scales.double()[at_n][:, at_k]
+
+
+def rows64(x):
+    """(codes, scales) of rows by the definition; every power of two comes from a table, every border from a comparison."""
+    rows, k = x.shape
+    x = x.double()
+    powers = torch.tensor([2.0 ** p for p in range(-126, 129)], dtype=torch.float64, device=x.device)
+    binades = torch.tensor([2.0 ** p for p in range(-6, 10)], dtype=torch.float64, device=x.device)
+    codes, scales = torch.empty_like(x), torch.empty(rows, -(-k // BLOCK), dtype=torch.float64, device=x.device)
+    for b in range(scales.shape[1]):
+        part = x[:, b * BLOCK:(b + 1) * BLOCK]
+        largest = part.abs().max(1).values
+        at = (448.0 * powers[None] < largest[:, None]).sum(1).clamp(max=len(powers) - 1)
+        s = torch.where(largest == 0, 1.0, powers[at])
+        s = torch.where(torch.isfinite(part).all(1), s, torch.nan)
+        scales[:, b] = s
+        v = part / s[:, None]
+        step = binades[((binades[None, None] <= v.abs()[..., None]).sum(-1) - 1).clamp(min=0)] / 8
+        codes[:, b * BLOCK:(b + 1) * BLOCK] = torch.round(v / step) * step
+    return codes, scales
+
+
+def widened_rows64(x):
+    codes, scales = rows64(x)
+    return codes * scales[:, torch.arange(x.shape[1], device=x.device) // BLOCK]
+
+
+def product64(x, matrix):
+    """(the product in 64 bits, a bound of what 32-bit sums may be off by).  A sum of 128 products of codes (each exact in 32 bits) and of the
+    runs' shares rounds at most 128 + 2 runs + 2 times, each time by at most a step of 2^-23 of what has been summed."""
+    rows, w = widened_rows64(x), matrix64(matrix)
+    runs = -(-x.shape[1] // BLOCK)
+    return rows @ w.t(), (BLOCK + 2 * runs + 2) * 2.0 ** -23 * (rows.abs() @ w.abs().t())
+
+
+def gated64(gate, up, act="swiglu", limit=7.0, alpha=1.702):
+    """(value, bound) of a gated unit of two (value, bound) pairs; g sigmoid(g) and its clamped form have slopes of at most 1.1."""
+    (g, eg), (u, eu) = gate, up
+    if act == "glu_clamp":
+        g, u = g.clamp(max=limit), u.clamp(-limit, limit) + 1
+    else:
+        alpha = 1.0
+    s = g * torch.sigmoid(alpha * g)
+    y = s * u
+    # (the exponential, the quotient and two products in 32 bits: 8 roundings, the exponential's argument among them)
+    return y, 1.1 * eg * (u.abs() + eu) + s.abs() * eu + 8 * 2.0 ** -23 * (1 + (alpha * g).abs()) * y.abs() + 2.0 ** -126
+
+
+def act64(value, act):
+    v, e = value
+    if act == "relu2":
+        r = v.clamp(min=0)
+        return r * r, 2 * r * e + e * e + 2.0 ** -23 * r * r
+    if act == "silu":
+        return gated64(value, (torch.ones_like(v), torch.zeros_like(v)))
+    if act == "gelu":
+        y = 0.5 * v * (1 + torch.erf(v * 0.5 ** 0.5))
+        return y, 1.2 * e + 8 * 2.0 ** -23 * v.abs() + 2.0 ** -126
+    return v, e
+
+
+def check(got, value, out_dtype, what=""):
+    """``got`` within the bound of the sums and half a step of its own type (bf16: 2^-8 of the value)."""
+    want, bound = value
+    bound = bound + (2.0 ** -8 * (want.abs() + bound) if out_dtype == torch.bfloat16 else 0.0)
+    assert got.dtype == out_dtype and got.shape == want.shape
+    off = (got.double() - want).abs()
+    bad = ~(off <= bound)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((off / bound.clamp(min=1e-300)).nan_to_num(9e9).max()):.2f} of the bound"

@@ -1,0 +1,318 @@
+"""Products of 8-bit block-scaled weights on the GPU against the definition in 64 bits (tests/block_scaled_oracle.py)."""
+import pytest
+import torch
+
+from block_scaled_oracle import act64, check, gated64, matrix64, product64, random_matrix, rows64, widened_rows64
+from gpu_common import need_gpu
+from torchinferno_b200.kernels import gemm, ops
+from torchinferno_b200.kernels.block_scaled import BlockScaledExperts, BlockScaledMatrix, BlockScaledWeight, quantize_rows
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def rows(m, k, seed, dtype=BF16, spread=2.0):
+    g = torch.Generator().manual_seed(1000 + seed)
+    x = torch.randn(m, k, generator=g) * (spread * torch.randn(m, 1, generator=g)).exp() * (torch.randn(1, k, generator=g)).exp()
+    return x.to(dtype).to(DEV)
+
+
+def error_word():
+    return torch.zeros(1, dtype=torch.int32, device=DEV)
+
+
+# ------------------------------------------------------------------------------------------------ rows to codes
+def same_codes(x):
+    codes, scales = quantize_rows(x)
+    want_codes, want_scales = rows64(x)
+    assert codes.shape == x.shape and scales.shape == want_scales.shape and codes.dtype == torch.float8_e4m3fn
+    assert torch.equal(scales.double().nan_to_num(-1.0), want_scales.nan_to_num(-1.0))
+    assert torch.equal(codes.double().nan_to_num(-1e9), want_codes.nan_to_num(-1e9))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m, k", [(1, 1), (1, 128), (3, 16), (8, 4096), (9, 129), (17, 127), (64, 520), (130, 1000), (5, 2055), (33, 15)])
+def test_rows_become_codes(m, k, dtype):
+    need_gpu()
+    same_codes(rows(m, k, m + k, dtype))
+
+
+def test_every_bf16_value_beside_every_border():
+    """All finite bf16 numbers of a sign change pattern, run after run of one size: scales over the whole range of exponents, borders of
+    448 * 2^p included."""
+    need_gpu()
+    bits = torch.arange(0x7f80, dtype=torch.int32)
+    x = (bits << 16).view(F32)[:0x7f80 // 128 * 128].view(-1, 128)
+    x = x * torch.where(torch.arange(128) % 3 == 0, -1.0, 1.0)
+    same_codes(x.to(BF16).to(DEV))
+    edges = torch.stack([torch.full((128,), 448.0 * 2.0 ** p) for p in range(-130, 119)])
+    for factor in (1.0, 1 + 2.0 ** -7, 1 - 2.0 ** -8):
+        same_codes((edges * factor).to(BF16).to(DEV))
+    same_codes((edges * (1 + 2.0 ** -23)).to(DEV))
+
+
+def test_rows_of_any_stride_and_alignment():
+    need_gpu()
+    wide = rows(20, 1500, 3)
+    same_codes(wide[:, 8:8 + 600])
+    same_codes(wide[:, 3:3 + 601])
+    same_codes(wide[::3, 1:130])
+    same_codes(rows(40, 777, 4, F32)[1::2, 5:5 + 300])
+    one = rows(1, 300, 5).expand(6, 300)
+    same_codes(one)
+
+
+def test_runs_that_are_empty_or_not_finite():
+    need_gpu()
+    x = rows(6, 400, 7, F32)
+    x[0] = 0
+    x[1, 130] = float("inf")
+    x[2, 5] = float("nan")
+    x[3, 399] = -float("inf")
+    x[4] = 1e-42                    # subnormal numbers
+    x[5, :128] = 3e38
+    same_codes(x)
+    same_codes(x[:4].to(BF16))
+    assert quantize_rows(x[:0])[0].shape == (0, 400)
+
+
+# ------------------------------------------------------------------------------------------------ one matrix
+SIZES = [(1, 1, 1), (1, 128, 128), (1, 4096, 512), (2, 129, 130), (7, 256, 127), (8, 1000, 1302), (15, 300, 257), (16, 2048, 384), (17, 640, 129),
+         (32, 384, 2), (33, 127, 640), (47, 1152, 200), (63, 512, 1000), (64, 4096, 256), (65, 200, 129), (96, 1024, 512), (127, 400, 300), (128, 128, 128),
+         (129, 2304, 136), (200, 512, 2560), (255, 1000, 258), (256, 256, 512), (257, 384, 770), (333, 1000, 1302), (520, 2048, 1280), (1030, 640, 390)]
+
+
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("m, k, n", SIZES)
+def test_linear(m, k, n, out_dtype):
+    need_gpu()
+    matrix, x, word = random_matrix(n, k, m + n, DEV), rows(m, k, m), error_word()
+    gemm.set_error_word(word)
+    try:
+        got = gemm.linear(x, BlockScaledWeight(matrix), out_dtype=out_dtype)
+    finally:
+        gemm.set_error_word(None)
+    check(got, product64(x, matrix), out_dtype)
+    assert int(word) == 0
+
+
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("m, k, n", [(1, 128, 1), (1, 4096, 1024), (3, 200, 130), (8, 1024, 257), (16, 2048, 640), (31, 500, 64), (64, 1024, 129), (65, 384, 130),
+                                     (130, 1000, 300), (256, 512, 256), (300, 2048, 513), (700, 256, 1000)])
+def test_linear_swiglu(m, k, n, out_dtype):
+    need_gpu()
+    gate, up = random_matrix(n, k, 1, DEV, (0.005, 0.2)), random_matrix(n, k, 2, DEV, (0.005, 0.2))
+    x, weight = rows(m, k, m, spread=0.5), BlockScaledWeight(gate, up, epilogue="swiglu")
+    check(gemm.linear_swiglu(x, weight, out_dtype=out_dtype), gated64(product64(x, gate), product64(x, up)), out_dtype)
+    # (and without the activation: the two products side by side, row pairs)
+    both = gemm.linear(x, weight, out_dtype=F32)
+    for part, matrix in ((0, gate), (1, up)):
+        check(both[:, part::2].contiguous(), product64(x, matrix), F32)
+
+
+@pytest.mark.parametrize("m", [1, 20, 90, 300])
+def test_32_bit_rows(m):
+    need_gpu()
+    matrix, x = random_matrix(260, 520, 5, DEV), rows(m, 520, m, F32)
+    check(gemm.linear(x, BlockScaledWeight(matrix)), product64(x, matrix), F32)
+    check(gemm.linear(x, BlockScaledWeight(matrix), out_dtype=BF16), product64(x, matrix), BF16)
+
+
+@pytest.mark.parametrize("m", [1, 5, 64, 65, 140, 600])
+def test_several_matrices_side_by_side(m):
+    """Those whose rows end inside a block among them; into a slice of wider rows, whose other columns stay as they are."""
+    need_gpu()
+    parts = [random_matrix(n, 333, n, DEV) for n in (256, 130, 64, 1, 200)]
+    weight, x = BlockScaledWeight(*parts), rows(m, 333, m)
+    total = sum(p.shape[0] for p in parts)
+    wide = torch.full((m, total + 7), 5.0, dtype=BF16, device=DEV)
+    got = gemm.linear(x, weight, out=wide[:, 3:3 + total])
+    assert got.data_ptr() == wide[:, 3:].data_ptr() and (wide[:, :3] == 5).all() and (wide[:, 3 + total:] == 5).all()
+    want, bound = (torch.cat(t, 1) for t in zip(*(product64(x, p) for p in parts)))
+    check(got, (want, bound), BF16)
+    check(gemm.linear(x, weight.rows(128, 400)), (want[:, 128:400], bound[:, 128:400]), BF16)
+
+
+@pytest.mark.parametrize("m", [4, 70, 300])
+def test_strided_and_unaligned_rows(m):
+    need_gpu()
+    matrix, wide = random_matrix(200, 301, 5, DEV), rows(2 * m, 1000, m)
+    for x in (wide[:m, 8:309], wide[:m, 3:304], wide[::2, 1:302], wide[:1, 16:317].expand(m, 301)):
+        check(gemm.linear(x, BlockScaledWeight(matrix)), product64(x, matrix), BF16)
+
+
+@pytest.mark.parametrize("m", [3, 64, 100, 400])
+def test_rows_of_zeros_and_not_finite(m):
+    """Rows of zeros give zeros; an infinity or a NaN makes its own row NaN and no other; NaN codes and scales their own features."""
+    need_gpu()
+    matrix, x = random_matrix(150, 300, 9, DEV), rows(m, 300, 1)
+    x[0] = 0
+    weight = BlockScaledWeight(matrix)
+    clean = gemm.linear(x, weight)
+    assert not clean[0].any()
+    x[1, 290], x[2, 0] = float("inf"), float("nan")
+    got = gemm.linear(x, weight)
+    assert got[1:3].isnan().all() and torch.equal(got[3:], clean[3:]) and torch.equal(got[0], clean[0])
+    codes, scales = matrix.codes.clone(), matrix.scales.clone()
+    codes.view(torch.uint8)[7, 11] = 0x7f
+    scales[1, 0] = float("nan")
+    got = gemm.linear(x[3:] if m > 3 else x[:1], BlockScaledWeight(BlockScaledMatrix(codes, scales)))
+    assert got[:, 7].isnan().all() and got[:, 128:].isnan().all() and not got[:, :7].isnan().any() and not got[:, 8:128].isnan().any()
+
+
+@pytest.mark.parametrize("m", [2, 66, 260])
+def test_sizes_at_the_ends_of_the_range(m):
+    need_gpu()
+    matrix = random_matrix(140, 256, 3, DEV, (1.0, 1.0))
+    for size in (2.0 ** -100, 2.0 ** 90):
+        x = (rows(m, 256, 1, F32, 0.1) * size).to(BF16)
+        got, (want, bound) = gemm.linear(x, BlockScaledWeight(matrix), out_dtype=F32), product64(x, matrix)
+        check(got / size, (want / size, bound / size), F32)
+
+
+def test_no_rows():
+    need_gpu()
+    weight = BlockScaledWeight(random_matrix(100, 200, 1, DEV))
+    assert gemm.linear(rows(0, 200, 1), weight).shape == (0, 100)
+
+
+def test_refusals():
+    need_gpu()
+    weight, x = BlockScaledWeight(random_matrix(100, 200, 1, DEV)), rows(4, 200, 1)
+    gated = BlockScaledWeight(random_matrix(100, 200, 1, DEV), random_matrix(100, 200, 2, DEV), epilogue="swiglu")
+    for call in (lambda: gemm.linear(x[:, :199], weight), lambda: gemm.linear(x.half(), weight), lambda: gemm.linear(x, weight, out_dtype=torch.float16),
+                 lambda: gemm.linear(x.t().contiguous().t(), weight), lambda: gemm.linear(x[0], weight), lambda: gemm.linear_swiglu(x, weight),
+                 lambda: gemm.linear(x, weight, out=torch.empty(4, 99, dtype=BF16, device=DEV)), lambda: gemm.linear_swiglu(x.cpu(), gated),
+                 lambda: gemm.linear(x, weight, out=torch.empty(100, 4, dtype=BF16, device=DEV).t()),
+                 lambda: gemm.linear(x, BlockScaledWeight(random_matrix(100, 200, 1)))):
+        with pytest.raises(ops.KernelError):
+            call()
+
+
+@pytest.mark.parametrize("m", [1, 8, 64, 100, 300])
+def test_a_row_does_not_depend_on_the_others(m):
+    """In a step of the same kernel: the same bits wherever a row stands, and from call to call."""
+    need_gpu()
+    weight, x = BlockScaledWeight(random_matrix(390, 1100, 3, DEV)), rows(m, 1100, 2)
+    first = gemm.linear(x, weight)
+    assert torch.equal(first, gemm.linear(x, weight))
+    turned = torch.roll(x, 1, 0)
+    assert torch.equal(torch.roll(first, 1, 0), gemm.linear(turned, weight))
+
+
+@pytest.mark.parametrize("m", [3, 100, 300])
+def test_captured_and_on_two_streams(m):
+    need_gpu()
+    gate, up, down = random_matrix(260, 400, 1, DEV, (0.01, 0.1)), random_matrix(260, 400, 2, DEV, (0.01, 0.1)), random_matrix(400, 260, 3, DEV)
+    w1, w2 = BlockScaledWeight(gate, up, epilogue="swiglu"), BlockScaledWeight(down)
+    inputs = [rows(m, 400, i) for i in range(4)]
+
+    def pass_of(x):
+        return gemm.linear(gemm.linear_swiglu(x, w1), w2)
+    want = [pass_of(x) for x in inputs]
+    torch.cuda.synchronize()
+    graphs, statics = [], []
+    for i in range(2):                         # (two captured passes, replayed side by side: they share nothing but the weights)
+        x = inputs[i].clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = pass_of(x)
+        graphs.append(graph), statics.append((x, y))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for turn in range(8):
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                statics[i][0].copy_(inputs[(turn + i) % 4])
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(statics[i][1], want[(turn + i) % 4])
+    outs = []
+    for turn in range(6):
+        with torch.cuda.stream(streams[turn % 2]):
+            outs.append(pass_of(inputs[turn % 4]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[turn % 4]) for turn, y in enumerate(outs))
+
+
+# ------------------------------------------------------------------------------------------------ rows sorted by expert
+def routing(tokens, top, experts, seed, empty=(), absent=0):
+    """offsets, order, and ids of pairs sorted by expert; experts in ``empty`` get none; ``absent`` pairs at the end have no expert at all."""
+    g = torch.Generator().manual_seed(seed)
+    allowed = [e for e in range(experts) if e not in empty]
+    ids = torch.tensor([allowed[i] for i in torch.randint(0, len(allowed), (tokens * top,), generator=g).tolist()])
+    if absent:
+        ids[torch.randperm(len(ids), generator=g)[:absent]] = experts
+    order = torch.sort(ids, stable=True).indices.to(torch.int32)
+    counts = torch.bincount(ids, minlength=experts + 1)[:experts]
+    offsets = torch.cat([counts.new_zeros(1), counts.cumsum(0)]).to(torch.int32)
+    return offsets.to(DEV), order.to(DEV), ids
+
+
+@pytest.mark.parametrize("act", ["none", "relu2", "silu", "gelu", "swiglu", "glu_clamp"])
+@pytest.mark.parametrize("by_pair", [True, False])
+@pytest.mark.parametrize("tokens, top, experts, k, n, out_dtype", [
+    (1, 1, 1, 128, 128, F32), (1, 4, 8, 256, 96, BF16), (8, 4, 32, 1024, 256, BF16), (5, 3, 7, 200, 130, F32), (40, 2, 6, 640, 129, BF16),
+    (100, 3, 5, 300, 200, F32), (150, 4, 4, 512, 256, BF16), (700, 2, 3, 200, 140, BF16), (64, 1, 300, 128, 64, F32)])
+def test_expert_products(tokens, top, experts, k, n, out_dtype, by_pair, act):
+    need_gpu()
+    gated = act in ops.MOE_GATED
+    sizes = (0.005, 0.2) if act != "none" else (0.02, 3.0)
+    stacks = [[random_matrix(n, k, 100 * part + e, DEV, sizes) for e in range(min(experts, 6))] for part in range(2 if gated else 1)]
+    stacks = [[stack[e % len(stack)] for e in range(experts)] for stack in stacks]
+    empty = (0, experts - 1) if experts > 3 else ()
+    pairs, absent = tokens * top, tokens if tokens * top > 8 else 0
+    offsets, order, ids = routing(tokens, top, experts, tokens, empty, absent)
+    x = rows(tokens if by_pair else pairs, k, tokens, spread=0.5)
+    scale = torch.rand(pairs, generator=torch.Generator().manual_seed(1)).to(DEV) + 0.5 if act in ("glu_clamp", "none") else None
+    y = torch.full((pairs, n), 9.0, dtype=out_dtype, device=DEV)
+    word = error_word()
+    assert ops.moe_expert_product(x, BlockScaledExperts(*stacks), y, offsets, order, top, x_by_pair=by_pair, act=act, limit=2.0, alpha=1.702,
+                                  row_scale=scale, error_word=word) is y
+    assert int(word) == 0
+    ends = offsets.tolist()
+    assert (y[ends[-1]:] == 9).all()                                 # (rows behind the last expert's: left as they were)
+    for e in range(experts):
+        at = torch.arange(ends[e], ends[e + 1], device=DEV)
+        if len(at) == 0:
+            continue
+        source = order[at].long() // top if by_pair else at
+        sums = [product64(x[source], stack[e]) for stack in stacks]
+        if scale is not None:
+            s = scale[order[at].long()].double()[:, None]
+            sums = [(v * s, b * s + 2.0 ** -23 * (v * s).abs()) for v, b in sums]
+        want = gated64(*sums, act=act, limit=2.0) if gated else act64(sums[0], act)
+        check(y[at], want, out_dtype, f"expert {e}")
+
+
+def test_expert_refusals():
+    need_gpu()
+    experts = BlockScaledExperts([random_matrix(64, 100, i, DEV) for i in range(4)])
+    offsets, order, _ = routing(6, 2, 4, 0)
+    x, y = rows(6, 100, 0), torch.empty(12, 64, dtype=BF16, device=DEV)
+    good = dict(x_by_pair=True)
+    ops.moe_expert_product(x, experts, y, offsets, order, 2, **good)
+    for call in (lambda: ops.moe_expert_product(x, experts, y, offsets, order, 2, x_by_pair=False),               # rows by pair, not by token
+                 lambda: ops.moe_expert_product(x, experts, y, offsets, order, 2, act="swiglu", **good),          # no gate rows
+                 lambda: ops.moe_expert_product(x, experts, y, offsets, order, 2, act="tanh", **good),
+                 lambda: ops.moe_expert_product(x, experts, y, offsets, order, 1, **good),                        # more sources than rows
+                 lambda: ops.moe_expert_product(x, experts, y, offsets, order, 0, **good),
+                 lambda: ops.moe_expert_product(x[:, :99], experts, y, offsets, order, 2, **good),
+                 lambda: ops.moe_expert_product(x, experts, y[:11], offsets, order, 2, **good),
+                 lambda: ops.moe_expert_product(x, experts, y, offsets[:4], order, 2, **good),
+                 lambda: ops.moe_expert_product(x, experts, y, offsets, order.long(), 2, **good),
+                 lambda: ops.moe_expert_product(x, experts, y, offsets.cpu(), order, 2, **good),
+                 lambda: ops.moe_expert_product(x, experts, y, offsets, order, 2, row_scale=torch.ones(5, device=DEV), **good)):
+        with pytest.raises(ops.KernelError):
+            call()
+
+
+def test_the_definition_by_itself():
+    """The oracle's rows and matrices are what the tensors stand for (torch's own widening of e4m3)."""
+    need_gpu()
+    m, x = random_matrix(130, 200, 0, DEV), rows(9, 200, 1)
+    assert torch.equal(m.widened(torch.float32).double(), matrix64(m).float().double())
+    codes, scales = quantize_rows(x)
+    assert torch.equal(widened_rows64(x), codes.double() * scales.double().repeat_interleave(128, 1)[:, :200])

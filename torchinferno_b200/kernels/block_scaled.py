@@ -1,0 +1,252 @@
+"""8-bit weights with a scale for each block of 128 x 128, and the products of rows with them.
+
+A matrix [N, K] is held as e4m3 codes with one fp32 scale S for each block of 128 x 128 (the last ones may be short): number (n, k)
+stands for code(n, k) * S[n // 128, k // 128].  The rows x [M, K] of a product are quantised on the way: run b of 128
+columns of a row, with the largest absolute value a, has the scale s = 2^p, p the smallest integer (at least -126) with
+a * 2^-p <= 448 (1 where a is 0), and its codes are x / s rounded to e4m3, to nearest and ties to even.  Then
+
+    y[m, n] = sum over b of s[m, b] * S[n // 128, b] * (sum over run b of code_x[m, k] * code_w[n, k])
+
+with 32-bit sums and one rounding of y at the end.  (A power of two as a run's scale: it divides without rounding, and e4m3 being a float format
+it has the same relative precision anywhere in its range.)  A run that holds an infinity or a NaN makes its whole output row NaN.
+
+There is no backward pass: this is an inference engine's weight format.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Sequence
+
+import torch
+
+from torchinferno_b200.kernels import ops
+
+BLOCK = 128
+CODE_DTYPE = torch.float8_e4m3fn
+
+
+def blocks(count: int) -> int:
+    return -(-count // BLOCK)
+
+
+@dataclass(frozen=True)
+class BlockScaledMatrix:
+    """A matrix as a checkpoint stores it: ``codes`` [N, K] in e4m3 and ``scales`` [blocks of N, blocks of K] in fp32."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    def __post_init__(self) -> None:
+        if self.codes.dtype != CODE_DTYPE or self.codes.dim() != 2 or 0 in self.codes.shape:
+            raise ValueError(f"codes must be a non-empty 2-D tensor of {CODE_DTYPE}, got {self.codes.dtype} {tuple(self.codes.shape)}")
+        wanted = tuple(blocks(d) for d in self.codes.shape)
+        if self.scales.dtype != torch.float32 or tuple(self.scales.shape) != wanted:
+            raise ValueError(f"scales of a {tuple(self.codes.shape)} matrix must be float32 {wanted}, got {self.scales.dtype} {tuple(self.scales.shape)}")
+        if self.codes.device != self.scales.device:
+            raise ValueError(f"codes are on {self.codes.device}, scales on {self.scales.device}")
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def to(self, device: torch.device | str) -> "BlockScaledMatrix":
+        return BlockScaledMatrix(self.codes.to(device), self.scales.to(device))
+
+    def widened(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The numbers the matrix stands for (on any device)."""
+        n, k = self.codes.shape
+        scales = self.scales.repeat_interleave(BLOCK, 0)[:n].repeat_interleave(BLOCK, 1)[:, :k]
+        return (self.codes.to(torch.float32) * scales).to(dtype)
+
+
+def quantize_matrix(matrix: torch.Tensor) -> BlockScaledMatrix:
+    """The e4m3 form of ``matrix`` [N, K]: a block's scale is its largest absolute value / 448 (1 for a block of zeros)."""
+    if matrix.dim() != 2 or 0 in matrix.shape:
+        raise ValueError(f"quantize_matrix takes a non-empty matrix, got {tuple(matrix.shape)}")
+    n, k = matrix.shape
+    tiles = torch.nn.functional.pad(matrix.to(torch.float32), (0, -k % BLOCK, 0, -n % BLOCK)).view(blocks(n), BLOCK, blocks(k), BLOCK)
+    scales = tiles.abs().amax((1, 3)) / 448.0
+    scales = torch.where(scales == 0, 1.0, scales).clamp(min=torch.finfo(torch.float32).tiny)
+    codes = (tiles / scales[:, None, :, None]).clamp(-448.0, 448.0).view(blocks(n) * BLOCK, -1)[:n, :k]
+    return BlockScaledMatrix(codes.to(CODE_DTYPE).contiguous(), scales.contiguous())
+
+
+def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes [M, K], scales [M, runs of 128]) of the rows ``x`` [M, K] (bfloat16 or float32, any row stride); see the module's text."""
+    codes, scales = _quantized(x)
+    return codes[:, :x.shape[1]], scales[:, :x.shape[0]].t()
+
+
+def _quantized(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes and scales as the products read them: columns padded to whole runs; a run's scales side by side, rows rounded up to 4."""
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ops.KernelError(f"rows to quantise must be [rows, columns], got {tuple(x.shape)}")
+    rows, runs = x.shape[0], blocks(x.shape[1])
+    codes = torch.empty((rows, runs * BLOCK), dtype=CODE_DTYPE, device=x.device)
+    scales = torch.empty((runs, -(-rows // 4) * 4), dtype=torch.float32, device=x.device)
+    ops.quantize_rows(x, codes, scales)
+    return codes, scales
+
+
+def _laid_out(matrices: Sequence[BlockScaledMatrix], ups: Sequence[BlockScaledMatrix] | None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes [matrices, N, K rounded up to 128] and scales [matrices, blocks of N, blocks of K] of equally large matrices; with ``ups``
+    the rows of either alternate (gate i, up i; gate block j, up block j)."""
+    shape, device = matrices[0].shape, matrices[0].device
+    for m in [*matrices, *(ups or ())]:
+        if m.shape != shape or m.device != device:
+            raise ValueError(f"matrices of one weight must be alike: {tuple(m.shape)} on {m.device}, {tuple(shape)} on {device}")
+    if ups is not None and len(ups) != len(matrices):
+        raise ValueError(f"{len(matrices)} gate and {len(ups)} up matrices")
+    n, k = shape
+    parts = 1 if ups is None else 2
+    codes = torch.zeros((len(matrices), n, parts, blocks(k) * BLOCK), dtype=torch.uint8, device=device)      # (columns behind K: zero codes)
+    scales = torch.empty((len(matrices), blocks(n), parts, blocks(k)), dtype=torch.float32, device=device)
+    for part, stack in enumerate((matrices,) if ups is None else (matrices, ups)):
+        for i, m in enumerate(stack):
+            codes[i, :, part, :k] = m.codes.view(torch.uint8)
+            scales[i, :, part] = m.scales
+    return codes.view(CODE_DTYPE).view(len(matrices), n * parts, -1), scales.view(len(matrices), blocks(n) * parts, -1)
+
+
+class BlockScaledWeight:
+    """A projection of 8-bit blocks, laid out for the kernels.  ``BlockScaledWeight(matrix)``; several matrices over the same columns
+    (``BlockScaledWeight(q, k, v)``) give their outputs side by side; ``BlockScaledWeight(gate, up, epilogue="swiglu")`` is what
+    :func:`gemm.linear_swiglu` takes."""
+
+    def __init__(self, *matrices: BlockScaledMatrix, epilogue: str = "none") -> None:
+        if epilogue not in ("none", "swiglu"):
+            raise ValueError(f"unknown epilogue {epilogue!r}")
+        if not matrices or any(not isinstance(m, BlockScaledMatrix) for m in matrices):
+            raise ValueError("a block-scaled weight is made of block-scaled matrices")
+        if epilogue == "swiglu" and len(matrices) != 2:
+            raise ValueError("the swiglu epilogue takes a gate and an up matrix")
+        if any(m.shape[1] != matrices[0].shape[1] or m.device != matrices[0].device for m in matrices):
+            raise ValueError("the matrices of a weight need the same columns and device")
+        self.epilogue, self.in_features = epilogue, matrices[0].shape[1]
+        self.out_features = sum(m.shape[0] for m in matrices)
+        # (first output, codes, scales) of every product to run.  Matrices are put together while the ones before end with a whole block;
+        # where one does not, its blocks' borders would not be the joint matrix's: it starts a product of its own.
+        self.parts: list[tuple[int, torch.Tensor, torch.Tensor]] = []
+        if epilogue == "swiglu":
+            self.parts.append((0, *_laid_out(matrices[:1], matrices[1:])))
+            return
+        first, run = 0, []
+        for i, m in enumerate(matrices):
+            run.append(m)
+            if m.shape[0] % BLOCK or i == len(matrices) - 1:
+                joint = run[0] if len(run) == 1 else BlockScaledMatrix(
+                    torch.cat([r.codes.view(torch.uint8) for r in run]).view(CODE_DTYPE), torch.cat([r.scales for r in run]))
+                self.parts.append((first, *_laid_out([joint], None)))
+                first, run = first + joint.shape[0], []
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return CODE_DTYPE
+
+    @property
+    def device(self) -> torch.device:
+        return self.parts[0][1].device
+
+    def nbytes(self) -> int:
+        return sum(codes.numel() + 4 * scales.numel() for _, codes, scales in self.parts)
+
+    def rows(self, start: int, stop: int) -> "BlockScaledWeight":
+        """The projection onto output features start .. stop-1 (views; ``start`` a whole number of blocks into its matrix)."""
+        if self.epilogue != "none" or not 0 <= start < stop <= self.out_features:
+            raise ValueError(f"no features {start} .. {stop - 1} of {self.out_features} to take")
+        view = object.__new__(BlockScaledWeight)
+        view.epilogue, view.in_features, view.out_features, view.parts = "none", self.in_features, stop - start, []
+        for first, codes, scales in self.parts:
+            lo, hi = max(start - first, 0), min(stop - first, codes.shape[1])
+            if lo < hi:
+                if lo % BLOCK:
+                    raise ValueError(f"feature {start} lies inside a block")
+                view.parts.append((first + lo - start, codes[:, lo:hi], scales[:, lo // BLOCK:blocks(hi)]))
+        return view
+
+    def _checked(self, x: torch.Tensor, out_dtype: torch.dtype | None, width: int, out: torch.Tensor | None) -> torch.Tensor:
+        """The tensor that the product is written to."""
+        if x.dim() != 2 or x.shape[1] != self.in_features:
+            raise ops.KernelError(f"linear: shapes {tuple(x.shape)} and {(self.out_features, self.in_features)} do not fit")
+        if not x.is_cuda:
+            raise ops.KernelError("linear: operands must be CUDA tensors (there is no CPU path)")
+        if x.device != self.device:
+            raise ops.KernelError(f"linear: x is on {x.device}, the weight on {self.device}")
+        out_dtype = out_dtype or x.dtype
+        if out_dtype not in (torch.bfloat16, torch.float32):
+            raise ops.KernelError(f"linear: unsupported output dtype {out_dtype}")
+        if out is None or out.dtype != out_dtype:
+            return torch.empty((x.shape[0], width), dtype=out_dtype, device=x.device)
+        if out.shape != (x.shape[0], width) or out.stride(1) != 1 or out.device != x.device:
+            raise ops.KernelError(f"linear: out is {tuple(out.shape)}, wanted {(x.shape[0], width)} with unit inner stride on {x.device}")
+        return out
+
+    def product(self, x: torch.Tensor, *, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
+                error_word: torch.Tensor | None = None) -> torch.Tensor:
+        """x [tokens, in] times the weight: [tokens, out] (a swiglu weight's gate and up sums side by side)."""
+        out = self._checked(x, out_dtype, self.out_features, out)
+        if x.shape[0] == 0:
+            return out
+        rows = _quantized(x)
+        for first, codes, scales in self.parts:
+            ops.block_scaled_product(*rows, codes, scales, out[:, first:first + codes.shape[1]], paired=self.epilogue == "swiglu", error_word=error_word)
+        return out
+
+    def swiglu(self, x: torch.Tensor, *, out_dtype: torch.dtype | None = None, error_word: torch.Tensor | None = None) -> torch.Tensor:
+        """silu(gate) * up of the 32-bit sums: [tokens, out / 2]."""
+        if self.epilogue != "swiglu":
+            raise ops.KernelError("linear_swiglu: the weight was not bound with epilogue='swiglu'")
+        out = self._checked(x, out_dtype, self.out_features // 2, None)
+        if x.shape[0] == 0:
+            return out
+        _, codes, scales = self.parts[0]
+        return ops.block_scaled_product(*_quantized(x), codes, scales, out, paired=True, act="swiglu", error_word=error_word)
+
+
+class BlockScaledExperts:
+    """The experts' matrices of one product of a routed feed-forward, all of one size: ``BlockScaledExperts(matrices)``, or
+    ``BlockScaledExperts(gates, ups)`` for a gated unit.  :func:`ops.moe_expert_product` takes it in place of a tensor."""
+
+    def __init__(self, matrices: Sequence[BlockScaledMatrix], ups: Sequence[BlockScaledMatrix] | None = None) -> None:
+        if not matrices:
+            raise ValueError("a product of experts needs at least one")
+        self.paired = ups is not None
+        self.codes, self.scales = _laid_out(matrices, ups)
+        self.experts, self.in_features = len(matrices), matrices[0].shape[1]
+        self.out_features = matrices[0].shape[0] * (2 if self.paired else 1)
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + 4 * self.scales.numel()
+
+    def product(self, x: torch.Tensor, y: torch.Tensor, offsets: torch.Tensor, order: torch.Tensor, top: int, *, x_by_pair: bool,
+                act: str = "none", limit: float = 0.0, alpha: float = 1.0, row_scale: torch.Tensor | None = None,
+                error_word: torch.Tensor | None = None) -> torch.Tensor:
+        """See :func:`ops.moe_expert_product`."""
+        if act not in ops.MOE_ACT:
+            raise ops.KernelError(f"moe_expert_product: unknown activation {act!r}")
+        gated = act in ops.MOE_GATED
+        if gated != self.paired and act != "none":
+            raise ops.KernelError(f"moe_expert_product: activation {act!r} does not fit experts with{'' if self.paired else 'out'} gate and up rows")
+        pairs, width = order.numel(), self.out_features // 2 if gated else self.out_features
+        if (x.dim() != 2 or x.shape[1] != self.in_features or y.shape != (pairs, width) or offsets.numel() != self.experts + 1 or top < 1
+                or (pairs % top if x_by_pair else x.shape[0] < pairs) or (x_by_pair and x.shape[0] < pairs // top)):
+            raise ops.KernelError("moe_expert_product: shapes do not fit")
+        for name, t in (("x", x), ("y", y), ("offsets", offsets), ("order", order)):
+            if not t.is_cuda or t.device != self.device:
+                raise ops.KernelError(f"moe_expert_product: {name} is on {t.device}, the experts on {self.device}")
+        ops._need(offsets, "offsets", torch.int32), ops._need(order, "order", torch.int32)
+        if row_scale is not None:
+            ops._need(row_scale, "row_scale", torch.float32)
+            if row_scale.numel() != pairs:
+                raise ops.KernelError("moe_expert_product: row_scale must hold one factor per pair")
+        if pairs == 0:
+            return y
+        return ops.block_scaled_product(*_quantized(x), self.codes, self.scales, y, paired=self.paired, act=act, limit=limit, alpha=alpha,
+                                        routing=(offsets, order, top, x_by_pair), row_scale=row_scale, error_word=error_word)

@@ -14,6 +14,7 @@ import weakref
 import torch
 
 from torchinferno_b200.kernels import ops
+from torchinferno_b200.kernels.block_scaled import BlockScaledWeight
 
 # Which kernel multiplies bf16 operands:
 #   "auto"     whichever is faster on this GPU.  Many rows go to cuBLAS.  At few rows (decode steps) neither the
@@ -130,9 +131,12 @@ class LinearWeight:
         return self.tensor.numel() * self.tensor.element_size()
 
 
-def linear(x: torch.Tensor, weight: "torch.Tensor | LinearWeight", *, out_dtype: torch.dtype | None = None,
+def linear(x: torch.Tensor, weight: "torch.Tensor | LinearWeight | BlockScaledWeight", *, out_dtype: torch.dtype | None = None,
            out: torch.Tensor | None = None) -> torch.Tensor:
-    """``x``: [tokens, in]; ``weight``: [out, in] (or a :class:`LinearWeight`); returns [tokens, out] in ``out_dtype``."""
+    """``x``: [tokens, in]; ``weight``: [out, in] (or a :class:`LinearWeight`, or a
+    :class:`~torchinferno_b200.kernels.block_scaled.BlockScaledWeight`); returns [tokens, out] in ``out_dtype``."""
+    if isinstance(weight, BlockScaledWeight):
+        return weight.product(x, out_dtype=out_dtype, out=out, error_word=_error_word)
     few_rows = 0
     if isinstance(weight, LinearWeight):
         if weight.transposed:
@@ -158,9 +162,14 @@ def linear(x: torch.Tensor, weight: "torch.Tensor | LinearWeight", *, out_dtype:
     return _linear_bf16(x, weight, out_dtype, out, few_rows)
 
 
-def linear_swiglu(x: torch.Tensor, weight: LinearWeight) -> torch.Tensor:
+def linear_swiglu(x: torch.Tensor, weight: "LinearWeight | BlockScaledWeight", *, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """silu(gate) * up of the product with a weight whose rows are (gate i, up i) pairs: [tokens, out / 2].
-    At few rows the few-rows kernel applies it in its epilogue; else the product is followed by the SwiGLU kernel."""
+    At few rows the few-rows kernel applies it in its epilogue; else the product is followed by the SwiGLU kernel.
+    A block-scaled weight activates its 32-bit sums at any number of rows, and may leave another type than x's."""
+    if isinstance(weight, BlockScaledWeight):
+        return weight.swiglu(x, out_dtype=out_dtype, error_word=_error_word)
+    if out_dtype not in (None, x.dtype):
+        raise ops.KernelError("linear_swiglu: another output type than x's is for block-scaled weights")
     if weight.epilogue != "swiglu":
         raise ops.KernelError("linear_swiglu: the weight was not bound with epilogue='swiglu'")
     m, inter = x.shape[0], weight.out_features // 2

@@ -1192,7 +1192,10 @@ def moe_expert_product(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor, offset
     ``x_by_pair``: the source of sorted row s is token order[s] // top, else row s itself.  ``act="glu_clamp"``: the rows
     of ``w`` are (gate i, up i) pairs and y has N / 2 columns: g * sigmoid(alpha g) * (u + 1) with g = min(g, limit),
     u = clamp(u, -limit, limit); ``act="swiglu"``: silu(g) * u over the same pairs.  ``row_scale``: one fp32 factor per
-    (token, choice) pair, or None."""
+    (token, choice) pair, or None.  ``w`` may also be a :class:`~torchinferno_b200.kernels.block_scaled.BlockScaledExperts`."""
+    if not isinstance(w, torch.Tensor):      # (experts in 8-bit blocks: block_scaled.BlockScaledExperts)
+        return w.product(x, y, offsets, order, top, x_by_pair=x_by_pair, act=act, limit=limit, alpha=alpha, row_scale=row_scale,
+                         error_word=error_word)
     _rows_of(x, "x"), _need(w, "w"), _rows_of(y, "y")
     experts, n, k = w.shape
     pairs = order.numel()
@@ -1248,6 +1251,47 @@ def moe_combine(y: torch.Tensor, place: torch.Tensor, weights: torch.Tensor | No
         _ptr(gate), ld_gate, _ptr(out), _code(out.dtype), n, width, _ptr(ids),
         identity_from, _ptr(x if ids is not None else None), ldx, _stream()))
     return out
+
+
+# ---------------------------------------------------------------------------
+# 8-bit block-scaled operands (csrc/block_scaled.cu); their Python types are in kernels/block_scaled.py.
+def _on_current_device(t: torch.Tensor, name: str) -> None:
+    if not t.is_cuda:
+        raise KernelError(f"{name} must be a CUDA tensor (there is no CPU path)")
+    if t.device.index != torch._C._cuda_getDevice():
+        raise KernelError(f"{name} is on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+
+
+def quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
+    """Codes [rows, K rounded up to 128] (8 bits) and scales [runs of 128 columns, at least rows] of the rows ``x`` [rows, K]."""
+    _on_current_device(x, "x"), _rows_of(x, "x")
+    _need(codes, "codes", torch.float8_e4m3fn), _need(scales, "scales", torch.float32)
+    rows, k = x.shape
+    if codes.shape != (rows, -(-k // 128) * 128) or scales.dim() != 2 or scales.shape[0] != -(-k // 128) or scales.shape[1] < rows:
+        raise KernelError("quantize_rows: shapes do not fit")
+    _check("quantize_rows", lib().tib_quantize_rows(_ptr(x), _code(x.dtype), x.stride(0), _ptr(codes), codes.stride(0), _ptr(scales),
+                                                    scales.shape[1], rows, k, _stream()))
+
+
+def block_scaled_product(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, y: torch.Tensor, *,
+                         paired: bool = False, act: str = "none", limit: float = 0.0, alpha: float = 1.0,
+                         routing: tuple[torch.Tensor, torch.Tensor, int, bool] | None = None, row_scale: torch.Tensor | None = None,
+                         error_word: torch.Tensor | None = None) -> torch.Tensor:
+    """Rows of codes times matrices of codes: ``codes`` / ``scales`` as :func:`quantize_rows` leaves them, ``w`` [experts, N, runs * 128],
+    ``w_scales`` [experts, rows of scales, runs] (``paired``: of (gate, up) row pairs).  ``routing`` = (offsets, order, top, x_by_pair) sorts the
+    rows of ``y`` by expert as in :func:`moe_expert_product`; without it there is one matrix and row m of ``y`` is that of row m."""
+    _need(codes, "codes", torch.float8_e4m3fn), _need(scales, "scales", torch.float32), _need(w, "w", torch.float8_e4m3fn)
+    _need(w_scales, "w_scales", torch.float32), _rows_of(y, "y")
+    experts, n, k = w.shape
+    offsets, order, top, x_by_pair = routing if routing is not None else (None, None, 1, False)
+    n_out = n // 2 if act in MOE_GATED else n
+    if k % 128 or codes.shape[1] != k or w_scales.shape[0] != experts or w_scales.shape[2] != k // 128 or scales.shape[0] != k // 128 or y.shape[1] != n_out:
+        raise KernelError("block_scaled_product: shapes do not fit")
+    _check("block_scaled_product", lib().tib_block_scaled_product(
+        _ptr(codes), _ptr(scales), scales.shape[1], _ptr(w), _ptr(w_scales), w_scales.shape[1], int(paired), _ptr(y), _code(y.dtype),
+        y.stride(0), y.shape[0], n, k // 128, _ptr(offsets), _ptr(order), experts, top, int(x_by_pair), MOE_ACT[act], limit, alpha,
+        _ptr(row_scale), _ptr(error_word), _stream()))
+    return y
 
 
 def glu_clamp(gate_up: torch.Tensor, out: torch.Tensor, limit: float, alpha: float) -> torch.Tensor:
