@@ -1,0 +1,566 @@
+// Products of 8-bit block-scaled operands on the 5th-generation tensor cores, for few rows and for rows sorted by expert:
+//     y[m, n] = act(sum over runs b of s[m, b] S[n's block, b] (sum over the 128 columns of run b of x[m, k] w[n, k]))
+//
+// The weights are the 128-row operand of the MMA and the rows its N dimension: a tile is 128 features x up to NT rows, the rows rounded up to 16
+// only, and the accumulator is the transposed output (TMEM lane = feature, column = row).  A step of the loop is one run: 128 columns, the 128-byte
+// row of the swizzle, four MMAs into an accumulator of its own in tensor memory, which the summing warps take out, multiply by its scales and add to
+// 32-bit sums in registers (packed fp32, two instructions for two sums).  kBufs accumulators rotate, so the tensor cores run ahead of the sums.
+//   warp 0             TMA producer: 16 KB of codes of w a step, and the rows' codes where they exist: boxes of 32 rows that lie side by side, or
+//                      four rows by their numbers at a time (gather4) where they are sorted
+//   warp 1             issues tcgen05.mma; owns the TMEM allocation
+//   the next 4 or 8    sums and epilogue (eight for 128 rows: four for each half of the columns)
+//   the last 4         helpers, each every fourth step: the rows' scales into the ring's stage; from rows that are no codes yet they make
+//                      these, straight into the swizzled stage (a step of few rows then has no kernel ahead of its products)
+// A matrix of few tiles is split by runs over a cluster of up to eight blocks, whose sums meet in distributed shared memory, added in the
+// blocks' order.  Weights do not depend on the kernel before: a first ring of them is requested before griddepcontrol.wait (not for sorted rows, whose
+// tiles that kernel's counts decide).  Every wait is bounded and reports in error_word; a warp that gave up goes through the motions to the
+// end, so that nobody waits for it.
+#include "block_scaled.cuh"
+#include "mma.cuh"
+#include "cluster.cuh"
+
+namespace tib {
+
+constexpr int kBsMaxExperts = 1024, kBsMaxStages = 16;
+constexpr uint32_t kBsWBytes = 128 * kBlk;
+
+template <int NT> struct BsShape {
+  static constexpr int kStorers = NT >= 128 ? 8 : 4, kHelpers = 4, kThreads = 64 + 32 * (kStorers + kHelpers);
+  static constexpr int kBufs = 4, kCols = NT / (kStorers / 4);      // accumulators; columns of a summing thread
+  static constexpr uint32_t kTmemCols = kBufs * NT < 32 ? 32 : kBufs * NT;
+  static constexpr uint32_t kStage = kBsWBytes + NT * kBlk;
+  static constexpr int kRedStride = NT + 4;                         // floats of a feature's sums (16-byte steps that fall on all banks)
+};
+
+struct BsTile { int expert, first, rows, feature; };
+
+struct BsArgs {
+  const void* x;               // codes [rows, runs * 128], or rows of the activations' type
+  int64_t ldx;                 // (of the latter)
+  const float* x_scales;       // [runs, lds] beside codes
+  int64_t lds;
+  const float* w_scales;
+  int scale_rows, pairs, vec;
+  int M, N, K, runs, stages;
+  const int* offsets;          // null: one matrix
+  const int* order;
+  int experts, top, x_by_pair;
+  MoeEpilogue ep;
+  int* error_word;
+};
+
+__device__ __forceinline__ void umma_f8_warp(uint32_t leader, uint32_t tmem_d, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n.reg .pred p, q;\n.reg .b64 a, b;\nmov.b64 a, {%1, %6};\nmov.b64 b, {%2, %6};\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+               "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, p;\n}\n"
+               ::"r"(tmem_d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(leader), "r"(kUmmaDescHigh) : "memory");
+}
+// four rows of 128 bytes by their numbers, one under the other
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int x, const int (&row)[4], uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];\n"
+               ::"r"(dst), "l"(map), "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void bs_fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+
+template <int NT, typename TX, typename TO>
+__global__ void __launch_bounds__(BsShape<NT>::kThreads, 1)
+block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const BsArgs a,
+                            TO* __restrict__ y, int64_t ldy) {
+  using S = BsShape<NT>;
+  constexpr bool kCodes = std::is_same_v<TX, uint8_t>;
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char* smem_gen = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t bars = base + a.stages * S::kStage;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (kBsMaxStages + s); };
+  auto acc_full_bar = [&](int b) { return bars + 8u * (2 * kBsMaxStages + b); };
+  auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * kBsMaxStages + S::kBufs + b); };
+  const uint32_t red_bar = bars + 8u * (2 * kBsMaxStages + 2 * S::kBufs), tmem_slot = red_bar + 8;
+  static_assert(8 * (2 * kBsMaxStages + 2 * S::kBufs) + 16 <= 384, "the barriers' share of shared memory");
+  volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem_gen + (tmem_slot - base));
+  float* row_scales = reinterpret_cast<float*>(smem_gen + (bars - base) + 384);           // [stages][NT]
+  float* red = row_scales + a.stages * NT;                                                // [128][kRedStride] in all
+  int* tiles_before = reinterpret_cast<int*>(red + 128 * S::kRedStride);                  // [experts + 1] where rows are sorted
+
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int splits = (int)cluster_size(), rank = (int)cluster_rank();
+  const int cluster_id = blockIdx.x / splits, clusters = gridDim.x / splits;
+  const int kb0 = (int)((int64_t)a.runs * rank / splits), kb1 = (int)((int64_t)a.runs * (rank + 1) / splits);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      mbar_init(full_bar(s), 2);                  // the producer and one helper
+      mbar_init(empty_bar(s), S::kStorers);       // (a sum that has been taken out is one whose MMAs have read their stage)
+    }
+    for (int b = 0; b < S::kBufs; ++b) {
+      mbar_init(acc_full_bar(b), 1);
+      mbar_init(acc_empty_bar(b), S::kStorers);
+    }
+    mbar_init(red_bar, S::kStorers * splits);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tmem_slot), "r"(S::kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  if (a.offsets) {
+    pdl_wait();
+    if (warp == 0) {      // the experts' row tiles, summed
+      int before = 0;
+      for (int e0 = 0; e0 < a.experts; e0 += 32) {
+        const int e = e0 + lane;
+        int sum = e < a.experts ? (a.offsets[e + 1] - a.offsets[e] + NT - 1) / NT : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += up;
+        }
+        if (e < a.experts) tiles_before[e + 1] = before + sum;
+        before += __shfl_sync(0xffffffffu, sum, 31);
+      }
+      if (lane == 0) tiles_before[0] = 0;
+    }
+  }
+  pdl_trigger();
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot_ptr, 0);
+  if (splits > 1) cluster_sync_all();             // every block of the cluster runs and has its barriers
+
+  const int f_tiles = (a.N + 127) >> 7;
+  const int row_tiles = a.offsets ? tiles_before[a.experts] : (a.M + NT - 1) / NT;
+  const int num_tiles = row_tiles * f_tiles;
+  auto tile_of = [&](int t) {                     // (feature tiles run fastest: blocks that run together read the same rows)
+    const int row_tile = t / f_tiles;
+    BsTile m;
+    int begin = 0, n = a.M, tiles = row_tiles, j = row_tile;
+    m.expert = 0;
+    if (a.offsets) {
+      int lo = 0, hi = a.experts;                 // tiles_before[lo] <= row_tile < tiles_before[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (tiles_before[mid] <= row_tile) lo = mid; else hi = mid;
+      }
+      begin = a.offsets[lo];
+      n = a.offsets[lo + 1] - begin;
+      tiles = tiles_before[lo + 1] - tiles_before[lo];
+      j = row_tile - tiles_before[lo];
+      m.expert = lo;
+    }
+    const int per = ((n + tiles - 1) / tiles + 15) & ~15;      // equal tiles (at most NT rows, and the last is not empty)
+    m.first = begin + j * per;
+    m.rows = min(per, n - j * per);
+    m.feature = (t - row_tile * f_tiles) << 7;
+    return m;
+  };
+  auto source = [&](const BsTile& m, int r) {     // the row of x that the tile's row r is
+    const int at = m.first + min(r, m.rows - 1);
+    return a.offsets && a.x_by_pair ? a.order[at] / a.top : at;
+  };
+
+  if (warp == 0) {
+    const uint32_t leader = umma_leader();
+    int ahead = 0, it = 0, s = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    const bool gather = kCodes && a.offsets && a.x_by_pair;
+    auto bytes = [&](const BsTile& m) {
+      return kBsWBytes + (!kCodes ? 0 : gather ? ((m.rows + 3) >> 2) * 4 * kBlk : ((m.rows + 31) >> 5) * 32 * kBlk);
+    };
+    if (!a.offsets) {
+      for (int t = cluster_id; t < num_tiles && ahead < a.stages; t += clusters) {
+        const BsTile m = tile_of(t);
+          for (int kb = kb0; kb < kb1 && ahead < a.stages; ++kb, ++ahead)
+          if (leader) {
+            mbar_expect_tx(full_bar(ahead), bytes(m));
+            tma_load_2d(base + ahead * S::kStage, &map_w, kb * kBlk, m.expert * a.N + m.feature, full_bar(ahead));
+          }
+      }
+      pdl_wait();
+    }
+    for (int t = cluster_id; t < num_tiles && ok; t += clusters) {
+      const BsTile m = tile_of(t);
+      int rows[NT > 128 ? 2 : 1][4];              // the rows of this lane's gathers
+      if (gather) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) rows[0][j] = source(m, 4 * lane + j);
+      }
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const uint32_t stage = base + s * S::kStage;
+        if (it >= ahead) {
+          if (!mbar_wait_warp(empty_bar(s), phase)) {
+            if (a.error_word && leader) atomicExch(a.error_word, 0x7C00C1);
+            ok = false;
+            break;
+          }
+          if (leader) {
+            mbar_expect_tx(full_bar(s), bytes(m));
+            tma_load_2d(stage, &map_w, kb * kBlk, m.expert * a.N + m.feature, full_bar(s));      // (a tile may reach into the next expert's features, or past the last: such lanes are never stored)
+          }
+          __syncwarp();
+        }
+        if constexpr (kCodes) {
+          if (gather) {
+            if (4 * lane < m.rows) tma_gather4(stage + kBsWBytes + lane * 4 * kBlk, &map_x, kb * kBlk, rows[0], full_bar(s));
+          } else if (leader) {
+#pragma unroll
+            for (int i = 0; i < NT / 32; ++i)     // (likewise a last box into the next tile's rows, or past the last)
+              if (32 * i < m.rows) tma_load_2d(stage + kBsWBytes + i * 32 * kBlk, &map_x, kb * kBlk, m.first + 32 * i, full_bar(s));
+          }
+          __syncwarp();
+        }
+        if (++s == a.stages) { s = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t leader = umma_leader();
+    int s = 0, b = 0;
+    uint32_t phase = 0, acc_phase = 1;
+    bool ok = true;
+    for (int t = cluster_id; t < num_tiles && ok; t += clusters) {
+      const BsTile m = tile_of(t);
+      // D fp32, A and B e4m3, both K-major, N = the rows, M = 128
+      const uint32_t idesc = (1u << 4) | ((uint32_t)((m.rows + 15) >> 4) << 18) | ((128u >> 4) << 24);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait_warp(acc_empty_bar(b), acc_phase)) {
+          if (a.error_word && leader) atomicExch(a.error_word, 0x7C00C4);
+          ok = false;
+          break;
+        }
+        if (!mbar_wait_warp(full_bar(s), phase)) {
+          if (a.error_word && leader) atomicExch(a.error_word, 0x7C00C2);
+          ok = false;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        const uint32_t w_src = umma_low_k128(base + s * S::kStage), x_src = w_src + (kBsWBytes >> 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_f8_warp(leader, tmem_base + b * NT, w_src + 2 * k, x_src + 2 * k, idesc, k != 0);
+        if (leader) umma_commit(acc_full_bar(b));
+        __syncwarp();
+        if (++s == a.stages) { s = 0; phase ^= 1; }
+        if (++b == S::kBufs) { b = 0; acc_phase ^= 1; }
+      }
+    }
+  } else if (warp < 2 + S::kStorers) {
+    const int quarter = warp & 3, c0 = ((warp - 2) >> 2) * S::kCols;
+    const int et = threadIdx.x - 64;
+    int s = 0, b = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    bool ok = true;
+    if (!a.offsets) pdl_wait();                   // (y may be memory that the kernel before still reads)
+    for (int t = cluster_id; t < num_tiles; t += clusters) {
+      const BsTile m = tile_of(t);
+      const float* ws = a.w_scales + ((size_t)m.expert * a.scale_rows + bs_scale_row(m.feature, a.pairs)) * a.runs;
+      f32x2 sum[S::kCols / 2];
+#pragma unroll
+      for (int c = 0; c < S::kCols / 2; ++c) sum[c] = f2_pack(0.f, 0.f);
+      float even = 0.f, odd = 0.f;                // the scales of the next 32 runs, a lane each (of gate and up rows)
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int i = (kb - kb0) & 31;
+        if (i == 0) {
+          const int at = min(kb + lane, a.runs - 1);
+          even = ws[at];
+          odd = a.pairs ? ws[a.runs + at] : even;
+        }
+        if (ok && !(mbar_wait_warp(acc_full_bar(b), acc_phase) && mbar_wait_warp(full_bar(s), phase))) {
+          if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00C3);
+          ok = false;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        const float w_even = __shfl_sync(0xffffffffu, even, i), w_odd = __shfl_sync(0xffffffffu, odd, i);
+        const float w = lane & 1 ? w_odd : w_even;
+        const f32x2 w2 = f2_pack(w, w);
+        const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + b * NT + c0;
+        const float* xs = row_scales + s * NT + c0;
+#pragma unroll
+        for (int c = 0; c < S::kCols; c += 16) {
+          if (c0 + c < m.rows) {
+            uint32_t v[16];
+            tmem_ld16(acc + c, v);
+            float4 scale[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) scale[q] = reinterpret_cast<const float4*>(xs + c)[q];
+            asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              f32x2& lo = sum[c / 2 + 2 * q];
+              f32x2& hi = sum[c / 2 + 2 * q + 1];
+              lo = f2_fma(f2_pack(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1])), f2_mul(f2_pack(scale[q].x, scale[q].y), w2), lo);
+              hi = f2_fma(f2_pack(__uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3])), f2_mul(f2_pack(scale[q].z, scale[q].w), w2), hi);
+            }
+          }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(acc_empty_bar(b));
+          mbar_arrive(empty_bar(s));
+        }
+        if (++s == a.stages) { s = 0; phase ^= 1; }
+        if (++b == S::kBufs) { b = 0; acc_phase ^= 1; }
+      }
+      // The sums cross shared memory, where a rolled loop finishes them (unrolled, the activations' code would be fetched anew for every tile),
+      // consecutive threads consecutive features.  Block r of a cluster finishes features r * per .. of the tile.
+      const int per = 128 / splits, feature = quarter * 32 + lane;
+      asm volatile("bar.sync 1, %0;\n" ::"r"(32 * S::kStorers) : "memory");       // (the last tile's sums have been read)
+      if (splits == 1) {
+        float4* dst = reinterpret_cast<float4*>(red + feature * S::kRedStride + c0);
+#pragma unroll
+        for (int q = 0; q < S::kCols / 4; ++q) {
+          float4 v;
+          f2_unpack(sum[2 * q], v.x, v.y);
+          f2_unpack(sum[2 * q + 1], v.z, v.w);
+          dst[q] = v;
+        }
+        asm volatile("bar.sync 1, %0;\n" ::"r"(32 * S::kStorers) : "memory");
+      } else {
+        const uint32_t dst = map_to_cta(smem_u32(red + (rank * per + feature % per) * S::kRedStride + c0), feature / per);
+#pragma unroll
+        for (int q = 0; q < S::kCols / 4; ++q) {
+          float4 v;
+          f2_unpack(sum[2 * q], v.x, v.y);
+          f2_unpack(sum[2 * q + 1], v.z, v.w);
+          st_cluster_f32x4(dst + 16 * q, v.x, v.y, v.z, v.w);
+        }
+        __syncwarp();
+        if (lane < splits) mbar_arrive_remote(map_to_cta(red_bar, lane));
+        if (!mbar_wait_cluster(red_bar, 0)) {
+          if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00C5);
+          ok = false;
+        }
+      }
+      if (!ok) continue;
+      const bool gated = moe_act_gated(a.ep.act);
+      const int wide = gated ? per / 2 : per, first_out = (m.feature + rank * per) >> (gated ? 1 : 0);
+      const int n_out = gated ? a.N >> 1 : a.N;
+      auto summed = [&](int f, int c) {           // the four columns from c of this block's feature f
+        float4 v = *reinterpret_cast<const float4*>(red + f * S::kRedStride + c);
+        for (int r = 1; r < splits; ++r) {
+          const float4 o = *reinterpret_cast<const float4*>(red + (r * per + f) * S::kRedStride + c);
+          v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+        }
+        return v;
+      };
+      for (int i = et; i < wide * ((m.rows + 3) >> 2); i += 32 * S::kStorers) {
+        const int c = i / wide * 4, f = i % wide;
+        if (first_out + f >= n_out) continue;
+        const float4 u = summed(gated ? 2 * f : f, c), v = gated ? summed(2 * f + 1, c) : u;
+        const float first_sum[4] = {u.x, u.y, u.z, u.w}, second_sum[4] = {v.x, v.y, v.z, v.w};
+        TO* dst = y + (size_t)(m.first + c) * ldy + first_out + f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (c + j >= m.rows) break;
+          const float scale = a.ep.row_scale ? a.ep.row_scale[a.order[m.first + c + j]] : 1.f;
+          const float g = first_sum[j] * scale;
+          dst[(size_t)j * ldy] = from_f32<TO>(gated ? moe_gated(g, second_sum[j] * scale, a.ep.act, a.ep.limit, a.ep.alpha) : moe_act(g, a.ep.act));
+        }
+      }
+    }
+  } else {
+    const int helper = warp - 2 - S::kStorers;
+    int it = 0, s = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    if (!a.offsets) pdl_wait();
+    for (int t = cluster_id; t < num_tiles && ok; t += clusters) {
+      const BsTile m = tile_of(t);
+      int from[(NT + 31) / 32];                   // (codes) the rows whose scales this lane copies
+      if constexpr (kCodes) {
+#pragma unroll
+        for (int i = 0; i < (NT + 31) / 32; ++i) from[i] = source(m, lane + 32 * i);
+      }
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        if ((it & (S::kHelpers - 1)) == helper) {
+          float* scales = row_scales + s * NT;
+          if constexpr (kCodes) {
+            float v[(NT + 31) / 32];
+#pragma unroll
+            for (int i = 0; i < (NT + 31) / 32; ++i) v[i] = a.x_scales[(size_t)kb * a.lds + from[i]];
+            if (!mbar_wait_warp(empty_bar(s), phase)) ok = false;
+#pragma unroll
+            for (int i = 0; i < (NT + 31) / 32; ++i)
+              if (lane + 32 * i < NT) scales[lane + 32 * i] = v[i];
+          } else {
+            // eight lanes a row, sixteen columns each; two rows a lane at a time
+            const TX* x = reinterpret_cast<const TX*>(a.x);
+            unsigned char* codes = smem_gen + s * S::kStage + kBsWBytes;
+            const int sub = lane >> 3, eighth = lane & 7, col = kb * kBlk + eighth * 16;
+            bool free = false;
+#pragma unroll 1
+            for (int r0 = 0; r0 < m.rows; r0 += 8) {
+              float v[2][16];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int r = r0 + 4 * h + sub;
+                const TX* p = x + (size_t)source(m, r) * a.ldx + min(col, a.K - 1);
+                const int n = r < m.rows ? a.K - col : 0;
+                if (a.vec) bs_load16<TX, true>(p, n, v[h]);
+                else bs_load16<TX, false>(p, n, v[h]);
+              }
+              if (!free) {
+                if (!mbar_wait_warp(empty_bar(s), phase)) ok = false;
+                free = true;
+              }
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int r = r0 + 4 * h + sub;
+                uint32_t largest = 0;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) largest = max(largest, __float_as_uint(v[h][j]) & 0x7fffffffu);
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+                float scale, inverse;
+                bs_run_scale(largest, scale, inverse);
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  w[j] = bs_codes4(v[h][4 * j] * inverse, v[h][4 * j + 1] * inverse, v[h][4 * j + 2] * inverse, v[h][4 * j + 3] * inverse);
+                if (r < m.rows && ok) {
+                  *reinterpret_cast<uint4*>(codes + r * kBlk + ((eighth ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                  if (eighth == 0) scales[r] = scale;
+                }
+              }
+            }
+            bs_fence_async_shared();
+          }
+          if (!ok) {
+            if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00C6);
+            break;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full_bar(s));
+        }
+        if (++s == a.stages) { s = 0; phase ^= 1; }
+      }
+    }
+  }
+  __syncwarp();
+  if (splits > 1) cluster_sync_all();             // no block leaves while a peer may still write to it
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
+  }
+}
+
+// Codes [rows, bytes a row], read in boxes of box_rows x 128 with 128-byte swizzle (box_rows 1: by gathers of four).
+static int bs_make_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t bytes, int box_rows) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return TIB_E_ARG;
+  const cuuint64_t dims[2] = {(cuuint64_t)bytes, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)bytes};
+  const cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
+  const cuuint32_t elem[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? TIB_OK : TIB_E_ARG;
+}
+
+template <int NT>
+static constexpr uint32_t bs_smem(int stages, int experts) {
+  return 1024u + stages * (BsShape<NT>::kStage + NT * 4) + 384u + 128 * BsShape<NT>::kRedStride * 4 + 4 * (experts + 1);
+}
+
+template <int NT, typename TX, typename TO>
+static int launch_block_scaled(const CUtensorMap& map_w, const CUtensorMap& map_x, BsArgs& a, void* y, int64_t ldy, int splits, cudaStream_t stream) {
+  const int experts = a.offsets ? a.experts : 0;
+  const int64_t row_tiles = a.offsets ? a.M / NT + (a.M < a.experts ? a.M : a.experts) : ceil_div(a.M, NT);
+  const int64_t tiles = row_tiles * ceil_div(a.N, 128);
+  if (tiles * splits > 0x7fffffff) return TIB_E_SIZE;
+  const int grid = (int)(splits > 1 ? tiles * splits : tiles < 148 ? tiles : 148);      // (a cluster has one tile: its sums' place is used once)
+  const int64_t steps = (int64_t)ceil_div(a.runs, splits) * ceil_div64(tiles * splits, grid);      // of a block, at most
+  a.stages = 1;
+  while (a.stages < kBsMaxStages && a.stages < steps && bs_smem<NT>(a.stages + 1, experts) <= (uint32_t)kMostSmem) ++a.stages;
+  auto kern = block_scaled_tcgen05_kernel<NT, TX, TO>;
+  static bool allowed[64];      // (by device: the attribute belongs to its context)
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess && !(device < 64 && allowed[device])) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
+  if (e != cudaSuccess) return (int)e;
+  if (device < 64) allowed[device] = true;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(BsShape<NT>::kThreads);
+  cfg.dynamicSmemBytes = bs_smem<NT>(a.stages, experts);
+  cfg.stream = stream;
+  cfg.gridDim = dim3((unsigned)grid);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // (see launch_dependent in common.cuh)
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent_launch_flag() ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, kern, map_w, map_x, (const BsArgs)a, (TO*)y, ldy);
+  if (e != cudaSuccess) return (int)e;
+  TIB_LAUNCH_CHECK();
+  return TIB_OK;
+}
+
+// The blocks that share a tile's runs: as many as make the GPU's worth of blocks of few tiles, each with two runs or more.
+static int bs_splits(int64_t tiles, int runs) {
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= 148 && runs >= 4 * splits) splits *= 2;
+  return splits;
+}
+
+}  // namespace tib
+
+using namespace tib;
+
+// x_dtype TIB_BF16 or TIB_F32: rows [rows, K] (row stride ldx) that are quantised on the way, once for each tile of 128 features; -1: codes
+// [x_rows, runs * 128] and scales [runs, lds] as tib_quantize_rows leaves them.  w: codes [experts, N, runs * 128] and scales
+// [experts, scale_rows, runs] (`pairs`: of (gate, up) row pairs); y: [M, N] in y_dtype (row stride ldy), or [M, N / 2] of a gated activation.
+// offsets [experts + 1] and order [M]: rows sorted by expert as tib_moe_expert_product takes them; offsets null: one matrix for all rows.
+TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, int x_rows, const float* x_scales, int64_t lds, const void* w,
+                                     const float* w_scales, int scale_rows, int pairs, void* y, int y_dtype, int64_t ldy, int M, int N, int K,
+                                     const int* offsets, const int* order, int experts, int top, int x_by_pair, int act, float limit,
+                                     float alpha, const float* row_scale, int* error_word, cudaStream_t stream) {
+  if (M == 0 || N == 0) return TIB_OK;
+  const bool is_codes = x_dtype < 0;
+  if (!x || !w || !w_scales || !y || M < 0 || N < 0 || K < 1 || experts < 1 || top < 1 || x_rows < 1) return TIB_E_ARG;
+  if ((is_codes && !x_scales) || (offsets && !order) || (row_scale && !order)) return TIB_E_ARG;
+  if (act < MOE_ACT_NONE || act > MOE_ACT_GELU || (moe_act_gated(act) && !pairs) || (pairs && N % 2)) return TIB_E_SIZE;
+  if (x_dtype > TIB_BF16 || (y_dtype != TIB_BF16 && y_dtype != TIB_F32)) return TIB_E_DTYPE;
+  if (experts > kBsMaxExperts || (int64_t)experts * N > 0x7fffffff - 128) return TIB_E_SIZE;
+  if ((((uintptr_t)w) & 15) || (is_codes && (((uintptr_t)x) & 15))) return TIB_E_ALIGN;
+  BsArgs a;
+  a.x = x; a.ldx = ldx; a.x_scales = x_scales; a.lds = lds; a.w_scales = w_scales; a.scale_rows = scale_rows; a.pairs = pairs;
+  a.vec = !is_codes && ((uintptr_t)x & 15) == 0 && (ldx * (x_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
+  a.M = M; a.N = N; a.K = K; a.runs = ceil_div(K, kBlk); a.offsets = offsets; a.order = order; a.experts = experts; a.top = top;
+  a.x_by_pair = x_by_pair; a.error_word = error_word;
+  a.ep.act = act; a.ep.limit = limit; a.ep.alpha = alpha; a.ep.row_scale = row_scale;
+  CUtensorMap map_w, map_x;
+  int rc = bs_make_map(&map_w, w, (int64_t)experts * N, (int64_t)a.runs * kBlk, 128);
+  if (rc != TIB_OK) return rc;
+  map_x = map_w;
+  if (is_codes) {
+    rc = bs_make_map(&map_x, x, x_rows, (int64_t)a.runs * kBlk, offsets && x_by_pair ? 1 : 32);
+    if (rc != TIB_OK) return rc;
+  }
+  const int rows = offsets ? ceil_div(M, experts) : M;      // (of an expert, on average)
+  auto splits = [&](int nt) { return offsets ? 1 : bs_splits((int64_t)ceil_div(M, nt) * ceil_div(N, 128), a.runs); };
+#define TIB_BS_GO(NT, TX)                                                                                                  \
+  return y_dtype == TIB_BF16 ? launch_block_scaled<NT, TX, __nv_bfloat16>(map_w, map_x, a, y, ldy, splits(NT), stream)      \
+                             : launch_block_scaled<NT, TX, float>(map_w, map_x, a, y, ldy, splits(NT), stream)
+  if (is_codes) {
+    if (rows <= 32) TIB_BS_GO(32, uint8_t);
+    if (rows <= 64) TIB_BS_GO(64, uint8_t);
+    TIB_BS_GO(128, uint8_t);
+  }
+  if (x_dtype == TIB_BF16) {
+    if (rows <= 16) TIB_BS_GO(16, __nv_bfloat16);
+    if (rows <= 32) TIB_BS_GO(32, __nv_bfloat16);
+    TIB_BS_GO(64, __nv_bfloat16);
+  }
+  if (rows <= 16) TIB_BS_GO(16, float);
+  if (rows <= 32) TIB_BS_GO(32, float);
+  TIB_BS_GO(64, float);
+#undef TIB_BS_GO
+}
+
+// The calls the Python parts make (common.cuh).
+TIB_PACKED(tib_block_scaled_tcgen05)

@@ -23,6 +23,9 @@ from torchinferno_b200.kernels import ops
 
 BLOCK = 128
 CODE_DTYPE = torch.float8_e4m3fn
+# Up to so many rows (of an expert: on average) a product's kernel quantises its rows itself, in every tile of 128 features anew.
+FEW_ROWS = 64
+FEW_EXPERT_ROWS = 16
 
 
 def blocks(count: int) -> int:
@@ -89,6 +92,11 @@ def _quantized(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     scales = torch.empty((runs, -(-rows // 4) * 4), dtype=torch.float32, device=x.device)
     ops.quantize_rows(x, codes, scales)
     return codes, scales
+
+
+def _rows_for(x: torch.Tensor, rows: int, few: int) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """What a product over so many ``rows`` of a matrix reads: up to ``few`` of them its kernel quantises itself, more are quantised ahead of it."""
+    return (x, None) if rows <= few else _quantized(x)
 
 
 def _laid_out(matrices: Sequence[BlockScaledMatrix], ups: Sequence[BlockScaledMatrix] | None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -190,9 +198,10 @@ class BlockScaledWeight:
         out = self._checked(x, out_dtype, self.out_features, out)
         if x.shape[0] == 0:
             return out
-        rows = _quantized(x)
+        rows = _rows_for(x, x.shape[0], FEW_ROWS)
         for first, codes, scales in self.parts:
-            ops.block_scaled_product(*rows, codes, scales, out[:, first:first + codes.shape[1]], paired=self.epilogue == "swiglu", error_word=error_word)
+            ops.block_scaled_product(*rows, codes, scales, out if len(self.parts) == 1 else out[:, first:first + codes.shape[1]],
+                                     columns=self.in_features, paired=self.epilogue == "swiglu", error_word=error_word)
         return out
 
     def swiglu(self, x: torch.Tensor, *, out_dtype: torch.dtype | None = None, error_word: torch.Tensor | None = None) -> torch.Tensor:
@@ -203,7 +212,8 @@ class BlockScaledWeight:
         if x.shape[0] == 0:
             return out
         _, codes, scales = self.parts[0]
-        return ops.block_scaled_product(*_quantized(x), codes, scales, out, paired=True, act="swiglu", error_word=error_word)
+        return ops.block_scaled_product(*_rows_for(x, x.shape[0], FEW_ROWS), codes, scales, out, columns=self.in_features, paired=True, act="swiglu",
+                                        error_word=error_word)
 
 
 class BlockScaledExperts:
@@ -248,5 +258,5 @@ class BlockScaledExperts:
                 raise ops.KernelError("moe_expert_product: row_scale must hold one factor per pair")
         if pairs == 0:
             return y
-        return ops.block_scaled_product(*_quantized(x), self.codes, self.scales, y, paired=self.paired, act=act, limit=limit, alpha=alpha,
-                                        routing=(offsets, order, top, x_by_pair), row_scale=row_scale, error_word=error_word)
+        return ops.block_scaled_product(*_rows_for(x, -(-pairs // self.experts), FEW_EXPERT_ROWS), self.codes, self.scales, y,
+                                        columns=self.in_features, paired=self.paired, act=act, limit=limit, alpha=alpha, routing=(offsets, order, top, x_by_pair), row_scale=row_scale, error_word=error_word)

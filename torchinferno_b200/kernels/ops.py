@@ -1273,24 +1273,26 @@ def quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) ->
                                                     scales.shape[1], rows, k, _stream()))
 
 
-def block_scaled_product(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, y: torch.Tensor, *,
-                         paired: bool = False, act: str = "none", limit: float = 0.0, alpha: float = 1.0,
+def block_scaled_product(x: torch.Tensor, scales: torch.Tensor | None, w: torch.Tensor, w_scales: torch.Tensor, y: torch.Tensor, *,
+                         columns: int, paired: bool = False, act: str = "none", limit: float = 0.0, alpha: float = 1.0,
                          routing: tuple[torch.Tensor, torch.Tensor, int, bool] | None = None, row_scale: torch.Tensor | None = None,
                          error_word: torch.Tensor | None = None) -> torch.Tensor:
-    """Rows of codes times matrices of codes: ``codes`` / ``scales`` as :func:`quantize_rows` leaves them, ``w`` [experts, N, runs * 128],
-    ``w_scales`` [experts, rows of scales, runs] (``paired``: of (gate, up) row pairs).  ``routing`` = (offsets, order, top, x_by_pair) sorts the
-    rows of ``y`` by expert as in :func:`moe_expert_product`; without it there is one matrix and row m of ``y`` is that of row m."""
-    _need(codes, "codes", torch.float8_e4m3fn), _need(scales, "scales", torch.float32), _need(w, "w", torch.float8_e4m3fn)
-    _need(w_scales, "w_scales", torch.float32), _rows_of(y, "y")
+    """Rows times matrices of codes.  ``x``: codes with their ``scales`` as :func:`quantize_rows` leaves them, or (``scales`` None) rows that the
+    product's kernel quantises itself; ``w``: [experts, N, ``columns`` rounded up to 128], ``w_scales`` [experts, rows of scales, runs] (``paired``: of
+    (gate, up) row pairs).  ``routing`` = (offsets, order, top, x_by_pair) sorts the rows of ``y`` by expert as in
+    :func:`moe_expert_product`; without it there is one matrix and row m of ``y`` is that of row m."""
+    _on_current_device(x, "x"), _rows_of(x, "x"), _rows_of(y, "y"), _need(w, "w", torch.float8_e4m3fn), _need(w_scales, "w_scales", torch.float32)
     experts, n, k = w.shape
     offsets, order, top, x_by_pair = routing if routing is not None else (None, None, 1, False)
-    n_out = n // 2 if act in MOE_GATED else n
-    if k % 128 or codes.shape[1] != k or w_scales.shape[0] != experts or w_scales.shape[2] != k // 128 or scales.shape[0] != k // 128 or y.shape[1] != n_out:
+    if scales is not None:
+        _need(x, "x", torch.float8_e4m3fn), _need(scales, "scales", torch.float32)
+    if (k != -(-columns // 128) * 128 or x.shape[1] != (columns if scales is None else k) or w_scales.shape[0] != experts or w_scales.shape[2] != k // 128
+            or y.shape[1] != (n // 2 if act in MOE_GATED else n) or (routing is None and y.shape[0] != x.shape[0])):
         raise KernelError("block_scaled_product: shapes do not fit")
-    _check("block_scaled_product", lib().tib_block_scaled_product(
-        _ptr(codes), _ptr(scales), scales.shape[1], _ptr(w), _ptr(w_scales), w_scales.shape[1], int(paired), _ptr(y), _code(y.dtype),
-        y.stride(0), y.shape[0], n, k // 128, _ptr(offsets), _ptr(order), experts, top, int(x_by_pair), MOE_ACT[act], limit, alpha,
-        _ptr(row_scale), _ptr(error_word), _stream()))
+    _check("block_scaled_product", lib().tib_block_scaled_tcgen05(
+        _ptr(x), _code(x.dtype) if scales is None else -1, x.stride(0), x.shape[0], _ptr(scales), 0 if scales is None else scales.shape[1], _ptr(w),
+        _ptr(w_scales), w_scales.shape[1], int(paired), _ptr(y), _code(y.dtype), y.stride(0), y.shape[0], n, columns, _ptr(offsets), _ptr(order), experts,
+        top, int(x_by_pair), MOE_ACT[act], limit, alpha, _ptr(row_scale), _ptr(error_word), _stream()))
     return y
 
 
