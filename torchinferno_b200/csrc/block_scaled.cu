@@ -11,16 +11,16 @@ namespace tib {
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
 quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scales,
-                     int64_t lds, int rows, int K, int runs) {
+                     int64_t lds, int rows, int K, int runs, const int* __restrict__ order, int top, const int* __restrict__ sorted) {
   pdl_wait();
   pdl_trigger();
   // thread = (row of 8, run of 4, eighth of the run)
   const int groups = (runs + 3) >> 2, row8 = blockIdx.x / groups;
   const int eighth = threadIdx.x & 7, row = row8 * 8 + (threadIdx.x >> 5), run = (blockIdx.x - row8 * groups) * 4 + ((threadIdx.x >> 3) & 3);
-  const bool in = row < rows && run < runs;
-  const int col = run * kBlk + eighth * 16;
+  const bool in = row < (order ? min(rows, *sorted) : rows) && run < runs;
+  const int col = run * kBlk + eighth * 16, from = !in ? 0 : order ? order[row] / top : row;
   float v[16];
-  bs_load16<T, VEC>(x + (size_t)(in ? row : 0) * ldx + (in ? col : 0), in ? K - col : 0, v);
+  bs_load16<T, VEC>(x + (size_t)from * ldx + (in ? col : 0), in ? K - col : 0, v);
   uint32_t largest = 0;
 #pragma unroll
   for (int j = 0; j < 16; ++j) largest = max(largest, __float_as_uint(v[j]) & 0x7fffffffu);
@@ -41,11 +41,11 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__
 using namespace tib;
 
 // x: rows [rows, K] in x_dtype (row stride ldx); codes: [rows, ldc], ldc = K rounded up to 128, behind column K zeros; scales:
-// [runs of 128 columns, lds], lds at least rows.
+// [runs of 128 columns, lds], lds at least rows.  order [rows]: row r is made of row order[r] / top of x, for the first *sorted rows; null: of row r.
 TIB_API int tib_quantize_rows(const void* x, int x_dtype, int64_t ldx, void* codes, int64_t ldc, float* scales, int64_t lds, int rows,
-                              int K, cudaStream_t stream) {
+                              int K, const int* order, int top, const int* sorted, cudaStream_t stream) {
   if (rows == 0) return TIB_OK;
-  if (!x || !codes || !scales || rows < 0 || K < 1) return TIB_E_ARG;
+  if (!x || !codes || !scales || rows < 0 || K < 1 || (order && (top < 1 || !sorted))) return TIB_E_ARG;
   if (x_dtype != TIB_BF16 && x_dtype != TIB_F32) return TIB_E_DTYPE;
   const int runs = ceil_div(K, kBlk);
   if (ldc < (int64_t)runs * kBlk || lds < rows) return TIB_E_SIZE;
@@ -54,7 +54,7 @@ TIB_API int tib_quantize_rows(const void* x, int x_dtype, int64_t ldx, void* cod
   if (grid > 0x7fffffff) return TIB_E_SIZE;
   const bool vec = ((uintptr_t)x & 15) == 0 && (ldx * (x_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
 #define TIB_QUANT_GO(T, VEC) \
-  TIB_LAUNCH_DEPENDENT((quantize_rows_kernel<T, VEC>), (unsigned)grid, 256, 0, stream, (const T*)x, ldx, (uint8_t*)codes, ldc, scales, lds, rows, K, runs)
+  TIB_LAUNCH_DEPENDENT((quantize_rows_kernel<T, VEC>), (unsigned)grid, 256, 0, stream, (const T*)x, ldx, (uint8_t*)codes, ldc, scales, lds, rows, K, runs, order, top, sorted)
   if (x_dtype == TIB_BF16) {
     if (vec) TIB_QUANT_GO(__nv_bfloat16, true);
     else TIB_QUANT_GO(__nv_bfloat16, false);

@@ -7,8 +7,8 @@
 // Rows x [M, K] have one power of two for each run of 128 columns; their scales lie [runs, M rounded up to 4].
 #pragma once
 
-#include "common.cuh"
 #include "moe.cuh"
+#include "tcgen05.cuh"
 
 namespace tib {
 
@@ -69,6 +69,19 @@ __device__ __forceinline__ void bs_load16(const T* p, int n, float (&v)[16]) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = j < n ? to_f32(p[j]) : 0.f;
   }
+}
+
+// Codes [rows, bytes a row], read in boxes of box_rows x 128 with 128-byte swizzle.
+static inline int bs_make_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t bytes, int box_rows) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return TIB_E_ARG;
+  const cuuint64_t dims[2] = {(cuuint64_t)bytes, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)bytes};
+  const cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
+  const cuuint32_t elem[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? TIB_OK : TIB_E_ARG;
 }
 
 }  // namespace tib

@@ -1,0 +1,322 @@
+// Products of 8-bit block-scaled operands for many rows, on pairs of SMs: out[M, N] = x . w^T with `tcgen05.mma.cta_group::2`, where
+//     out[m, n] = sum over runs b of s[m, b] S[n's block, b] (sum over the 128 columns of run b of x[m, k] w[n, k]).
+//
+// Two blocks (a cluster of two) compute a tile of 256 rows x 256 features, as in gemm_tcgen05_2cta.cu: block r holds rows r * 128 .. of the
+// x slice and features r * 128 .. of the w slice, and gets rows r * 128 .. of the accumulator.  A step is one run: 128 columns, the 128-byte row of the
+// swizzle, four MMAs into one of two accumulators of 256 columns.  The sums over runs are taken in registers, since every run has its own scales:
+// eight warps, 32 rows x 128 features each, read the accumulator in pieces of 32 columns, the next piece on its way under the multiply-adds of
+// the last, and add it to 128 sums a thread, times the scale of (its row, run) and (the features' block, run).  Two sums are one packed
+// multiply-add; in a matrix of (gate, up) row pairs the two have different scales, which the packed form takes as it comes.
+//   warp 0       TMA producer into a ring of six stages      warp 1 (of the even block)   issues the MMAs; either owns its block's TMEM
+//   warps 4..11  sums, then the epilogue: plain, or silu(gate) * up.  These take registers that the first four warps give up (168 a thread at launch,
+//                40 + 2 x 232 after)
+// For a step the tensor cores need 512 cycles at their peak, the sums 256 of the tensor memory's reads and 256 of the fp32 pipe.
+// Every wait is bounded and reports in error_word; no block leaves before its partner is done; every copy lands in the block that issued it.
+#include "block_scaled.cuh"
+#include "cluster.cuh"
+
+namespace tib {
+
+constexpr int kB2Stages = 6, kB2Threads = 384;
+constexpr uint32_t kB2Half = 128 * kBlk, kB2Stage = 2 * kB2Half;
+constexpr uint32_t kB2Smem = kB2Stages * kB2Stage + 1024 /* alignment */ + 256 /* barriers */;
+// D fp32, A and B e4m3, both K-major, N = 256, M = 256 over the pair
+constexpr uint32_t kB2Idesc = (1u << 4) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
+
+__device__ __forceinline__ void b2_tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t cluster_bar) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n"
+               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void b2_umma(uint32_t leader, uint32_t tmem_d, uint32_t a_low, uint32_t b_low, uint32_t accumulate) {
+  asm volatile("{\n.reg .pred p, q;\n.reg .b64 a, b;\nmov.b64 a, {%1, %6};\nmov.b64 b, {%2, %6};\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+               "@q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %3, p;\n}\n"
+               ::"r"(tmem_d), "r"(a_low), "r"(b_low), "r"(kB2Idesc), "r"(accumulate), "r"(leader), "r"(kUmmaDescHigh) : "memory");
+}
+// Arrive, once the MMAs issued so far are done, on the barrier at this offset in both blocks of the pair.
+__device__ __forceinline__ void b2_commit_both(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
+               ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ bool b2_wait_cluster(uint32_t bar, uint32_t parity) {
+  for (uint32_t i = 0; i < (1u << 18); ++i) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000u) : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+
+// An arrival at the even block's barrier without a fence: what it orders is the reading of tensor memory, which tcgen05.fence has ordered (with
+// .release.cluster a step waits for a fence of the warp's whole memory traffic: 2,048 x 4,096 -> 6,144 took XX us, YY so).
+__device__ __forceinline__ void b2_arrive_even(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_bar) : "memory");
+}
+
+struct B2Args {
+  const float* x_scales;       // [runs, lds]
+  int64_t lds;
+  const float* w_scales;       // [rows of scales, runs]
+  int scale_rows, pairs, M, N, runs;
+  int* error_word;
+};
+
+__device__ __forceinline__ float b2_silu_times(float g, float u) {
+  // (g / (1 + e^-g) * u with the approximate exponential and reciprocal, a few units in the last place: a tile takes 128 of them a thread.  Where
+  // the reciprocal would be below 2^-126, at g under -87, it is 0.)
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-g)));
+  return g * r * u;
+}
+
+// Persistent: pair p walks the tiles t = p, p + pairs, ...; tile t is row tile t % m_tiles of feature tile t / m_tiles, so pairs that run together
+// share slices of w.
+template <bool SWIGLU, typename TO>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kB2Threads, 1)
+block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const B2Args a,
+                         TO* __restrict__ out, int64_t ldo, int wide_stores) {
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t bars = base + kB2Stages * kB2Stage;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (kB2Stages + s); };
+  auto acc_full_bar = [&](int b) { return bars + 8u * (2 * kB2Stages + b); };
+  auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * kB2Stages + 2 + b); };
+  const uint32_t tmem_slot = bars + 8u * (2 * kB2Stages + 4);
+  volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem_raw + (tmem_slot - smem_u32(smem_raw)));
+
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();                    // 0: the even block of the pair, which issues the MMAs
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int m_tiles = (a.M + 255) >> 8, num_tiles = m_tiles * ((a.N + 255) >> 8);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kB2Stages; ++s) {
+      mbar_init(full_bar(s), 1);          // (used in the even block: its producer's arrival, plus the bytes of both)
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full_bar(b), 1);
+      mbar_init(acc_empty_bar(b), 16);    // (used in the even block: eight summing warps of each block)
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tmem_slot), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  cluster_sync_all();                                      // both blocks have their barriers before either is signalled
+  asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot_ptr, 0);
+  pdl_wait();
+  pdl_trigger();
+
+  if (warp >= 4) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;\n");
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    int b = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int t = pair; t < num_tiles && ok; t += pairs) {
+      const int n_tile = t / m_tiles, row = (t - n_tile * m_tiles) * 256 + (int)rank * 128 + quarter * 32 + lane;
+      const int col0 = n_tile * 256 + half * 128;
+      // (features beyond the last have some scale of the matrix: they are not stored)
+      const float* xs = a.x_scales + min(row, a.M - 1);
+      const int block = a.pairs ? n_tile * 2 : n_tile * 2 + half;
+      const float* we = a.w_scales + (size_t)min(block, a.scale_rows - 1) * a.runs;
+      const float* wo = a.pairs ? we + a.runs : we;
+      f32x2 sum[64];
+#pragma unroll
+      for (int c = 0; c < 64; ++c) sum[c] = f2_pack(0.f, 0.f);
+      // a step's scales are asked for two steps ahead, into the registers of the step before last (a move from one to the other would wait)
+      float x[2], e[2], o[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = min(i, a.runs - 1);
+        x[i] = xs[(size_t)at * a.lds]; e[i] = we[at]; o[i] = wo[at];
+      }
+      auto step = [&](int kb, int i) {
+        const f32x2 scale = f2_pack(x[i] * e[i], x[i] * o[i]);
+        const int at = min(kb + 2, a.runs - 1);
+        x[i] = xs[(size_t)at * a.lds]; e[i] = we[at]; o[i] = wo[at];
+        if (!mbar_wait_warp(acc_full_bar(b), acc_phase)) {
+          if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00D3);
+          ok = false;
+          return;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + b * 256 + half * 128;
+        uint32_t v[2][32];
+        tmem_ld32(acc, v[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+          if (c < 3) tmem_ld32(acc + 32 * (c + 1), v[(c + 1) & 1]);
+          else {                               // read: tell the MMA warp (in the even block)
+            asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) b2_arrive_even(map_to_cta(acc_empty_bar(b), 0));
+          }
+#pragma unroll
+          for (int q = 0; q < 16; ++q)
+            sum[16 * c + q] = f2_fma(f2_pack(__uint_as_float(v[c & 1][2 * q]), __uint_as_float(v[c & 1][2 * q + 1])), scale, sum[16 * c + q]);
+        }
+        if (++b == 2) { b = 0; acc_phase ^= 1; }
+      };
+#pragma unroll 1
+      for (int kb = 0; kb < a.runs && ok; kb += 2) {
+        step(kb, 0);
+        if (kb + 1 < a.runs && ok) step(kb + 1, 1);
+      }
+      if (!ok || row >= a.M) continue;
+      constexpr int kOut = SWIGLU ? 64 : 128;                  // outputs of this thread
+      const int first = SWIGLU ? col0 >> 1 : col0, n_out = SWIGLU ? a.N >> 1 : a.N;
+      TO* dst = out + (size_t)row * ldo + first;
+      constexpr int kVec = 16 / sizeof(TO);
+#pragma unroll
+      for (int c = 0; c < kOut; c += kVec) {
+        float y[kVec];
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          if constexpr (SWIGLU) {
+            float g, u;
+            f2_unpack(sum[c + j], g, u);
+            y[j] = b2_silu_times(g, u);
+          } else {
+            float lo, hi;
+            f2_unpack(sum[(c + j) >> 1], lo, hi);
+            y[j] = j & 1 ? hi : lo;
+          }
+        }
+        if (wide_stores && first + c + kVec <= n_out) {
+          uint4 w;
+          if constexpr (sizeof(TO) == 2) {
+            __nv_bfloat162 p[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = __floats2bfloat162_rn(y[2 * j], y[2 * j + 1]);
+            w = *reinterpret_cast<const uint4*>(p);
+          } else {
+            w = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+          }
+          *reinterpret_cast<uint4*>(dst + c) = w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < kVec; ++j)
+            if (first + c + j < n_out) dst[c + j] = from_f32<TO>(y[j]);
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;\n");
+    if (warp == 0) {
+      const uint32_t leader = umma_leader();
+      int s = 0;
+      uint32_t phase = 1;
+      bool ok = true;
+      for (int t = pair; t < num_tiles && ok; t += pairs) {
+        const int n_tile = t / m_tiles, m0 = (t - n_tile * m_tiles) * 256 + (int)rank * 128, n0 = n_tile * 256 + (int)rank * 128;
+        for (int kb = 0; kb < a.runs; ++kb) {
+          if (!mbar_wait_warp(empty_bar(s), phase)) {
+            if (a.error_word && leader) atomicExch(a.error_word, 0x7C00D1);
+            ok = false;
+            break;
+          }
+          if (leader) {
+            if (rank == 0) mbar_expect_tx(full_bar(s), 2 * kB2Stage);
+            const uint32_t bar0 = map_to_cta(full_bar(s), 0);
+            b2_tma_load(base + s * kB2Stage, &map_x, kb * kBlk, m0, bar0);
+            b2_tma_load(base + s * kB2Stage + kB2Half, &map_w, kb * kBlk, n0, bar0);
+          }
+          __syncwarp();
+          if (++s == kB2Stages) { s = 0; phase ^= 1; }
+        }
+      }
+    } else if (warp == 1) {
+      if (rank == 0) {
+        const uint32_t leader = umma_leader();
+        int s = 0, b = 0;
+        uint32_t phase = 0, acc_phase = 1;
+        bool ok = true;
+        for (int t = pair; t < num_tiles && ok; t += pairs) {
+          for (int kb = 0; kb < a.runs; ++kb) {
+            if (!__all_sync(0xffffffffu, b2_wait_cluster(acc_empty_bar(b), acc_phase))) {      // both blocks have read this accumulator
+              if (a.error_word && leader) atomicExch(a.error_word, 0x7C00D4);
+              ok = false;
+              break;
+            }
+            if (!__all_sync(0xffffffffu, b2_wait_cluster(full_bar(s), phase))) {
+              if (a.error_word && leader) atomicExch(a.error_word, 0x7C00D2);
+              ok = false;
+              break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+            const uint32_t x_src = umma_low_k128(base + s * kB2Stage), w_src = x_src + (kB2Half >> 4);
+  #pragma unroll
+            for (int k = 0; k < 4; ++k) b2_umma(leader, tmem_base + b * 256, x_src + 2 * k, w_src + 2 * k, k != 0);
+            if (leader) {
+              b2_commit_both(acc_full_bar(b));
+              b2_commit_both(empty_bar(s));      // the stage is free in both blocks once these MMAs have read it
+            }
+            __syncwarp();
+            if (++s == kB2Stages) { s = 0; phase ^= 1; }
+            if (++b == 2) { b = 0; acc_phase ^= 1; }
+          }
+        }
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  cluster_sync_all();   // neither block leaves (or frees tensor memory) while its partner may still signal it
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(512u) : "memory");
+  }
+}
+
+template <bool SWIGLU, typename TO>
+static int launch_b2(const CUtensorMap& map_x, const CUtensorMap& map_w, const B2Args& a, void* out, int64_t ldo, cudaStream_t stream) {
+  auto kern = block_scaled_2cta_kernel<SWIGLU, TO>;
+  static bool allowed[64];      // (by device: the attribute belongs to its context)
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess && !(device < 64 && allowed[device])) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kB2Smem);
+  if (e != cudaSuccess) return (int)e;
+  if (device < 64) allowed[device] = true;
+  const int64_t tiles = (int64_t)ceil_div(a.M, 256) * ceil_div(a.N, 256);
+  if (tiles > 0x7fffffff) return TIB_E_SIZE;
+  const int wide = ((uintptr_t)out & 15) == 0 && (ldo * sizeof(TO)) % 16 == 0;
+  TIB_LAUNCH_DEPENDENT(kern, 2 * (int)(tiles < 74 ? tiles : 74), kB2Threads, kB2Smem, stream, map_x, map_w, a, (TO*)out, ldo, wide);
+  return TIB_OK;
+}
+
+}  // namespace tib
+
+using namespace tib;
+
+// x: codes [M, runs * 128] and scales [runs, lds] as tib_quantize_rows leaves them; w: codes [N, runs * 128] and scales [scale_rows, runs] (`pairs`:
+// of (gate, up) row pairs, N and scale_rows even); out: [M, N] in out_dtype (row stride ldo), or [M, N / 2] with `swiglu`.
+TIB_API int tib_block_scaled_2cta(const void* x, const float* x_scales, int64_t lds, const void* w, const float* w_scales, int scale_rows, int pairs,
+                                  int swiglu, void* out, int out_dtype, int64_t ldo, int M, int N, int K, int* error_word, cudaStream_t stream) {
+  if (M == 0 || N == 0) return TIB_OK;
+  if (!x || !x_scales || !w || !w_scales || !out || M < 0 || N < 0 || K < 1 || scale_rows < 1) return TIB_E_ARG;
+  if ((swiglu && !pairs) || (pairs && (N % 2 || scale_rows % 2)) || lds < M) return TIB_E_SIZE;
+  if (out_dtype != TIB_BF16 && out_dtype != TIB_F32) return TIB_E_DTYPE;
+  if (((uintptr_t)x | (uintptr_t)w) & 15) return TIB_E_ALIGN;
+  B2Args a;
+  a.x_scales = x_scales; a.lds = lds; a.w_scales = w_scales; a.scale_rows = pairs ? scale_rows - 1 : scale_rows; a.pairs = pairs;
+  a.M = M; a.N = N; a.runs = ceil_div(K, kBlk); a.error_word = error_word;
+  CUtensorMap map_x, map_w;
+  int rc = bs_make_map(&map_x, x, M, (int64_t)a.runs * kBlk, 128);
+  if (rc != TIB_OK) return rc;
+  rc = bs_make_map(&map_w, w, N, (int64_t)a.runs * kBlk, 128);
+  if (rc != TIB_OK) return rc;
+  if (swiglu)
+    return out_dtype == TIB_BF16 ? launch_b2<true, __nv_bfloat16>(map_x, map_w, a, out, ldo, stream) : launch_b2<true, float>(map_x, map_w, a, out, ldo, stream);
+  return out_dtype == TIB_BF16 ? launch_b2<false, __nv_bfloat16>(map_x, map_w, a, out, ldo, stream) : launch_b2<false, float>(map_x, map_w, a, out, ldo, stream);
+}
+
+// The call the Python parts make (common.cuh).
+TIB_PACKED(tib_block_scaled_2cta)

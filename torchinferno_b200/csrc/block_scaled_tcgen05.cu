@@ -3,13 +3,13 @@
 //
 // The weights are the 128-row operand of the MMA and the rows its N dimension: a tile is 128 features x up to NT rows, the rows rounded up to 16
 // only, and the accumulator is the transposed output (TMEM lane = feature, column = row).  A step of the loop is one run: 128 columns, the 128-byte
-// row of the swizzle, four MMAs into an accumulator of its own in tensor memory, which the summing warps take out, multiply by its scales and add to
-// 32-bit sums in registers (packed fp32, two instructions for two sums).  kBufs accumulators rotate, so the tensor cores run ahead of the sums.
-//   warp 0             TMA producer: 16 KB of codes of w a step, and the rows' codes where they exist: boxes of 32 rows that lie side by side, or
-//                      four rows by their numbers at a time (gather4) where they are sorted
+// row of the swizzle, four MMAs into an accumulator of its own in tensor memory, which the summing warps take out and add to 32-bit sums in
+// registers, times the scale of (row, run) and (block of features, run), whose product is made once a row and step (packed fp32, one multiply-add for
+// two sums).  kBufs accumulators rotate, so the tensor cores run ahead of the sums.
+//   warp 0             TMA producer: 16 KB of codes of w a step, and the rows' codes where they exist, in boxes of 32 rows
 //   warp 1             issues tcgen05.mma; owns the TMEM allocation
 //   the next 4 or 8    sums and epilogue (eight for 128 rows: four for each half of the columns)
-//   the last 4         helpers, each every fourth step: the rows' scales into the ring's stage; from rows that are no codes yet they make
+//   the last 2 or 4    helpers, taking turns: the products of scales into the ring's stage; from rows that are no codes yet they (then four) make
 //                      these, straight into the swizzled stage (a step of few rows then has no kernel ahead of its products)
 // A matrix of few tiles is split by runs over a cluster of up to eight blocks, whose sums meet in distributed shared memory, added in the
 // blocks' order.  Weights do not depend on the kernel before: a first ring of them is requested before griddepcontrol.wait (not for sorted rows, whose
@@ -24,12 +24,13 @@ namespace tib {
 constexpr int kBsMaxExperts = 1024, kBsMaxStages = 16;
 constexpr uint32_t kBsWBytes = 128 * kBlk;
 
-template <int NT> struct BsShape {
-  static constexpr int kStorers = NT >= 128 ? 8 : 4, kHelpers = 4, kThreads = 64 + 32 * (kStorers + kHelpers);
+template <int NT, bool CODES> struct BsShape {
+  static constexpr int kStorers = NT >= 128 ? 8 : 4, kHelpers = CODES ? 2 : 4, kThreads = 64 + 32 * (kStorers + kHelpers);
   static constexpr int kBufs = 4, kCols = NT / (kStorers / 4);      // accumulators; columns of a summing thread
   static constexpr uint32_t kTmemCols = kBufs * NT < 32 ? 32 : kBufs * NT;
   static constexpr uint32_t kStage = kBsWBytes + NT * kBlk;
   static constexpr int kRedStride = NT + 4;                         // floats of a feature's sums (16-byte steps that fall on all banks)
+  static constexpr int kScales = 2 * (NT + 4);                      // of a stage: for even features, for odd ones (on other banks)
 };
 
 struct BsTile { int expert, first, rows, feature; };
@@ -54,19 +55,14 @@ __device__ __forceinline__ void umma_f8_warp(uint32_t leader, uint32_t tmem_d, u
                "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, p;\n}\n"
                ::"r"(tmem_d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(leader), "r"(kUmmaDescHigh) : "memory");
 }
-// four rows of 128 bytes by their numbers, one under the other
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int x, const int (&row)[4], uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];\n"
-               ::"r"(dst), "l"(map), "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar) : "memory");
-}
 __device__ __forceinline__ void bs_fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 
 template <int NT, typename TX, typename TO>
-__global__ void __launch_bounds__(BsShape<NT>::kThreads, 1)
+__global__ void __launch_bounds__(BsShape<NT, std::is_same_v<TX, uint8_t>>::kThreads, 1)
 block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const BsArgs a,
                             TO* __restrict__ y, int64_t ldy) {
-  using S = BsShape<NT>;
   constexpr bool kCodes = std::is_same_v<TX, uint8_t>;
+  using S = BsShape<NT, kCodes>;
   extern __shared__ unsigned char smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* smem_gen = smem_raw + (base - smem_u32(smem_raw));
@@ -78,8 +74,8 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
   const uint32_t red_bar = bars + 8u * (2 * kBsMaxStages + 2 * S::kBufs), tmem_slot = red_bar + 8;
   static_assert(8 * (2 * kBsMaxStages + 2 * S::kBufs) + 16 <= 384, "the barriers' share of shared memory");
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem_gen + (tmem_slot - base));
-  float* row_scales = reinterpret_cast<float*>(smem_gen + (bars - base) + 384);           // [stages][NT]
-  float* red = row_scales + a.stages * NT;                                                // [128][kRedStride] in all
+  float* step_scales = reinterpret_cast<float*>(smem_gen + (bars - base) + 384);          // [stages][kScales]
+  float* red = step_scales + a.stages * S::kScales;                                                // [128][kRedStride] in all
   int* tiles_before = reinterpret_cast<int*>(red + 128 * S::kRedStride);                  // [experts + 1] where rows are sorted
 
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -163,10 +159,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     int ahead = 0, it = 0, s = 0;
     uint32_t phase = 1;
     bool ok = true;
-    const bool gather = kCodes && a.offsets && a.x_by_pair;
-    auto bytes = [&](const BsTile& m) {
-      return kBsWBytes + (!kCodes ? 0 : gather ? ((m.rows + 3) >> 2) * 4 * kBlk : ((m.rows + 31) >> 5) * 32 * kBlk);
-    };
+    auto bytes = [&](const BsTile& m) { return kBsWBytes + (kCodes ? ((m.rows + 31) >> 5) * 32 * kBlk : 0); };
     if (!a.offsets) {
       for (int t = cluster_id; t < num_tiles && ahead < a.stages; t += clusters) {
         const BsTile m = tile_of(t);
@@ -180,11 +173,6 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     }
     for (int t = cluster_id; t < num_tiles && ok; t += clusters) {
       const BsTile m = tile_of(t);
-      int rows[NT > 128 ? 2 : 1][4];              // the rows of this lane's gathers
-      if (gather) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) rows[0][j] = source(m, 4 * lane + j);
-      }
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const uint32_t stage = base + s * S::kStage;
         if (it >= ahead) {
@@ -200,9 +188,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
           __syncwarp();
         }
         if constexpr (kCodes) {
-          if (gather) {
-            if (4 * lane < m.rows) tma_gather4(stage + kBsWBytes + lane * 4 * kBlk, &map_x, kb * kBlk, rows[0], full_bar(s));
-          } else if (leader) {
+          if (leader) {
 #pragma unroll
             for (int i = 0; i < NT / 32; ++i)     // (likewise a last box into the next tile's rows, or past the last)
               if (32 * i < m.rows) tma_load_2d(stage + kBsWBytes + i * 32 * kBlk, &map_x, kb * kBlk, m.first + 32 * i, full_bar(s));
@@ -251,46 +237,38 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     if (!a.offsets) pdl_wait();                   // (y may be memory that the kernel before still reads)
     for (int t = cluster_id; t < num_tiles; t += clusters) {
       const BsTile m = tile_of(t);
-      const float* ws = a.w_scales + ((size_t)m.expert * a.scale_rows + bs_scale_row(m.feature, a.pairs)) * a.runs;
       f32x2 sum[S::kCols / 2];
 #pragma unroll
       for (int c = 0; c < S::kCols / 2; ++c) sum[c] = f2_pack(0.f, 0.f);
-      float even = 0.f, odd = 0.f;                // the scales of the next 32 runs, a lane each (of gate and up rows)
       for (int kb = kb0; kb < kb1; ++kb) {
-        const int i = (kb - kb0) & 31;
-        if (i == 0) {
-          const int at = min(kb + lane, a.runs - 1);
-          even = ws[at];
-          odd = a.pairs ? ws[a.runs + at] : even;
-        }
         if (ok && !(mbar_wait_warp(acc_full_bar(b), acc_phase) && mbar_wait_warp(full_bar(s), phase))) {
           if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00C3);
           ok = false;
         }
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        const float w_even = __shfl_sync(0xffffffffu, even, i), w_odd = __shfl_sync(0xffffffffu, odd, i);
-        const float w = lane & 1 ? w_odd : w_even;
-        const f32x2 w2 = f2_pack(w, w);
         const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + b * NT + c0;
-        const float* xs = row_scales + s * NT + c0;
+        const float* scales = step_scales + s * S::kScales + (lane & 1) * (NT + 4) + c0;
+        constexpr int kPart = S::kCols < 32 ? S::kCols : 32;
+        uint32_t v[S::kCols / kPart][kPart];
 #pragma unroll
-        for (int c = 0; c < S::kCols; c += 16) {
-          if (c0 + c < m.rows) {
-            uint32_t v[16];
-            tmem_ld16(acc + c, v);
-            float4 scale[4];
+        for (int p = 0; p < S::kCols / kPart; ++p)
+          if (c0 + p * kPart < m.rows) {
+            if constexpr (kPart == 16) tmem_ld16(acc, v[p]);
+            else tmem_ld32(acc + p * kPart, v[p]);
+          }
+        asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
-            for (int q = 0; q < 4; ++q) scale[q] = reinterpret_cast<const float4*>(xs + c)[q];
-            asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+        for (int p = 0; p < S::kCols / kPart; ++p)
+          if (c0 + p * kPart < m.rows) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              f32x2& lo = sum[c / 2 + 2 * q];
-              f32x2& hi = sum[c / 2 + 2 * q + 1];
-              lo = f2_fma(f2_pack(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1])), f2_mul(f2_pack(scale[q].x, scale[q].y), w2), lo);
-              hi = f2_fma(f2_pack(__uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3])), f2_mul(f2_pack(scale[q].z, scale[q].w), w2), hi);
+            for (int q = 0; q < kPart; q += 4) {
+              const ulonglong2 scale = *reinterpret_cast<const ulonglong2*>(scales + p * kPart + q);
+              f32x2& lo = sum[(p * kPart + q) / 2];
+              f32x2& hi = sum[(p * kPart + q) / 2 + 1];
+              lo = f2_fma(f2_pack(__uint_as_float(v[p][q]), __uint_as_float(v[p][q + 1])), scale.x, lo);
+              hi = f2_fma(f2_pack(__uint_as_float(v[p][q + 2]), __uint_as_float(v[p][q + 3])), scale.y, hi);
             }
           }
-        }
         asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
         __syncwarp();
         if (lane == 0) {
@@ -365,22 +343,21 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     if (!a.offsets) pdl_wait();
     for (int t = cluster_id; t < num_tiles && ok; t += clusters) {
       const BsTile m = tile_of(t);
-      int from[(NT + 31) / 32];                   // (codes) the rows whose scales this lane copies
-      if constexpr (kCodes) {
-#pragma unroll
-        for (int i = 0; i < (NT + 31) / 32; ++i) from[i] = source(m, lane + 32 * i);
-      }
+      const float* ws = a.w_scales + ((size_t)m.expert * a.scale_rows + bs_scale_row(m.feature, a.pairs)) * a.runs;
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        if ((it & (S::kHelpers - 1)) == helper) {
-          float* scales = row_scales + s * NT;
+        if (it % S::kHelpers == helper) {
+          float* scales = step_scales + s * S::kScales;
+          const float even = ws[kb], odd = a.pairs ? ws[a.runs + kb] : even;
           if constexpr (kCodes) {
-            float v[(NT + 31) / 32];
+            float v[NT / 32];
 #pragma unroll
-            for (int i = 0; i < (NT + 31) / 32; ++i) v[i] = a.x_scales[(size_t)kb * a.lds + from[i]];
+            for (int i = 0; i < NT / 32; ++i) v[i] = a.x_scales[(size_t)kb * a.lds + m.first + min(lane + 32 * i, m.rows - 1)];
             if (!mbar_wait_warp(empty_bar(s), phase)) ok = false;
 #pragma unroll
-            for (int i = 0; i < (NT + 31) / 32; ++i)
-              if (lane + 32 * i < NT) scales[lane + 32 * i] = v[i];
+            for (int i = 0; i < NT / 32; ++i) {
+              scales[lane + 32 * i] = v[i] * even;
+              scales[NT + 4 + lane + 32 * i] = v[i] * odd;
+            }
           } else {
             // eight lanes a row, sixteen columns each; two rows a lane at a time
             const TX* x = reinterpret_cast<const TX*>(a.x);
@@ -418,7 +395,10 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
                   w[j] = bs_codes4(v[h][4 * j] * inverse, v[h][4 * j + 1] * inverse, v[h][4 * j + 2] * inverse, v[h][4 * j + 3] * inverse);
                 if (r < m.rows && ok) {
                   *reinterpret_cast<uint4*>(codes + r * kBlk + ((eighth ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                  if (eighth == 0) scales[r] = scale;
+                  if (eighth == 0) {
+                    scales[r] = scale * even;
+                    scales[NT + 4 + r] = scale * odd;
+                  }
                 }
               }
             }
@@ -445,22 +425,10 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
   }
 }
 
-// Codes [rows, bytes a row], read in boxes of box_rows x 128 with 128-byte swizzle (box_rows 1: by gathers of four).
-static int bs_make_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t bytes, int box_rows) {
-  EncodeTiledFn fn = encode_tiled_fn();
-  if (!fn) return TIB_E_ARG;
-  const cuuint64_t dims[2] = {(cuuint64_t)bytes, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)bytes};
-  const cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
-  const cuuint32_t elem[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? TIB_OK : TIB_E_ARG;
-}
-
 template <int NT>
 static constexpr uint32_t bs_smem(int stages, int experts) {
-  return 1024u + stages * (BsShape<NT>::kStage + NT * 4) + 384u + 128 * BsShape<NT>::kRedStride * 4 + 4 * (experts + 1);
+  using S = BsShape<NT, true>;
+  return 1024u + stages * (S::kStage + S::kScales * 4) + 384u + 128 * S::kRedStride * 4 + 4 * (experts + 1);
 }
 
 template <int NT, typename TX, typename TO>
@@ -481,7 +449,7 @@ static int launch_block_scaled(const CUtensorMap& map_w, const CUtensorMap& map_
   if (e != cudaSuccess) return (int)e;
   if (device < 64) allowed[device] = true;
   cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(BsShape<NT>::kThreads);
+  cfg.blockDim = dim3(BsShape<NT, std::is_same_v<TX, uint8_t>>::kThreads);
   cfg.dynamicSmemBytes = bs_smem<NT>(a.stages, experts);
   cfg.stream = stream;
   cfg.gridDim = dim3((unsigned)grid);
@@ -512,7 +480,7 @@ static int bs_splits(int64_t tiles, int runs) {
 using namespace tib;
 
 // x_dtype TIB_BF16 or TIB_F32: rows [rows, K] (row stride ldx) that are quantised on the way, once for each tile of 128 features; -1: codes
-// [x_rows, runs * 128] and scales [runs, lds] as tib_quantize_rows leaves them.  w: codes [experts, N, runs * 128] and scales
+// [x_rows, runs * 128] and scales [runs, lds] as tib_quantize_rows leaves them, row m of them for row m of y.  w: codes [experts, N, runs * 128] and scales
 // [experts, scale_rows, runs] (`pairs`: of (gate, up) row pairs); y: [M, N] in y_dtype (row stride ldy), or [M, N / 2] of a gated activation.
 // offsets [experts + 1] and order [M]: rows sorted by expert as tib_moe_expert_product takes them; offsets null: one matrix for all rows.
 TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, int x_rows, const float* x_scales, int64_t lds, const void* w,
@@ -522,7 +490,7 @@ TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, in
   if (M == 0 || N == 0) return TIB_OK;
   const bool is_codes = x_dtype < 0;
   if (!x || !w || !w_scales || !y || M < 0 || N < 0 || K < 1 || experts < 1 || top < 1 || x_rows < 1) return TIB_E_ARG;
-  if ((is_codes && !x_scales) || (offsets && !order) || (row_scale && !order)) return TIB_E_ARG;
+  if ((is_codes && (!x_scales || (offsets && x_by_pair) || x_rows < M || lds < M)) || (offsets && !order) || (row_scale && !order)) return TIB_E_ARG;
   if (act < MOE_ACT_NONE || act > MOE_ACT_GELU || (moe_act_gated(act) && !pairs) || (pairs && N % 2)) return TIB_E_SIZE;
   if (x_dtype > TIB_BF16 || (y_dtype != TIB_BF16 && y_dtype != TIB_F32)) return TIB_E_DTYPE;
   if (experts > kBsMaxExperts || (int64_t)experts * N > 0x7fffffff - 128) return TIB_E_SIZE;
@@ -538,7 +506,7 @@ TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, in
   if (rc != TIB_OK) return rc;
   map_x = map_w;
   if (is_codes) {
-    rc = bs_make_map(&map_x, x, x_rows, (int64_t)a.runs * kBlk, offsets && x_by_pair ? 1 : 32);
+    rc = bs_make_map(&map_x, x, x_rows, (int64_t)a.runs * kBlk, 32);
     if (rc != TIB_OK) return rc;
   }
   const int rows = offsets ? ceil_div(M, experts) : M;      // (of an expert, on average)

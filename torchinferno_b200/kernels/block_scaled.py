@@ -83,20 +83,16 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return codes[:, :x.shape[1]], scales[:, :x.shape[0]].t()
 
 
-def _quantized(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """Codes and scales as the products read them: columns padded to whole runs; a run's scales side by side, rows rounded up to 4."""
+def _quantized(x: torch.Tensor, routing: tuple[torch.Tensor, torch.Tensor, int] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes and scales as the products read them: columns padded to whole runs; a run's scales side by side, rows rounded up to 4.  ``routing`` =
+    (offsets, order, top): the rows of the pairs sorted by expert."""
     if x.dim() != 2 or x.shape[1] == 0:
         raise ops.KernelError(f"rows to quantise must be [rows, columns], got {tuple(x.shape)}")
-    rows, runs = x.shape[0], blocks(x.shape[1])
+    rows, runs = x.shape[0] if routing is None else routing[1].numel(), blocks(x.shape[1])
     codes = torch.empty((rows, runs * BLOCK), dtype=CODE_DTYPE, device=x.device)
     scales = torch.empty((runs, -(-rows // 4) * 4), dtype=torch.float32, device=x.device)
-    ops.quantize_rows(x, codes, scales)
+    ops.quantize_rows(x, codes, scales, routing)
     return codes, scales
-
-
-def _rows_for(x: torch.Tensor, rows: int, few: int) -> tuple[torch.Tensor, torch.Tensor | None]:
-    """What a product over so many ``rows`` of a matrix reads: up to ``few`` of them its kernel quantises itself, more are quantised ahead of it."""
-    return (x, None) if rows <= few else _quantized(x)
 
 
 def _laid_out(matrices: Sequence[BlockScaledMatrix], ups: Sequence[BlockScaledMatrix] | None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -198,7 +194,7 @@ class BlockScaledWeight:
         out = self._checked(x, out_dtype, self.out_features, out)
         if x.shape[0] == 0:
             return out
-        rows = _rows_for(x, x.shape[0], FEW_ROWS)
+        rows = (x, None) if x.shape[0] <= FEW_ROWS else _quantized(x)
         for first, codes, scales in self.parts:
             ops.block_scaled_product(*rows, codes, scales, out if len(self.parts) == 1 else out[:, first:first + codes.shape[1]],
                                      columns=self.in_features, paired=self.epilogue == "swiglu", error_word=error_word)
@@ -212,7 +208,8 @@ class BlockScaledWeight:
         if x.shape[0] == 0:
             return out
         _, codes, scales = self.parts[0]
-        return ops.block_scaled_product(*_rows_for(x, x.shape[0], FEW_ROWS), codes, scales, out, columns=self.in_features, paired=True, act="swiglu",
+        rows = (x, None) if x.shape[0] <= FEW_ROWS else _quantized(x)
+        return ops.block_scaled_product(*rows, codes, scales, out, columns=self.in_features, paired=True, act="swiglu",
                                         error_word=error_word)
 
 
@@ -258,5 +255,9 @@ class BlockScaledExperts:
                 raise ops.KernelError("moe_expert_product: row_scale must hold one factor per pair")
         if pairs == 0:
             return y
-        return ops.block_scaled_product(*_rows_for(x, -(-pairs // self.experts), FEW_EXPERT_ROWS), self.codes, self.scales, y,
-                                        columns=self.in_features, paired=self.paired, act=act, limit=limit, alpha=alpha, routing=(offsets, order, top, x_by_pair), row_scale=row_scale, error_word=error_word)
+        if pairs <= FEW_EXPERT_ROWS * self.experts:
+            rows, routing = (x, None), (offsets, order, top, x_by_pair)
+        else:                                   # (the pairs' rows, sorted on the way)
+            rows, routing = _quantized(x if x_by_pair else x[:pairs], (offsets, order, top) if x_by_pair else None), (offsets, order, top, False)
+        return ops.block_scaled_product(*rows, self.codes, self.scales, y, columns=self.in_features, paired=self.paired, act=act, limit=limit,
+                                        alpha=alpha, routing=routing, row_scale=row_scale, error_word=error_word)

@@ -1262,15 +1262,22 @@ def _on_current_device(t: torch.Tensor, name: str) -> None:
         raise KernelError(f"{name} is on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
 
 
-def quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
-    """Codes [rows, K rounded up to 128] (8 bits) and scales [runs of 128 columns, at least rows] of the rows ``x`` [rows, K]."""
+def quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, routing: tuple[torch.Tensor, torch.Tensor, int] | None = None) -> None:
+    """Codes [rows, K rounded up to 128] (8 bits) and scales [runs of 128 columns, at least rows] of the rows ``x`` [rows, K].  ``routing`` =
+    (offsets, order, top): one row of codes for each pair sorted by expert, made of row order[s] // top of ``x`` (none behind the last expert's)."""
     _on_current_device(x, "x"), _rows_of(x, "x")
     _need(codes, "codes", torch.float8_e4m3fn), _need(scales, "scales", torch.float32)
-    rows, k = x.shape
+    offsets, order, top = routing if routing is not None else (None, None, 1)
+    rows, k = x.shape[0] if order is None else order.numel(), x.shape[1]
     if codes.shape != (rows, -(-k // 128) * 128) or scales.dim() != 2 or scales.shape[0] != -(-k // 128) or scales.shape[1] < rows:
         raise KernelError("quantize_rows: shapes do not fit")
     _check("quantize_rows", lib().tib_quantize_rows(_ptr(x), _code(x.dtype), x.stride(0), _ptr(codes), codes.stride(0), _ptr(scales),
-                                                    scales.shape[1], rows, k, _stream()))
+                                                    scales.shape[1], rows, k, _ptr(order), top, 0 if offsets is None else _ptr(offsets[-1:]), _stream()))
+
+
+def block_scaled_pairs_of_sms(rows: int, features: int) -> bool:
+    """Whether a product of codes runs on pairs of SMs, in tiles of 256 rows x 256 features."""
+    return -(-rows // 256) * -(-features // 256) >= 24
 
 
 def block_scaled_product(x: torch.Tensor, scales: torch.Tensor | None, w: torch.Tensor, w_scales: torch.Tensor, y: torch.Tensor, *,
@@ -1289,6 +1296,11 @@ def block_scaled_product(x: torch.Tensor, scales: torch.Tensor | None, w: torch.
     if (k != -(-columns // 128) * 128 or x.shape[1] != (columns if scales is None else k) or w_scales.shape[0] != experts or w_scales.shape[2] != k // 128
             or y.shape[1] != (n // 2 if act in MOE_GATED else n) or (routing is None and y.shape[0] != x.shape[0])):
         raise KernelError("block_scaled_product: shapes do not fit")
+    if scales is not None and routing is None and act in ("none", "swiglu") and block_scaled_pairs_of_sms(y.shape[0], n):
+        _check("block_scaled_product", lib().tib_block_scaled_2cta(
+            _ptr(x), _ptr(scales), scales.shape[1], _ptr(w), _ptr(w_scales), w_scales.shape[1], int(paired), int(act == "swiglu"), _ptr(y), _code(y.dtype),
+            y.stride(0), y.shape[0], n, columns, _ptr(error_word), _stream()))
+        return y
     _check("block_scaled_product", lib().tib_block_scaled_tcgen05(
         _ptr(x), _code(x.dtype) if scales is None else -1, x.stride(0), x.shape[0], _ptr(scales), 0 if scales is None else scales.shape[1], _ptr(w),
         _ptr(w_scales), w_scales.shape[1], int(paired), _ptr(y), _code(y.dtype), y.stride(0), y.shape[0], n, columns, _ptr(offsets), _ptr(order), experts,
