@@ -30,6 +30,14 @@ __device__ __forceinline__ void bs_run_scale(uint32_t largest, float& scale, flo
   if (largest >= 0x7f800000u) scale = inverse = __uint_as_float(0x7fc00000u);
 }
 
+// 1 / (1 + e^-x) with the approximate exponential and reciprocal: a relative error of a few 2^-23 (1 + |x|).  Where e^-x is beyond 2^126, at x under
+// -87, it is 0.
+__device__ __forceinline__ float bs_sigmoid(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-x)));
+  return r;
+}
+
 // two floats to two codes (the first in the lower byte), to nearest, ties to even; a NaN stays one
 __device__ __forceinline__ uint32_t bs_codes2(float lo, float hi) {
   uint16_t r;

@@ -4,7 +4,7 @@
 // Two blocks (a cluster of two) compute a tile of 256 rows x 256 features, as in gemm_tcgen05_2cta.cu: block r holds rows r * 128 .. of the
 // x slice and features r * 128 .. of the w slice, and gets rows r * 128 .. of the accumulator.  A step is one run: 128 columns, the 128-byte row of the
 // swizzle, four MMAs into one of two accumulators of 256 columns.  The sums over runs are taken in registers, since every run has its own scales:
-// eight warps, 32 rows x 128 features each, read the accumulator in pieces of 32 columns, the next piece on its way under the multiply-adds of
+// eight warps, 32 rows x 128 features each, read the accumulator in pieces of 16 columns, the next piece on its way under the multiply-adds of
 // the last, and add it to 128 sums a thread, times the scale of (its row, run) and (the features' block, run).  Two sums are one packed
 // multiply-add; in a matrix of (gate, up) row pairs the two have different scales, which the packed form takes as it comes.
 //   warp 0       TMA producer into a ring of six stages      warp 1 (of the even block)   issues the MMAs; either owns its block's TMEM
@@ -60,14 +60,6 @@ struct B2Args {
   int scale_rows, pairs, M, N, runs;
   int* error_word;
 };
-
-__device__ __forceinline__ float b2_silu_times(float g, float u) {
-  // (g / (1 + e^-g) * u with the approximate exponential and reciprocal, a few units in the last place: a tile takes 128 of them a thread.  Where
-  // the reciprocal would be below 2^-126, at g under -87, it is 0.)
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-g)));
-  return g * r * u;
-}
 
 // Persistent: pair p walks the tiles t = p, p + pairs, ...; tile t is row tile t % m_tiles of feature tile t / m_tiles, so pairs that run together
 // share slices of w.
@@ -148,20 +140,20 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
         }
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + b * 256 + half * 128;
-        uint32_t v[2][32];
-        tmem_ld32(acc, v[0]);
+        uint32_t v[2][16];
+        tmem_ld16(acc, v[0]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 8; ++c) {
           asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-          if (c < 3) tmem_ld32(acc + 32 * (c + 1), v[(c + 1) & 1]);
+          if (c < 7) tmem_ld16(acc + 16 * (c + 1), v[(c + 1) & 1]);
           else {                               // read: tell the MMA warp (in the even block)
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
             __syncwarp();
             if (lane == 0) b2_arrive_even(map_to_cta(acc_empty_bar(b), 0));
           }
 #pragma unroll
-          for (int q = 0; q < 16; ++q)
-            sum[16 * c + q] = f2_fma(f2_pack(__uint_as_float(v[c & 1][2 * q]), __uint_as_float(v[c & 1][2 * q + 1])), scale, sum[16 * c + q]);
+          for (int q = 0; q < 8; ++q)
+            sum[8 * c + q] = f2_fma(f2_pack(__uint_as_float(v[c & 1][2 * q]), __uint_as_float(v[c & 1][2 * q + 1])), scale, sum[8 * c + q]);
         }
         if (++b == 2) { b = 0; acc_phase ^= 1; }
       };
@@ -183,7 +175,7 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
           if constexpr (SWIGLU) {
             float g, u;
             f2_unpack(sum[c + j], g, u);
-            y[j] = b2_silu_times(g, u);
+            y[j] = g * bs_sigmoid(g) * u;
           } else {
             float lo, hi;
             f2_unpack(sum[(c + j) >> 1], lo, hi);
@@ -241,13 +233,13 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
         bool ok = true;
         for (int t = pair; t < num_tiles && ok; t += pairs) {
           for (int kb = 0; kb < a.runs; ++kb) {
-            if (!__all_sync(0xffffffffu, b2_wait_cluster(acc_empty_bar(b), acc_phase))) {      // both blocks have read this accumulator
-              if (a.error_word && leader) atomicExch(a.error_word, 0x7C00D4);
+            if (!__all_sync(0xffffffffu, b2_wait_cluster(full_bar(s), phase))) {
+              if (a.error_word && leader) atomicExch(a.error_word, 0x7C00D2);
               ok = false;
               break;
             }
-            if (!__all_sync(0xffffffffu, b2_wait_cluster(full_bar(s), phase))) {
-              if (a.error_word && leader) atomicExch(a.error_word, 0x7C00D2);
+            if (!__all_sync(0xffffffffu, b2_wait_cluster(acc_empty_bar(b), acc_phase))) {      // both blocks have read this accumulator
+              if (a.error_word && leader) atomicExch(a.error_word, 0x7C00D4);
               ok = false;
               break;
             }

@@ -9,8 +9,10 @@
 //   warp 0             TMA producer: 16 KB of codes of w a step, and the rows' codes where they exist, in boxes of 32 rows
 //   warp 1             issues tcgen05.mma; owns the TMEM allocation
 //   the next 4 or 8    sums and epilogue (eight for 128 rows: four for each half of the columns)
-//   the last 2 or 4    helpers, taking turns: the products of scales into the ring's stage; from rows that are no codes yet they (then four) make
+//   the last 2 or 4    helpers, taking turns: the products of scales into a ring of their own; from rows that are no codes yet they (then four) make
 //                      these, straight into the swizzled stage (a step of few rows then has no kernel ahead of its products)
+// A summing thread takes two columns in eight of four features (tcgen05.ld 16x256b), and so reads a quarter of a step's scales: shared memory is what
+// the MMAs of 128 x 128 x 128 wait for (their operands and the copies that bring them take it for 512 of a step's cycles, the tensor cores 256).
 // A matrix of few tiles is split by runs over a cluster of up to eight blocks, whose sums meet in distributed shared memory, added in the
 // blocks' order.  Weights do not depend on the kernel before: a first ring of them is requested before griddepcontrol.wait (not for sorted rows, whose
 // tiles that kernel's counts decide).  Every wait is bounded and reports in error_word; a warp that gave up goes through the motions to the
@@ -21,7 +23,8 @@
 
 namespace tib {
 
-constexpr int kBsMaxExperts = 1024, kBsMaxStages = 16;
+constexpr int kBsMaxExperts = 1024, kBsMaxStages = 16, kBsSlots = 16;      // (slots: of the ring of scales)
+constexpr uint32_t kBsBarBytes = 640;
 constexpr uint32_t kBsWBytes = 128 * kBlk;
 
 template <int NT, bool CODES> struct BsShape {
@@ -29,9 +32,11 @@ template <int NT, bool CODES> struct BsShape {
   static constexpr int kBufs = 4, kCols = NT / (kStorers / 4);      // accumulators; columns of a summing thread
   static constexpr uint32_t kTmemCols = kBufs * NT < 32 ? 32 : kBufs * NT;
   static constexpr uint32_t kStage = kBsWBytes + NT * kBlk;
-  static constexpr int kRedStride = NT + 4;                         // floats of a feature's sums (16-byte steps that fall on all banks)
-  static constexpr int kScales = 2 * (NT + 4);                      // of a stage: for even features, for odd ones (on other banks)
+  static constexpr int kScales = 2 * NT + 8;                        // of a step: for even features, behind them for odd ones (on other banks)
 };
+
+// (a column's 128 / splits sums and four more: the eight features and four columns that a warp writes at a time then fall on all banks)
+template <int NT> __host__ __device__ constexpr int bs_red_floats(int splits) { return NT * (128 + 4 * splits); }
 
 struct BsTile { int expert, first, rows, feature; };
 
@@ -41,7 +46,7 @@ struct BsArgs {
   const float* x_scales;       // [runs, lds] beside codes
   int64_t lds;
   const float* w_scales;
-  int scale_rows, pairs, vec;
+  int scale_rows, pairs, vec, wide;      // vec: rows of x, wide: of y, are 16-byte aligned
   int M, N, K, runs, stages;
   const int* offsets;          // null: one matrix
   const int* order;
@@ -55,7 +60,87 @@ __device__ __forceinline__ void umma_f8_warp(uint32_t leader, uint32_t tmem_d, u
                "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, p;\n}\n"
                ::"r"(tmem_d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(leader), "r"(kUmmaDescHigh) : "memory");
 }
+// 16 lanes of tensor memory, COLS columns of them: register 4 j + 2 h + i is lane (thread / 4) + 8 h, column 8 j + 2 (thread % 4) + i
+template <int COLS> __device__ __forceinline__ void tmem_ld_16x256b(uint32_t taddr, uint32_t (&r)[COLS / 2]) {
+  static_assert(COLS == 16 || COLS == 32 || COLS == 64, "columns");
+  if constexpr (COLS == 16)
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr));
+  else if constexpr (COLS == 32)
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr));
+  else
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]) : "r"(taddr));
+}
 __device__ __forceinline__ void bs_fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+
+// A block's share of a tile from its sums in shared memory (and the other blocks' beside them) through the activation to y: eight outputs of a
+// column a thread and turn.  A function for each activation: with the choice inside the loop a turn took 1,250 cycles, most of them fetching code.
+template <int ACT, int NT, typename TO>
+__device__ __forceinline__ void bs_finish(const float* red, int log_splits, int rank, const BsTile& m, const BsArgs& a, TO* __restrict__ y, int64_t ldy,
+                                          int thread, int threads) {
+  constexpr int kGated = moe_act_gated(ACT);
+  const int per = 128 >> log_splits, stride = per + 4, splits = 1 << log_splits;
+  const int log_wide = 4 - log_splits - kGated;           // eights of outputs in a column
+  const int first_out = (m.feature + rank * per) >> kGated, n_out = a.N >> kGated;
+#pragma unroll 1
+  for (int i = thread; i < m.rows << log_wide; i += threads) {
+    const int c = i >> log_wide, f = (i - (c << log_wide)) * 8;
+    if (first_out + f >= n_out) continue;
+    float v[8 << kGated];
+    const float* from = red + c * stride + (f << kGated);
+#pragma unroll
+    for (int j = 0; j < 8 << kGated; j += 4) {
+      const float4 p = *reinterpret_cast<const float4*>(from + j);
+      v[j] = p.x; v[j + 1] = p.y; v[j + 2] = p.z; v[j + 3] = p.w;
+    }
+    for (int r = 1; r < splits; ++r) {
+      from += NT * stride;
+#pragma unroll
+      for (int j = 0; j < 8 << kGated; j += 4) {
+        const float4 p = *reinterpret_cast<const float4*>(from + j);
+        v[j] += p.x; v[j + 1] += p.y; v[j + 2] += p.z; v[j + 3] += p.w;
+      }
+    }
+    if (a.ep.row_scale) {
+      const float scale = a.ep.row_scale[a.order[m.first + c]];
+#pragma unroll
+      for (int j = 0; j < 8 << kGated; ++j) v[j] *= scale;
+    }
+    float out[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (ACT == MOE_ACT_SWIGLU) out[j] = v[2 * j] * bs_sigmoid(v[2 * j]) * v[2 * j + 1];
+      else if constexpr (ACT == MOE_ACT_GLU_CLAMP) {
+        const float g = fminf(v[2 * j], a.ep.limit), u = fminf(fmaxf(v[2 * j + 1], -a.ep.limit), a.ep.limit);
+        out[j] = g * bs_sigmoid(a.ep.alpha * g) * (u + 1.f);
+      } else if constexpr (ACT == MOE_ACT_SILU) out[j] = v[j] * bs_sigmoid(v[j]);
+      else out[j] = moe_act(v[j], ACT);
+    }
+    TO* dst = y + (size_t)(m.first + c) * ldy + first_out + f;
+    if (a.wide && first_out + f + 8 <= n_out) {
+      if constexpr (sizeof(TO) == 2) {
+        __nv_bfloat162 p[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = __floats2bfloat162_rn(out[2 * j], out[2 * j + 1]);
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(p);
+      } else {
+        reinterpret_cast<float4*>(dst)[0] = make_float4(out[0], out[1], out[2], out[3]);
+        reinterpret_cast<float4*>(dst)[1] = make_float4(out[4], out[5], out[6], out[7]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (first_out + f + j < n_out) dst[j] = from_f32<TO>(out[j]);
+    }
+  }
+}
 
 template <int NT, typename TX, typename TO>
 __global__ void __launch_bounds__(BsShape<NT, std::is_same_v<TX, uint8_t>>::kThreads, 1)
@@ -63,6 +148,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
                             TO* __restrict__ y, int64_t ldy) {
   constexpr bool kCodes = std::is_same_v<TX, uint8_t>;
   using S = BsShape<NT, kCodes>;
+  const int splits = (int)cluster_size(), rank = (int)cluster_rank();
   extern __shared__ unsigned char smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* smem_gen = smem_raw + (base - smem_u32(smem_raw));
@@ -71,21 +157,27 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
   auto empty_bar = [&](int s) { return bars + 8u * (kBsMaxStages + s); };
   auto acc_full_bar = [&](int b) { return bars + 8u * (2 * kBsMaxStages + b); };
   auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * kBsMaxStages + S::kBufs + b); };
-  const uint32_t red_bar = bars + 8u * (2 * kBsMaxStages + 2 * S::kBufs), tmem_slot = red_bar + 8;
-  static_assert(8 * (2 * kBsMaxStages + 2 * S::kBufs) + 16 <= 384, "the barriers' share of shared memory");
+  auto scale_full_bar = [&](int i) { return bars + 8u * (2 * kBsMaxStages + 2 * S::kBufs + i); };
+  auto scale_empty_bar = [&](int i) { return bars + 8u * (2 * kBsMaxStages + 2 * S::kBufs + kBsSlots + i); };
+  const uint32_t red_bar = bars + 8u * (2 * kBsMaxStages + 2 * S::kBufs + 2 * kBsSlots), tmem_slot = red_bar + 8;
+  static_assert(8 * (2 * kBsMaxStages + 2 * S::kBufs + 2 * kBsSlots) + 16 <= kBsBarBytes, "the barriers' share of shared memory");
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem_gen + (tmem_slot - base));
-  float* step_scales = reinterpret_cast<float*>(smem_gen + (bars - base) + 384);          // [stages][kScales]
-  float* red = step_scales + a.stages * S::kScales;                                                // [128][kRedStride] in all
-  int* tiles_before = reinterpret_cast<int*>(red + 128 * S::kRedStride);                  // [experts + 1] where rows are sorted
+  float* step_scales = reinterpret_cast<float*>(smem_gen + (bars - base) + kBsBarBytes);  // [kBsSlots][kScales]
+  float* red = step_scales + kBsSlots * S::kScales;                                       // [splits][NT][128 / splits + 4] sums
+  int* tiles_before = reinterpret_cast<int*>(red + bs_red_floats<NT>(splits));            // [experts + 1] where rows are sorted, and
+  int* first_row = tiles_before + a.experts + 1;                                          // [experts + 1] their offsets
 
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int splits = (int)cluster_size(), rank = (int)cluster_rank();
   const int cluster_id = blockIdx.x / splits, clusters = gridDim.x / splits;
   const int kb0 = (int)((int64_t)a.runs * rank / splits), kb1 = (int)((int64_t)a.runs * (rank + 1) / splits);
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.stages; ++s) {
-      mbar_init(full_bar(s), 2);                  // the producer and one helper
-      mbar_init(empty_bar(s), S::kStorers);       // (a sum that has been taken out is one whose MMAs have read their stage)
+      mbar_init(full_bar(s), kCodes ? 1 : 2);     // the producer, and the helper that makes codes
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int i = 0; i < kBsSlots; ++i) {
+      mbar_init(scale_full_bar(i), 1);
+      mbar_init(scale_empty_bar(i), S::kStorers);
     }
     for (int b = 0; b < S::kBufs; ++b) {
       mbar_init(acc_full_bar(b), 1);
@@ -103,8 +195,9 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     if (warp == 0) {      // the experts' row tiles, summed
       int before = 0;
       for (int e0 = 0; e0 < a.experts; e0 += 32) {
-        const int e = e0 + lane;
-        int sum = e < a.experts ? (a.offsets[e + 1] - a.offsets[e] + NT - 1) / NT : 0;
+        const int e = e0 + lane, begin = e < a.experts ? a.offsets[e] : 0, end = e < a.experts ? a.offsets[e + 1] : 0;
+        int sum = (end - begin + NT - 1) / NT;
+        if (e < a.experts) first_row[e + 1] = end;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int up = __shfl_up_sync(0xffffffffu, sum, o);
@@ -113,7 +206,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
         if (e < a.experts) tiles_before[e + 1] = before + sum;
         before += __shfl_sync(0xffffffffu, sum, 31);
       }
-      if (lane == 0) tiles_before[0] = 0;
+      if (lane == 0) tiles_before[0] = 0, first_row[0] = a.offsets[0];
     }
   }
   pdl_trigger();
@@ -137,8 +230,8 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
         const int mid = (lo + hi) >> 1;
         if (tiles_before[mid] <= row_tile) lo = mid; else hi = mid;
       }
-      begin = a.offsets[lo];
-      n = a.offsets[lo + 1] - begin;
+      begin = first_row[lo];
+      n = first_row[lo + 1] - begin;
       tiles = tiles_before[lo + 1] - tiles_before[lo];
       j = row_tile - tiles_before[lo];
       m.expert = lo;
@@ -222,7 +315,10 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
         const uint32_t w_src = umma_low_k128(base + s * S::kStage), x_src = w_src + (kBsWBytes >> 4);
 #pragma unroll
         for (int k = 0; k < 4; ++k) umma_f8_warp(leader, tmem_base + b * NT, w_src + 2 * k, x_src + 2 * k, idesc, k != 0);
-        if (leader) umma_commit(acc_full_bar(b));
+        if (leader) {
+          umma_commit(acc_full_bar(b));
+          umma_commit(empty_bar(s));
+        }
         __syncwarp();
         if (++s == a.stages) { s = 0; phase ^= 1; }
         if (++b == S::kBufs) { b = 0; acc_phase ^= 1; }
@@ -230,77 +326,81 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     }
   } else if (warp < 2 + S::kStorers) {
     const int quarter = warp & 3, c0 = ((warp - 2) >> 2) * S::kCols;
-    const int et = threadIdx.x - 64;
-    int s = 0, b = 0;
-    uint32_t phase = 0, acc_phase = 0;
+    const int et = threadIdx.x - 64, lane8 = lane >> 2, pair = (lane & 3) * 2;
+    int slot = 0, b = 0;
+    uint32_t slot_phase = 0, acc_phase = 0;
     bool ok = true;
     if (!a.offsets) pdl_wait();                   // (y may be memory that the kernel before still reads)
     for (int t = cluster_id; t < num_tiles; t += clusters) {
       const BsTile m = tile_of(t);
-      f32x2 sum[S::kCols / 2];
+      // sums of features quarter * 32 + 16 h + lane8 + 8 i, columns c0 + 8 j + pair and the next: [h][2 j + i]
+      f32x2 sum[2][S::kCols / 4];
 #pragma unroll
-      for (int c = 0; c < S::kCols / 2; ++c) sum[c] = f2_pack(0.f, 0.f);
+      for (int c = 0; c < S::kCols / 4; ++c) sum[0][c] = sum[1][c] = f2_pack(0.f, 0.f);
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (ok && !(mbar_wait_warp(acc_full_bar(b), acc_phase) && mbar_wait_warp(full_bar(s), phase))) {
+        if (ok && !(mbar_wait_warp(scale_full_bar(slot), slot_phase) && mbar_wait_warp(acc_full_bar(b), acc_phase))) {
           if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00C3);
           ok = false;
         }
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + b * NT + c0;
-        const float* scales = step_scales + s * S::kScales + (lane & 1) * (NT + 4) + c0;
-        constexpr int kPart = S::kCols < 32 ? S::kCols : 32;
-        uint32_t v[S::kCols / kPart][kPart];
+        const float* scales = step_scales + slot * S::kScales + (lane8 & 1) * (NT + 8) + c0 + pair;
+        uint32_t v[2][S::kCols / 2];
+        tmem_ld_16x256b<S::kCols>(acc, v[0]);
+        f32x2 scale[S::kCols / 8];
 #pragma unroll
-        for (int p = 0; p < S::kCols / kPart; ++p)
-          if (c0 + p * kPart < m.rows) {
-            if constexpr (kPart == 16) tmem_ld16(acc, v[p]);
-            else tmem_ld32(acc + p * kPart, v[p]);
-          }
+        for (int j = 0; j < S::kCols / 8; ++j) scale[j] = *reinterpret_cast<const f32x2*>(scales + 8 * j);
         asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+        tmem_ld_16x256b<S::kCols>(acc + (16u << 16), v[1]);
 #pragma unroll
-        for (int p = 0; p < S::kCols / kPart; ++p)
-          if (c0 + p * kPart < m.rows) {
-#pragma unroll
-            for (int q = 0; q < kPart; q += 4) {
-              const ulonglong2 scale = *reinterpret_cast<const ulonglong2*>(scales + p * kPart + q);
-              f32x2& lo = sum[(p * kPart + q) / 2];
-              f32x2& hi = sum[(p * kPart + q) / 2 + 1];
-              lo = f2_fma(f2_pack(__uint_as_float(v[p][q]), __uint_as_float(v[p][q + 1])), scale.x, lo);
-              hi = f2_fma(f2_pack(__uint_as_float(v[p][q + 2]), __uint_as_float(v[p][q + 3])), scale.y, hi);
+        for (int h = 0; h < 2; ++h) {
+          if (h) {
+            asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(acc_empty_bar(b));
+              mbar_arrive(scale_empty_bar(slot));
             }
           }
-        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(acc_empty_bar(b));
-          mbar_arrive(empty_bar(s));
+#pragma unroll
+          for (int j = 0; j < S::kCols / 8; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              sum[h][2 * j + i] = f2_fma(f2_pack(__uint_as_float(v[h][4 * j + 2 * i]), __uint_as_float(v[h][4 * j + 2 * i + 1])), scale[j], sum[h][2 * j + i]);
         }
-        if (++s == a.stages) { s = 0; phase ^= 1; }
+        if (++slot == kBsSlots) { slot = 0; slot_phase ^= 1; }
         if (++b == S::kBufs) { b = 0; acc_phase ^= 1; }
       }
-      // The sums cross shared memory, where a rolled loop finishes them (unrolled, the activations' code would be fetched anew for every tile),
-      // consecutive threads consecutive features.  Block r of a cluster finishes features r * per .. of the tile.
-      const int per = 128 / splits, feature = quarter * 32 + lane;
+      // The sums cross shared memory, column by column, where a rolled loop finishes them, eight outputs of a column a thread (unrolled over a
+      // thread's own sums, the activations' code would be fetched anew for every tile).  Block r of a cluster finishes features r * per .. of the tile.
+      const int log_splits = 31 - __clz(splits), per = 128 >> log_splits, stride = per + 4;
       asm volatile("bar.sync 1, %0;\n" ::"r"(32 * S::kStorers) : "memory");       // (the last tile's sums have been read)
       if (splits == 1) {
-        float4* dst = reinterpret_cast<float4*>(red + feature * S::kRedStride + c0);
+        float* dst = red + (c0 + pair) * 132 + quarter * 32 + lane8;
 #pragma unroll
-        for (int q = 0; q < S::kCols / 4; ++q) {
-          float4 v;
-          f2_unpack(sum[2 * q], v.x, v.y);
-          f2_unpack(sum[2 * q + 1], v.z, v.w);
-          dst[q] = v;
-        }
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int q = 0; q < S::kCols / 4; ++q) {
+            float* at = dst + (q >> 1) * 8 * 132 + 16 * h + 8 * (q & 1);
+            f2_unpack(sum[h][q], at[0], at[132]);
+          }
         asm volatile("bar.sync 1, %0;\n" ::"r"(32 * S::kStorers) : "memory");
       } else {
-        const uint32_t dst = map_to_cta(smem_u32(red + (rank * per + feature % per) * S::kRedStride + c0), feature / per);
 #pragma unroll
-        for (int q = 0; q < S::kCols / 4; ++q) {
-          float4 v;
-          f2_unpack(sum[2 * q], v.x, v.y);
-          f2_unpack(sum[2 * q + 1], v.z, v.w);
-          st_cluster_f32x4(dst + 16 * q, v.x, v.y, v.z, v.w);
-        }
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int feature = quarter * 32 + 16 * h + 8 * i + lane8;
+            const uint32_t dst = map_to_cta(smem_u32(red + (rank * NT + c0 + pair) * stride + (feature & (per - 1))), feature >> (7 - log_splits));
+#pragma unroll
+            for (int j = 0; j < S::kCols / 8; ++j) {
+              float lo, hi;
+              f2_unpack(sum[h][2 * j + i], lo, hi);
+              st_cluster_f32(dst + 8 * j * stride * 4, lo);
+              st_cluster_f32(dst + (8 * j + 1) * stride * 4, hi);
+            }
+          }
         __syncwarp();
         if (lane < splits) mbar_arrive_remote(map_to_cta(red_bar, lane));
         if (!mbar_wait_cluster(red_bar, 0)) {
@@ -309,36 +409,19 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
         }
       }
       if (!ok) continue;
-      const bool gated = moe_act_gated(a.ep.act);
-      const int wide = gated ? per / 2 : per, first_out = (m.feature + rank * per) >> (gated ? 1 : 0);
-      const int n_out = gated ? a.N >> 1 : a.N;
-      auto summed = [&](int f, int c) {           // the four columns from c of this block's feature f
-        float4 v = *reinterpret_cast<const float4*>(red + f * S::kRedStride + c);
-        for (int r = 1; r < splits; ++r) {
-          const float4 o = *reinterpret_cast<const float4*>(red + (r * per + f) * S::kRedStride + c);
-          v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-        }
-        return v;
-      };
-      for (int i = et; i < wide * ((m.rows + 3) >> 2); i += 32 * S::kStorers) {
-        const int c = i / wide * 4, f = i % wide;
-        if (first_out + f >= n_out) continue;
-        const float4 u = summed(gated ? 2 * f : f, c), v = gated ? summed(2 * f + 1, c) : u;
-        const float first_sum[4] = {u.x, u.y, u.z, u.w}, second_sum[4] = {v.x, v.y, v.z, v.w};
-        TO* dst = y + (size_t)(m.first + c) * ldy + first_out + f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (c + j >= m.rows) break;
-          const float scale = a.ep.row_scale ? a.ep.row_scale[a.order[m.first + c + j]] : 1.f;
-          const float g = first_sum[j] * scale;
-          dst[(size_t)j * ldy] = from_f32<TO>(gated ? moe_gated(g, second_sum[j] * scale, a.ep.act, a.ep.limit, a.ep.alpha) : moe_act(g, a.ep.act));
-        }
+      switch (a.ep.act) {
+        case MOE_ACT_NONE: bs_finish<MOE_ACT_NONE, NT>(red, log_splits, rank, m, a, y, ldy, et, 32 * S::kStorers); break;
+        case MOE_ACT_RELU2: bs_finish<MOE_ACT_RELU2, NT>(red, log_splits, rank, m, a, y, ldy, et, 32 * S::kStorers); break;
+        case MOE_ACT_SILU: bs_finish<MOE_ACT_SILU, NT>(red, log_splits, rank, m, a, y, ldy, et, 32 * S::kStorers); break;
+        case MOE_ACT_GELU: bs_finish<MOE_ACT_GELU, NT>(red, log_splits, rank, m, a, y, ldy, et, 32 * S::kStorers); break;
+        case MOE_ACT_GLU_CLAMP: bs_finish<MOE_ACT_GLU_CLAMP, NT>(red, log_splits, rank, m, a, y, ldy, et, 32 * S::kStorers); break;
+        default: bs_finish<MOE_ACT_SWIGLU, NT>(red, log_splits, rank, m, a, y, ldy, et, 32 * S::kStorers); break;
       }
     }
   } else {
     const int helper = warp - 2 - S::kStorers;
-    int it = 0, s = 0;
-    uint32_t phase = 1;
+    int it = 0, s = 0, slot = 0;
+    uint32_t phase = 1, slot_phase = 1;
     bool ok = true;
     if (!a.offsets) pdl_wait();
     for (int t = cluster_id; t < num_tiles && ok; t += clusters) {
@@ -346,17 +429,17 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
       const float* ws = a.w_scales + ((size_t)m.expert * a.scale_rows + bs_scale_row(m.feature, a.pairs)) * a.runs;
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
         if (it % S::kHelpers == helper) {
-          float* scales = step_scales + s * S::kScales;
+          float* scales = step_scales + slot * S::kScales;
           const float even = ws[kb], odd = a.pairs ? ws[a.runs + kb] : even;
           if constexpr (kCodes) {
             float v[NT / 32];
 #pragma unroll
             for (int i = 0; i < NT / 32; ++i) v[i] = a.x_scales[(size_t)kb * a.lds + m.first + min(lane + 32 * i, m.rows - 1)];
-            if (!mbar_wait_warp(empty_bar(s), phase)) ok = false;
+            if (!mbar_wait_warp(scale_empty_bar(slot), slot_phase)) ok = false;
 #pragma unroll
             for (int i = 0; i < NT / 32; ++i) {
               scales[lane + 32 * i] = v[i] * even;
-              scales[NT + 4 + lane + 32 * i] = v[i] * odd;
+              scales[NT + 8 + lane + 32 * i] = v[i] * odd;
             }
           } else {
             // eight lanes a row, sixteen columns each; two rows a lane at a time
@@ -376,7 +459,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
                 else bs_load16<TX, false>(p, n, v[h]);
               }
               if (!free) {
-                if (!mbar_wait_warp(empty_bar(s), phase)) ok = false;
+                if (!(mbar_wait_warp(empty_bar(s), phase) && mbar_wait_warp(scale_empty_bar(slot), slot_phase))) ok = false;
                 free = true;
               }
 #pragma unroll
@@ -397,7 +480,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
                   *reinterpret_cast<uint4*>(codes + r * kBlk + ((eighth ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                   if (eighth == 0) {
                     scales[r] = scale * even;
-                    scales[NT + 4 + r] = scale * odd;
+                    scales[NT + 8 + r] = scale * odd;
                   }
                 }
               }
@@ -409,9 +492,13 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
             break;
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(full_bar(s));
+          if (lane == 0) {
+            mbar_arrive(scale_full_bar(slot));
+            if constexpr (!kCodes) mbar_arrive(full_bar(s));
+          }
         }
         if (++s == a.stages) { s = 0; phase ^= 1; }
+        if (++slot == kBsSlots) { slot = 0; slot_phase ^= 1; }
       }
     }
   }
@@ -426,9 +513,9 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
 }
 
 template <int NT>
-static constexpr uint32_t bs_smem(int stages, int experts) {
+static constexpr uint32_t bs_smem(int stages, int splits, int experts) {
   using S = BsShape<NT, true>;
-  return 1024u + stages * (S::kStage + S::kScales * 4) + 384u + 128 * S::kRedStride * 4 + 4 * (experts + 1);
+  return 1024u + stages * S::kStage + kBsBarBytes + 4 * (kBsSlots * S::kScales + bs_red_floats<NT>(splits) + 2 * (experts + 1));
 }
 
 template <int NT, typename TX, typename TO>
@@ -440,7 +527,7 @@ static int launch_block_scaled(const CUtensorMap& map_w, const CUtensorMap& map_
   const int grid = (int)(splits > 1 ? tiles * splits : tiles < 148 ? tiles : 148);      // (a cluster has one tile: its sums' place is used once)
   const int64_t steps = (int64_t)ceil_div(a.runs, splits) * ceil_div64(tiles * splits, grid);      // of a block, at most
   a.stages = 1;
-  while (a.stages < kBsMaxStages && a.stages < steps && bs_smem<NT>(a.stages + 1, experts) <= (uint32_t)kMostSmem) ++a.stages;
+  while (a.stages < kBsMaxStages && a.stages < steps && bs_smem<NT>(a.stages + 1, splits, experts) <= (uint32_t)kMostSmem) ++a.stages;
   auto kern = block_scaled_tcgen05_kernel<NT, TX, TO>;
   static bool allowed[64];      // (by device: the attribute belongs to its context)
   int device = 0;
@@ -450,7 +537,7 @@ static int launch_block_scaled(const CUtensorMap& map_w, const CUtensorMap& map_
   if (device < 64) allowed[device] = true;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(BsShape<NT, std::is_same_v<TX, uint8_t>>::kThreads);
-  cfg.dynamicSmemBytes = bs_smem<NT>(a.stages, experts);
+  cfg.dynamicSmemBytes = bs_smem<NT>(a.stages, splits, experts);
   cfg.stream = stream;
   cfg.gridDim = dim3((unsigned)grid);
   cudaLaunchAttribute attr[2];
@@ -498,6 +585,7 @@ TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, in
   BsArgs a;
   a.x = x; a.ldx = ldx; a.x_scales = x_scales; a.lds = lds; a.w_scales = w_scales; a.scale_rows = scale_rows; a.pairs = pairs;
   a.vec = !is_codes && ((uintptr_t)x & 15) == 0 && (ldx * (x_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
+  a.wide = ((uintptr_t)y & 15) == 0 && (ldy * (y_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
   a.M = M; a.N = N; a.K = K; a.runs = ceil_div(K, kBlk); a.offsets = offsets; a.order = order; a.experts = experts; a.top = top;
   a.x_by_pair = x_by_pair; a.error_word = error_word;
   a.ep.act = act; a.ep.limit = limit; a.ep.alpha = alpha; a.ep.row_scale = row_scale;
