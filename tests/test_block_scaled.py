@@ -36,17 +36,25 @@ def test_weights_that_do_not_fit_are_refused(make):
         make(random_matrix(130, 200, 0), random_matrix(64, 200, 1), random_matrix(130, 100, 2))
 
 
+def flat(x, n):
+    """The rows of codes in blocks [blocks, runs, 128, 128]."""
+    return x.view(torch.uint8).transpose(1, 2).reshape(x.shape[0] * 128, -1)[:n]
+
+
 def test_a_weight_keeps_its_matrices_in_whole_blocks():
     a, b, c = random_matrix(256, 200, 0), random_matrix(130, 200, 1), random_matrix(64, 200, 2)
     w = BlockScaledWeight(a, b, c)
     assert (w.out_features, w.in_features, w.dtype) == (450, 200, CODES)
-    assert [(first, tuple(x.shape), tuple(s.shape)) for first, x, s in w.parts] == [(0, (1, 386, 256), (1, 4, 2)), (386, (1, 64, 256), (1, 1, 2))]
-    _, x, s = w.parts[0]
-    assert torch.equal(x[0, :256, :200].view(torch.uint8), a.codes.view(torch.uint8)) and torch.equal(s[0, 2:], b.scales)
-    assert not x[..., 200:].view(torch.uint8).any()
-    assert w.nbytes() == 450 * 256 + 4 * (8 + 2)
+    assert [(first, n, tuple(x.shape), tuple(s.shape)) for first, n, x, s in w.parts] == \
+        [(0, 386, (1, 4, 2, 128, 128), (1, 4, 2)), (386, 64, (1, 1, 2, 128, 128), (1, 1, 2))]
+    _, _, x, s = w.parts[0]
+    assert torch.equal(flat(x[0], 256)[:, :200], a.codes.view(torch.uint8)) and torch.equal(s[0, 2:], b.scales)
+    assert torch.equal(flat(x[0], 386)[256:, :200], b.codes.view(torch.uint8))
+    assert not flat(x[0], 512)[:, 200:].any() and not flat(x[0], 512)[386:].any()
+    assert w.nbytes() == 5 * 2 * 128 * 128 + 4 * (8 + 2)
     view = w.rows(128, 400)
-    assert view.out_features == 272 and [(first, x.shape[1], s.shape[1]) for first, x, s in view.parts] == [(0, 258, 3), (258, 14, 1)]
+    assert view.out_features == 272 and [(first, n, x.shape[1], s.shape[1]) for first, n, x, s in view.parts] == [(0, 258, 3, 3), (258, 14, 1, 1)]
+    assert torch.equal(view.parts[0][2].view(torch.uint8), w.parts[0][2][:, 1:].view(torch.uint8))
     for start, stop in ((64, 130), (0, 451), (5, 5), (-1, 4)):
         with pytest.raises(ValueError):
             w.rows(start, stop)
@@ -54,12 +62,13 @@ def test_a_weight_keeps_its_matrices_in_whole_blocks():
 
 def test_gate_and_up_alternate():
     g, u = random_matrix(130, 300, 0), random_matrix(130, 300, 1)
-    _, x, s = BlockScaledWeight(g, u, epilogue="swiglu").parts[0]
-    x = x.view(torch.uint8)
-    assert torch.equal(x[0, 0::2, :300], g.codes.view(torch.uint8)) and torch.equal(x[0, 1::2, :300], u.codes.view(torch.uint8))
+    _, n, x, s = BlockScaledWeight(g, u, epilogue="swiglu").parts[0]
+    x = flat(x[0], 260)
+    assert n == 260
+    assert torch.equal(x[0::2, :300], g.codes.view(torch.uint8)) and torch.equal(x[1::2, :300], u.codes.view(torch.uint8))
     assert torch.equal(s[0, 0::2], g.scales) and torch.equal(s[0, 1::2], u.scales)
     e = BlockScaledExperts([g, u], [u, g])
-    assert e.out_features == 260 and torch.equal(e.codes.view(torch.uint8)[1, 0::2, :300], u.codes.view(torch.uint8))
+    assert e.out_features == 260 and torch.equal(flat(e.codes[1], 260)[0::2, :300], u.codes.view(torch.uint8))
 
 
 def test_products_need_a_gpu():

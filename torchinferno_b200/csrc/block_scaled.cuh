@@ -1,8 +1,8 @@
 // What the products of 8-bit block-scaled operands share.
 //
 // Codes are e4m3 (a sign, four bits of exponent with bias 7, three of mantissa; largest 448, one NaN, no infinity).  A matrix
-// [N, K] has one fp32 scale for each block of 128 x 128; its rows are padded with zero codes to whole runs of 128 columns when it is laid
-// out (so every row starts on a 128-byte boundary), its scales are [blocks of rows, blocks of columns].  In a matrix of (gate, up) row
+// [N, K] has one fp32 scale for each block of 128 x 128.  It is laid out block by block, [blocks of rows, blocks of columns, 128, 128], padded with
+// zero codes to whole blocks, so that a step's 16 KB lie side by side in memory; its scales are [blocks of rows, blocks of columns].  In a matrix of (gate, up) row
 // pairs (row 2i = gate i, 2i + 1 = up i) the scales' rows alternate likewise: row 2j of them is the gate's block j, 2j + 1 the up's.
 // Rows x [M, K] have one power of two for each run of 128 columns; their scales lie [runs, M rounded up to 4].
 #pragma once

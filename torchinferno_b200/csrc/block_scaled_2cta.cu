@@ -208,7 +208,7 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
       uint32_t phase = 1;
       bool ok = true;
       for (int t = pair; t < num_tiles && ok; t += pairs) {
-        const int n_tile = t / m_tiles, m0 = (t - n_tile * m_tiles) * 256 + (int)rank * 128, n0 = n_tile * 256 + (int)rank * 128;
+        const int n_tile = t / m_tiles, m0 = (t - n_tile * m_tiles) * 256 + (int)rank * 128, w0 = (n_tile * 2 + (int)rank) * a.runs;
         for (int kb = 0; kb < a.runs; ++kb) {
           if (!mbar_wait_warp(empty_bar(s), phase)) {
             if (a.error_word && leader) atomicExch(a.error_word, 0x7C00D1);
@@ -219,7 +219,7 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
             if (rank == 0) mbar_expect_tx(full_bar(s), 2 * kB2Stage);
             const uint32_t bar0 = map_to_cta(full_bar(s), 0);
             b2_tma_load(base + s * kB2Stage, &map_x, kb * kBlk, m0, bar0);
-            b2_tma_load(base + s * kB2Stage + kB2Half, &map_w, kb * kBlk, n0, bar0);
+            b2_tma_load(base + s * kB2Stage + kB2Half, &map_w, 0, (w0 + kb) << 7, bar0);
           }
           __syncwarp();
           if (++s == kB2Stages) { s = 0; phase ^= 1; }
@@ -288,13 +288,15 @@ static int launch_b2(const CUtensorMap& map_x, const CUtensorMap& map_w, const B
 
 using namespace tib;
 
-// x: codes [M, runs * 128] and scales [runs, lds] as tib_quantize_rows leaves them; w: codes [N, runs * 128] and scales [scale_rows, runs] (`pairs`:
+// x: codes [M, runs * 128] and scales [runs, lds] as tib_quantize_rows leaves them; w: codes in blocks [ceil(N / 128), runs, 128, 128] and
+// scales [scale_rows, runs] (`pairs`:
 // of (gate, up) row pairs, N and scale_rows even); out: [M, N] in out_dtype (row stride ldo), or [M, N / 2] with `swiglu`.
 TIB_API int tib_block_scaled_2cta(const void* x, const float* x_scales, int64_t lds, const void* w, const float* w_scales, int scale_rows, int pairs,
                                   int swiglu, void* out, int out_dtype, int64_t ldo, int M, int N, int K, int* error_word, cudaStream_t stream) {
   if (M == 0 || N == 0) return TIB_OK;
   if (!x || !x_scales || !w || !w_scales || !out || M < 0 || N < 0 || K < 1 || scale_rows < 1) return TIB_E_ARG;
   if ((swiglu && !pairs) || (pairs && (N % 2 || scale_rows % 2)) || lds < M) return TIB_E_SIZE;
+  if ((int64_t)(ceil_div(N, 128) + 2) * ceil_div(K, kBlk) > (0x7fffffff >> 7)) return TIB_E_SIZE;
   if (out_dtype != TIB_BF16 && out_dtype != TIB_F32) return TIB_E_DTYPE;
   if (((uintptr_t)x | (uintptr_t)w) & 15) return TIB_E_ALIGN;
   B2Args a;
@@ -303,7 +305,7 @@ TIB_API int tib_block_scaled_2cta(const void* x, const float* x_scales, int64_t 
   CUtensorMap map_x, map_w;
   int rc = bs_make_map(&map_x, x, M, (int64_t)a.runs * kBlk, 128);
   if (rc != TIB_OK) return rc;
-  rc = bs_make_map(&map_w, w, N, (int64_t)a.runs * kBlk, 128);
+  rc = bs_make_map(&map_w, w, (int64_t)ceil_div(N, 128) * a.runs * 128, kBlk, 128);
   if (rc != TIB_OK) return rc;
   if (swiglu)
     return out_dtype == TIB_BF16 ? launch_b2<true, __nv_bfloat16>(map_x, map_w, a, out, ldo, stream) : launch_b2<true, float>(map_x, map_w, a, out, ldo, stream);

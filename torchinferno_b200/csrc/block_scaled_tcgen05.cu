@@ -6,7 +6,8 @@
 // row of the swizzle, four MMAs into an accumulator of its own in tensor memory, which the summing warps take out and add to 32-bit sums in
 // registers, times the scale of (row, run) and (block of features, run), whose product is made once a row and step (packed fp32, one multiply-add for
 // two sums).  kBufs accumulators rotate, so the tensor cores run ahead of the sums.
-//   warp 0             TMA producer: 16 KB of codes of w a step, and the rows' codes where they exist, in boxes of 32 rows
+//   warp 0             TMA producer: 16 KB of codes of w a step, one block of the matrix, which lies in memory as such (rows of 128 bytes a
+//                      matrix row apart came from memory at half the rate), and the rows' codes where they exist, in boxes of 32 rows
 //   warp 1             issues tcgen05.mma; owns the TMEM allocation
 //   the next 4 or 8    sums and epilogue (eight for 128 rows: four for each half of the columns)
 //   the last 2 or 4    helpers, taking turns: the products of scales into a ring of their own; from rows that are no codes yet they (then four) make
@@ -29,6 +30,7 @@ constexpr uint32_t kBsWBytes = 128 * kBlk;
 
 template <int NT, bool CODES> struct BsShape {
   static constexpr int kStorers = NT >= 128 ? 8 : 4, kHelpers = CODES ? 2 : 4, kThreads = 64 + 32 * (kStorers + kHelpers);
+  static constexpr int kPerSm = NT <= 32 ? 2 : 1;                   // blocks of an SM
   static constexpr int kBufs = 4, kCols = NT / (kStorers / 4);      // accumulators; columns of a summing thread
   static constexpr uint32_t kTmemCols = kBufs * NT < 32 ? 32 : kBufs * NT;
   static constexpr uint32_t kStage = kBsWBytes + NT * kBlk;
@@ -45,7 +47,7 @@ struct BsArgs {
   int64_t ldx;                 // (of the latter)
   const float* x_scales;       // [runs, lds] beside codes
   int64_t lds;
-  const float* w_scales;
+  const float* w_scales;       // [experts, scale_rows, runs]
   int scale_rows, pairs, vec, wide;      // vec: rows of x, wide: of y, are 16-byte aligned
   int M, N, K, runs, stages;
   const int* offsets;          // null: one matrix
@@ -143,7 +145,7 @@ __device__ __forceinline__ void bs_finish(const float* red, int log_splits, int 
 }
 
 template <int NT, typename TX, typename TO>
-__global__ void __launch_bounds__(BsShape<NT, std::is_same_v<TX, uint8_t>>::kThreads, 1)
+__global__ void __launch_bounds__(BsShape<NT, std::is_same_v<TX, uint8_t>>::kThreads, BsShape<NT, std::is_same_v<TX, uint8_t>>::kPerSm)
 block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const BsArgs a,
                             TO* __restrict__ y, int64_t ldy) {
   constexpr bool kCodes = std::is_same_v<TX, uint8_t>;
@@ -170,20 +172,20 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int cluster_id = blockIdx.x / splits, clusters = gridDim.x / splits;
   const int kb0 = (int)((int64_t)a.runs * rank / splits), kb1 = (int)((int64_t)a.runs * (rank + 1) / splits);
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < a.stages; ++s) {
-      mbar_init(full_bar(s), kCodes ? 1 : 2);     // the producer, and the helper that makes codes
-      mbar_init(empty_bar(s), 1);
+  if (warp == 0) {
+    if (lane < a.stages) {
+      mbar_init(full_bar(lane), kCodes ? 1 : 2);  // the producer, and the helper that makes codes
+      mbar_init(empty_bar(lane), 1);
     }
-    for (int i = 0; i < kBsSlots; ++i) {
-      mbar_init(scale_full_bar(i), 1);
-      mbar_init(scale_empty_bar(i), S::kStorers);
+    if (lane < kBsSlots) {
+      mbar_init(scale_full_bar(lane), 1);
+      mbar_init(scale_empty_bar(lane), S::kStorers);
     }
-    for (int b = 0; b < S::kBufs; ++b) {
-      mbar_init(acc_full_bar(b), 1);
-      mbar_init(acc_empty_bar(b), S::kStorers);
+    if (lane < S::kBufs) {
+      mbar_init(acc_full_bar(lane), 1);
+      mbar_init(acc_empty_bar(lane), S::kStorers);
     }
-    mbar_init(red_bar, S::kStorers * splits);
+    if (lane == 0) mbar_init(red_bar, S::kStorers * splits);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 1) {
@@ -242,6 +244,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     m.feature = (t - row_tile * f_tiles) << 7;
     return m;
   };
+  auto w_row = [&](const BsTile& m, int kb) { return ((m.expert * f_tiles + (m.feature >> 7)) * a.runs + kb) << 7; };      // of the tile's block in the matrix of blocks
   auto source = [&](const BsTile& m, int r) {     // the row of x that the tile's row r is
     const int at = m.first + min(r, m.rows - 1);
     return a.offsets && a.x_by_pair ? a.order[at] / a.top : at;
@@ -259,7 +262,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
           for (int kb = kb0; kb < kb1 && ahead < a.stages; ++kb, ++ahead)
           if (leader) {
             mbar_expect_tx(full_bar(ahead), bytes(m));
-            tma_load_2d(base + ahead * S::kStage, &map_w, kb * kBlk, m.expert * a.N + m.feature, full_bar(ahead));
+            tma_load_2d(base + ahead * S::kStage, &map_w, 0, w_row(m, kb), full_bar(ahead));
           }
       }
       pdl_wait();
@@ -276,14 +279,14 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
           }
           if (leader) {
             mbar_expect_tx(full_bar(s), bytes(m));
-            tma_load_2d(stage, &map_w, kb * kBlk, m.expert * a.N + m.feature, full_bar(s));      // (a tile may reach into the next expert's features, or past the last: such lanes are never stored)
+            tma_load_2d(stage, &map_w, 0, w_row(m, kb), full_bar(s));
           }
           __syncwarp();
         }
         if constexpr (kCodes) {
           if (leader) {
 #pragma unroll
-            for (int i = 0; i < NT / 32; ++i)     // (likewise a last box into the next tile's rows, or past the last)
+            for (int i = 0; i < NT / 32; ++i)     // (the last box may reach into the next tile's rows, or past the last: such columns are never stored)
               if (32 * i < m.rows) tma_load_2d(stage + kBsWBytes + i * 32 * kBlk, &map_x, kb * kBlk, m.first + 32 * i, full_bar(s));
           }
           __syncwarp();
@@ -524,10 +527,11 @@ static int launch_block_scaled(const CUtensorMap& map_w, const CUtensorMap& map_
   const int64_t row_tiles = a.offsets ? a.M / NT + (a.M < a.experts ? a.M : a.experts) : ceil_div(a.M, NT);
   const int64_t tiles = row_tiles * ceil_div(a.N, 128);
   if (tiles * splits > 0x7fffffff) return TIB_E_SIZE;
-  const int grid = (int)(splits > 1 ? tiles * splits : tiles < 148 ? tiles : 148);      // (a cluster has one tile: its sums' place is used once)
+  constexpr int kBlocks = 148 * BsShape<NT, std::is_same_v<TX, uint8_t>>::kPerSm;
+  const int grid = (int)(splits > 1 ? tiles * splits : tiles < kBlocks ? tiles : kBlocks);      // (a cluster has one tile: its sums' place is used once)
   const int64_t steps = (int64_t)ceil_div(a.runs, splits) * ceil_div64(tiles * splits, grid);      // of a block, at most
   a.stages = 1;
-  while (a.stages < kBsMaxStages && a.stages < steps && bs_smem<NT>(a.stages + 1, splits, experts) <= (uint32_t)kMostSmem) ++a.stages;
+  while (a.stages < kBsMaxStages && a.stages < steps && bs_smem<NT>(a.stages + 1, splits, experts) <= (kBlocks > 148 ? 113u * 1024 : (uint32_t)kMostSmem)) ++a.stages;
   auto kern = block_scaled_tcgen05_kernel<NT, TX, TO>;
   static bool allowed[64];      // (by device: the attribute belongs to its context)
   int device = 0;
@@ -567,8 +571,8 @@ static int bs_splits(int64_t tiles, int runs) {
 using namespace tib;
 
 // x_dtype TIB_BF16 or TIB_F32: rows [rows, K] (row stride ldx) that are quantised on the way, once for each tile of 128 features; -1: codes
-// [x_rows, runs * 128] and scales [runs, lds] as tib_quantize_rows leaves them, row m of them for row m of y.  w: codes [experts, N, runs * 128] and scales
-// [experts, scale_rows, runs] (`pairs`: of (gate, up) row pairs); y: [M, N] in y_dtype (row stride ldy), or [M, N / 2] of a gated activation.
+// [x_rows, runs * 128] and scales [runs, lds] as tib_quantize_rows leaves them, row m of them for row m of y.  w: codes in blocks
+// [experts, ceil(N / 128), runs, 128, 128], features and columns behind the last zero, and scales [experts, scale_rows, runs] (`pairs`: of (gate, up) row pairs); y: [M, N] in y_dtype (row stride ldy), or [M, N / 2] of a gated activation.
 // offsets [experts + 1] and order [M]: rows sorted by expert as tib_moe_expert_product takes them; offsets null: one matrix for all rows.
 TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, int x_rows, const float* x_scales, int64_t lds, const void* w,
                                      const float* w_scales, int scale_rows, int pairs, void* y, int y_dtype, int64_t ldy, int M, int N, int K,
@@ -580,7 +584,7 @@ TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, in
   if ((is_codes && (!x_scales || (offsets && x_by_pair) || x_rows < M || lds < M)) || (offsets && !order) || (row_scale && !order)) return TIB_E_ARG;
   if (act < MOE_ACT_NONE || act > MOE_ACT_GELU || (moe_act_gated(act) && !pairs) || (pairs && N % 2)) return TIB_E_SIZE;
   if (x_dtype > TIB_BF16 || (y_dtype != TIB_BF16 && y_dtype != TIB_F32)) return TIB_E_DTYPE;
-  if (experts > kBsMaxExperts || (int64_t)experts * N > 0x7fffffff - 128) return TIB_E_SIZE;
+  if (experts > kBsMaxExperts || (int64_t)experts * ceil_div(N, 128) * ceil_div(K, kBlk) > (0x7fffffff >> 7)) return TIB_E_SIZE;
   if ((((uintptr_t)w) & 15) || (is_codes && (((uintptr_t)x) & 15))) return TIB_E_ALIGN;
   BsArgs a;
   a.x = x; a.ldx = ldx; a.x_scales = x_scales; a.lds = lds; a.w_scales = w_scales; a.scale_rows = scale_rows; a.pairs = pairs;
@@ -590,7 +594,7 @@ TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, in
   a.x_by_pair = x_by_pair; a.error_word = error_word;
   a.ep.act = act; a.ep.limit = limit; a.ep.alpha = alpha; a.ep.row_scale = row_scale;
   CUtensorMap map_w, map_x;
-  int rc = bs_make_map(&map_w, w, (int64_t)experts * N, (int64_t)a.runs * kBlk, 128);
+  int rc = bs_make_map(&map_w, w, (int64_t)experts * ceil_div(N, 128) * a.runs * 128, kBlk, 128);
   if (rc != TIB_OK) return rc;
   map_x = map_w;
   if (is_codes) {

@@ -96,8 +96,8 @@ def _quantized(x: torch.Tensor, routing: tuple[torch.Tensor, torch.Tensor, int] 
 
 
 def _laid_out(matrices: Sequence[BlockScaledMatrix], ups: Sequence[BlockScaledMatrix] | None) -> tuple[torch.Tensor, torch.Tensor]:
-    """Codes [matrices, N, K rounded up to 128] and scales [matrices, blocks of N, blocks of K] of equally large matrices; with ``ups``
-    the rows of either alternate (gate i, up i; gate block j, up block j)."""
+    """Codes [matrices, blocks of N, blocks of K, 128, 128], padded with zeros, and scales [matrices, blocks of N, blocks of K] of equally large
+    matrices; with ``ups`` the rows of either alternate (gate i, up i; gate block j, up block j)."""
     shape, device = matrices[0].shape, matrices[0].device
     for m in [*matrices, *(ups or ())]:
         if m.shape != shape or m.device != device:
@@ -105,14 +105,17 @@ def _laid_out(matrices: Sequence[BlockScaledMatrix], ups: Sequence[BlockScaledMa
     if ups is not None and len(ups) != len(matrices):
         raise ValueError(f"{len(matrices)} gate and {len(ups)} up matrices")
     n, k = shape
-    parts = 1 if ups is None else 2
-    codes = torch.zeros((len(matrices), n, parts, blocks(k) * BLOCK), dtype=torch.uint8, device=device)      # (columns behind K: zero codes)
-    scales = torch.empty((len(matrices), blocks(n), parts, blocks(k)), dtype=torch.float32, device=device)
-    for part, stack in enumerate((matrices,) if ups is None else (matrices, ups)):
-        for i, m in enumerate(stack):
-            codes[i, :, part, :k] = m.codes.view(torch.uint8)
-            scales[i, :, part] = m.scales
-    return codes.view(CODE_DTYPE).view(len(matrices), n * parts, -1), scales.view(len(matrices), blocks(n) * parts, -1)
+    parts, runs = 1 if ups is None else 2, blocks(k)
+    tiles = blocks(n * parts)
+    codes = torch.empty((len(matrices), tiles, runs, BLOCK, BLOCK), dtype=torch.uint8, device=device)
+    scales = torch.empty((len(matrices), blocks(n), parts, runs), dtype=torch.float32, device=device)
+    for i, m in enumerate(matrices):
+        flat = torch.zeros((tiles * BLOCK, runs * BLOCK), dtype=torch.uint8, device=device)
+        for part, stack in enumerate((matrices,) if ups is None else (matrices, ups)):
+            flat[part:n * parts:parts, :k] = stack[i].codes.view(torch.uint8)
+            scales[i, :, part] = stack[i].scales
+        codes[i] = flat.view(tiles, BLOCK, runs, BLOCK).transpose(1, 2)
+    return codes.view(CODE_DTYPE), scales.view(len(matrices), blocks(n) * parts, -1)
 
 
 class BlockScaledWeight:
@@ -131,11 +134,11 @@ class BlockScaledWeight:
             raise ValueError("the matrices of a weight need the same columns and device")
         self.epilogue, self.in_features = epilogue, matrices[0].shape[1]
         self.out_features = sum(m.shape[0] for m in matrices)
-        # (first output, codes, scales) of every product to run.  Matrices are put together while the ones before end with a whole block;
+        # (first output, outputs, codes, scales) of every product to run.  Matrices are put together while the ones before end with a whole block;
         # where one does not, its blocks' borders would not be the joint matrix's: it starts a product of its own.
-        self.parts: list[tuple[int, torch.Tensor, torch.Tensor]] = []
+        self.parts: list[tuple[int, int, torch.Tensor, torch.Tensor]] = []
         if epilogue == "swiglu":
-            self.parts.append((0, *_laid_out(matrices[:1], matrices[1:])))
+            self.parts.append((0, self.out_features, *_laid_out(matrices[:1], matrices[1:])))
             return
         first, run = 0, []
         for i, m in enumerate(matrices):
@@ -143,7 +146,7 @@ class BlockScaledWeight:
             if m.shape[0] % BLOCK or i == len(matrices) - 1:
                 joint = run[0] if len(run) == 1 else BlockScaledMatrix(
                     torch.cat([r.codes.view(torch.uint8) for r in run]).view(CODE_DTYPE), torch.cat([r.scales for r in run]))
-                self.parts.append((first, *_laid_out([joint], None)))
+                self.parts.append((first, joint.shape[0], *_laid_out([joint], None)))
                 first, run = first + joint.shape[0], []
 
     @property
@@ -152,10 +155,10 @@ class BlockScaledWeight:
 
     @property
     def device(self) -> torch.device:
-        return self.parts[0][1].device
+        return self.parts[0][2].device
 
     def nbytes(self) -> int:
-        return sum(codes.numel() + 4 * scales.numel() for _, codes, scales in self.parts)
+        return sum(codes.numel() + 4 * scales.numel() for _, _, codes, scales in self.parts)
 
     def rows(self, start: int, stop: int) -> "BlockScaledWeight":
         """The projection onto output features start .. stop-1 (views; ``start`` a whole number of blocks into its matrix)."""
@@ -163,12 +166,12 @@ class BlockScaledWeight:
             raise ValueError(f"no features {start} .. {stop - 1} of {self.out_features} to take")
         view = object.__new__(BlockScaledWeight)
         view.epilogue, view.in_features, view.out_features, view.parts = "none", self.in_features, stop - start, []
-        for first, codes, scales in self.parts:
-            lo, hi = max(start - first, 0), min(stop - first, codes.shape[1])
+        for first, count, codes, scales in self.parts:
+            lo, hi = max(start - first, 0), min(stop - first, count)
             if lo < hi:
                 if lo % BLOCK:
                     raise ValueError(f"feature {start} lies inside a block")
-                view.parts.append((first + lo - start, codes[:, lo:hi], scales[:, lo // BLOCK:blocks(hi)]))
+                view.parts.append((first + lo - start, hi - lo, codes[:, lo // BLOCK:blocks(hi)], scales[:, lo // BLOCK:blocks(hi)]))
         return view
 
     def _checked(self, x: torch.Tensor, out_dtype: torch.dtype | None, width: int, out: torch.Tensor | None) -> torch.Tensor:
@@ -195,8 +198,8 @@ class BlockScaledWeight:
         if x.shape[0] == 0:
             return out
         rows = (x, None) if x.shape[0] <= FEW_ROWS else _quantized(x)
-        for first, codes, scales in self.parts:
-            ops.block_scaled_product(*rows, codes, scales, out if len(self.parts) == 1 else out[:, first:first + codes.shape[1]],
+        for first, count, codes, scales in self.parts:
+            ops.block_scaled_product(*rows, codes, scales, out if len(self.parts) == 1 else out[:, first:first + count], features=count,
                                      columns=self.in_features, paired=self.epilogue == "swiglu", error_word=error_word)
         return out
 
@@ -207,9 +210,9 @@ class BlockScaledWeight:
         out = self._checked(x, out_dtype, self.out_features // 2, None)
         if x.shape[0] == 0:
             return out
-        _, codes, scales = self.parts[0]
+        _, count, codes, scales = self.parts[0]
         rows = (x, None) if x.shape[0] <= FEW_ROWS else _quantized(x)
-        return ops.block_scaled_product(*rows, codes, scales, out, columns=self.in_features, paired=True, act="swiglu",
+        return ops.block_scaled_product(*rows, codes, scales, out, features=count, columns=self.in_features, paired=True, act="swiglu",
                                         error_word=error_word)
 
 
@@ -259,5 +262,5 @@ class BlockScaledExperts:
             rows, routing = (x, None), (offsets, order, top, x_by_pair)
         else:                                   # (the pairs' rows, sorted on the way)
             rows, routing = _quantized(x if x_by_pair else x[:pairs], (offsets, order, top) if x_by_pair else None), (offsets, order, top, False)
-        return ops.block_scaled_product(*rows, self.codes, self.scales, y, columns=self.in_features, paired=self.paired, act=act, limit=limit,
+        return ops.block_scaled_product(*rows, self.codes, self.scales, y, features=self.out_features, columns=self.in_features, paired=self.paired, act=act, limit=limit,
                                         alpha=alpha, routing=routing, row_scale=row_scale, error_word=error_word)

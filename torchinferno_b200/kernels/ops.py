@@ -1281,20 +1281,20 @@ def block_scaled_pairs_of_sms(rows: int, features: int) -> bool:
 
 
 def block_scaled_product(x: torch.Tensor, scales: torch.Tensor | None, w: torch.Tensor, w_scales: torch.Tensor, y: torch.Tensor, *,
-                         columns: int, paired: bool = False, act: str = "none", limit: float = 0.0, alpha: float = 1.0,
+                         features: int, columns: int, paired: bool = False, act: str = "none", limit: float = 0.0, alpha: float = 1.0,
                          routing: tuple[torch.Tensor, torch.Tensor, int, bool] | None = None, row_scale: torch.Tensor | None = None,
                          error_word: torch.Tensor | None = None) -> torch.Tensor:
     """Rows times matrices of codes.  ``x``: codes with their ``scales`` as :func:`quantize_rows` leaves them, or (``scales`` None) rows that the
-    product's kernel quantises itself; ``w``: [experts, N, ``columns`` rounded up to 128], ``w_scales`` [experts, rows of scales, runs] (``paired``: of
-    (gate, up) row pairs).  ``routing`` = (offsets, order, top, x_by_pair) sorts the rows of ``y`` by expert as in
+    product's kernel quantises itself; ``w``: blocks [experts, blocks of features, runs, 128, 128], ``w_scales`` [experts, rows of scales, runs]
+    (``paired``: of (gate, up) row pairs); ``features`` x ``columns`` of a matrix count.  ``routing`` = (offsets, order, top, x_by_pair) sorts the rows of ``y`` by expert as in
     :func:`moe_expert_product`; without it there is one matrix and row m of ``y`` is that of row m."""
     _on_current_device(x, "x"), _rows_of(x, "x"), _rows_of(y, "y"), _need(w, "w", torch.float8_e4m3fn), _need(w_scales, "w_scales", torch.float32)
-    experts, n, k = w.shape
+    experts, n, runs = w.shape[0], features, -(-columns // 128)
     offsets, order, top, x_by_pair = routing if routing is not None else (None, None, 1, False)
     if scales is not None:
         _need(x, "x", torch.float8_e4m3fn), _need(scales, "scales", torch.float32)
-    if (k != -(-columns // 128) * 128 or x.shape[1] != (columns if scales is None else k) or w_scales.shape[0] != experts or w_scales.shape[2] != k // 128
-            or y.shape[1] != (n // 2 if act in MOE_GATED else n) or (routing is None and y.shape[0] != x.shape[0])):
+    if (w.shape[1:] != (-(-n // 128), runs, 128, 128) or x.shape[1] != (columns if scales is None else runs * 128) or w_scales.shape[0] != experts
+            or w_scales.shape[2] != runs or y.shape[1] != (n // 2 if act in MOE_GATED else n) or (routing is None and y.shape[0] != x.shape[0])):
         raise KernelError("block_scaled_product: shapes do not fit")
     if scales is not None and routing is None and act in ("none", "swiglu") and block_scaled_pairs_of_sms(y.shape[0], n):
         _check("block_scaled_product", lib().tib_block_scaled_2cta(
