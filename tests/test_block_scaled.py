@@ -45,16 +45,17 @@ def test_a_weight_keeps_its_matrices_in_whole_blocks():
     a, b, c = random_matrix(256, 200, 0), random_matrix(130, 200, 1), random_matrix(64, 200, 2)
     w = BlockScaledWeight(a, b, c)
     assert (w.out_features, w.in_features, w.dtype) == (450, 200, CODES)
-    assert [(first, n, tuple(x.shape), tuple(s.shape)) for first, n, x, s in w.parts] == \
-        [(0, 386, (1, 4, 2, 128, 128), (1, 4, 2)), (386, 64, (1, 1, 2, 128, 128), (1, 1, 2))]
-    _, _, x, s = w.parts[0]
+    def shapes(weight):
+        return [(first, p.features, tuple(p.codes.shape), tuple(p.scales.shape)) for first, p in weight.parts]
+    assert shapes(w) == [(0, 386, (1, 4, 2, 128, 128), (1, 4, 2)), (386, 64, (1, 1, 2, 128, 128), (1, 1, 2))]
+    x, s = w.parts[0][1].codes, w.parts[0][1].scales
     assert torch.equal(flat(x[0], 256)[:, :200], a.codes.view(torch.uint8)) and torch.equal(s[0, 2:], b.scales)
     assert torch.equal(flat(x[0], 386)[256:, :200], b.codes.view(torch.uint8))
     assert not flat(x[0], 512)[:, 200:].any() and not flat(x[0], 512)[386:].any()
     assert w.nbytes() == 5 * 2 * 128 * 128 + 4 * (8 + 2)
     view = w.rows(128, 400)
-    assert view.out_features == 272 and [(first, n, x.shape[1], s.shape[1]) for first, n, x, s in view.parts] == [(0, 258, 3, 3), (258, 14, 1, 1)]
-    assert torch.equal(view.parts[0][2].view(torch.uint8), w.parts[0][2][:, 1:].view(torch.uint8))
+    assert view.out_features == 272 and shapes(view) == [(0, 258, (1, 3, 2, 128, 128), (1, 3, 2)), (258, 14, (1, 1, 2, 128, 128), (1, 1, 2))]
+    assert torch.equal(view.parts[0][1].codes.view(torch.uint8), x[:, 1:].view(torch.uint8))
     for start, stop in ((64, 130), (0, 451), (5, 5), (-1, 4)):
         with pytest.raises(ValueError):
             w.rows(start, stop)
@@ -62,13 +63,13 @@ def test_a_weight_keeps_its_matrices_in_whole_blocks():
 
 def test_gate_and_up_alternate():
     g, u = random_matrix(130, 300, 0), random_matrix(130, 300, 1)
-    _, n, x, s = BlockScaledWeight(g, u, epilogue="swiglu").parts[0]
-    x = flat(x[0], 260)
-    assert n == 260
+    part = BlockScaledWeight(g, u, epilogue="swiglu").parts[0][1]
+    x, s = flat(part.codes[0], 260), part.scales
+    assert part.features == 260 and part.paired
     assert torch.equal(x[0::2, :300], g.codes.view(torch.uint8)) and torch.equal(x[1::2, :300], u.codes.view(torch.uint8))
     assert torch.equal(s[0, 0::2], g.scales) and torch.equal(s[0, 1::2], u.scales)
     e = BlockScaledExperts([g, u], [u, g])
-    assert e.out_features == 260 and torch.equal(flat(e.codes[1], 260)[0::2, :300], u.codes.view(torch.uint8))
+    assert e.out_features == 260 and torch.equal(flat(e.blocks.codes[1], 260)[0::2, :300], u.codes.view(torch.uint8))
 
 
 def test_products_need_a_gpu():

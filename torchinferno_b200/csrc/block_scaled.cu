@@ -19,8 +19,10 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__
   const int eighth = threadIdx.x & 7, row = row8 * 8 + (threadIdx.x >> 5), run = (blockIdx.x - row8 * groups) * 4 + ((threadIdx.x >> 3) & 3);
   const bool in = row < (order ? min(rows, *sorted) : rows) && run < runs;
   const int col = run * kBlk + eighth * 16, from = !in ? 0 : order ? order[row] / top : row;
+  uint4 raw[sizeof(T)];
   float v[16];
-  bs_load16<T, VEC>(x + (size_t)from * ldx + (in ? col : 0), in ? K - col : 0, v);
+  bs_ask16<T, VEC>(x + (size_t)from * ldx + (in ? col : 0), in ? K - col : 0, raw);
+  bs_floats16<T>(raw, v);
   uint32_t largest = 0;
 #pragma unroll
   for (int j = 0; j < 16; ++j) largest = max(largest, __float_as_uint(v[j]) & 0x7fffffffu);

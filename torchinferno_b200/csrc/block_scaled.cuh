@@ -46,36 +46,32 @@ __device__ __forceinline__ uint32_t bs_codes2(float lo, float hi) {
 }
 __device__ __forceinline__ uint32_t bs_codes4(float a, float b, float c, float d) { return bs_codes2(a, b) | (bs_codes2(c, d) << 16); }
 
-// sixteen numbers of a row as floats, those from the n-th on zero; VEC: p is 16-byte aligned
-template <typename T, bool VEC>
-__device__ __forceinline__ void bs_load16(const T* p, int n, float (&v)[16]) {
-  if constexpr (VEC) {
-    constexpr int kPer = 16 / sizeof(T);
+// Sixteen numbers of a row, those from the n-th on zero, as they lie in memory (VEC: p is 16-byte aligned), and as floats.  (Two steps, so that a
+// load may be on its way while others are worked on.)
+template <typename T, bool VEC> __device__ __forceinline__ void bs_ask16(const T* p, int n, uint4 (&raw)[sizeof(T)]) {
+  constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
-    for (int i = 0; i < 16 / kPer; ++i) {
-      uint4 raw = make_uint4(0, 0, 0, 0);
-      if (n >= (i + 1) * kPer) raw = reinterpret_cast<const uint4*>(p)[i];
-      else if (n > i * kPer) {
-        T piece[kPer];
+  for (int i = 0; i < (int)sizeof(T); ++i) {
+    if (VEC && n >= (i + 1) * kPer) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+    else {
+      T piece[kPer];
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) piece[j] = i * kPer + j < n ? p[i * kPer + j] : from_f32<T>(0.f);
-        raw = *reinterpret_cast<const uint4*>(piece);
-      }
-      if constexpr (sizeof(T) == 2) {
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
-          v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-        }
-      } else {
-        v[4 * i] = __uint_as_float(raw.x); v[4 * i + 1] = __uint_as_float(raw.y);
-        v[4 * i + 2] = __uint_as_float(raw.z); v[4 * i + 3] = __uint_as_float(raw.w);
-      }
+      for (int j = 0; j < kPer; ++j) piece[j] = i * kPer + j < n ? p[i * kPer + j] : from_f32<T>(0.f);
+      raw[i] = *reinterpret_cast<const uint4*>(piece);
     }
-  } else {
+  }
+}
+template <typename T> __device__ __forceinline__ void bs_floats16(const uint4 (&raw)[sizeof(T)], float (&v)[16]) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = j < n ? to_f32(p[j]) : 0.f;
+  for (int i = 0; i < (int)sizeof(T); ++i) {
+    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 2) {
+        v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
+        v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      } else v[4 * i + j] = __uint_as_float(w[j]);
+    }
   }
 }
 

@@ -19,7 +19,7 @@ namespace tib {
 
 constexpr int kB2Stages = 6, kB2Threads = 384;
 constexpr uint32_t kB2Half = 128 * kBlk, kB2Stage = 2 * kB2Half;
-constexpr uint32_t kB2Smem = kB2Stages * kB2Stage + 1024 /* alignment */ + 256 /* barriers */;
+constexpr uint32_t kB2Smem = kB2Stages * kB2Stage + 1024 /* alignment */ + 256 /* barriers */ + 8 * 4096 /* outputs */;
 // D fp32, A and B e4m3, both K-major, N = 256, M = 256 over the pair
 constexpr uint32_t kB2Idesc = (1u << 4) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
 
@@ -162,42 +162,58 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
         step(kb, 0);
         if (kb + 1 < a.runs && ok) step(kb + 1, 1);
       }
-      if (!ok || row >= a.M) continue;
-      constexpr int kOut = SWIGLU ? 64 : 128;                  // outputs of this thread
+      if (!ok) continue;
+      // A row's outputs lie in one thread: a warp's 32 rows cross its 4 KB of shared memory, 128 bytes of each at a time (16-byte pieces, swizzled by row),
+      // and leave as whole lines.  (Stored by their threads, 16 bytes of 32 rows an instruction, a tile's outputs took 3 us.)
+      constexpr int kOut = SWIGLU ? 64 : 128, kVec = 16 / sizeof(TO), kTurn = 8 * kVec;      // outputs of a thread, a piece, a turn
       const int first = SWIGLU ? col0 >> 1 : col0, n_out = SWIGLU ? a.N >> 1 : a.N;
-      TO* dst = out + (size_t)row * ldo + first;
-      constexpr int kVec = 16 / sizeof(TO);
+      unsigned char* mine = smem_raw + (base - smem_u32(smem_raw)) + kB2Stages * kB2Stage + 256 + (warp - 4) * 4096;
 #pragma unroll
-      for (int c = 0; c < kOut; c += kVec) {
-        float y[kVec];
+      for (int turn = 0; turn < kOut / kTurn; ++turn) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-          if constexpr (SWIGLU) {
-            float g, u;
-            f2_unpack(sum[c + j], g, u);
-            y[j] = g * bs_sigmoid(g) * u;
-          } else {
-            float lo, hi;
-            f2_unpack(sum[(c + j) >> 1], lo, hi);
-            y[j] = j & 1 ? hi : lo;
+        for (int p = 0; p < 8; ++p) {
+          float y[kVec];
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) {
+            const int c = turn * kTurn + p * kVec + j;
+            if constexpr (SWIGLU) {
+              float g, u;
+              f2_unpack(sum[c], g, u);
+              y[j] = g * bs_sigmoid(g) * u;
+            } else {
+              float lo, hi;
+              f2_unpack(sum[c >> 1], lo, hi);
+              y[j] = c & 1 ? hi : lo;
+            }
           }
-        }
-        if (wide_stores && first + c + kVec <= n_out) {
           uint4 w;
           if constexpr (sizeof(TO) == 2) {
-            __nv_bfloat162 p[4];
+            __nv_bfloat162 b2[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = __floats2bfloat162_rn(y[2 * j], y[2 * j + 1]);
-            w = *reinterpret_cast<const uint4*>(p);
+            for (int j = 0; j < 4; ++j) b2[j] = __floats2bfloat162_rn(y[2 * j], y[2 * j + 1]);
+            w = *reinterpret_cast<const uint4*>(b2);
           } else {
             w = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
           }
-          *reinterpret_cast<uint4*>(dst + c) = w;
-        } else {
-#pragma unroll
-          for (int j = 0; j < kVec; ++j)
-            if (first + c + j < n_out) dst[c + j] = from_f32<TO>(y[j]);
+          *reinterpret_cast<uint4*>(mine + lane * 128 + ((p ^ (lane & 7)) << 4)) = w;
         }
+        __syncwarp();
+        const int p = lane & 7, col = first + turn * kTurn + p * kVec;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = 4 * i + (lane >> 3);
+          const uint4 w = *reinterpret_cast<const uint4*>(mine + r * 128 + ((p ^ (r & 7)) << 4));
+          if (row - lane + r >= a.M) continue;
+          TO* dst = out + (size_t)(row - lane + r) * ldo + col;
+          if (wide_stores && col + kVec <= n_out) *reinterpret_cast<uint4*>(dst) = w;
+          else {
+            const TO* one = reinterpret_cast<const TO*>(&w);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j)
+              if (col + j < n_out) dst[j] = one[j];
+          }
+        }
+        __syncwarp();
       }
     }
   } else {

@@ -6,8 +6,7 @@
 // row of the swizzle, four MMAs into an accumulator of its own in tensor memory, which the summing warps take out and add to 32-bit sums in
 // registers, times the scale of (row, run) and (block of features, run), whose product is made once a row and step (packed fp32, one multiply-add for
 // two sums).  kBufs accumulators rotate, so the tensor cores run ahead of the sums.
-//   warp 0             TMA producer: 16 KB of codes of w a step, one block of the matrix, which lies in memory as such (rows of 128 bytes a
-//                      matrix row apart came from memory at half the rate), and the rows' codes where they exist, in boxes of 32 rows
+//   warp 0             TMA producer: 16 KB of codes of w a step, one block of the matrix, and the rows' codes where they exist, in boxes of 32 rows
 //   warp 1             issues tcgen05.mma; owns the TMEM allocation
 //   the next 4 or 8    sums and epilogue (eight for 128 rows: four for each half of the columns)
 //   the last 2 or 4    helpers, taking turns: the products of scales into a ring of their own; from rows that are no codes yet they (then four) make
@@ -173,6 +172,10 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
   const int cluster_id = blockIdx.x / splits, clusters = gridDim.x / splits;
   const int kb0 = (int)((int64_t)a.runs * rank / splits), kb1 = (int)((int64_t)a.runs * (rank + 1) / splits);
   if (warp == 0) {
+    if (lane == 0) {
+      asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map_w) : "memory");
+      if constexpr (kCodes) asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map_x) : "memory");
+    }
     if (lane < a.stages) {
       mbar_init(full_bar(lane), kCodes ? 1 : 2);  // the producer, and the helper that makes codes
       mbar_init(empty_bar(lane), 1);
@@ -185,7 +188,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
       mbar_init(acc_full_bar(lane), 1);
       mbar_init(acc_empty_bar(lane), S::kStorers);
     }
-    if (lane == 0) mbar_init(red_bar, S::kStorers * splits);
+    if (lane == 0) mbar_init(red_bar, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 1) {
@@ -395,17 +398,18 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int feature = quarter * 32 + 16 * h + 8 * i + lane8;
-            const uint32_t dst = map_to_cta(smem_u32(red + (rank * NT + c0 + pair) * stride + (feature & (per - 1))), feature >> (7 - log_splits));
+            const int owner = feature >> (7 - log_splits);
+            const uint32_t dst = map_to_cta(smem_u32(red + (rank * NT + c0 + pair) * stride + (feature & (per - 1))), owner);
+            const uint32_t bar = map_to_cta(red_bar, owner);
 #pragma unroll
             for (int j = 0; j < S::kCols / 8; ++j) {
               float lo, hi;
               f2_unpack(sum[h][2 * j + i], lo, hi);
-              st_cluster_f32(dst + 8 * j * stride * 4, lo);
-              st_cluster_f32(dst + (8 * j + 1) * stride * 4, hi);
+              st_async_f32(dst + 8 * j * stride * 4, lo, bar);
+              st_async_f32(dst + (8 * j + 1) * stride * 4, hi, bar);
             }
           }
-        __syncwarp();
-        if (lane < splits) mbar_arrive_remote(map_to_cta(red_bar, lane));
+        if (et == 0) mbar_expect_tx(red_bar, 128 * NT * 4);      // (the stores themselves count on the owner's barrier: no fence, no arrivals)
         if (!mbar_wait_cluster(red_bar, 0)) {
           if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00C5);
           ok = false;
@@ -422,87 +426,122 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
       }
     }
   } else {
-    const int helper = warp - 2 - S::kStorers;
-    int it = 0, s = 0, slot = 0;
-    uint32_t phase = 1, slot_phase = 1;
+    // this helper's steps: the first, and every kHelpers-th after it
+    int kb = kb0 + warp - 2 - S::kStorers, s = (warp - 2 - S::kStorers) % a.stages, slot = warp - 2 - S::kStorers;
+    uint32_t phase = 1 ^ (((warp - 2 - S::kStorers) / a.stages) & 1), slot_phase = 1;
     bool ok = true;
+    auto advance = [&]() {
+      kb += S::kHelpers;
+      for (s += S::kHelpers; s >= a.stages; s -= a.stages) phase ^= 1;
+      if ((slot += S::kHelpers) >= kBsSlots) { slot -= kBsSlots; slot_phase ^= 1; }
+    };
     if (!a.offsets) pdl_wait();
-    for (int t = cluster_id; t < num_tiles && ok; t += clusters) {
+    for (int t = cluster_id; t < num_tiles && ok; t += clusters, kb -= kb1 - kb0) {
       const BsTile m = tile_of(t);
       const float* ws = a.w_scales + ((size_t)m.expert * a.scale_rows + bs_scale_row(m.feature, a.pairs)) * a.runs;
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        if (it % S::kHelpers == helper) {
-          float* scales = step_scales + slot * S::kScales;
-          const float even = ws[kb], odd = a.pairs ? ws[a.runs + kb] : even;
-          if constexpr (kCodes) {
-            float v[NT / 32];
+      if constexpr (kCodes) {
+        // (four of this helper's steps at a time: their loads are on their way together)
+        while (kb < kb1 && ok) {
+          float v[4][NT / 32], even[4], odd[4];
 #pragma unroll
-            for (int i = 0; i < NT / 32; ++i) v[i] = a.x_scales[(size_t)kb * a.lds + m.first + min(lane + 32 * i, m.rows - 1)];
-            if (!mbar_wait_warp(scale_empty_bar(slot), slot_phase)) ok = false;
+          for (int j = 0; j < 4; ++j) {
+            const int at = min(kb + j * S::kHelpers, kb1 - 1);
+            even[j] = ws[at];
+            odd[j] = a.pairs ? ws[a.runs + at] : even[j];
+#pragma unroll
+            for (int i = 0; i < NT / 32; ++i) v[j][i] = a.x_scales[(size_t)at * a.lds + m.first + min(lane + 32 * i, m.rows - 1)];
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (kb >= kb1) break;
+            if (!mbar_wait_warp(scale_empty_bar(slot), slot_phase)) {
+              ok = false;
+              break;
+            }
+            float* scales = step_scales + slot * S::kScales;
 #pragma unroll
             for (int i = 0; i < NT / 32; ++i) {
-              scales[lane + 32 * i] = v[i] * even;
-              scales[NT + 8 + lane + 32 * i] = v[i] * odd;
+              scales[lane + 32 * i] = v[j][i] * even[j];
+              scales[NT + 8 + lane + 32 * i] = v[j][i] * odd[j];
             }
-          } else {
-            // eight lanes a row, sixteen columns each; two rows a lane at a time
-            const TX* x = reinterpret_cast<const TX*>(a.x);
-            unsigned char* codes = smem_gen + s * S::kStage + kBsWBytes;
-            const int sub = lane >> 3, eighth = lane & 7, col = kb * kBlk + eighth * 16;
-            bool free = false;
-#pragma unroll 1
-            for (int r0 = 0; r0 < m.rows; r0 += 8) {
-              float v[2][16];
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int r = r0 + 4 * h + sub;
-                const TX* p = x + (size_t)source(m, r) * a.ldx + min(col, a.K - 1);
-                const int n = r < m.rows ? a.K - col : 0;
-                if (a.vec) bs_load16<TX, true>(p, n, v[h]);
-                else bs_load16<TX, false>(p, n, v[h]);
-              }
-              if (!free) {
-                if (!(mbar_wait_warp(empty_bar(s), phase) && mbar_wait_warp(scale_empty_bar(slot), slot_phase))) ok = false;
-                free = true;
-              }
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int r = r0 + 4 * h + sub;
-                uint32_t largest = 0;
-#pragma unroll
-                for (int j = 0; j < 16; ++j) largest = max(largest, __float_as_uint(v[h][j]) & 0x7fffffffu);
-#pragma unroll
-                for (int o = 1; o < 8; o <<= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-                float scale, inverse;
-                bs_run_scale(largest, scale, inverse);
-                uint32_t w[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  w[j] = bs_codes4(v[h][4 * j] * inverse, v[h][4 * j + 1] * inverse, v[h][4 * j + 2] * inverse, v[h][4 * j + 3] * inverse);
-                if (r < m.rows && ok) {
-                  *reinterpret_cast<uint4*>(codes + r * kBlk + ((eighth ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                  if (eighth == 0) {
-                    scales[r] = scale * even;
-                    scales[NT + 8 + r] = scale * odd;
-                  }
-                }
-              }
-            }
-            bs_fence_async_shared();
-          }
-          if (!ok) {
-            if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00C6);
-            break;
-          }
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(scale_full_bar(slot));
-            if constexpr (!kCodes) mbar_arrive(full_bar(s));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(scale_full_bar(slot));
+            advance();
           }
         }
-        if (++s == a.stages) { s = 0; phase ^= 1; }
-        if (++slot == kBsSlots) { slot = 0; slot_phase ^= 1; }
+      } else {
+        // Eight lanes a row, sixteen columns each; two rows a lane at a time, the next two (of this step or this helper's next) on their way.
+        const TX* x = reinterpret_cast<const TX*>(a.x);
+        const int sub = lane >> 3, eighth = lane & 7;
+        struct Rows { uint4 raw[2][sizeof(TX)]; float even, odd; };
+        auto ask = [&](Rows& q, int step, int r0) {
+          if (step >= kb1) return;
+          const int col = step * kBlk + eighth * 16;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = r0 + 4 * h + sub;
+            const TX* p = x + (size_t)source(m, r) * a.ldx + min(col, a.K - 1);
+            const int n = r < m.rows ? a.K - col : 0;
+            if (a.vec) bs_ask16<TX, true>(p, n, q.raw[h]);
+            else bs_ask16<TX, false>(p, n, q.raw[h]);
+          }
+          q.even = ws[step];
+          q.odd = a.pairs ? ws[a.runs + step] : q.even;
+        };
+        int r0 = 0;
+        auto turn = [&](Rows& now, Rows& next) {
+          const bool last = r0 + 8 >= m.rows;
+          ask(next, last ? kb + S::kHelpers : kb, last ? 0 : r0 + 8);
+          if (r0 == 0 && !(mbar_wait_warp(empty_bar(s), phase) && mbar_wait_warp(scale_empty_bar(slot), slot_phase))) {
+            ok = false;
+            return;
+          }
+          float* scales = step_scales + slot * S::kScales;
+          unsigned char* codes = smem_gen + s * S::kStage + kBsWBytes;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = r0 + 4 * h + sub;
+            float v[16];
+            bs_floats16<TX>(now.raw[h], v);
+            uint32_t largest = 0;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) largest = max(largest, __float_as_uint(v[j]) & 0x7fffffffu);
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+            float scale, inverse;
+            bs_run_scale(largest, scale, inverse);
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              w[j] = bs_codes4(v[4 * j] * inverse, v[4 * j + 1] * inverse, v[4 * j + 2] * inverse, v[4 * j + 3] * inverse);
+            if (r < m.rows) {
+              *reinterpret_cast<uint4*>(codes + r * kBlk + ((eighth ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+              if (eighth == 0) {
+                scales[r] = scale * now.even;
+                scales[NT + 8 + r] = scale * now.odd;
+              }
+            }
+          }
+          if (last) {
+            bs_fence_async_shared();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(scale_full_bar(slot));
+              mbar_arrive(full_bar(s));
+            }
+            advance();
+            r0 = 0;
+          } else r0 += 8;
+        };
+        Rows p, q;
+        ask(p, kb, 0);
+        while (kb < kb1 && ok) {
+          turn(p, q);
+          if (kb < kb1 && ok) turn(q, p);
+          else break;
+        }
       }
+      if (!ok && a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00C6);
     }
   }
   __syncwarp();
@@ -559,10 +598,12 @@ static int launch_block_scaled(const CUtensorMap& map_w, const CUtensorMap& map_
   return TIB_OK;
 }
 
-// The blocks that share a tile's runs: as many as make the GPU's worth of blocks of few tiles, each with two runs or more.
-static int bs_splits(int64_t tiles, int runs) {
+// The blocks that share a tile's runs: as many as there is room for beside the other tiles', four runs each at least, and eight blocks only for 64 runs.
+// (8 rows, us, by 1 / 2 / 4 / 8 blocks a tile: 4,096 -> 4,096 14.2 / 9.8 / 8.3 / 9.0, 14,336 -> 4,096 43 / 25 / 16.7 / 15.0, 4,096 -> 6,144 14.2 / 10.6 /
+// 9.1 / 14.8, 4,096 -> 14,336 16.3 / 13.6 / 19.0 / 30.4, 2,048 -> 2,048 8.2 / 6.5 / 5.9 / 6.1.)
+static int bs_splits(int64_t tiles, int runs, int blocks) {
   int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= 148 && runs >= 4 * splits) splits *= 2;
+  while (splits < 8 && tiles * splits * 2 <= blocks && runs >= (splits < 4 ? 4 * splits : 64)) splits *= 2;
   return splits;
 }
 
@@ -570,7 +611,8 @@ static int bs_splits(int64_t tiles, int runs) {
 
 using namespace tib;
 
-// x_dtype TIB_BF16 or TIB_F32: rows [rows, K] (row stride ldx) that are quantised on the way, once for each tile of 128 features; -1: codes
+// x_dtype TIB_BF16 or TIB_F32: rows [rows, K] (row stride ldx) that are quantised on the way, for each tile of 16 rows x
+// 128 features; -1: codes
 // [x_rows, runs * 128] and scales [runs, lds] as tib_quantize_rows leaves them, row m of them for row m of y.  w: codes in blocks
 // [experts, ceil(N / 128), runs, 128, 128], features and columns behind the last zero, and scales [experts, scale_rows, runs] (`pairs`: of (gate, up) row pairs); y: [M, N] in y_dtype (row stride ldy), or [M, N / 2] of a gated activation.
 // offsets [experts + 1] and order [M]: rows sorted by expert as tib_moe_expert_product takes them; offsets null: one matrix for all rows.
@@ -602,7 +644,7 @@ TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, in
     if (rc != TIB_OK) return rc;
   }
   const int rows = offsets ? ceil_div(M, experts) : M;      // (of an expert, on average)
-  auto splits = [&](int nt) { return offsets ? 1 : bs_splits((int64_t)ceil_div(M, nt) * ceil_div(N, 128), a.runs); };
+  auto splits = [&](int nt) { return offsets ? 1 : bs_splits((int64_t)ceil_div(M, nt) * ceil_div(N, 128), a.runs, nt <= 32 ? 296 : 148); };
 #define TIB_BS_GO(NT, TX)                                                                                                  \
   return y_dtype == TIB_BF16 ? launch_block_scaled<NT, TX, __nv_bfloat16>(map_w, map_x, a, y, ldy, splits(NT), stream)      \
                              : launch_block_scaled<NT, TX, float>(map_w, map_x, a, y, ldy, splits(NT), stream)
@@ -611,14 +653,8 @@ TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, in
     if (rows <= 64) TIB_BS_GO(64, uint8_t);
     TIB_BS_GO(128, uint8_t);
   }
-  if (x_dtype == TIB_BF16) {
-    if (rows <= 16) TIB_BS_GO(16, __nv_bfloat16);
-    if (rows <= 32) TIB_BS_GO(32, __nv_bfloat16);
-    TIB_BS_GO(64, __nv_bfloat16);
-  }
-  if (rows <= 16) TIB_BS_GO(16, float);
-  if (rows <= 32) TIB_BS_GO(32, float);
-  TIB_BS_GO(64, float);
+  if (x_dtype == TIB_BF16) TIB_BS_GO(16, __nv_bfloat16);
+  TIB_BS_GO(16, float);
 #undef TIB_BS_GO
 }
 

@@ -23,9 +23,11 @@ from torchinferno_b200.kernels import ops
 
 BLOCK = 128
 CODE_DTYPE = torch.float8_e4m3fn
-# Up to so many rows (of an expert: on average) a product's kernel quantises its rows itself, in every tile of 128 features anew.
-FEW_ROWS = 64
-FEW_EXPERT_ROWS = 16
+# Up to so many rows (of an expert: on average) a product's kernel quantises its rows itself, in every tile of 128 features anew; more are quantised ahead
+# of it.  (us, itself / ahead: 8 rows 4,096 -> 4,096 8.1 / 9.8, 4,096 -> 28,672 20.6 / 23.4, 14,336 -> 4,096 13.5 / 16.5; 12 rows 9.3 / 9.7, 27.2 / 23.5,
+# 16.0 / 16.7; 24 rows 12.2 / 9.8, 37.4 / 22.9, 20.5 / 16.8.)
+FEW_ROWS = 8
+FEW_EXPERT_ROWS = 8
 
 
 def blocks(count: int) -> int:
@@ -79,25 +81,49 @@ def quantize_matrix(matrix: torch.Tensor) -> BlockScaledMatrix:
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(codes [M, K], scales [M, runs of 128]) of the rows ``x`` [M, K] (bfloat16 or float32, any row stride); see the module's text."""
-    codes, scales = _quantized(x)
-    return codes[:, :x.shape[1]], scales[:, :x.shape[0]].t()
+    rows, columns = _row_shape(x)
+    runs = blocks(columns)
+    lds = (rows + 3) & ~3
+    codes = torch.empty((rows, runs * BLOCK), dtype=CODE_DTYPE, device=x.device)
+    scales = torch.empty_strided((lds, runs), (1, lds), dtype=torch.float32, device=x.device)
+    ops.quantize_rows(x, columns, codes.data_ptr(), scales.data_ptr(), lds)
+    return codes if columns == runs * BLOCK else codes[:, :columns], scales if lds == rows else scales[:rows]
 
 
-def _quantized(x: torch.Tensor, routing: tuple[torch.Tensor, torch.Tensor, int] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """Codes and scales as the products read them: columns padded to whole runs; a run's scales side by side, rows rounded up to 4.  ``routing`` =
-    (offsets, order, top): the rows of the pairs sorted by expert."""
+def _row_shape(x: torch.Tensor) -> tuple[int, int]:
     if x.dim() != 2 or x.shape[1] == 0:
         raise ops.KernelError(f"rows to quantise must be [rows, columns], got {tuple(x.shape)}")
-    rows, runs = x.shape[0] if routing is None else routing[1].numel(), blocks(x.shape[1])
-    codes = torch.empty((rows, runs * BLOCK), dtype=CODE_DTYPE, device=x.device)
-    scales = torch.empty((runs, -(-rows // 4) * 4), dtype=torch.float32, device=x.device)
-    ops.quantize_rows(x, codes, scales, routing)
-    return codes, scales
+    return x.shape[0], x.shape[1]
 
 
-def _laid_out(matrices: Sequence[BlockScaledMatrix], ups: Sequence[BlockScaledMatrix] | None) -> tuple[torch.Tensor, torch.Tensor]:
-    """Codes [matrices, blocks of N, blocks of K, 128, 128], padded with zeros, and scales [matrices, blocks of N, blocks of K] of equally large
-    matrices; with ``ups`` the rows of either alternate (gate i, up i; gate block j, up block j)."""
+def _quantized(x: torch.Tensor, columns: int, routing: tuple[torch.Tensor, torch.Tensor, int] | None = None) -> tuple[torch.Tensor, tuple[int, int, int]]:
+    """The rows' codes and scales as the products read them: a buffer (to be held until the product is launched), and what
+    :func:`ops.block_scaled_product` takes.  ``routing`` = (offsets, order, top): the rows of the pairs sorted by expert."""
+    rows, runs = x.shape[0] if routing is None else routing[1].numel(), -(-columns // BLOCK)
+    lds = (rows + 3) & ~3
+    buffer = torch.empty(rows * runs * BLOCK + 4 * lds * runs, dtype=torch.uint8, device=x.device)
+    at = buffer.data_ptr()
+    codes = (at, at + rows * runs * BLOCK, lds)
+    ops.quantize_rows(x, columns, *codes, routing)
+    return buffer, codes
+
+
+class Blocks:
+    """Matrices of one size as the kernels read them: ``codes`` [matrices, blocks of N, blocks of K, 128, 128], padded with zeros, and ``scales`` [matrices,
+    blocks of N, blocks of K]; ``paired``: the matrices' rows are (gate i, up i), their scales' rows (gate block j, up block j)."""
+    __slots__ = ("codes", "scales", "features", "paired", "codes_at", "scales_at", "scale_rows")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, features: int, paired: bool) -> None:
+        if codes.shape[1] != blocks(features) or scales.shape[1:] != (codes.shape[1] if not paired else 2 * blocks(features // 2), codes.shape[2]):
+            raise ValueError(f"blocks {tuple(codes.shape)} and scales {tuple(scales.shape)} do not make matrices of {features} rows")
+        if not codes.is_contiguous() or not scales.is_contiguous():
+            raise ValueError("blocks and their scales must be contiguous")
+        self.codes, self.scales, self.features, self.paired = codes, scales, features, paired
+        self.codes_at, self.scales_at, self.scale_rows = codes.data_ptr(), scales.data_ptr(), scales.shape[1]
+
+
+def _laid_out(matrices: Sequence[BlockScaledMatrix], ups: Sequence[BlockScaledMatrix] | None) -> Blocks:
+    """Equally large matrices in blocks; with ``ups`` the rows of either alternate (gate i, up i; gate block j, up block j)."""
     shape, device = matrices[0].shape, matrices[0].device
     for m in [*matrices, *(ups or ())]:
         if m.shape != shape or m.device != device:
@@ -115,7 +141,7 @@ def _laid_out(matrices: Sequence[BlockScaledMatrix], ups: Sequence[BlockScaledMa
             flat[part:n * parts:parts, :k] = stack[i].codes.view(torch.uint8)
             scales[i, :, part] = stack[i].scales
         codes[i] = flat.view(tiles, BLOCK, runs, BLOCK).transpose(1, 2)
-    return codes.view(CODE_DTYPE), scales.view(len(matrices), blocks(n) * parts, -1)
+    return Blocks(codes.view(CODE_DTYPE), scales.view(len(matrices), blocks(n) * parts, -1), n * parts, ups is not None)
 
 
 class BlockScaledWeight:
@@ -134,11 +160,11 @@ class BlockScaledWeight:
             raise ValueError("the matrices of a weight need the same columns and device")
         self.epilogue, self.in_features = epilogue, matrices[0].shape[1]
         self.out_features = sum(m.shape[0] for m in matrices)
-        # (first output, outputs, codes, scales) of every product to run.  Matrices are put together while the ones before end with a whole block;
-        # where one does not, its blocks' borders would not be the joint matrix's: it starts a product of its own.
-        self.parts: list[tuple[int, int, torch.Tensor, torch.Tensor]] = []
+        # (first output, blocks) of every product to run.  Matrices are put together while the ones before end with a whole block; where one
+        # does not, its blocks' borders would not be the joint matrix's: it starts a product of its own.
+        self.parts: list[tuple[int, Blocks]] = []
         if epilogue == "swiglu":
-            self.parts.append((0, self.out_features, *_laid_out(matrices[:1], matrices[1:])))
+            self.parts.append((0, _laid_out(matrices[:1], matrices[1:])))
             return
         first, run = 0, []
         for i, m in enumerate(matrices):
@@ -146,7 +172,7 @@ class BlockScaledWeight:
             if m.shape[0] % BLOCK or i == len(matrices) - 1:
                 joint = run[0] if len(run) == 1 else BlockScaledMatrix(
                     torch.cat([r.codes.view(torch.uint8) for r in run]).view(CODE_DTYPE), torch.cat([r.scales for r in run]))
-                self.parts.append((first, joint.shape[0], *_laid_out([joint], None)))
+                self.parts.append((first, _laid_out([joint], None)))
                 first, run = first + joint.shape[0], []
 
     @property
@@ -155,10 +181,10 @@ class BlockScaledWeight:
 
     @property
     def device(self) -> torch.device:
-        return self.parts[0][2].device
+        return self.parts[0][1].codes.device
 
     def nbytes(self) -> int:
-        return sum(codes.numel() + 4 * scales.numel() for _, _, codes, scales in self.parts)
+        return sum(part.codes.numel() + 4 * part.scales.numel() for _, part in self.parts)
 
     def rows(self, start: int, stop: int) -> "BlockScaledWeight":
         """The projection onto output features start .. stop-1 (views; ``start`` a whole number of blocks into its matrix)."""
@@ -166,27 +192,26 @@ class BlockScaledWeight:
             raise ValueError(f"no features {start} .. {stop - 1} of {self.out_features} to take")
         view = object.__new__(BlockScaledWeight)
         view.epilogue, view.in_features, view.out_features, view.parts = "none", self.in_features, stop - start, []
-        for first, count, codes, scales in self.parts:
-            lo, hi = max(start - first, 0), min(stop - first, count)
+        for first, part in self.parts:
+            lo, hi = max(start - first, 0), min(stop - first, part.features)
             if lo < hi:
                 if lo % BLOCK:
                     raise ValueError(f"feature {start} lies inside a block")
-                view.parts.append((first + lo - start, hi - lo, codes[:, lo // BLOCK:blocks(hi)], scales[:, lo // BLOCK:blocks(hi)]))
+                view.parts.append((first + lo - start, Blocks(part.codes[:, lo // BLOCK:blocks(hi)], part.scales[:, lo // BLOCK:blocks(hi)], hi - lo, False)))
         return view
 
-    def _checked(self, x: torch.Tensor, out_dtype: torch.dtype | None, width: int, out: torch.Tensor | None) -> torch.Tensor:
+    def _target(self, x: torch.Tensor, out_dtype: torch.dtype | None, width: int, out: torch.Tensor | None) -> torch.Tensor:
         """The tensor that the product is written to."""
         if x.dim() != 2 or x.shape[1] != self.in_features:
             raise ops.KernelError(f"linear: shapes {tuple(x.shape)} and {(self.out_features, self.in_features)} do not fit")
-        if not x.is_cuda:
-            raise ops.KernelError("linear: operands must be CUDA tensors (there is no CPU path)")
-        if x.device != self.device:
-            raise ops.KernelError(f"linear: x is on {x.device}, the weight on {self.device}")
-        out_dtype = out_dtype or x.dtype
+        if x.get_device() != self.parts[0][1].codes.get_device() or not x.is_cuda:
+            raise ops.KernelError(f"linear: x is on {x.device}, the weight on {self.device} (there is no CPU path)")
+        if out_dtype is None:
+            out_dtype = x.dtype
         if out_dtype not in (torch.bfloat16, torch.float32):
             raise ops.KernelError(f"linear: unsupported output dtype {out_dtype}")
         if out is None or out.dtype != out_dtype:
-            return torch.empty((x.shape[0], width), dtype=out_dtype, device=x.device)
+            return x.new_empty((x.shape[0], width)) if x.dtype == out_dtype else x.new_empty((x.shape[0], width), dtype=out_dtype)
         if out.shape != (x.shape[0], width) or out.stride(1) != 1 or out.device != x.device:
             raise ops.KernelError(f"linear: out is {tuple(out.shape)}, wanted {(x.shape[0], width)} with unit inner stride on {x.device}")
         return out
@@ -194,26 +219,24 @@ class BlockScaledWeight:
     def product(self, x: torch.Tensor, *, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
                 error_word: torch.Tensor | None = None) -> torch.Tensor:
         """x [tokens, in] times the weight: [tokens, out] (a swiglu weight's gate and up sums side by side)."""
-        out = self._checked(x, out_dtype, self.out_features, out)
+        out = self._target(x, out_dtype, self.out_features, out)
         if x.shape[0] == 0:
             return out
-        rows = (x, None) if x.shape[0] <= FEW_ROWS else _quantized(x)
-        for first, count, codes, scales in self.parts:
-            ops.block_scaled_product(*rows, codes, scales, out if len(self.parts) == 1 else out[:, first:first + count], features=count,
-                                     columns=self.in_features, paired=self.epilogue == "swiglu", error_word=error_word)
+        _held, codes = (None, None) if x.shape[0] <= FEW_ROWS else _quantized(x, self.in_features)
+        for first, part in self.parts:
+            ops.block_scaled_product(x, codes, part, self.in_features, out if len(self.parts) == 1 else out[:, first:first + part.features],
+                                     error_word=error_word)
         return out
 
     def swiglu(self, x: torch.Tensor, *, out_dtype: torch.dtype | None = None, error_word: torch.Tensor | None = None) -> torch.Tensor:
         """silu(gate) * up of the 32-bit sums: [tokens, out / 2]."""
         if self.epilogue != "swiglu":
             raise ops.KernelError("linear_swiglu: the weight was not bound with epilogue='swiglu'")
-        out = self._checked(x, out_dtype, self.out_features // 2, None)
+        out = self._target(x, out_dtype, self.out_features // 2, None)
         if x.shape[0] == 0:
             return out
-        _, count, codes, scales = self.parts[0]
-        rows = (x, None) if x.shape[0] <= FEW_ROWS else _quantized(x)
-        return ops.block_scaled_product(*rows, codes, scales, out, features=count, columns=self.in_features, paired=True, act="swiglu",
-                                        error_word=error_word)
+        _held, codes = (None, None) if x.shape[0] <= FEW_ROWS else _quantized(x, self.in_features)
+        return ops.block_scaled_product(x, codes, self.parts[0][1], self.in_features, out, act="swiglu", error_word=error_word)
 
 
 class BlockScaledExperts:
@@ -224,16 +247,16 @@ class BlockScaledExperts:
         if not matrices:
             raise ValueError("a product of experts needs at least one")
         self.paired = ups is not None
-        self.codes, self.scales = _laid_out(matrices, ups)
+        self.blocks = _laid_out(matrices, ups)
         self.experts, self.in_features = len(matrices), matrices[0].shape[1]
         self.out_features = matrices[0].shape[0] * (2 if self.paired else 1)
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self.blocks.codes.device
 
     def nbytes(self) -> int:
-        return self.codes.numel() + 4 * self.scales.numel()
+        return self.blocks.codes.numel() + 4 * self.blocks.scales.numel()
 
     def product(self, x: torch.Tensor, y: torch.Tensor, offsets: torch.Tensor, order: torch.Tensor, top: int, *, x_by_pair: bool,
                 act: str = "none", limit: float = 0.0, alpha: float = 1.0, row_scale: torch.Tensor | None = None,
@@ -248,9 +271,12 @@ class BlockScaledExperts:
         if (x.dim() != 2 or x.shape[1] != self.in_features or y.shape != (pairs, width) or offsets.numel() != self.experts + 1 or top < 1
                 or (pairs % top if x_by_pair else x.shape[0] < pairs) or (x_by_pair and x.shape[0] < pairs // top)):
             raise ops.KernelError("moe_expert_product: shapes do not fit")
+        here = self.blocks.codes.get_device()
         for name, t in (("x", x), ("y", y), ("offsets", offsets), ("order", order)):
-            if not t.is_cuda or t.device != self.device:
-                raise ops.KernelError(f"moe_expert_product: {name} is on {t.device}, the experts on {self.device}")
+            if t.get_device() != here or here < 0:
+                raise ops.KernelError(f"moe_expert_product: {name} is on {t.device}, the experts on {self.device} (there is no CPU path)")
+        if y.stride(1) != 1:
+            raise ops.KernelError("moe_expert_product: y needs unit inner stride")
         ops._need(offsets, "offsets", torch.int32), ops._need(order, "order", torch.int32)
         if row_scale is not None:
             ops._need(row_scale, "row_scale", torch.float32)
@@ -259,8 +285,8 @@ class BlockScaledExperts:
         if pairs == 0:
             return y
         if pairs <= FEW_EXPERT_ROWS * self.experts:
-            rows, routing = (x, None), (offsets, order, top, x_by_pair)
+            _held, codes = None, None
         else:                                   # (the pairs' rows, sorted on the way)
-            rows, routing = _quantized(x if x_by_pair else x[:pairs], (offsets, order, top) if x_by_pair else None), (offsets, order, top, False)
-        return ops.block_scaled_product(*rows, self.codes, self.scales, y, features=self.out_features, columns=self.in_features, paired=self.paired, act=act, limit=limit,
-                                        alpha=alpha, routing=routing, row_scale=row_scale, error_word=error_word)
+            _held, codes = _quantized(x if x_by_pair else x[:pairs], self.in_features, (offsets, order, top) if x_by_pair else None)
+        return ops.block_scaled_product(x, codes, self.blocks, self.in_features, y, act=act, limit=limit, alpha=alpha,
+                                        routing=(offsets, order, top, x_by_pair), row_scale=row_scale, error_word=error_word)

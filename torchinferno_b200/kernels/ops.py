@@ -1254,57 +1254,61 @@ def moe_combine(y: torch.Tensor, place: torch.Tensor, weights: torch.Tensor | No
 
 
 # ---------------------------------------------------------------------------
-# 8-bit block-scaled operands (csrc/block_scaled.cu); their Python types are in kernels/block_scaled.py.
-def _on_current_device(t: torch.Tensor, name: str) -> None:
-    if not t.is_cuda:
-        raise KernelError(f"{name} must be a CUDA tensor (there is no CPU path)")
-    if t.device.index != torch._C._cuda_getDevice():
-        raise KernelError(f"{name} is on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+# 8-bit block-scaled operands (csrc/block_scaled*.cu).  Their Python types (kernels/block_scaled.py) check shapes and own the buffers; these take addresses, as
+# a call with few rows is as long as what the host does for it.
+def _rows_here(x: torch.Tensor, columns: int, name: str) -> None:
+    """Rows of ``columns`` numbers on the current device, with unit inner stride."""
+    device = x.get_device()
+    if device < 0:
+        raise KernelError(f"{name}: x must be a CUDA tensor (there is no CPU path)")
+    if device != torch._C._cuda_getDevice():
+        raise KernelError(f"{name}: x is on {x.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    if x.dim() != 2 or x.shape[1] != columns or (x.stride(1) != 1 and columns > 1):
+        raise KernelError(f"{name}: rows of {columns} numbers with unit inner stride are wanted, not {tuple(x.shape)} with strides {x.stride()}")
 
 
-def quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, routing: tuple[torch.Tensor, torch.Tensor, int] | None = None) -> None:
-    """Codes [rows, K rounded up to 128] (8 bits) and scales [runs of 128 columns, at least rows] of the rows ``x`` [rows, K].  ``routing`` =
+def quantize_rows(x: torch.Tensor, columns: int, codes: int, scales: int, lds: int, routing: tuple[torch.Tensor, torch.Tensor, int] | None = None) -> None:
+    """Codes [rows, ``columns`` rounded up to 128] (8 bits) and scales [runs of 128 columns, ``lds``] of the rows ``x``, to these addresses.  ``routing`` =
     (offsets, order, top): one row of codes for each pair sorted by expert, made of row order[s] // top of ``x`` (none behind the last expert's)."""
-    _on_current_device(x, "x"), _rows_of(x, "x")
-    _need(codes, "codes", torch.float8_e4m3fn), _need(scales, "scales", torch.float32)
-    offsets, order, top = routing if routing is not None else (None, None, 1)
-    rows, k = x.shape[0] if order is None else order.numel(), x.shape[1]
-    if codes.shape != (rows, -(-k // 128) * 128) or scales.dim() != 2 or scales.shape[0] != -(-k // 128) or scales.shape[1] < rows:
-        raise KernelError("quantize_rows: shapes do not fit")
-    _check("quantize_rows", lib().tib_quantize_rows(_ptr(x), _code(x.dtype), x.stride(0), _ptr(codes), codes.stride(0), _ptr(scales),
-                                                    scales.shape[1], rows, k, _ptr(order), top, 0 if offsets is None else _ptr(offsets[-1:]), _stream()))
+    _rows_here(x, columns, "quantize_rows")
+    rows, order, top, end = x.shape[0], 0, 1, 0
+    if routing is not None:
+        rows, order, top, end = routing[1].numel(), routing[1].data_ptr(), routing[2], routing[0].data_ptr() + 4 * (routing[0].numel() - 1)
+    _check("quantize_rows", lib().tib_quantize_rows(x.data_ptr(), _code(x.dtype), x.stride(0), codes, -(-columns // 128) * 128, scales, lds, rows, columns,
+                                                    order, top, end, _stream()))
 
 
 def block_scaled_pairs_of_sms(rows: int, features: int) -> bool:
-    """Whether a product of codes runs on pairs of SMs, in tiles of 256 rows x 256 features."""
-    return -(-rows // 256) * -(-features // 256) >= 24
+    """Whether a product of codes runs on pairs of SMs, in tiles of 256 rows x 256 features: where tiles of 128 x 128 would be more than one for each of
+    148 SMs.  (us, tiles of 128 / pairs: 4,096 -> 4,096 512 rows 22.9 / 22.8, 768 rows 39 / 24; 4,096 -> 6,144 384 rows 23.1 / 25.2, 512 rows 39 / 26;
+    14,336 -> 4,096 512 rows 62 / 60, 768 rows 110 / 62.)  Up to 128 rows the weights are the work: 4,096 -> 28,672 128 rows 38 / 42, 64 rows 29 / 39, 192
+    rows 69 / 42."""
+    return rows > 128 and -(-rows // 128) * -(-features // 128) > 148
 
 
-def block_scaled_product(x: torch.Tensor, scales: torch.Tensor | None, w: torch.Tensor, w_scales: torch.Tensor, y: torch.Tensor, *,
-                         features: int, columns: int, paired: bool = False, act: str = "none", limit: float = 0.0, alpha: float = 1.0,
-                         routing: tuple[torch.Tensor, torch.Tensor, int, bool] | None = None, row_scale: torch.Tensor | None = None,
-                         error_word: torch.Tensor | None = None) -> torch.Tensor:
-    """Rows times matrices of codes.  ``x``: codes with their ``scales`` as :func:`quantize_rows` leaves them, or (``scales`` None) rows that the
-    product's kernel quantises itself; ``w``: blocks [experts, blocks of features, runs, 128, 128], ``w_scales`` [experts, rows of scales, runs]
-    (``paired``: of (gate, up) row pairs); ``features`` x ``columns`` of a matrix count.  ``routing`` = (offsets, order, top, x_by_pair) sorts the rows of ``y`` by expert as in
-    :func:`moe_expert_product`; without it there is one matrix and row m of ``y`` is that of row m."""
-    _on_current_device(x, "x"), _rows_of(x, "x"), _rows_of(y, "y"), _need(w, "w", torch.float8_e4m3fn), _need(w_scales, "w_scales", torch.float32)
-    experts, n, runs = w.shape[0], features, -(-columns // 128)
-    offsets, order, top, x_by_pair = routing if routing is not None else (None, None, 1, False)
-    if scales is not None:
-        _need(x, "x", torch.float8_e4m3fn), _need(scales, "scales", torch.float32)
-    if (w.shape[1:] != (-(-n // 128), runs, 128, 128) or x.shape[1] != (columns if scales is None else runs * 128) or w_scales.shape[0] != experts
-            or w_scales.shape[2] != runs or y.shape[1] != (n // 2 if act in MOE_GATED else n) or (routing is None and y.shape[0] != x.shape[0])):
-        raise KernelError("block_scaled_product: shapes do not fit")
-    if scales is not None and routing is None and act in ("none", "swiglu") and block_scaled_pairs_of_sms(y.shape[0], n):
+def block_scaled_product(x: torch.Tensor, codes: tuple[int, int, int] | None, blocks, columns: int, y: torch.Tensor, *, act: str = "none", limit: float = 0.0,
+                         alpha: float = 1.0, routing: tuple[torch.Tensor, torch.Tensor, int, bool] | None = None,
+                         row_scale: torch.Tensor | None = None, error_word: torch.Tensor | None = None) -> torch.Tensor:
+    """The rows ``x`` times matrices of 8-bit blocks (a block_scaled.Blocks).  ``codes``: the addresses of the rows' codes and scales and the latter's
+    row length, as :func:`quantize_rows` left them (for rows sorted by expert: sorted); None: the product's kernel quantises the rows itself.  ``routing``
+    = (offsets, order, top, x_by_pair) sorts the rows of ``y`` by expert as in :func:`moe_expert_product`; without it row m of ``y`` is that of row m."""
+    _rows_here(x, columns, "block_scaled_product")
+    rows = y.shape[0]
+    if codes is not None and routing is None and act in ("none", "swiglu") and block_scaled_pairs_of_sms(rows, blocks.features):
         _check("block_scaled_product", lib().tib_block_scaled_2cta(
-            _ptr(x), _ptr(scales), scales.shape[1], _ptr(w), _ptr(w_scales), w_scales.shape[1], int(paired), int(act == "swiglu"), _ptr(y), _code(y.dtype),
-            y.stride(0), y.shape[0], n, columns, _ptr(error_word), _stream()))
+            codes[0], codes[1], codes[2], blocks.codes_at, blocks.scales_at, blocks.scale_rows, blocks.paired, act == "swiglu", y.data_ptr(), _code(y.dtype),
+            y.stride(0), rows, blocks.features, columns, _ptr(error_word), _stream()))
         return y
+    offsets = order = 0
+    top = experts = 1
+    x_by_pair = False
+    if routing is not None:
+        offsets, order, top, x_by_pair, experts = routing[0].data_ptr(), routing[1].data_ptr(), routing[2], routing[3] and codes is None, routing[0].numel() - 1
+    at, kind, ldx, x_scales, lds = (x.data_ptr(), _code(x.dtype), x.stride(0), 0, 0) if codes is None else (codes[0], -1, 0, codes[1], codes[2])
     _check("block_scaled_product", lib().tib_block_scaled_tcgen05(
-        _ptr(x), _code(x.dtype) if scales is None else -1, x.stride(0), x.shape[0], _ptr(scales), 0 if scales is None else scales.shape[1], _ptr(w),
-        _ptr(w_scales), w_scales.shape[1], int(paired), _ptr(y), _code(y.dtype), y.stride(0), y.shape[0], n, columns, _ptr(offsets), _ptr(order), experts,
-        top, int(x_by_pair), MOE_ACT[act], limit, alpha, _ptr(row_scale), _ptr(error_word), _stream()))
+        at, kind, ldx, x.shape[0] if codes is None else rows, x_scales, lds, blocks.codes_at, blocks.scales_at, blocks.scale_rows, blocks.paired, y.data_ptr(),
+        _code(y.dtype), y.stride(0), rows, blocks.features, columns, offsets, order, experts, top, x_by_pair, MOE_ACT[act], limit, alpha, _ptr(row_scale),
+        _ptr(error_word), _stream()))
     return y
 
 
