@@ -89,3 +89,30 @@ def check(got, value, out_dtype, what=""):
     off = (got.double() - want).abs()
     bad = ~(off <= bound)
     assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((off / bound.clamp(min=1e-300)).nan_to_num(9e9).max()):.2f} of the bound"
+
+
+def requantised64(value, bf16=True):
+    """Rows known within a bound, as a product reads them: (the widened codes of the value, how far those of the true rows may be off).  Rounding is
+    monotonic for a given scale; the run's scale may be that of the largest number less or plus its bound, too."""
+    h, e = value
+    if bf16:
+        e = e + 2.0 ** -8 * (h.abs() + e)
+    want = widened_rows64(h)
+    lo, hi = (h.abs() - e).clamp(min=0), h.abs() + e
+    off = torch.zeros_like(h)
+    for scales in (rows64(lo)[1], rows64(hi)[1], rows64(h)[1]):
+        s = scales[:, torch.arange(h.shape[1], device=h.device) // BLOCK]
+        for v in (h - e, h, h + e):
+            # (a run's largest as it is for this scale, so that the codes are made with it)
+            c = (v / s).clamp(-448, 448)
+            step = 2.0 ** (torch.floor(torch.log2(c.abs().clamp(min=2.0 ** -6))) - 3)
+            off = torch.maximum(off, (torch.round(c / step) * step * s - want).abs())
+    return want, off
+
+
+def product_of_known64(known, matrix):
+    """A product of rows of :func:`requantised64`."""
+    rows, off = known
+    w = matrix64(matrix)
+    runs = -(-rows.shape[1] // BLOCK)
+    return rows @ w.t(), off @ w.abs().t() + (BLOCK + 2 * runs + 2) * 2.0 ** -23 * ((rows.abs() + off) @ w.abs().t())

@@ -102,3 +102,103 @@ def test_the_oracle_rounds_as_e4m3_does():
     v = torch.cat([v, torch.full((len(v), 1), 448.0)], 1)                      # (so that every run's scale is 1)
     c, s = rows64(v)
     assert (s == 1).all() and torch.equal(c.float(), v.to(CODES).float())
+
+
+# ------------------------------------------------------------------------------------------------ checkpoints
+FP8 = {"quant_method": "fp8", "fmt": "e4m3", "weight_block_size": [128, 128], "activation_scheme": "dynamic"}
+
+
+def test_quantization_config():
+    from torchinferno_b200.config.model_config import ConfigError
+    from torchinferno_b200.config.quantization import BlockQuantization
+    assert BlockQuantization.from_config({}) is None and BlockQuantization.from_config({"quantization_config": None}) is None
+    assert BlockQuantization.from_config({"quantization_config": {"quant_method": "other"}}) is None
+    q = BlockQuantization.from_config({"quantization_config": {**FP8, "modules_to_not_convert": ["lm_head", "layers.1.mlp", "o_proj"]}})
+    assert [q.converts(n) for n in ("lm_head.weight", "model.layers.1.mlp.up_proj.weight", "model.layers.11.mlp.up_proj.weight",
+                                    "model.layers.0.self_attn.o_proj.weight", "model.layers.0.self_attn.q_proj.weight")] == [False, False, True, False, True]
+    for bad in ("fp8", {"quant_method": "fp8"}, {**FP8, "weight_block_size": [64, 128]}, {**FP8, "fmt": "e5m2"}, {**FP8, "activation_scheme": "static"},
+                {**FP8, "modules_to_not_convert": "lm_head"}):
+        with pytest.raises(ConfigError):
+            BlockQuantization.from_config({"quantization_config": bad})
+
+
+def _folder(tmp_path, config, **changes):
+    """A random model folder with these tensors changed, and its tensors as they were."""
+    from safetensors.torch import load_file, save_file
+    from torchinferno_b200.weights.random_init import write_random_model
+    write_random_model(config, tmp_path, seed=0)
+    tensors = {k: v.clone() for k, v in load_file(str(tmp_path / "model.safetensors")).items()}      # (clones: the file is mapped)
+    save_file({**tensors, **changes}, str(tmp_path / "model.safetensors"))
+    return tensors
+
+
+def test_a_checkpoint_of_blocks_is_bound_in_blocks(tmp_path):
+    from conftest import TINY_B
+    from torchinferno_b200.kernels.gemm import LinearWeight
+    from torchinferno_b200.weights.loader import load_weights
+    from torchinferno_b200.weights.random_init import build_model
+    config = {**TINY_B, "quantization_config": {**FP8, "modules_to_not_convert": ["model.layers.2.self_attn"]}}
+    tensors = _folder(tmp_path, config)
+    model = build_model(config, dtype=torch.bfloat16, device="cpu")
+    report = load_weights(model, tmp_path)
+    assert report["stored_dtypes"] == ["bfloat16", "float8_e4m3fn"]
+    name = "model.layers.0.mlp.down_proj.weight"
+    assert tensors[name].dtype == CODES and tensors[name + "_scale_inv"].shape == (2, 4)
+    block = model.blocks[0]
+    down = block.feed_forward.down_weight
+    assert isinstance(down, BlockScaledWeight) and torch.equal(flat(down.parts[0][1].codes[0], 192), tensors[name].view(torch.uint8))
+    assert isinstance(block.mixer.qkv_weight, BlockScaledWeight) and isinstance(block.feed_forward.gate_up_weight, BlockScaledWeight)
+    assert isinstance(model.blocks[2].mixer.qkv_weight, LinearWeight) and isinstance(model.blocks[2].feed_forward.down_weight, BlockScaledWeight)
+    assert model.embedding.dtype == torch.bfloat16
+    # the block is not one for the native call, and its bytes count once each
+    from torchinferno_b200.kernels import native_block
+    assert native_block.block_weights(block) is None
+    plain = build_model(TINY_B, dtype=torch.bfloat16, device="cpu")
+    from torchinferno_b200.weights.random_init import init_random_weights
+    init_random_weights(plain, 0)
+    assert model.weight_bytes() < plain.weight_bytes()
+    # in 32 bits the numbers they stand for
+    wide = build_model(config, dtype=torch.float32, device="cpu")
+    load_weights(wide, tmp_path)
+    want = BlockScaledMatrix(tensors[name], tensors[name + "_scale_inv"]).widened()
+    assert torch.equal(wide.blocks[0].feed_forward.down_weight.tensor, want)
+
+
+@pytest.mark.parametrize("name, tensor, message", [
+    ("model.layers.0.mlp.up_proj.weight_scale_inv", torch.ones(3, 2), "a scale for each 128 x 128"),
+    ("model.layers.0.mlp.up_proj.weight", torch.zeros(512, 192), "not stored as e4m3"),
+    ("model.layers.0.mlp.up_proj.weight", torch.zeros(512, 191, dtype=torch.uint8).view(CODES), "up_proj.weight: file"),
+    ("model.norm.weight_scale_inv", torch.ones(1, 1), "unexpected")])
+def test_checkpoints_that_do_not_fit_are_refused(tmp_path, name, tensor, message):
+    from conftest import TINY_B
+    from torchinferno_b200.weights.loader import WeightError, load_weights
+    from torchinferno_b200.weights.random_init import build_model
+    config = {**TINY_B, "quantization_config": FP8}
+    _folder(tmp_path, config, **{name: tensor})
+    with pytest.raises(WeightError, match=message):
+        load_weights(build_model(config, dtype=torch.bfloat16, device="cpu"), tmp_path)
+
+
+def test_fused_projections_are_stored_alike(tmp_path):
+    from conftest import TINY_B
+    from torchinferno_b200.weights.loader import load_weights
+    from torchinferno_b200.weights.random_init import build_model
+    config = {**TINY_B, "quantization_config": {**FP8, "modules_to_not_convert": ["k_proj"]}}
+    _folder(tmp_path, config)
+    with pytest.raises(ValueError, match="all be stored in 8-bit blocks, or none"):
+        load_weights(build_model(config, dtype=torch.bfloat16, device="cpu"), tmp_path)
+
+
+def test_experts_are_bound_in_blocks():
+    """Every design with routed experts takes them in blocks; gated ones as row pairs, the router never."""
+    from giforax_configs import GA
+    from torchinferno_b200.kernels.block_scaled import BlockScaledExperts
+    from torchinferno_b200.weights.random_init import build_model, init_random_weights
+    config = {**GA, "quantization_config": FP8}
+    model = build_model(config, dtype=torch.bfloat16, device="cpu")
+    init_random_weights(model, 1, config=config)
+    moes = [b.feed_forward for b in model.blocks if type(b.feed_forward).__name__ == "RoutedExperts"]
+    assert moes
+    for moe in moes:
+        assert isinstance(moe.up_weight, BlockScaledExperts) and moe.up_weight.paired == moe.glu and moe.up_weight.experts == moe.experts
+        assert isinstance(moe.down_weight, BlockScaledExperts) and moe.router_weight.dtype == torch.float32

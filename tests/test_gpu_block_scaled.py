@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from block_scaled_oracle import act64, check, gated64, matrix64, product64, random_matrix, rows64, widened_rows64
+from block_scaled_oracle import act64, check, gated64, matrix64, product64, product_of_known64, random_matrix, requantised64, rows64, widened_rows64
 from gpu_common import need_gpu
 from torchinferno_b200.kernels import gemm, ops
 from torchinferno_b200.kernels.block_scaled import BlockScaledExperts, BlockScaledMatrix, BlockScaledWeight, quantize_rows
@@ -316,3 +316,150 @@ def test_the_definition_by_itself():
     assert torch.equal(m.widened(torch.float32).double(), matrix64(m).float().double())
     codes, scales = quantize_rows(x)
     assert torch.equal(widened_rows64(x), codes.double() * scales.double().repeat_interleave(128, 1)[:, :200])
+
+
+# ------------------------------------------------------------------------------------------------ as the engine uses them
+FP8 = {"quant_method": "fp8", "weight_block_size": [128, 128]}
+
+
+@pytest.mark.parametrize("tokens", [1, 8, 40, 300])
+def test_a_feed_forward_in_blocks(tokens):
+    """Both products behind one another; the activation between them is known up to its own rounding, and so are its codes."""
+    need_gpu()
+    from torchinferno_b200.parts.base import PartSpec, build_part
+    hidden, inter = 320, 450
+    part = build_part("feed_forward", PartSpec("swiglu", {"hidden_size": hidden, "intermediate_size": inter}), dtype=BF16, device=torch.device(DEV))
+    gate, up, down = random_matrix(inter, hidden, 1, DEV, (0.005, 0.1)), random_matrix(inter, hidden, 2, DEV, (0.005, 0.1)), random_matrix(hidden, inter, 3, DEV)
+    part.bind(dict(zip(part.names, (gate, up, down))))
+    x = rows(tokens, hidden, tokens, spread=0.5)
+    act = gated64(product64(x, gate), product64(x, up))
+    check(part.forward(x, None), product_of_known64(requantised64(act), down), BF16)
+
+
+@pytest.mark.parametrize("activation, on_input", [("relu2", False), ("swiglu", False), ("glu_clamp", True), ("gelu", False)])
+@pytest.mark.parametrize("tokens", [1, 7, 90, 400])
+def test_routed_experts_in_blocks(tokens, activation, on_input):
+    need_gpu()
+    from torchinferno_b200.parts.base import PartSpec, build_part
+    hidden, inter, experts, top, limit = 200, 140, 6, 2, 2.0
+    part = build_part("feed_forward", PartSpec("routed_experts", {
+        "hidden_size": hidden, "experts": experts, "top": top, "expert_size": inter, "activation": activation, "weight_on_input": on_input,
+        "limit": limit}), dtype=BF16, device=torch.device(DEV))
+    weights = {spec.name: random_matrix(*spec.shape, i, DEV, (0.005, 0.15) if spec.shape[0] == inter else (0.02, 3.0)) if spec.block_scaled else
+               torch.randn(spec.shape, generator=torch.Generator().manual_seed(i)).to(DEV) * 0.1 for i, spec in enumerate(part.weight_specs())}
+    part.bind(weights)
+    x = rows(tokens, hidden, tokens, spread=0.5)
+    logits = torch.empty(tokens, experts, device=DEV)
+    ops.router_logits(x, part.router_weight, logits)
+    ids, shares = torch.empty(tokens, top, dtype=torch.int32, device=DEV), torch.empty(tokens, top, device=DEV)
+    ops.moe_route(logits, experts, top, ids, shares, normalize=True)
+    want, bound = torch.zeros(tokens, hidden, dtype=torch.float64, device=DEV), torch.zeros(tokens, hidden, dtype=torch.float64, device=DEV)
+    for e in range(experts):
+        at, choice = (ids == e).nonzero(as_tuple=True)
+        if len(at) == 0:
+            continue
+        share = shares[at, choice].double()[:, None]
+        sums = [product64(x[at], weights[f"e{e}.{n}"]) for n in (("gate", "up") if part.glu else ("up",))]
+        if on_input:
+            sums = [(v * share, b * share + 2.0 ** -23 * (v * share).abs()) for v, b in sums]
+        act = gated64(*sums, act=activation, limit=limit) if part.glu else act64(sums[0], activation)
+        y, b = product_of_known64(requantised64(act), weights[f"e{e}.down"])
+        share = torch.ones_like(share) if on_input else share
+        want[at] += share * y
+        # (the products with the shares and the sum over the choices: one rounding each)
+        bound[at] += share * b + 2 * top * 2.0 ** -23 * (share * y).abs()
+    check(part.forward(x, None), (want, bound), BF16)
+
+
+def _blocks_folder(tmp_path, config, seed):
+    from torchinferno_b200.weights.random_init import write_random_model
+    return write_random_model({**config, "quantization_config": FP8}, tmp_path, seed)
+
+
+def _engine(folder, dtype, **options):
+    from torchinferno_b200.config.engine_config import EngineConfig
+    from torchinferno_b200.engine.engine import InferenceEngine
+    return InferenceEngine.from_config(EngineConfig(model=str(folder), dtype=dtype, **options))
+
+
+def _generate(engine, prompts, tokens):
+    from torchinferno_b200.engine.types import GenerateRequest, SamplingConfig
+    return [list(o.token_ids) for o in engine.generate_many([GenerateRequest(f"g{i}", prompt_token_ids=p, sampling=SamplingConfig(tokens))
+                                                             for i, p in enumerate(prompts)])]
+
+
+@pytest.mark.parametrize("name", ["B", "D"])
+def test_a_model_in_blocks(tmp_path, name):
+    """In float32 the engine gives the tokens of the numbers the blocks stand for; in bfloat16 every decode step is captured, gives the same tokens as
+    uncaptured ones and run ahead or not, and its logits point where the float32 engine's do."""
+    need_gpu()
+    import numpy as np
+    import plain_llama
+    from conftest import TINY
+    from gpu_common import requests_for
+    from replay_util import InProcessReplayer, gather, trace_tail_decode
+    config, seed = TINY[name]
+    folder = _blocks_folder(tmp_path, config, seed)
+    cfg, stored = plain_llama.read_model_folder(folder)
+    widened = {n: w if n + "_scale_inv" not in stored else
+               w * stored[n + "_scale_inv"].repeat_interleave(128, 0)[:w.shape[0]].repeat_interleave(128, 1)[:, :w.shape[1]]
+               for n, w in stored.items() if not n.endswith("_scale_inv")}
+    # (the engine's float32 weights are the products of code and scale rounded to 24 bits)
+    widened = {n: w.float().double() for n, w in widened.items()}
+    wanted = requests_for(config, seed, [9, 21, 3, 14])
+    prompts = list(wanted.values())
+    with _engine(folder, "float32", page_size=16, max_batch_size=4) as engine:
+        assert _generate(engine, prompts, 8) == [plain_llama.generate_greedy(cfg, widened, p, 8) for p in prompts]
+    outs = []
+    for ahead in (True, False):
+        with _engine(folder, "bfloat16", page_size=16, max_batch_size=4, async_scheduling=ahead) as engine:
+            outs.append(_generate(engine, prompts, 12))
+            assert engine.runner.counters["graph_steps"] > 0
+    assert outs[0] == outs[1]
+    rows_by_dtype = {}
+    for dtype in ("float32", "bfloat16"):
+        steps, index = trace_tail_decode(wanted, 3)
+        rows_by_dtype[dtype] = gather(InProcessReplayer(folder, dtype, 512).run(steps), index)
+    # A product's terms are off by at most half a step of e4m3 (2^-4), by 2^-4 / sqrt(3) = 0.036 in the mean, and so is the product, its terms' errors
+    # being independent.  A layer adds to the residual what four products behind one another make: gate, up and down 0.036 sqrt(3) x 1.5 (the
+    # activation's slope) = 0.09, projections in and out of attention 0.05 twice over for the softmax = 0.1; three layers: 0.14 sqrt(3) = 0.24 of the
+    # logits at the most, a cosine of 1 - 0.24^2 / 2 = 0.97.
+    pairs = [tuple(np.asarray(rows_by_dtype[d][k][0], dtype=np.float64) for d in ("float32", "bfloat16")) for k in rows_by_dtype["float32"]]
+    assert len(pairs) == 4 * 4 - 1      # (one prompt is shorter than its decoded tail)
+    cosines = [float((a * b).sum() / np.sqrt((a * a).sum() * (b * b).sum())) for a, b in pairs]
+    assert min(cosines) >= 0.97, min(cosines)
+
+
+@pytest.mark.parametrize("module, name", [("giforax_configs", "GA"), ("vofidra_configs", "VA"), ("zipedra_configs", "ZA"), ("tadalorn_configs", "TB")])
+def test_designs_with_experts_in_blocks(tmp_path, module, name):
+    """Their experts are bound in blocks and a random model generates: prompts in portions beside decode steps, the same tokens twice."""
+    need_gpu()
+    import importlib
+    config, seed = importlib.import_module(module).CONFIGS[name]
+    folder = _blocks_folder(tmp_path, config, seed)
+    vocab = config["vocab"]
+    g = torch.Generator().manual_seed(seed)
+    prompts = [torch.randint(0, vocab, (n,), generator=g).tolist() for n in (11, 30, 2)]
+    outs = []
+    for _ in range(2):
+        with _engine(folder, "bfloat16", page_size=16, max_batch_size=4, prefill_chunk_size=16) as engine:
+            assert any(type(getattr(b.feed_forward, "up_weight", None)).__name__ == "BlockScaledExperts" for b in engine.runner.model.blocks
+                       if getattr(b, "feed_forward", None) is not None)
+            outs.append(_generate(engine, prompts, 6))
+    assert outs[0] == outs[1] and all(len(o) == 6 for o in outs[0])
+
+
+def test_command_line_with_a_model_in_blocks(tmp_path):
+    need_gpu()
+    import json
+    import subprocess
+    import sys
+    from pathlib import Path
+    from conftest import TINY_D
+    root = Path(__file__).resolve().parent.parent
+    (tmp_path / "config.json").write_text(json.dumps({**TINY_D, "quantization_config": FP8}))
+    run = [sys.executable, "-m", "torchinferno_b200"]
+    subprocess.run([*run, "random-model", str(tmp_path / "config.json"), str(tmp_path / "model"), "--seed", "3"], check=True, cwd=root, timeout=300)
+    out = subprocess.run([*run, "generate", str(tmp_path / "model"), "--input-ids", "1", "2", "3", "--new-tokens", "4"], check=True, cwd=root, timeout=300,
+                         capture_output=True, text=True).stdout
+    assert out.strip()

@@ -56,7 +56,7 @@ def random_model(config: Mapping[str, Any], seed: int, *, dtype: str | torch.dty
     """Build the model ``config`` names with seeded random weights made on the device."""
     device = require_cuda(device)
     model = build_model(config, dtype=parse_dtype(dtype, config), device=device)
-    init_random_weights(model, seed)
+    init_random_weights(model, seed, config=config)
     return model
 
 

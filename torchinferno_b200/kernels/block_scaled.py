@@ -183,6 +183,9 @@ class BlockScaledWeight:
     def device(self) -> torch.device:
         return self.parts[0][1].codes.device
 
+    def address(self) -> int:
+        return self.parts[0][1].codes_at
+
     def nbytes(self) -> int:
         return sum(part.codes.numel() + 4 * part.scales.numel() for _, part in self.parts)
 
@@ -254,6 +257,9 @@ class BlockScaledExperts:
     @property
     def device(self) -> torch.device:
         return self.blocks.codes.device
+
+    def address(self) -> int:
+        return self.blocks.codes_at
 
     def nbytes(self) -> int:
         return self.blocks.codes.numel() + 4 * self.blocks.scales.numel()

@@ -14,7 +14,7 @@ import weakref
 import torch
 
 from torchinferno_b200.kernels import ops
-from torchinferno_b200.kernels.block_scaled import BlockScaledWeight
+from torchinferno_b200.kernels.block_scaled import BlockScaledExperts, BlockScaledMatrix, BlockScaledWeight
 
 # Which kernel multiplies bf16 operands:
 #   "auto"     whichever is faster on this GPU.  Many rows go to cuBLAS.  At few rows (decode steps) neither the
@@ -129,6 +129,41 @@ class LinearWeight:
 
     def nbytes(self) -> int:
         return self.tensor.numel() * self.tensor.element_size()
+
+
+def _block_scaled(matrices: "tuple[torch.Tensor | BlockScaledMatrix, ...]") -> bool:
+    """Whether matrices that make one product are 8-bit blocks: all of them or none."""
+    kinds = {isinstance(m, BlockScaledMatrix) for m in matrices}
+    if len(kinds) != 1:
+        raise ValueError("matrices that run as one product must all be stored in 8-bit blocks, or none of them")
+    return kinds.pop()
+
+
+def projection(*matrices: "torch.Tensor | BlockScaledMatrix") -> "LinearWeight | BlockScaledWeight":
+    """The weight of a part's projection from its checkpoint matrices [out, in], whose outputs lie side by side.  (Which kernel takes the products of few
+    rows is measured per shape once the whole model is bound.)"""
+    if _block_scaled(matrices):
+        return BlockScaledWeight(*matrices)
+    return LinearWeight(matrices[0] if len(matrices) == 1 else torch.cat(matrices, dim=0), few_rows_tcgen05=None)
+
+
+def row_pairs(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
+    """Row 2i = gate i, row 2i + 1 = up i."""
+    return torch.stack([gate, up], dim=1).reshape(2 * gate.shape[0], gate.shape[1])
+
+
+def gated_projection(gate: "torch.Tensor | BlockScaledMatrix", up: "torch.Tensor | BlockScaledMatrix", *, epilogue: str = "swiglu") -> "LinearWeight | BlockScaledWeight":
+    """The same of a gate and an up matrix, as (gate i, up i) row pairs.  ``epilogue="none"``: the pairs' activation is the caller's."""
+    if _block_scaled((gate, up)):
+        return BlockScaledWeight(gate, up, epilogue="swiglu")
+    return LinearWeight(row_pairs(gate, up), few_rows_tcgen05=None, epilogue=epilogue)
+
+
+def expert_matrices(matrices: "list[torch.Tensor | BlockScaledMatrix]", ups: "list[torch.Tensor | BlockScaledMatrix] | None" = None) -> "torch.Tensor | BlockScaledExperts":
+    """One product's matrices of all experts (of gated ones: ``matrices`` the gates), as :func:`ops.moe_expert_product` takes them."""
+    if _block_scaled((*matrices, *(ups or ()))):
+        return BlockScaledExperts(matrices, ups)
+    return torch.stack(matrices if ups is None else [row_pairs(g, u) for g, u in zip(matrices, ups)]).contiguous()
 
 
 def linear(x: torch.Tensor, weight: "torch.Tensor | LinearWeight | BlockScaledWeight", *, out_dtype: torch.dtype | None = None,

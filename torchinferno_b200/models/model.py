@@ -13,6 +13,7 @@ from typing import Mapping
 import torch
 
 from torchinferno_b200.kernels import gemm, ops
+from torchinferno_b200.kernels.block_scaled import BlockScaledExperts, BlockScaledWeight
 from torchinferno_b200.kernels.gemm import linear
 from torchinferno_b200.models.spec import ModelSpec, StageCall
 from torchinferno_b200.parts.base import (Block, CacheSpec, KVBinding, LayerContext, ResidualStream,
@@ -57,7 +58,7 @@ class CausalLM:
         for prefix, part in self._owned_parts():
             for ws in part.weight_specs():
                 name = prefix + ws.name
-                expected[name] = WeightSpec(name, ws.shape, ws.init, ws.std, ws.role, ws.optional, ws.free_dims)
+                expected[name] = WeightSpec(name, ws.shape, ws.init, ws.std, ws.role, ws.optional, ws.free_dims, ws.block_scaled)
             for ws in part.shared_weight_specs():
                 if ws.name in expected and tuple(expected[ws.name].shape) != tuple(ws.shape):
                     raise ValueError(f"{ws.name}: parts that share it declare shapes {expected[ws.name].shape} and {ws.shape}")
@@ -113,7 +114,10 @@ class CausalLM:
         for _, part in self._owned_parts():
             for key, value in vars(part).items():
                 if key.endswith("weight"):
-                    note(getattr(value, "tensor", value) if not isinstance(value, torch.Tensor) else value)
+                    if isinstance(value, (BlockScaledWeight, BlockScaledExperts)):
+                        seen[value.address()] = value.nbytes()
+                    else:
+                        note(getattr(value, "tensor", value) if not isinstance(value, torch.Tensor) else value)
         return sum(seen.values())
 
     # -------------------------------------------------------------- needs

@@ -19,7 +19,8 @@ from typing import Mapping
 import torch
 
 from torchinferno_b200.kernels import attention as attention_kernels
-from torchinferno_b200.kernels.gemm import LinearWeight, linear
+from torchinferno_b200.kernels.block_scaled import BlockScaledWeight
+from torchinferno_b200.kernels.gemm import LinearWeight, linear, projection
 from torchinferno_b200.parts.base import (CacheSpec, LayerContext, Mixer, PartSpec, WeightSpec,
                                           build_part, register_part)
 
@@ -40,20 +41,18 @@ class GQAAttention(Mixer):
         if not isinstance(position, PartSpec):
             position = PartSpec(**position)
         self.position = build_part("position", position, dtype=dtype, device=device)
-        self.qkv_weight: LinearWeight | None = None
-        self.o_weight: LinearWeight | None = None
+        self.qkv_weight: LinearWeight | BlockScaledWeight | None = None
+        self.o_weight: LinearWeight | BlockScaledWeight | None = None
 
     def weight_specs(self) -> list[WeightSpec]:
         q, k, v, o = self.names
         qw, kw = self.heads * self.head_dim, self.kv_heads * self.head_dim
-        return [WeightSpec(q, (qw, self.hidden_size)), WeightSpec(k, (kw, self.hidden_size)),
-                WeightSpec(v, (kw, self.hidden_size)), WeightSpec(o, (self.hidden_size, qw))]
+        return [WeightSpec(name, shape, block_scaled=True) for name, shape in
+                ((q, (qw, self.hidden_size)), (k, (kw, self.hidden_size)), (v, (kw, self.hidden_size)), (o, (self.hidden_size, qw)))]
 
     def bind(self, weights: Mapping[str, torch.Tensor]) -> None:
         q, k, v, o = self.names
-        self.qkv_weight = LinearWeight(torch.cat([weights[q], weights[k], weights[v]], dim=0), few_rows_tcgen05=None)
-        # (which kernel takes the products of few rows is measured per shape once the whole model is bound)
-        self.o_weight = LinearWeight(weights[o], few_rows_tcgen05=None)
+        self.qkv_weight, self.o_weight = projection(weights[q], weights[k], weights[v]), projection(weights[o])
 
     def cache_spec(self) -> CacheSpec:
         return CacheSpec(self.kv_heads, self.head_dim, self.window)

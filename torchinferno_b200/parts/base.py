@@ -50,6 +50,8 @@ class WeightSpec:
     optional: bool = False     # may be absent from the file (then the part copes)
     free_dims: tuple[int, ...] = ()   # dimensions whose size the file decides (``shape`` holds what random weights get);
                                       # the part reads the size off the tensor it is bound to
+    block_scaled: bool = False        # may be stored as e4m3 codes with a 32-bit scale for each block of 128 x 128 (a tensor named
+                                      # name + "_scale_inv"); in bfloat16 the part is then bound to a kernels.block_scaled.BlockScaledMatrix
 
 
 @dataclass(frozen=True)

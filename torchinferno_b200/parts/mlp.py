@@ -15,7 +15,8 @@ from typing import Mapping
 import torch
 
 from torchinferno_b200.kernels import ops
-from torchinferno_b200.kernels.gemm import LinearWeight, linear, linear_swiglu
+from torchinferno_b200.kernels.block_scaled import BlockScaledWeight
+from torchinferno_b200.kernels.gemm import LinearWeight, gated_projection, linear, linear_swiglu, projection
 from torchinferno_b200.parts.base import FeedForward, LayerContext, WeightSpec, register_part
 
 
@@ -26,20 +27,18 @@ class SwiGLUFeedForward(FeedForward):
         super().__init__(dtype=dtype, device=device)
         self.hidden_size, self.intermediate_size = hidden_size, intermediate_size
         self.names = (gate_name, up_name, down_name)
-        self.gate_up_weight: LinearWeight | None = None
-        self.down_weight: LinearWeight | None = None
+        self.gate_up_weight: LinearWeight | BlockScaledWeight | None = None
+        self.down_weight: LinearWeight | BlockScaledWeight | None = None
 
     def weight_specs(self) -> list[WeightSpec]:
         g, u, d = self.names
-        return [WeightSpec(g, (self.intermediate_size, self.hidden_size)),
-                WeightSpec(u, (self.intermediate_size, self.hidden_size)),
-                WeightSpec(d, (self.hidden_size, self.intermediate_size))]
+        return [WeightSpec(g, (self.intermediate_size, self.hidden_size), block_scaled=True),
+                WeightSpec(u, (self.intermediate_size, self.hidden_size), block_scaled=True),
+                WeightSpec(d, (self.hidden_size, self.intermediate_size), block_scaled=True)]
 
     def bind(self, weights: Mapping[str, torch.Tensor]) -> None:
         g, u, d = self.names
-        pairs = torch.stack([weights[g], weights[u]], dim=1).reshape(2 * self.intermediate_size, self.hidden_size)
-        self.gate_up_weight = LinearWeight(pairs, few_rows_tcgen05=None, epilogue="swiglu")
-        self.down_weight = LinearWeight(weights[d], few_rows_tcgen05=None)
+        self.gate_up_weight, self.down_weight = gated_projection(weights[g], weights[u]), projection(weights[d])
 
     def forward(self, x: torch.Tensor, ctx: LayerContext) -> torch.Tensor:
         return linear(linear_swiglu(x, self.gate_up_weight), self.down_weight)
@@ -58,18 +57,17 @@ class DenseFeedForward(FeedForward):
             raise ValueError(f"unknown activation {activation!r}; known: ['relu2']")
         self.hidden_size, self.intermediate_size, self.activation = hidden_size, intermediate_size, activation
         self.names = (up_name, down_name)
-        self.up_weight: LinearWeight | None = None
-        self.down_weight: LinearWeight | None = None
+        self.up_weight: LinearWeight | BlockScaledWeight | None = None
+        self.down_weight: LinearWeight | BlockScaledWeight | None = None
 
     def weight_specs(self) -> list[WeightSpec]:
         u, d = self.names
-        return [WeightSpec(u, (self.intermediate_size, self.hidden_size), std=self.hidden_size ** -0.5),
-                WeightSpec(d, (self.hidden_size, self.intermediate_size), std=self.intermediate_size ** -0.5)]
+        return [WeightSpec(u, (self.intermediate_size, self.hidden_size), std=self.hidden_size ** -0.5, block_scaled=True),
+                WeightSpec(d, (self.hidden_size, self.intermediate_size), std=self.intermediate_size ** -0.5, block_scaled=True)]
 
     def bind(self, weights: Mapping[str, torch.Tensor]) -> None:
         u, d = self.names
-        self.up_weight = LinearWeight(weights[u], few_rows_tcgen05=None)
-        self.down_weight = LinearWeight(weights[d], few_rows_tcgen05=None)
+        self.up_weight, self.down_weight = projection(weights[u]), projection(weights[d])
 
     def forward(self, x: torch.Tensor, ctx: LayerContext) -> torch.Tensor:
         hidden = linear(x, self.up_weight)

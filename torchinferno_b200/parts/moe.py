@@ -34,7 +34,7 @@ from typing import Mapping
 import torch
 
 from torchinferno_b200.kernels import ops
-from torchinferno_b200.kernels.gemm import LinearWeight, linear
+from torchinferno_b200.kernels.gemm import expert_matrices, gated_projection, linear, projection
 from torchinferno_b200.parts.base import FeedForward, LayerContext, WeightSpec, register_part
 
 
@@ -88,14 +88,14 @@ class RoutedExperts(FeedForward):
             specs.append(WeightSpec(self.correction_name, (self.routed,), std=0.05, role="vector"))
         for e in range(self.experts):
             if self.glu:
-                specs.append(WeightSpec(self._expert(e, "gate"), (self.expert_size, self.hidden_size), std=std))
-            specs += [WeightSpec(self._expert(e, "up"), (self.expert_size, self.hidden_size), std=std),
-                      WeightSpec(self._expert(e, "down"), (self.hidden_size, self.expert_size), std=self.expert_size ** -0.5)]
+                specs.append(WeightSpec(self._expert(e, "gate"), (self.expert_size, self.hidden_size), std=std, block_scaled=True))
+            specs += [WeightSpec(self._expert(e, "up"), (self.expert_size, self.hidden_size), std=std, block_scaled=True),
+                      WeightSpec(self._expert(e, "down"), (self.hidden_size, self.expert_size), std=self.expert_size ** -0.5, block_scaled=True)]
         if self.shared_size:
             if self.glu:
-                specs.append(WeightSpec(shared + self.gate_name, (self.shared_size, self.hidden_size), std=std))
-            specs += [WeightSpec(shared + up, (self.shared_size, self.hidden_size), std=std),
-                      WeightSpec(shared + down, (self.hidden_size, self.shared_size), std=self.shared_size ** -0.5)]
+                specs.append(WeightSpec(shared + self.gate_name, (self.shared_size, self.hidden_size), std=std, block_scaled=True))
+            specs += [WeightSpec(shared + up, (self.shared_size, self.hidden_size), std=std, block_scaled=True),
+                      WeightSpec(shared + down, (self.hidden_size, self.shared_size), std=self.shared_size ** -0.5, block_scaled=True)]
             if self.shared_gate:
                 specs.append(WeightSpec(shared + gate, (1, self.hidden_size), std=std))
         return specs
@@ -109,19 +109,16 @@ class RoutedExperts(FeedForward):
             self.router_bias = torch.cat([bias, bias.new_zeros(len(self.router_weight) - self.routed)]).contiguous()      # (none on a gate row)
         if self.has_correction:
             self.correction = weights[self.correction_name].to(torch.float32).contiguous()
-        def first(name_of) -> torch.Tensor:
-            """The first product's matrix: up, or (gate i, up i) row pairs for the gated unit."""
-            if not self.glu:
-                return name_of("up")
-            g, u = name_of("gate"), name_of("up")
-            return torch.stack([g, u], dim=1).reshape(2 * g.shape[0], g.shape[1])
+        def of_all(which: str) -> list:
+            return [weights[self._expert(e, which)] for e in range(self.experts)]
 
-        self.up_weight = torch.stack([first(lambda which, e=e: weights[self._expert(e, which)]) for e in range(self.experts)]).contiguous()
-        self.down_weight = torch.stack([weights[self._expert(e, "down")] for e in range(self.experts)]).contiguous()
+        # the first product's matrices: up, or (gate i, up i) row pairs for the gated units
+        self.up_weight = expert_matrices(of_all("gate"), of_all("up")) if self.glu else expert_matrices(of_all("up"))
+        self.down_weight = expert_matrices(of_all("down"))
         if self.shared_size:
-            self.shared_up_weight = LinearWeight(first(lambda which: weights[shared + {"up": up, "gate": self.gate_name}[which]]),
-                                                 few_rows_tcgen05=None)
-            self.shared_down_weight = LinearWeight(weights[shared + down], few_rows_tcgen05=None)
+            self.shared_up_weight = gated_projection(weights[shared + self.gate_name], weights[shared + up], epilogue="none") if self.glu else \
+                projection(weights[shared + up])
+            self.shared_down_weight = projection(weights[shared + down])
 
     def forward(self, x: torch.Tensor, ctx: LayerContext) -> torch.Tensor:
         n, dev, top = x.shape[0], x.device, self.top

@@ -11,7 +11,10 @@ the wrong shape.
 Storage rule: a tensor stored in bfloat16 stays bfloat16 and one stored in
 32-bit stays 32-bit when the engine computes in bfloat16; norm vectors are
 widened to fp32 (lossless); integer tables become int32.  When the engine
-computes in float32 every floating tensor is widened to fp32.
+computes in float32 every floating tensor is widened to fp32.  A matrix that its
+part takes in 8-bit blocks (``WeightSpec.block_scaled``) and that is stored as e4m3
+codes with a tensor of scales beside it (its name and ``_scale_inv``) stays so in
+bfloat16, and is widened to the numbers it stands for in float32.
 """
 from __future__ import annotations
 
@@ -20,6 +23,9 @@ from pathlib import Path
 from typing import Iterable
 
 import torch
+
+from torchinferno_b200.config.quantization import SCALE_SUFFIX
+from torchinferno_b200.kernels.block_scaled import BlockScaledMatrix, blocks
 
 SINGLE_FILE = "model.safetensors"
 INDEX_FILE = "model.safetensors.index.json"
@@ -89,8 +95,10 @@ def load_weights(model, folder: str | Path) -> dict[str, object]:
 
     try:
         missing = [n for n, ws in expected.items() if n not in files and not ws.optional]
+        scales = {n + SCALE_SUFFIX: n for n, ws in expected.items() if ws.block_scaled and n in files}
+        in_blocks = {n for s, n in scales.items() if s in files}
         ignored = sorted(n for n in files if n not in expected and n.endswith(IGNORED_SUFFIXES))
-        unexpected = [n for n in files if n not in expected and n not in ignored]
+        unexpected = [n for n in files if n not in expected and n not in ignored and scales.get(n) not in in_blocks]
         # a head that the model ties to its embedding is not read even if the file stores a copy
         unused = set(model.unused_optional_tensors()) if hasattr(model, "unused_optional_tensors") else set()
         wrong: list[str] = []
@@ -102,6 +110,12 @@ def load_weights(model, folder: str | Path) -> dict[str, object]:
             free = getattr(ws, "free_dims", ())
             if len(shape) != len(ws.shape) or any(a != b for d, (a, b) in enumerate(zip(shape, ws.shape)) if d not in free):
                 wrong.append(f"{name}: file {list(shape)} vs model {list(ws.shape)}")
+            if name in in_blocks:
+                found = list(handle_of(files[name + SCALE_SUFFIX]).get_slice(name + SCALE_SUFFIX).get_shape())
+                if found != [blocks(d) for d in shape]:
+                    wrong.append(f"{name + SCALE_SUFFIX}: file {found} vs a scale for each 128 x 128 of {list(shape)}")
+                elif str(view.get_dtype()) != "F8_E4M3":
+                    wrong.append(f"{name}: has scales beside it but is not stored as e4m3 codes")
         if missing or unexpected or wrong:
             parts = [f"checkpoint {folder} does not fit the model ({model.spec.architecture}):"]
             if missing:
@@ -119,7 +133,11 @@ def load_weights(model, folder: str | Path) -> dict[str, object]:
                 continue
             tensor = handle_of(files[name]).get_tensor(name)
             stored[name] = str(tensor.dtype).replace("torch.", "")
-            tensors[name] = place(tensor, ws.role, model.dtype, model.device)
+            if name in in_blocks:
+                matrix = BlockScaledMatrix(tensor.contiguous(), handle_of(files[name + SCALE_SUFFIX]).get_tensor(name + SCALE_SUFFIX).to(torch.float32).contiguous())
+                tensors[name] = place_blocks(matrix, model.dtype, model.device)
+            else:
+                tensors[name] = place(tensor, ws.role, model.dtype, model.device)
     finally:
         for handle in handles.values():
             handle.__exit__(None, None, None)
@@ -127,6 +145,12 @@ def load_weights(model, folder: str | Path) -> dict[str, object]:
     model.bind(tensors, consume=True)      # (each part's source tensors are dropped as it binds them)
     return {"tensors": count, "stored_dtypes": sorted(set(stored.values())), "ignored": ignored,
             "not_read": sorted(unused & set(files))}
+
+
+def place_blocks(matrix: BlockScaledMatrix, compute_dtype: torch.dtype, device: torch.device) -> "BlockScaledMatrix | torch.Tensor":
+    """The same for a matrix in 8-bit blocks."""
+    matrix = matrix.to(device)
+    return matrix.widened(torch.float32) if compute_dtype == torch.float32 else matrix
 
 
 def place(tensor: torch.Tensor, role: str, compute_dtype: torch.dtype, device: torch.device) -> torch.Tensor:

@@ -6,6 +6,8 @@ tensor's values do not depend on which other tensors exist or on their order.
 The reference has no such mode; its tests build an eager model under
 ``torch.manual_seed`` and write it out to load it back
 (tests/test_model_variants.py:319-354 in the reference project).
+
+With ``quantization_config`` in config.json (config/quantization.py) the matrices it covers are quantised to 8-bit blocks.
 """
 from __future__ import annotations
 
@@ -16,8 +18,10 @@ from typing import Any, Mapping
 
 import torch
 
+from torchinferno_b200.config.quantization import SCALE_SUFFIX, BlockQuantization
 from torchinferno_b200.config.registry import resolve_architecture
-from torchinferno_b200.weights.loader import SINGLE_FILE, place
+from torchinferno_b200.kernels.block_scaled import quantize_matrix
+from torchinferno_b200.weights.loader import SINGLE_FILE, place, place_blocks
 
 
 def _tensor_seed(seed: int, name: str) -> int:
@@ -52,6 +56,11 @@ def build_model(config: Mapping[str, Any], *, dtype: torch.dtype, device: torch.
     return CausalLM(entry.build(typed), dtype=dtype, device=device)
 
 
+def _in_blocks(quantization: BlockQuantization | None, spec) -> bool:
+    """Whether config.json has this tensor stored in 8-bit blocks."""
+    return spec.block_scaled and quantization is not None and quantization.converts(spec.name)
+
+
 def write_random_model(config: Mapping[str, Any], folder: str | Path, seed: int,
                        dtype: torch.dtype = torch.bfloat16) -> Path:
     """Write ``config.json`` and ``model.safetensors`` with seeded random weights."""
@@ -61,21 +70,31 @@ def write_random_model(config: Mapping[str, Any], folder: str | Path, seed: int,
     config = dict(config)
     config["torch_dtype"] = str(dtype).replace("torch.", "")
     model = build_model(config, dtype=torch.float32, device="cpu")
+    quantization = BlockQuantization.from_config(config)
     tensors = {}
     for name, spec in model.expected_tensors().items():
         if spec.optional:
             continue  # e.g. a head tied to the embedding is not stored
+        if _in_blocks(quantization, spec):
+            matrix = quantize_matrix(random_tensor(spec, seed))
+            tensors[name], tensors[name + SCALE_SUFFIX] = matrix.codes, matrix.scales
+            continue
         tensors[name] = random_tensor(spec, seed, dtype=dtype).contiguous()
     (folder / "config.json").write_text(json.dumps(config, indent=1) + "\n")
     save_file(tensors, str(folder / SINGLE_FILE), metadata={"format": "pt", "seed": str(seed)})
     return folder
 
 
-def init_random_weights(model, seed: int, storage_dtype: torch.dtype = torch.bfloat16) -> None:
-    """Bind seeded random weights generated on the model's device (nothing touches the disk)."""
+def init_random_weights(model, seed: int, storage_dtype: torch.dtype = torch.bfloat16, config: Mapping[str, Any] | None = None) -> None:
+    """Bind seeded random weights generated on the model's device (nothing touches the disk).  ``config``: the config.json whose
+    ``quantization_config`` says which matrices are stored in 8-bit blocks (None: none)."""
+    quantization = None if config is None else BlockQuantization.from_config(config)
     tensors = {}
     for name, spec in model.expected_tensors().items():
         if spec.optional:
+            continue
+        if _in_blocks(quantization, spec):
+            tensors[name] = place_blocks(quantize_matrix(random_tensor(spec, seed, device=model.device)), model.dtype, model.device)
             continue
         raw = random_tensor(spec, seed, device=model.device, dtype=storage_dtype)
         tensors[name] = place(raw, spec.role, model.dtype, model.device)
