@@ -20,21 +20,14 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__
   const bool in = row < (order ? min(rows, *sorted) : rows) && run < runs;
   const int col = run * kBlk + eighth * 16, from = !in ? 0 : order ? order[row] / top : row;
   uint4 raw[sizeof(T)];
-  float v[16];
   bs_ask16<T, VEC>(x + (size_t)from * ldx + (in ? col : 0), in ? K - col : 0, raw);
-  bs_floats16<T>(raw, v);
-  uint32_t largest = 0;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) largest = max(largest, __float_as_uint(v[j]) & 0x7fffffffu);
+  uint32_t largest = bs_largest16<T>(raw);
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
   float scale, inverse;
   bs_run_scale(largest, scale, inverse);
   if (!in) return;
-  uint32_t w[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = bs_codes4(v[4 * j] * inverse, v[4 * j + 1] * inverse, v[4 * j + 2] * inverse, v[4 * j + 3] * inverse);
-  *reinterpret_cast<uint4*>(codes + (size_t)row * ldc + col) = make_uint4(w[0], w[1], w[2], w[3]);
+  *reinterpret_cast<uint4*>(codes + (size_t)row * ldc + col) = bs_codes16<T>(raw, inverse);
   if (eighth == 0) scales[(size_t)run * lds + row] = scale;
 }
 

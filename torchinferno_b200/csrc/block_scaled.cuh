@@ -75,6 +75,35 @@ template <typename T> __device__ __forceinline__ void bs_floats16(const uint4 (&
   }
 }
 
+// The bits of the largest absolute value of sixteen numbers: of bf16, two at a time by their halves of a word.
+template <typename T> __device__ __forceinline__ uint32_t bs_largest16(const uint4 (&raw)[sizeof(T)]) {
+  uint32_t w[4 * sizeof(T)];
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T); ++i) {
+    w[4 * i] = raw[i].x; w[4 * i + 1] = raw[i].y; w[4 * i + 2] = raw[i].z; w[4 * i + 3] = raw[i].w;
+  }
+  constexpr uint32_t kMask = sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu;
+#pragma unroll
+  for (int i = 0; i < 4 * (int)sizeof(T); ++i) w[i] &= kMask;
+#pragma unroll
+  for (int n = 2 * sizeof(T); n > 0; n >>= 1)
+#pragma unroll
+    for (int i = 0; i < n; ++i) w[i] = sizeof(T) == 2 ? __vmaxu2(w[i], w[i + n]) : max(w[i], w[i + n]);
+  return sizeof(T) == 2 ? max(w[0] << 16, w[0] & 0xffff0000u) : w[0];
+}
+// Sixteen codes of sixteen numbers times `inverse`.
+template <typename T> __device__ __forceinline__ uint4 bs_codes16(const uint4 (&raw)[sizeof(T)], float inverse) {
+  float v[16];
+  bs_floats16<T>(raw, v);
+  const f32x2 inverse2 = f2_pack(inverse, inverse);
+#pragma unroll
+  for (int j = 0; j < 16; j += 2) f2_unpack(f2_mul(f2_pack(v[j], v[j + 1]), inverse2), v[j], v[j + 1]);
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = bs_codes4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // Codes [rows, bytes a row], read in boxes of box_rows x 128 with 128-byte swizzle.
 static inline int bs_make_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t bytes, int box_rows) {
   EncodeTiledFn fn = encode_tiled_fn();

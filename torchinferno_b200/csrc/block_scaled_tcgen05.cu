@@ -501,21 +501,13 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int r = r0 + 4 * h + sub;
-            float v[16];
-            bs_floats16<TX>(now.raw[h], v);
-            uint32_t largest = 0;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) largest = max(largest, __float_as_uint(v[j]) & 0x7fffffffu);
+            uint32_t largest = bs_largest16<TX>(now.raw[h]);
 #pragma unroll
             for (int o = 1; o < 8; o <<= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
             float scale, inverse;
             bs_run_scale(largest, scale, inverse);
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              w[j] = bs_codes4(v[4 * j] * inverse, v[4 * j + 1] * inverse, v[4 * j + 2] * inverse, v[4 * j + 3] * inverse);
             if (r < m.rows) {
-              *reinterpret_cast<uint4*>(codes + r * kBlk + ((eighth ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4*>(codes + r * kBlk + ((eighth ^ (r & 7)) << 4)) = bs_codes16<TX>(now.raw[h], inverse);
               if (eighth == 0) {
                 scales[r] = scale * now.even;
                 scales[NT + 8 + r] = scale * now.odd;
@@ -571,6 +563,9 @@ static int launch_block_scaled(const CUtensorMap& map_w, const CUtensorMap& map_
   const int64_t steps = (int64_t)ceil_div(a.runs, splits) * ceil_div64(tiles * splits, grid);      // of a block, at most
   a.stages = 1;
   while (a.stages < kBsMaxStages && a.stages < steps && bs_smem<NT>(a.stages + 1, splits, experts) <= (kBlocks > 148 ? 113u * 1024 : (uint32_t)kMostSmem)) ++a.stages;
+  // (A wait by parity tells a stage's last use from the one before only while a helper's step before implies the latter is over: with no more helpers
+  // than stages, or every stage used once.)
+  if (!std::is_same_v<TX, uint8_t> && a.stages < BsShape<NT, false>::kHelpers && a.stages < steps) return TIB_E_SMEM;
   auto kern = block_scaled_tcgen05_kernel<NT, TX, TO>;
   static bool allowed[64];      // (by device: the attribute belongs to its context)
   int device = 0;
