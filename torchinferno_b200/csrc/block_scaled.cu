@@ -61,5 +61,38 @@ TIB_API int tib_quantize_rows(const void* x, int x_dtype, int64_t ldx, void* cod
   return TIB_OK;
 }
 
+// Whether a product of codes runs on pairs of SMs, in tiles of 256 rows x 256 features: where tiles of 128 x 128 would be more than one for each of 148 SMs.
+// (us, tiles of 128 / pairs: 4,096 -> 4,096 512 rows 22.9 / 22.8, 768 rows 39 / 24; 4,096 -> 6,144 384 rows 23.1 / 25.2, 512 rows 39 / 26; 14,336 -> 4,096
+// 512 rows 62 / 60, 768 rows 110 / 62.)  Up to 128 rows the weights are the work: 4,096 -> 28,672 128 rows 38 / 42, 64 rows 29 / 39, 192 rows 69 / 42.
+static bool on_pairs_of_sms(int rows, int features) { return rows > 128 && (int64_t)ceil_div(rows, 128) * ceil_div(features, 128) > 148; }
+
+// A product as its callers see it: rows x [x_rows, K] times matrices in blocks (the other arguments as tib_block_scaled_tcgen05).  codes: where the rows'
+// codes [M, runs * 128] and scales [runs, M rounded up to 4] go, ahead of the product (`make`; not made: they are there from a call before); null: the
+// product's kernel quantises the rows itself.
+TIB_API int tib_block_scaled_product(const void* x, int x_dtype, int64_t ldx, int x_rows, void* codes, int make, const void* w, const float* w_scales,
+                                     int scale_rows, int pairs, void* y, int y_dtype, int64_t ldy, int M, int N, int K, const int* offsets,
+                                     const int* order, int experts, int top, int x_by_pair, int act, float limit, float alpha,
+                                     const float* row_scale, int* error_word, cudaStream_t stream) {
+  if (M == 0 || N == 0) return TIB_OK;
+  if (!codes)
+    return tib_block_scaled_tcgen05(x, x_dtype, ldx, x_rows, nullptr, 0, w, w_scales, scale_rows, pairs, y, y_dtype, ldy, M, N, K, offsets, order, experts,
+                                    top, x_by_pair, act, limit, alpha, row_scale, error_word, stream);
+  if (M < 0 || K < 1 || (offsets && experts < 1)) return TIB_E_ARG;
+  const int runs = ceil_div(K, kBlk);
+  const int64_t lds = ((int64_t)M + 3) & ~(int64_t)3;
+  float* scales = reinterpret_cast<float*>(static_cast<char*>(codes) + (int64_t)M * runs * kBlk);
+  if (make) {
+    const bool gather = offsets && x_by_pair;      // (the pairs' rows, sorted on the way)
+    const int rc = tib_quantize_rows(x, x_dtype, ldx, codes, (int64_t)runs * kBlk, scales, lds, M, K, gather ? order : nullptr, top,
+                                     gather ? offsets + experts : nullptr, stream);
+    if (rc != TIB_OK) return rc;
+  }
+  if (!offsets && (act == MOE_ACT_NONE || act == MOE_ACT_SWIGLU) && !row_scale && on_pairs_of_sms(M, N))
+    return tib_block_scaled_2cta(codes, scales, lds, w, w_scales, scale_rows, pairs, act == MOE_ACT_SWIGLU, y, y_dtype, ldy, M, N, K, error_word, stream);
+  return tib_block_scaled_tcgen05(codes, -1, 0, M, scales, lds, w, w_scales, scale_rows, pairs, y, y_dtype, ldy, M, N, K, offsets, order, experts, top, 0, act,
+                                  limit, alpha, row_scale, error_word, stream);
+}
+
 // The calls the Python parts make (common.cuh).
 TIB_PACKED(tib_quantize_rows)
+TIB_PACKED(tib_block_scaled_product)

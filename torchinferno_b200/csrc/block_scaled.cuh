@@ -118,3 +118,15 @@ static inline int bs_make_map(CUtensorMap* map, const void* ptr, int64_t rows, i
 }
 
 }  // namespace tib
+
+// What a product of block-scaled operands is made of (block_scaled.cu, block_scaled_tcgen05.cu, block_scaled_2cta.cu).
+extern "C" {
+int tib_quantize_rows(const void* x, int x_dtype, int64_t ldx, void* codes, int64_t ldc, float* scales, int64_t lds, int rows, int K,
+                      const int* order, int top, const int* sorted, cudaStream_t stream);
+int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, int x_rows, const float* x_scales, int64_t lds, const void* w,
+                             const float* w_scales, int scale_rows, int pairs, void* y, int y_dtype, int64_t ldy, int M, int N, int K,
+                             const int* offsets, const int* order, int experts, int top, int x_by_pair, int act, float limit, float alpha,
+                             const float* row_scale, int* error_word, cudaStream_t stream);
+int tib_block_scaled_2cta(const void* x, const float* x_scales, int64_t lds, const void* w, const float* w_scales, int scale_rows, int pairs,
+                          int swiglu, void* out, int out_dtype, int64_t ldo, int M, int N, int K, int* error_word, cudaStream_t stream);
+}

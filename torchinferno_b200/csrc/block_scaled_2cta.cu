@@ -327,6 +327,3 @@ TIB_API int tib_block_scaled_2cta(const void* x, const float* x_scales, int64_t 
     return out_dtype == TIB_BF16 ? launch_b2<true, __nv_bfloat16>(map_x, map_w, a, out, ldo, stream) : launch_b2<true, float>(map_x, map_w, a, out, ldo, stream);
   return out_dtype == TIB_BF16 ? launch_b2<false, __nv_bfloat16>(map_x, map_w, a, out, ldo, stream) : launch_b2<false, float>(map_x, map_w, a, out, ldo, stream);
 }
-
-// The call the Python parts make (common.cuh).
-TIB_PACKED(tib_block_scaled_2cta)

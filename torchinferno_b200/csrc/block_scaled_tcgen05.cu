@@ -652,6 +652,3 @@ TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, in
   TIB_BS_GO(16, float);
 #undef TIB_BS_GO
 }
-
-// The calls the Python parts make (common.cuh).
-TIB_PACKED(tib_block_scaled_tcgen05)

@@ -79,46 +79,50 @@ def quantize_matrix(matrix: torch.Tensor) -> BlockScaledMatrix:
     return BlockScaledMatrix(codes.to(CODE_DTYPE).contiguous(), scales.contiguous())
 
 
+def _checked_rows(x: torch.Tensor, columns: int | None, device: int | None, what: str) -> int:
+    """The number of rows of ``x``, which must be [rows, ``columns``] with unit inner stride on the current device (and on ``device``)."""
+    shape = x.shape
+    if len(shape) != 2 or shape[1] == 0 or (columns is not None and shape[1] != columns):
+        raise ops.KernelError(f"{what}: rows of {columns or 'one number or more'} are wanted, not {tuple(shape)}")
+    here = x.get_device()
+    if here < 0:
+        raise ops.KernelError(f"{what}: operands must be CUDA tensors (there is no CPU path)")
+    if (device is not None and here != device) or here != torch._C._cuda_getDevice():
+        raise ops.KernelError(f"{what}: the rows are on cuda:{here}, the weight on cuda:{device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    if x.stride(1) != 1 and shape[1] > 1:
+        raise ops.KernelError(f"{what}: rows need unit inner stride, not {x.stride()}")
+    return shape[0]
+
+
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(codes [M, K], scales [M, runs of 128]) of the rows ``x`` [M, K] (bfloat16 or float32, any row stride); see the module's text."""
-    rows, columns = _row_shape(x)
-    runs = blocks(columns)
-    lds = (rows + 3) & ~3
-    codes = torch.empty((rows, runs * BLOCK), dtype=CODE_DTYPE, device=x.device)
-    scales = torch.empty_strided((lds, runs), (1, lds), dtype=torch.float32, device=x.device)
-    ops.quantize_rows(x, columns, codes.data_ptr(), scales.data_ptr(), lds)
-    return codes if columns == runs * BLOCK else codes[:, :columns], scales if lds == rows else scales[:rows]
+    rows = _checked_rows(x, None, None, "quantize_rows")
+    columns = x.shape[1]
+    runs, lds = blocks(columns), (rows + 3) & ~3
+    codes = x.new_empty((rows, runs * BLOCK), dtype=CODE_DTYPE)
+    scales = torch.empty_strided((rows, runs), (1, lds), dtype=torch.float32, device=x.device) if lds == rows else \
+        torch.empty_strided((lds, runs), (1, lds), dtype=torch.float32, device=x.device)[:rows]
+    ops.quantize_rows(x, codes.data_ptr(), scales.data_ptr(), lds)
+    return codes if columns == runs * BLOCK else codes[:, :columns], scales
 
 
-def _row_shape(x: torch.Tensor) -> tuple[int, int]:
-    if x.dim() != 2 or x.shape[1] == 0:
-        raise ops.KernelError(f"rows to quantise must be [rows, columns], got {tuple(x.shape)}")
-    return x.shape[0], x.shape[1]
-
-
-def _quantized(x: torch.Tensor, columns: int, routing: tuple[torch.Tensor, torch.Tensor, int] | None = None) -> tuple[torch.Tensor, tuple[int, int, int]]:
-    """The rows' codes and scales as the products read them: a buffer (to be held until the product is launched), and what
-    :func:`ops.block_scaled_product` takes.  ``routing`` = (offsets, order, top): the rows of the pairs sorted by expert."""
-    rows, runs = x.shape[0] if routing is None else routing[1].numel(), -(-columns // BLOCK)
-    lds = (rows + 3) & ~3
-    buffer = torch.empty(rows * runs * BLOCK + 4 * lds * runs, dtype=torch.uint8, device=x.device)
-    at = buffer.data_ptr()
-    codes = (at, at + rows * runs * BLOCK, lds)
-    ops.quantize_rows(x, columns, *codes, routing)
-    return buffer, codes
+def _code_buffer(x: torch.Tensor, rows: int, columns: int) -> torch.Tensor:
+    """Room for the codes and scales of ``rows`` rows (see :func:`ops.block_scaled_product`)."""
+    runs = -(-columns // BLOCK)
+    return x.new_empty(runs * (rows * BLOCK + 4 * ((rows + 3) & ~3)), dtype=torch.uint8)
 
 
 class Blocks:
     """Matrices of one size as the kernels read them: ``codes`` [matrices, blocks of N, blocks of K, 128, 128], padded with zeros, and ``scales`` [matrices,
     blocks of N, blocks of K]; ``paired``: the matrices' rows are (gate i, up i), their scales' rows (gate block j, up block j)."""
-    __slots__ = ("codes", "scales", "features", "paired", "codes_at", "scales_at", "scale_rows")
+    __slots__ = ("codes", "scales", "count", "features", "columns", "paired", "codes_at", "scales_at", "scale_rows")
 
-    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, features: int, paired: bool) -> None:
-        if codes.shape[1] != blocks(features) or scales.shape[1:] != (codes.shape[1] if not paired else 2 * blocks(features // 2), codes.shape[2]):
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, features: int, columns: int, paired: bool) -> None:
+        if codes.shape[1] != blocks(features) or codes.shape[2] != blocks(columns) or scales.shape[1:] != (codes.shape[1] if not paired else 2 * blocks(features // 2), codes.shape[2]):
             raise ValueError(f"blocks {tuple(codes.shape)} and scales {tuple(scales.shape)} do not make matrices of {features} rows")
         if not codes.is_contiguous() or not scales.is_contiguous():
             raise ValueError("blocks and their scales must be contiguous")
-        self.codes, self.scales, self.features, self.paired = codes, scales, features, paired
+        self.codes, self.scales, self.count, self.features, self.columns, self.paired = codes, scales, codes.shape[0], features, columns, paired
         self.codes_at, self.scales_at, self.scale_rows = codes.data_ptr(), scales.data_ptr(), scales.shape[1]
 
 
@@ -132,16 +136,19 @@ def _laid_out(matrices: Sequence[BlockScaledMatrix], ups: Sequence[BlockScaledMa
         raise ValueError(f"{len(matrices)} gate and {len(ups)} up matrices")
     n, k = shape
     parts, runs = 1 if ups is None else 2, blocks(k)
-    tiles = blocks(n * parts)
-    codes = torch.empty((len(matrices), tiles, runs, BLOCK, BLOCK), dtype=torch.uint8, device=device)
+    tiles, each = blocks(n * parts), BLOCK // parts
+    codes = torch.empty((len(matrices), tiles, runs, each, parts, BLOCK), dtype=torch.uint8, device=device)
     scales = torch.empty((len(matrices), blocks(n), parts, runs), dtype=torch.float32, device=device)
-    for i, m in enumerate(matrices):
-        flat = torch.zeros((tiles * BLOCK, runs * BLOCK), dtype=torch.uint8, device=device)
-        for part, stack in enumerate((matrices,) if ups is None else (matrices, ups)):
-            flat[part:n * parts:parts, :k] = stack[i].codes.view(torch.uint8)
-            scales[i, :, part] = stack[i].scales
-        codes[i] = flat.view(tiles, BLOCK, runs, BLOCK).transpose(1, 2)
-    return Blocks(codes.view(CODE_DTYPE), scales.view(len(matrices), blocks(n) * parts, -1), n * parts, ups is not None)
+    pad = (0, runs * BLOCK - k, 0, tiles * each - n)
+    for part, stack in enumerate((matrices,) if ups is None else (matrices, ups)):
+        for i, m in enumerate(stack):
+            stored = m.codes.view(torch.uint8)
+            if any(pad):
+                stored = torch.nn.functional.pad(stored, pad)
+            codes[i, :, :, :, part].copy_(stored.view(tiles, each, runs, BLOCK).transpose(1, 2))
+            scales[i, :, part].copy_(m.scales)
+    return Blocks(codes.view(len(matrices), tiles, runs, BLOCK, BLOCK).view(CODE_DTYPE), scales.view(len(matrices), blocks(n) * parts, -1), n * parts, k,
+                  ups is not None)
 
 
 class BlockScaledWeight:
@@ -200,46 +207,41 @@ class BlockScaledWeight:
             if lo < hi:
                 if lo % BLOCK:
                     raise ValueError(f"feature {start} lies inside a block")
-                view.parts.append((first + lo - start, Blocks(part.codes[:, lo // BLOCK:blocks(hi)], part.scales[:, lo // BLOCK:blocks(hi)], hi - lo, False)))
+                view.parts.append((first + lo - start, Blocks(part.codes[:, lo // BLOCK:blocks(hi)], part.scales[:, lo // BLOCK:blocks(hi)], hi - lo, self.in_features, False)))
         return view
 
-    def _target(self, x: torch.Tensor, out_dtype: torch.dtype | None, width: int, out: torch.Tensor | None) -> torch.Tensor:
-        """The tensor that the product is written to."""
-        if x.dim() != 2 or x.shape[1] != self.in_features:
-            raise ops.KernelError(f"linear: shapes {tuple(x.shape)} and {(self.out_features, self.in_features)} do not fit")
-        if x.get_device() != self.parts[0][1].codes.get_device() or not x.is_cuda:
-            raise ops.KernelError(f"linear: x is on {x.device}, the weight on {self.device} (there is no CPU path)")
-        if out_dtype is None:
-            out_dtype = x.dtype
-        if out_dtype not in (torch.bfloat16, torch.float32):
-            raise ops.KernelError(f"linear: unsupported output dtype {out_dtype}")
-        if out is None or out.dtype != out_dtype:
-            return x.new_empty((x.shape[0], width)) if x.dtype == out_dtype else x.new_empty((x.shape[0], width), dtype=out_dtype)
-        if out.shape != (x.shape[0], width) or out.stride(1) != 1 or out.device != x.device:
-            raise ops.KernelError(f"linear: out is {tuple(out.shape)}, wanted {(x.shape[0], width)} with unit inner stride on {x.device}")
+    def _run(self, x: torch.Tensor, act: str, width: int, out_dtype: torch.dtype | None, out: torch.Tensor | None, error_word: torch.Tensor | None) -> torch.Tensor:
+        rows = _checked_rows(x, self.in_features, self.parts[0][1].codes.get_device(), "linear")
+        if out_dtype is not None and out_dtype != x.dtype:
+            if out_dtype not in (torch.bfloat16, torch.float32):
+                raise ops.KernelError(f"linear: unsupported output dtype {out_dtype}")
+            if out is None or out.dtype != out_dtype:
+                out = x.new_empty((rows, width), dtype=out_dtype)
+        elif out is None or out.dtype != x.dtype:
+            out = x.new_empty((rows, width))
+        if out.shape != (rows, width) or (out.stride(1) != 1 and width > 1) or out.get_device() != x.get_device():
+            raise ops.KernelError(f"linear: out is {tuple(out.shape)} on {out.device}, wanted {(rows, width)} with unit inner stride on {x.device}")
+        if rows == 0:
+            return out
+        held = None if rows <= FEW_ROWS else _code_buffer(x, rows, self.in_features)
+        codes = 0 if held is None else held.data_ptr()
+        if len(self.parts) == 1:
+            ops.block_scaled_product(x, codes, True, self.parts[0][1], out, act, 0.0, 0.0, 0, 0, 1, False, None, error_word)
+        else:
+            for i, (first, part) in enumerate(self.parts):
+                ops.block_scaled_product(x, codes, i == 0, part, out[:, first:first + part.features], act, 0.0, 0.0, 0, 0, 1, False, None, error_word)
         return out
 
     def product(self, x: torch.Tensor, *, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
                 error_word: torch.Tensor | None = None) -> torch.Tensor:
         """x [tokens, in] times the weight: [tokens, out] (a swiglu weight's gate and up sums side by side)."""
-        out = self._target(x, out_dtype, self.out_features, out)
-        if x.shape[0] == 0:
-            return out
-        _held, codes = (None, None) if x.shape[0] <= FEW_ROWS else _quantized(x, self.in_features)
-        for first, part in self.parts:
-            ops.block_scaled_product(x, codes, part, self.in_features, out if len(self.parts) == 1 else out[:, first:first + part.features],
-                                     error_word=error_word)
-        return out
+        return self._run(x, "none", self.out_features, out_dtype, out, error_word)
 
     def swiglu(self, x: torch.Tensor, *, out_dtype: torch.dtype | None = None, error_word: torch.Tensor | None = None) -> torch.Tensor:
         """silu(gate) * up of the 32-bit sums: [tokens, out / 2]."""
         if self.epilogue != "swiglu":
             raise ops.KernelError("linear_swiglu: the weight was not bound with epilogue='swiglu'")
-        out = self._target(x, out_dtype, self.out_features // 2, None)
-        if x.shape[0] == 0:
-            return out
-        _held, codes = (None, None) if x.shape[0] <= FEW_ROWS else _quantized(x, self.in_features)
-        return ops.block_scaled_product(x, codes, self.parts[0][1], self.in_features, out, act="swiglu", error_word=error_word)
+        return self._run(x, "swiglu", self.out_features // 2, out_dtype, None, error_word)
 
 
 class BlockScaledExperts:
@@ -274,25 +276,20 @@ class BlockScaledExperts:
         if gated != self.paired and act != "none":
             raise ops.KernelError(f"moe_expert_product: activation {act!r} does not fit experts with{'' if self.paired else 'out'} gate and up rows")
         pairs, width = order.numel(), self.out_features // 2 if gated else self.out_features
-        if (x.dim() != 2 or x.shape[1] != self.in_features or y.shape != (pairs, width) or offsets.numel() != self.experts + 1 or top < 1
-                or (pairs % top if x_by_pair else x.shape[0] < pairs) or (x_by_pair and x.shape[0] < pairs // top)):
-            raise ops.KernelError("moe_expert_product: shapes do not fit")
         here = self.blocks.codes.get_device()
-        for name, t in (("x", x), ("y", y), ("offsets", offsets), ("order", order)):
-            if t.get_device() != here or here < 0:
-                raise ops.KernelError(f"moe_expert_product: {name} is on {t.device}, the experts on {self.device} (there is no CPU path)")
-        if y.stride(1) != 1:
-            raise ops.KernelError("moe_expert_product: y needs unit inner stride")
-        ops._need(offsets, "offsets", torch.int32), ops._need(order, "order", torch.int32)
-        if row_scale is not None:
-            ops._need(row_scale, "row_scale", torch.float32)
-            if row_scale.numel() != pairs:
-                raise ops.KernelError("moe_expert_product: row_scale must hold one factor per pair")
+        rows = _checked_rows(x, self.in_features, here, "moe_expert_product")
+        if y.shape != (pairs, width) or offsets.numel() != self.experts + 1 or top < 1 or (pairs % top or rows < pairs // top if x_by_pair else rows < pairs):
+            raise ops.KernelError("moe_expert_product: shapes do not fit")
+        for name, t, dtype in (("offsets", offsets, torch.int32), ("order", order, torch.int32), ("row_scale", row_scale, torch.float32)):
+            if t is not None and (t.dtype != dtype or t.get_device() != here or not t.is_contiguous()):
+                raise ops.KernelError(f"moe_expert_product: {name} must be contiguous {dtype} on cuda:{here}, not {t.dtype} on {t.device}")
+        if y.get_device() != here or (y.stride(1) != 1 and width > 1):
+            raise ops.KernelError(f"moe_expert_product: y must be rows with unit inner stride on cuda:{here}")
+        if row_scale is not None and row_scale.numel() != pairs:
+            raise ops.KernelError("moe_expert_product: row_scale must hold one factor per pair")
         if pairs == 0:
             return y
-        if pairs <= FEW_EXPERT_ROWS * self.experts:
-            _held, codes = None, None
-        else:                                   # (the pairs' rows, sorted on the way)
-            _held, codes = _quantized(x if x_by_pair else x[:pairs], self.in_features, (offsets, order, top) if x_by_pair else None)
-        return ops.block_scaled_product(x, codes, self.blocks, self.in_features, y, act=act, limit=limit, alpha=alpha,
-                                        routing=(offsets, order, top, x_by_pair), row_scale=row_scale, error_word=error_word)
+        held = None if pairs <= FEW_EXPERT_ROWS * self.experts else _code_buffer(x, pairs, self.in_features)
+        ops.block_scaled_product(x, 0 if held is None else held.data_ptr(), True, self.blocks, y, act, limit, alpha, offsets.data_ptr(), order.data_ptr(), top,
+                                 x_by_pair, row_scale, error_word)
+        return y

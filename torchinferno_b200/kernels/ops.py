@@ -1254,62 +1254,26 @@ def moe_combine(y: torch.Tensor, place: torch.Tensor, weights: torch.Tensor | No
 
 
 # ---------------------------------------------------------------------------
-# 8-bit block-scaled operands (csrc/block_scaled*.cu).  Their Python types (kernels/block_scaled.py) check shapes and own the buffers; these take addresses, as
-# a call with few rows is as long as what the host does for it.
-def _rows_here(x: torch.Tensor, columns: int, name: str) -> None:
-    """Rows of ``columns`` numbers on the current device, with unit inner stride."""
-    device = x.get_device()
-    if device < 0:
-        raise KernelError(f"{name}: x must be a CUDA tensor (there is no CPU path)")
-    if device != torch._C._cuda_getDevice():
-        raise KernelError(f"{name}: x is on {x.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
-    if x.dim() != 2 or x.shape[1] != columns or (x.stride(1) != 1 and columns > 1):
-        raise KernelError(f"{name}: rows of {columns} numbers with unit inner stride are wanted, not {tuple(x.shape)} with strides {x.stride()}")
-
-
-def quantize_rows(x: torch.Tensor, columns: int, codes: int, scales: int, lds: int, routing: tuple[torch.Tensor, torch.Tensor, int] | None = None) -> None:
-    """Codes [rows, ``columns`` rounded up to 128] (8 bits) and scales [runs of 128 columns, ``lds``] of the rows ``x``, to these addresses.  ``routing`` =
-    (offsets, order, top): one row of codes for each pair sorted by expert, made of row order[s] // top of ``x`` (none behind the last expert's)."""
-    _rows_here(x, columns, "quantize_rows")
-    rows, order, top, end = x.shape[0], 0, 1, 0
-    if routing is not None:
-        rows, order, top, end = routing[1].numel(), routing[1].data_ptr(), routing[2], routing[0].data_ptr() + 4 * (routing[0].numel() - 1)
+# 8-bit block-scaled operands (csrc/block_scaled*.cu).  Their Python types (kernels/block_scaled.py) check what they are given and own the buffers; these
+# take addresses, as a call with few rows is as long as what the host does for it.
+def quantize_rows(x: torch.Tensor, codes: int, scales: int, lds: int) -> None:
+    """Codes [rows, columns rounded up to 128] (8 bits) and scales [runs of 128 columns, ``lds``] of the rows ``x``, to these addresses."""
+    rows, columns = x.shape
     _check("quantize_rows", lib().tib_quantize_rows(x.data_ptr(), _code(x.dtype), x.stride(0), codes, -(-columns // 128) * 128, scales, lds, rows, columns,
-                                                    order, top, end, _stream()))
+                                                    0, 1, 0, _stream()))
 
 
-def block_scaled_pairs_of_sms(rows: int, features: int) -> bool:
-    """Whether a product of codes runs on pairs of SMs, in tiles of 256 rows x 256 features: where tiles of 128 x 128 would be more than one for each of
-    148 SMs.  (us, tiles of 128 / pairs: 4,096 -> 4,096 512 rows 22.9 / 22.8, 768 rows 39 / 24; 4,096 -> 6,144 384 rows 23.1 / 25.2, 512 rows 39 / 26;
-    14,336 -> 4,096 512 rows 62 / 60, 768 rows 110 / 62.)  Up to 128 rows the weights are the work: 4,096 -> 28,672 128 rows 38 / 42, 64 rows 29 / 39, 192
-    rows 69 / 42."""
-    return rows > 128 and -(-rows // 128) * -(-features // 128) > 148
-
-
-def block_scaled_product(x: torch.Tensor, codes: tuple[int, int, int] | None, blocks, columns: int, y: torch.Tensor, *, act: str = "none", limit: float = 0.0,
-                         alpha: float = 1.0, routing: tuple[torch.Tensor, torch.Tensor, int, bool] | None = None,
-                         row_scale: torch.Tensor | None = None, error_word: torch.Tensor | None = None) -> torch.Tensor:
-    """The rows ``x`` times matrices of 8-bit blocks (a block_scaled.Blocks).  ``codes``: the addresses of the rows' codes and scales and the latter's
-    row length, as :func:`quantize_rows` left them (for rows sorted by expert: sorted); None: the product's kernel quantises the rows itself.  ``routing``
-    = (offsets, order, top, x_by_pair) sorts the rows of ``y`` by expert as in :func:`moe_expert_product`; without it row m of ``y`` is that of row m."""
-    _rows_here(x, columns, "block_scaled_product")
-    rows = y.shape[0]
-    if codes is not None and routing is None and act in ("none", "swiglu") and block_scaled_pairs_of_sms(rows, blocks.features):
-        _check("block_scaled_product", lib().tib_block_scaled_2cta(
-            codes[0], codes[1], codes[2], blocks.codes_at, blocks.scales_at, blocks.scale_rows, blocks.paired, act == "swiglu", y.data_ptr(), _code(y.dtype),
-            y.stride(0), rows, blocks.features, columns, _ptr(error_word), _stream()))
-        return y
-    offsets = order = 0
-    top = experts = 1
-    x_by_pair = False
-    if routing is not None:
-        offsets, order, top, x_by_pair, experts = routing[0].data_ptr(), routing[1].data_ptr(), routing[2], routing[3] and codes is None, routing[0].numel() - 1
-    at, kind, ldx, x_scales, lds = (x.data_ptr(), _code(x.dtype), x.stride(0), 0, 0) if codes is None else (codes[0], -1, 0, codes[1], codes[2])
-    _check("block_scaled_product", lib().tib_block_scaled_tcgen05(
-        at, kind, ldx, x.shape[0] if codes is None else rows, x_scales, lds, blocks.codes_at, blocks.scales_at, blocks.scale_rows, blocks.paired, y.data_ptr(),
-        _code(y.dtype), y.stride(0), rows, blocks.features, columns, offsets, order, experts, top, x_by_pair, MOE_ACT[act], limit, alpha, _ptr(row_scale),
-        _ptr(error_word), _stream()))
-    return y
+def block_scaled_product(x: torch.Tensor, codes: int, make: bool, blocks, y: torch.Tensor, act: str, limit: float, alpha: float, offsets: int, order: int,
+                         top: int, x_by_pair: bool, row_scale: torch.Tensor | None, error_word: torch.Tensor | None) -> None:
+    """The rows ``x`` times matrices of 8-bit blocks (a block_scaled.Blocks), into ``y``.  ``codes``: the address of M * runs * 128 + 4 * runs * (M rounded up
+    to 4) bytes for the codes of the M rows of ``y``, which are made there first (``make``) or are there from a call before; 0: the product's kernel
+    quantises the rows itself.  ``offsets`` / ``order``: addresses of what sorts the rows of ``y`` by expert as in :func:`moe_expert_product`, or 0."""
+    if codes and make:
+        _counter["launches"] += 1
+    _check("block_scaled_product", lib().tib_block_scaled_product(
+        x.data_ptr(), _code(x.dtype), x.stride(0), x.shape[0], codes, make, blocks.codes_at, blocks.scales_at, blocks.scale_rows, blocks.paired, y.data_ptr(),
+        _code(y.dtype), y.stride(0), y.shape[0], blocks.features, blocks.columns, offsets, order, blocks.count, top, x_by_pair, MOE_ACT[act], limit, alpha,
+        0 if row_scale is None else row_scale.data_ptr(), 0 if error_word is None else error_word.data_ptr(), _stream()))
 
 
 def glu_clamp(gate_up: torch.Tensor, out: torch.Tensor, limit: float, alpha: float) -> torch.Tensor:
