@@ -66,6 +66,10 @@ TIB_API int tib_quantize_rows(const void* x, int x_dtype, int64_t ldx, void* cod
 // 512 rows 62 / 60, 768 rows 110 / 62.)  Up to 128 rows the weights are the work: 4,096 -> 28,672 128 rows 38 / 42, 64 rows 29 / 39, 192 rows 69 / 42.
 static bool on_pairs_of_sms(int rows, int features) { return rows > 128 && (int64_t)ceil_div(rows, 128) * ceil_div(features, 128) > 148; }
 
+// Rows sorted by expert run there from so many rows an expert on, on average.  (32 experts 2,048 -> 1,024, us, tiles of 128 / pairs: 64 rows an expert 26.2 / 27.6,
+// 96 28.2 / 29.2, 128 37.2 / 29.8, 192 47.8 / 32.6, 256 60.7 / 45.1, 512 98.4 / 71.4; gated, 256: 95.3 / 73.9.)
+constexpr int kBsPairRows = 100;
+
 // A product as its callers see it: rows x [x_rows, K] times matrices in blocks (the other arguments as tib_block_scaled_tcgen05).  codes: where the rows'
 // codes [M, runs * 128] and scales [runs, M rounded up to 4] go, ahead of the product (`make`; not made: they are there from a call before); null: the
 // product's kernel quantises the rows itself.
@@ -87,8 +91,9 @@ TIB_API int tib_block_scaled_product(const void* x, int x_dtype, int64_t ldx, in
                                      gather ? offsets + experts : nullptr, stream);
     if (rc != TIB_OK) return rc;
   }
-  if (!offsets && (act == MOE_ACT_NONE || act == MOE_ACT_SWIGLU) && !row_scale && on_pairs_of_sms(M, N))
-    return tib_block_scaled_2cta(codes, scales, lds, w, w_scales, scale_rows, pairs, act == MOE_ACT_SWIGLU, y, y_dtype, ldy, M, N, K, error_word, stream);
+  if (offsets ? M >= (int64_t)experts * kBsPairRows && experts <= tib_block_scaled_2cta_experts() : on_pairs_of_sms(M, N))
+    return tib_block_scaled_2cta(codes, scales, lds, w, w_scales, scale_rows, pairs, y, y_dtype, ldy, M, N, K, offsets, order, experts, act, limit, alpha,
+                                 row_scale, error_word, stream);
   return tib_block_scaled_tcgen05(codes, -1, 0, M, scales, lds, w, w_scales, scale_rows, pairs, y, y_dtype, ldy, M, N, K, offsets, order, experts, top, 0, act,
                                   limit, alpha, row_scale, error_word, stream);
 }

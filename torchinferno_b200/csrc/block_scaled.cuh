@@ -38,6 +38,15 @@ __device__ __forceinline__ float bs_sigmoid(float x) {
   return r;
 }
 
+// The experts' activations (moe.cuh) with this sigmoid.
+template <int ACT> __device__ __forceinline__ float bs_act(float v) { return ACT == MOE_ACT_SILU ? v * bs_sigmoid(v) : moe_act(v, ACT); }
+template <int ACT> __device__ __forceinline__ float bs_gated(float g, float u, float limit, float alpha) {
+  if (ACT == MOE_ACT_SWIGLU) return g * bs_sigmoid(g) * u;
+  g = fminf(g, limit);
+  u = fminf(fmaxf(u, -limit), limit);
+  return g * bs_sigmoid(alpha * g) * (u + 1.f);
+}
+
 // two floats to two codes (the first in the lower byte), to nearest, ties to even; a NaN stays one
 __device__ __forceinline__ uint32_t bs_codes2(float lo, float hi) {
   uint16_t r;
@@ -127,6 +136,8 @@ int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, int x_rows
                              const float* w_scales, int scale_rows, int pairs, void* y, int y_dtype, int64_t ldy, int M, int N, int K,
                              const int* offsets, const int* order, int experts, int top, int x_by_pair, int act, float limit, float alpha,
                              const float* row_scale, int* error_word, cudaStream_t stream);
+int tib_block_scaled_2cta_experts();
 int tib_block_scaled_2cta(const void* x, const float* x_scales, int64_t lds, const void* w, const float* w_scales, int scale_rows, int pairs,
-                          int swiglu, void* out, int out_dtype, int64_t ldo, int M, int N, int K, int* error_word, cudaStream_t stream);
+                          void* out, int out_dtype, int64_t ldo, int M, int N, int K, const int* offsets, const int* order, int experts, int act,
+                          float limit, float alpha, const float* row_scale, int* error_word, cudaStream_t stream);
 }

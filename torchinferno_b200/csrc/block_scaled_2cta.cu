@@ -1,4 +1,5 @@
-// Products of 8-bit block-scaled operands for many rows, on pairs of SMs: out[M, N] = x . w^T with `tcgen05.mma.cta_group::2`, where
+// Products of 8-bit block-scaled operands for many rows, plain or sorted by expert, on pairs of SMs: out[M, N] = x . w^T with
+// `tcgen05.mma.cta_group::2`, where
 //     out[m, n] = sum over runs b of s[m, b] S[n's block, b] (sum over the 128 columns of run b of x[m, k] w[n, k]).
 //
 // Two blocks (a cluster of two) compute a tile of 256 rows x 256 features, as in gemm_tcgen05_2cta.cu: block r holds rows r * 128 .. of the
@@ -8,7 +9,7 @@
 // the last, and add it to 128 sums a thread, times the scale of (its row, run) and (the features' block, run).  Two sums are one packed
 // multiply-add; in a matrix of (gate, up) row pairs the two have different scales, which the packed form takes as it comes.
 //   warp 0       TMA producer into a ring of six stages      warp 1 (of the even block)   issues the MMAs; either owns its block's TMEM
-//   warps 4..11  sums, then the epilogue: plain, or silu(gate) * up.  These take registers that the first four warps give up (168 a thread at launch,
+//   warps 4..11  sums, then the epilogue with its activation.  These take registers that the first four warps give up (168 a thread at launch,
 //                40 + 2 x 232 after)
 // For a step the tensor cores need 512 cycles at their peak, the sums 256 of the tensor memory's reads and 256 of the fp32 pipe.
 // Every wait is bounded and reports in error_word; no block leaves before its partner is done; every copy lands in the block that issued it.
@@ -20,6 +21,7 @@ namespace tib {
 constexpr int kB2Stages = 6, kB2Threads = 384;
 constexpr uint32_t kB2Half = 128 * kBlk, kB2Stage = 2 * kB2Half;
 constexpr uint32_t kB2Smem = kB2Stages * kB2Stage + 1024 /* alignment */ + 256 /* barriers */ + 8 * 4096 /* outputs */;
+constexpr int kB2MaxExperts = (kMostSmem - (int)kB2Smem) / 8 - 1;      // (two numbers each in what is left of shared memory)
 // D fp32, A and B e4m3, both K-major, N = 256, M = 256 over the pair
 constexpr uint32_t kB2Idesc = (1u << 4) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
 
@@ -58,12 +60,18 @@ struct B2Args {
   int64_t lds;
   const float* w_scales;       // [rows of scales, runs]
   int scale_rows, pairs, M, N, runs;
+  const int* offsets;          // [experts + 1] of rows sorted by expert, or null: one matrix
+  const int* order;
+  int experts;
+  MoeEpilogue ep;
   int* error_word;
 };
 
-// Persistent: pair p walks the tiles t = p, p + pairs, ...; tile t is row tile t % m_tiles of feature tile t / m_tiles, so pairs that run together
-// share slices of w.
-template <bool SWIGLU, typename TO>
+struct B2Tile { int expert, first, rows, n_tile; };      // rows first .. first + rows - 1 of x (at most 256), features n_tile * 256 ..
+
+// Persistent: pair p walks the tiles t = p, p + pairs, ...  Of one matrix, tile t is row tile t % m_tiles of feature tile t / m_tiles, so pairs that run
+// together share slices of w; of rows sorted by expert, feature tiles run fastest.
+template <int ACT, typename TO>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kB2Threads, 1)
 block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const B2Args a,
                          TO* __restrict__ out, int64_t ldo, int wide_stores) {
@@ -80,7 +88,9 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();                    // 0: the even block of the pair, which issues the MMAs
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int m_tiles = (a.M + 255) >> 8, num_tiles = m_tiles * ((a.N + 255) >> 8);
+  const int n_tiles = (a.N + 255) >> 8;
+  int* tiles_before = reinterpret_cast<int*>(smem_raw + (bars - smem_u32(smem_raw)) + 256 + 8 * 4096);      // [experts + 1] where rows are sorted, and
+  int* first_row = tiles_before + a.experts + 1;                                                            // [experts + 1] their offsets
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kB2Stages; ++s) {
@@ -97,13 +107,50 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tmem_slot), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
   }
+  pdl_wait();
+  pdl_trigger();
+  if (a.offsets && warp == 0) {                            // the experts' row tiles, summed
+    int before = 0;
+    for (int e0 = 0; e0 < a.experts; e0 += 32) {
+      const int e = e0 + lane, begin = e < a.experts ? a.offsets[e] : 0, end = e < a.experts ? a.offsets[e + 1] : 0;
+      int sum = (end - begin + 255) >> 8;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += up;
+      }
+      if (e < a.experts) tiles_before[e + 1] = before + sum, first_row[e + 1] = end;
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (lane == 0) tiles_before[0] = 0, first_row[0] = a.offsets[0];
+  }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
   cluster_sync_all();                                      // both blocks have their barriers before either is signalled
   asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot_ptr, 0);
-  pdl_wait();
-  pdl_trigger();
+  const int m_tiles = a.offsets ? tiles_before[a.experts] : (a.M + 255) >> 8, num_tiles = m_tiles * n_tiles;
+  auto tile_of = [&](int t) {
+    B2Tile m;
+    if (!a.offsets) {
+      m.n_tile = t / m_tiles;
+      m.expert = 0;
+      m.first = (t - m.n_tile * m_tiles) * 256;
+      m.rows = min(256, a.M - m.first);
+      return m;
+    }
+    const int row_tile = t / n_tiles;
+    m.n_tile = t - row_tile * n_tiles;
+    int lo = 0, hi = a.experts;                            // tiles_before[lo] <= row_tile < tiles_before[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (tiles_before[mid] <= row_tile) lo = mid; else hi = mid;
+    }
+    m.expert = lo;
+    m.first = first_row[lo] + (row_tile - tiles_before[lo]) * 256;
+    m.rows = min(256, first_row[lo + 1] - m.first);
+    return m;
+  };
 
   if (warp >= 4) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;\n");
@@ -112,12 +159,13 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
     uint32_t acc_phase = 0;
     bool ok = true;
     for (int t = pair; t < num_tiles && ok; t += pairs) {
-      const int n_tile = t / m_tiles, row = (t - n_tile * m_tiles) * 256 + (int)rank * 128 + quarter * 32 + lane;
-      const int col0 = n_tile * 256 + half * 128;
+      const B2Tile m = tile_of(t);
+      const int in_tile = (int)rank * 128 + quarter * 32 + lane, row = m.first + in_tile, last = m.first + m.rows;      // (rows from `last` on are not stored)
+      const int col0 = m.n_tile * 256 + half * 128;
       // (features beyond the last have some scale of the matrix: they are not stored)
-      const float* xs = a.x_scales + min(row, a.M - 1);
-      const int block = a.pairs ? n_tile * 2 : n_tile * 2 + half;
-      const float* we = a.w_scales + (size_t)min(block, a.scale_rows - 1) * a.runs;
+      const float* xs = a.x_scales + min(row, last - 1);
+      const int block = a.pairs ? m.n_tile * 2 : min(m.n_tile * 2 + half, a.scale_rows - 1);
+      const float* we = a.w_scales + ((size_t)m.expert * a.scale_rows + block) * a.runs;
       const float* wo = a.pairs ? we + a.runs : we;
       f32x2 sum[64];
 #pragma unroll
@@ -163,10 +211,17 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
         if (kb + 1 < a.runs && ok) step(kb + 1, 1);
       }
       if (!ok) continue;
+      if (a.ep.row_scale) {
+        const float scale = a.ep.row_scale[a.order[min(row, last - 1)]];
+        const f32x2 scale2 = f2_pack(scale, scale);
+#pragma unroll
+        for (int c = 0; c < 64; ++c) sum[c] = f2_mul(sum[c], scale2);
+      }
       // A row's outputs lie in one thread: a warp's 32 rows cross its 4 KB of shared memory, 128 bytes of each at a time (16-byte pieces, swizzled by row),
       // and leave as whole lines.  (Stored by their threads, 16 bytes of 32 rows an instruction, a tile's outputs took 3 us.)
-      constexpr int kOut = SWIGLU ? 64 : 128, kVec = 16 / sizeof(TO), kTurn = 8 * kVec;      // outputs of a thread, a piece, a turn
-      const int first = SWIGLU ? col0 >> 1 : col0, n_out = SWIGLU ? a.N >> 1 : a.N;
+      constexpr bool kGated = moe_act_gated(ACT);
+      constexpr int kOut = kGated ? 64 : 128, kVec = 16 / sizeof(TO), kTurn = 8 * kVec;      // outputs of a thread, a piece, a turn
+      const int first = col0 >> kGated, n_out = a.N >> kGated;
       unsigned char* mine = smem_raw + (base - smem_u32(smem_raw)) + kB2Stages * kB2Stage + 256 + (warp - 4) * 4096;
 #pragma unroll
       for (int turn = 0; turn < kOut / kTurn; ++turn) {
@@ -176,15 +231,9 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
 #pragma unroll
           for (int j = 0; j < kVec; ++j) {
             const int c = turn * kTurn + p * kVec + j;
-            if constexpr (SWIGLU) {
-              float g, u;
-              f2_unpack(sum[c], g, u);
-              y[j] = g * bs_sigmoid(g) * u;
-            } else {
-              float lo, hi;
-              f2_unpack(sum[c >> 1], lo, hi);
-              y[j] = c & 1 ? hi : lo;
-            }
+            float lo, hi;
+            f2_unpack(sum[kGated ? c : c >> 1], lo, hi);
+            y[j] = kGated ? bs_gated<ACT>(lo, hi, a.ep.limit, a.ep.alpha) : bs_act<ACT>(c & 1 ? hi : lo);
           }
           uint4 w;
           if constexpr (sizeof(TO) == 2) {
@@ -203,7 +252,7 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
         for (int i = 0; i < 8; ++i) {
           const int r = 4 * i + (lane >> 3);
           const uint4 w = *reinterpret_cast<const uint4*>(mine + r * 128 + ((p ^ (r & 7)) << 4));
-          if (row - lane + r >= a.M) continue;
+          if (row - lane + r >= last) continue;
           TO* dst = out + (size_t)(row - lane + r) * ldo + col;
           if (wide_stores && col + kVec <= n_out) *reinterpret_cast<uint4*>(dst) = w;
           else {
@@ -224,7 +273,11 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
       uint32_t phase = 1;
       bool ok = true;
       for (int t = pair; t < num_tiles && ok; t += pairs) {
-        const int n_tile = t / m_tiles, m0 = (t - n_tile * m_tiles) * 256 + (int)rank * 128, w0 = (n_tile * 2 + (int)rank) * a.runs;
+        const B2Tile m = tile_of(t);
+        const int m0 = m.first + (int)rank * 128;          // (behind the tile's rows come others', which are not stored, or zeros)
+        const int w_block = m.n_tile * 2 + (int)rank, blocks = (a.N + 127) >> 7;
+        // (a pair's second block of features may lie behind the matrix: it reads some block of it instead, which is not stored)
+        const int w0 = (m.expert * blocks + min(w_block, blocks - 1)) * a.runs;
         for (int kb = 0; kb < a.runs; ++kb) {
           if (!mbar_wait_warp(empty_bar(s), phase)) {
             if (a.error_word && leader) atomicExch(a.error_word, 0x7C00D1);
@@ -284,19 +337,21 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
   }
 }
 
-template <bool SWIGLU, typename TO>
+template <int ACT, typename TO>
 static int launch_b2(const CUtensorMap& map_x, const CUtensorMap& map_w, const B2Args& a, void* out, int64_t ldo, cudaStream_t stream) {
-  auto kern = block_scaled_2cta_kernel<SWIGLU, TO>;
+  auto kern = block_scaled_2cta_kernel<ACT, TO>;
   static bool allowed[64];      // (by device: the attribute belongs to its context)
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
-  if (e == cudaSuccess && !(device < 64 && allowed[device])) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kB2Smem);
+  if (e == cudaSuccess && !(device < 64 && allowed[device])) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
   if (e != cudaSuccess) return (int)e;
   if (device < 64) allowed[device] = true;
-  const int64_t tiles = (int64_t)ceil_div(a.M, 256) * ceil_div(a.N, 256);
+  const int64_t row_tiles = a.offsets ? a.M / 256 + (a.M < a.experts ? a.M : a.experts) : ceil_div(a.M, 256);
+  const int64_t tiles = row_tiles * ceil_div(a.N, 256);
   if (tiles > 0x7fffffff) return TIB_E_SIZE;
   const int wide = ((uintptr_t)out & 15) == 0 && (ldo * sizeof(TO)) % 16 == 0;
-  TIB_LAUNCH_DEPENDENT(kern, 2 * (int)(tiles < 74 ? tiles : 74), kB2Threads, kB2Smem, stream, map_x, map_w, a, (TO*)out, ldo, wide);
+  TIB_LAUNCH_DEPENDENT(kern, 2 * (int)(tiles < 74 ? tiles : 74), kB2Threads, kB2Smem + (a.offsets ? 8 * (a.experts + 1) : 0), stream, map_x, map_w, a, (TO*)out,
+                       ldo, wide);
   return TIB_OK;
 }
 
@@ -304,26 +359,40 @@ static int launch_b2(const CUtensorMap& map_x, const CUtensorMap& map_w, const B
 
 using namespace tib;
 
-// x: codes [M, runs * 128] and scales [runs, lds] as tib_quantize_rows leaves them; w: codes in blocks [ceil(N / 128), runs, 128, 128] and
-// scales [scale_rows, runs] (`pairs`:
-// of (gate, up) row pairs, N and scale_rows even); out: [M, N] in out_dtype (row stride ldo), or [M, N / 2] with `swiglu`.
+TIB_API int tib_block_scaled_2cta_experts() { return kB2MaxExperts; }
+
+// x: codes [M, runs * 128] and scales [runs, lds] as tib_quantize_rows leaves them; w: codes in blocks [experts, ceil(N / 128), runs, 128, 128] and
+// scales [experts, scale_rows, runs] (`pairs`: of (gate, up) row pairs, N and scale_rows even); out: [M, N] in out_dtype (row stride ldo), or [M, N / 2] of a
+// gated activation.  offsets [experts + 1] and order [M]: rows sorted by expert, at most kB2MaxExperts of them; offsets null: one matrix for all rows.
 TIB_API int tib_block_scaled_2cta(const void* x, const float* x_scales, int64_t lds, const void* w, const float* w_scales, int scale_rows, int pairs,
-                                  int swiglu, void* out, int out_dtype, int64_t ldo, int M, int N, int K, int* error_word, cudaStream_t stream) {
+                                  void* out, int out_dtype, int64_t ldo, int M, int N, int K, const int* offsets, const int* order, int experts, int act,
+                                  float limit, float alpha, const float* row_scale, int* error_word, cudaStream_t stream) {
   if (M == 0 || N == 0) return TIB_OK;
-  if (!x || !x_scales || !w || !w_scales || !out || M < 0 || N < 0 || K < 1 || scale_rows < 1) return TIB_E_ARG;
-  if ((swiglu && !pairs) || (pairs && (N % 2 || scale_rows % 2)) || lds < M) return TIB_E_SIZE;
-  if ((int64_t)(ceil_div(N, 128) + 2) * ceil_div(K, kBlk) > (0x7fffffff >> 7)) return TIB_E_SIZE;
+  if (!x || !x_scales || !w || !w_scales || !out || M < 0 || N < 0 || K < 1 || scale_rows < 1 || experts < 1) return TIB_E_ARG;
+  if ((offsets && !order) || (row_scale && !order)) return TIB_E_ARG;
+  if (act < MOE_ACT_NONE || act > MOE_ACT_GELU || (moe_act_gated(act) && !pairs) || (pairs && (N % 2 || scale_rows % 2)) || lds < M) return TIB_E_SIZE;
+  if (experts > kB2MaxExperts || (int64_t)experts * ceil_div(N, 128) * ceil_div(K, kBlk) > (0x7fffffff >> 7)) return TIB_E_SIZE;
   if (out_dtype != TIB_BF16 && out_dtype != TIB_F32) return TIB_E_DTYPE;
   if (((uintptr_t)x | (uintptr_t)w) & 15) return TIB_E_ALIGN;
   B2Args a;
-  a.x_scales = x_scales; a.lds = lds; a.w_scales = w_scales; a.scale_rows = pairs ? scale_rows - 1 : scale_rows; a.pairs = pairs;
-  a.M = M; a.N = N; a.runs = ceil_div(K, kBlk); a.error_word = error_word;
+  a.x_scales = x_scales; a.lds = lds; a.w_scales = w_scales; a.scale_rows = scale_rows; a.pairs = pairs;
+  a.M = M; a.N = N; a.runs = ceil_div(K, kBlk); a.offsets = offsets; a.order = order; a.experts = experts; a.error_word = error_word;
+  a.ep.act = act; a.ep.limit = limit; a.ep.alpha = alpha; a.ep.row_scale = row_scale;
   CUtensorMap map_x, map_w;
   int rc = bs_make_map(&map_x, x, M, (int64_t)a.runs * kBlk, 128);
   if (rc != TIB_OK) return rc;
-  rc = bs_make_map(&map_w, w, (int64_t)ceil_div(N, 128) * a.runs * 128, kBlk, 128);
+  rc = bs_make_map(&map_w, w, (int64_t)experts * ceil_div(N, 128) * a.runs * 128, kBlk, 128);
   if (rc != TIB_OK) return rc;
-  if (swiglu)
-    return out_dtype == TIB_BF16 ? launch_b2<true, __nv_bfloat16>(map_x, map_w, a, out, ldo, stream) : launch_b2<true, float>(map_x, map_w, a, out, ldo, stream);
-  return out_dtype == TIB_BF16 ? launch_b2<false, __nv_bfloat16>(map_x, map_w, a, out, ldo, stream) : launch_b2<false, float>(map_x, map_w, a, out, ldo, stream);
+#define TIB_B2_GO(ACT) \
+  case ACT: return out_dtype == TIB_BF16 ? launch_b2<ACT, __nv_bfloat16>(map_x, map_w, a, out, ldo, stream) : launch_b2<ACT, float>(map_x, map_w, a, out, ldo, stream)
+  switch (act) {
+    TIB_B2_GO(MOE_ACT_NONE);
+    TIB_B2_GO(MOE_ACT_RELU2);
+    TIB_B2_GO(MOE_ACT_SILU);
+    TIB_B2_GO(MOE_ACT_GELU);
+    TIB_B2_GO(MOE_ACT_GLU_CLAMP);
+    TIB_B2_GO(MOE_ACT_SWIGLU);
+  }
+#undef TIB_B2_GO
+  return TIB_E_SIZE;
 }

@@ -117,12 +117,8 @@ __device__ __forceinline__ void bs_finish(const float* red, int log_splits, int 
     float out[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if constexpr (ACT == MOE_ACT_SWIGLU) out[j] = v[2 * j] * bs_sigmoid(v[2 * j]) * v[2 * j + 1];
-      else if constexpr (ACT == MOE_ACT_GLU_CLAMP) {
-        const float g = fminf(v[2 * j], a.ep.limit), u = fminf(fmaxf(v[2 * j + 1], -a.ep.limit), a.ep.limit);
-        out[j] = g * bs_sigmoid(a.ep.alpha * g) * (u + 1.f);
-      } else if constexpr (ACT == MOE_ACT_SILU) out[j] = v[j] * bs_sigmoid(v[j]);
-      else out[j] = moe_act(v[j], ACT);
+      if constexpr (kGated) out[j] = bs_gated<ACT>(v[2 * j], v[2 * j + 1], a.ep.limit, a.ep.alpha);
+      else out[j] = bs_act<ACT>(v[j]);
     }
     TO* dst = y + (size_t)(m.first + c) * ldy + first_out + f;
     if (a.wide && first_out + f + 8 <= n_out) {
