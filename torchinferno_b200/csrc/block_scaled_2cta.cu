@@ -247,19 +247,31 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
           *reinterpret_cast<uint4*>(mine + lane * 128 + ((p ^ (lane & 7)) << 4)) = w;
         }
         __syncwarp();
-        const int p = lane & 7, col = first + turn * kTurn + p * kVec;
+        if (wide_stores) {
+          const int p = lane & 7, col = first + turn * kTurn + p * kVec;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = 4 * i + (lane >> 3);
-          const uint4 w = *reinterpret_cast<const uint4*>(mine + r * 128 + ((p ^ (r & 7)) << 4));
-          if (row - lane + r >= last) continue;
-          TO* dst = out + (size_t)(row - lane + r) * ldo + col;
-          if (wide_stores && col + kVec <= n_out) *reinterpret_cast<uint4*>(dst) = w;
-          else {
-            const TO* one = reinterpret_cast<const TO*>(&w);
+          for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + (lane >> 3);
+            const uint4 w = *reinterpret_cast<const uint4*>(mine + r * 128 + ((p ^ (r & 7)) << 4));
+            if (row - lane + r >= last) continue;
+            TO* dst = out + (size_t)(row - lane + r) * ldo + col;
+            if (col + kVec <= n_out) *reinterpret_cast<uint4*>(dst) = w;
+            else {
+              const TO* one = reinterpret_cast<const TO*>(&w);
 #pragma unroll
-            for (int j = 0; j < kVec; ++j)
-              if (col + j < n_out) dst[j] = one[j];
+              for (int j = 0; j < kVec; ++j)
+                if (col + j < n_out) dst[j] = one[j];
+            }
+          }
+        } else {      // (rows that are not 16-byte aligned: consecutive lanes write consecutive outputs of one row)
+#pragma unroll 1
+          for (int r = 0; r < min(32, last - (row - lane)); ++r) {
+#pragma unroll
+            for (int c = lane; c < kTurn; c += 32) {
+              const TO v = *reinterpret_cast<const TO*>(mine + r * 128 + (((c / kVec) ^ (r & 7)) << 4) + (c % kVec) * sizeof(TO));
+              const int col = first + turn * kTurn + c;
+              if (col < n_out) out[(size_t)(row - lane + r) * ldo + col] = v;
+            }
           }
         }
         __syncwarp();

@@ -92,7 +92,26 @@ __device__ __forceinline__ void bs_finish(const float* red, int log_splits, int 
   const int first_out = (m.feature + rank * per) >> kGated, n_out = a.N >> kGated;
 #pragma unroll 1
   for (int i = thread; i < m.rows << log_wide; i += threads) {
-    const int c = i >> log_wide, f = (i - (c << log_wide)) * 8;
+    const int c = i >> log_wide, place = i - (c << log_wide), f = place * 8;
+    if (!a.wide) {
+      // rows that are not 16-byte aligned: a thread's eight outputs lie apart, so that consecutive threads write consecutive ones
+      const float scale = a.ep.row_scale ? a.ep.row_scale[a.order[m.first + c]] : 1.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int o = place + (j << log_wide);
+        const float* from = red + c * stride + (o << kGated);
+        float g = from[0], u = from[kGated];
+        for (int r = 1; r < splits; ++r) {
+          from += NT * stride;
+          g += from[0];
+          u += from[kGated];
+        }
+        g *= scale;
+        if (first_out + o < n_out)
+          y[(size_t)(m.first + c) * ldy + first_out + o] = from_f32<TO>(kGated ? bs_gated<ACT>(g, u * scale, a.ep.limit, a.ep.alpha) : bs_act<ACT>(g));
+      }
+      continue;
+    }
     if (first_out + f >= n_out) continue;
     float v[8 << kGated];
     const float* from = red + c * stride + (f << kGated);
@@ -121,7 +140,7 @@ __device__ __forceinline__ void bs_finish(const float* red, int log_splits, int 
       else out[j] = bs_act<ACT>(v[j]);
     }
     TO* dst = y + (size_t)(m.first + c) * ldy + first_out + f;
-    if (a.wide && first_out + f + 8 <= n_out) {
+    if (first_out + f + 8 <= n_out) {
       if constexpr (sizeof(TO) == 2) {
         __nv_bfloat162 p[4];
 #pragma unroll
@@ -589,13 +608,16 @@ static int launch_block_scaled(const CUtensorMap& map_w, const CUtensorMap& map_
   return TIB_OK;
 }
 
-// The blocks that share a tile's runs: as many as there is room for beside the other tiles', four runs each at least, and eight blocks only for 64 runs.
-// (8 rows, us, by 1 / 2 / 4 / 8 blocks a tile: 4,096 -> 4,096 14.2 / 9.8 / 8.3 / 9.0, 14,336 -> 4,096 43 / 25 / 16.7 / 15.0, 4,096 -> 6,144 14.2 / 10.6 /
-// 9.1 / 14.8, 4,096 -> 14,336 16.3 / 13.6 / 19.0 / 30.4, 2,048 -> 2,048 8.2 / 6.5 / 5.9 / 6.1.)
-static int bs_splits(int64_t tiles, int runs, int blocks) {
-  int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= blocks && runs >= (splits < 4 ? 4 * splits : 64)) splits *= 2;
-  return splits;
+// The blocks that share a tile's runs: 8, 4 or 2 where there is room for them beside the other tiles' and the runs are enough to pay for the exchange.
+// (us by 1 / 2 / 4 / 8 blocks a tile: 8 rows 4,096 -> 4,096 14.2 / 9.8 / 8.3 / 9.0, 14,336 -> 4,096 43 / 25 / 16.7 / 15.0, 4,096 -> 6,144 14.2 / 10.6 /
+// 9.1 / 14.8, 2,048 -> 2,048 8.2 / 6.5 / 5.9 / 6.1; 4 rows 512 -> 1,024 4.0 / 4.5 / 4.3; 20 rows 512 -> 1,024 5.5 / 6.3 / 5.9; in tiles of 128 rows, whose exchange
+// is the largest, 128 rows 4,096 -> 4,096 20 / 17 / 14.8, 256 rows 20.4 / 18.3, 100 rows 2,048 -> 2,048 12.5 / 12.8 / 11.3, 300 rows 13.0 / 13.7, 333 rows
+// 1,024 -> 1,280 9.4 / 11.3 / 11.0.)
+static int bs_splits(int64_t tiles, int runs, int nt) {
+  const int blocks = nt <= 32 ? 296 : 148;
+  if (tiles * 8 <= blocks && runs >= 64) return 8;
+  if (tiles * 4 <= blocks && runs >= (nt < 128 ? 8 : 16)) return 4;
+  return tiles * 2 <= blocks && runs >= (nt < 128 ? 8 : 32) ? 2 : 1;
 }
 
 }  // namespace tib
@@ -635,7 +657,7 @@ TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, in
     if (rc != TIB_OK) return rc;
   }
   const int rows = offsets ? ceil_div(M, experts) : M;      // (of an expert, on average)
-  auto splits = [&](int nt) { return offsets ? 1 : bs_splits((int64_t)ceil_div(M, nt) * ceil_div(N, 128), a.runs, nt <= 32 ? 296 : 148); };
+  auto splits = [&](int nt) { return offsets ? 1 : bs_splits((int64_t)ceil_div(M, nt) * ceil_div(N, 128), a.runs, nt); };
 #define TIB_BS_GO(NT, TX)                                                                                                  \
   return y_dtype == TIB_BF16 ? launch_block_scaled<NT, TX, __nv_bfloat16>(map_w, map_x, a, y, ldy, splits(NT), stream)      \
                              : launch_block_scaled<NT, TX, float>(map_w, map_x, a, y, ldy, splits(NT), stream)
