@@ -314,6 +314,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     }
   } else if (warp == 1) {
     const uint32_t leader = umma_leader();
+    if (!a.offsets) pdl_wait();                   // (the bounded waits begin when the kernel before is over)
     int s = 0, b = 0;
     uint32_t phase = 0, acc_phase = 1;
     bool ok = true;
@@ -552,7 +553,10 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     }
   }
   __syncwarp();
-  if (splits > 1) cluster_sync_all();             // no block leaves while a peer may still write to it
+  if (splits > 1) {
+    cluster_sync_all();                           // every block has sent its sums, also one that gave up waiting for others',
+    if (warp == 0) mbar_wait_warp(red_bar, 0);    // and none leaves before what was sent to it has come
+  }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
   if (warp == 1) {
