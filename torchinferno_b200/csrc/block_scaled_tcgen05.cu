@@ -240,7 +240,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
   const int row_tiles = a.offsets ? tiles_before[a.experts] : (a.M + NT - 1) / NT;
   const int num_tiles = row_tiles * f_tiles;
   auto tile_of = [&](int t) {                     // (feature tiles run fastest: blocks that run together read the same rows)
-    const int row_tile = t / f_tiles;
+    const int row_tile = row_tiles == 1 ? 0 : t / f_tiles;
     BsTile m;
     int begin = 0, n = a.M, tiles = row_tiles, j = row_tile;
     m.expert = 0;
@@ -443,19 +443,21 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     }
   } else {
     // this helper's steps: the first, and every kHelpers-th after it
-    int kb = kb0 + warp - 2 - S::kStorers, s = (warp - 2 - S::kStorers) % a.stages, slot = warp - 2 - S::kStorers;
-    uint32_t phase = 1 ^ (((warp - 2 - S::kStorers) / a.stages) & 1), slot_phase = 1;
-    bool ok = true;
+    const int helper = warp - 2 - S::kStorers;
+    int kb = kb0 + helper, s = helper % a.stages, slot = helper;
+    uint32_t phase = 1 ^ ((helper / a.stages) & 1), slot_phase = 1;
+    bool ok = true, waited = a.offsets != nullptr;
     auto advance = [&]() {
       kb += S::kHelpers;
       for (s += S::kHelpers; s >= a.stages; s -= a.stages) phase ^= 1;
       if ((slot += S::kHelpers) >= kBsSlots) { slot -= kBsSlots; slot_phase ^= 1; }
     };
-    if (!a.offsets) pdl_wait();
     for (int t = cluster_id; t < num_tiles && ok; t += clusters, kb -= kb1 - kb0) {
       const BsTile m = tile_of(t);
       const float* ws = a.w_scales + ((size_t)m.expert * a.scale_rows + bs_scale_row(m.feature, a.pairs)) * a.runs;
       if constexpr (kCodes) {
+        if (!waited) pdl_wait();
+        waited = true;
         // (four of this helper's steps at a time: their loads are on their way together)
         while (kb < kb1 && ok) {
           float v[4][NT / 32], even[4], odd[4];
@@ -486,29 +488,36 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
           }
         }
       } else {
-        // Eight lanes a row, sixteen columns each; two rows a lane at a time, the next two (of this step or this helper's next) on their way.
+        // Eight lanes a row, sixteen columns each; two rows a lane at a time (`turn`: rows 8 half + sub and the fourth after it), the next two (of this
+        // step or this helper's next) on their way.  What the first MMA waits for is this warp's instructions between the kernel before and the first
+        // codes, one behind the other: all that does not need x is done ahead of them.
+        static_assert(NT == 16, "two halves of eight rows");
         const TX* x = reinterpret_cast<const TX*>(a.x);
         const int sub = lane >> 3, eighth = lane & 7;
+        const TX* row[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) row[i] = x + (size_t)source(m, 4 * i + sub) * a.ldx + eighth * 16;
         struct Rows { uint4 raw[2][sizeof(TX)]; float even, odd; };
-        auto ask = [&](Rows& q, int step, int r0) {
+        auto ask = [&](Rows& q, int step, bool half) {
           if (step >= kb1) return;
-          const int col = step * kBlk + eighth * 16;
+          const bool whole = a.vec && (step + 1) * kBlk <= a.K;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int r = r0 + 4 * h + sub;
-            const TX* p = x + (size_t)source(m, r) * a.ldx + min(col, a.K - 1);
-            const int n = r < m.rows ? a.K - col : 0;
-            if (a.vec) bs_ask16<TX, true>(p, n, q.raw[h]);
-            else bs_ask16<TX, false>(p, n, q.raw[h]);
+            const TX* p = (half ? row[2 + h] : row[h]) + step * kBlk;
+            const bool in = (half ? 8 : 0) + 4 * h + sub < m.rows;
+            if (whole) {
+#pragma unroll
+              for (int i = 0; i < (int)sizeof(TX); ++i) q.raw[h][i] = in ? reinterpret_cast<const uint4*>(p)[i] : make_uint4(0, 0, 0, 0);
+            } else bs_ask16<TX, false>(p, in ? a.K - step * kBlk - eighth * 16 : 0, q.raw[h]);
           }
           q.even = ws[step];
           q.odd = a.pairs ? ws[a.runs + step] : q.even;
         };
-        int r0 = 0;
+        bool half = false;
         auto turn = [&](Rows& now, Rows& next) {
-          const bool last = r0 + 8 >= m.rows;
-          ask(next, last ? kb + S::kHelpers : kb, last ? 0 : r0 + 8);
-          if (r0 == 0 && !(mbar_wait_warp(empty_bar(s), phase) && mbar_wait_warp(scale_empty_bar(slot), slot_phase))) {
+          const bool last = half || m.rows <= 8;
+          ask(next, last ? kb + S::kHelpers : kb, !last);
+          if (!half && !(mbar_wait_warp(empty_bar(s), phase) && mbar_wait_warp(scale_empty_bar(slot), slot_phase))) {
             ok = false;
             return;
           }
@@ -516,7 +525,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
           unsigned char* codes = smem_gen + s * S::kStage + kBsWBytes;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int r = r0 + 4 * h + sub;
+            const int r = (half ? 8 : 0) + 4 * h + sub;
             uint32_t largest = bs_largest16<TX>(now.raw[h]);
 #pragma unroll
             for (int o = 1; o < 8; o <<= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
@@ -538,11 +547,13 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
               mbar_arrive(full_bar(s));
             }
             advance();
-            r0 = 0;
-          } else r0 += 8;
+          }
+          half = !last;
         };
         Rows p, q;
-        ask(p, kb, 0);
+        if (!waited) pdl_wait();
+        waited = true;
+        ask(p, kb, false);
         while (kb < kb1 && ok) {
           turn(p, q);
           if (kb < kb1 && ok) turn(q, p);
