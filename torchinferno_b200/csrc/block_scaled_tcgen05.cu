@@ -90,15 +90,17 @@ __device__ __forceinline__ void bs_finish(const float* red, int log_splits, int 
   const int per = 128 >> log_splits, stride = per + 4, splits = 1 << log_splits;
   const int log_wide = 4 - log_splits - kGated;           // eights of outputs in a column
   const int first_out = (m.feature + rank * per) >> kGated, n_out = a.N >> kGated;
+  if (!a.wide) {
+    // Rows of y that are not 16-byte aligned: a warp takes a row, its lanes consecutive outputs.
+    const int lane = thread & 31, outs = per >> kGated;
 #pragma unroll 1
-  for (int i = thread; i < m.rows << log_wide; i += threads) {
-    const int c = i >> log_wide, place = i - (c << log_wide), f = place * 8;
-    if (!a.wide) {
-      // rows that are not 16-byte aligned: a thread's eight outputs lie apart, so that consecutive threads write consecutive ones
+    for (int c = thread >> 5; c < m.rows; c += threads >> 5) {
       const float scale = a.ep.row_scale ? a.ep.row_scale[a.order[m.first + c]] : 1.f;
+      TO* dst = y + (size_t)(m.first + c) * ldy + first_out;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int o = place + (j << log_wide);
+      for (int j = 0; j < 4 >> kGated; ++j) {
+        const int o = 32 * j + lane;
+        if (o >= outs) break;
         const float* from = red + c * stride + (o << kGated);
         float g = from[0], u = from[kGated];
         for (int r = 1; r < splits; ++r) {
@@ -107,11 +109,14 @@ __device__ __forceinline__ void bs_finish(const float* red, int log_splits, int 
           u += from[kGated];
         }
         g *= scale;
-        if (first_out + o < n_out)
-          y[(size_t)(m.first + c) * ldy + first_out + o] = from_f32<TO>(kGated ? bs_gated<ACT>(g, u * scale, a.ep.limit, a.ep.alpha) : bs_act<ACT>(g));
+        if (first_out + o < n_out) dst[o] = from_f32<TO>(kGated ? bs_gated<ACT>(g, u * scale, a.ep.limit, a.ep.alpha) : bs_act<ACT>(g));
       }
-      continue;
     }
+    return;
+  }
+#pragma unroll 1
+  for (int i = thread; i < m.rows << log_wide; i += threads) {
+    const int c = i >> log_wide, f = (i - (c << log_wide)) * 8;
     if (first_out + f >= n_out) continue;
     float v[8 << kGated];
     const float* from = red + c * stride + (f << kGated);
@@ -174,9 +179,9 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
   auto acc_full_bar = [&](int b) { return bars + 8u * (2 * kBsMaxStages + b); };
   auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * kBsMaxStages + S::kBufs + b); };
   auto scale_full_bar = [&](int i) { return bars + 8u * (2 * kBsMaxStages + 2 * S::kBufs + i); };
-  auto scale_empty_bar = [&](int i) { return bars + 8u * (2 * kBsMaxStages + 2 * S::kBufs + kBsSlots + i); };
-  const uint32_t red_bar = bars + 8u * (2 * kBsMaxStages + 2 * S::kBufs + 2 * kBsSlots), tmem_slot = red_bar + 8;
-  static_assert(8 * (2 * kBsMaxStages + 2 * S::kBufs + 2 * kBsSlots) + 16 <= kBsBarBytes, "the barriers' share of shared memory");
+  auto scale_empty_bar = [&](int slot) { return bars + 8u * (2 * kBsMaxStages + 2 * S::kBufs + kBsSlots + slot / 4); };      // (four slots are freed together)
+  const uint32_t red_bar = bars + 8u * (2 * kBsMaxStages + 2 * S::kBufs + kBsSlots + kBsSlots / 4), tmem_slot = red_bar + 8;
+  static_assert(8 * (2 * kBsMaxStages + 2 * S::kBufs + kBsSlots + kBsSlots / 4) + 16 <= kBsBarBytes, "the barriers' share of shared memory");
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem_gen + (tmem_slot - base));
   float* step_scales = reinterpret_cast<float*>(smem_gen + (bars - base) + kBsBarBytes);  // [kBsSlots][kScales]
   float* red = step_scales + kBsSlots * S::kScales;                                       // [splits][NT][128 / splits + 4] sums
@@ -195,10 +200,8 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
       mbar_init(full_bar(lane), kCodes ? 1 : 2);  // the producer, and the helper that makes codes
       mbar_init(empty_bar(lane), 1);
     }
-    if (lane < kBsSlots) {
-      mbar_init(scale_full_bar(lane), 1);
-      mbar_init(scale_empty_bar(lane), S::kStorers);
-    }
+    if (lane < kBsSlots) mbar_init(scale_full_bar(lane), 1);
+    if (lane < kBsSlots / 4) mbar_init(scale_empty_bar(4 * lane), S::kStorers);
     if (lane < S::kBufs) {
       mbar_init(acc_full_bar(lane), 1);
       mbar_init(acc_empty_bar(lane), S::kStorers);
@@ -359,38 +362,57 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
       f32x2 sum[2][S::kCols / 4];
 #pragma unroll
       for (int c = 0; c < S::kCols / 4; ++c) sum[0][c] = sum[1][c] = f2_pack(0.f, 0.f);
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (ok && !(mbar_wait_warp(scale_full_bar(slot), slot_phase) && mbar_wait_warp(acc_full_bar(b), acc_phase))) {
-          if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00C3);
+      f32x2 scale[S::kCols / 8];
+      auto wait_scales = [&]() {
+        if (ok && !mbar_wait_warp(scale_full_bar(slot), slot_phase)) {
+          if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00C7);
           ok = false;
         }
-        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+      };
+      auto read_scales = [&]() {
+        const float* from = step_scales + slot * S::kScales + (lane8 & 1) * (NT + 8) + c0 + pair;
+#pragma unroll
+        for (int j = 0; j < S::kCols / 8; ++j) scale[j] = *reinterpret_cast<const f32x2*>(from + 8 * j);
+      };
+      for (int kb = kb0; kb < kb1; ++kb) {
         const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + b * NT + c0;
-        const float* scales = step_scales + slot * S::kScales + (lane8 & 1) * (NT + 8) + c0 + pair;
         uint32_t v[2][S::kCols / 2];
-        tmem_ld_16x256b<S::kCols>(acc, v[0]);
-        f32x2 scale[S::kCols / 8];
-#pragma unroll
-        for (int j = 0; j < S::kCols / 8; ++j) scale[j] = *reinterpret_cast<const f32x2*>(scales + 8 * j);
-        asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-        tmem_ld_16x256b<S::kCols>(acc + (16u << 16), v[1]);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (h) {
-            asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-            asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-            __syncwarp();
-            if (lane == 0) {
-              mbar_arrive(acc_empty_bar(b));
-              mbar_arrive(scale_empty_bar(slot));
-            }
-          }
+        auto add = [&](int h) {
 #pragma unroll
           for (int j = 0; j < S::kCols / 8; ++j)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
               sum[h][2 * j + i] = f2_fma(f2_pack(__uint_as_float(v[h][4 * j + 2 * i]), __uint_as_float(v[h][4 * j + 2 * i + 1])), scale[j], sum[h][2 * j + i]);
+        };
+        // What bounds tiles of up to 64 rows is this loop's latency: both loads are on their way while the scales are waited for and read (of 32 and 64
+        // rows, 112 steps: 38.2 and 37.3 us; waited for ahead of one load after the other 38.8 and 42.0).  Of 128 rows it is shared memory, and the first
+        // load's sums are added under the second (55.3 us, 67.0 the other way).
+        if constexpr (NT >= 128) wait_scales();
+        if (ok && !mbar_wait_warp(acc_full_bar(b), acc_phase)) {
+          if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00C3);
+          ok = false;
         }
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        tmem_ld_16x256b<S::kCols>(acc, v[0]);
+        if constexpr (NT >= 128) {
+          read_scales();
+          asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+          tmem_ld_16x256b<S::kCols>(acc + (16u << 16), v[1]);
+          add(0);
+        } else {
+          tmem_ld_16x256b<S::kCols>(acc + (16u << 16), v[1]);
+          wait_scales();
+          read_scales();
+        }
+        asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(acc_empty_bar(b));
+          if ((slot & 3) == 3) mbar_arrive(scale_empty_bar(slot));      // (this step's scales have been read, and those of the three before)
+        }
+        if constexpr (NT < 128) add(0);
+        add(1);
         if (++slot == kBsSlots) { slot = 0; slot_phase ^= 1; }
         if (++b == S::kBufs) { b = 0; acc_phase ^= 1; }
       }
@@ -444,11 +466,12 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
   } else {
     // this helper's steps: the first, and every kHelpers-th after it
     const int helper = warp - 2 - S::kStorers;
-    int kb = kb0 + helper, s = helper % a.stages, slot = helper;
+    int kb = kb0 + helper, step = helper, s = helper % a.stages, slot = helper;      // (step: counted over all tiles)
     uint32_t phase = 1 ^ ((helper / a.stages) & 1), slot_phase = 1;
     bool ok = true, waited = a.offsets != nullptr;
     auto advance = [&]() {
       kb += S::kHelpers;
+      step += S::kHelpers;
       for (s += S::kHelpers; s >= a.stages; s -= a.stages) phase ^= 1;
       if ((slot += S::kHelpers) >= kBsSlots) { slot -= kBsSlots; slot_phase ^= 1; }
     };
@@ -498,26 +521,26 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
 #pragma unroll
         for (int i = 0; i < 4; ++i) row[i] = x + (size_t)source(m, 4 * i + sub) * a.ldx + eighth * 16;
         struct Rows { uint4 raw[2][sizeof(TX)]; float even, odd; };
-        auto ask = [&](Rows& q, int step, bool half) {
-          if (step >= kb1) return;
-          const bool whole = a.vec && (step + 1) * kBlk <= a.K;
+        auto ask = [&](Rows& q, int run, bool half) {
+          if (run >= kb1) return;
+          const bool whole = a.vec && (run + 1) * kBlk <= a.K;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const TX* p = (half ? row[2 + h] : row[h]) + step * kBlk;
+            const TX* p = (half ? row[2 + h] : row[h]) + run * kBlk;
             const bool in = (half ? 8 : 0) + 4 * h + sub < m.rows;
             if (whole) {
 #pragma unroll
               for (int i = 0; i < (int)sizeof(TX); ++i) q.raw[h][i] = in ? reinterpret_cast<const uint4*>(p)[i] : make_uint4(0, 0, 0, 0);
-            } else bs_ask16<TX, false>(p, in ? a.K - step * kBlk - eighth * 16 : 0, q.raw[h]);
+            } else bs_ask16<TX, false>(p, in ? a.K - run * kBlk - eighth * 16 : 0, q.raw[h]);
           }
-          q.even = ws[step];
-          q.odd = a.pairs ? ws[a.runs + step] : q.even;
+          q.even = ws[run];
+          q.odd = a.pairs ? ws[a.runs + run] : q.even;
         };
         bool half = false;
         auto turn = [&](Rows& now, Rows& next) {
           const bool last = half || m.rows <= 8;
           ask(next, last ? kb + S::kHelpers : kb, !last);
-          if (!half && !(mbar_wait_warp(empty_bar(s), phase) && mbar_wait_warp(scale_empty_bar(slot), slot_phase))) {
+          if (!half && ((step >= a.stages && !mbar_wait_warp(empty_bar(s), phase)) || (step >= kBsSlots && !mbar_wait_warp(scale_empty_bar(slot), slot_phase)))) {
             ok = false;
             return;
           }
@@ -626,13 +649,20 @@ static int launch_block_scaled(const CUtensorMap& map_w, const CUtensorMap& map_
 // The blocks that share a tile's runs: 8, 4 or 2 where there is room for them beside the other tiles' and the runs are enough to pay for the exchange.
 // (us by 1 / 2 / 4 / 8 blocks a tile: 8 rows 4,096 -> 4,096 14.2 / 9.8 / 8.3 / 9.0, 14,336 -> 4,096 43 / 25 / 16.7 / 15.0, 4,096 -> 6,144 14.2 / 10.6 /
 // 9.1 / 14.8, 2,048 -> 2,048 8.2 / 6.5 / 5.9 / 6.1; 4 rows 512 -> 1,024 4.0 / 4.5 / 4.3; 20 rows 512 -> 1,024 5.5 / 6.3 / 5.9; in tiles of 128 rows, whose exchange
-// is the largest, 128 rows 4,096 -> 4,096 20 / 17 / 14.8, 256 rows 20.4 / 18.3, 100 rows 2,048 -> 2,048 12.5 / 12.8 / 11.3, 300 rows 13.0 / 13.7, 333 rows
-// 1,024 -> 1,280 9.4 / 11.3 / 11.0.)
-static int bs_splits(int64_t tiles, int runs, int nt) {
-  const int blocks = nt <= 32 ? 296 : 148;
+// is the largest, 128 rows 4,096 -> 4,096 20 / 17 / 14.8, 100 rows 2,048 -> 2,048 12.5 / 12.8 / 11.3, 300 rows 13.0 / 13.7.)
+static int bs_splits(int64_t tiles, int runs, int nt, int blocks) {
   if (tiles * 8 <= blocks && runs >= 64) return 8;
   if (tiles * 4 <= blocks && runs >= (nt < 128 ? 8 : 16)) return 4;
   return tiles * 2 <= blocks && runs >= (nt < 128 ? 8 : 32) ? 2 : 1;
+}
+// Rows of a tile of codes: the fewest that give no more tiles than SMs; of a long matrix (64 runs) not fewer than 64 while there are that many rows, as every row tile
+// reads the weights again.  (us in tiles of 32 / 64 / 128 rows: 333 rows 1,000 -> 1,302 8.2 / 9.5 / 11.4, 128 rows 4,096 -> 4,096 13.7 / 14.1 / 15.6, 256 rows
+// 18.0 / 16.7 / 20.0, 100 rows 2,048 -> 2,048 8.9 / 10.2 / 11.8, 64 rows 14,336 -> 4,096 19.2 / 18.1 / 25.5, 128 rows 28.1 / 26.1 / 26.3, 128 rows 4,096 ->
+// 14,336 29.2 / 27.9 / 24.9.)
+static int bs_tile_rows(int rows, int features, int runs) {
+  const int64_t f_tiles = ceil_div(features, 128);
+  if (rows <= 32 || (ceil_div(rows, 32) * f_tiles <= 148 && runs < 64)) return 32;
+  return rows <= 64 || ceil_div(rows, 64) * f_tiles <= 148 ? 64 : 128;
 }
 
 }  // namespace tib
@@ -671,14 +701,16 @@ TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, in
     rc = bs_make_map(&map_x, x, x_rows, (int64_t)a.runs * kBlk, 32);
     if (rc != TIB_OK) return rc;
   }
-  const int rows = offsets ? ceil_div(M, experts) : M;      // (of an expert, on average)
-  auto splits = [&](int nt) { return offsets ? 1 : bs_splits((int64_t)ceil_div(M, nt) * ceil_div(N, 128), a.runs, nt); };
+  auto splits = [&](int nt) { return offsets ? 1 : bs_splits((int64_t)ceil_div(M, nt) * ceil_div(N, 128), a.runs, nt, is_codes ? 148 : 296); };
 #define TIB_BS_GO(NT, TX)                                                                                                  \
   return y_dtype == TIB_BF16 ? launch_block_scaled<NT, TX, __nv_bfloat16>(map_w, map_x, a, y, ldy, splits(NT), stream)      \
                              : launch_block_scaled<NT, TX, float>(map_w, map_x, a, y, ldy, splits(NT), stream)
   if (is_codes) {
-    if (rows <= 32) TIB_BS_GO(32, uint8_t);
-    if (rows <= 64) TIB_BS_GO(64, uint8_t);
+    // (Of sorted rows tiles of 32 are ahead, or near, up to where pairs of SMs take over.  32 / 64 / 128 rows a tile, us: 25 rows an expert 19.5 / 18.5 / 24.3, 50
+    // 21.5 / 25.0 / 25.6, 87 30.7 / 33.1 / 35.5, 32 of 28 experts 17.4 / 20.0 / 23.6; with a skew 16.2 / 16.2 / 20.7.)
+    const int nt = !offsets ? bs_tile_rows(M, N, a.runs) : M < (int64_t)experts * 128 ? 32 : 128;
+    if (nt == 32) TIB_BS_GO(32, uint8_t);
+    if (nt == 64) TIB_BS_GO(64, uint8_t);
     TIB_BS_GO(128, uint8_t);
   }
   if (x_dtype == TIB_BF16) TIB_BS_GO(16, __nv_bfloat16);

@@ -100,8 +100,7 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     columns = x.shape[1]
     runs, lds = blocks(columns), (rows + 3) & ~3
     codes = x.new_empty((rows, runs * BLOCK), dtype=CODE_DTYPE)
-    scales = torch.empty_strided((rows, runs), (1, lds), dtype=torch.float32, device=x.device) if lds == rows else \
-        torch.empty_strided((lds, runs), (1, lds), dtype=torch.float32, device=x.device)[:rows]
+    scales = torch.empty_strided((rows, runs), (1, lds), dtype=torch.float32, device=x.device)
     ops.quantize_rows(x, codes.data_ptr(), scales.data_ptr(), lds)
     return codes if columns == runs * BLOCK else codes[:, :columns], scales
 
