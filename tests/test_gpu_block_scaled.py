@@ -287,6 +287,30 @@ def test_expert_products(tokens, top, experts, k, n, out_dtype, by_pair, act):
         check(y[at], want, out_dtype, f"expert {e}")
 
 
+@pytest.mark.parametrize("act", ["none", "relu2", "silu", "gelu", "swiglu", "glu_clamp"])
+@pytest.mark.parametrize("tokens", [4, 60, 400])
+def test_rows_that_are_not_finite_show_through_every_activation(tokens, act):
+    need_gpu()
+    stacks = [[random_matrix(140, 200, 100 * part + e, DEV, (0.005, 0.2)) for e in range(2)] for part in range(2 if act in ops.MOE_GATED else 1)]
+    offsets, order, _ = routing(tokens, 1, 2, tokens)
+    x = rows(tokens, 200, tokens, spread=0.5)
+    x[1, 7], x[2, 150] = float("nan"), float("inf")
+    y = torch.empty(tokens, 140, dtype=BF16, device=DEV)
+    ops.moe_expert_product(x, BlockScaledExperts(*stacks), y, offsets, order, 1, x_by_pair=True, act=act, limit=2.0, alpha=1.702)
+    bad = ((order == 1) | (order == 2))
+    assert y[bad].isnan().all() and not y[~bad].isnan().any()
+
+
+def test_matrices_of_any_stride():
+    need_gpu()
+    wide = random_matrix(256, 512, 3, DEV)
+    part = BlockScaledMatrix(wide.codes[:, 128:384], wide.scales[:, 1:3])
+    turned = BlockScaledMatrix(wide.codes.view(torch.uint8)[:, :256].t().view(torch.float8_e4m3fn), wide.scales[:, :2].t())
+    x = rows(5, 256, 1)
+    for matrix in (part, turned):
+        check(gemm.linear(x, BlockScaledWeight(matrix)), product64(x, matrix), BF16)
+
+
 def test_expert_refusals():
     need_gpu()
     experts = BlockScaledExperts([random_matrix(64, 100, i, DEV) for i in range(4)])

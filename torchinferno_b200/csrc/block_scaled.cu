@@ -11,14 +11,14 @@ namespace tib {
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
 quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scales,
-                     int64_t lds, int rows, int K, int runs, const int* __restrict__ order, int top, const int* __restrict__ sorted) {
+                     int64_t lds, int rows, int K, int runs, const int* __restrict__ order, int top, const int* __restrict__ sorted, int x_rows) {
   pdl_wait();
   pdl_trigger();
   // thread = (row of 8, run of 4, eighth of the run)
   const int groups = (runs + 3) >> 2, row8 = blockIdx.x / groups;
   const int eighth = threadIdx.x & 7, row = row8 * 8 + (threadIdx.x >> 5), run = (blockIdx.x - row8 * groups) * 4 + ((threadIdx.x >> 3) & 3);
   const bool in = row < (order ? min(rows, *sorted) : rows) && run < runs;
-  const int col = run * kBlk + eighth * 16, from = !in ? 0 : order ? order[row] / top : row;
+  const int col = run * kBlk + eighth * 16, from = !in ? 0 : order ? min(bs_pair(order, row, rows) / top, x_rows - 1) : row;
   uint4 raw[sizeof(T)];
   bs_ask16<T, VEC>(x + (size_t)from * ldx + (in ? col : 0), in ? K - col : 0, raw);
   uint32_t largest = bs_largest16<T>(raw);
@@ -35,12 +35,12 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__
 
 using namespace tib;
 
-// x: rows [rows, K] in x_dtype (row stride ldx); codes: [rows, ldc], ldc = K rounded up to 128, behind column K zeros; scales:
+// x: rows [x_rows, K] in x_dtype (row stride ldx); codes: [rows, ldc], ldc = K rounded up to 128, behind column K zeros; scales:
 // [runs of 128 columns, lds], lds at least rows.  order [rows]: row r is made of row order[r] / top of x, for the first *sorted rows; null: of row r.
 TIB_API int tib_quantize_rows(const void* x, int x_dtype, int64_t ldx, void* codes, int64_t ldc, float* scales, int64_t lds, int rows,
-                              int K, const int* order, int top, const int* sorted, cudaStream_t stream) {
+                              int K, const int* order, int top, const int* sorted, int x_rows, cudaStream_t stream) {
   if (rows == 0) return TIB_OK;
-  if (!x || !codes || !scales || rows < 0 || K < 1 || (order && (top < 1 || !sorted))) return TIB_E_ARG;
+  if (!x || !codes || !scales || rows < 0 || K < 1 || (order ? top < 1 || !sorted || x_rows < 1 : x_rows < rows)) return TIB_E_ARG;
   if (x_dtype != TIB_BF16 && x_dtype != TIB_F32) return TIB_E_DTYPE;
   const int runs = ceil_div(K, kBlk);
   if (ldc < (int64_t)runs * kBlk || lds < rows) return TIB_E_SIZE;
@@ -49,7 +49,7 @@ TIB_API int tib_quantize_rows(const void* x, int x_dtype, int64_t ldx, void* cod
   if (grid > 0x7fffffff) return TIB_E_SIZE;
   const bool vec = ((uintptr_t)x & 15) == 0 && (ldx * (x_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
 #define TIB_QUANT_GO(T, VEC) \
-  TIB_LAUNCH_DEPENDENT((quantize_rows_kernel<T, VEC>), (unsigned)grid, 256, 0, stream, (const T*)x, ldx, (uint8_t*)codes, ldc, scales, lds, rows, K, runs, order, top, sorted)
+  TIB_LAUNCH_DEPENDENT((quantize_rows_kernel<T, VEC>), (unsigned)grid, 256, 0, stream, (const T*)x, ldx, (uint8_t*)codes, ldc, scales, lds, rows, K, runs, order, top, sorted, x_rows)
   if (x_dtype == TIB_BF16) {
     if (vec) TIB_QUANT_GO(__nv_bfloat16, true);
     else TIB_QUANT_GO(__nv_bfloat16, false);
@@ -88,7 +88,7 @@ TIB_API int tib_block_scaled_product(const void* x, int x_dtype, int64_t ldx, in
   if (make) {
     const bool gather = offsets && x_by_pair;      // (the pairs' rows, sorted on the way)
     const int rc = tib_quantize_rows(x, x_dtype, ldx, codes, (int64_t)runs * kBlk, scales, lds, M, K, gather ? order : nullptr, top,
-                                     gather ? offsets + experts : nullptr, stream);
+                                     gather ? offsets + experts : nullptr, x_rows, stream);
     if (rc != TIB_OK) return rc;
   }
   if (offsets ? M >= (int64_t)experts * kBsPairRows && experts <= tib_block_scaled_2cta_experts() : on_pairs_of_sms(M, N))

@@ -38,14 +38,22 @@ __device__ __forceinline__ float bs_sigmoid(float x) {
   return r;
 }
 
-// The experts' activations (moe.cuh) with this sigmoid.
-template <int ACT> __device__ __forceinline__ float bs_act(float v) { return ACT == MOE_ACT_SILU ? v * bs_sigmoid(v) : moe_act(v, ACT); }
+// The experts' activations (moe.cuh) with this sigmoid; a NaN stays one (a minimum or maximum of floats would pass over it).
+template <int ACT> __device__ __forceinline__ float bs_act(float v) {
+  if (ACT == MOE_ACT_RELU2) return v < 0.f ? 0.f : v * v;
+  if (ACT == MOE_ACT_SILU) return v * bs_sigmoid(v);
+  return ACT == MOE_ACT_GELU ? gelu_erf(v) : v;
+}
 template <int ACT> __device__ __forceinline__ float bs_gated(float g, float u, float limit, float alpha) {
   if (ACT == MOE_ACT_SWIGLU) return g * bs_sigmoid(g) * u;
-  g = fminf(g, limit);
-  u = fminf(fmaxf(u, -limit), limit);
+  g = g > limit ? limit : g;
+  u = u > limit ? limit : u < -limit ? -limit : u;
   return g * bs_sigmoid(alpha * g) * (u + 1.f);
 }
+
+// Rows sorted by expert, kept within what there is: expert e's first row and the one behind its last, and the pair that sorted row `at` is.
+__device__ __forceinline__ int bs_offset(const int* __restrict__ offsets, int e, int M) { return min(max(offsets[e], 0), M); }
+__device__ __forceinline__ int bs_pair(const int* __restrict__ order, int at, int M) { return min(max(order[at], 0), M - 1); }
 
 // two floats to two codes (the first in the lower byte), to nearest, ties to even; a NaN stays one
 __device__ __forceinline__ uint32_t bs_codes2(float lo, float hi) {
@@ -131,7 +139,7 @@ static inline int bs_make_map(CUtensorMap* map, const void* ptr, int64_t rows, i
 // What a product of block-scaled operands is made of (block_scaled.cu, block_scaled_tcgen05.cu, block_scaled_2cta.cu).
 extern "C" {
 int tib_quantize_rows(const void* x, int x_dtype, int64_t ldx, void* codes, int64_t ldc, float* scales, int64_t lds, int rows, int K,
-                      const int* order, int top, const int* sorted, cudaStream_t stream);
+                      const int* order, int top, const int* sorted, int x_rows, cudaStream_t stream);
 int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, int x_rows, const float* x_scales, int64_t lds, const void* w,
                              const float* w_scales, int scale_rows, int pairs, void* y, int y_dtype, int64_t ldy, int M, int N, int K,
                              const int* offsets, const int* order, int experts, int top, int x_by_pair, int act, float limit, float alpha,

@@ -112,7 +112,8 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
   if (a.offsets && warp == 0) {                            // the experts' row tiles, summed
     int before = 0;
     for (int e0 = 0; e0 < a.experts; e0 += 32) {
-      const int e = e0 + lane, begin = e < a.experts ? a.offsets[e] : 0, end = e < a.experts ? a.offsets[e + 1] : 0;
+      const int e = e0 + lane, begin = e < a.experts ? bs_offset(a.offsets, e, a.M) : 0;
+      const int end = e < a.experts ? max(begin, bs_offset(a.offsets, e + 1, a.M)) : 0;
       int sum = (end - begin + 255) >> 8;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -122,7 +123,7 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
       if (e < a.experts) tiles_before[e + 1] = before + sum, first_row[e + 1] = end;
       before += __shfl_sync(0xffffffffu, sum, 31);
     }
-    if (lane == 0) tiles_before[0] = 0, first_row[0] = a.offsets[0];
+    if (lane == 0) tiles_before[0] = 0, first_row[0] = bs_offset(a.offsets, 0, a.M);
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
@@ -212,7 +213,7 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
       }
       if (!ok) continue;
       if (a.ep.row_scale) {
-        const float scale = a.ep.row_scale[a.order[min(row, last - 1)]];
+        const float scale = a.ep.row_scale[bs_pair(a.order, min(row, last - 1), a.M)];
         const f32x2 scale2 = f2_pack(scale, scale);
 #pragma unroll
         for (int c = 0; c < 64; ++c) sum[c] = f2_mul(sum[c], scale2);

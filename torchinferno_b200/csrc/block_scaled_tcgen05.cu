@@ -48,7 +48,7 @@ struct BsArgs {
   int64_t lds;
   const float* w_scales;       // [experts, scale_rows, runs]
   int scale_rows, pairs, vec, wide;      // vec: rows of x, wide: of y, are 16-byte aligned
-  int M, N, K, runs, stages;
+  int M, N, K, runs, x_rows, stages;
   const int* offsets;          // null: one matrix
   const int* order;
   int experts, top, x_by_pair;
@@ -95,7 +95,7 @@ __device__ __forceinline__ void bs_finish(const float* red, int log_splits, int 
     const int lane = thread & 31, outs = per >> kGated;
 #pragma unroll 1
     for (int c = thread >> 5; c < m.rows; c += threads >> 5) {
-      const float scale = a.ep.row_scale ? a.ep.row_scale[a.order[m.first + c]] : 1.f;
+      const float scale = a.ep.row_scale ? a.ep.row_scale[bs_pair(a.order, m.first + c, a.M)] : 1.f;
       TO* dst = y + (size_t)(m.first + c) * ldy + first_out;
 #pragma unroll
       for (int j = 0; j < 4 >> kGated; ++j) {
@@ -134,7 +134,7 @@ __device__ __forceinline__ void bs_finish(const float* red, int log_splits, int 
       }
     }
     if (a.ep.row_scale) {
-      const float scale = a.ep.row_scale[a.order[m.first + c]];
+      const float scale = a.ep.row_scale[bs_pair(a.order, m.first + c, a.M)];
 #pragma unroll
       for (int j = 0; j < 8 << kGated; ++j) v[j] *= scale;
     }
@@ -218,7 +218,8 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     if (warp == 0) {      // the experts' row tiles, summed
       int before = 0;
       for (int e0 = 0; e0 < a.experts; e0 += 32) {
-        const int e = e0 + lane, begin = e < a.experts ? a.offsets[e] : 0, end = e < a.experts ? a.offsets[e + 1] : 0;
+        const int e = e0 + lane, begin = e < a.experts ? bs_offset(a.offsets, e, a.M) : 0;
+        const int end = e < a.experts ? max(begin, bs_offset(a.offsets, e + 1, a.M)) : 0;
         int sum = (end - begin + NT - 1) / NT;
         if (e < a.experts) first_row[e + 1] = end;
 #pragma unroll
@@ -229,7 +230,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
         if (e < a.experts) tiles_before[e + 1] = before + sum;
         before += __shfl_sync(0xffffffffu, sum, 31);
       }
-      if (lane == 0) tiles_before[0] = 0, first_row[0] = a.offsets[0];
+      if (lane == 0) tiles_before[0] = 0, first_row[0] = bs_offset(a.offsets, 0, a.M);
     }
   }
   pdl_trigger();
@@ -268,7 +269,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
   auto w_row = [&](const BsTile& m, int kb) { return ((m.expert * f_tiles + (m.feature >> 7)) * a.runs + kb) << 7; };      // of the tile's block in the matrix of blocks
   auto source = [&](const BsTile& m, int r) {     // the row of x that the tile's row r is
     const int at = m.first + min(r, m.rows - 1);
-    return a.offsets && a.x_by_pair ? a.order[at] / a.top : at;
+    return a.offsets && a.x_by_pair ? min(bs_pair(a.order, at, a.M) / a.top, a.x_rows - 1) : at;
   };
 
   if (warp == 0) {
@@ -690,7 +691,7 @@ TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, in
   a.x = x; a.ldx = ldx; a.x_scales = x_scales; a.lds = lds; a.w_scales = w_scales; a.scale_rows = scale_rows; a.pairs = pairs;
   a.vec = !is_codes && ((uintptr_t)x & 15) == 0 && (ldx * (x_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
   a.wide = ((uintptr_t)y & 15) == 0 && (ldy * (y_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
-  a.M = M; a.N = N; a.K = K; a.runs = ceil_div(K, kBlk); a.offsets = offsets; a.order = order; a.experts = experts; a.top = top;
+  a.M = M; a.N = N; a.K = K; a.x_rows = x_rows; a.runs = ceil_div(K, kBlk); a.offsets = offsets; a.order = order; a.experts = experts; a.top = top;
   a.x_by_pair = x_by_pair; a.error_word = error_word;
   a.ep.act = act; a.ep.limit = limit; a.ep.alpha = alpha; a.ep.row_scale = row_scale;
   CUtensorMap map_w, map_x;

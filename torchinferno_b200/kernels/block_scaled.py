@@ -144,7 +144,7 @@ def _laid_out(matrices: Sequence[BlockScaledMatrix], ups: Sequence[BlockScaledMa
             stored = m.codes.view(torch.uint8)
             if any(pad):
                 stored = torch.nn.functional.pad(stored, pad)
-            codes[i, :, :, :, part].copy_(stored.view(tiles, each, runs, BLOCK).transpose(1, 2))
+            codes[i, :, :, :, part].copy_(stored.reshape(tiles, each, runs, BLOCK).transpose(1, 2))
             scales[i, :, part].copy_(m.scales)
     return Blocks(codes.view(len(matrices), tiles, runs, BLOCK, BLOCK).view(CODE_DTYPE), scales.view(len(matrices), blocks(n) * parts, -1), n * parts, k,
                   ups is not None)

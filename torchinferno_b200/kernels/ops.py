@@ -1260,7 +1260,7 @@ def quantize_rows(x: torch.Tensor, codes: int, scales: int, lds: int) -> None:
     """Codes [rows, columns rounded up to 128] (8 bits) and scales [runs of 128 columns, ``lds``] of the rows ``x``, to these addresses."""
     rows, columns = x.shape
     _check("quantize_rows", lib().tib_quantize_rows(x.data_ptr(), _code(x.dtype), x.stride(0), codes, -(-columns // 128) * 128, scales, lds, rows, columns,
-                                                    0, 1, 0, _stream()))
+                                                    0, 1, 0, rows, _stream()))
 
 
 def block_scaled_product(x: torch.Tensor, codes: int, make: bool, blocks, y: torch.Tensor, act: str, limit: float, alpha: float, offsets: int, order: int,
