@@ -11,7 +11,10 @@
 //   warp 0       TMA producer into a ring of six stages      warp 1 (of the even block)   issues the MMAs; either owns its block's TMEM
 //   warps 4..11  sums, then the epilogue with its activation.  These take registers that the first four warps give up (168 a thread at launch,
 //                40 + 2 x 232 after)
-// For a step the tensor cores need 512 cycles at their peak, the sums 256 of the tensor memory's reads and 256 of the fp32 pipe.
+// What bounds it: shared memory.  A step's MMAs read 64 KB of operands from it while 32 KB of the next step's arrive: without the sums a step takes 700 cycles, with
+// them 800 (the tensor cores' own time is 537, the sums alone take 340).  8,192 rows 4,096 -> 2 x 14,336 with silu(gate) * up: 0.90 ms, 2,140 TFLOP/s (1.03 ms,
+// 1,870 under the power limit); 2,048 rows 4,096 -> 6,144 with its codes 59 us, 1,740, a third round of tiles included that is 0.6 full.  Tried: pieces of 32 columns
+// (the scales' registers spilled, and every step waited for their loads: 1.10 ms), waits by polling without a time hint (no gain).
 // Every wait is bounded and reports in error_word; no block leaves before its partner is done; every copy lands in the block that issued it.
 #include "block_scaled.cuh"
 #include "cluster.cuh"
@@ -49,8 +52,8 @@ __device__ __forceinline__ bool b2_wait_cluster(uint32_t bar, uint32_t parity) {
   return false;
 }
 
-// An arrival at the even block's barrier without a fence: what it orders is the reading of tensor memory, which tcgen05.fence has ordered (with
-// .release.cluster a step waits for a fence of the warp's whole memory traffic: 2,048 x 4,096 -> 6,144 took XX us, YY so).
+// An arrival at the even block's barrier without a fence of the cluster: what it orders is the reading of tensor memory, which tcgen05.fence has ordered.
+// (With .release.cluster every step waited for the warp's whole memory traffic, the largest of the kernel's stalls.)
 __device__ __forceinline__ void b2_arrive_even(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_bar) : "memory");
 }
