@@ -287,6 +287,29 @@ def test_expert_products(tokens, top, experts, k, n, out_dtype, by_pair, act):
         check(y[at], want, out_dtype, f"expert {e}")
 
 
+@pytest.mark.parametrize("experts, tokens, act", [(300, 40000, "none"), (300, 40000, "swiglu"), (200, 25000, "relu2"), (1024, 3000, "none")])
+def test_many_experts(experts, tokens, act):
+    """More than the pairs of SMs take, about as many, and the most; matrices repeat, so that the oracle is one product a matrix."""
+    need_gpu()
+    gated = act in ops.MOE_GATED
+    stacks = [[random_matrix(60, 130, 100 * part + e, DEV, (0.005, 0.2)) for e in range(4)] for part in range(2 if gated else 1)]
+    offsets, order, ids = routing(tokens, 1, experts, 3, empty=(1, experts - 1))
+    x = rows(tokens, 130, 5, spread=0.5)
+    y = torch.empty(tokens, 60, dtype=F32, device=DEV)
+    word = error_word()
+    ops.moe_expert_product(x, BlockScaledExperts(*([s[e % 4] for e in range(experts)] for s in stacks)), y, offsets, order, 1, x_by_pair=True, act=act,
+                           error_word=word)
+    assert int(word) == 0
+    kind = ids.to(DEV)[order.long()] % 4
+    for i in range(4):
+        at = (kind == i).nonzero()[:, 0]
+        sums = [product64(x[order[at].long()], s[i]) for s in stacks]
+        check(y[at], gated64(*sums, act=act) if gated else act64(sums[0], act), F32)
+    with pytest.raises(ops.KernelError):
+        ops.moe_expert_product(x[:1], BlockScaledExperts([stacks[0][0]] * 1025), y[:1], torch.zeros(1026, dtype=torch.int32, device=DEV),
+                               torch.zeros(1, dtype=torch.int32, device=DEV), 1, x_by_pair=True)
+
+
 @pytest.mark.parametrize("act", ["none", "relu2", "silu", "gelu", "swiglu", "glu_clamp"])
 @pytest.mark.parametrize("tokens", [4, 60, 400])
 def test_rows_that_are_not_finite_show_through_every_activation(tokens, act):

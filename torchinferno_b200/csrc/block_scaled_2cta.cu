@@ -116,17 +116,16 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
     int before = 0;
     for (int e0 = 0; e0 < a.experts; e0 += 32) {
       const int e = e0 + lane, begin = e < a.experts ? bs_offset(a.offsets, e, a.M) : 0;
-      const int end = e < a.experts ? max(begin, bs_offset(a.offsets, e + 1, a.M)) : 0;
-      int sum = (end - begin + 255) >> 8;
+      int sum = e < a.experts ? (max(0, bs_offset(a.offsets, e + 1, a.M) - begin) + 255) >> 8 : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int up = __shfl_up_sync(0xffffffffu, sum, o);
         if (lane >= o) sum += up;
       }
-      if (e < a.experts) tiles_before[e + 1] = before + sum, first_row[e + 1] = end;
+      if (e < a.experts) tiles_before[e + 1] = before + sum, first_row[e] = begin;
       before += __shfl_sync(0xffffffffu, sum, 31);
     }
-    if (lane == 0) tiles_before[0] = 0, first_row[0] = bs_offset(a.offsets, 0, a.M);
+    if (lane == 0) tiles_before[0] = 0, first_row[a.experts] = bs_offset(a.offsets, a.experts, a.M);
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();

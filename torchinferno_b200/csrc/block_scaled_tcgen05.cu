@@ -224,9 +224,8 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
       int before = 0;
       for (int e0 = 0; e0 < a.experts; e0 += 32) {
         const int e = e0 + lane, begin = e < a.experts ? bs_offset(a.offsets, e, a.M) : 0;
-        const int end = e < a.experts ? max(begin, bs_offset(a.offsets, e + 1, a.M)) : 0;
-        int sum = (end - begin + NT - 1) / NT;
-        if (e < a.experts) first_row[e + 1] = end;
+        int sum = e < a.experts ? (max(0, bs_offset(a.offsets, e + 1, a.M) - begin) + NT - 1) / NT : 0;
+        if (e < a.experts) first_row[e] = begin;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int up = __shfl_up_sync(0xffffffffu, sum, o);
@@ -235,7 +234,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
         if (e < a.experts) tiles_before[e + 1] = before + sum;
         before += __shfl_sync(0xffffffffu, sum, 31);
       }
-      if (lane == 0) tiles_before[0] = 0, first_row[0] = bs_offset(a.offsets, 0, a.M);
+      if (lane == 0) tiles_before[0] = 0, first_row[a.experts] = bs_offset(a.offsets, a.experts, a.M);
     }
   }
   pdl_trigger();
@@ -286,7 +285,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     if (!a.offsets) {
       for (int t = cluster_id; t < num_tiles && ahead < a.stages; t += clusters) {
         const BsTile m = tile_of(t);
-          for (int kb = kb0; kb < kb1 && ahead < a.stages; ++kb, ++ahead)
+        for (int kb = kb0; kb < kb1 && ahead < a.stages; ++kb, ++ahead)
           if (leader) {
             mbar_expect_tx(full_bar(ahead), bytes(m));
             tma_load_2d(base + ahead * S::kStage, &map_w, 0, w_row(m, kb), full_bar(ahead));
