@@ -23,6 +23,7 @@ from torchinferno_b200.kernels import ops
 
 BLOCK = 128
 CODE_DTYPE = torch.float8_e4m3fn
+_OUT_DTYPES = (torch.bfloat16, torch.float32)
 # Up to so many rows (of an expert: on average) a product's kernel quantises its rows itself, in every tile of 128 features anew; more are quantised ahead
 # of it.  (us, itself / ahead: 8 rows 4,096 -> 4,096 8.1 / 9.8, 4,096 -> 28,672 20.6 / 23.4, 14,336 -> 4,096 13.5 / 16.5; 12 rows 9.3 / 9.7, 27.2 / 23.5,
 # 16.0 / 16.7; 24 rows 12.2 / 9.8, 37.4 / 22.9, 20.5 / 16.8.)
@@ -100,7 +101,7 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     columns = x.shape[1]
     runs, lds = blocks(columns), (rows + 3) & ~3
     codes = x.new_empty((rows, runs * BLOCK), dtype=CODE_DTYPE)
-    scales = torch.empty_strided((rows, runs), (1, lds), dtype=torch.float32, device=x.device)
+    scales = x.new_empty_strided((rows, runs), (1, lds), dtype=torch.float32)
     ops.quantize_rows(x, codes.data_ptr(), scales.data_ptr(), lds)
     return codes if columns == runs * BLOCK else codes[:, :columns], scales
 
@@ -114,7 +115,7 @@ def _code_buffer(x: torch.Tensor, rows: int, columns: int) -> torch.Tensor:
 class Blocks:
     """Matrices of one size as the kernels read them: ``codes`` [matrices, blocks of N, blocks of K, 128, 128], padded with zeros, and ``scales`` [matrices,
     blocks of N, blocks of K]; ``paired``: the matrices' rows are (gate i, up i), their scales' rows (gate block j, up block j)."""
-    __slots__ = ("codes", "scales", "count", "features", "columns", "paired", "codes_at", "scales_at", "scale_rows")
+    __slots__ = ("codes", "scales", "count", "features", "columns", "paired", "codes_at", "scales_at", "scale_rows", "device_index")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, features: int, columns: int, paired: bool) -> None:
         if codes.shape[1] != blocks(features) or codes.shape[2] != blocks(columns) or scales.shape[1:] != (codes.shape[1] if not paired else 2 * blocks(features // 2), codes.shape[2]):
@@ -122,7 +123,7 @@ class Blocks:
         if not codes.is_contiguous() or not scales.is_contiguous():
             raise ValueError("blocks and their scales must be contiguous")
         self.codes, self.scales, self.count, self.features, self.columns, self.paired = codes, scales, codes.shape[0], features, columns, paired
-        self.codes_at, self.scales_at, self.scale_rows = codes.data_ptr(), scales.data_ptr(), scales.shape[1]
+        self.codes_at, self.scales_at, self.scale_rows, self.device_index = codes.data_ptr(), scales.data_ptr(), scales.shape[1], codes.get_device()
 
 
 def _laid_out(matrices: Sequence[BlockScaledMatrix], ups: Sequence[BlockScaledMatrix] | None) -> Blocks:
@@ -210,15 +211,13 @@ class BlockScaledWeight:
         return view
 
     def _run(self, x: torch.Tensor, act: str, width: int, out_dtype: torch.dtype | None, out: torch.Tensor | None, error_word: torch.Tensor | None) -> torch.Tensor:
-        rows = _checked_rows(x, self.in_features, self.parts[0][1].codes.get_device(), "linear")
-        if out_dtype is not None and out_dtype != x.dtype:
-            if out_dtype not in (torch.bfloat16, torch.float32):
-                raise ops.KernelError(f"linear: unsupported output dtype {out_dtype}")
-            if out is None or out.dtype != out_dtype:
-                out = x.new_empty((rows, width), dtype=out_dtype)
-        elif out is None or out.dtype != x.dtype:
-            out = x.new_empty((rows, width))
-        if out.shape != (rows, width) or (out.stride(1) != 1 and width > 1) or out.get_device() != x.get_device():
+        rows = _checked_rows(x, self.in_features, self.parts[0][1].device_index, "linear")
+        dtype = x.dtype if out_dtype is None else out_dtype
+        if out is None or out.dtype != dtype:
+            if dtype not in _OUT_DTYPES:
+                raise ops.KernelError(f"linear: unsupported output dtype {dtype}")
+            out = x.new_empty((rows, width)) if dtype == x.dtype else x.new_empty((rows, width), dtype=dtype)
+        elif out.shape != (rows, width) or (out.stride(1) != 1 and width > 1) or out.get_device() != x.get_device():
             raise ops.KernelError(f"linear: out is {tuple(out.shape)} on {out.device}, wanted {(rows, width)} with unit inner stride on {x.device}")
         if rows == 0:
             return out
@@ -275,7 +274,7 @@ class BlockScaledExperts:
         if gated != self.paired and act != "none":
             raise ops.KernelError(f"moe_expert_product: activation {act!r} does not fit experts with{'' if self.paired else 'out'} gate and up rows")
         pairs, width = order.numel(), self.out_features // 2 if gated else self.out_features
-        here = self.blocks.codes.get_device()
+        here = self.blocks.device_index
         rows = _checked_rows(x, self.in_features, here, "moe_expert_product")
         if y.shape != (pairs, width) or offsets.numel() != self.experts + 1 or top < 1 or (pairs % top or rows < pairs // top if x_by_pair else rows < pairs):
             raise ops.KernelError("moe_expert_product: shapes do not fit")

@@ -71,9 +71,9 @@ def launch_count() -> int:
 
 
 def _code(dtype: torch.dtype) -> int:
-    if dtype == torch.float32:
+    if dtype is torch.float32:
         return F32
-    if dtype == torch.bfloat16:
+    if dtype is torch.bfloat16:
         return BF16
     raise KernelError(f"dtype {dtype} is not supported by the kernels (float32 or bfloat16)")
 
@@ -1271,8 +1271,8 @@ def block_scaled_product(x: torch.Tensor, codes: int, make: bool, blocks, y: tor
     if codes and make:
         _counter["launches"] += 1
     _check("block_scaled_product", lib().tib_block_scaled_product(
-        x.data_ptr(), _code(x.dtype), x.stride(0), x.shape[0], codes, make, blocks.codes_at, blocks.scales_at, blocks.scale_rows, blocks.paired, y.data_ptr(),
-        _code(y.dtype), y.stride(0), y.shape[0], blocks.features, blocks.columns, offsets, order, blocks.count, top, x_by_pair, MOE_ACT[act], limit, alpha,
+        x.data_ptr(), _code(x.dtype), x.stride(0), len(x), codes, make, blocks.codes_at, blocks.scales_at, blocks.scale_rows, blocks.paired, y.data_ptr(),
+        _code(y.dtype), y.stride(0), len(y), blocks.features, blocks.columns, offsets, order, blocks.count, top, x_by_pair, MOE_ACT[act], limit, alpha,
         0 if row_scale is None else row_scale.data_ptr(), 0 if error_word is None else error_word.data_ptr(), _stream()))
 
 
