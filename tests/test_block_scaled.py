@@ -179,6 +179,33 @@ def test_checkpoints_that_do_not_fit_are_refused(tmp_path, name, tensor, message
         load_weights(build_model(config, dtype=torch.bfloat16, device="cpu"), tmp_path)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("name", ["model.layers.0.self_attn.o_proj.weight", "model.layers.1.mlp.down_proj.weight", "model.layers.0.self_attn.k_proj.weight"])
+def test_codes_without_their_scales_are_refused(tmp_path, name, dtype):
+    """A lost tensor of scales is named, whether or not the matrix shares its product with others; unscaled codes are never bound as numbers."""
+    from conftest import TINY_B
+    from safetensors.torch import save_file
+    from torchinferno_b200.weights.loader import WeightError, load_weights
+    from torchinferno_b200.weights.random_init import build_model
+    config = {**TINY_B, "quantization_config": FP8}
+    tensors = _folder(tmp_path, config)
+    del tensors[name + "_scale_inv"]
+    save_file(tensors, str(tmp_path / "model.safetensors"))
+    with pytest.raises(WeightError, match=name + ": stored as F8_E4M3 without " + name + "_scale_inv"):
+        load_weights(build_model(config, dtype=dtype, device="cpu"), tmp_path)
+
+
+@pytest.mark.parametrize("code", [CODES, torch.float8_e5m2])
+def test_codes_of_what_is_never_in_blocks_are_refused(tmp_path, code):
+    from conftest import TINY_B
+    from torchinferno_b200.weights.loader import WeightError, load_weights
+    from torchinferno_b200.weights.random_init import build_model
+    shape = build_model(TINY_B, dtype=torch.bfloat16, device="cpu").expected_tensors()["model.norm.weight"].shape
+    _folder(tmp_path, TINY_B, **{"model.norm.weight": torch.ones(shape).to(code)})
+    with pytest.raises(WeightError, match="model.norm.weight: stored as F8_"):
+        load_weights(build_model(TINY_B, dtype=torch.bfloat16, device="cpu"), tmp_path)
+
+
 def test_fused_projections_are_stored_alike(tmp_path):
     from conftest import TINY_B
     from torchinferno_b200.weights.loader import load_weights

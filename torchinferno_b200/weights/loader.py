@@ -14,7 +14,8 @@ widened to fp32 (lossless); integer tables become int32.  When the engine
 computes in float32 every floating tensor is widened to fp32.  A matrix that its
 part takes in 8-bit blocks (``WeightSpec.block_scaled``) and that is stored as e4m3
 codes with a tensor of scales beside it (its name and ``_scale_inv``) stays so in
-bfloat16, and is widened to the numbers it stands for in float32.
+bfloat16, and is widened to the numbers it stands for in float32.  Codes without their
+scales are refused.
 """
 from __future__ import annotations
 
@@ -110,12 +111,15 @@ def load_weights(model, folder: str | Path) -> dict[str, object]:
             free = getattr(ws, "free_dims", ())
             if len(shape) != len(ws.shape) or any(a != b for d, (a, b) in enumerate(zip(shape, ws.shape)) if d not in free):
                 wrong.append(f"{name}: file {list(shape)} vs model {list(ws.shape)}")
+            dtype = str(view.get_dtype())
             if name in in_blocks:
                 found = list(handle_of(files[name + SCALE_SUFFIX]).get_slice(name + SCALE_SUFFIX).get_shape())
                 if found != [blocks(d) for d in shape]:
                     wrong.append(f"{name + SCALE_SUFFIX}: file {found} vs a scale for each 128 x 128 of {list(shape)}")
-                elif str(view.get_dtype()) != "F8_E4M3":
+                elif dtype != "F8_E4M3":
                     wrong.append(f"{name}: has scales beside it but is not stored as e4m3 codes")
+            elif dtype.startswith("F8") and name not in unused:      # (codes stand for nothing without their scales)
+                wrong.append(f"{name}: stored as {dtype} without {name + SCALE_SUFFIX}" if ws.block_scaled else f"{name}: stored as {dtype}, which the model does not take")
         if missing or unexpected or wrong:
             parts = [f"checkpoint {folder} does not fit the model ({model.spec.architecture}):"]
             if missing:
