@@ -206,6 +206,26 @@ def test_codes_of_what_is_never_in_blocks_are_refused(tmp_path, code):
         load_weights(build_model(TINY_B, dtype=torch.bfloat16, device="cpu"), tmp_path)
 
 
+@pytest.mark.parametrize("change", [{"weight_block_size": [96, 128]}, {"weight_block_size": None}, {"activation_scheme": "static"}, {"fmt": "e5m2"}])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_blocks_of_another_form_are_refused(tmp_path, change, dtype):
+    """Scales of blocks of 96 rows have the shape of those of 128 where the rows are 192: only config.json tells them apart.  The same folder without a
+    tensor in 8 bits loads whatever its config.json says of them."""
+    import json
+    from conftest import TINY_B
+    from torchinferno_b200.weights.loader import WeightError, load_weights
+    from torchinferno_b200.weights.random_init import build_model, write_random_model
+    _folder(tmp_path, {**TINY_B, "quantization_config": FP8})
+    said = json.loads((tmp_path / "config.json").read_text())
+    said["quantization_config"] = {**FP8, **change}
+    (tmp_path / "config.json").write_text(json.dumps(said))
+    with pytest.raises(WeightError, match="8-bit blocks, but quantization_config." + next(iter(change))):
+        load_weights(build_model(TINY_B, dtype=dtype, device="cpu"), tmp_path)
+    write_random_model(TINY_B, tmp_path, seed=0)
+    (tmp_path / "config.json").write_text(json.dumps(said))
+    load_weights(build_model(TINY_B, dtype=dtype, device="cpu"), tmp_path)
+
+
 def test_fused_projections_are_stored_alike(tmp_path):
     from conftest import TINY_B
     from torchinferno_b200.weights.loader import load_weights

@@ -15,7 +15,8 @@ computes in float32 every floating tensor is widened to fp32.  A matrix that its
 part takes in 8-bit blocks (``WeightSpec.block_scaled``) and that is stored as e4m3
 codes with a tensor of scales beside it (its name and ``_scale_inv``) stays so in
 bfloat16, and is widened to the numbers it stands for in float32.  Codes without their
-scales are refused.
+scales are refused, and so are those of a folder whose ``quantization_config`` names
+another form of 8-bit weights (config/quantization.py).
 """
 from __future__ import annotations
 
@@ -25,11 +26,13 @@ from typing import Iterable
 
 import torch
 
-from torchinferno_b200.config.quantization import SCALE_SUFFIX
+from torchinferno_b200.config.model_config import ConfigError
+from torchinferno_b200.config.quantization import SCALE_SUFFIX, BlockQuantization
 from torchinferno_b200.kernels.block_scaled import BlockScaledMatrix, blocks
 
 SINGLE_FILE = "model.safetensors"
 INDEX_FILE = "model.safetensors.index.json"
+CONFIG_FILE = "config.json"
 
 
 class WeightError(ValueError):
@@ -130,6 +133,11 @@ def load_weights(model, folder: str | Path) -> dict[str, object]:
                 parts.append(f"  wrong shape ({len(wrong)}): " + "; ".join(sorted(wrong)[:12])
                              + (f"; ... (+{len(wrong) - 12} more)" if len(wrong) > 12 else ""))
             raise WeightError("\n".join(parts))
+        if in_blocks and (Path(folder) / CONFIG_FILE).is_file():
+            try:
+                BlockQuantization.from_config(json.loads((Path(folder) / CONFIG_FILE).read_text()))
+            except ConfigError as exc:
+                raise WeightError(f"checkpoint {folder} holds 8-bit blocks, but {exc}") from None
         tensors: dict[str, torch.Tensor] = {}
         stored: dict[str, str] = {}
         for name, ws in expected.items():
