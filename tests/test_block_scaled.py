@@ -226,6 +226,18 @@ def test_blocks_of_another_form_are_refused(tmp_path, change, dtype):
     load_weights(build_model(TINY_B, dtype=dtype, device="cpu"), tmp_path)
 
 
+def test_scales_that_are_no_numbers_are_refused(tmp_path):
+    """Bytes beside codes (exponents, say) are not read as numbers."""
+    from conftest import TINY_B
+    from torchinferno_b200.weights.loader import WeightError, load_weights
+    from torchinferno_b200.weights.random_init import build_model
+    config = {**TINY_B, "quantization_config": FP8}
+    name = "model.layers.0.mlp.down_proj.weight_scale_inv"
+    _folder(tmp_path, config, **{name: torch.full((2, 4), 120, dtype=torch.uint8)})
+    with pytest.raises(WeightError, match="stored as U8"):
+        load_weights(build_model(config, dtype=torch.bfloat16, device="cpu"), tmp_path)
+
+
 def test_fused_projections_are_stored_alike(tmp_path):
     from conftest import TINY_B
     from torchinferno_b200.weights.loader import load_weights

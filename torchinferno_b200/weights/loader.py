@@ -116,11 +116,14 @@ def load_weights(model, folder: str | Path) -> dict[str, object]:
                 wrong.append(f"{name}: file {list(shape)} vs model {list(ws.shape)}")
             dtype = str(view.get_dtype())
             if name in in_blocks:
-                found = list(handle_of(files[name + SCALE_SUFFIX]).get_slice(name + SCALE_SUFFIX).get_shape())
+                beside = handle_of(files[name + SCALE_SUFFIX]).get_slice(name + SCALE_SUFFIX)
+                found = list(beside.get_shape())
                 if found != [blocks(d) for d in shape]:
                     wrong.append(f"{name + SCALE_SUFFIX}: file {found} vs a scale for each 128 x 128 of {list(shape)}")
                 elif dtype != "F8_E4M3":
                     wrong.append(f"{name}: has scales beside it but is not stored as e4m3 codes")
+                elif not str(beside.get_dtype()).startswith(("F", "BF")):
+                    wrong.append(f"{name + SCALE_SUFFIX}: stored as {beside.get_dtype()}, scales are floating-point numbers")
             elif dtype.startswith("F8") and name not in unused:      # (codes stand for nothing without their scales)
                 wrong.append(f"{name}: stored as {dtype} without {name + SCALE_SUFFIX}" if ws.block_scaled else f"{name}: stored as {dtype}, which the model does not take")
         if missing or unexpected or wrong:
