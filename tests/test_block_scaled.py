@@ -238,6 +238,21 @@ def test_scales_that_are_no_numbers_are_refused(tmp_path):
         load_weights(build_model(config, dtype=torch.bfloat16, device="cpu"), tmp_path)
 
 
+@pytest.mark.parametrize("quantization", [{"quant_method": "fp8"}, {**FP8, "weight_block_size": [1, 128]}, {**FP8, "activation_scheme": "static"}, "fp8"])
+def test_random_models_run_whatever_form_config_json_names(tmp_path, quantization):
+    """A form of 8-bit weights that is not read is no reason against random ones: they are what they are without it."""
+    from conftest import TINY_B
+    from torchinferno_b200.weights.loader import load_weights
+    from torchinferno_b200.weights.random_init import build_model, init_random_weights, write_random_model
+    config = {**TINY_B, "quantization_config": quantization}
+    models = [build_model(c, dtype=torch.bfloat16, device="cpu") for c in (TINY_B, config, config)]
+    init_random_weights(models[0], 0, config=TINY_B)
+    init_random_weights(models[1], 0, config=config)
+    load_weights(models[2], write_random_model(config, tmp_path, 0))
+    downs = [m.blocks[0].feed_forward.down_weight.tensor for m in models]
+    assert torch.equal(downs[0], downs[1]) and torch.equal(downs[0], downs[2])
+
+
 def test_fused_projections_are_stored_alike(tmp_path):
     from conftest import TINY_B
     from torchinferno_b200.weights.loader import load_weights

@@ -7,7 +7,8 @@ The reference has no such mode; its tests build an eager model under
 ``torch.manual_seed`` and write it out to load it back
 (tests/test_model_variants.py:319-354 in the reference project).
 
-With ``quantization_config`` in config.json (config/quantization.py) the matrices it covers are quantised to 8-bit blocks.
+With ``quantization_config`` in config.json (config/quantization.py) the matrices it covers are quantised to 8-bit blocks; where it names
+a form that is not read, random weights are of the model's own type, as without it.
 """
 from __future__ import annotations
 
@@ -18,6 +19,7 @@ from typing import Any, Mapping
 
 import torch
 
+from torchinferno_b200.config.model_config import ConfigError
 from torchinferno_b200.config.quantization import SCALE_SUFFIX, BlockQuantization
 from torchinferno_b200.config.registry import resolve_architecture
 from torchinferno_b200.kernels.block_scaled import quantize_matrix
@@ -56,6 +58,14 @@ def build_model(config: Mapping[str, Any], *, dtype: torch.dtype, device: torch.
     return CausalLM(entry.build(typed), dtype=dtype, device=device)
 
 
+def _quantization(config: Mapping[str, Any]) -> BlockQuantization | None:
+    """What config.json has stored in 8-bit blocks.  (A form of 8-bit weights that is not read concerns files, and their loader: a random model has none.)"""
+    try:
+        return BlockQuantization.from_config(config)
+    except ConfigError:
+        return None
+
+
 def _in_blocks(quantization: BlockQuantization | None, spec) -> bool:
     """Whether config.json has this tensor stored in 8-bit blocks."""
     return spec.block_scaled and quantization is not None and quantization.converts(spec.name)
@@ -70,7 +80,7 @@ def write_random_model(config: Mapping[str, Any], folder: str | Path, seed: int,
     config = dict(config)
     config["torch_dtype"] = str(dtype).replace("torch.", "")
     model = build_model(config, dtype=torch.float32, device="cpu")
-    quantization = BlockQuantization.from_config(config)
+    quantization = _quantization(config)
     tensors = {}
     for name, spec in model.expected_tensors().items():
         if spec.optional:
@@ -88,7 +98,7 @@ def write_random_model(config: Mapping[str, Any], folder: str | Path, seed: int,
 def init_random_weights(model, seed: int, storage_dtype: torch.dtype = torch.bfloat16, config: Mapping[str, Any] | None = None) -> None:
     """Bind seeded random weights generated on the model's device (nothing touches the disk).  ``config``: the config.json whose
     ``quantization_config`` says which matrices are stored in 8-bit blocks (None: none)."""
-    quantization = None if config is None else BlockQuantization.from_config(config)
+    quantization = None if config is None else _quantization(config)
     tensors = {}
     for name, spec in model.expected_tensors().items():
         if spec.optional:
