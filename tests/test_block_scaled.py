@@ -122,6 +122,14 @@ def test_quantization_config():
             BlockQuantization.from_config({"quantization_config": bad})
 
 
+@pytest.mark.parametrize("names", [5, True, {"lm_head": 1}, [1], ["lm_head", None]])
+def test_modules_that_are_no_list_of_names_are_refused(names):
+    from torchinferno_b200.config.model_config import ConfigError
+    from torchinferno_b200.config.quantization import BlockQuantization
+    with pytest.raises(ConfigError, match="list of names"):
+        BlockQuantization.from_config({"quantization_config": {**FP8, "modules_to_not_convert": names}})
+
+
 def _folder(tmp_path, config, **changes):
     """A random model folder with these tensors changed, and its tensors as they were."""
     from safetensors.torch import load_file, save_file

@@ -37,7 +37,7 @@ class BlockQuantization:
         if str(data.get("activation_scheme", "dynamic")).lower() != "dynamic":
             raise ConfigError(f"quantization_config.activation_scheme={data['activation_scheme']!r} is not supported (dynamic)")
         names = data.get("modules_to_not_convert") or data.get("ignored_layers") or ()
-        if isinstance(names, str) or not all(isinstance(n, str) for n in names):
+        if not isinstance(names, (list, tuple)) or not all(isinstance(n, str) for n in names):
             raise ConfigError("quantization_config.modules_to_not_convert must be a list of names")
         return cls(tuple(names))
 
