@@ -72,6 +72,22 @@ def test_gate_and_up_alternate():
     assert e.out_features == 260 and torch.equal(flat(e.blocks.codes[1], 260)[0::2, :300], u.codes.view(torch.uint8))
 
 
+@pytest.mark.parametrize("scales, low, high", [
+    ([1.0], -126, 120), ([0.0], -126, 120), ([2.0 ** -10], -116, 120), ([-2.0 ** -10, 1.9], -116, 120), ([1.99 * 2.0 ** -10], -116, 120), ([2.0 ** -126], 0, 120),
+    ([2.0 ** -149], 0, 120), ([2.0 ** 8], -126, 119), ([1.9 * 2.0 ** 7], -126, 120), ([2.0 ** 127], -126, 0), ([2.0 ** -126, 2.0 ** 127], 0, 0),
+    ([float("nan"), 2.0 ** -20, float("inf")], -106, 120)])
+def test_rows_scales_that_a_matrix_keeps_normal(scales, low, high):
+    """The range that the kernels compare with: all of it gives normal products (or powers of at least 1), a power outside of it does not."""
+    import math
+    codes_ = torch.zeros(128, 128 * len(scales), dtype=torch.uint8).view(CODES)
+    part = BlockScaledWeight(BlockScaledMatrix(codes_, torch.tensor([scales]))).parts[0][1]
+    assert (part.far_from, part.far_span) == ((low + 127) << 23, (high - low) << 23)
+
+    def normal(p):
+        return all(s == 0 or not math.isfinite(s) or (2.0 ** p * abs(s) < 2.0 ** 128 and (p >= 0 or 2.0 ** p * abs(s) >= 2.0 ** -126)) for s in scales)
+    assert all(normal(p) for p in range(low, high + 1)) and (low == -126 or not normal(low - 1)) and (high == 120 or not normal(high + 1))
+
+
 def test_products_need_a_gpu():
     w = BlockScaledWeight(random_matrix(64, 64, 0))
     for call in (lambda: gemm.linear(torch.zeros(2, 64), w), lambda: gemm.linear(torch.zeros(2, 63), w), lambda: quantize_rows(torch.zeros(2, 64)),

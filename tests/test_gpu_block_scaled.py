@@ -171,6 +171,121 @@ def test_sizes_at_the_ends_of_the_range(m):
         check(got / size, (want / size, bound / size), F32)
 
 
+# ------------------------------------------------------------------------------------------------ scales whose product no 32-bit number holds
+def far_rows(m, k, seed):
+    """32-bit rows whose runs are of sizes from 2^-140 to 2^118, every run of a size of its own."""
+    g = torch.Generator().manual_seed(seed)
+    sizes = torch.tensor([-140.0, -118.0, -100.0, -60.0, 0.0, 60.0, 100.0, 118.0], dtype=torch.float64)
+    power = sizes[torch.randint(0, len(sizes), (m, -(-k // 128)), generator=g)].repeat_interleave(128, 1)[:, :k]
+    return (torch.randn(m, k, generator=g, dtype=torch.float64).clamp(-200, 200) * 2.0 ** power).to(F32).to(DEV)
+
+
+def far_matrix(n, k, seed):
+    """Scales over the whole range of 32-bit numbers, subnormal ones, zeros and either sign among them; some features are zeros."""
+    matrix = random_matrix(n, k, seed)
+    g = torch.Generator().manual_seed(seed)
+    sizes = torch.tensor([0.0, 2.0 ** -149, 2.0 ** -130, 1.3 * 2.0 ** -100, -1.37 * 2.0 ** -10, 1.7, 1.1 * 2.0 ** 8, -2.0 ** 30, 1.9 * 2.0 ** 100, 2.0 ** 127], dtype=torch.float64)
+    codes = matrix.codes.clone()
+    codes.view(torch.uint8)[3::130] = 0
+    return BlockScaledMatrix(codes, sizes[torch.randint(0, len(sizes), tuple(matrix.scales.shape), generator=g)].to(F32)).to(DEV)
+
+
+def check_far(got, x, matrix):
+    """Where no partial sum leaves the range.  A subnormal sum or share of one is a multiple of 2^-149: half of that more for every run, and for the last rounding."""
+    want, bound = product64(x, matrix)
+    size = widened_rows64(x).abs() @ matrix64(matrix).abs().t()
+    kept = size < 2.0 ** 126
+    assert kept.double().mean() > 0.3 and got.dtype == F32
+    off = (got.double() - want).abs()
+    bad = kept & ~(off <= bound + 2.0 ** -149 * (x.shape[1] / 128 + 2))
+    assert not bad.any(), f"{int(bad.sum())} of {int(kept.sum())} off, {int((bad & got.isnan()).sum())} NaN, {int((bad & (got == 0)).sum())} zeros"
+
+
+# (the kernel's own codes; tiles of 32, 64 and 128 rows; pairs of SMs)
+FAR = [(5, 9600), (20, 9600), (60, 9600), (100, 9600), (200, 9600), (5, 300)]
+
+
+@pytest.mark.parametrize("m, n", FAR)
+def test_scales_whose_product_leaves_the_range(m, n):
+    need_gpu()
+    x, matrix = far_rows(m, 300, m), far_matrix(n, 300, 7)
+    check_far(gemm.linear(x, BlockScaledWeight(matrix)), x, matrix)
+
+
+@pytest.mark.parametrize("m, n", FAR)
+def test_scales_of_gate_and_up_whose_product_leaves_the_range(m, n):
+    need_gpu()
+    x, gate, up = far_rows(m, 300, m), far_matrix(n // 2, 300, 8), far_matrix(n // 2, 300, 9)
+    both = gemm.linear(x, BlockScaledWeight(gate, up, epilogue="swiglu"))
+    check_far(both[:, 0::2].contiguous(), x, gate)
+    check_far(both[:, 1::2].contiguous(), x, up)
+
+
+@pytest.mark.parametrize("pairs", [6, 100, 500])
+def test_scales_of_experts_whose_product_leaves_the_range(pairs):
+    need_gpu()
+    matrices, x = [far_matrix(300, 300, e) for e in range(4)], far_rows(pairs, 300, pairs)
+    offsets, order, ids = routing(pairs, 1, 4, 1)
+    y = torch.empty(pairs, 300, dtype=F32, device=DEV)
+    ops.moe_expert_product(x, BlockScaledExperts(matrices), y, offsets, order, 1, x_by_pair=True)
+    ends = offsets.tolist()
+    for e in range(4):
+        at = order[ends[e]:ends[e + 1]].long()
+        if len(at):
+            check_far(y[ends[e]:ends[e + 1]], x[at], matrices[e])
+
+
+@pytest.mark.parametrize("m, n", FAR)
+def test_small_gates_and_large_ups(m, n):
+    """Gates of about 2^-120 whose scales' product is below the range, ups of about 2^30: the unit is far inside of it."""
+    need_gpu()
+    x = (rows(m, 300, m, F32, 0.1) * 2.0 ** -100).contiguous()
+    gate, up = random_matrix(n // 2, 300, 1, DEV, (60 * 2.0 ** -31, 60 * 2.0 ** -30)), random_matrix(n // 2, 300, 2, DEV, (60 * 2.0 ** 119, 60 * 2.0 ** 120))
+    got = gemm.linear_swiglu(x, BlockScaledWeight(gate, up, epilogue="swiglu"))
+    # (a sum of subnormal size is a multiple of 2^-149 as well; its share in the bound: 2^-147 times the other factor)
+    (g, eg), (u, eu) = product64(x, gate), product64(x, up)
+    want, bound = gated64((g, eg + 2.0 ** -147), (u, eu))
+    check(got, (want, bound), F32)
+    assert want.abs().median() > 2.0 ** -105
+
+
+@pytest.mark.parametrize("act", ["none", "relu2", "silu", "gelu", "swiglu", "glu_clamp"])
+@pytest.mark.parametrize("pairs, out_dtype", [(6, F32), (100, F32), (500, F32), (6, BF16), (500, BF16)])
+def test_activations_of_sums_with_far_scales(pairs, out_dtype, act):
+    need_gpu()
+    n = 130
+    stacks = [[random_matrix(n, 300, e, DEV, (60 * 2.0 ** -31, 60 * 2.0 ** -30)) for e in range(3)]]
+    if act in ops.MOE_GATED:
+        stacks.append([random_matrix(n, 300, 10 + e, DEV, (60 * 2.0 ** 99, 60 * 2.0 ** 100)) for e in range(3)])
+    x = (rows(pairs, 300, pairs, F32, 0.1) * 2.0 ** -100).contiguous()
+    offsets, order, _ = routing(pairs, 1, 3, 1)
+    scale = torch.rand(pairs, generator=torch.Generator().manual_seed(1)).to(DEV) + 0.5
+    y = torch.empty(pairs, n, dtype=out_dtype, device=DEV)
+    ops.moe_expert_product(x, BlockScaledExperts(*stacks), y, offsets, order, 1, x_by_pair=True, act=act, limit=2.0, alpha=1.702, row_scale=scale)
+    ends = offsets.tolist()
+    for e in range(3):
+        at = order[ends[e]:ends[e + 1]].long()
+        if len(at) == 0:
+            continue
+        s = scale[at].double()[:, None]
+        sums = [product64(x[at], stack[e]) for stack in stacks]
+        sums = [(v * s, b * s + 2.0 ** -23 * (v * s).abs() + 2.0 ** -147) for v, b in sums]
+        want, bound = gated64(*sums, act=act, limit=2.0) if act in ops.MOE_GATED else act64(sums[0], act)
+        check(y[ends[e]:ends[e + 1]], (want, bound + 2.0 ** -133), out_dtype)
+
+
+@pytest.mark.parametrize("m, n", FAR)
+def test_a_row_does_not_depend_on_others_of_far_sizes(m, n):
+    """The same bits beside rows whose scales' product leaves the range."""
+    need_gpu()
+    weight, x = BlockScaledWeight(random_matrix(n, 300, 3, DEV, (1e-3, 1e-2))), rows(m, 300, 2, F32)
+    before = gemm.linear(x, weight)
+    x[1::3] = far_rows(m, 300, 5)[1::3]
+    after = gemm.linear(x, weight)
+    for at in (slice(0, None, 3), slice(2, None, 3)):
+        assert torch.equal(before[at], after[at])
+
+
 def test_no_rows():
     need_gpu()
     weight = BlockScaledWeight(random_matrix(100, 200, 1, DEV))

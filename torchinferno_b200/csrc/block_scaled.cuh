@@ -7,6 +7,8 @@
 // Rows x [M, K] have one power of two for each run of 128 columns; their scales lie [runs, M rounded up to 4].
 #pragma once
 
+#include <cuda_fp16.h>
+
 #include "moe.cuh"
 #include "tcgen05.cuh"
 
@@ -121,6 +123,121 @@ template <typename T> __device__ __forceinline__ uint4 bs_codes16(const uint4 (&
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// The scale of a (row, run) and (block, run) is s S, s = 2^p: exact where it is a normal number (or s is at least 1), which is all but everywhere.  Elsewhere the
+// sum v of the run's products, 0 or of a size from 2^-18 to 2^25, may still have a share v s S that is a normal number while s S is none.  Such a scale is "far".
+// The kernels' loops only notice that a row's s is outside of what the matrix's scales keep normal (`from`, `span`: of the bits of s); behind their tiles the
+// outputs with a far scale are made again, by themselves.  No other output changes: a row's bits are its own.  (Shares of far scales made inside the loops cost
+// every call 1 to 13 %, a look at the sums as they are finished 1 to 45 %; this costs 0.1 us of 5 to 14 at few rows, nothing at many.)
+struct BsFar {
+  uint32_t from, span;
+  __device__ __forceinline__ bool outside(float s) const { return __float_as_uint(s) - from > span; }      // (so is a NaN)
+};
+__device__ __forceinline__ bool bs_is_far(float s, float s_of_block) {
+  const float block = fabsf(s_of_block), product = s * block;
+  return product < fminf(block, 0x1p-126f) || (product > 3.402823466e38f && block < INFINITY);      // (a NaN is not)
+}
+
+// The sum of 16 products of codes.
+__device__ __forceinline__ float bs_dot16(uint4 a, uint4 b) {
+  const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint32_t p, q;      // (a code is a half without rounding)
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(p) : "h"((uint16_t)(x[i >> 1] >> (16 * (i & 1)))));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(q) : "h"((uint16_t)(y[i >> 1] >> (16 * (i & 1)))));
+    const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&p)), v = __half22float2(*reinterpret_cast<const __half2*>(&q));
+    sum = fmaf(u.x, v.x, fmaf(u.y, v.y, sum));
+  }
+  return sum;
+}
+
+// A row of x (codes, TX uint8_t, with scales `lds` apart; or as it is) and the matrix it meets.
+template <typename TX> struct BsApart {
+  const TX* x;
+  const float* x_scales;
+  int64_t lds;
+  const unsigned char* w;      // the expert's blocks
+  const float* w_scales;       // and their scales
+  int pairs, runs, K, act;
+  float row_scale, limit, alpha;
+
+  __device__ float run_scale(int b, float& inverse) const {
+    if constexpr (sizeof(TX) == 1) return x_scales[(size_t)b * lds];
+    else {
+      uint32_t largest = 0;
+      float scale;
+#pragma unroll 1
+      for (int i = 0; i < kBlk; i += 16) {
+        uint4 raw[sizeof(TX)];
+        bs_ask16<TX, false>(x + b * kBlk + i, K - b * kBlk - i, raw);
+        largest = max(largest, bs_largest16<TX>(raw));
+      }
+      bs_run_scale(largest, scale, inverse);
+      return scale;
+    }
+  }
+  __device__ bool far(int f) const {      // whether feature f's sum has a far scale
+    const float* ws = w_scales + (size_t)bs_scale_row(f, pairs) * runs;
+    float inverse;
+    bool far = false;
+    for (int b = 0; b < runs; ++b) {
+      const float s = run_scale(b, inverse);
+      if (isnan(s)) return false;         // (the row's outputs are NaN)
+      far = far || bs_is_far(s, ws[b]);
+    }
+    return far;
+  }
+  // By one thread, 16 columns at a time.  A far scale's share is made in two steps, s shifted by 2^64 (without rounding) and the share shifted back:
+  // v (s 2^64 S) 2^-64 where S is below 1 and s S too
+  // small, v (s 2^-64 S) 2^64 where it is too large (s is at most 2^120: that takes an S of 2^8).
+  __device__ float sum(int f) const {
+    const float* ws = w_scales + (size_t)bs_scale_row(f, pairs) * runs;
+    float inverse = 0.f, sum = 0.f;
+    const unsigned char* codes = w + ((size_t)(f >> 7) * runs * kBlk + (f & 127)) * kBlk;
+#pragma unroll 1
+    for (int b = 0; b < runs; ++b, codes += kBlk * kBlk) {
+      const float s = run_scale(b, inverse), block = ws[b];
+      float v = 0.f;
+#pragma unroll 2
+      for (int i = 0; i < kBlk; i += 16) {
+        const uint4 wc = *reinterpret_cast<const uint4*>(codes + i);
+        if constexpr (sizeof(TX) == 1) v += bs_dot16(*reinterpret_cast<const uint4*>(x + b * kBlk + i), wc);
+        else {
+          uint4 raw[sizeof(TX)];
+          bs_ask16<TX, false>(x + b * kBlk + i, K - b * kBlk - i, raw);
+          v += bs_dot16(bs_codes16<TX>(raw, inverse), wc);
+        }
+      }
+      if (bs_is_far(s, block)) {
+        const bool small = fabsf(block) < 1.f;
+        // (a shifted scale beyond the range: v is 0, or its share an infinity either way)
+        const float shifted = fminf(fmaxf(s * (small ? 0x1p64f : 0x1p-64f) * block, -3.402823466e38f), 3.402823466e38f);
+        sum = fmaf(v * shifted, small ? 0x1p-64f : 0x1p64f, sum);
+      } else {
+        sum = fmaf(v, s * block, sum);
+      }
+    }
+    return sum * row_scale;
+  }
+};
+// The row's output o, if it has a far scale, to y.  (Not inline: it is never in a hurry, and the kernels' registers are not for it.)
+template <typename TX, typename TO>
+__device__ __noinline__ void bs_output_apart(const BsApart<TX>& a, int o, TO* __restrict__ y) {
+  const int gated = moe_act_gated(a.act) ? 1 : 0;
+  if (!a.far(o << gated) && !(gated && a.far((o << gated) + 1))) return;
+  const float g = a.sum(o << gated), u = gated ? a.sum((o << gated) + 1) : 0.f;
+  float v = g;
+  switch (a.act) {
+    case MOE_ACT_RELU2: v = bs_act<MOE_ACT_RELU2>(g); break;
+    case MOE_ACT_SILU: v = bs_act<MOE_ACT_SILU>(g); break;
+    case MOE_ACT_GELU: v = bs_act<MOE_ACT_GELU>(g); break;
+    case MOE_ACT_GLU_CLAMP: v = bs_gated<MOE_ACT_GLU_CLAMP>(g, u, a.limit, a.alpha); break;
+    case MOE_ACT_SWIGLU: v = bs_gated<MOE_ACT_SWIGLU>(g, u, a.limit, a.alpha); break;
+  }
+  y[o] = from_f32<TO>(v);
+}
+
 // Codes [rows, bytes a row], read in boxes of box_rows x 128 with 128-byte swizzle.
 static inline int bs_make_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t bytes, int box_rows) {
   EncodeTiledFn fn = encode_tiled_fn();
@@ -143,9 +260,9 @@ int tib_quantize_rows(const void* x, int x_dtype, int64_t ldx, void* codes, int6
 int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, int x_rows, const float* x_scales, int64_t lds, const void* w,
                              const float* w_scales, int scale_rows, int pairs, void* y, int y_dtype, int64_t ldy, int M, int N, int K,
                              const int* offsets, const int* order, int experts, int top, int x_by_pair, int act, float limit, float alpha,
-                             const float* row_scale, int* error_word, cudaStream_t stream);
+                             const float* row_scale, int far_from, int far_span, int* error_word, cudaStream_t stream);
 int tib_block_scaled_2cta_experts();
 int tib_block_scaled_2cta(const void* x, const float* x_scales, int64_t lds, const void* w, const float* w_scales, int scale_rows, int pairs,
                           void* out, int out_dtype, int64_t ldo, int M, int N, int K, const int* offsets, const int* order, int experts, int act,
-                          float limit, float alpha, const float* row_scale, int* error_word, cudaStream_t stream);
+                          float limit, float alpha, const float* row_scale, int far_from, int far_span, int* error_word, cudaStream_t stream);
 }

@@ -59,6 +59,9 @@ __device__ __forceinline__ void b2_arrive_even(uint32_t cluster_bar) {
 }
 
 struct B2Args {
+  const unsigned char* x;      // codes [M, runs * 128]
+  const unsigned char* w;      // codes in blocks
+  BsFar far;
   const float* x_scales;       // [runs, lds]
   int64_t lds;
   const float* w_scales;       // [rows of scales, runs]
@@ -72,11 +75,37 @@ struct B2Args {
 
 struct B2Tile { int expert, first, rows, n_tile; };      // rows first .. first + rows - 1 of x (at most 256), features n_tile * 256 ..
 
+// Rows row0 .. of a warp in a tile whose outputs are `first` ..: those outputs that have a far scale, made again, a lane an output.
+template <int ACT, typename TO>
+__device__ __noinline__ void b2_rows_apart(const B2Args* args, int row0, int rows, int expert, int first, TO* __restrict__ out, int64_t ldo) {
+  const B2Args& a = *args;
+  constexpr int kGated = moe_act_gated(ACT);
+  const int lane = threadIdx.x & 31;
+  bool outside = false;
+  if (lane < rows)
+    for (int b = 0; b < a.runs; ++b) {
+      const float scale = a.x_scales[(size_t)b * a.lds + row0 + lane];
+      outside |= a.far.outside(scale) && !isnan(scale);
+    }
+  for (uint32_t rest = __ballot_sync(0xffffffffu, outside); rest; rest &= rest - 1) {
+    const int r = row0 + __ffs(rest) - 1;
+    BsApart<uint8_t> apart;
+    apart.x = a.x + (size_t)r * a.runs * kBlk;
+    apart.x_scales = a.x_scales + r;
+    apart.lds = a.lds; apart.pairs = a.pairs; apart.runs = a.runs; apart.K = 0; apart.act = ACT;
+    apart.limit = a.ep.limit; apart.alpha = a.ep.alpha;
+    apart.row_scale = a.ep.row_scale ? a.ep.row_scale[bs_pair(a.order, r, a.M)] : 1.f;
+    apart.w = a.w + ((size_t)expert * ((a.N + 127) >> 7) * a.runs << 14);
+    apart.w_scales = a.w_scales + (size_t)expert * a.scale_rows * a.runs;
+    for (int c = first + lane; c < min(first + (128 >> kGated), a.N >> kGated); c += 32) bs_output_apart<uint8_t, TO>(apart, c, out + (size_t)r * ldo);
+  }
+}
+
 // Persistent: pair p walks the tiles t = p, p + pairs, ...  Of one matrix, tile t is row tile t % m_tiles of feature tile t / m_tiles, so pairs that run
 // together share slices of w; of rows sorted by expert, feature tiles run fastest.
 template <int ACT, typename TO>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kB2Threads, 1)
-block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const B2Args a,
+block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ B2Args a,
                          TO* __restrict__ out, int64_t ldo, int wide_stores) {
   extern __shared__ unsigned char smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -160,7 +189,7 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     int b = 0;
     uint32_t acc_phase = 0;
-    bool ok = true;
+    bool ok = true, outside = false;           // (outside: a run of one of this thread's rows, of BsFar's range)
     for (int t = pair; t < num_tiles && ok; t += pairs) {
       const B2Tile m = tile_of(t);
       const int in_tile = (int)rank * 128 + quarter * 32 + lane, row = m.first + in_tile, last = m.first + m.rows;      // (rows from `last` on are not stored)
@@ -181,6 +210,7 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
         x[i] = xs[(size_t)at * a.lds]; e[i] = we[at]; o[i] = wo[at];
       }
       auto step = [&](int kb, int i) {
+        outside |= a.far.outside(x[i]);
         const f32x2 scale = f2_pack(x[i] * e[i], x[i] * o[i]);
         const int at = min(kb + 2, a.runs - 1);
         x[i] = xs[(size_t)at * a.lds]; e[i] = we[at]; o[i] = wo[at];
@@ -280,6 +310,12 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
         __syncwarp();
       }
     }
+    if (__any_sync(0xffffffffu, outside) && ok)      // (behind all tiles: among them it would take registers from their loop)
+      for (int t = pair; t < num_tiles; t += pairs) {
+        const B2Tile m = tile_of(t);
+        const int row0 = (int)rank * 128 + quarter * 32;
+        if (row0 < m.rows) b2_rows_apart<ACT>(&a, m.first + row0, min(32, m.rows - row0), m.expert, (m.n_tile * 256 + half * 128) >> moe_act_gated(ACT), out, ldo);
+      }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;\n");
     if (warp == 0) {
@@ -379,9 +415,10 @@ TIB_API int tib_block_scaled_2cta_experts() { return kB2MaxExperts; }
 // x: codes [M, runs * 128] and scales [runs, lds] as tib_quantize_rows leaves them; w: codes in blocks [experts, ceil(N / 128), runs, 128, 128] and
 // scales [experts, scale_rows, runs] (`pairs`: of (gate, up) row pairs, N and scale_rows even); out: [M, N] in out_dtype (row stride ldo), or [M, N / 2] of a
 // gated activation.  offsets [experts + 1] and order [M]: rows sorted by expert, at most kB2MaxExperts of them; offsets null: one matrix for all rows.
+// far_from, far_span: see BsFar.
 TIB_API int tib_block_scaled_2cta(const void* x, const float* x_scales, int64_t lds, const void* w, const float* w_scales, int scale_rows, int pairs,
                                   void* out, int out_dtype, int64_t ldo, int M, int N, int K, const int* offsets, const int* order, int experts, int act,
-                                  float limit, float alpha, const float* row_scale, int* error_word, cudaStream_t stream) {
+                                  float limit, float alpha, const float* row_scale, int far_from, int far_span, int* error_word, cudaStream_t stream) {
   if (M == 0 || N == 0) return TIB_OK;
   if (!x || !x_scales || !w || !w_scales || !out || M < 0 || N < 0 || K < 1 || scale_rows < 1 || experts < 1) return TIB_E_ARG;
   if ((offsets && !order) || (row_scale && !order)) return TIB_E_ARG;
@@ -390,6 +427,7 @@ TIB_API int tib_block_scaled_2cta(const void* x, const float* x_scales, int64_t 
   if (out_dtype != TIB_BF16 && out_dtype != TIB_F32) return TIB_E_DTYPE;
   if (((uintptr_t)x | (uintptr_t)w) & 15) return TIB_E_ALIGN;
   B2Args a;
+  a.x = static_cast<const unsigned char*>(x); a.w = static_cast<const unsigned char*>(w); a.far = BsFar{(uint32_t)far_from, (uint32_t)far_span};
   a.x_scales = x_scales; a.lds = lds; a.w_scales = w_scales; a.scale_rows = scale_rows; a.pairs = pairs;
   a.M = M; a.N = N; a.runs = ceil_div(K, kBlk); a.offsets = offsets; a.order = order; a.experts = experts; a.error_word = error_word;
   a.ep.act = act; a.ep.limit = limit; a.ep.alpha = alpha; a.ep.row_scale = row_scale;

@@ -48,6 +48,8 @@ struct BsTile { int expert, first, rows, feature; };
 
 struct BsArgs {
   const void* x;               // codes [rows, runs * 128], or rows of the activations' type
+  const unsigned char* w;      // codes in blocks
+  BsFar far;
   int64_t ldx;                 // (of the latter)
   const float* x_scales;       // [runs, lds] beside codes
   int64_t lds;
@@ -60,6 +62,11 @@ struct BsArgs {
   MoeEpilogue ep;
   int* error_word;
 };
+
+__device__ __forceinline__ int bs_source(const BsArgs& a, const BsTile& m, int r) {      // the row of x that the tile's row r is
+  const int at = m.first + min(r, m.rows - 1);
+  return a.offsets && a.x_by_pair ? min(bs_pair(a.order, at, a.M) / a.top, a.x_rows - 1) : at;
+}
 
 __device__ __forceinline__ void umma_f8_warp(uint32_t leader, uint32_t tmem_d, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
   asm volatile("{\n.reg .pred p, q;\n.reg .b64 a, b;\nmov.b64 a, {%1, %6};\nmov.b64 b, {%2, %6};\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
@@ -168,6 +175,32 @@ __device__ __forceinline__ void bs_finish(const float* red, int log_splits, int 
   }
 }
 
+// The outputs of a block's share of a tile that have a far scale, made again by a warp.
+template <typename TX, typename TO>
+__device__ __forceinline__ void bs_tile_apart(const BsArgs& a, const BsTile& m, int rank, int splits, int lane, TO* __restrict__ y, int64_t ldy) {
+  constexpr bool kCodes = std::is_same_v<TX, uint8_t>;
+  const int gated = moe_act_gated(a.ep.act) ? 1 : 0, outs = 128 / splits >> gated, first = (m.feature >> gated) + rank * outs, n_out = a.N >> gated;
+#pragma unroll 1
+  for (int c = 0; c < m.rows; ++c) {
+    BsApart<TX> apart;
+    apart.x = static_cast<const TX*>(a.x) + (kCodes ? (size_t)(m.first + c) * a.runs * kBlk : (size_t)bs_source(a, m, c) * a.ldx);
+    apart.x_scales = a.x_scales + (kCodes ? m.first + c : 0);
+    apart.lds = a.lds; apart.pairs = a.pairs; apart.runs = a.runs; apart.K = a.K; apart.act = a.ep.act;
+    apart.limit = a.ep.limit; apart.alpha = a.ep.alpha;
+    bool outside = false;
+    for (int kb = lane; kb < a.runs; kb += 32) {
+      float inverse;
+      const float scale = apart.run_scale(kb, inverse);
+      outside |= a.far.outside(scale) && !isnan(scale);
+    }
+    if (!__any_sync(0xffffffffu, outside)) continue;
+    apart.row_scale = a.ep.row_scale ? a.ep.row_scale[bs_pair(a.order, m.first + c, a.M)] : 1.f;
+    apart.w = a.w + ((size_t)m.expert * ((a.N + 127) >> 7) * a.runs << 14);
+    apart.w_scales = a.w_scales + (size_t)m.expert * a.scale_rows * a.runs;
+    for (int o = first + lane; o < min(first + outs, n_out); o += 32) bs_output_apart<TX, TO>(apart, o, y + (size_t)(m.first + c) * ldy);
+  }
+}
+
 template <int NT, typename TX, typename TO>
 __global__ void __launch_bounds__(BsShape<NT, std::is_same_v<TX, uint8_t>>::kThreads, BsShape<NT, std::is_same_v<TX, uint8_t>>::kPerSm)
 block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const BsArgs a,
@@ -185,7 +218,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
   auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * kBsMaxStages + S::kBufs + b); };
   auto scale_full_bar = [&](int i) { return bars + 8u * (2 * kBsMaxStages + 2 * S::kBufs + i); };
   auto scale_empty_bar = [&](int slot) { return bars + 8u * (2 * kBsMaxStages + 2 * S::kBufs + kBsSlots + slot / 4); };      // (four slots are freed together)
-  const uint32_t red_bar = bars + 8u * (2 * kBsMaxStages + 2 * S::kBufs + kBsSlots + kBsSlots / 4), tmem_slot = red_bar + 8;
+  const uint32_t red_bar = bars + 8u * (2 * kBsMaxStages + 2 * S::kBufs + kBsSlots + kBsSlots / 4), tmem_slot = red_bar + 8, far_seen = red_bar + 12;      // (not 0: some row's scale is outside, BsFar)
   static_assert(8 * (2 * kBsMaxStages + 2 * S::kBufs + kBsSlots + kBsSlots / 4) + 16 <= kBsBarBytes, "the barriers' share of shared memory");
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem_gen + (tmem_slot - base));
   float* step_scales = reinterpret_cast<float*>(smem_gen + (bars - base) + kBsBarBytes);  // [kBsSlots][kScales]
@@ -211,7 +244,10 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
       mbar_init(acc_full_bar(lane), 1);
       mbar_init(acc_empty_bar(lane), S::kStorers);
     }
-    if (lane == 0) mbar_init(red_bar, 1);
+    if (lane == 0) {
+      mbar_init(red_bar, 1);
+      *reinterpret_cast<uint32_t*>(smem_gen + (far_seen - base)) = 0;
+    }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 1) {
@@ -271,6 +307,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     return m;
   };
   auto w_row = [&](const BsTile& m, int kb) { return ((m.expert * f_tiles + (m.feature >> 7)) * a.runs + kb) << 7; };      // of the tile's block in the matrix of blocks
+
   auto source = [&](const BsTile& m, int r) {     // the row of x that the tile's row r is
     const int at = m.first + min(r, m.rows - 1);
     return a.offsets && a.x_by_pair ? min(bs_pair(a.order, at, a.M) / a.top, a.x_rows - 1) : at;
@@ -473,7 +510,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     const int helper = warp - 2 - S::kStorers;
     int kb = kb0 + helper, step = helper, s = helper % a.stages, slot = helper;      // (step: counted over all tiles)
     uint32_t phase = 1 ^ ((helper / a.stages) & 1), slot_phase = 1;
-    bool ok = true, waited = a.offsets != nullptr;
+    bool ok = true, waited = a.offsets != nullptr, outside = false;
     auto advance = [&]() {
       kb += S::kHelpers;
       step += S::kHelpers;
@@ -507,6 +544,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
             float* scales = step_scales + slot * S::kScales;
 #pragma unroll
             for (int i = 0; i < NT / 32; ++i) {
+              outside |= a.far.outside(v[j][i]);
               scales[lane + 32 * i] = v[j][i] * even[j];
               scales[NT + 8 + lane + 32 * i] = v[j][i] * odd[j];
             }
@@ -559,6 +597,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
             for (int o = 1; o < 8; o <<= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
             float scale, inverse;
             bs_run_scale(largest, scale, inverse);
+            outside |= a.far.outside(scale);
             if (r < m.rows) {
               *reinterpret_cast<uint4*>(codes + r * kBlk + ((eighth ^ (r & 7)) << 4)) = bs_codes16<TX>(now.raw[h], inverse);
               if (eighth == 0) {
@@ -590,6 +629,8 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
       }
       if (!ok && a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00C6);
     }
+    if (outside)      // (any block of the cluster finishes outputs of these rows)
+      for (int r = 0; r < splits; ++r) st_cluster_u32(map_to_cta(far_seen, r), 1u);
   }
   __syncwarp();
   if (splits > 1) {
@@ -602,6 +643,9 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
   }
+  // Rows with far scales: by the producer's warp, whose instructions here delay no other.  
+  if (warp == 0 && *reinterpret_cast<volatile uint32_t*>(smem_gen + (far_seen - base)))
+    for (int t = cluster_id; t < num_tiles; t += clusters) bs_tile_apart<TX, TO>(a, tile_of(t), rank, splits, lane, y, ldy);
 }
 
 template <int NT>
@@ -678,11 +722,12 @@ using namespace tib;
 // 128 features; -1: codes
 // [x_rows, runs * 128] and scales [runs, lds] as tib_quantize_rows leaves them, row m of them for row m of y.  w: codes in blocks
 // [experts, ceil(N / 128), runs, 128, 128], features and columns behind the last zero, and scales [experts, scale_rows, runs] (`pairs`: of (gate, up) row pairs); y: [M, N] in y_dtype (row stride ldy), or [M, N / 2] of a gated activation.
-// offsets [experts + 1] and order [M]: rows sorted by expert as tib_moe_expert_product takes them; offsets null: one matrix for all rows.
+// offsets [experts + 1] and order [M]: rows sorted by expert as tib_moe_expert_product takes them; offsets null: one matrix for all rows.  far_from, far_span:
+// which rows' scales keep normal with every one of w's (BsFar).
 TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, int x_rows, const float* x_scales, int64_t lds, const void* w,
                                      const float* w_scales, int scale_rows, int pairs, void* y, int y_dtype, int64_t ldy, int M, int N, int K,
                                      const int* offsets, const int* order, int experts, int top, int x_by_pair, int act, float limit,
-                                     float alpha, const float* row_scale, int* error_word, cudaStream_t stream) {
+                                     float alpha, const float* row_scale, int far_from, int far_span, int* error_word, cudaStream_t stream) {
   if (M == 0 || N == 0) return TIB_OK;
   const bool is_codes = x_dtype < 0;
   if (!x || !w || !w_scales || !y || M < 0 || N < 0 || K < 1 || experts < 1 || top < 1 || x_rows < 1) return TIB_E_ARG;
@@ -692,7 +737,8 @@ TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, in
   if (experts > kBsMaxExperts || (int64_t)experts * ceil_div(N, 128) * ceil_div(K, kBlk) > (0x7fffffff >> 7)) return TIB_E_SIZE;
   if ((((uintptr_t)w) & 15) || (is_codes && (((uintptr_t)x) & 15))) return TIB_E_ALIGN;
   BsArgs a;
-  a.x = x; a.ldx = ldx; a.x_scales = x_scales; a.lds = lds; a.w_scales = w_scales; a.scale_rows = scale_rows; a.pairs = pairs;
+  a.x = x; a.w = static_cast<const unsigned char*>(w); a.far = BsFar{(uint32_t)far_from, (uint32_t)far_span}; a.ldx = ldx;
+  a.x_scales = x_scales; a.lds = lds; a.w_scales = w_scales; a.scale_rows = scale_rows; a.pairs = pairs;
   a.vec = !is_codes && ((uintptr_t)x & 15) == 0 && (ldx * (x_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
   a.wide = ((uintptr_t)y & 15) == 0 && (ldy * (y_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
   a.M = M; a.N = N; a.K = K; a.x_rows = x_rows; a.runs = ceil_div(K, kBlk); a.offsets = offsets; a.order = order; a.experts = experts; a.top = top;
