@@ -16,6 +16,35 @@ def random_matrix(n, k, seed, device="cpu", sizes=(0.02, 3.0)):
     return BlockScaledMatrix(codes.to(torch.float8_e4m3fn).to(device), scales.to(device))
 
 
+# Products that between them take every way through the kernels: (rows, columns, features, (rows of a tile, blocks that share it, steps of a block, stages of its
+# ring)).  Rings wrap where a block has more steps than stages, the ring of scales of tiles of up to 128 rows from 17 steps on; features that are no whole
+# blocks, columns that are no whole runs, more tiles than blocks among them.
+PLAIN_PATHS = [
+    (8, 4096, 9600, (16, 2, 16, 5)), (8, 4096, 19200, (16, 1, 32, 5)), (7, 600, 38530, (16, 1, 10, 5)), (8, 8320, 500, (16, 8, 9, 5)), (3, 4000, 3201, (16, 4, 8, 5)),
+    (20, 2500, 19200, (32, 1, 20, 4)), (31, 300, 38530, (32, 1, 6, 4)), (20, 8320, 500, (32, 8, 9, 4)), (9, 4096, 3001, (32, 4, 8, 4)), (17, 4096, 9100, (32, 2, 16, 4)),
+    (64, 8320, 500, (64, 8, 9, 7)), (64, 8320, 3200, (64, 4, 17, 7)), (50, 8320, 9001, (64, 2, 33, 7)), (520, 4096, 1280, (64, 1, 32, 7)), (50, 1100, 19300, (64, 1, 18, 7)),
+    (100, 2500, 19200, (128, 1, 40, 4)), (128, 1100, 9601, (128, 1, 9, 4)), (1000, 1100, 2300, (128, 1, 9, 4)),
+    (1100, 1100, 4001, (256, 1, 18, 6)), (700, 2600, 4001, (256, 1, 21, 6)), (2000, 128, 5000, (256, 1, 3, 6))]
+# The same with a gate and an up matrix of half the features each.
+GATED_PATHS = [
+    (8, 4096, 19200, (16, 1, 32, 5)), (5, 8320, 500, (16, 8, 9, 5)), (20, 2500, 19206, (32, 1, 20, 4)), (50, 8320, 9002, (64, 2, 33, 7)), (520, 4096, 1280, (64, 1, 32, 7)),
+    (100, 2500, 19202, (128, 1, 40, 4)), (1100, 1100, 4006, (256, 1, 18, 6)), (700, 2600, 4002, (256, 1, 21, 6))]
+# Rows sorted by expert: (pairs, experts, columns, features, ...); steps are those of the most tiles that so many pairs may be.
+EXPERT_PATHS = [
+    (250, 32, 2100, 2050, (16, 1, 51, 5)), (840, 28, 1200, 1416, (32, 1, 30, 4)), (31200, 240, 1100, 200, (128, 1, 63, 4)), (2400, 6, 1200, 2001, (256, 1, 20, 6)),
+    (22300, 223, 300, 130, (256, 1, 15, 6))]
+
+
+def plan(rows, columns, features, experts=0):
+    """The library's own account of how such a product runs."""
+    import ctypes
+    from torchinferno_b200.kernels import block_scaled, ops
+    few = rows <= (block_scaled.FEW_EXPERT_ROWS * experts if experts else block_scaled.FEW_ROWS)
+    found = (ctypes.c_int * 4)()
+    assert ops.lib().tib_block_scaled_plan(int(not few), rows, features, columns, experts, ctypes.addressof(found)) == 0
+    return tuple(found)
+
+
 def matrix64(matrix):
     n, k = matrix.shape
     at_n, at_k = torch.arange(n, device=matrix.device) // BLOCK, torch.arange(k, device=matrix.device) // BLOCK

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from block_scaled_oracle import matrix64, random_matrix, rows64
+from block_scaled_oracle import EXPERT_PATHS, GATED_PATHS, PLAIN_PATHS, matrix64, plan, random_matrix, rows64
 from torchinferno_b200.kernels import gemm, ops
 from torchinferno_b200.kernels.block_scaled import BlockScaledExperts, BlockScaledMatrix, BlockScaledWeight, quantize_matrix, quantize_rows
 
@@ -118,6 +118,35 @@ def test_the_oracle_rounds_as_e4m3_does():
     v = torch.cat([v, torch.full((len(v), 1), 448.0)], 1)                      # (so that every run's scale is 1)
     c, s = rows64(v)
     assert (s == 1).all() and torch.equal(c.float(), v.to(CODES).float())
+
+
+# ------------------------------------------------------------------------------------------------ which kernel runs, and how
+def test_the_ways_through_the_kernels_are_those_that_the_gpu_tests_name():
+    """Each of their sizes runs as it says, and between them they take every tile and split there is, with rings that wrap."""
+    for rows, columns, features, want in (*PLAIN_PATHS, *GATED_PATHS):
+        assert plan(rows, columns, features) == want, (rows, columns, features)
+    for pairs, experts, columns, features, want in EXPERT_PATHS:
+        assert plan(pairs, columns, features, experts) == want, (pairs, experts, columns, features)
+    found = {plan(m, k, 128 * f)[:2] for m in (*range(1, 140, 3), *range(140, 2000, 117)) for f in range(1, 320) for k in (128, 1024, 4096, 8192)}
+    assert found == {want[:2] for *_, want in PLAIN_PATHS}
+    assert not {tiles for tiles in found if tiles[0] >= 128 and tiles[1] > 1}
+    for paths in (PLAIN_PATHS, GATED_PATHS, EXPERT_PATHS):
+        for rows in (16, 32, 64, 128, 256):
+            deep = [want for *_, want in paths if want[0] == rows]
+            assert any(steps > max(stages, 16 if rows <= 128 else 0) for _, _, steps, stages in deep) or (paths is EXPERT_PATHS and rows == 64)
+    # more tiles than blocks, for each height of a tile
+    blocks_of = {16: 296, 32: 296, 64: 148, 128: 148, 256: 74}
+    for rows, blocks in blocks_of.items():
+        edge = 256 if rows == 256 else 128
+        assert any(want[0] == rows and want[1] == 1 and -(-m // rows) * -(-n // edge) > blocks for m, _, n, want in PLAIN_PATHS)
+
+
+@pytest.mark.parametrize("codes, m, n, k, experts", [(0, 0, 8, 8, 0), (1, 8, 0, 8, 0), (1, 8, 8, 0, 0), (1, 8, 8, 8, -1), (0, 8, 8, 8, 1025)])
+def test_no_plan_for_no_product(codes, m, n, k, experts):
+    import ctypes
+    found = (ctypes.c_int * 4)()
+    assert ops.lib().tib_block_scaled_plan(codes, m, n, k, experts, ctypes.addressof(found)) < 0
+    assert ops.lib().tib_block_scaled_plan(1, 8, 8, 8, 0, 0) < 0
 
 
 # ------------------------------------------------------------------------------------------------ checkpoints

@@ -70,6 +70,17 @@ static bool on_pairs_of_sms(int rows, int features) { return rows > 128 && (int6
 // 96 28.2 / 29.2, 128 37.2 / 29.8, 192 47.8 / 32.6, 256 60.7 / 45.1, 512 98.4 / 71.4; gated, 256: 95.3 / 73.9.)
 constexpr int kBsPairRows = 100;
 
+static bool takes_pairs_of_sms(int M, int N, int experts) {      // experts: 0 for one matrix
+  return experts ? M >= (int64_t)experts * kBsPairRows && experts <= tib_block_scaled_2cta_experts() : on_pairs_of_sms(M, N);
+}
+
+// How a product runs whose rows come as they are (codes 0) or as codes: {rows of a tile at most, blocks that share a tile, steps of a block at most, stages of its
+// ring}; tiles of 256 rows are those of pairs of SMs.  experts: 0 for one matrix.
+TIB_API int tib_block_scaled_plan(int codes, int M, int N, int K, int experts, int* plan) {
+  if (!codes || !takes_pairs_of_sms(M, N, experts)) return tib_block_scaled_tcgen05_plan(codes, M, N, K, experts, plan);
+  return tib_block_scaled_2cta_plan(M, N, K, experts, plan);
+}
+
 // A product as its callers see it: rows x [x_rows, K] times matrices in blocks (the other arguments as tib_block_scaled_tcgen05).  codes: where the rows'
 // codes [M, runs * 128] and scales [runs, M rounded up to 4] go, ahead of the product (`make`; not made: they are there from a call before); null: the
 // product's kernel quantises the rows itself.
@@ -91,7 +102,7 @@ TIB_API int tib_block_scaled_product(const void* x, int x_dtype, int64_t ldx, in
                                      gather ? offsets + experts : nullptr, x_rows, stream);
     if (rc != TIB_OK) return rc;
   }
-  if (offsets ? M >= (int64_t)experts * kBsPairRows && experts <= tib_block_scaled_2cta_experts() : on_pairs_of_sms(M, N))
+  if (takes_pairs_of_sms(M, N, offsets ? experts : 0))
     return tib_block_scaled_2cta(codes, scales, lds, w, w_scales, scale_rows, pairs, y, y_dtype, ldy, M, N, K, offsets, order, experts, act, limit, alpha,
                                  row_scale, far_from, far_span, error_word, stream);
   return tib_block_scaled_tcgen05(codes, -1, 0, M, scales, lds, w, w_scales, scale_rows, pairs, y, y_dtype, ldy, M, N, K, offsets, order, experts, top, 0, act,
@@ -101,3 +112,4 @@ TIB_API int tib_block_scaled_product(const void* x, int x_dtype, int64_t ldx, in
 // The calls the Python parts make (common.cuh).
 TIB_PACKED(tib_quantize_rows)
 TIB_PACKED(tib_block_scaled_product)
+TIB_PACKED(tib_block_scaled_plan)

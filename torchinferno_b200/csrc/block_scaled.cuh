@@ -261,7 +261,9 @@ int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, int x_rows
                              const float* w_scales, int scale_rows, int pairs, void* y, int y_dtype, int64_t ldy, int M, int N, int K,
                              const int* offsets, const int* order, int experts, int top, int x_by_pair, int act, float limit, float alpha,
                              const float* row_scale, int far_from, int far_span, int* error_word, cudaStream_t stream);
+int tib_block_scaled_tcgen05_plan(int codes, int M, int N, int K, int experts, int* plan);
 int tib_block_scaled_2cta_experts();
+int tib_block_scaled_2cta_plan(int M, int N, int K, int experts, int* plan);
 int tib_block_scaled_2cta(const void* x, const float* x_scales, int64_t lds, const void* w, const float* w_scales, int scale_rows, int pairs,
                           void* out, int out_dtype, int64_t ldo, int M, int N, int K, const int* offsets, const int* order, int experts, int act,
                           float limit, float alpha, const float* row_scale, int far_from, int far_span, int* error_word, cudaStream_t stream);

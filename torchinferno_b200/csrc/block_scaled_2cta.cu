@@ -388,6 +388,10 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
   }
 }
 
+static int64_t b2_tiles(int M, int N, int experts) {      // at most; experts: 0 for one matrix
+  return (int64_t)(experts ? M / 256 + (M < experts ? M : experts) : ceil_div(M, 256)) * ceil_div(N, 256);
+}
+
 template <int ACT, typename TO>
 static int launch_b2(const CUtensorMap& map_x, const CUtensorMap& map_w, const B2Args& a, void* out, int64_t ldo, cudaStream_t stream) {
   auto kern = block_scaled_2cta_kernel<ACT, TO>;
@@ -397,8 +401,7 @@ static int launch_b2(const CUtensorMap& map_x, const CUtensorMap& map_w, const B
   if (e == cudaSuccess && !(device < 64 && allowed[device])) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
   if (e != cudaSuccess) return (int)e;
   if (device < 64) allowed[device] = true;
-  const int64_t row_tiles = a.offsets ? a.M / 256 + (a.M < a.experts ? a.M : a.experts) : ceil_div(a.M, 256);
-  const int64_t tiles = row_tiles * ceil_div(a.N, 256);
+  const int64_t tiles = b2_tiles(a.M, a.N, a.offsets ? a.experts : 0);
   if (tiles > 0x7fffffff) return TIB_E_SIZE;
   const int wide = ((uintptr_t)out & 15) == 0 && (ldo * sizeof(TO)) % 16 == 0;
   TIB_LAUNCH_DEPENDENT(kern, 2 * (int)(tiles < 74 ? tiles : 74), kB2Threads, kB2Smem + (a.offsets ? 8 * (a.experts + 1) : 0), stream, map_x, map_w, a, (TO*)out,
@@ -411,6 +414,14 @@ static int launch_b2(const CUtensorMap& map_x, const CUtensorMap& map_w, const B
 using namespace tib;
 
 TIB_API int tib_block_scaled_2cta_experts() { return kB2MaxExperts; }
+
+// See tib_block_scaled_plan.
+TIB_API int tib_block_scaled_2cta_plan(int M, int N, int K, int experts, int* plan) {
+  if (!plan || M < 1 || N < 1 || K < 1 || experts < 0 || experts > kB2MaxExperts) return TIB_E_ARG;
+  const int64_t tiles = b2_tiles(M, N, experts), steps = ceil_div(K, kBlk) * ceil_div64(tiles, tiles < 74 ? tiles : 74);
+  plan[0] = 256; plan[1] = 1; plan[2] = (int)(steps < 0x7fffffff ? steps : 0x7fffffff); plan[3] = kB2Stages;
+  return TIB_OK;
+}
 
 // x: codes [M, runs * 128] and scales [runs, lds] as tib_quantize_rows leaves them; w: codes in blocks [experts, ceil(N / 128), runs, 128, 128] and
 // scales [experts, scale_rows, runs] (`pairs`: of (gate, up) row pairs, N and scale_rows even); out: [M, N] in out_dtype (row stride ldo), or [M, N / 2] of a

@@ -207,7 +207,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
                             TO* __restrict__ y, int64_t ldy) {
   constexpr bool kCodes = std::is_same_v<TX, uint8_t>;
   using S = BsShape<NT, kCodes>;
-  const int splits = (int)cluster_size(), rank = (int)cluster_rank();
+  const int splits = NT >= 128 ? 1 : (int)cluster_size(), rank = NT >= 128 ? 0 : (int)cluster_rank();
   extern __shared__ unsigned char smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* smem_gen = smem_raw + (base - smem_u32(smem_raw));
@@ -654,20 +654,56 @@ static constexpr uint32_t bs_smem(int stages, int splits, int experts) {
   return 1024u + stages * S::kStage + kBsBarBytes + 4 * (kBsSlots * S::kScales + bs_red_floats<NT>(splits) + 2 * (experts + 1));
 }
 
-template <int NT, typename TX, typename TO>
-static int launch_block_scaled(const CUtensorMap& map_w, const CUtensorMap& map_x, BsArgs& a, void* y, int64_t ldy, int splits, cudaStream_t stream) {
-  const int experts = a.offsets ? a.experts : 0;
-  const int64_t row_tiles = a.offsets ? a.M / NT + (a.M < a.experts ? a.M : a.experts) : ceil_div(a.M, NT);
-  const int64_t tiles = row_tiles * ceil_div(a.N, 128);
-  if (tiles * splits > 0x7fffffff) return TIB_E_SIZE;
-  constexpr int kBlocks = 148 * BsShape<NT, std::is_same_v<TX, uint8_t>>::kPerSm;
-  const int grid = (int)(splits > 1 ? tiles * splits : tiles < kBlocks ? tiles : kBlocks);      // (a cluster has one tile: its sums' place is used once)
-  const int64_t steps = (int64_t)ceil_div(a.runs, splits) * ceil_div64(tiles * splits, grid);      // of a block, at most
-  a.stages = 1;
-  while (a.stages < kBsMaxStages && a.stages < steps && bs_smem<NT>(a.stages + 1, splits, experts) <= (kBlocks > 148 ? 113u * 1024 : (uint32_t)kMostSmem)) ++a.stages;
+// The blocks that share a tile's runs: 8, 4 or 2 where there is room for them beside the other tiles' and the runs are enough to pay for the exchange.
+// (us by 1 / 2 / 4 / 8 blocks a tile: 8 rows 4,096 -> 4,096 14.2 / 9.8 / 8.3 / 9.0, 14,336 -> 4,096 43 / 25 / 16.7 / 15.0, 4,096 -> 6,144 14.2 / 10.6 /
+// 9.1 / 14.8, 2,048 -> 2,048 8.2 / 6.5 / 5.9 / 6.1; 4 rows 512 -> 1,024 4.0 / 4.5 / 4.3; 20 rows 512 -> 1,024 5.5 / 6.3 / 5.9.)
+static int bs_splits(int64_t tiles, int runs, int blocks) {
+  if (tiles * 8 <= blocks && runs >= 64) return 8;
+  if (tiles * 4 <= blocks && runs >= 8) return 4;
+  return tiles * 2 <= blocks && runs >= 8 ? 2 : 1;
+}
+// Rows of a tile of codes: the fewest that give no more tiles than SMs; of a long matrix (64 runs) not fewer than 64 while there are that many rows, as every row tile
+// reads the weights again.  (us in tiles of 32 / 64 / 128 rows: 333 rows 1,000 -> 1,302 8.2 / 9.5 / 11.4, 128 rows 4,096 -> 4,096 13.7 / 14.1 / 15.6, 256 rows
+// 18.0 / 16.7 / 20.0, 100 rows 2,048 -> 2,048 8.9 / 10.2 / 11.8, 64 rows 14,336 -> 4,096 19.2 / 18.1 / 25.5, 128 rows 28.1 / 26.1 / 26.3, 128 rows 4,096 ->
+// 14,336 29.2 / 27.9 / 24.9.)
+static int bs_tile_rows(int rows, int features, int runs) {
+  const int64_t f_tiles = ceil_div(features, 128);
+  if (rows <= 32 || (ceil_div(rows, 32) * f_tiles <= 148 && runs < 64)) return 32;
+  return rows <= 64 || ceil_div(rows, 64) * f_tiles <= 148 ? 64 : 128;
+}
+
+// How a product runs: blocks in the grid, those that share a tile, steps of a block at most, stages of its ring.
+struct BsPlan { int grid, splits, steps, stages; };
+template <int NT, bool CODES> static int bs_plan(int M, int N, int runs, int experts, BsPlan& p) {      // experts: 0 for one matrix
+  using S = BsShape<NT, CODES>;
+  constexpr int kBlocks = 148 * S::kPerSm;
+  const int64_t row_tiles = experts ? M / NT + (M < experts ? M : experts) : ceil_div(M, NT), tiles = row_tiles * ceil_div(N, 128);
+  // (a tile of 128 rows is never shared: bs_tile_rows takes such tiles where smaller ones are more than the SMs)
+  p.splits = experts || NT >= 128 ? 1 : bs_splits(tiles, runs, CODES ? 148 : 296);
+  if (tiles * p.splits > 0x7fffffff) return TIB_E_SIZE;
+  p.grid = (int)(p.splits > 1 ? tiles * p.splits : tiles < kBlocks ? tiles : kBlocks);      // (a cluster has one tile: its sums' place is used once)
+  const int64_t steps = (int64_t)ceil_div(runs, p.splits) * ceil_div64(tiles * p.splits, p.grid);
+  p.steps = (int)(steps < 0x7fffffff ? steps : 0x7fffffff);
+  p.stages = 1;
+  while (p.stages < kBsMaxStages && p.stages < p.steps && bs_smem<NT>(p.stages + 1, p.splits, experts) <= (S::kPerSm > 1 ? 113u * 1024 : (uint32_t)kMostSmem)) ++p.stages;
   // (A wait by parity tells a stage's last use from the one before only while a helper's step before implies the latter is over: with no more helpers
   // than stages, or every stage used once.)
-  if (!std::is_same_v<TX, uint8_t> && a.stages < BsShape<NT, false>::kHelpers && a.stages < steps) return TIB_E_SMEM;
+  return !CODES && p.stages < S::kHelpers && p.stages < p.steps ? TIB_E_SMEM : TIB_OK;
+}
+// Rows of a tile for rows given as codes.  (Of sorted rows tiles of 32 are ahead, or near, up to where pairs of SMs take over.  32 / 64 / 128 rows a tile, us: 25 rows
+// an expert 19.5 / 18.5 / 24.3, 50 21.5 / 25.0 / 25.6, 87 30.7 / 33.1 / 35.5, 32 of 28 experts 17.4 / 20.0 / 23.6; with a skew 16.2 / 16.2 / 20.7.)
+static int bs_code_rows(int M, int N, int runs, int experts) {
+  return !experts ? bs_tile_rows(M, N, runs) : M < (int64_t)experts * 128 ? 32 : 128;
+}
+
+template <int NT, typename TX, typename TO>
+static int launch_block_scaled(const CUtensorMap& map_w, const CUtensorMap& map_x, BsArgs& a, void* y, int64_t ldy, cudaStream_t stream) {
+  constexpr bool kCodes = std::is_same_v<TX, uint8_t>;
+  const int experts = a.offsets ? a.experts : 0;
+  BsPlan plan;
+  const int rc = bs_plan<NT, kCodes>(a.M, a.N, a.runs, experts, plan);
+  if (rc != TIB_OK) return rc;
+  a.stages = plan.stages;
   auto kern = block_scaled_tcgen05_kernel<NT, TX, TO>;
   static bool allowed[64];      // (by device: the attribute belongs to its context)
   int device = 0;
@@ -676,13 +712,13 @@ static int launch_block_scaled(const CUtensorMap& map_w, const CUtensorMap& map_
   if (e != cudaSuccess) return (int)e;
   if (device < 64) allowed[device] = true;
   cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(BsShape<NT, std::is_same_v<TX, uint8_t>>::kThreads);
-  cfg.dynamicSmemBytes = bs_smem<NT>(a.stages, splits, experts);
+  cfg.blockDim = dim3(BsShape<NT, kCodes>::kThreads);
+  cfg.dynamicSmemBytes = bs_smem<NT>(plan.stages, plan.splits, experts);
   cfg.stream = stream;
-  cfg.gridDim = dim3((unsigned)grid);
+  cfg.gridDim = dim3((unsigned)plan.grid);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)splits;
+  attr[0].val.clusterDim.x = (unsigned)plan.splits;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // (see launch_dependent in common.cuh)
@@ -693,25 +729,6 @@ static int launch_block_scaled(const CUtensorMap& map_w, const CUtensorMap& map_
   if (e != cudaSuccess) return (int)e;
   TIB_LAUNCH_CHECK();
   return TIB_OK;
-}
-
-// The blocks that share a tile's runs: 8, 4 or 2 where there is room for them beside the other tiles' and the runs are enough to pay for the exchange.
-// (us by 1 / 2 / 4 / 8 blocks a tile: 8 rows 4,096 -> 4,096 14.2 / 9.8 / 8.3 / 9.0, 14,336 -> 4,096 43 / 25 / 16.7 / 15.0, 4,096 -> 6,144 14.2 / 10.6 /
-// 9.1 / 14.8, 2,048 -> 2,048 8.2 / 6.5 / 5.9 / 6.1; 4 rows 512 -> 1,024 4.0 / 4.5 / 4.3; 20 rows 512 -> 1,024 5.5 / 6.3 / 5.9; in tiles of 128 rows, whose exchange
-// is the largest, 128 rows 4,096 -> 4,096 20 / 17 / 14.8, 100 rows 2,048 -> 2,048 12.5 / 12.8 / 11.3, 300 rows 13.0 / 13.7.)
-static int bs_splits(int64_t tiles, int runs, int nt, int blocks) {
-  if (tiles * 8 <= blocks && runs >= 64) return 8;
-  if (tiles * 4 <= blocks && runs >= (nt < 128 ? 8 : 16)) return 4;
-  return tiles * 2 <= blocks && runs >= (nt < 128 ? 8 : 32) ? 2 : 1;
-}
-// Rows of a tile of codes: the fewest that give no more tiles than SMs; of a long matrix (64 runs) not fewer than 64 while there are that many rows, as every row tile
-// reads the weights again.  (us in tiles of 32 / 64 / 128 rows: 333 rows 1,000 -> 1,302 8.2 / 9.5 / 11.4, 128 rows 4,096 -> 4,096 13.7 / 14.1 / 15.6, 256 rows
-// 18.0 / 16.7 / 20.0, 100 rows 2,048 -> 2,048 8.9 / 10.2 / 11.8, 64 rows 14,336 -> 4,096 19.2 / 18.1 / 25.5, 128 rows 28.1 / 26.1 / 26.3, 128 rows 4,096 ->
-// 14,336 29.2 / 27.9 / 24.9.)
-static int bs_tile_rows(int rows, int features, int runs) {
-  const int64_t f_tiles = ceil_div(features, 128);
-  if (rows <= 32 || (ceil_div(rows, 32) * f_tiles <= 148 && runs < 64)) return 32;
-  return rows <= 64 || ceil_div(rows, 64) * f_tiles <= 148 ? 64 : 128;
 }
 
 }  // namespace tib
@@ -752,14 +769,11 @@ TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, in
     rc = bs_make_map(&map_x, x, x_rows, (int64_t)a.runs * kBlk, 32);
     if (rc != TIB_OK) return rc;
   }
-  auto splits = [&](int nt) { return offsets ? 1 : bs_splits((int64_t)ceil_div(M, nt) * ceil_div(N, 128), a.runs, nt, is_codes ? 148 : 296); };
 #define TIB_BS_GO(NT, TX)                                                                                                  \
-  return y_dtype == TIB_BF16 ? launch_block_scaled<NT, TX, __nv_bfloat16>(map_w, map_x, a, y, ldy, splits(NT), stream)      \
-                             : launch_block_scaled<NT, TX, float>(map_w, map_x, a, y, ldy, splits(NT), stream)
+  return y_dtype == TIB_BF16 ? launch_block_scaled<NT, TX, __nv_bfloat16>(map_w, map_x, a, y, ldy, stream)                 \
+                             : launch_block_scaled<NT, TX, float>(map_w, map_x, a, y, ldy, stream)
   if (is_codes) {
-    // (Of sorted rows tiles of 32 are ahead, or near, up to where pairs of SMs take over.  32 / 64 / 128 rows a tile, us: 25 rows an expert 19.5 / 18.5 / 24.3, 50
-    // 21.5 / 25.0 / 25.6, 87 30.7 / 33.1 / 35.5, 32 of 28 experts 17.4 / 20.0 / 23.6; with a skew 16.2 / 16.2 / 20.7.)
-    const int nt = !offsets ? bs_tile_rows(M, N, a.runs) : M < (int64_t)experts * 128 ? 32 : 128;
+    const int nt = bs_code_rows(M, N, a.runs, offsets ? experts : 0);
     if (nt == 32) TIB_BS_GO(32, uint8_t);
     if (nt == 64) TIB_BS_GO(64, uint8_t);
     TIB_BS_GO(128, uint8_t);
@@ -767,4 +781,16 @@ TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, in
   if (x_dtype == TIB_BF16) TIB_BS_GO(16, __nv_bfloat16);
   TIB_BS_GO(16, float);
 #undef TIB_BS_GO
+}
+
+// How a product of M rows (codes, or not) with one matrix (experts 0) or sorted by expert runs here: {rows of a tile at most, blocks that share a tile, steps of a
+// block at most, stages of its ring}.
+TIB_API int tib_block_scaled_tcgen05_plan(int codes, int M, int N, int K, int experts, int* plan) {
+  if (!plan || M < 1 || N < 1 || K < 1 || experts < 0 || experts > kBsMaxExperts) return TIB_E_ARG;
+  const int runs = ceil_div(K, kBlk), nt = codes ? bs_code_rows(M, N, runs, experts) : 16;
+  BsPlan p;
+  const int rc = nt == 16 ? bs_plan<16, false>(M, N, runs, experts, p) : nt == 32 ? bs_plan<32, true>(M, N, runs, experts, p)
+               : nt == 64 ? bs_plan<64, true>(M, N, runs, experts, p) : bs_plan<128, true>(M, N, runs, experts, p);
+  plan[0] = nt; plan[1] = p.splits; plan[2] = p.steps; plan[3] = p.stages;
+  return rc;
 }
