@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from block_scaled_oracle import act64, check, gated64, matrix64, product64, product_of_known64, random_matrix, requantised64, rows64, widened_rows64
+from block_scaled_oracle import EXPERT_PATHS, GATED_PATHS, PLAIN_PATHS, act64, check, gated64, matrix64, product64, product_of_known64, random_matrix, requantised64, rows64, widened_rows64
 from gpu_common import need_gpu
 from torchinferno_b200.kernels import gemm, ops
 from torchinferno_b200.kernels.block_scaled import BlockScaledExperts, BlockScaledMatrix, BlockScaledWeight, quantize_rows
@@ -350,6 +350,59 @@ def test_captured_and_on_two_streams(m):
             outs.append(pass_of(inputs[turn % 4]))
     torch.cuda.synchronize()
     assert all(torch.equal(y, want[turn % 4]) for turn, y in enumerate(outs))
+
+
+# ------------------------------------------------------------------------------------------------ every way through the kernels
+def device_matrix(n, k, seed, size=1.0):
+    """A large matrix, made on the device: codes of all sizes, scales up to ``size`` / 60."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    codes = (torch.randn(n, k, generator=g, device=DEV) * 60).clamp(-448, 448).to(torch.float8_e4m3fn)
+    scales = (torch.rand(-(-n // 128), -(-k // 128), generator=g, device=DEV) + 0.02) * (size / 60)
+    return BlockScaledMatrix(codes, scales)
+
+
+def in_both_types(call, want):
+    """``call(out type, error word)`` in 32 bits and in bf16, within the bound, with no wait run out, and the same bits again."""
+    for dtype in (F32, BF16):
+        word = error_word()
+        got = call(dtype, word)
+        check(got, want, dtype)
+        assert torch.equal(got, call(dtype, word)) and int(word) == 0
+
+
+@pytest.mark.parametrize("m, k, n", [sizes[:3] for sizes in PLAIN_PATHS])
+def test_every_way_of_a_product(m, k, n):
+    need_gpu()
+    matrix, x = device_matrix(n, k, 1), rows(m, k, m)
+    weight = BlockScaledWeight(matrix)
+    in_both_types(lambda dtype, word: weight.product(x, out_dtype=dtype, error_word=word), product64(x, matrix))
+
+
+@pytest.mark.parametrize("m, k, n", [sizes[:3] for sizes in GATED_PATHS])
+def test_every_way_of_a_gated_product(m, k, n):
+    need_gpu()
+    gate, up = (device_matrix(n // 2, k, seed, (128 / k) ** 0.5 / 10) for seed in (1, 2))
+    x, weight = rows(m, k, m, spread=0.5), BlockScaledWeight(gate, up, epilogue="swiglu")
+    in_both_types(lambda dtype, word: weight.swiglu(x, out_dtype=dtype, error_word=word), gated64(product64(x, gate), product64(x, up)))
+
+
+@pytest.mark.parametrize("act", ["none", "swiglu"])
+@pytest.mark.parametrize("pairs, count, k, n", [sizes[:4] for sizes in EXPERT_PATHS])
+def test_every_way_of_experts(pairs, count, k, n, act):
+    need_gpu()
+    n = n // 2 if act == "swiglu" else n          # (features of either matrix)
+    stacks = [[device_matrix(n, k, 100 * part + e, (128 / k) ** 0.5 / 10) for e in range(min(count, 4))] for part in range(2 if act == "swiglu" else 1)]
+    offsets, order, ids = routing(pairs, 1, count, 3, empty=(1,))
+    x, weight = rows(pairs, k, 5, spread=0.5), BlockScaledExperts(*([s[e % len(s)] for e in range(count)] for s in stacks))
+    kind = ids.to(DEV)[order.long()] % len(stacks[0])
+    want = [torch.empty(pairs, n, dtype=torch.float64, device=DEV) for _ in range(2)]
+    for i in range(len(stacks[0])):
+        at = (kind == i).nonzero()[:, 0]
+        sums = [product64(x[order[at].long()], s[i]) for s in stacks]
+        for to, part in zip(want, gated64(*sums) if act == "swiglu" else sums[0]):
+            to[at] = part
+    in_both_types(lambda dtype, word: ops.moe_expert_product(x, weight, torch.empty(pairs, n, dtype=dtype, device=DEV), offsets, order, 1, x_by_pair=True,
+                                                             act=act, error_word=word), tuple(want))
 
 
 # ------------------------------------------------------------------------------------------------ rows sorted by expert
