@@ -15,7 +15,8 @@
 // them 800 (the tensor cores' own time is 537, the sums alone take 340).  8,192 rows 4,096 -> 2 x 14,336 with silu(gate) * up: 0.90 ms, 2,140 TFLOP/s (1.03 ms,
 // 1,870 under the power limit); 2,048 rows 4,096 -> 6,144 with its codes 59 us, 1,740, a third round of tiles included that is 0.6 full.  Tried: pieces of 32 columns
 // (the scales' registers spilled, and every step waited for their loads: 1.10 ms), waits by polling without a time hint (no gain).
-// Every wait is bounded and reports in error_word; no block leaves before its partner is done; every copy lands in the block that issued it.
+// Every wait is bounded and reports in error_word; no block leaves before its partner is done and what was sent to it has come; every copy lands in the block that
+// issued it.
 #include "block_scaled.cuh"
 #include "cluster.cuh"
 
@@ -344,6 +345,14 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
           __syncwarp();
           if (++s == kB2Stages) { s = 0; phase ^= 1; }
         }
+      }
+      // The even block's last releases of the stages arrive here as well: they have come before this block leaves.
+      for (int i = 0; i < kB2Stages && ok; ++i) {
+        if (!mbar_wait_warp(empty_bar(s), phase)) {
+          if (a.error_word && leader) atomicExch(a.error_word, 0x7C00D1);
+          ok = false;
+        }
+        if (++s == kB2Stages) { s = 0; phase ^= 1; }
       }
     } else if (warp == 1) {
       if (rank == 0) {
