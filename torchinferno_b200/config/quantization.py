@@ -2,8 +2,10 @@
 
 One form is read, ``"quant_method": "fp8"`` with a scale for each block of 128 x 128 (``"weight_block_size": [128, 128]``): a matrix ``name`` is e4m3
 codes, its scales are the 32-bit tensor ``name + "_scale_inv"``, and activations are quantised as they come (``"activation_scheme": "dynamic"``).
+The rows' scales are powers of two (kernels/block_scaled.py), whether or not the file says so (``scale_fmt``).
 Which of a model's matrices may be stored so is up to its parts (``WeightSpec.block_scaled``); which of them are is seen from the file.
-Other methods are left to the loader, which refuses tensors that the model does not know.
+Other methods are left to the loader, which refuses tensors that the model does not know; a file with 8-bit blocks is checked against this form, and random
+models leave any other aside.
 """
 from __future__ import annotations
 

@@ -21,8 +21,10 @@ __host__ __device__ __forceinline__ int bs_scale_row(int f, int pairs) { return 
 
 // The scale of a run whose largest absolute value has these bits, and what its numbers are multiplied by: 2^p and 2^-p with p the smallest integer, at
 // least -126, for which the largest is at most 448 * 2^p (448 = 1.75 * 2^8: the exponent less 8, one more where the mantissa is above 1.75); 1 for a run
-// of zeros; NaN where the largest is an infinity or a NaN, so that such a row shows in every output.  A power of two costs a float format no
-// precision, divides without rounding and multiplies another scale without rounding.
+// of zeros; NaN where the largest is an infinity or a NaN, so that such a row shows in every output.  A power of two divides without rounding, so that codes are
+// the same on any machine, and multiplies another scale without rounding (but see BsFar).  What it costs: with (largest / 448) as its scale a run's largest number is
+// a code exactly, here it is rounded like any other.  Relative rms error of rows and of products with them, this / that: Gaussian rows 0.0266 / 0.0257,
+// silu(g) u of Gaussian ones 0.0265 / 0.0226, rows with one column in a hundred 20 times as large 0.0266 / 0.016.
 __device__ __forceinline__ void bs_run_scale(uint32_t largest, float& scale, float& inverse) {
   int p = (int)(largest >> 23) - 127 - 8 + ((largest & 0x7fffffu) > 0x600000u);
   p = p < -126 ? -126 : p;

@@ -11,10 +11,11 @@
 //   warp 0       TMA producer into a ring of six stages      warp 1 (of the even block)   issues the MMAs; either owns its block's TMEM
 //   warps 4..11  sums, then the epilogue with its activation.  These take registers that the first four warps give up (168 a thread at launch,
 //                40 + 2 x 232 after)
-// What bounds it: shared memory.  A step's MMAs read 64 KB of operands from it while 32 KB of the next step's arrive: without the sums a step takes 700 cycles, with
-// them 800 (the tensor cores' own time is 537, the sums alone take 340).  8,192 rows 4,096 -> 2 x 14,336 with silu(gate) * up: 0.90 ms, 2,140 TFLOP/s (1.03 ms,
-// 1,870 under the power limit); 2,048 rows 4,096 -> 6,144 with its codes 59 us, 1,740, a third round of tiles included that is 0.6 full.  Tried: pieces of 32 columns
-// (the scales' registers spilled, and every step waited for their loads: 1.10 ms), waits by polling without a time hint (no gain).
+// What bounds it: the step.  It takes 880 to 930 cycles of the warp that issues the MMAs, whose own time is 537: 135 to 160 in the wait for operands,
+// 190 to 250 in that for an accumulator to be read, the rest in issuing.  Without the sums it takes 700, the sums alone 340.  (The bf16 kernel of the same tiles,
+// whose accumulator changes hands once a tile and not once a step, takes about 550.)  8,192 rows 4,096 -> 2 x 14,336 with silu(gate) * up: 0.90 ms,
+// 2,140 TFLOP/s (1.03 to 1.07 ms, 1,800 to 1,870 under the power limit); 2,048 rows 4,096 -> 6,144 with its codes 58 to 60 us, 1,740, a third round of tiles included that
+// is 0.6 full.  Tried: pieces of 32 columns (the scales' registers spilled, and every step waited for their loads: 1.10 ms), waits by polling without a time hint (no gain).
 // Every wait is bounded and reports in error_word; no block leaves before its partner is done and what was sent to it has come; every copy lands in the block that
 // issued it.
 #include "block_scaled.cuh"

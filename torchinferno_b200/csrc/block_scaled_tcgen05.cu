@@ -17,11 +17,11 @@
 // blocks' order.  Weights do not depend on the kernel before: a first ring of them is requested before griddepcontrol.wait (not for sorted rows, whose
 // tiles that kernel's counts decide).
 //
-// What bounds it, at few rows: memory.  8 rows 4,096 -> 2 x 14,336: 21.3 us for 117 MB (5.5 TB/s, 84 % of the measured copy bandwidth; two blocks an SM: with one,
-// whose second round of tiles is half empty, 31); 14,336 -> 4,096 13.7 us for 59 MB; 21 of 32 experts' 88 MB 14.3 us.  One row 4,096 -> 4,096 takes 7.2 us for the
-// 2.6 of its stream: about 3,000 cycles pass between the kernel before's end and the first sums, 1,400 in the exchange, 1,100 at the end, and one SM's share of the
-// launch is 1.4 us.  In tiles of 128 rows shared memory, in smaller ones the summing warps' loop (300 to 400 cycles a step).  Every wait is bounded and reports in error_word; a warp that gave up goes through the motions to the
-// end, so that nobody waits for it.
+// What bounds it, at few rows: memory.  8 rows 4,096 -> 2 x 14,336: 21.2 us for 117 MB (5.5 TB/s, 84 % of the measured copy bandwidth; two blocks an SM: with one,
+// whose second round of tiles is half empty, 31); 14,336 -> 4,096 13.7 to 14.1 us for 59 MB; 21 of 32 experts' 88 MB 14.3 us.  One row 4,096 -> 4,096 takes 7.6 us for
+// the 2.6 of its stream: about 3,000 cycles pass between the kernel before's end and the first sums, 1,400 in the exchange, 1,100 at the end, and one SM's share of the
+// launch is 1.4 us.  In tiles of 128 rows shared memory, in smaller ones the summing warps' loop (300 to 400 cycles a step).  Every wait is bounded and reports in
+// error_word; a warp that gave up goes through the motions to the end, so that nobody waits for it.
 #include "block_scaled.cuh"
 #include "mma.cuh"
 #include "cluster.cuh"
@@ -656,7 +656,9 @@ static constexpr uint32_t bs_smem(int stages, int splits, int experts) {
 
 // The blocks that share a tile's runs: 8, 4 or 2 where there is room for them beside the other tiles' and the runs are enough to pay for the exchange.
 // (us by 1 / 2 / 4 / 8 blocks a tile: 8 rows 4,096 -> 4,096 14.2 / 9.8 / 8.3 / 9.0, 14,336 -> 4,096 43 / 25 / 16.7 / 15.0, 4,096 -> 6,144 14.2 / 10.6 /
-// 9.1 / 14.8, 2,048 -> 2,048 8.2 / 6.5 / 5.9 / 6.1; 4 rows 512 -> 1,024 4.0 / 4.5 / 4.3; 20 rows 512 -> 1,024 5.5 / 6.3 / 5.9.)
+// 9.1 / 14.8, 2,048 -> 2,048 8.2 / 6.5 / 5.9 / 6.1; 4 rows 512 -> 1,024 4.0 / 4.5 / 4.3; 20 rows 512 -> 1,024 5.5 / 6.3 / 5.9.  By 4 / 8 about the 64 runs from which
+// it is 8, at 32, 40, 48, 56, 64, 80 runs: 8 rows and 4,096 features 7.8 / 8.1, 8.4 / 8.9, 9.2 / 9.4, 9.8 / 9.8, 10.6 / 10.3, 12.1 / 11.6; 2,048 features 7.0 / 6.1,
+// 7.6 / 6.8, 8.4 / 7.2, 9.0 / 7.5, 9.7 / 8.0, 11.0 / 8.7; 20 rows and 2,048 features 8.7 / 9.7, 9.5 / 10.5, 10.1 / 11.0, 10.7 / 11.4, 11.2 / 12.0, 12.4 / 12.6.)
 static int bs_splits(int64_t tiles, int runs, int blocks) {
   if (tiles * 8 <= blocks && runs >= 64) return 8;
   if (tiles * 4 <= blocks && runs >= 8) return 4;
@@ -665,7 +667,9 @@ static int bs_splits(int64_t tiles, int runs, int blocks) {
 // Rows of a tile of codes: the fewest that give no more tiles than SMs; of a long matrix (64 runs) not fewer than 64 while there are that many rows, as every row tile
 // reads the weights again.  (us in tiles of 32 / 64 / 128 rows: 333 rows 1,000 -> 1,302 8.2 / 9.5 / 11.4, 128 rows 4,096 -> 4,096 13.7 / 14.1 / 15.6, 256 rows
 // 18.0 / 16.7 / 20.0, 100 rows 2,048 -> 2,048 8.9 / 10.2 / 11.8, 64 rows 14,336 -> 4,096 19.2 / 18.1 / 25.5, 128 rows 28.1 / 26.1 / 26.3, 128 rows 4,096 ->
-// 14,336 29.2 / 27.9 / 24.9.)
+// 14,336 29.2 / 27.9 / 24.9.  32 / 64 about those 64 runs, at 32, 40, 48, 56, 64, 80 runs and 4,096 features: 64 rows 12.0 / 12.0, 13.1 / 12.5, 14.2 / 13.1, 15.3 / 13.7,
+// 16.5 / 14.2, 18.9 / 15.9; 128 rows 14.8 / 13.8, 17.2 / 15.1, 19.4 / 16.3, 21.6 / 17.5, 23.5 / 18.6, 28.0 / 21.1.  Where eight blocks share a tile it is the other way:
+// 64 rows and 2,048 features at 64 runs 11.8 / 19.9, which the rule does not know.)
 static int bs_tile_rows(int rows, int features, int runs) {
   const int64_t f_tiles = ceil_div(features, 128);
   if (rows <= 32 || (ceil_div(rows, 32) * f_tiles <= 148 && runs < 64)) return 32;
