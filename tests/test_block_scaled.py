@@ -81,7 +81,7 @@ def test_rows_scales_that_a_matrix_keeps_normal(scales, low, high):
     import math
     codes_ = torch.zeros(128, 128 * len(scales), dtype=torch.uint8).view(CODES)
     part = BlockScaledWeight(BlockScaledMatrix(codes_, torch.tensor([scales]))).parts[0][1]
-    assert (part.far_from, part.far_span) == ((low + 127) << 23, (high - low) << 23)
+    assert (part.far_low, part.far_high) == (2.0 ** low, 2.0 ** high)
 
     def normal(p):
         return all(s == 0 or not math.isfinite(s) or (2.0 ** p * abs(s) < 2.0 ** 128 and (p >= 0 or 2.0 ** p * abs(s) >= 2.0 ** -126)) for s in scales)

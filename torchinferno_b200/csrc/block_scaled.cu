@@ -87,11 +87,11 @@ TIB_API int tib_block_scaled_plan(int codes, int M, int N, int K, int experts, i
 TIB_API int tib_block_scaled_product(const void* x, int x_dtype, int64_t ldx, int x_rows, void* codes, int make, const void* w, const float* w_scales,
                                      int scale_rows, int pairs, void* y, int y_dtype, int64_t ldy, int M, int N, int K, const int* offsets,
                                      const int* order, int experts, int top, int x_by_pair, int act, float limit, float alpha,
-                                     const float* row_scale, int far_from, int far_span, int* error_word, cudaStream_t stream) {
+                                     const float* row_scale, float far_low, float far_high, int* error_word, cudaStream_t stream) {
   if (M == 0 || N == 0) return TIB_OK;
   if (!codes)
     return tib_block_scaled_tcgen05(x, x_dtype, ldx, x_rows, nullptr, 0, w, w_scales, scale_rows, pairs, y, y_dtype, ldy, M, N, K, offsets, order, experts,
-                                    top, x_by_pair, act, limit, alpha, row_scale, far_from, far_span, error_word, stream);
+                                    top, x_by_pair, act, limit, alpha, row_scale, far_low, far_high, error_word, stream);
   if (M < 0 || K < 1 || (offsets && experts < 1)) return TIB_E_ARG;
   const int runs = ceil_div(K, kBlk);
   const int64_t lds = ((int64_t)M + 3) & ~(int64_t)3;
@@ -104,9 +104,9 @@ TIB_API int tib_block_scaled_product(const void* x, int x_dtype, int64_t ldx, in
   }
   if (takes_pairs_of_sms(M, N, offsets ? experts : 0))
     return tib_block_scaled_2cta(codes, scales, lds, w, w_scales, scale_rows, pairs, y, y_dtype, ldy, M, N, K, offsets, order, experts, act, limit, alpha,
-                                 row_scale, far_from, far_span, error_word, stream);
+                                 row_scale, far_low, far_high, error_word, stream);
   return tib_block_scaled_tcgen05(codes, -1, 0, M, scales, lds, w, w_scales, scale_rows, pairs, y, y_dtype, ldy, M, N, K, offsets, order, experts, top, 0, act,
-                                  limit, alpha, row_scale, far_from, far_span, error_word, stream);
+                                  limit, alpha, row_scale, far_low, far_high, error_word, stream);
 }
 
 // The calls the Python parts make (common.cuh).

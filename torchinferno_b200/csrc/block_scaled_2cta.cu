@@ -85,10 +85,7 @@ __device__ __noinline__ void b2_rows_apart(const B2Args* args, int row0, int row
   const int lane = threadIdx.x & 31;
   bool outside = false;
   if (lane < rows)
-    for (int b = 0; b < a.runs; ++b) {
-      const float scale = a.x_scales[(size_t)b * a.lds + row0 + lane];
-      outside |= a.far.outside(scale) && !isnan(scale);
-    }
+    for (int b = 0; b < a.runs; ++b) outside |= a.far.outside(a.x_scales[(size_t)b * a.lds + row0 + lane]);
   for (uint32_t rest = __ballot_sync(0xffffffffu, outside); rest; rest &= rest - 1) {
     const int r = row0 + __ffs(rest) - 1;
     BsApart<uint8_t> apart;
@@ -436,10 +433,10 @@ TIB_API int tib_block_scaled_2cta_plan(int M, int N, int K, int experts, int* pl
 // x: codes [M, runs * 128] and scales [runs, lds] as tib_quantize_rows leaves them; w: codes in blocks [experts, ceil(N / 128), runs, 128, 128] and
 // scales [experts, scale_rows, runs] (`pairs`: of (gate, up) row pairs, N and scale_rows even); out: [M, N] in out_dtype (row stride ldo), or [M, N / 2] of a
 // gated activation.  offsets [experts + 1] and order [M]: rows sorted by expert, at most kB2MaxExperts of them; offsets null: one matrix for all rows.
-// far_from, far_span: see BsFar.
+// far_low, far_high: see BsFar.
 TIB_API int tib_block_scaled_2cta(const void* x, const float* x_scales, int64_t lds, const void* w, const float* w_scales, int scale_rows, int pairs,
                                   void* out, int out_dtype, int64_t ldo, int M, int N, int K, const int* offsets, const int* order, int experts, int act,
-                                  float limit, float alpha, const float* row_scale, int far_from, int far_span, int* error_word, cudaStream_t stream) {
+                                  float limit, float alpha, const float* row_scale, float far_low, float far_high, int* error_word, cudaStream_t stream) {
   if (M == 0 || N == 0) return TIB_OK;
   if (!x || !x_scales || !w || !w_scales || !out || M < 0 || N < 0 || K < 1 || scale_rows < 1 || experts < 1) return TIB_E_ARG;
   if ((offsets && !order) || (row_scale && !order)) return TIB_E_ARG;
@@ -448,7 +445,7 @@ TIB_API int tib_block_scaled_2cta(const void* x, const float* x_scales, int64_t 
   if (out_dtype != TIB_BF16 && out_dtype != TIB_F32) return TIB_E_DTYPE;
   if (((uintptr_t)x | (uintptr_t)w) & 15) return TIB_E_ALIGN;
   B2Args a;
-  a.x = static_cast<const unsigned char*>(x); a.w = static_cast<const unsigned char*>(w); a.far = BsFar{(uint32_t)far_from, (uint32_t)far_span};
+  a.x = static_cast<const unsigned char*>(x); a.w = static_cast<const unsigned char*>(w); a.far = BsFar{far_low, far_high};
   a.x_scales = x_scales; a.lds = lds; a.w_scales = w_scales; a.scale_rows = scale_rows; a.pairs = pairs;
   a.M = M; a.N = N; a.runs = ceil_div(K, kBlk); a.offsets = offsets; a.order = order; a.experts = experts; a.error_word = error_word;
   a.ep.act = act; a.ep.limit = limit; a.ep.alpha = alpha; a.ep.row_scale = row_scale;

@@ -190,8 +190,7 @@ __device__ __forceinline__ void bs_tile_apart(const BsArgs& a, const BsTile& m, 
     bool outside = false;
     for (int kb = lane; kb < a.runs; kb += 32) {
       float inverse;
-      const float scale = apart.run_scale(kb, inverse);
-      outside |= a.far.outside(scale) && !isnan(scale);
+      outside |= a.far.outside(apart.run_scale(kb, inverse));
     }
     if (!__any_sync(0xffffffffu, outside)) continue;
     apart.row_scale = a.ep.row_scale ? a.ep.row_scale[bs_pair(a.order, m.first + c, a.M)] : 1.f;
@@ -743,12 +742,12 @@ using namespace tib;
 // 128 features; -1: codes
 // [x_rows, runs * 128] and scales [runs, lds] as tib_quantize_rows leaves them, row m of them for row m of y.  w: codes in blocks
 // [experts, ceil(N / 128), runs, 128, 128], features and columns behind the last zero, and scales [experts, scale_rows, runs] (`pairs`: of (gate, up) row pairs); y: [M, N] in y_dtype (row stride ldy), or [M, N / 2] of a gated activation.
-// offsets [experts + 1] and order [M]: rows sorted by expert as tib_moe_expert_product takes them; offsets null: one matrix for all rows.  far_from, far_span:
+// offsets [experts + 1] and order [M]: rows sorted by expert as tib_moe_expert_product takes them; offsets null: one matrix for all rows.  far_low, far_high:
 // which rows' scales keep normal with every one of w's (BsFar).
 TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, int x_rows, const float* x_scales, int64_t lds, const void* w,
                                      const float* w_scales, int scale_rows, int pairs, void* y, int y_dtype, int64_t ldy, int M, int N, int K,
                                      const int* offsets, const int* order, int experts, int top, int x_by_pair, int act, float limit,
-                                     float alpha, const float* row_scale, int far_from, int far_span, int* error_word, cudaStream_t stream) {
+                                     float alpha, const float* row_scale, float far_low, float far_high, int* error_word, cudaStream_t stream) {
   if (M == 0 || N == 0) return TIB_OK;
   const bool is_codes = x_dtype < 0;
   if (!x || !w || !w_scales || !y || M < 0 || N < 0 || K < 1 || experts < 1 || top < 1 || x_rows < 1) return TIB_E_ARG;
@@ -758,7 +757,7 @@ TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, in
   if (experts > kBsMaxExperts || (int64_t)experts * ceil_div(N, 128) * ceil_div(K, kBlk) > (0x7fffffff >> 7)) return TIB_E_SIZE;
   if ((((uintptr_t)w) & 15) || (is_codes && (((uintptr_t)x) & 15))) return TIB_E_ALIGN;
   BsArgs a;
-  a.x = x; a.w = static_cast<const unsigned char*>(w); a.far = BsFar{(uint32_t)far_from, (uint32_t)far_span}; a.ldx = ldx;
+  a.x = x; a.w = static_cast<const unsigned char*>(w); a.far = BsFar{far_low, far_high}; a.ldx = ldx;
   a.x_scales = x_scales; a.lds = lds; a.w_scales = w_scales; a.scale_rows = scale_rows; a.pairs = pairs;
   a.vec = !is_codes && ((uintptr_t)x & 15) == 0 && (ldx * (x_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
   a.wide = ((uintptr_t)y & 15) == 0 && (ldy * (y_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;

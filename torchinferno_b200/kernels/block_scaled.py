@@ -120,8 +120,8 @@ def _code_buffer(x: torch.Tensor, rows: int, columns: int) -> torch.Tensor:
     return x.new_empty(runs * (rows * BLOCK + 4 * ((rows + 3) & ~3)), dtype=torch.uint8)
 
 
-def _normal_range(scales: torch.Tensor) -> tuple[int, int]:
-    """(first, span) of the bits of the powers of two whose product with every one of ``scales`` is a normal 32-bit number, or exact all the same
+def _normal_range(scales: torch.Tensor) -> tuple[float, float]:
+    """The least and the largest of the powers of two whose product with every one of ``scales`` is a normal 32-bit number, or exact all the same
     (powers of at least 1: 1 always is one of them); the kernels look after other products one by one."""
     sizes = scales.abs()
     least = torch.where(sizes > 0, sizes, math.inf).amin()
@@ -129,22 +129,22 @@ def _normal_range(scales: torch.Tensor) -> tuple[int, int]:
     least, most = torch.stack([least, most]).tolist()
     low = -126 if math.isinf(least) else max(min(-125 - math.frexp(least)[1], 0), -126)      # (least is at least 2^(its exponent - 1))
     high = 120 if most == 0 else min(128 - math.frexp(most)[1], 120)                         # (most is less than 2^(its exponent))
-    return (low + 127) << 23, (high - low) << 23
+    return 2.0 ** low, 2.0 ** high
 
 
 class Blocks:
     """Matrices of one size as the kernels read them: ``codes`` [matrices, blocks of N, blocks of K, 128, 128], padded with zeros, and ``scales`` [matrices,
     blocks of N, blocks of K]; ``paired``: the matrices' rows are (gate i, up i), their scales' rows (gate block j, up block j)."""
-    __slots__ = ("codes", "scales", "count", "features", "columns", "paired", "codes_at", "scales_at", "scale_rows", "device_index", "far_from", "far_span")
+    __slots__ = ("codes", "scales", "count", "features", "columns", "paired", "codes_at", "scales_at", "scale_rows", "device_index", "far_low", "far_high")
 
-    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, features: int, columns: int, paired: bool, far: "tuple[int, int] | None" = None) -> None:
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, features: int, columns: int, paired: bool, far: "tuple[float, float] | None" = None) -> None:
         if codes.shape[1] != blocks(features) or codes.shape[2] != blocks(columns) or scales.shape[1:] != (codes.shape[1] if not paired else 2 * blocks(features // 2), codes.shape[2]):
             raise ValueError(f"blocks {tuple(codes.shape)} and scales {tuple(scales.shape)} do not make matrices of {features} rows")
         if not codes.is_contiguous() or not scales.is_contiguous():
             raise ValueError("blocks and their scales must be contiguous")
         self.codes, self.scales, self.count, self.features, self.columns, self.paired = codes, scales, codes.shape[0], features, columns, paired
         self.codes_at, self.scales_at, self.scale_rows, self.device_index = codes.data_ptr(), scales.data_ptr(), scales.shape[1], codes.get_device()
-        self.far_from, self.far_span = _normal_range(scales) if far is None else far      # (the scales are read: once a weight)
+        self.far_low, self.far_high = _normal_range(scales) if far is None else far      # (the scales are read: once a weight)
 
 
 def _laid_out(matrices: Sequence[BlockScaledMatrix], ups: Sequence[BlockScaledMatrix] | None) -> Blocks:
@@ -229,7 +229,7 @@ class BlockScaledWeight:
                 if lo % BLOCK:
                     raise ValueError(f"feature {start} lies inside a block")
                 view.parts.append((first + lo - start, Blocks(part.codes[:, lo // BLOCK:blocks(hi)], part.scales[:, lo // BLOCK:blocks(hi)], hi - lo, self.in_features, False,
-                                                          (part.far_from, part.far_span))))
+                                                          (part.far_low, part.far_high))))
         return view
 
     def _run(self, x: torch.Tensor, act: str, width: int, out_dtype: torch.dtype | None, out: torch.Tensor | None, error_word: torch.Tensor | None) -> torch.Tensor:

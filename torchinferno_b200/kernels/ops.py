@@ -1273,7 +1273,7 @@ def block_scaled_product(x: torch.Tensor, codes: int, make: bool, blocks, y: tor
     _check("block_scaled_product", lib().tib_block_scaled_product(
         x.data_ptr(), _code(x.dtype), x.stride(0), len(x), codes, make, blocks.codes_at, blocks.scales_at, blocks.scale_rows, blocks.paired, y.data_ptr(),
         _code(y.dtype), y.stride(0), len(y), blocks.features, blocks.columns, offsets, order, blocks.count, top, x_by_pair, MOE_ACT[act], limit, alpha,
-        0 if row_scale is None else row_scale.data_ptr(), blocks.far_from, blocks.far_span, 0 if error_word is None else error_word.data_ptr(), _stream()))
+        0 if row_scale is None else row_scale.data_ptr(), blocks.far_low, blocks.far_high, 0 if error_word is None else error_word.data_ptr(), _stream()))
 
 
 def glu_clamp(gate_up: torch.Tensor, out: torch.Tensor, limit: float, alpha: float) -> torch.Tensor:
