@@ -30,30 +30,11 @@ constexpr int kB2MaxExperts = (kMostSmem - (int)kB2Smem) / 8 - 1;      // (two n
 // D fp32, A and B e4m3, both K-major, N = 256, M = 256 over the pair
 constexpr uint32_t kB2Idesc = (1u << 4) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
 
-__device__ __forceinline__ void b2_tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t cluster_bar) {
-  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n"
-               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(cluster_bar) : "memory");
-}
 __device__ __forceinline__ void b2_umma(uint32_t leader, uint32_t tmem_d, uint32_t a_low, uint32_t b_low, uint32_t accumulate) {
   asm volatile("{\n.reg .pred p, q;\n.reg .b64 a, b;\nmov.b64 a, {%1, %6};\nmov.b64 b, {%2, %6};\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
                "@q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %3, p;\n}\n"
                ::"r"(tmem_d), "r"(a_low), "r"(b_low), "r"(kB2Idesc), "r"(accumulate), "r"(leader), "r"(kUmmaDescHigh) : "memory");
 }
-// Arrive, once the MMAs issued so far are done, on the barrier at this offset in both blocks of the pair.
-__device__ __forceinline__ void b2_commit_both(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
-               ::"r"(bar), "h"((uint16_t)3) : "memory");
-}
-__device__ __forceinline__ bool b2_wait_cluster(uint32_t bar, uint32_t parity) {
-  for (uint32_t i = 0; i < (1u << 18); ++i) {
-    uint32_t ok;
-    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n"
-                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000u) : "memory");
-    if (ok) return true;
-  }
-  return false;
-}
-
 // An arrival at the even block's barrier without a fence of the cluster: what it orders is the reading of tensor memory, which tcgen05.fence has ordered.
 // (With .release.cluster every step waited for the warp's whole memory traffic, the largest of the kernel's stalls.)
 __device__ __forceinline__ void b2_arrive_even(uint32_t cluster_bar) {
@@ -337,8 +318,8 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
           if (leader) {
             if (rank == 0) mbar_expect_tx(full_bar(s), 2 * kB2Stage);
             const uint32_t bar0 = map_to_cta(full_bar(s), 0);
-            b2_tma_load(base + s * kB2Stage, &map_x, kb * kBlk, m0, bar0);
-            b2_tma_load(base + s * kB2Stage + kB2Half, &map_w, 0, (w0 + kb) << 7, bar0);
+            pair_tma_load(base + s * kB2Stage, &map_x, kb * kBlk, m0, bar0);
+            pair_tma_load(base + s * kB2Stage + kB2Half, &map_w, 0, (w0 + kb) << 7, bar0);
           }
           __syncwarp();
           if (++s == kB2Stages) { s = 0; phase ^= 1; }
@@ -360,12 +341,12 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
         bool ok = true;
         for (int t = pair; t < num_tiles && ok; t += pairs) {
           for (int kb = 0; kb < a.runs; ++kb) {
-            if (!__all_sync(0xffffffffu, b2_wait_cluster(full_bar(s), phase))) {
+            if (!__all_sync(0xffffffffu, pair_wait(full_bar(s), phase))) {
               if (a.error_word && leader) atomicExch(a.error_word, 0x7C00D2);
               ok = false;
               break;
             }
-            if (!__all_sync(0xffffffffu, b2_wait_cluster(acc_empty_bar(b), acc_phase))) {      // both blocks have read this accumulator
+            if (!__all_sync(0xffffffffu, pair_wait(acc_empty_bar(b), acc_phase))) {      // both blocks have read this accumulator
               if (a.error_word && leader) atomicExch(a.error_word, 0x7C00D4);
               ok = false;
               break;
@@ -375,8 +356,8 @@ block_scaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
   #pragma unroll
             for (int k = 0; k < 4; ++k) b2_umma(leader, tmem_base + b * 256, x_src + 2 * k, w_src + 2 * k, k != 0);
             if (leader) {
-              b2_commit_both(acc_full_bar(b));
-              b2_commit_both(empty_bar(s));      // the stage is free in both blocks once these MMAs have read it
+              pair_commit_both(acc_full_bar(b));
+              pair_commit_both(empty_bar(s));      // the stage is free in both blocks once these MMAs have read it
             }
             __syncwarp();
             if (++s == kB2Stages) { s = 0; phase ^= 1; }

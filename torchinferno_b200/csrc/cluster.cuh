@@ -1,5 +1,5 @@
-// Thread-block-cluster pieces shared by the few-rows products: ranks, cluster barriers, stores and mbarrier
-// arrivals in a peer's shared memory, and the tensor map of a bf16 matrix read in 64-wide swizzled boxes.
+// Thread-block-cluster pieces shared by the products: ranks, cluster barriers, stores and mbarrier arrivals in a peer's shared memory, copies, commits and
+// waits of pairs of SMs, and the tensor map of a bf16 matrix read in 64-wide swizzled boxes.
 #pragma once
 
 #include "tcgen05.cuh"
@@ -45,6 +45,28 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity)
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     if (ok) return true;
     if (i > 64) __nanosleep(32);
+  }
+  return false;
+}
+
+// ----- pairs of SMs (cta_group::2)
+// A tile copy whose completion is counted on a barrier given by its cluster address (the even block's).
+__device__ __forceinline__ void pair_tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t cluster_bar) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n"
+               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(cluster_bar) : "memory");
+}
+// Arrive, once the MMAs issued so far are done, on the barrier at this offset in both blocks of the pair.
+__device__ __forceinline__ void pair_commit_both(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
+               ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+// Bounded wait for what either block has signalled; a try suspends the thread for about a microsecond, as in mbar_wait.
+__device__ __forceinline__ bool pair_wait(uint32_t bar, uint32_t parity) {
+  for (uint32_t i = 0; i < (1u << 18); ++i) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000u) : "memory");
+    if (ok) return true;
   }
   return false;
 }

@@ -17,7 +17,7 @@
 // lands in the shared memory of the block that issued it.
 //
 // The reference sends these products to cuBLAS (src/torchinferno/models/llama3/tensor_parallel.py:11176-11198).
-#include "tcgen05.cuh"
+#include "cluster.cuh"
 
 namespace tib {
 
@@ -35,46 +35,10 @@ constexpr uint32_t t2_idesc(int bn) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(kT2BM >> 4) << 24);
 }
 
-__device__ __forceinline__ uint32_t t2_cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t t2_map(uint32_t smem_addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(smem_addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void t2_cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
-// A tile copy whose completion is counted on a barrier given by its cluster address (the even block's).
-__device__ __forceinline__ void t2_tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t cluster_bar) {
-  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n"
-               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(cluster_bar) : "memory");
-}
 __device__ __forceinline__ void t2_umma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
                "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
                ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
-}
-// Arrive, once the MMAs issued so far are done, on the barrier at this offset in both blocks of the pair.
-__device__ __forceinline__ void t2_commit_both(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
-               ::"r"(bar), "h"((uint16_t)3) : "memory");
-}
-__device__ __forceinline__ void t2_arrive_cluster(uint32_t cluster_bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_bar) : "memory");
-}
-__device__ __forceinline__ bool t2_wait_cluster(uint32_t bar, uint32_t parity) {
-  for (uint32_t i = 0; i < (1u << 18); ++i) {
-    uint32_t ok;
-    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n"
-                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000u) : "memory");
-    if (ok) return true;
-  }
-  return false;
 }
 
 // Persistent: pair p walks the tiles t = p, p + pairs, ...; tile t is row tile t % m_tiles of column tile
@@ -94,7 +58,7 @@ gemm_tcgen05_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem_raw + (tmem_slot - smem_u32(smem_raw)));
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = t2_cluster_rank();                 // 0: the even block of the pair, which issues the MMAs
+  const uint32_t rank = cluster_rank();                    // 0: the even block of the pair, which issues the MMAs
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int k_blocks = K / kT2BK;
   constexpr uint32_t kBBytes = (BN / 2) * kT2BK * 2;       // this block's rows of w
@@ -118,7 +82,7 @@ gemm_tcgen05_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
-  t2_cluster_sync();                                       // both blocks have their barriers before either is signalled
+  cluster_sync_all();                                      // both blocks have their barriers before either is signalled
   asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
   const uint32_t tmem_base = *tmem_slot_ptr;
 
@@ -138,9 +102,9 @@ gemm_tcgen05_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
           }
           if (rank == 0) mbar_expect_tx(full_bar(s), 2 * (kT2ABytes + kBBytes));
           const uint32_t a_dst = base + s * kT2StageBytes, b_dst = a_dst + kT2ABytes;
-          const uint32_t bar0 = t2_map(full_bar(s), 0);
-          t2_tma_load(a_dst, &map_x, kb * kT2BK, m0, bar0);
-          t2_tma_load(b_dst, &map_w, kb * kT2BK, n0, bar0);
+          const uint32_t bar0 = map_to_cta(full_bar(s), 0);
+          pair_tma_load(a_dst, &map_x, kb * kT2BK, m0, bar0);
+          pair_tma_load(b_dst, &map_w, kb * kT2BK, n0, bar0);
         }
       }
     }
@@ -152,7 +116,7 @@ gemm_tcgen05_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
       for (int t = pair; t < num_tiles && ok; t += pairs, ++j) {
         const int b = j & 1;
         const uint32_t tmem_acc = tmem_base + b * kT2AccStride;
-        if (!t2_wait_cluster(acc_empty_bar(b), ((j >> 1) & 1) ^ 1)) {   // both epilogues have drained this accumulator
+        if (!pair_wait(acc_empty_bar(b), ((j >> 1) & 1) ^ 1)) {   // both epilogues have drained this accumulator
           if (error_word) atomicExch(error_word, 0x7C0054);
           ok = false;
           break;
@@ -161,7 +125,7 @@ gemm_tcgen05_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
         for (int kb = 0; kb < k_blocks; ++kb, ++it) {
           const int s = it % kT2Stages;
           const uint32_t phase = (it / kT2Stages) & 1;
-          if (!t2_wait_cluster(full_bar(s), phase)) {
+          if (!pair_wait(full_bar(s), phase)) {
             if (error_word) atomicExch(error_word, 0x7C0052);
             ok = false;
             break;
@@ -171,9 +135,9 @@ gemm_tcgen05_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
 #pragma unroll
           for (int k = 0; k < kT2BK / 16; ++k)
             t2_umma(tmem_acc, umma_desc_k128(a_src + k * 32), umma_desc_k128(b_src + k * 32), t2_idesc(BN), (kb | k) != 0);
-          t2_commit_both(empty_bar(s));   // the stage is free in both blocks once these MMAs have read it
+          pair_commit_both(empty_bar(s));   // the stage is free in both blocks once these MMAs have read it
         }
-        t2_commit_both(acc_full_bar(b));  // (also on failure, so that the epilogues do not wait in vain)
+        pair_commit_both(acc_full_bar(b));  // (also on failure, so that the epilogues do not wait in vain)
       }
     }
   } else {
@@ -217,12 +181,12 @@ gemm_tcgen05_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
       // this warp has read its quarter of the accumulator: tell the MMA thread (in the even block)
       asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
       __syncwarp();
-      if (lane == 0) t2_arrive_cluster(t2_map(acc_empty_bar(b), 0));
+      if (lane == 0) mbar_arrive_remote(map_to_cta(acc_empty_bar(b), 0));
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
-  t2_cluster_sync();   // neither block leaves (or frees tensor memory) while its partner may still signal it
+  cluster_sync_all();   // neither block leaves (or frees tensor memory) while its partner may still signal it
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(2u * kT2AccStride) : "memory");
