@@ -56,6 +56,8 @@ struct B2Args {
   int* error_word;
 };
 
+static_assert(2 * sizeof(CUtensorMap) + sizeof(B2Args) + 20 <= 416, "the kernel's parameters (see block_scaled_tcgen05.cu)");
+
 struct B2Tile { int expert, first, rows, n_tile; };      // rows first .. first + rows - 1 of x (at most 256), features n_tile * 256 ..
 
 // Rows row0 .. of a warp in a tile whose outputs are `first` ..: those outputs that have a far scale, made again, a lane an output.

@@ -49,19 +49,20 @@ struct BsTile { int expert, first, rows, feature; };
 struct BsArgs {
   const void* x;               // codes [rows, runs * 128], or rows of the activations' type
   const unsigned char* w;      // codes in blocks
-  BsFar far;
-  int64_t ldx;                 // (of the latter)
+  int64_t ldx;                 // (of rows of the activations' type)
   const float* x_scales;       // [runs, lds] beside codes
   int64_t lds;
   const float* w_scales;       // [experts, scale_rows, runs]
-  int scale_rows, pairs, vec, wide;      // vec: rows of x, wide: of y, are 16-byte aligned
-  int M, N, K, runs, x_rows, stages;
   const int* offsets;          // null: one matrix
   const int* order;
-  int experts, top, x_by_pair;
-  MoeEpilogue ep;
   int* error_word;
+  MoeEpilogue ep;
+  BsFar far;
+  int scale_rows, M, N, K, runs, x_rows, experts, top;
+  unsigned stages : 8, pairs : 1, x_by_pair : 1, vec : 1, wide : 1;      // vec: rows of x, wide: of y, are 16-byte aligned
 };
+// (On the host a launch with more than 416 bytes of parameters takes 0.3 us of 2.8 more: two tensor maps, these, y and its stride.)
+static_assert(2 * sizeof(CUtensorMap) + sizeof(BsArgs) + 16 <= 416, "the kernel's parameters");
 
 __device__ __forceinline__ int bs_source(const BsArgs& a, const BsTile& m, int r) {      // the row of x that the tile's row r is
   const int at = m.first + min(r, m.rows - 1);
@@ -233,7 +234,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
       asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map_w) : "memory");
       if constexpr (kCodes) asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map_x) : "memory");
     }
-    if (lane < a.stages) {
+    if (lane < (int)a.stages) {
       mbar_init(full_bar(lane), kCodes ? 1 : 2);  // the producer, and the helper that makes codes
       mbar_init(empty_bar(lane), 1);
     }
@@ -319,9 +320,9 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     bool ok = true;
     auto bytes = [&](const BsTile& m) { return kBsWBytes + (kCodes ? ((m.rows + 31) >> 5) * 32 * kBlk : 0); };
     if (!a.offsets) {
-      for (int t = cluster_id; t < num_tiles && ahead < a.stages; t += clusters) {
+      for (int t = cluster_id; t < num_tiles && ahead < (int)a.stages; t += clusters) {
         const BsTile m = tile_of(t);
-        for (int kb = kb0; kb < kb1 && ahead < a.stages; ++kb, ++ahead)
+        for (int kb = kb0; kb < kb1 && ahead < (int)a.stages; ++kb, ++ahead)
           if (leader) {
             mbar_expect_tx(full_bar(ahead), bytes(m));
             tma_load_2d(base + ahead * S::kStage, &map_w, 0, w_row(m, kb), full_bar(ahead));
@@ -353,7 +354,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
           }
           __syncwarp();
         }
-        if (++s == a.stages) { s = 0; phase ^= 1; }
+        if (++s == (int)a.stages) { s = 0; phase ^= 1; }
       }
     }
   } else if (warp == 1) {
@@ -386,7 +387,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
           umma_commit(empty_bar(s));
         }
         __syncwarp();
-        if (++s == a.stages) { s = 0; phase ^= 1; }
+        if (++s == (int)a.stages) { s = 0; phase ^= 1; }
         if (++b == S::kBufs) { b = 0; acc_phase ^= 1; }
       }
     }
@@ -758,11 +759,11 @@ TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, in
   if ((((uintptr_t)w) & 15) || (is_codes && (((uintptr_t)x) & 15))) return TIB_E_ALIGN;
   BsArgs a;
   a.x = x; a.w = static_cast<const unsigned char*>(w); a.far = BsFar{far_low, far_high}; a.ldx = ldx;
-  a.x_scales = x_scales; a.lds = lds; a.w_scales = w_scales; a.scale_rows = scale_rows; a.pairs = pairs;
+  a.x_scales = x_scales; a.lds = lds; a.w_scales = w_scales; a.scale_rows = scale_rows; a.pairs = pairs != 0;
   a.vec = !is_codes && ((uintptr_t)x & 15) == 0 && (ldx * (x_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
   a.wide = ((uintptr_t)y & 15) == 0 && (ldy * (y_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
   a.M = M; a.N = N; a.K = K; a.x_rows = x_rows; a.runs = ceil_div(K, kBlk); a.offsets = offsets; a.order = order; a.experts = experts; a.top = top;
-  a.x_by_pair = x_by_pair; a.error_word = error_word;
+  a.x_by_pair = x_by_pair != 0; a.error_word = error_word;
   a.ep.act = act; a.ep.limit = limit; a.ep.alpha = alpha; a.ep.row_scale = row_scale;
   CUtensorMap map_w, map_x;
   int rc = bs_make_map(&map_w, w, (int64_t)experts * ceil_div(N, 128) * a.runs * 128, kBlk, 128);
