@@ -48,25 +48,31 @@ struct BsTile { int expert, first, rows, feature; };
 
 struct BsArgs {
   const void* x;               // codes [rows, runs * 128], or rows of the activations' type
-  const unsigned char* w;      // codes in blocks
-  int64_t ldx;                 // (of rows of the activations' type)
+  int64_t ldx;                 // (of the latter)
   const float* x_scales;       // [runs, lds] beside codes
-  int64_t lds;
+  const unsigned char* w;      // codes in blocks
   const float* w_scales;       // [experts, scale_rows, runs]
+  int scale_rows, pairs, vec, lds;       // vec: rows of x are 16-byte aligned
+  int M, N, K, runs, x_rows, stages;
   const int* offsets;          // null: one matrix
   const int* order;
+  int experts, top, modes;     // modes: kBsByPair, kBsWide
+  float far_low;               // (BsFar)
+  int act;
+  float limit, alpha, far_high;
+  const float* row_scale;
   int* error_word;
-  MoeEpilogue ep;
-  BsFar far;
-  int scale_rows, M, N, K, runs, x_rows, experts, top;
-  unsigned stages : 8, pairs : 1, x_by_pair : 1, vec : 1, wide : 1;      // vec: rows of x, wide: of y, are 16-byte aligned
+
+  __device__ __forceinline__ bool outside(float s) const { return BsFar{far_low, far_high}.outside(s); }
 };
-// (On the host a launch with more than 416 bytes of parameters takes 0.3 us of 2.8 more: two tensor maps, these, y and its stride.)
+constexpr int kBsByPair = 1, kBsWide = 2;      // a row of x is a token's, not a pair's; rows of y are 16-byte aligned
+// (Two tensor maps, these, y and its stride.  On the host a launch with more than 416 bytes takes 0.3 us of 2.8 more; on the device flags packed into bits of one word
+// cost 0.1 us of 5 to 14 at few rows.)
 static_assert(2 * sizeof(CUtensorMap) + sizeof(BsArgs) + 16 <= 416, "the kernel's parameters");
 
 __device__ __forceinline__ int bs_source(const BsArgs& a, const BsTile& m, int r) {      // the row of x that the tile's row r is
   const int at = m.first + min(r, m.rows - 1);
-  return a.offsets && a.x_by_pair ? min(bs_pair(a.order, at, a.M) / a.top, a.x_rows - 1) : at;
+  return a.offsets && (a.modes & kBsByPair) ? min(bs_pair(a.order, at, a.M) / a.top, a.x_rows - 1) : at;
 }
 
 __device__ __forceinline__ void umma_f8_warp(uint32_t leader, uint32_t tmem_d, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
@@ -103,12 +109,12 @@ __device__ __forceinline__ void bs_finish(const float* red, int log_splits, int 
   const int per = 128 >> log_splits, stride = per + 4, splits = 1 << log_splits;
   const int log_wide = 4 - log_splits - kGated;           // eights of outputs in a column
   const int first_out = (m.feature + rank * per) >> kGated, n_out = a.N >> kGated;
-  if (!a.wide) {
+  if (!(a.modes & kBsWide)) {
     // Rows of y that are not 16-byte aligned: a warp takes a row, its lanes consecutive outputs.
     const int lane = thread & 31, outs = per >> kGated;
 #pragma unroll 1
     for (int c = thread >> 5; c < m.rows; c += threads >> 5) {
-      const float scale = a.ep.row_scale ? a.ep.row_scale[bs_pair(a.order, m.first + c, a.M)] : 1.f;
+      const float scale = a.row_scale ? a.row_scale[bs_pair(a.order, m.first + c, a.M)] : 1.f;
       TO* dst = y + (size_t)(m.first + c) * ldy + first_out;
 #pragma unroll
       for (int j = 0; j < 4 >> kGated; ++j) {
@@ -122,7 +128,7 @@ __device__ __forceinline__ void bs_finish(const float* red, int log_splits, int 
           u += from[kGated];
         }
         g *= scale;
-        if (first_out + o < n_out) dst[o] = from_f32<TO>(kGated ? bs_gated<ACT>(g, u * scale, a.ep.limit, a.ep.alpha) : bs_act<ACT>(g));
+        if (first_out + o < n_out) dst[o] = from_f32<TO>(kGated ? bs_gated<ACT>(g, u * scale, a.limit, a.alpha) : bs_act<ACT>(g));
       }
     }
     return;
@@ -146,15 +152,15 @@ __device__ __forceinline__ void bs_finish(const float* red, int log_splits, int 
         v[j] += p.x; v[j + 1] += p.y; v[j + 2] += p.z; v[j + 3] += p.w;
       }
     }
-    if (a.ep.row_scale) {
-      const float scale = a.ep.row_scale[bs_pair(a.order, m.first + c, a.M)];
+    if (a.row_scale) {
+      const float scale = a.row_scale[bs_pair(a.order, m.first + c, a.M)];
 #pragma unroll
       for (int j = 0; j < 8 << kGated; ++j) v[j] *= scale;
     }
     float out[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if constexpr (kGated) out[j] = bs_gated<ACT>(v[2 * j], v[2 * j + 1], a.ep.limit, a.ep.alpha);
+      if constexpr (kGated) out[j] = bs_gated<ACT>(v[2 * j], v[2 * j + 1], a.limit, a.alpha);
       else out[j] = bs_act<ACT>(v[j]);
     }
     TO* dst = y + (size_t)(m.first + c) * ldy + first_out + f;
@@ -180,21 +186,21 @@ __device__ __forceinline__ void bs_finish(const float* red, int log_splits, int 
 template <typename TX, typename TO>
 __device__ __forceinline__ void bs_tile_apart(const BsArgs& a, const BsTile& m, int rank, int splits, int lane, TO* __restrict__ y, int64_t ldy) {
   constexpr bool kCodes = std::is_same_v<TX, uint8_t>;
-  const int gated = moe_act_gated(a.ep.act) ? 1 : 0, outs = 128 / splits >> gated, first = (m.feature >> gated) + rank * outs, n_out = a.N >> gated;
+  const int gated = moe_act_gated(a.act) ? 1 : 0, outs = 128 / splits >> gated, first = (m.feature >> gated) + rank * outs, n_out = a.N >> gated;
 #pragma unroll 1
   for (int c = 0; c < m.rows; ++c) {
     BsApart<TX> apart;
     apart.x = static_cast<const TX*>(a.x) + (kCodes ? (size_t)(m.first + c) * a.runs * kBlk : (size_t)bs_source(a, m, c) * a.ldx);
     apart.x_scales = a.x_scales + (kCodes ? m.first + c : 0);
-    apart.lds = a.lds; apart.pairs = a.pairs; apart.runs = a.runs; apart.K = a.K; apart.act = a.ep.act;
-    apart.limit = a.ep.limit; apart.alpha = a.ep.alpha;
+    apart.lds = a.lds; apart.pairs = a.pairs; apart.runs = a.runs; apart.K = a.K; apart.act = a.act;
+    apart.limit = a.limit; apart.alpha = a.alpha;
     bool outside = false;
     for (int kb = lane; kb < a.runs; kb += 32) {
       float inverse;
-      outside |= a.far.outside(apart.run_scale(kb, inverse));
+      outside |= a.outside(apart.run_scale(kb, inverse));
     }
     if (!__any_sync(0xffffffffu, outside)) continue;
-    apart.row_scale = a.ep.row_scale ? a.ep.row_scale[bs_pair(a.order, m.first + c, a.M)] : 1.f;
+    apart.row_scale = a.row_scale ? a.row_scale[bs_pair(a.order, m.first + c, a.M)] : 1.f;
     apart.w = a.w + ((size_t)m.expert * ((a.N + 127) >> 7) * a.runs << 14);
     apart.w_scales = a.w_scales + (size_t)m.expert * a.scale_rows * a.runs;
     for (int o = first + lane; o < min(first + outs, n_out); o += 32) bs_output_apart<TX, TO>(apart, o, y + (size_t)(m.first + c) * ldy);
@@ -234,7 +240,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
       asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map_w) : "memory");
       if constexpr (kCodes) asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map_x) : "memory");
     }
-    if (lane < (int)a.stages) {
+    if (lane < a.stages) {
       mbar_init(full_bar(lane), kCodes ? 1 : 2);  // the producer, and the helper that makes codes
       mbar_init(empty_bar(lane), 1);
     }
@@ -310,7 +316,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
 
   auto source = [&](const BsTile& m, int r) {     // the row of x that the tile's row r is
     const int at = m.first + min(r, m.rows - 1);
-    return a.offsets && a.x_by_pair ? min(bs_pair(a.order, at, a.M) / a.top, a.x_rows - 1) : at;
+    return a.offsets && (a.modes & kBsByPair) ? min(bs_pair(a.order, at, a.M) / a.top, a.x_rows - 1) : at;
   };
 
   if (warp == 0) {
@@ -320,9 +326,9 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     bool ok = true;
     auto bytes = [&](const BsTile& m) { return kBsWBytes + (kCodes ? ((m.rows + 31) >> 5) * 32 * kBlk : 0); };
     if (!a.offsets) {
-      for (int t = cluster_id; t < num_tiles && ahead < (int)a.stages; t += clusters) {
+      for (int t = cluster_id; t < num_tiles && ahead < a.stages; t += clusters) {
         const BsTile m = tile_of(t);
-        for (int kb = kb0; kb < kb1 && ahead < (int)a.stages; ++kb, ++ahead)
+        for (int kb = kb0; kb < kb1 && ahead < a.stages; ++kb, ++ahead)
           if (leader) {
             mbar_expect_tx(full_bar(ahead), bytes(m));
             tma_load_2d(base + ahead * S::kStage, &map_w, 0, w_row(m, kb), full_bar(ahead));
@@ -354,7 +360,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
           }
           __syncwarp();
         }
-        if (++s == (int)a.stages) { s = 0; phase ^= 1; }
+        if (++s == a.stages) { s = 0; phase ^= 1; }
       }
     }
   } else if (warp == 1) {
@@ -387,7 +393,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
           umma_commit(empty_bar(s));
         }
         __syncwarp();
-        if (++s == (int)a.stages) { s = 0; phase ^= 1; }
+        if (++s == a.stages) { s = 0; phase ^= 1; }
         if (++b == S::kBufs) { b = 0; acc_phase ^= 1; }
       }
     }
@@ -496,7 +502,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
         }
       }
       if (!ok) continue;
-      switch (a.ep.act) {
+      switch (a.act) {
         case MOE_ACT_NONE: bs_finish<MOE_ACT_NONE, NT>(red, log_splits, rank, m, a, y, ldy, et, 32 * S::kStorers); break;
         case MOE_ACT_RELU2: bs_finish<MOE_ACT_RELU2, NT>(red, log_splits, rank, m, a, y, ldy, et, 32 * S::kStorers); break;
         case MOE_ACT_SILU: bs_finish<MOE_ACT_SILU, NT>(red, log_splits, rank, m, a, y, ldy, et, 32 * S::kStorers); break;
@@ -544,7 +550,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
             float* scales = step_scales + slot * S::kScales;
 #pragma unroll
             for (int i = 0; i < NT / 32; ++i) {
-              outside |= a.far.outside(v[j][i]);
+              outside |= a.outside(v[j][i]);
               scales[lane + 32 * i] = v[j][i] * even[j];
               scales[NT + 8 + lane + 32 * i] = v[j][i] * odd[j];
             }
@@ -597,7 +603,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
             for (int o = 1; o < 8; o <<= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
             float scale, inverse;
             bs_run_scale(largest, scale, inverse);
-            outside |= a.far.outside(scale);
+            outside |= a.outside(scale);
             if (r < m.rows) {
               *reinterpret_cast<uint4*>(codes + r * kBlk + ((eighth ^ (r & 7)) << 4)) = bs_codes16<TX>(now.raw[h], inverse);
               if (eighth == 0) {
@@ -643,7 +649,7 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
   }
-  // Rows with far scales: by the producer's warp, whose instructions here delay no other.  
+  // Rows with far scales: by the producer's warp, whose instructions here delay no other.
   if (warp == 0 && *reinterpret_cast<volatile uint32_t*>(smem_gen + (far_seen - base)))
     for (int t = cluster_id; t < num_tiles; t += clusters) bs_tile_apart<TX, TO>(a, tile_of(t), rank, splits, lane, y, ldy);
 }
@@ -752,19 +758,19 @@ TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, in
   if (M == 0 || N == 0) return TIB_OK;
   const bool is_codes = x_dtype < 0;
   if (!x || !w || !w_scales || !y || M < 0 || N < 0 || K < 1 || experts < 1 || top < 1 || x_rows < 1) return TIB_E_ARG;
-  if ((is_codes && (!x_scales || (offsets && x_by_pair) || x_rows < M || lds < M)) || (offsets && !order) || (row_scale && !order)) return TIB_E_ARG;
+  if ((is_codes && (!x_scales || (offsets && x_by_pair) || x_rows < M || lds < M || lds > 0x7fffffff)) || (offsets && !order) || (row_scale && !order)) return TIB_E_ARG;
   if (act < MOE_ACT_NONE || act > MOE_ACT_GELU || (moe_act_gated(act) && !pairs) || (pairs && N % 2)) return TIB_E_SIZE;
   if (x_dtype > TIB_BF16 || (y_dtype != TIB_BF16 && y_dtype != TIB_F32)) return TIB_E_DTYPE;
   if (experts > kBsMaxExperts || (int64_t)experts * ceil_div(N, 128) * ceil_div(K, kBlk) > (0x7fffffff >> 7)) return TIB_E_SIZE;
   if ((((uintptr_t)w) & 15) || (is_codes && (((uintptr_t)x) & 15))) return TIB_E_ALIGN;
   BsArgs a;
-  a.x = x; a.w = static_cast<const unsigned char*>(w); a.far = BsFar{far_low, far_high}; a.ldx = ldx;
-  a.x_scales = x_scales; a.lds = lds; a.w_scales = w_scales; a.scale_rows = scale_rows; a.pairs = pairs != 0;
+  a.x = x; a.ldx = ldx; a.x_scales = x_scales; a.w = static_cast<const unsigned char*>(w); a.w_scales = w_scales; a.scale_rows = scale_rows; a.pairs = pairs;
   a.vec = !is_codes && ((uintptr_t)x & 15) == 0 && (ldx * (x_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
-  a.wide = ((uintptr_t)y & 15) == 0 && (ldy * (y_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
-  a.M = M; a.N = N; a.K = K; a.x_rows = x_rows; a.runs = ceil_div(K, kBlk); a.offsets = offsets; a.order = order; a.experts = experts; a.top = top;
-  a.x_by_pair = x_by_pair != 0; a.error_word = error_word;
-  a.ep.act = act; a.ep.limit = limit; a.ep.alpha = alpha; a.ep.row_scale = row_scale;
+  a.lds = (int)lds; a.M = M; a.N = N; a.K = K; a.runs = ceil_div(K, kBlk); a.x_rows = x_rows; a.offsets = offsets; a.order = order; a.experts = experts; a.top = top;
+  const bool wide = ((uintptr_t)y & 15) == 0 && (ldy * (y_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
+  a.modes = (x_by_pair ? kBsByPair : 0) | (wide ? kBsWide : 0);
+  a.far_low = far_low; a.far_high = far_high;
+  a.act = act; a.limit = limit; a.alpha = alpha; a.row_scale = row_scale; a.error_word = error_word;
   CUtensorMap map_w, map_x;
   int rc = bs_make_map(&map_w, w, (int64_t)experts * ceil_div(N, 128) * a.runs * 128, kBlk, 128);
   if (rc != TIB_OK) return rc;
