@@ -124,9 +124,10 @@ def _normal_range(scales: torch.Tensor) -> tuple[float, float]:
     """The least and the largest of the powers of two whose product with every one of ``scales`` is a normal 32-bit number, or exact all the same
     (powers of at least 1: 1 always is one of them); the kernels look after other products one by one."""
     sizes = scales.abs()
-    least = torch.where(sizes > 0, sizes, math.inf).amin()
-    most = torch.where(torch.isfinite(sizes), sizes, 0.0).amax()
-    least, most = torch.stack([least, most]).tolist()
+    least, most = torch.stack(torch.aminmax(sizes)).tolist()
+    if not (least > 0 and most < math.inf):      # (zeros are products already, infinities and NaNs remain ones)
+        least = torch.where(sizes > 0, sizes, math.inf).amin().item()
+        most = torch.where(torch.isfinite(sizes), sizes, 0.0).amax().item()
     low = -126 if math.isinf(least) else max(min(-125 - math.frexp(least)[1], 0), -126)      # (least is at least 2^(its exponent - 1))
     high = 120 if most == 0 else min(128 - math.frexp(most)[1], 120)                         # (most is less than 2^(its exponent))
     return 2.0 ** low, 2.0 ** high
