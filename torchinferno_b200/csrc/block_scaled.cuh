@@ -192,8 +192,7 @@ template <typename TX> struct BsApart {
     return far;
   }
   // By one thread, 16 columns at a time.  A far scale's share is made in two steps, s shifted by 2^64 (without rounding) and the share shifted back:
-  // v (s 2^64 S) 2^-64 where S is below 1 and s S too
-  // small, v (s 2^-64 S) 2^64 where it is too large (s is at most 2^120: that takes an S of 2^8).
+  // v (s 2^64 S) 2^-64 where S is below 1 and s S too small, v (s 2^-64 S) 2^64 where it is too large (s is at most 2^120: that takes an S of 2^8).
   __device__ float sum(int f) const {
     const float* ws = w_scales + (size_t)bs_scale_row(f, pairs) * runs;
     float inverse = 0.f, sum = 0.f;
