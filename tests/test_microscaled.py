@@ -1,0 +1,135 @@
+"""4-bit microscaled matrices on the host: their types, how they are laid out, and what is refused before a kernel runs."""
+import pytest
+import torch
+
+from microscaled_oracle import CODES, matrix64, nearest, random_matrix
+from torchinferno_b200.kernels import block_scaled, gemm, microscaled, ops
+from torchinferno_b200.kernels.microscaled import MicroscaledExperts, MicroscaledMatrix, MicroscaledWeight, quantize_matrix, quantize_rows
+
+
+def test_a_matrix_stands_for_its_numbers():
+    for n, k in ((1, 1), (3, 16), (5, 33), (130, 100)):
+        matrix = random_matrix(n, k, n + k)
+        assert matrix.shape == (n, k) and torch.equal(matrix.widened().double(), matrix64(matrix).float().double())
+        assert matrix.widened(torch.bfloat16).dtype == torch.bfloat16
+
+
+@pytest.mark.parametrize("n, k", [(1, 1), (7, 16), (40, 333), (3, 1000)])
+def test_quantising_a_matrix(n, k):
+    g = torch.Generator().manual_seed(n)
+    w = torch.randn(n, k, generator=g) * torch.randn(n, 1, generator=g).exp()
+    made = quantize_matrix(w)
+    # a number lies between codes at most 2 apart, of a size up to 6 scales: it is off by at most one scale, and by what a scale rounded down (2^-4) cuts off above 6
+    scale = made.scales.float().double()[:, torch.arange(k) // 16] * made.factor.double()
+    assert ((made.widened().double() - w.double()).abs() <= scale * (1 + 2.0 ** -20)).all()
+    # and no code is nearer than the one taken (but for the borders themselves)
+    size = (w.double() / torch.where(scale == 0, 1.0, scale)).abs()
+    best = torch.tensor(CODES, dtype=torch.float64)[nearest(size, CODES)]
+    taken = (made.widened().double() / torch.where(scale == 0, 1.0, scale)).abs()
+    assert ((taken - size).abs() <= (best - size).abs() + 1e-5).all()
+    assert torch.equal(quantize_matrix(torch.zeros(2, 20)).widened(), torch.zeros(2, 20))
+
+
+def number(tiles, i, n, k):
+    """Number (n, k) of matrix i, read from where the kernels look for it."""
+    tile, row, step, column = n // 128, n % 128, k // 256, k % 256
+    byte = int(tiles.codes[i, tile, step, row, column // 2])
+    scales = tiles.scales[i, tile, step].view(torch.float8_e4m3fn)
+    at = (column // 64) * 512 + (row % 32) * 16 + (row // 32) * 4 + (column % 64) // 16
+    code = byte >> 4 if column % 2 else byte & 15
+    return CODES[code & 7] * (-1 if code > 7 else 1) * float(scales[at]) * float(tiles.factors[i, n])
+
+
+def test_where_the_kernels_find_a_matrix():
+    a, b = random_matrix(150, 301, 1), random_matrix(20, 301, 2, factor=0.5)
+    tiles = MicroscaledWeight(a, b).tiles
+    assert tiles.codes.shape == (1, 2, 2, 128, 128) and tiles.scales.shape == (1, 2, 2, 2048) and tiles.features == 170
+    wide = torch.cat([a.widened(), b.widened()])
+    for n in (0, 1, 31, 32, 127, 128, 149, 150, 169):
+        for k in (0, 1, 15, 16, 63, 64, 255, 256, 300):
+            assert number(tiles, 0, n, k) == pytest.approx(float(wide[n, k]), rel=1e-6)
+    assert not tiles.codes[0, 1, :, 42:].any() and not (tiles.codes[0, :, 1, :, 23:]).any()
+    gates, ups = [random_matrix(70, 64, i) for i in (3, 4)], [random_matrix(70, 64, i, factor=0.3) for i in (5, 6)]
+    tiles = MicroscaledExperts(gates, ups).tiles
+    for i in range(2):
+        for n in (0, 1, 64, 69):
+            assert number(tiles, i, 2 * n, 20) == pytest.approx(float(gates[i].widened()[n, 20]), rel=1e-6)
+            assert number(tiles, i, 2 * n + 1, 20) == pytest.approx(float(ups[i].widened()[n, 20]), rel=1e-6)
+
+
+def test_views_of_a_weight():
+    weight = MicroscaledWeight(random_matrix(300, 40, 1))
+    view = weight.rows(128, 290)
+    assert view.out_features == 162 and view.tiles.features == 162 and view.tiles.codes.shape[1] == 2
+    assert view.tiles.codes_at == weight.tiles.codes[:, 1].data_ptr() and view.tiles.factors_at == weight.tiles.factors[:, 128:].data_ptr()
+    with pytest.raises(ValueError, match="inside a tile"):
+        weight.rows(64, 128)
+    for start, stop in ((0, 301), (5, 5), (-1, 3)):
+        with pytest.raises(ValueError, match="no features"):
+            weight.rows(start, stop)
+    assert weight.nbytes() == 3 * 128 * 128 + 3 * 2048 + 4 * 300 and weight.device.type == "cpu"
+
+
+def test_matrices_that_are_refused():
+    good = random_matrix(4, 32, 1)
+    with pytest.raises(ValueError, match="uint8"):
+        MicroscaledMatrix(good.codes.to(torch.int32), good.scales, good.factor)
+    with pytest.raises(ValueError, match="bytes of codes"):
+        MicroscaledMatrix(good.codes, good.scales, good.factor, columns=30)
+    with pytest.raises(ValueError, match="scales of a"):
+        MicroscaledMatrix(good.codes, good.scales[:, :1], good.factor)
+    with pytest.raises(ValueError, match="scales of a"):
+        MicroscaledMatrix(good.codes, good.scales.float(), good.factor)
+    with pytest.raises(ValueError, match="one float32 number"):
+        MicroscaledMatrix(good.codes, good.scales, good.factor.expand(2))
+    for bad in (-1.0, float("nan")):
+        scales = good.scales.float()
+        scales[2, 1] = bad
+        with pytest.raises(ValueError, match="none of them negative"):
+            MicroscaledWeight(MicroscaledMatrix(good.codes, scales.to(torch.float8_e4m3fn), good.factor))
+    with pytest.raises(ValueError, match="alike"):
+        MicroscaledWeight(good, random_matrix(4, 48, 2))
+    with pytest.raises(ValueError, match="gate and an up"):
+        MicroscaledWeight(good, epilogue="swiglu")
+    with pytest.raises(ValueError, match="of one size"):
+        MicroscaledWeight(good, random_matrix(5, 32, 2), epilogue="swiglu")
+    with pytest.raises(ValueError, match="unknown epilogue"):
+        MicroscaledWeight(good, epilogue="gelu")
+    with pytest.raises(ValueError, match="made of microscaled"):
+        MicroscaledWeight(torch.zeros(3, 3))
+    with pytest.raises(ValueError, match="at least one"):
+        MicroscaledExperts([])
+    with pytest.raises(ValueError, match="1 gate and 2 up"):
+        MicroscaledExperts([good], [good, good])
+    with pytest.raises(ValueError, match="non-empty matrix"):
+        quantize_matrix(torch.zeros(0, 3))
+
+
+def test_weights_from_matrices():
+    four, eight = random_matrix(4, 32, 1), block_scaled.quantize_matrix(torch.ones(4, 32))
+    assert isinstance(gemm.projection(four, four), MicroscaledWeight) and isinstance(gemm.gated_projection(four, four), MicroscaledWeight)
+    assert isinstance(gemm.expert_matrices([four, four]), MicroscaledExperts)
+    for other in (eight, torch.ones(4, 32)):
+        with pytest.raises(ValueError, match="all be stored in 4-bit codes, or none"):
+            gemm.projection(four, other)
+
+
+def test_calls_that_are_refused_without_a_gpu():
+    x, weight, residual = torch.zeros(2, 32), MicroscaledWeight(random_matrix(4, 32, 1)), torch.zeros(2, 32)
+    for call in (lambda: quantize_rows(x), lambda: gemm.linear(x, weight), lambda: microscaled.add_rmsnorm(None, residual, torch.ones(32), 1e-5)):
+        with pytest.raises(ops.KernelError, match="CUDA"):
+            call()
+    with pytest.raises(ops.KernelError, match="rows of 32"):
+        gemm.linear(torch.zeros(2, 31), weight)
+    with pytest.raises(ops.KernelError, match="epilogue='swiglu'"):
+        gemm.linear_swiglu(x, weight)
+    with pytest.raises(ops.KernelError, match="delta is"):
+        microscaled.add_rmsnorm(x, residual, torch.ones(32), 1e-5, dtype=torch.bfloat16)
+    eight_rows = block_scaled.BlockScaledRows(x, 2, 32, torch.bfloat16)
+    with pytest.raises(ops.KernelError, match="not BlockScaledRows"):
+        gemm.linear(eight_rows, weight)
+    with pytest.raises(ops.KernelError, match="not MicroscaledRows"):
+        gemm.linear(microscaled.MicroscaledRows(x, 2, 32, torch.bfloat16), block_scaled.BlockScaledWeight(block_scaled.quantize_matrix(torch.ones(4, 32))))
+    for product in (gemm.linear, gemm.linear_swiglu):
+        with pytest.raises(ops.KernelError, match="quantised rows are for quantised weights"):
+            product(eight_rows, gemm.LinearWeight(torch.ones(4, 32), few_rows_tcgen05=False))

@@ -1,4 +1,4 @@
-// Rows of activations to 8-bit codes with a power of two for each run of 128 columns (block_scaled.cuh).
+// Rows of activations to 8-bit codes with a power of two for each run of 128 columns (block_scaled.cuh), and back.
 //
 // Eight lanes take a run, 16 columns each: their largest absolute value by its bits as an integer (a NaN is then the
 // largest of all, where a maximum of floats would pass over it), a butterfly of three steps, one multiplication and one
@@ -31,6 +31,39 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__
   if (eighth == 0) scales[(size_t)run * lds + row] = scale;
 }
 
+// The numbers that codes stand for: a thread takes sixteen.
+template <typename TO>
+__global__ void __launch_bounds__(256)
+widen_rows_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const float* __restrict__ scales, int64_t lds, TO* __restrict__ out, int64_t ldo, int rows, int K, int wide) {
+  pdl_wait();
+  pdl_trigger();
+  const int parts = (K + 15) >> 4;
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int row = (int)(i / parts), col = (int)(i - (int64_t)row * parts) << 4;
+  if (row >= rows) return;
+  const uint4 c = *reinterpret_cast<const uint4*>(codes + (size_t)row * ldc + col);
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  const float s = scales[(size_t)(col >> 7) * lds + row];
+  TO v[16];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    uint32_t p;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(p) : "h"((uint16_t)(w[j >> 1] >> (16 * (j & 1)))));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
+    v[2 * j] = from_f32<TO>(f.x * s);
+    v[2 * j + 1] = from_f32<TO>(f.y * s);
+  }
+  TO* dst = out + (size_t)row * ldo + col;
+  if (wide && col + 16 <= K) {
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(TO); ++j) reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(v)[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (col + j < K) dst[j] = v[j];
+  }
+}
+
 }  // namespace tib
 
 using namespace tib;
@@ -58,6 +91,21 @@ TIB_API int tib_quantize_rows(const void* x, int x_dtype, int64_t ldx, void* cod
     else TIB_QUANT_GO(float, false);
   }
 #undef TIB_QUANT_GO
+  return TIB_OK;
+}
+
+// The numbers [rows, K] that codes [rows, ldc] and scales [runs, lds], as tib_quantize_rows leaves them, stand for, in out_dtype (row stride ldo).
+TIB_API int tib_widen_rows(const void* codes, int64_t ldc, const float* scales, int64_t lds, void* out, int out_dtype, int64_t ldo, int rows, int K, cudaStream_t stream) {
+  if (rows == 0) return TIB_OK;
+  if (!codes || !scales || !out || rows < 0 || K < 1) return TIB_E_ARG;
+  if (out_dtype != TIB_BF16 && out_dtype != TIB_F32) return TIB_E_DTYPE;
+  if (ldc < (int64_t)ceil_div(K, kBlk) * kBlk || lds < rows) return TIB_E_SIZE;
+  if (((uintptr_t)codes & 15) || ldc % 16) return TIB_E_ALIGN;
+  const int64_t grid = ceil_div64((int64_t)rows * ceil_div(K, 16), 256);
+  if (grid > 0x7fffffff) return TIB_E_SIZE;
+  const int wide = ((uintptr_t)out & 15) == 0 && (ldo * (out_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
+  if (out_dtype == TIB_BF16) TIB_LAUNCH_DEPENDENT(widen_rows_kernel<__nv_bfloat16>, (unsigned)grid, 256, 0, stream, (const uint8_t*)codes, ldc, scales, lds, (__nv_bfloat16*)out, ldo, rows, K, wide);
+  else TIB_LAUNCH_DEPENDENT(widen_rows_kernel<float>, (unsigned)grid, 256, 0, stream, (const uint8_t*)codes, ldc, scales, lds, (float*)out, ldo, rows, K, wide);
   return TIB_OK;
 }
 
@@ -111,5 +159,6 @@ TIB_API int tib_block_scaled_product(const void* x, int x_dtype, int64_t ldx, in
 
 // The calls the Python parts make (common.cuh).
 TIB_PACKED(tib_quantize_rows)
+TIB_PACKED(tib_widen_rows)
 TIB_PACKED(tib_block_scaled_product)
 TIB_PACKED(tib_block_scaled_plan)

@@ -209,6 +209,11 @@ static inline cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, dim3
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
+// Threads of a block that norms a row: about four numbers each.
+static inline int norm_threads(int hidden) {
+  const int t = ((hidden + 3) / 4 + 31) / 32 * 32;
+  return t < 32 ? 32 : t > 1024 ? 1024 : t;
+}
 static inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 static inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 

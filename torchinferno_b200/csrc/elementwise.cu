@@ -283,13 +283,6 @@ __global__ void decode_inputs_kernel(int* __restrict__ records, const int* __res
   }
 }
 
-static inline int norm_threads(int hidden) {
-  int t = ((hidden + 3) / 4 + 31) / 32 * 32;  // about four elements a thread
-  if (t < 32) t = 32;
-  if (t > 1024) t = 1024;
-  return t;
-}
-
 }  // namespace tib
 
 using namespace tib;

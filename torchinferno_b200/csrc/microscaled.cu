@@ -1,0 +1,254 @@
+// Rows of activations to 4-bit codes with their scales (microscaled.cuh) and back, and the product of such rows with 4-bit matrices.
+#include "microscaled.cuh"
+
+namespace tib {
+
+// the largest of a block's values, for up to 1024 threads; `scratch`: 32 words, not in use by an earlier call
+__device__ __forceinline__ uint32_t ms_block_max(uint32_t v, uint32_t* scratch) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  if (blockDim.x <= 32) return v;
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+  __syncthreads();
+  const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+  return __reduce_max_sync(0xffffffffu, lane < warps ? scratch[lane] : 0u);
+}
+
+// A block takes a row, a thread runs of 16 columns of it, up to kMsHeld of which it keeps: the row's largest number has to be known before the
+// first code is.  (Wider rows are read again, from the L2.)
+constexpr int kMsHeld = 4;
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+microscaled_rows_kernel(const T* __restrict__ x, int64_t ldx, int x_rows, unsigned char* __restrict__ codes, unsigned char* __restrict__ scales,
+                        float* __restrict__ factors, int rows, int K, int steps, const int* __restrict__ offsets, const int* __restrict__ order,
+                        int experts, int top, int x_by_pair) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ uint32_t scratch[32];
+  const int row = blockIdx.x, runs = steps * (kMsStep / kMsRun);
+  int from = row, tile = row >> 7, at = row & 127;
+  if (offsets) {
+    if (row >= bs_offset(offsets, experts, rows)) return;
+    int lo = 0, hi = experts;      // offsets[lo] <= row < offsets[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (bs_offset(offsets, mid, rows) <= row) lo = mid; else hi = mid;
+    }
+    const int first = bs_offset(offsets, lo, rows);
+    if (row < first) return;       // (rows ahead of the first expert's are none's)
+    tile = ms_first_tile(first, lo) + ((row - first) >> 7);
+    at = (row - first) & 127;
+    if (x_by_pair) from = min(bs_pair(order, row, rows) / top, x_rows - 1);
+  }
+  const T* src = x + (size_t)from * ldx;
+  uint4 held[kMsHeld][sizeof(T)];
+  uint32_t largest = 0;
+#pragma unroll
+  for (int i = 0; i < kMsHeld; ++i) {
+    const int run = threadIdx.x + i * blockDim.x;
+    bs_ask16<T, VEC>(src + run * kMsRun, run < runs ? K - run * kMsRun : 0, held[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kMsHeld; ++i) largest = max(largest, bs_largest16<T>(held[i]));
+  for (int run = threadIdx.x + kMsHeld * blockDim.x; run < runs; run += blockDim.x) {
+    uint4 raw[sizeof(T)];
+    bs_ask16<T, VEC>(src + run * kMsRun, K - run * kMsRun, raw);
+    largest = max(largest, bs_largest16<T>(raw));
+  }
+  float r, inverse;
+  ms_row_scale(ms_block_max(largest, scratch), r, inverse);
+  if (threadIdx.x == 0) factors[row] = r;
+  unsigned char* codes_row = codes + (size_t)row * steps * kMsStepBytes;
+  unsigned char* scales_row = scales + (size_t)tile * steps * kMsStepScales + ms_scale_at(at);
+  auto finish = [&](int run, const uint4 (&raw)[sizeof(T)]) {      // (whole quarters of a warp: runs and block sizes are multiples of 16)
+    if (run >= runs) return;
+    const float t = __uint_as_float(bs_largest16<T>(raw)) * inverse;
+    const uint32_t scale = inverse == 0.f ? 0u : ms_run_scale<T>(t);
+    const float reciprocal = ms_reciprocal(ms_scale_value(scale));
+    float v[16], lo[8], hi[8];
+    bs_floats16<T>(raw, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) lo[j] = v[j], hi[j] = v[8 + j];
+    const uint2 c = scale == 0 ? make_uint2(0, 0) : make_uint2(ms_codes8<T>(lo, inverse, reciprocal), ms_codes8<T>(hi, inverse, reciprocal));
+    *reinterpret_cast<uint2*>(codes_row + run * (kMsRun / 2)) = c;
+    const uint32_t mask = 0xfu << (threadIdx.x & 28), base = threadIdx.x & 28;
+    uint32_t four = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) four |= __shfl_sync(mask, scale, base + j) << (8 * j);
+    if ((threadIdx.x & 3) == 0) *reinterpret_cast<uint32_t*>(scales_row + (size_t)(run >> 2) * kMsChunkBytes) = four;
+  };
+#pragma unroll
+  for (int i = 0; i < kMsHeld; ++i) finish(threadIdx.x + i * blockDim.x, held[i]);
+  for (int run = threadIdx.x + kMsHeld * blockDim.x; run < runs; run += blockDim.x) {
+    uint4 raw[sizeof(T)];
+    bs_ask16<T, VEC>(src + run * kMsRun, K - run * kMsRun, raw);
+    finish(run, raw);
+  }
+}
+
+// The numbers that quantised rows stand for: a thread takes a run.
+template <typename TO>
+__global__ void __launch_bounds__(256)
+microscaled_widen_kernel(MsRows x, TO* __restrict__ out, int64_t ldo, int rows, int K, int steps, int wide) {
+  pdl_wait();
+  pdl_trigger();
+  const int runs = (K + kMsRun - 1) / kMsRun;
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int row = (int)(i / runs), run = (int)(i - (int64_t)row * runs);
+  if (row >= rows) return;
+  const uint2 c = *reinterpret_cast<const uint2*>(x.codes + ((size_t)row * steps * kMsStepBytes + run * (kMsRun / 2)));
+  const float s = ms_scale_value(x.scales[((size_t)(row >> 7) * steps * 4 + (run >> 2)) * kMsChunkBytes + ms_scale_at(row & 127) + (run & 3)]), r = x.factors[row];
+  float v[16];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float2 p = ms_numbers2(((j < 4 ? c.x : c.y) >> (8 * (j & 3))) & 0xffu);
+    v[2 * j] = p.x * s * r;
+    v[2 * j + 1] = p.y * s * r;
+  }
+  TO* dst = out + (size_t)row * ldo + run * kMsRun;
+  TO w[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) w[j] = from_f32<TO>(v[j]);
+  if (wide && run * kMsRun + kMsRun <= K) {
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(TO); ++j) reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(w)[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (run * kMsRun + j < K) dst[j] = w[j];
+  }
+}
+
+// A product, a thread for each output.
+__device__ float ms_dot(const unsigned char* x, const unsigned char* xs, const unsigned char* w, const unsigned char* ws, int steps) {
+  float sum = 0.f;
+  for (int step = 0; step < steps; ++step) {
+    for (int run = 0; run < 16; ++run) {
+      float v = 0.f;
+      for (int i = 0; i < 8; ++i) {
+        const float2 a = ms_numbers2(x[run * 8 + i]), b = ms_numbers2(w[run * 8 + i]);
+        v += a.x * b.x + a.y * b.y;
+      }
+      const int at = (run >> 2) * kMsChunkBytes + (run & 3);
+      sum += v * (ms_scale_value(xs[at]) * ms_scale_value(ws[at]));
+    }
+    x += kMsStepBytes; xs += kMsStepScales; w += kMsTileRows * kMsStepBytes; ws += kMsStepScales;
+  }
+  return sum;
+}
+template <typename TO>
+__global__ void __launch_bounds__(256)
+microscaled_product_kernel(MsArgs a, int act, TO* __restrict__ y, int64_t ldy) {
+  pdl_wait();
+  pdl_trigger();
+  const int gated = moe_act_gated(act) ? 1 : 0, n_out = a.N >> gated, row = blockIdx.y, o = blockIdx.x * blockDim.x + threadIdx.x;
+  if (o >= n_out) return;
+  int expert = 0, first = 0, tile = 0;
+  if (a.offsets) {
+    if (row >= bs_offset(a.offsets, a.experts, a.M)) return;
+    int hi = a.experts;
+    while (hi - expert > 1) {
+      const int mid = (expert + hi) >> 1;
+      if (bs_offset(a.offsets, mid, a.M) <= row) expert = mid; else hi = mid;
+    }
+    first = bs_offset(a.offsets, expert, a.M);
+    if (row < first) return;
+    tile = ms_first_tile(first, expert);
+  }
+  const int in = row - first, f_tiles = (a.N + 127) >> 7;
+  const unsigned char* x = a.x.codes + (size_t)row * a.steps * kMsStepBytes;
+  const unsigned char* xs = a.x.scales + (size_t)(tile + (in >> 7)) * a.steps * kMsStepScales + ms_scale_at(in & 127);
+  auto sum = [&](int f) {
+    const size_t block = (size_t)expert * f_tiles + (f >> 7);
+    const float v = ms_dot(x, xs, a.w + (block * a.steps * kMsTileRows + (f & 127)) * kMsStepBytes, a.w_scales + block * a.steps * kMsStepScales + ms_scale_at(f & 127), a.steps);
+    const float scaled = v * a.w_factors[(size_t)expert * a.N + f] * a.x.factors[row];
+    return a.row_scale ? scaled * a.row_scale[bs_pair(a.order, row, a.M)] : scaled;
+  };
+  const float g = sum(o << gated), u = gated ? sum((o << gated) + 1) : 0.f;
+  float v = g;
+  switch (act) {
+    case MOE_ACT_RELU2: v = bs_act<MOE_ACT_RELU2>(g); break;
+    case MOE_ACT_SILU: v = bs_act<MOE_ACT_SILU>(g); break;
+    case MOE_ACT_GELU: v = bs_act<MOE_ACT_GELU>(g); break;
+    case MOE_ACT_GLU_CLAMP: v = bs_gated<MOE_ACT_GLU_CLAMP>(g, u, a.limit, a.alpha); break;
+    case MOE_ACT_SWIGLU: v = bs_gated<MOE_ACT_SWIGLU>(g, u, a.limit, a.alpha); break;
+  }
+  y[(size_t)row * ldy + o] = from_f32<TO>(v);
+}
+
+}  // namespace tib
+
+using namespace tib;
+
+// x: rows [x_rows, K] in x_dtype (row stride ldx); codes, scales, factors: as microscaled.cuh has them, of `rows` rows.  offsets [experts + 1] (and with x_by_pair order
+// [rows]: row m is made of row order[m] / top of x, else of row m): rows sorted by expert; null: one matrix for all.
+TIB_API int tib_microscaled_rows(const void* x, int x_dtype, int64_t ldx, int x_rows, void* codes, void* scales, float* factors, int rows, int K,
+                                 const int* offsets, const int* order, int experts, int top, int x_by_pair, cudaStream_t stream) {
+  if (rows == 0) return TIB_OK;
+  if (!x || !codes || !scales || !factors || rows < 0 || K < 1 || x_rows < 1 || experts < 1 || top < 1) return TIB_E_ARG;
+  if ((offsets && x_by_pair) ? !order : x_rows < rows) return TIB_E_ARG;
+  if (x_dtype != TIB_BF16 && x_dtype != TIB_F32) return TIB_E_DTYPE;
+  if (((uintptr_t)codes | (uintptr_t)scales) & 15) return TIB_E_ALIGN;
+  const int steps = ms_steps(K), runs = steps * (kMsStep / kMsRun), threads = runs >= 256 ? 256 : (runs + 31) / 32 * 32;
+  const bool vec = ((uintptr_t)x & 15) == 0 && (ldx * (x_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
+#define TIB_MS_ROWS_GO(T, VEC)                                                                                                                           \
+  TIB_LAUNCH_DEPENDENT((microscaled_rows_kernel<T, VEC>), (unsigned)rows, threads, 0, stream, (const T*)x, ldx, x_rows, (unsigned char*)codes,              \
+                       (unsigned char*)scales, factors, rows, K, steps, offsets, order, experts, top, x_by_pair)
+  if (x_dtype == TIB_BF16) {
+    if (vec) TIB_MS_ROWS_GO(__nv_bfloat16, true);
+    else TIB_MS_ROWS_GO(__nv_bfloat16, false);
+  } else {
+    if (vec) TIB_MS_ROWS_GO(float, true);
+    else TIB_MS_ROWS_GO(float, false);
+  }
+#undef TIB_MS_ROWS_GO
+  return TIB_OK;
+}
+
+// The numbers [rows, K] that rows as tib_microscaled_rows leaves them (offsets null) stand for, in out_dtype (row stride ldo).
+TIB_API int tib_microscaled_widen(const void* codes, const void* scales, const float* factors, void* out, int out_dtype, int64_t ldo, int rows, int K,
+                                  cudaStream_t stream) {
+  if (rows == 0) return TIB_OK;
+  if (!codes || !scales || !factors || !out || rows < 0 || K < 1) return TIB_E_ARG;
+  if (out_dtype != TIB_BF16 && out_dtype != TIB_F32) return TIB_E_DTYPE;
+  if (((uintptr_t)codes | (uintptr_t)scales) & 15) return TIB_E_ALIGN;
+  const int64_t grid = ceil_div64((int64_t)rows * ceil_div(K, kMsRun), 256);
+  if (grid > 0x7fffffff) return TIB_E_SIZE;
+  const MsRows r{(const unsigned char*)codes, (const unsigned char*)scales, factors};
+  const int wide = ((uintptr_t)out & 15) == 0 && (ldo * (out_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
+  if (out_dtype == TIB_BF16) TIB_LAUNCH_DEPENDENT(microscaled_widen_kernel<__nv_bfloat16>, (unsigned)grid, 256, 0, stream, r, (__nv_bfloat16*)out, ldo, rows, K, ms_steps(K), wide);
+  else TIB_LAUNCH_DEPENDENT(microscaled_widen_kernel<float>, (unsigned)grid, 256, 0, stream, r, (float*)out, ldo, rows, K, ms_steps(K), wide);
+  return TIB_OK;
+}
+
+// A product as its callers see it: y [M, N] (or [M, N / 2] of a gated activation) in y_dtype, row stride ldy.  codes, scales, factors: where the quantised rows
+// are, or (`make`) are put first, from rows x [x_rows, K].  w: codes, scales and factors [experts, N] of the matrices (`pairs`: of (gate, up) row pairs).
+// offsets [experts + 1], order [M], top, x_by_pair: rows sorted by expert as tib_moe_expert_product takes them; offsets null: one matrix for all rows.
+TIB_API int tib_microscaled_product(const void* x, int x_dtype, int64_t ldx, int x_rows, void* codes, void* scales, float* factors, int make, const void* w,
+                                    const void* w_scales, const float* w_factors, int pairs, void* y, int y_dtype, int64_t ldy, int M, int N, int K,
+                                    const int* offsets, const int* order, int experts, int top, int x_by_pair, int act, float limit, float alpha,
+                                    const float* row_scale, int* error_word, cudaStream_t stream) {
+  if (M == 0 || N == 0) return TIB_OK;
+  if (!codes || !scales || !factors || !w || !w_scales || !w_factors || !y || M < 0 || N < 0 || K < 1 || experts < 1 || top < 1) return TIB_E_ARG;
+  if ((offsets && !order) || (row_scale && !order)) return TIB_E_ARG;
+  if (act < MOE_ACT_NONE || act > MOE_ACT_GELU || (moe_act_gated(act) && !pairs) || (pairs && N % 2)) return TIB_E_SIZE;
+  if (y_dtype != TIB_BF16 && y_dtype != TIB_F32) return TIB_E_DTYPE;
+  if (((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)w | (uintptr_t)w_scales) & 15) return TIB_E_ALIGN;
+  if (make) {
+    const int rc = tib_microscaled_rows(x, x_dtype, ldx, x_rows, codes, scales, factors, M, K, offsets, order, experts, top, x_by_pair, stream);
+    if (rc != TIB_OK) return rc;
+  }
+  MsArgs a;
+  a.x = MsRows{(const unsigned char*)codes, (const unsigned char*)scales, factors};
+  a.w = (const unsigned char*)w; a.w_scales = (const unsigned char*)w_scales; a.w_factors = w_factors;
+  a.M = M; a.N = N; a.steps = ms_steps(K); a.offsets = offsets; a.order = order; a.experts = experts; a.limit = limit; a.alpha = alpha;
+  a.row_scale = row_scale;
+  (void)error_word;
+  const dim3 grid(ceil_div(N >> (moe_act_gated(act) ? 1 : 0), 256), M);
+  if (y_dtype == TIB_BF16) TIB_LAUNCH_DEPENDENT(microscaled_product_kernel<__nv_bfloat16>, grid, 256, 0, stream, a, act, (__nv_bfloat16*)y, ldy);
+  else TIB_LAUNCH_DEPENDENT(microscaled_product_kernel<float>, grid, 256, 0, stream, a, act, (float*)y, ldy);
+  return TIB_OK;
+}
+
+TIB_PACKED(tib_microscaled_rows)
+TIB_PACKED(tib_microscaled_widen)
+TIB_PACKED(tib_microscaled_product)

@@ -1,0 +1,153 @@
+// What the kernels of 4-bit microscaled operands share.
+//
+// A code is an e2m1 number (a sign, two bits of exponent, one of mantissa: 0, 1/2, 1, 3/2, 2, 3, 4, 6), two in a byte, the even column in the lower half.
+// Sixteen columns have one e4m3 scale (never negative).  A matrix [N, K] has one fp32 factor, held for each of its rows; rows x [M, K] have a power
+// of two each.  Columns are padded with zeros to whole steps of 256 (128 bytes of codes, the row of the 128-byte swizzle; four MMAs of 64 columns).
+//   codes of a matrix   [tiles of 128 rows][steps][128][128 bytes]: a step's 16 KB lie side by side in memory
+//   codes of rows       [M][steps][128 bytes]
+//   scales of both      [tiles of 128 rows][steps][4 chunks of 64 columns][512 bytes], row i of a tile at (i % 32) * 16 + (i / 32) * 4, a byte for each run of
+//                       16 columns: a chunk is what one tcgen05.cp of 32 x 128 bits brings to tensor memory, where lane i % 32 of column i / 32 then
+//                       holds the four scales of row i
+// The tiles of rows sorted by expert begin with the experts' first rows: expert e, whose rows begin at o_e, has the scales' tiles from
+// ceil(o_e / 128) + e on.  (o_e + n_e = o_(e + 1), so these end before the next expert's begin; all are fewer than ceil(M / 128) + experts.)
+#pragma once
+
+#include "block_scaled.cuh"
+#include "cluster.cuh"
+
+namespace tib {
+
+constexpr int kMsRun = 16, kMsStep = 256, kMsStepBytes = 128, kMsChunkBytes = 512, kMsStepScales = 4 * kMsChunkBytes, kMsTileRows = 128;
+
+static inline int ms_steps(int K) { return ceil_div(K, kMsStep); }
+__host__ __device__ __forceinline__ int ms_first_tile(int first_row, int expert) { return ((first_row + kMsTileRows - 1) >> 7) + expert; }
+// the place of row i of a tile's four scales of a chunk
+__host__ __device__ __forceinline__ int ms_scale_at(int i) { return ((i & 31) << 4) + ((i >> 5) << 2); }
+
+// A row whose largest absolute value has these bits: 2^p and 2^-p, p the smallest integer, at least -126, for which the largest is at most 2688 * 2^p (2688 =
+// 6 * 448 = 1.3125 * 2^11: the largest code times the largest scale); 1 for a row of zeros.  A power of two divides without rounding and leaves
+// the scales their three bits of mantissa over the 17 binades of e4m3.  A row that holds an infinity or a NaN gets a NaN, which shows in every output, and codes of 0.
+__device__ __forceinline__ void ms_row_scale(uint32_t largest, float& r, float& inverse) {
+  int p = (int)(largest >> 23) - 127 - 11 + ((largest & 0x7fffffu) > 0x280000u);
+  p = p < -126 ? -126 : p;
+  if (largest == 0) p = 0;
+  r = __uint_as_float((uint32_t)(p + 127) << 23);
+  inverse = __uint_as_float((uint32_t)(127 - p) << 23);
+  if (largest >= 0x7f800000u) { r = __uint_as_float(0x7fc00000u); inverse = 0.f; }
+}
+
+// Quotients are made with an approximate reciprocal and still rounded as the exact quotient is.  A border between two codes (or two scales) times the divisor has at
+// most seven significant bits, so a number of up to twelve is either on the border or off by 2^-12 of it, far more than the 2^-22 that the
+// product with the reciprocal is off by: rounded to 16 bits, it is on the border if and only if the exact quotient is.  A bf16 has eight bits; a 32-bit number
+// is first cut to twelve, the last of them set where any that was cut off is (which leaves it on the same side of every number of fewer bits).
+template <typename T> __device__ __forceinline__ float ms_odd12(float v) {
+  if constexpr (sizeof(T) == 2) return v;
+  const uint32_t b = __float_as_uint(v);
+  return __uint_as_float((b & 0xfffff000u) | (((b & 0xfffu) + 0xfffu) & 0x1000u));
+}
+__device__ __forceinline__ float ms_round16(float v) { return __uint_as_float((__float_as_uint(v) + 0x80u) & 0xffffff00u); }
+
+// The scale of a run whose largest number, times the row's inverse, is t: its e4m3 code; and what it stands for.
+template <typename T> __device__ __forceinline__ uint32_t ms_run_scale(float t) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(ms_round16(ms_odd12<T>(t) * (1.f / 6.f))));
+  return r & 0xffu;
+}
+__device__ __forceinline__ float ms_scale_value(uint32_t code) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)code));
+  return __half2float(__ushort_as_half((unsigned short)(h & 0xffffu)));
+}
+__device__ __forceinline__ float ms_reciprocal(float s) {      // 0 for 0
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  return s == 0.f ? 0.f : r;
+}
+// Eight numbers times `inverse` (a power of two) and `reciprocal` to eight codes, the first in the lowest four bits.
+template <typename T> __device__ __forceinline__ uint32_t ms_codes8(const float (&v)[8], float inverse, float reciprocal) {
+  const f32x2 inverse2 = f2_pack(inverse, inverse), reciprocal2 = f2_pack(reciprocal, reciprocal);
+  uint32_t codes = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    float a, b;
+    f2_unpack(f2_mul(f2_mul(f2_pack(ms_odd12<T>(v[j]), ms_odd12<T>(v[j + 1])), inverse2), reciprocal2), a, b);
+    uint32_t c;
+    asm("{\n.reg .b8 b;\ncvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\ncvt.u32.u8 %0, b;\n}\n" : "=r"(c) : "f"(ms_round16(b)), "f"(ms_round16(a)));
+    codes |= c << (4 * j);
+  }
+  return codes;
+}
+// two codes (a byte) to two floats
+__device__ __forceinline__ float2 ms_numbers2(uint32_t byte) {
+  uint32_t h;
+  asm("{\n.reg .b8 b;\ncvt.u8.u32 b, %1;\ncvt.rn.f16x2.e2m1x2 %0, b;\n}\n" : "=r"(h) : "r"(byte));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// D fp32 in tensor memory (+)= the product of a chunk's 64 columns: A and B e2m1 in shared memory, K-major (descriptors by their lower halves), each
+// row's four e4m3 scales in tensor memory.  The instruction descriptor but for N and M: both types e2m1, unsigned e4m3 scales.
+constexpr uint32_t kMsIdesc = (1u << 7) | (1u << 10);
+template <int CTAS>
+__device__ __forceinline__ void ms_umma(uint32_t leader, uint32_t tmem_d, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t a_scales, uint32_t b_scales,
+                                        uint32_t accumulate) {
+  static_assert(CTAS == 1 || CTAS == 2, "blocks of a tile");
+  if constexpr (CTAS == 1)
+    asm volatile("{\n.reg .pred p, q;\n.reg .b64 a, b;\nmov.b64 a, {%1, %8};\nmov.b64 b, {%2, %8};\nsetp.ne.b32 p, %6, 0;\nsetp.ne.b32 q, %7, 0;\n"
+                 "@q tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], a, b, %3, [%4], [%5], p;\n}\n"
+                 ::"r"(tmem_d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate), "r"(leader), "r"(kUmmaDescHigh) : "memory");
+  else
+    asm volatile("{\n.reg .pred p, q;\n.reg .b64 a, b;\nmov.b64 a, {%1, %8};\nmov.b64 b, {%2, %8};\nsetp.ne.b32 p, %6, 0;\nsetp.ne.b32 q, %7, 0;\n"
+                 "@q tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], a, b, %3, [%4], [%5], p;\n}\n"
+                 ::"r"(tmem_d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate), "r"(leader), "r"(kUmmaDescHigh) : "memory");
+}
+// A chunk's scales (512 bytes of shared memory: 32 rows of 16) to four columns of tensor memory, once for each of its four groups of lanes.  The descriptor: no
+// swizzle, groups of eight rows 128 bytes apart.
+template <int CTAS> __device__ __forceinline__ void ms_copy_scales(uint32_t leader, uint32_t tmem, uint32_t smem) {
+  const uint32_t low = (smem & 0x3FFFF) >> 4, high = (128u >> 4) | (1u << 14);
+  if constexpr (CTAS == 1)
+    asm volatile("{\n.reg .pred q;\n.reg .b64 s;\nmov.b64 s, {%1, %2};\nsetp.ne.b32 q, %3, 0;\n@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], s;\n}\n"
+                 ::"r"(tmem), "r"(low), "r"(high), "r"(leader) : "memory");
+  else
+    asm volatile("{\n.reg .pred q;\n.reg .b64 s;\nmov.b64 s, {%1, %2};\nsetp.ne.b32 q, %3, 0;\n@q tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], s;\n}\n"
+                 ::"r"(tmem), "r"(low), "r"(high), "r"(leader) : "memory");
+}
+// Bytes side by side in memory to shared memory (both 16-byte aligned, a multiple of 16), counted on a barrier.
+__device__ __forceinline__ void ms_bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// The rows of a product: x as codes.
+struct MsRows {
+  const unsigned char* codes;      // [M, steps * 128]
+  const unsigned char* scales;     // [tiles, steps, 2048]
+  const float* factors;            // [M]
+};
+
+// A product's arguments.
+struct MsArgs {
+  MsRows x;
+  const unsigned char* w;          // codes of the matrices
+  const unsigned char* w_scales;
+  const float* w_factors;          // [experts, N]
+  int M, N, steps, stages;
+  const int* offsets;              // [experts + 1] of rows sorted by expert, or null: one matrix
+  const int* order;
+  int experts;
+  float limit, alpha;              // of the clamped gated unit
+  const float* row_scale;          // [M] by pair, or null
+  int* error_word;
+};
+
+// An output from its sum(s): times the matrix's factor, the row's (a power of two) and the pair's, in turn, so that nothing leaves the range of 32 bits but what the
+// output itself does.
+__device__ __forceinline__ float ms_scaled(float sum, float w_factor, float x_factor, float row_scale) { return sum * w_factor * x_factor * row_scale; }
+
+}  // namespace tib
+
+extern "C" {
+int tib_microscaled_rows(const void* x, int x_dtype, int64_t ldx, int x_rows, void* codes, void* scales, float* factors, int rows, int K, const int* offsets,
+                         const int* order, int experts, int top, int x_by_pair, cudaStream_t stream);
+int tib_microscaled_tcgen05(const void* codes, const void* scales, const float* factors, const void* w, const void* w_scales, const float* w_factors, void* y,
+                            int y_dtype, int64_t ldy, int M, int N, int K, const int* offsets, const int* order, int experts, int act, float limit, float alpha,
+                            const float* row_scale, int* error_word, cudaStream_t stream);
+}

@@ -1,0 +1,211 @@
+// Root-mean-square norm with the residual's addition, as tib_add_rmsnorm, whose rows leave as codes and scales: in 4 bits (microscaled.cuh) or in 8
+// (block_scaled.cuh).
+//     h = residual + delta (32 bits; kept as the next residual),  v = h / sqrt(mean(h^2) + eps) * weight, rounded to the rows' type,  codes and scales of v
+// A block takes a row.  The sums run in tib_add_rmsnorm's order and the codes are made of what it writes, so that codes, scales and residual are bit for
+// bit those of the three steps one by one.
+#include "microscaled.cuh"
+
+namespace tib {
+
+struct QnArgs {
+  const void* delta;           // [rows, hidden] in the rows' type, or null
+  const float* residual;
+  float* sum;                  // where h goes: null where it is not kept
+  const int* rows;             // or null: every row
+  const float* weight;
+  void* out;                   // the normed rows [n_out, hidden], or null
+  unsigned char* codes;        // 4 bits: [n_out, steps * 128]; 8 bits: [n_out, runs * 128]
+  unsigned char* scales;       // of 4 bits
+  float* factors;              // 4 bits: [n_out]; 8 bits: the scales [runs, lds]
+  int64_t lds;
+  int hidden;
+  float eps;
+};
+
+// Eight numbers to eight 8-bit codes
+__device__ __forceinline__ uint2 qn_bytes8(const float (&v)[8], float inverse) {
+  return make_uint2(bs_codes4(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse),
+                    bs_codes4(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse));
+}
+template <typename T> __device__ __forceinline__ uint32_t qn_largest8(const float (&v)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  return m;
+}
+
+// What a thread does with eight numbers of a row (columns 8 g .. of it, zeros behind the last); all threads of a warp call it together.  largest: of the row
+// (4 bits).  Two threads have a run of 16, sixteen one of 128.
+template <typename T, bool BYTES>
+__device__ __forceinline__ void qn_codes8(const QnArgs& a, int row, int g, const float (&v)[8], float r, float inverse, int steps) {
+  uint32_t m = qn_largest8<T>(v);
+  if constexpr (BYTES) {
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const int runs = (a.hidden + kBlk - 1) / kBlk;
+    float s, back;
+    bs_run_scale(m, s, back);
+    if (g < runs * 16) *reinterpret_cast<uint2*>(a.codes + (size_t)row * runs * kBlk + g * 8) = qn_bytes8(v, back);
+    if (g < runs * 16 && (g & 15) == 0) a.factors[(size_t)(g >> 4) * a.lds + row] = s;
+  } else {
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    const uint32_t scale = inverse == 0.f ? 0u : ms_run_scale<T>(__uint_as_float(m) * inverse);
+    const uint32_t c = scale == 0 ? 0u : ms_codes8<T>(v, inverse, ms_reciprocal(ms_scale_value(scale)));
+    uint32_t four = scale << (8 * ((g >> 1) & 3));
+    four |= __shfl_xor_sync(0xffffffffu, four, 2);
+    four |= __shfl_xor_sync(0xffffffffu, four, 4);
+    if (g >= steps * (kMsStep / 8)) return;
+    *reinterpret_cast<uint32_t*>(a.codes + (size_t)row * steps * kMsStepBytes + g * 4) = c;
+    if ((g & 7) == 0)
+      *reinterpret_cast<uint32_t*>(a.scales + ((size_t)(row >> 7) * steps * 4 + (g >> 3)) * kMsChunkBytes + ms_scale_at(row & 127)) = four;
+    if (g == 0) a.factors[row] = r;
+  }
+}
+
+__device__ __forceinline__ uint32_t qn_block_max(uint32_t v, uint32_t* scratch) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  return __reduce_max_sync(0xffffffffu, lane < (int)(blockDim.x >> 5) ? scratch[lane] : 0u);
+}
+
+// bf16 rows whose width is a multiple of 8 and at most 8 * 1024: a thread keeps its eight numbers (as add_rmsnorm_bf16x8_kernel does), so the row is
+// read once.  The block's threads, a multiple of 32, cover whole steps of 256 columns.
+template <bool BYTES>
+__global__ void __launch_bounds__(1024)
+quantized_norm_bf16x8_kernel(const QnArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ float scratch[33];
+  __shared__ uint32_t scratch_max[32];
+  const int orow = blockIdx.x, srow = a.rows ? a.rows[orow] : orow, c = threadIdx.x * 8;
+  const bool active = c < a.hidden;
+  float h[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  float ss = 0.f;
+  if (active) {
+    const size_t at = (size_t)srow * a.hidden + c;
+    const float4 r0 = *reinterpret_cast<const float4*>(a.residual + at), r1 = *reinterpret_cast<const float4*>(a.residual + at + 4);
+    h[0] = r0.x; h[1] = r0.y; h[2] = r0.z; h[3] = r0.w; h[4] = r1.x; h[5] = r1.y; h[6] = r1.z; h[7] = r1.w;
+    if (a.delta) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.delta) + at);
+      const __nv_bfloat162* d2 = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = bf16x2_floats(d2[i]);
+        h[2 * i] += f.x;
+        h[2 * i + 1] += f.y;
+      }
+    }
+    if (a.sum) {
+      *reinterpret_cast<float4*>(a.sum + at) = make_float4(h[0], h[1], h[2], h[3]);
+      *reinterpret_cast<float4*>(a.sum + at + 4) = make_float4(h[4], h[5], h[6], h[7]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss += h[i] * h[i];
+  }
+  const float total = block_sum(ss, scratch);
+  const float inv = rsqrtf(total / (float)a.hidden + a.eps);
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (active) {
+    const float4 w0 = *reinterpret_cast<const float4*>(a.weight + c), w1 = *reinterpret_cast<const float4*>(a.weight + c + 4);
+    const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+    uint4 packed;
+    __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&packed);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o2[i] = __floats2bfloat162_rn(h[2 * i] * inv * w[2 * i], h[2 * i + 1] * inv * w[2 * i + 1]);
+      const float2 f = bf16x2_floats(o2[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+    if (a.out) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)orow * a.hidden + c) = packed;
+  }
+  float r = 1.f, inverse = 1.f;
+  if constexpr (!BYTES) ms_row_scale(qn_block_max(qn_largest8<__nv_bfloat16>(v), scratch_max), r, inverse);
+  qn_codes8<__nv_bfloat16, BYTES>(a, orow, threadIdx.x, v, r, inverse, (a.hidden + kMsStep - 1) / kMsStep);
+}
+
+// Any width, either type: the sums in add_rmsnorm_kernel's order (columns in turn), the codes eight columns a thread.
+template <typename T, bool BYTES>
+__global__ void quantized_norm_kernel(const QnArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ float scratch[33];
+  __shared__ uint32_t scratch_max[32];
+  const int orow = blockIdx.x, srow = a.rows ? a.rows[orow] : orow;
+  const float* res = a.residual + (size_t)srow * a.hidden;
+  const T* delta = a.delta ? static_cast<const T*>(a.delta) + (size_t)srow * a.hidden : nullptr;
+  // (h is added up anew where it is needed: residual and sum may be the same memory, where each thread reads and writes the columns of its own)
+  float* sum = a.sum ? a.sum + (size_t)srow * a.hidden : nullptr;
+  const bool kept = sum != nullptr;
+  float ss = 0.f;
+  for (int c = threadIdx.x; c < a.hidden; c += blockDim.x) {
+    float h = res[c];
+    if (delta) h += to_f32(delta[c]);
+    if (kept) sum[c] = h;
+    ss += h * h;
+  }
+  const float total = block_sum(ss, scratch);      // (its barriers make the block's sums readable to all of it)
+  const float inv = rsqrtf(total / (float)a.hidden + a.eps);
+  auto normed = [&](int c) {
+    if (c >= a.hidden) return 0.f;
+    float h = kept ? sum[c] : res[c];
+    if (!kept && delta) h += to_f32(delta[c]);
+    return to_f32(from_f32<T>(h * inv * a.weight[c]));
+  };
+  uint32_t largest = 0;
+  T* out = a.out ? static_cast<T*>(a.out) + (size_t)orow * a.hidden : nullptr;
+  if (!BYTES || out)
+    for (int c = threadIdx.x; c < a.hidden; c += blockDim.x) {
+      const float v = normed(c);
+      largest = max(largest, __float_as_uint(v) & 0x7fffffffu);
+      if (out) out[c] = from_f32<T>(v);
+    }
+  float r = 1.f, inverse = 1.f;
+  if constexpr (!BYTES) ms_row_scale(qn_block_max(largest, scratch_max), r, inverse);
+  const int steps = (a.hidden + kMsStep - 1) / kMsStep, eights = steps * (kMsStep / 8);
+  for (int g = threadIdx.x; g < eights; g += blockDim.x) {      // (whole warps: both are multiples of 32)
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = normed(g * 8 + i);
+    qn_codes8<T, BYTES>(a, orow, g, v, r, inverse, steps);
+  }
+}
+
+}  // namespace tib
+
+using namespace tib;
+
+// residual [rows, hidden] fp32, delta [rows, hidden] in dtype or null; sum [rows, hidden] fp32 takes residual + delta (it may be residual itself; null: it is not kept, and
+// with `rows`, indices of the n_out rows to norm, it has to be null).  bytes 0: codes, scales, factors as tib_microscaled_rows leaves them, 1: codes
+// [n_out, runs * 128] and factors = scales [runs, lds] as tib_quantize_rows does.  out: the normed rows in dtype, or null.
+TIB_API int tib_quantized_norm(const void* delta, const float* residual, float* sum, const int* rows, const float* weight, void* out, int bytes, void* codes,
+                               void* scales, float* factors, int64_t lds, int n_out, int hidden, float eps, int dtype, cudaStream_t stream) {
+  if (n_out == 0) return TIB_OK;
+  if (!residual || !weight || !codes || !factors || (!bytes && !scales) || n_out < 0 || hidden < 1 || (rows && sum)) return TIB_E_ARG;
+  if (dtype != TIB_BF16 && dtype != TIB_F32) return TIB_E_DTYPE;
+  if (bytes && lds < n_out) return TIB_E_SIZE;
+  if (((uintptr_t)codes | (uintptr_t)scales) & 15) return TIB_E_ALIGN;
+  const QnArgs a{delta, residual, sum, rows, weight, out, (unsigned char*)codes, (unsigned char*)scales, factors, lds, hidden, eps};
+  if (dtype == TIB_BF16 && hidden % 8 == 0 && hidden <= 8192 &&
+      (((uintptr_t)residual | (uintptr_t)sum | (uintptr_t)weight | (uintptr_t)out | (uintptr_t)delta) & 15) == 0) {
+    const int threads = (hidden / 8 + 31) / 32 * 32;
+    if (bytes) TIB_LAUNCH_DEPENDENT(quantized_norm_bf16x8_kernel<true>, n_out, threads, 0, stream, a);
+    else TIB_LAUNCH_DEPENDENT(quantized_norm_bf16x8_kernel<false>, n_out, threads, 0, stream, a);
+    return TIB_OK;
+  }
+  const int threads = norm_threads(hidden);
+#define TIB_QN_GO(T, BYTES) TIB_LAUNCH_DEPENDENT((quantized_norm_kernel<T, BYTES>), n_out, threads, 0, stream, a)
+  if (dtype == TIB_BF16) {
+    if (bytes) TIB_QN_GO(__nv_bfloat16, true);
+    else TIB_QN_GO(__nv_bfloat16, false);
+  } else {
+    if (bytes) TIB_QN_GO(float, true);
+    else TIB_QN_GO(float, false);
+  }
+#undef TIB_QN_GO
+  return TIB_OK;
+}
+
+TIB_PACKED(tib_quantized_norm)

@@ -88,24 +88,9 @@ def quantize_matrix(matrix: torch.Tensor) -> BlockScaledMatrix:
     return BlockScaledMatrix(codes.to(CODE_DTYPE).contiguous(), scales.contiguous())
 
 
-def _checked_rows(x: torch.Tensor, columns: int | None, device: int | None, what: str) -> int:
-    """The number of rows of ``x``, which must be [rows, ``columns``] with unit inner stride on the current device (and on ``device``)."""
-    shape = x.shape
-    if len(shape) != 2 or shape[1] == 0 or (columns is not None and shape[1] != columns):
-        raise ops.KernelError(f"{what}: rows of {columns or 'one number or more'} are wanted, not {tuple(shape)}")
-    here = x.get_device()
-    if here < 0:
-        raise ops.KernelError(f"{what}: operands must be CUDA tensors (there is no CPU path)")
-    if (device is not None and here != device) or here != torch._C._cuda_getDevice():
-        raise ops.KernelError(f"{what}: the rows are on cuda:{here}, the weight on cuda:{device}, the current device is cuda:{torch._C._cuda_getDevice()}")
-    if x.stride(1) != 1 and shape[1] > 1:
-        raise ops.KernelError(f"{what}: rows need unit inner stride, not {x.stride()}")
-    return shape[0]
-
-
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(codes [M, K], scales [M, runs of 128]) of the rows ``x`` [M, K] (bfloat16 or float32, any row stride); see the module's text."""
-    rows = _checked_rows(x, None, None, "quantize_rows")
+    rows = ops.need_rows(x, None, None, "quantize_rows")
     columns = x.shape[1]
     runs, lds = blocks(columns), (rows + 3) & ~3
     codes = x.new_empty((rows, runs * BLOCK), dtype=CODE_DTYPE)
@@ -118,6 +103,50 @@ def _code_buffer(x: torch.Tensor, rows: int, columns: int) -> torch.Tensor:
     """Room for the codes and scales of ``rows`` rows (see :func:`ops.block_scaled_product`)."""
     runs = -(-columns // BLOCK)
     return x.new_empty(runs * (rows * BLOCK + 4 * ((rows + 3) & ~3)), dtype=torch.uint8)
+
+
+class BlockScaledRows:
+    """Quantised rows [rows, columns] as the products read them, from :func:`add_rmsnorm`.  ``dtype``: the type that the rows were rounded to before."""
+    __slots__ = ("buffer", "shape", "dtype", "codes_at", "scales_at", "lds")
+
+    def __init__(self, like: torch.Tensor, rows: int, columns: int, dtype: torch.dtype) -> None:
+        self.buffer = _code_buffer(like, rows, columns)
+        self.shape, self.dtype, self.lds, self.codes_at = torch.Size((rows, columns)), dtype, (rows + 3) & ~3, self.buffer.data_ptr()
+        self.scales_at = self.codes_at + blocks(columns) * BLOCK * rows
+
+    @property
+    def device(self) -> torch.device:
+        return self.buffer.device
+
+    def get_device(self) -> int:
+        return self.buffer.get_device()
+
+    def __len__(self) -> int:
+        return self.shape[0]
+
+    def parts(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """(codes [rows, columns], scales [rows, runs of 128]), as :func:`quantize_rows` returns them (views)."""
+        rows, runs = len(self), blocks(self.shape[1])
+        codes, scales = self.buffer[:rows * runs * BLOCK], self.buffer[rows * runs * BLOCK:]
+        return codes.view(CODE_DTYPE).view(rows, runs * BLOCK)[:, :self.shape[1]], scales.view(torch.float32).view(runs, self.lds).t()[:rows]
+
+    def widened(self, dtype: torch.dtype | None = None) -> torch.Tensor:
+        """The numbers the rows stand for, in ``dtype`` (bfloat16 or float32; left out: the rows' own)."""
+        out = self.buffer.new_empty(self.shape, dtype=self.dtype if dtype is None else dtype)
+        ops.widen_rows(self.codes_at, self.scales_at, self.lds, out)
+        return out
+
+
+def add_rmsnorm(delta: torch.Tensor | None, residual: torch.Tensor, weight: torch.Tensor, eps: float, *, dtype: torch.dtype | None = None,
+                rows: torch.Tensor | None = None, out: torch.Tensor | None = None, new_residual: torch.Tensor | None = None) -> BlockScaledRows:
+    """:func:`ops.add_rmsnorm` whose rows leave in 8 bits, bit for bit those that :func:`quantize_rows` makes of its output.
+
+    ``dtype``: the type that the normed rows are rounded to before they are quantised (delta's; without a delta bfloat16).  ``rows``: indices of the rows to norm; the
+    residual is then left as it is.  ``out``: takes the normed rows too, in ``dtype``.  ``new_residual``: takes residual + delta in place of ``residual``."""
+    dtype, count = ops.quantized_norm_type(delta, dtype), residual.shape[0] if rows is None else rows.numel()
+    made = BlockScaledRows(residual, count, residual.shape[-1], dtype)
+    ops.quantized_norm(delta, residual, weight, eps, dtype, rows, out, new_residual, True, count, made.codes_at, 0, made.scales_at, made.lds)
+    return made
 
 
 def _normal_range(scales: torch.Tensor) -> tuple[float, float]:
@@ -233,32 +262,38 @@ class BlockScaledWeight:
                                                           (part.far_low, part.far_high))))
         return view
 
-    def _run(self, x: torch.Tensor, act: str, width: int, out_dtype: torch.dtype | None, out: torch.Tensor | None, error_word: torch.Tensor | None) -> torch.Tensor:
-        rows = _checked_rows(x, self.in_features, self.parts[0][1].device_index, "linear")
-        dtype = x.dtype if out_dtype is None else out_dtype
+    def _run(self, x: "torch.Tensor | BlockScaledRows", act: str, width: int, out_dtype: torch.dtype | None, out: torch.Tensor | None,
+             error_word: torch.Tensor | None) -> torch.Tensor:
+        ready = isinstance(x, BlockScaledRows)
+        if not ready and not isinstance(x, torch.Tensor):
+            raise ops.KernelError(f"linear: an 8-bit weight takes a tensor or BlockScaledRows, not {type(x).__name__}")
+        rows = ops.need_rows(x, self.in_features, self.parts[0][1].device_index, "linear")
+        like, dtype = x.buffer if ready else x, x.dtype if out_dtype is None else out_dtype
         if out is None or out.dtype != dtype:
             if dtype not in _OUT_DTYPES:
                 raise ops.KernelError(f"linear: unsupported output dtype {dtype}")
-            out = x.new_empty((rows, width)) if dtype == x.dtype else x.new_empty((rows, width), dtype=dtype)
+            out = like.new_empty((rows, width)) if dtype == like.dtype else like.new_empty((rows, width), dtype=dtype)
         elif out.shape != (rows, width) or (out.stride(1) != 1 and width > 1) or out.get_device() != x.get_device():
             raise ops.KernelError(f"linear: out is {tuple(out.shape)} on {out.device}, wanted {(rows, width)} with unit inner stride on {x.device}")
         if rows == 0:
             return out
-        held = None if rows <= FEW_ROWS else _code_buffer(x, rows, self.in_features)
-        codes = 0 if held is None else held.data_ptr()
+        # (codes that are there already: no kernel quantises them, at few rows neither)
+        held = None if ready or rows <= FEW_ROWS else _code_buffer(x, rows, self.in_features)
+        codes = x.codes_at if ready else 0 if held is None else held.data_ptr()
+        source = None if ready else x
         if len(self.parts) == 1:
-            ops.block_scaled_product(x, codes, True, self.parts[0][1], out, act, 0.0, 0.0, 0, 0, 1, False, None, error_word)
+            ops.block_scaled_product(source, codes, not ready, self.parts[0][1], out, act, 0.0, 0.0, 0, 0, 1, False, None, error_word)
         else:
             for i, (first, part) in enumerate(self.parts):
-                ops.block_scaled_product(x, codes, i == 0, part, out[:, first:first + part.features], act, 0.0, 0.0, 0, 0, 1, False, None, error_word)
+                ops.block_scaled_product(source, codes, not ready and i == 0, part, out[:, first:first + part.features], act, 0.0, 0.0, 0, 0, 1, False, None, error_word)
         return out
 
-    def product(self, x: torch.Tensor, *, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
+    def product(self, x: "torch.Tensor | BlockScaledRows", *, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
                 error_word: torch.Tensor | None = None) -> torch.Tensor:
         """x [tokens, in] times the weight: [tokens, out] (a swiglu weight's gate and up sums side by side)."""
         return self._run(x, "none", self.out_features, out_dtype, out, error_word)
 
-    def swiglu(self, x: torch.Tensor, *, out_dtype: torch.dtype | None = None, error_word: torch.Tensor | None = None) -> torch.Tensor:
+    def swiglu(self, x: "torch.Tensor | BlockScaledRows", *, out_dtype: torch.dtype | None = None, error_word: torch.Tensor | None = None) -> torch.Tensor:
         """silu(gate) * up of the 32-bit sums: [tokens, out / 2]."""
         if self.epilogue != "swiglu":
             raise ops.KernelError("linear_swiglu: the weight was not bound with epilogue='swiglu'")
@@ -291,23 +326,10 @@ class BlockScaledExperts:
                 act: str = "none", limit: float = 0.0, alpha: float = 1.0, row_scale: torch.Tensor | None = None,
                 error_word: torch.Tensor | None = None) -> torch.Tensor:
         """See :func:`ops.moe_expert_product`."""
-        if act not in ops.MOE_ACT:
-            raise ops.KernelError(f"moe_expert_product: unknown activation {act!r}")
-        gated = act in ops.MOE_GATED
-        if gated != self.paired and act != "none":
-            raise ops.KernelError(f"moe_expert_product: activation {act!r} does not fit experts with{'' if self.paired else 'out'} gate and up rows")
-        pairs, width = order.numel(), self.out_features // 2 if gated else self.out_features
-        here = self.blocks.device_index
-        rows = _checked_rows(x, self.in_features, here, "moe_expert_product")
-        if y.shape != (pairs, width) or offsets.numel() != self.experts + 1 or top < 1 or (pairs % top or rows < pairs // top if x_by_pair else rows < pairs):
-            raise ops.KernelError("moe_expert_product: shapes do not fit")
-        for name, t, dtype in (("offsets", offsets, torch.int32), ("order", order, torch.int32), ("row_scale", row_scale, torch.float32)):
-            if t is not None and (t.dtype != dtype or t.get_device() != here or not t.is_contiguous()):
-                raise ops.KernelError(f"moe_expert_product: {name} must be contiguous {dtype} on cuda:{here}, not {t.dtype} on {t.device}")
-        if y.get_device() != here or (y.stride(1) != 1 and width > 1):
-            raise ops.KernelError(f"moe_expert_product: y must be rows with unit inner stride on cuda:{here}")
-        if row_scale is not None and row_scale.numel() != pairs:
-            raise ops.KernelError("moe_expert_product: row_scale must hold one factor per pair")
+        if not isinstance(x, torch.Tensor):
+            raise ops.KernelError("moe_expert_product: rows by expert are quantised as they are sorted; they come as a tensor")
+        pairs = ops.need_expert_product(x, y, offsets, order, top, x_by_pair, act, row_scale, self.experts, self.in_features, self.out_features, self.paired,
+                                        self.blocks.device_index)
         if pairs == 0:
             return y
         held = None if pairs <= FEW_EXPERT_ROWS * self.experts else _code_buffer(x, pairs, self.in_features)

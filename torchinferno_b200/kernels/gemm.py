@@ -14,7 +14,14 @@ import weakref
 import torch
 
 from torchinferno_b200.kernels import ops
-from torchinferno_b200.kernels.block_scaled import BlockScaledExperts, BlockScaledMatrix, BlockScaledWeight
+from torchinferno_b200.kernels.block_scaled import BlockScaledExperts, BlockScaledMatrix, BlockScaledRows, BlockScaledWeight
+from torchinferno_b200.kernels.microscaled import MicroscaledExperts, MicroscaledMatrix, MicroscaledRows, MicroscaledWeight
+
+# How a matrix is stored: a tensor, 8-bit blocks or 4-bit codes; and what of it the products take.
+Matrix = torch.Tensor | BlockScaledMatrix | MicroscaledMatrix
+QuantizedWeight = BlockScaledWeight | MicroscaledWeight
+_QUANTIZED = (BlockScaledWeight, MicroscaledWeight)
+Rows = torch.Tensor | BlockScaledRows | MicroscaledRows
 
 # Which kernel multiplies bf16 operands:
 #   "auto"     whichever is faster on this GPU.  Many rows go to cuBLAS.  At few rows (decode steps) neither the
@@ -131,19 +138,25 @@ class LinearWeight:
         return self.tensor.numel() * self.tensor.element_size()
 
 
-def _block_scaled(matrices: "tuple[torch.Tensor | BlockScaledMatrix, ...]") -> bool:
-    """Whether matrices that make one product are 8-bit blocks: all of them or none."""
-    kinds = {isinstance(m, BlockScaledMatrix) for m in matrices}
+def _stored(matrices: "tuple[Matrix, ...]") -> type | None:
+    """The type that matrices which make one product are stored in: BlockScaledMatrix (8-bit blocks), MicroscaledMatrix (4-bit codes) or None (tensors), all alike."""
+    kinds = {BlockScaledMatrix if isinstance(m, BlockScaledMatrix) else MicroscaledMatrix if isinstance(m, MicroscaledMatrix) else None for m in matrices}
     if len(kinds) != 1:
-        raise ValueError("matrices that run as one product must all be stored in 8-bit blocks, or none of them")
+        raise ValueError("matrices that run as one product must all be stored in 8-bit blocks, or none of them" if MicroscaledMatrix not in kinds else
+                         "matrices that run as one product must all be stored in 4-bit codes, or none of them")
     return kinds.pop()
 
 
-def projection(*matrices: "torch.Tensor | BlockScaledMatrix") -> "LinearWeight | BlockScaledWeight":
+_WEIGHTS = {BlockScaledMatrix: BlockScaledWeight, MicroscaledMatrix: MicroscaledWeight}
+_EXPERTS = {BlockScaledMatrix: BlockScaledExperts, MicroscaledMatrix: MicroscaledExperts}
+
+
+def projection(*matrices: Matrix) -> "LinearWeight | QuantizedWeight":
     """The weight of a part's projection from its checkpoint matrices [out, in], whose outputs lie side by side.  (Which kernel takes the products of few
     rows is measured per shape once the whole model is bound.)"""
-    if _block_scaled(matrices):
-        return BlockScaledWeight(*matrices)
+    kind = _stored(matrices)
+    if kind is not None:
+        return _WEIGHTS[kind](*matrices)
     return LinearWeight(matrices[0] if len(matrices) == 1 else torch.cat(matrices, dim=0), few_rows_tcgen05=None)
 
 
@@ -152,26 +165,31 @@ def row_pairs(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     return torch.stack([gate, up], dim=1).reshape(2 * gate.shape[0], gate.shape[1])
 
 
-def gated_projection(gate: "torch.Tensor | BlockScaledMatrix", up: "torch.Tensor | BlockScaledMatrix", *, epilogue: str = "swiglu") -> "LinearWeight | BlockScaledWeight":
+def gated_projection(gate: Matrix, up: Matrix, *, epilogue: str = "swiglu") -> "LinearWeight | QuantizedWeight":
     """The same of a gate and an up matrix, as (gate i, up i) row pairs.  ``epilogue="none"``: the pairs' activation is the caller's."""
-    if _block_scaled((gate, up)):
-        return BlockScaledWeight(gate, up, epilogue="swiglu")
+    kind = _stored((gate, up))
+    if kind is not None:
+        return _WEIGHTS[kind](gate, up, epilogue="swiglu")
     return LinearWeight(row_pairs(gate, up), few_rows_tcgen05=None, epilogue=epilogue)
 
 
-def expert_matrices(matrices: "list[torch.Tensor | BlockScaledMatrix]", ups: "list[torch.Tensor | BlockScaledMatrix] | None" = None) -> "torch.Tensor | BlockScaledExperts":
+def expert_matrices(matrices: "list[Matrix]", ups: "list[Matrix] | None" = None) -> "torch.Tensor | BlockScaledExperts | MicroscaledExperts":
     """One product's matrices of all experts (of gated ones: ``matrices`` the gates), as :func:`ops.moe_expert_product` takes them."""
-    if _block_scaled((*matrices, *(ups or ()))):
-        return BlockScaledExperts(matrices, ups)
+    kind = _stored((*matrices, *(ups or ())))
+    if kind is not None:
+        return _EXPERTS[kind](matrices, ups)
     return torch.stack(matrices if ups is None else [row_pairs(g, u) for g, u in zip(matrices, ups)]).contiguous()
 
 
-def linear(x: torch.Tensor, weight: "torch.Tensor | LinearWeight | BlockScaledWeight", *, out_dtype: torch.dtype | None = None,
+def linear(x: Rows, weight: "torch.Tensor | LinearWeight | QuantizedWeight", *, out_dtype: torch.dtype | None = None,
            out: torch.Tensor | None = None) -> torch.Tensor:
     """``x``: [tokens, in]; ``weight``: [out, in] (or a :class:`LinearWeight`, or a
-    :class:`~torchinferno_b200.kernels.block_scaled.BlockScaledWeight`); returns [tokens, out] in ``out_dtype``."""
-    if isinstance(weight, BlockScaledWeight):
+    :class:`~torchinferno_b200.kernels.block_scaled.BlockScaledWeight` or :class:`~torchinferno_b200.kernels.microscaled.MicroscaledWeight`, which also
+    take the rows that a norm has quantised); returns [tokens, out] in ``out_dtype``."""
+    if isinstance(weight, _QUANTIZED):
         return weight.product(x, out_dtype=out_dtype, out=out, error_word=_error_word)
+    if not isinstance(x, torch.Tensor):
+        raise ops.KernelError("linear: quantised rows are for quantised weights")
     few_rows = 0
     if isinstance(weight, LinearWeight):
         if weight.transposed:
@@ -197,12 +215,14 @@ def linear(x: torch.Tensor, weight: "torch.Tensor | LinearWeight | BlockScaledWe
     return _linear_bf16(x, weight, out_dtype, out, few_rows)
 
 
-def linear_swiglu(x: torch.Tensor, weight: "LinearWeight | BlockScaledWeight", *, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+def linear_swiglu(x: Rows, weight: "LinearWeight | QuantizedWeight", *, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """silu(gate) * up of the product with a weight whose rows are (gate i, up i) pairs: [tokens, out / 2].
     At few rows the few-rows kernel applies it in its epilogue; else the product is followed by the SwiGLU kernel.
-    A block-scaled weight activates its 32-bit sums at any number of rows, and may leave another type than x's."""
-    if isinstance(weight, BlockScaledWeight):
+    A quantised weight activates its 32-bit sums at any number of rows, and may leave another type than x's."""
+    if isinstance(weight, _QUANTIZED):
         return weight.swiglu(x, out_dtype=out_dtype, error_word=_error_word)
+    if not isinstance(x, torch.Tensor):
+        raise ops.KernelError("linear_swiglu: quantised rows are for quantised weights")
     if out_dtype not in (None, x.dtype):
         raise ops.KernelError("linear_swiglu: another output type than x's is for block-scaled weights")
     if weight.epilogue != "swiglu":

@@ -1,0 +1,316 @@
+"""4-bit microscaled weights and rows: e2m1 codes with an e4m3 scale for each run of 16 columns, and the products of such rows with such weights.
+
+A code is one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 with a sign.  A matrix [N, K] has one fp32 factor f beside its scales S: number (n, k) stands for
+code(n, k) * S[n, k // 16] * f.  The rows x [M, K] of a product are quantised on the way, or come as :class:`MicroscaledRows` from
+:func:`quantize_rows` or from a norm that leaves them so (:func:`add_rmsnorm`).  With a the largest absolute value of a row, and a_b that of a run b:
+
+    r = 2^p, p the smallest integer (at least -126) with a * 2^-p <= 2688 = 6 * 448 (1 where a is 0)
+    s = a_b / (6 r) rounded to e4m3        codes = x / (s r) rounded to e2m1, at most 6 (0 where s is 0)
+    y[m, n] = r[m] f sum over b of s[m, b] S[n, b] (sum over run b of code_x[m, k] code_w[n, k])
+
+All rounding is to nearest, ties to even, of the exact quotient: codes are the same on any machine.  Sums have 32 bits, y is rounded once.  A row
+that holds an infinity or a NaN makes its whole output row NaN.  A row's codes are its own: they do not depend on the rows beside it.
+
+There is no backward pass: this is an inference engine's weight format.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Sequence
+
+import torch
+
+from torchinferno_b200.kernels import ops
+
+RUN = 16                # columns of a scale
+STEP = 256              # columns are padded to whole steps
+TILE = 128              # rows of a tile of scales
+SCALE_DTYPE = torch.float8_e4m3fn
+VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+BORDERS = (0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)       # (on a border the even code is taken: the one above 0.75, 1.75 and 3.5)
+LARGEST = 6.0 * 448.0
+_OUT_DTYPES = (torch.bfloat16, torch.float32)
+
+
+def _count(columns: int, each: int) -> int:
+    return -(-columns // each)
+
+
+@dataclass(frozen=True)
+class MicroscaledMatrix:
+    """A matrix as a checkpoint stores it: ``codes`` [N, ceil(K / 2)] (uint8, two codes a byte, the even column in the lower half), ``scales``
+    [N, ceil(K / 16)] in e4m3 (none negative) and ``factor``, one fp32 number.  ``columns``: K where it is odd (else twice the bytes)."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    factor: torch.Tensor
+    columns: int | None = None
+
+    def __post_init__(self) -> None:
+        if self.codes.dtype != torch.uint8 or self.codes.dim() != 2 or 0 in self.codes.shape:
+            raise ValueError(f"codes must be a non-empty 2-D tensor of uint8, got {self.codes.dtype} {tuple(self.codes.shape)}")
+        if self.columns is None:
+            object.__setattr__(self, "columns", 2 * self.codes.shape[1])
+        if _count(self.columns, 2) != self.codes.shape[1]:
+            raise ValueError(f"{self.columns} columns do not have {self.codes.shape[1]} bytes of codes")
+        wanted = (self.codes.shape[0], _count(self.columns, RUN))
+        if self.scales.dtype != SCALE_DTYPE or tuple(self.scales.shape) != wanted:
+            raise ValueError(f"scales of a {tuple(self.shape)} matrix must be {SCALE_DTYPE} {wanted}, got {self.scales.dtype} {tuple(self.scales.shape)}")
+        if self.factor.dtype != torch.float32 or self.factor.numel() != 1:
+            raise ValueError(f"the factor must be one float32 number, got {self.factor.dtype} {tuple(self.factor.shape)}")
+        if len({self.codes.device, self.scales.device, self.factor.device}) != 1:
+            raise ValueError(f"codes are on {self.codes.device}, scales on {self.scales.device}, the factor on {self.factor.device}")
+
+    @property
+    def shape(self) -> torch.Size:
+        return torch.Size((self.codes.shape[0], self.columns))
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def to(self, device: torch.device | str) -> "MicroscaledMatrix":
+        return MicroscaledMatrix(self.codes.to(device), self.scales.to(device), self.factor.to(device), self.columns)
+
+    def widened(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The numbers the matrix stands for (on any device)."""
+        n, k = self.shape
+        signed = torch.tensor(VALUES + tuple(-v for v in VALUES), dtype=torch.float32, device=self.device)
+        halves = torch.stack([self.codes & 15, self.codes >> 4], dim=2).view(n, -1)[:, :k]
+        scales = self.scales.to(torch.float32).repeat_interleave(RUN, 1)[:, :k]
+        return (signed[halves.long()] * scales * self.factor.reshape(())).to(dtype)
+
+
+def quantize_matrix(matrix: torch.Tensor) -> MicroscaledMatrix:
+    """The 4-bit form of ``matrix`` [N, K]: f = (its largest absolute value) / 2688, S = e4m3(a run's largest / (6 f)), codes the nearest ones."""
+    if matrix.dim() != 2 or 0 in matrix.shape:
+        raise ValueError(f"quantize_matrix takes a non-empty matrix, got {tuple(matrix.shape)}")
+    n, k = matrix.shape
+    runs = torch.nn.functional.pad(matrix.to(torch.float32), (0, -k % RUN)).view(n, -1, RUN)
+    factor = (runs.abs().amax() / LARGEST).clamp(min=torch.finfo(torch.float32).tiny)
+    scales = (runs.abs().amax(2) / 6.0 / factor).clamp(max=448.0).to(SCALE_DTYPE)
+    wide = scales.to(torch.float32)[..., None]
+    v = torch.where(wide == 0, 0.0, runs / torch.where(wide == 0, 1.0, wide) / factor).view(n, -1)
+    size = v.abs()
+    codes = torch.zeros_like(v, dtype=torch.uint8)
+    for i, border in enumerate(BORDERS):
+        codes += size >= border if i % 2 else size > border
+    codes += 8 * ((v < 0) & (codes > 0)).to(torch.uint8)
+    return MicroscaledMatrix((codes[:, 0::2] | (codes[:, 1::2] << 4))[:, :_count(k, 2)].contiguous(), scales.contiguous(), factor, k)
+
+
+# ------------------------------------------------------------------------------------------------ rows
+def _buffer(like: torch.Tensor, rows: int, columns: int, experts: int = 0) -> tuple[torch.Tensor, int, int]:
+    """(room for the codes, scales and factors of so many rows, where in it the scales begin, where the factors); see csrc/microscaled.cuh."""
+    steps = _count(columns, STEP)
+    codes, scales = rows * steps * (STEP // 2), (_count(rows, TILE) + experts) * steps * (TILE * STEP // RUN)
+    return like.new_empty(codes + scales + 4 * rows, dtype=torch.uint8), codes, codes + scales
+
+
+class MicroscaledRows:
+    """Quantised rows [rows, columns], as the kernels read them.  ``dtype``: the type of what they were made from."""
+    __slots__ = ("buffer", "shape", "dtype", "codes_at", "scales_at", "factors_at")
+
+    def __init__(self, like: torch.Tensor, rows: int, columns: int, dtype: torch.dtype) -> None:
+        self.buffer, scales, factors = _buffer(like, rows, columns)
+        self.shape, self.dtype, self.codes_at = torch.Size((rows, columns)), dtype, self.buffer.data_ptr()
+        self.scales_at, self.factors_at = self.codes_at + scales, self.codes_at + factors
+
+    @property
+    def device(self) -> torch.device:
+        return self.buffer.device
+
+    def get_device(self) -> int:
+        return self.buffer.get_device()
+
+    def __len__(self) -> int:
+        return self.shape[0]
+
+    def widened(self, dtype: torch.dtype | None = None) -> torch.Tensor:
+        """The numbers the rows stand for, in ``dtype`` (bfloat16, which holds them all but where they underflow, or float32; left out: the rows' own)."""
+        dtype = self.dtype if dtype is None else dtype
+        out = self.buffer.new_empty(self.shape, dtype=dtype)
+        ops.microscaled_widen(self.codes_at, self.scales_at, self.factors_at, out)
+        return out
+
+
+def quantize_rows(x: torch.Tensor) -> MicroscaledRows:
+    """The rows ``x`` [M, K] (bfloat16 or float32, any row stride) in 4 bits; see the module's text."""
+    ops.need_rows(x, None, None, "quantize_rows")
+    rows = MicroscaledRows(x, *x.shape, x.dtype)
+    ops.microscaled_rows(x, rows.codes_at, rows.scales_at, rows.factors_at)
+    return rows
+
+
+def add_rmsnorm(delta: torch.Tensor | None, residual: torch.Tensor, weight: torch.Tensor, eps: float, *, dtype: torch.dtype | None = None,
+                rows: torch.Tensor | None = None, out: torch.Tensor | None = None, new_residual: torch.Tensor | None = None) -> MicroscaledRows:
+    """:func:`ops.add_rmsnorm` whose rows leave in 4 bits, bit for bit those that :func:`quantize_rows` makes of its output.
+
+    ``dtype``: the type that the normed rows are rounded to before they are quantised (delta's; without a delta bfloat16).  ``rows``: indices of the rows to norm; the
+    residual is then left as it is.  ``out``: takes the normed rows too, in ``dtype``.  ``new_residual``: takes residual + delta in place of ``residual``."""
+    dtype, count = ops.quantized_norm_type(delta, dtype), residual.shape[0] if rows is None else rows.numel()
+    made = MicroscaledRows(residual, count, residual.shape[-1], dtype)
+    ops.quantized_norm(delta, residual, weight, eps, dtype, rows, out, new_residual, False, count, made.codes_at, made.scales_at, made.factors_at, 0)
+    return made
+
+
+# ------------------------------------------------------------------------------------------------ weights
+class Tiles:
+    """Matrices of one size as the kernels read them: ``codes`` [matrices, tiles of 128 rows, steps of 256 columns, 128, 128 bytes], ``scales``
+    [matrices, tiles, steps, 2048 bytes] and ``factors`` [matrices, N]; ``paired``: the matrices' rows are (gate i, up i)."""
+    __slots__ = ("codes", "scales", "factors", "count", "features", "columns", "paired", "codes_at", "scales_at", "factors_at", "device_index")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, factors: torch.Tensor, columns: int, paired: bool) -> None:
+        self.codes, self.scales, self.factors, self.count, self.features, self.columns, self.paired = codes, scales, factors, codes.shape[0], factors.shape[1], columns, paired
+        self.codes_at, self.scales_at, self.factors_at, self.device_index = codes.data_ptr(), scales.data_ptr(), factors.data_ptr(), codes.get_device()
+
+
+def _laid_out(stacks: Sequence[Sequence[MicroscaledMatrix]], paired: bool) -> Tiles:
+    """A stack of matrices over the same columns for each expert (or one): a stack's rows lie one behind the other, or (``paired``) alternate."""
+    columns, device = stacks[0][0].columns, stacks[0][0].device
+    heights = [m.shape[0] for m in stacks[0]]
+    for stack in stacks:
+        if [m.shape[0] for m in stack] != heights or any(m.columns != columns or m.device != device for m in stack):
+            raise ValueError("matrices of one weight must be alike: " + ", ".join(f"{tuple(m.shape)} on {m.device}" for m in (*stacks[0], *stack)))
+    if paired and (len(heights) != 2 or heights[0] != heights[1]):
+        raise ValueError(f"a gate and an up matrix are needed, of one size, not {heights} rows")
+    features, steps = sum(heights), _count(columns, STEP)
+    tiles = _count(features, TILE)
+    codes = torch.zeros((len(stacks), tiles * TILE, steps * (STEP // 2)), dtype=torch.uint8, device=device)
+    scales = torch.zeros((len(stacks), tiles * TILE, steps * (STEP // RUN)), dtype=torch.uint8, device=device)
+    factors = torch.empty((len(stacks), features), dtype=torch.float32, device=device)
+    for i, stack in enumerate(stacks):
+        first = 0
+        for j, m in enumerate(stack):
+            at = slice(j, features, 2) if paired else slice(first, first + m.shape[0])
+            codes[i, at, :m.codes.shape[1]] = m.codes
+            scales[i, at, :m.scales.shape[1]] = m.scales.view(torch.uint8)
+            factors[i, at] = m.factor.reshape(())
+            first += m.shape[0]
+    if columns % 2:      # (the half byte behind the last column)
+        codes[:, :, columns // 2] &= 15
+    if int(scales.max()) > 0x7e:
+        raise ValueError("the scales of a 4-bit matrix must be numbers, and none of them negative")
+    codes = codes.view(len(stacks), tiles, TILE, steps, STEP // 2).transpose(2, 3).contiguous()
+    # (row 32 a + b of a tile, run 4 c + d of a step: to [c][b][a][d])
+    scales = scales.view(len(stacks), tiles, 4, 32, steps, 4, 4).permute(0, 1, 4, 5, 3, 2, 6).contiguous()
+    return Tiles(codes, scales.view(len(stacks), tiles, steps, -1), factors, columns, paired)
+
+
+def _product(x: "torch.Tensor | MicroscaledRows", tiles: Tiles, y: torch.Tensor, act: str, limit: float, alpha: float, offsets: int, order: int, top: int,
+             x_by_pair: bool, row_scale: torch.Tensor | None, error_word: torch.Tensor | None) -> None:
+    if isinstance(x, MicroscaledRows):
+        ops.microscaled_product(None, x.codes_at, x.scales_at, x.factors_at, tiles, y, act, limit, alpha, offsets, order, top, x_by_pair, row_scale, error_word)
+        return
+    held, scales, factors = _buffer(x, len(y), tiles.columns, tiles.count if offsets else 0)
+    at = held.data_ptr()
+    ops.microscaled_product(x, at, at + scales, at + factors, tiles, y, act, limit, alpha, offsets, order, top, x_by_pair, row_scale, error_word)
+
+
+def _output(x: "torch.Tensor | MicroscaledRows", out: torch.Tensor | None, width: int, dtype: torch.dtype) -> torch.Tensor:
+    if dtype not in _OUT_DTYPES:
+        raise ops.KernelError(f"linear: unsupported output dtype {dtype}")
+    if out is None or out.dtype != dtype:
+        return torch.empty((len(x), width), dtype=dtype, device=x.device)
+    if out.shape != (len(x), width) or (out.stride(1) != 1 and width > 1) or out.get_device() != x.get_device():
+        raise ops.KernelError(f"linear: out is {tuple(out.shape)} on {out.device}, wanted {(len(x), width)} with unit inner stride on {x.device}")
+    return out
+
+
+class MicroscaledWeight:
+    """A projection of 4-bit codes, laid out for the kernels.  ``MicroscaledWeight(matrix)``; several matrices over the same columns
+    (``MicroscaledWeight(q, k, v)``) give their outputs side by side; ``MicroscaledWeight(gate, up, epilogue="swiglu")`` is what
+    :func:`gemm.linear_swiglu` takes."""
+
+    def __init__(self, *matrices: MicroscaledMatrix, epilogue: str = "none") -> None:
+        if epilogue not in ("none", "swiglu"):
+            raise ValueError(f"unknown epilogue {epilogue!r}")
+        if not matrices or any(not isinstance(m, MicroscaledMatrix) for m in matrices):
+            raise ValueError("a microscaled weight is made of microscaled matrices")
+        if epilogue == "swiglu" and len(matrices) != 2:
+            raise ValueError("the swiglu epilogue takes a gate and an up matrix")
+        self.epilogue, self.in_features = epilogue, matrices[0].columns
+        self.tiles = _laid_out([matrices], epilogue == "swiglu")
+        self.out_features = self.tiles.features
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return torch.uint8
+
+    @property
+    def device(self) -> torch.device:
+        return self.tiles.codes.device
+
+    def address(self) -> int:
+        return self.tiles.codes_at
+
+    def nbytes(self) -> int:
+        return self.tiles.codes.numel() + self.tiles.scales.numel() + 4 * self.tiles.factors.numel()
+
+    def rows(self, start: int, stop: int) -> "MicroscaledWeight":
+        """The projection onto output features start .. stop-1 (a view; ``start`` a whole number of tiles of 128)."""
+        if self.epilogue != "none" or not 0 <= start < stop <= self.out_features:
+            raise ValueError(f"no features {start} .. {stop - 1} of {self.out_features} to take")
+        if start % TILE:
+            raise ValueError(f"feature {start} lies inside a tile of {TILE}")
+        view = object.__new__(MicroscaledWeight)
+        view.epilogue, view.in_features, view.out_features = "none", self.in_features, stop - start
+        at = slice(start // TILE, _count(stop, TILE))
+        view.tiles = Tiles(self.tiles.codes[:, at], self.tiles.scales[:, at], self.tiles.factors[:, start:stop], self.in_features, False)
+        return view
+
+    def _run(self, x: "torch.Tensor | MicroscaledRows", act: str, width: int, out_dtype: torch.dtype | None, out: torch.Tensor | None,
+             error_word: torch.Tensor | None) -> torch.Tensor:
+        if not isinstance(x, (torch.Tensor, MicroscaledRows)):
+            raise ops.KernelError(f"linear: a 4-bit weight takes a tensor or MicroscaledRows, not {type(x).__name__}")
+        ops.need_rows(x, self.in_features, self.tiles.device_index, "linear")
+        y = _output(x, out, width, x.dtype if out_dtype is None else out_dtype)
+        if len(x):
+            _product(x, self.tiles, y, act, 0.0, 0.0, 0, 0, 1, False, None, error_word)
+        return y
+
+    def product(self, x: "torch.Tensor | MicroscaledRows", *, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
+                error_word: torch.Tensor | None = None) -> torch.Tensor:
+        """x [tokens, in] times the weight: [tokens, out] (a swiglu weight's gate and up sums side by side)."""
+        return self._run(x, "none", self.out_features, out_dtype, out, error_word)
+
+    def swiglu(self, x: "torch.Tensor | MicroscaledRows", *, out_dtype: torch.dtype | None = None, error_word: torch.Tensor | None = None) -> torch.Tensor:
+        """silu(gate) * up of the 32-bit sums: [tokens, out / 2]."""
+        if self.epilogue != "swiglu":
+            raise ops.KernelError("linear_swiglu: the weight was not bound with epilogue='swiglu'")
+        return self._run(x, "swiglu", self.out_features // 2, out_dtype, None, error_word)
+
+
+class MicroscaledExperts:
+    """The experts' matrices of one product of a routed feed-forward, all of one size: ``MicroscaledExperts(matrices)``, or
+    ``MicroscaledExperts(gates, ups)`` for a gated unit.  :func:`ops.moe_expert_product` takes it in place of a tensor."""
+
+    def __init__(self, matrices: Sequence[MicroscaledMatrix], ups: Sequence[MicroscaledMatrix] | None = None) -> None:
+        if not matrices:
+            raise ValueError("a product of experts needs at least one")
+        if ups is not None and len(ups) != len(matrices):
+            raise ValueError(f"{len(matrices)} gate and {len(ups)} up matrices")
+        self.paired = ups is not None
+        self.tiles = _laid_out([[m] for m in matrices] if ups is None else list(zip(matrices, ups)), self.paired)
+        self.experts, self.in_features, self.out_features = len(matrices), self.tiles.columns, self.tiles.features
+
+    @property
+    def device(self) -> torch.device:
+        return self.tiles.codes.device
+
+    def address(self) -> int:
+        return self.tiles.codes_at
+
+    def nbytes(self) -> int:
+        return self.tiles.codes.numel() + self.tiles.scales.numel() + 4 * self.tiles.factors.numel()
+
+    def product(self, x: torch.Tensor, y: torch.Tensor, offsets: torch.Tensor, order: torch.Tensor, top: int, *, x_by_pair: bool,
+                act: str = "none", limit: float = 0.0, alpha: float = 1.0, row_scale: torch.Tensor | None = None,
+                error_word: torch.Tensor | None = None) -> torch.Tensor:
+        """See :func:`ops.moe_expert_product`."""
+        if not isinstance(x, torch.Tensor):
+            raise ops.KernelError("moe_expert_product: rows by expert are quantised as they are sorted; they come as a tensor")
+        pairs = ops.need_expert_product(x, y, offsets, order, top, x_by_pair, act, row_scale, self.experts, self.in_features, self.out_features, self.paired,
+                                        self.tiles.device_index)
+        if pairs:
+            _product(x, self.tiles, y, act, limit, alpha, offsets.data_ptr(), order.data_ptr(), top, x_by_pair, row_scale, error_word)
+        return y

@@ -1253,6 +1253,44 @@ def moe_combine(y: torch.Tensor, place: torch.Tensor, weights: torch.Tensor | No
     return out
 
 
+def need_rows(x, columns: int | None, device: int | None, what: str) -> int:
+    """The number of rows of ``x``, which must be [rows, ``columns``] with unit inner stride on the current device (and on ``device``); quantised rows have
+    no strides."""
+    shape = x.shape
+    if len(shape) != 2 or shape[1] == 0 or (columns is not None and shape[1] != columns):
+        raise KernelError(f"{what}: rows of {columns or 'one number or more'} are wanted, not {tuple(shape)}")
+    here = x.get_device()
+    if here < 0:
+        raise KernelError(f"{what}: operands must be CUDA tensors (there is no CPU path)")
+    if (device is not None and here != device) or here != torch._C._cuda_getDevice():
+        raise KernelError(f"{what}: the rows are on cuda:{here}, the weight on cuda:{device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    if isinstance(x, torch.Tensor) and x.stride(1) != 1 and shape[1] > 1:
+        raise KernelError(f"{what}: rows need unit inner stride, not {x.stride()}")
+    return shape[0]
+
+
+def need_expert_product(x: torch.Tensor, y: torch.Tensor, offsets: torch.Tensor, order: torch.Tensor, top: int, x_by_pair: bool, act: str,
+                        row_scale: torch.Tensor | None, experts: int, columns: int, features: int, paired: bool, here: int) -> int:
+    """The number of pairs of a :func:`moe_expert_product` with quantised experts (``paired``: of gate and up rows) on cuda:``here``."""
+    if act not in MOE_ACT:
+        raise KernelError(f"moe_expert_product: unknown activation {act!r}")
+    gated = act in MOE_GATED
+    if gated != paired and act != "none":
+        raise KernelError(f"moe_expert_product: activation {act!r} does not fit experts with{'' if paired else 'out'} gate and up rows")
+    pairs, width = order.numel(), features // 2 if gated else features
+    rows = need_rows(x, columns, here, "moe_expert_product")
+    if y.shape != (pairs, width) or offsets.numel() != experts + 1 or top < 1 or (pairs % top or rows < pairs // top if x_by_pair else rows < pairs):
+        raise KernelError("moe_expert_product: shapes do not fit")
+    for name, t, dtype in (("offsets", offsets, torch.int32), ("order", order, torch.int32), ("row_scale", row_scale, torch.float32)):
+        if t is not None and (t.dtype != dtype or t.get_device() != here or not t.is_contiguous()):
+            raise KernelError(f"moe_expert_product: {name} must be contiguous {dtype} on cuda:{here}, not {t.dtype} on {t.device}")
+    if y.get_device() != here or (y.stride(1) != 1 and width > 1):
+        raise KernelError(f"moe_expert_product: y must be rows with unit inner stride on cuda:{here}")
+    if row_scale is not None and row_scale.numel() != pairs:
+        raise KernelError("moe_expert_product: row_scale must hold one factor per pair")
+    return pairs
+
+
 # ---------------------------------------------------------------------------
 # 8-bit block-scaled operands (csrc/block_scaled*.cu).  Their Python types (kernels/block_scaled.py) check what they are given and own the buffers; these
 # take addresses, as a call with few rows is as long as what the host does for it.
@@ -1263,17 +1301,85 @@ def quantize_rows(x: torch.Tensor, codes: int, scales: int, lds: int) -> None:
                                                     0, 1, 0, rows, _stream()))
 
 
-def block_scaled_product(x: torch.Tensor, codes: int, make: bool, blocks, y: torch.Tensor, act: str, limit: float, alpha: float, offsets: int, order: int,
+def _rows_at(x: torch.Tensor | None) -> tuple[int, int, int, int]:
+    """(address, type, row stride, rows) of a product's rows; None: they are there as codes."""
+    return (0, BF16, 0, 0) if x is None else (x.data_ptr(), _code(x.dtype), x.stride(0), len(x))
+
+
+def widen_rows(codes: int, scales: int, lds: int, out: torch.Tensor) -> None:
+    """The numbers that codes and scales at these addresses, as :func:`quantize_rows` leaves them, stand for."""
+    rows, columns = out.shape
+    _check("widen_rows", lib().tib_widen_rows(codes, -(-columns // 128) * 128, scales, lds, out.data_ptr(), _code(out.dtype), out.stride(0), rows, columns, _stream()))
+
+
+def block_scaled_product(x: torch.Tensor | None, codes: int, make: bool, blocks, y: torch.Tensor, act: str, limit: float, alpha: float, offsets: int, order: int,
                          top: int, x_by_pair: bool, row_scale: torch.Tensor | None, error_word: torch.Tensor | None) -> None:
     """The rows ``x`` times matrices of 8-bit blocks (a block_scaled.Blocks), into ``y``.  ``codes``: the address of M * runs * 128 + 4 * runs * (M rounded up
-    to 4) bytes for the codes of the M rows of ``y``, which are made there first (``make``) or are there from a call before; 0: the product's kernel
-    quantises the rows itself.  ``offsets`` / ``order``: addresses of what sorts the rows of ``y`` by expert as in :func:`moe_expert_product`, or 0."""
+    to 4) bytes for the codes of the M rows of ``y``, which are made there first (``make``) or are there from a call before (``x`` may then be None); 0: the product's
+    kernel quantises the rows itself.  ``offsets`` / ``order``: addresses of what sorts the rows of ``y`` by expert as in :func:`moe_expert_product`, or 0."""
     if codes and make:
         _counter["launches"] += 1
     _check("block_scaled_product", lib().tib_block_scaled_product(
-        x.data_ptr(), _code(x.dtype), x.stride(0), len(x), codes, make, blocks.codes_at, blocks.scales_at, blocks.scale_rows, blocks.paired, y.data_ptr(),
+        *_rows_at(x), codes, make, blocks.codes_at, blocks.scales_at, blocks.scale_rows, blocks.paired, y.data_ptr(),
         _code(y.dtype), y.stride(0), len(y), blocks.features, blocks.columns, offsets, order, blocks.count, top, x_by_pair, MOE_ACT[act], limit, alpha,
         0 if row_scale is None else row_scale.data_ptr(), blocks.far_low, blocks.far_high, 0 if error_word is None else error_word.data_ptr(), _stream()))
+
+
+# The same of 4-bit microscaled operands (csrc/microscaled*.cu, kernels/microscaled.py).
+def microscaled_rows(x: torch.Tensor, codes: int, scales: int, factors: int) -> None:
+    """Codes, scales and factors of the rows ``x``, to these addresses."""
+    rows, columns = x.shape
+    _check("microscaled_rows", lib().tib_microscaled_rows(*_rows_at(x), codes, scales, factors, rows, columns, 0, 0, 1, 1, False, _stream()))
+
+
+def microscaled_widen(codes: int, scales: int, factors: int, out: torch.Tensor) -> None:
+    """The numbers that codes, scales and factors at these addresses stand for."""
+    rows, columns = out.shape
+    _check("microscaled_widen", lib().tib_microscaled_widen(codes, scales, factors, out.data_ptr(), _code(out.dtype), out.stride(0), rows, columns, _stream()))
+
+
+def microscaled_product(x: torch.Tensor | None, codes: int, scales: int, factors: int, tiles, y: torch.Tensor, act: str, limit: float, alpha: float, offsets: int,
+                        order: int, top: int, x_by_pair: bool, row_scale: torch.Tensor | None, error_word: torch.Tensor | None) -> None:
+    """Rows times matrices of 4-bit codes (a microscaled.Tiles), into ``y``: the rows at these addresses, where those of ``x`` are put first (None: they
+    are there).  ``offsets`` / ``order``: addresses of what sorts the rows of ``y`` by expert as in :func:`moe_expert_product`, or 0."""
+    if x is not None:
+        _counter["launches"] += 1
+    _check("microscaled_product", lib().tib_microscaled_product(
+        *_rows_at(x), codes, scales, factors, x is not None, tiles.codes_at, tiles.scales_at, tiles.factors_at, tiles.paired, y.data_ptr(), _code(y.dtype), y.stride(0),
+        len(y), tiles.features, tiles.columns, offsets, order, tiles.count, top, x_by_pair, MOE_ACT[act], limit, alpha,
+        0 if row_scale is None else row_scale.data_ptr(), 0 if error_word is None else error_word.data_ptr(), _stream()))
+
+
+def quantized_norm_type(delta: torch.Tensor | None, dtype: torch.dtype | None) -> torch.dtype:
+    """The type that a norm's rows are rounded to before they are quantised."""
+    dtype = dtype or (torch.bfloat16 if delta is None else delta.dtype)
+    if delta is not None and delta.dtype != dtype:
+        raise KernelError(f"add_rmsnorm: delta is {delta.dtype}, the rows {dtype}")
+    return dtype
+
+
+def quantized_norm(delta: torch.Tensor | None, residual: torch.Tensor, weight: torch.Tensor, eps: float, dtype: torch.dtype, rows: torch.Tensor | None,
+                   out: torch.Tensor | None, new_residual: torch.Tensor | None, in_bytes: bool, count: int, codes: int, scales: int, factors: int, lds: int) -> None:
+    """:func:`add_rmsnorm` whose ``count`` rows go, as codes and scales, to these addresses: ``in_bytes`` as :func:`quantize_rows` leaves them (``factors``: the scales), else
+    as :func:`microscaled_rows` does."""
+    _need(residual, "residual", torch.float32), _need(weight, "weight", torch.float32)
+    if residual.dim() != 2 or not residual.shape[1] or weight.numel() != residual.shape[1]:
+        raise KernelError(f"add_rmsnorm: residual {tuple(residual.shape)} / weight {tuple(weight.shape)} do not fit")
+    device = residual.get_device()
+    if device != torch._C._cuda_getDevice():
+        raise KernelError(f"add_rmsnorm: the residual is on cuda:{device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    if rows is not None and new_residual is not None:
+        raise KernelError("add_rmsnorm: with rows the residual is left as it is")
+    for name, t, kind, shape in (("delta", delta, dtype, residual.shape), ("rows", rows, torch.int32, (count,)), ("weight", weight, torch.float32, weight.shape),
+                                 ("out", out, dtype, (count, residual.shape[1])), ("new_residual", new_residual, torch.float32, residual.shape)):
+        if t is None:
+            continue
+        _need(t, name, kind)
+        if t.get_device() != device or t.shape != shape:
+            raise KernelError(f"add_rmsnorm: {name} is {tuple(t.shape)} on {t.device}, wanted {tuple(shape)} on {residual.device}")
+    kept = new_residual if new_residual is not None else residual if delta is not None and rows is None else None
+    _check("add_rmsnorm", lib().tib_quantized_norm(_ptr(delta), _ptr(residual), _ptr(kept), _ptr(rows), _ptr(weight), _ptr(out), in_bytes, codes, scales, factors, lds, count,
+                                                   residual.shape[1], eps, _code(dtype), _stream()))
 
 
 def glu_clamp(gate_up: torch.Tensor, out: torch.Tensor, limit: float, alpha: float) -> torch.Tensor:
