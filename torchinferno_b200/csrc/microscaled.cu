@@ -1,4 +1,4 @@
-// Rows of activations to 4-bit codes with their scales (microscaled.cuh) and back, and the product of such rows with 4-bit matrices.
+// Rows of activations to 4-bit codes with their scales (microscaled.cuh) and back, and the way of a product with 4-bit matrices to its kernel.
 #include "microscaled.cuh"
 
 namespace tib {
@@ -118,63 +118,6 @@ microscaled_widen_kernel(MsRows x, TO* __restrict__ out, int64_t ldo, int rows, 
   }
 }
 
-// A product, a thread for each output.
-__device__ float ms_dot(const unsigned char* x, const unsigned char* xs, const unsigned char* w, const unsigned char* ws, int steps) {
-  float sum = 0.f;
-  for (int step = 0; step < steps; ++step) {
-    for (int run = 0; run < 16; ++run) {
-      float v = 0.f;
-      for (int i = 0; i < 8; ++i) {
-        const float2 a = ms_numbers2(x[run * 8 + i]), b = ms_numbers2(w[run * 8 + i]);
-        v += a.x * b.x + a.y * b.y;
-      }
-      const int at = (run >> 2) * kMsChunkBytes + (run & 3);
-      sum += v * (ms_scale_value(xs[at]) * ms_scale_value(ws[at]));
-    }
-    x += kMsStepBytes; xs += kMsStepScales; w += kMsTileRows * kMsStepBytes; ws += kMsStepScales;
-  }
-  return sum;
-}
-template <typename TO>
-__global__ void __launch_bounds__(256)
-microscaled_product_kernel(MsArgs a, int act, TO* __restrict__ y, int64_t ldy) {
-  pdl_wait();
-  pdl_trigger();
-  const int gated = moe_act_gated(act) ? 1 : 0, n_out = a.N >> gated, row = blockIdx.y, o = blockIdx.x * blockDim.x + threadIdx.x;
-  if (o >= n_out) return;
-  int expert = 0, first = 0, tile = 0;
-  if (a.offsets) {
-    if (row >= bs_offset(a.offsets, a.experts, a.M)) return;
-    int hi = a.experts;
-    while (hi - expert > 1) {
-      const int mid = (expert + hi) >> 1;
-      if (bs_offset(a.offsets, mid, a.M) <= row) expert = mid; else hi = mid;
-    }
-    first = bs_offset(a.offsets, expert, a.M);
-    if (row < first) return;
-    tile = ms_first_tile(first, expert);
-  }
-  const int in = row - first, f_tiles = (a.N + 127) >> 7;
-  const unsigned char* x = a.x.codes + (size_t)row * a.steps * kMsStepBytes;
-  const unsigned char* xs = a.x.scales + (size_t)(tile + (in >> 7)) * a.steps * kMsStepScales + ms_scale_at(in & 127);
-  auto sum = [&](int f) {
-    const size_t block = (size_t)expert * f_tiles + (f >> 7);
-    const float v = ms_dot(x, xs, a.w + (block * a.steps * kMsTileRows + (f & 127)) * kMsStepBytes, a.w_scales + block * a.steps * kMsStepScales + ms_scale_at(f & 127), a.steps);
-    const float scaled = v * a.w_factors[(size_t)expert * a.N + f] * a.x.factors[row];
-    return a.row_scale ? scaled * a.row_scale[bs_pair(a.order, row, a.M)] : scaled;
-  };
-  const float g = sum(o << gated), u = gated ? sum((o << gated) + 1) : 0.f;
-  float v = g;
-  switch (act) {
-    case MOE_ACT_RELU2: v = bs_act<MOE_ACT_RELU2>(g); break;
-    case MOE_ACT_SILU: v = bs_act<MOE_ACT_SILU>(g); break;
-    case MOE_ACT_GELU: v = bs_act<MOE_ACT_GELU>(g); break;
-    case MOE_ACT_GLU_CLAMP: v = bs_gated<MOE_ACT_GLU_CLAMP>(g, u, a.limit, a.alpha); break;
-    case MOE_ACT_SWIGLU: v = bs_gated<MOE_ACT_SWIGLU>(g, u, a.limit, a.alpha); break;
-  }
-  y[(size_t)row * ldy + o] = from_f32<TO>(v);
-}
-
 }  // namespace tib
 
 using namespace tib;
@@ -237,16 +180,8 @@ TIB_API int tib_microscaled_product(const void* x, int x_dtype, int64_t ldx, int
     const int rc = tib_microscaled_rows(x, x_dtype, ldx, x_rows, codes, scales, factors, M, K, offsets, order, experts, top, x_by_pair, stream);
     if (rc != TIB_OK) return rc;
   }
-  MsArgs a;
-  a.x = MsRows{(const unsigned char*)codes, (const unsigned char*)scales, factors};
-  a.w = (const unsigned char*)w; a.w_scales = (const unsigned char*)w_scales; a.w_factors = w_factors;
-  a.M = M; a.N = N; a.steps = ms_steps(K); a.offsets = offsets; a.order = order; a.experts = experts; a.limit = limit; a.alpha = alpha;
-  a.row_scale = row_scale;
-  (void)error_word;
-  const dim3 grid(ceil_div(N >> (moe_act_gated(act) ? 1 : 0), 256), M);
-  if (y_dtype == TIB_BF16) TIB_LAUNCH_DEPENDENT(microscaled_product_kernel<__nv_bfloat16>, grid, 256, 0, stream, a, act, (__nv_bfloat16*)y, ldy);
-  else TIB_LAUNCH_DEPENDENT(microscaled_product_kernel<float>, grid, 256, 0, stream, a, act, (float*)y, ldy);
-  return TIB_OK;
+  return tib_microscaled_tcgen05(codes, scales, factors, w, w_scales, w_factors, y, y_dtype, ldy, M, N, K, offsets, order, experts, act, limit, alpha, row_scale,
+                                 error_word, stream);
 }
 
 TIB_PACKED(tib_microscaled_rows)

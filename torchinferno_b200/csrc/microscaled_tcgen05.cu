@@ -1,0 +1,422 @@
+// Products of 4-bit microscaled operands on the 5th-generation tensor cores, for few rows and for rows sorted by expert:
+//     y[m, n] = act(r[m] f[n] (sum over runs b of s[m, b] S[n, b] (sum over the 16 columns of run b of x[m, k] w[n, k])))
+//
+// The weights are the 128-row operand of the MMA and the rows its N dimension: a tile is 128 features x up to NT rows, the rows rounded up to 16
+// only, and the accumulator, which stays in tensor memory for the whole sum, is the transposed output (TMEM lane = feature, column = row).  A step of the loop
+// is 256 columns: the 128-byte row of the swizzle, eight copies of scales (512 bytes each) to tensor memory, four MMAs.  The scales of a stage of the
+// ring have columns of their own, so that they are free when the stage is.
+//   warp 0       producer: 16 KB of codes of w a step and 2 KB of its scales, one run of memory each; the rows' codes in boxes of 32 rows, their scales
+//   warp 1       copies scales and issues tcgen05.mma; owns the TMEM allocation
+//   the next 4   epilogue: eight rows at a time, a lane a feature, so that a warp writes 32 outputs of a row side by side; two accumulators take turns
+// A matrix of few tiles is split by steps over a cluster of up to eight blocks, whose sums meet in distributed shared memory, added in the order of the
+// steps.  Every wait is bounded and reports in error_word.
+#include "microscaled.cuh"
+
+namespace tib {
+
+constexpr int kMtMaxExperts = 1024, kMtMaxStages = 8, kMtThreads = 192;
+constexpr uint32_t kMtWBytes = kMsTileRows * kMsStepBytes, kMtBarBytes = 256;
+
+template <int NT> struct MtShape {
+  static constexpr int kPerSm = NT <= 32 ? 2 : 1;                                // blocks of an SM
+  static constexpr uint32_t kTmemCols = 512 / kPerSm, kScaleCols = 2 * NT;       // two accumulators, then 32 columns of scales a stage
+  static constexpr int kStages = (kTmemCols - kScaleCols) / 32 < kMtMaxStages ? (kTmemCols - kScaleCols) / 32 : kMtMaxStages;
+  static constexpr uint32_t kStage = kMtWBytes + NT * kMsStepBytes + 2 * kMsStepScales;
+};
+// of the sums of a shared tile: (a column's 128 / splits sums and four more, so that those that a warp writes at a time fall on all banks)
+template <int NT> __host__ __device__ constexpr int mt_red_floats(int splits) { return splits > 1 ? NT * (128 + 4 * splits) : 0; }
+
+struct MtTile { int expert, first, rows, scale_tile, feature; };
+
+// An output (of a gated unit: from its gate g and up u).
+template <int ACT> __device__ __forceinline__ float mt_act(float g, float u, const MsArgs& a) {
+  if constexpr (moe_act_gated(ACT)) return bs_gated<ACT>(g, u, a.limit, a.alpha);
+  else return bs_act<ACT>(g);
+}
+
+template <int NT, int ACT, typename TO>
+__global__ void __launch_bounds__(kMtThreads, MtShape<NT>::kPerSm)
+microscaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ MsArgs a, TO* __restrict__ y,
+                           int64_t ldy) {
+  using S = MtShape<NT>;
+  constexpr int kGated = moe_act_gated(ACT) ? 1 : 0;
+  const int splits = (int)cluster_size(), rank = (int)cluster_rank();
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char* smem_gen = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t bars = base + a.stages * S::kStage;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (kMtMaxStages + s); };
+  auto acc_full_bar = [&](int b) { return bars + 8u * (2 * kMtMaxStages + b); };
+  auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * kMtMaxStages + 2 + b); };
+  const uint32_t red_bar = bars + 8u * (2 * kMtMaxStages + 4), tmem_slot = red_bar + 8;
+  static_assert(8 * (2 * kMtMaxStages + 5) + 8 <= kMtBarBytes, "the barriers' share of shared memory");
+  volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem_gen + (tmem_slot - base));
+  float* red = reinterpret_cast<float*>(smem_gen + (bars - base) + kMtBarBytes);         // [splits][NT][128 / splits + 4] sums
+  int* tiles_before = reinterpret_cast<int*>(red + mt_red_floats<NT>(splits));           // [experts + 1] where rows are sorted, and
+  int* first_row = tiles_before + a.experts + 1;                                         // [experts + 1] their offsets
+
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int cluster_id = blockIdx.x / splits, clusters = gridDim.x / splits;
+  const int step0 = (int)((int64_t)a.steps * rank / splits), step1 = (int)((int64_t)a.steps * (rank + 1) / splits);
+  if (warp == 0) {
+    if (lane == 0) {
+      asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map_w) : "memory");
+      asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map_x) : "memory");
+    }
+    if (lane < a.stages) {
+      mbar_init(full_bar(lane), 1);
+      mbar_init(empty_bar(lane), 1);
+    }
+    if (lane < 2) {
+      mbar_init(acc_full_bar(lane), 1);
+      mbar_init(acc_empty_bar(lane), 4);
+    }
+    if (lane == 0) mbar_init(red_bar, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tmem_slot), "r"(S::kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  if (a.offsets) {
+    pdl_wait();
+    if (warp == 0) {      // the experts' row tiles, summed
+      int before = 0;
+      for (int e0 = 0; e0 < a.experts; e0 += 32) {
+        const int e = e0 + lane, begin = e < a.experts ? bs_offset(a.offsets, e, a.M) : 0;
+        int sum = e < a.experts ? (max(0, bs_offset(a.offsets, e + 1, a.M) - begin) + NT - 1) / NT : 0;
+        if (e < a.experts) first_row[e] = begin;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += up;
+        }
+        if (e < a.experts) tiles_before[e + 1] = before + sum;
+        before += __shfl_sync(0xffffffffu, sum, 31);
+      }
+      if (lane == 0) tiles_before[0] = 0, first_row[a.experts] = bs_offset(a.offsets, a.experts, a.M);
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+  pdl_trigger();      // (tensor memory is this block's by now: a block of the kernel behind it cannot take it first)
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot_ptr, 0);
+  if (splits > 1) cluster_sync_all();             // every block of the cluster runs and has its barriers
+
+  const int f_tiles = (a.N + 127) >> 7;
+  const int row_tiles = a.offsets ? tiles_before[a.experts] : (a.M + NT - 1) / NT;
+  const int num_tiles = row_tiles * f_tiles;
+  auto tile_of = [&](int t) {                     // (feature tiles run fastest: blocks that run together read the same rows)
+    const int row_tile = row_tiles == 1 ? 0 : t / f_tiles;
+    MtTile m;
+    int begin = 0, n = a.M, j = row_tile;
+    m.expert = 0;
+    m.scale_tile = 0;
+    if (a.offsets) {
+      int lo = 0, hi = a.experts;                 // tiles_before[lo] <= row_tile < tiles_before[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (tiles_before[mid] <= row_tile) lo = mid; else hi = mid;
+      }
+      begin = first_row[lo];
+      n = first_row[lo + 1] - begin;
+      j = row_tile - tiles_before[lo];
+      m.expert = lo;
+      m.scale_tile = ms_first_tile(begin, lo);
+    }
+    m.first = begin + j * NT;
+    m.rows = min(NT, n - j * NT);
+    m.scale_tile += j * NT >> 7;                  // (tiles of fewer than 128 rows: the launch sees to it that there is one)
+    m.feature = (t - row_tile * f_tiles) << 7;
+    return m;
+  };
+
+  if (warp == 0) {
+    const uint32_t leader = umma_leader();
+    int ahead = 0, it = 0, s = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    auto ask_w = [&](const MtTile& m, int step, int s) {
+      const uint32_t stage = base + s * S::kStage;
+      const int block = (m.expert * f_tiles + (m.feature >> 7)) * a.steps + step;
+      mbar_expect_tx(full_bar(s), kMtWBytes + 2 * kMsStepScales + ((m.rows + 31) >> 5) * 32 * kMsStepBytes);
+      tma_load_2d(stage, &map_w, 0, block << 7, full_bar(s));
+      ms_bulk_load(stage + kMtWBytes + NT * kMsStepBytes, a.w_scales + (size_t)block * kMsStepScales, kMsStepScales, full_bar(s));
+    };
+    if (!a.offsets) {
+      for (int t = cluster_id; t < num_tiles && ahead < a.stages; t += clusters) {
+        const MtTile m = tile_of(t);
+        for (int step = step0; step < step1 && ahead < a.stages; ++step, ++ahead)
+          if (leader) ask_w(m, step, ahead);
+      }
+      pdl_wait();
+    }
+    for (int t = cluster_id; t < num_tiles && ok; t += clusters) {
+      const MtTile m = tile_of(t);
+      for (int step = step0; step < step1; ++step, ++it) {
+        if (it >= ahead) {
+          if (!mbar_wait_warp(empty_bar(s), phase)) {
+            if (a.error_word && leader) atomicExch(a.error_word, 0x7C00E1);
+            ok = false;
+            break;
+          }
+          if (leader) ask_w(m, step, s);
+          __syncwarp();
+        }
+        if (leader) {
+          const uint32_t rows_at = base + s * S::kStage + kMtWBytes;
+#pragma unroll
+          for (int i = 0; i < NT / 32; ++i)       // (the last box may reach into the next tile's rows, or past the last: such columns are never stored)
+            if (32 * i < m.rows) tma_load_2d(rows_at + i * 32 * kMsStepBytes, &map_x, step * kMsStepBytes, m.first + 32 * i, full_bar(s));
+          ms_bulk_load(rows_at + NT * kMsStepBytes + kMsStepScales, a.x.scales + ((size_t)m.scale_tile * a.steps + step) * kMsStepScales, kMsStepScales, full_bar(s));
+        }
+        __syncwarp();
+        if (++s == a.stages) { s = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t leader = umma_leader();
+    if (!a.offsets) pdl_wait();                   // (the bounded waits begin when the kernel before is over)
+    int s = 0, b = 0;
+    uint32_t phase = 0, acc_phase = 1;
+    bool ok = true;
+    for (int t = cluster_id; t < num_tiles && ok; t += clusters) {
+      const MtTile m = tile_of(t);
+      const uint32_t idesc = kMsIdesc | ((uint32_t)((m.rows + 15) >> 4) << 18) | ((128u >> 4) << 24);
+      if (!mbar_wait_warp(acc_empty_bar(b), acc_phase)) {
+        if (a.error_word && leader) atomicExch(a.error_word, 0x7C00E4);
+        break;
+      }
+      for (int step = step0; step < step1; ++step) {
+        if (!mbar_wait_warp(full_bar(s), phase)) {
+          if (a.error_word && leader) atomicExch(a.error_word, 0x7C00E2);
+          ok = false;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        const uint32_t stage = base + s * S::kStage, scales = stage + kMtWBytes + NT * kMsStepBytes;
+        const uint32_t w_src = umma_low_k128(stage), x_src = w_src + (kMtWBytes >> 4), columns = tmem_base + S::kScaleCols + 32 * s;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) ms_copy_scales<1>(leader, columns + 4 * k, scales + kMsChunkBytes * k);      // (four of w, four of the rows)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          ms_umma<1>(leader, tmem_base + b * NT, w_src + 2 * k, x_src + 2 * k, idesc, columns + 4 * k, columns + 16 + 4 * k, step != step0 || k != 0);
+        if (leader) umma_commit(empty_bar(s));
+        __syncwarp();
+        if (++s == a.stages) { s = 0; phase ^= 1; }
+      }
+      if (leader) umma_commit(acc_full_bar(b));
+      __syncwarp();
+      if (++b == 2) { b = 0; acc_phase ^= 1; }
+    }
+  } else {
+    const int quarter = warp & 3, et = threadIdx.x - 64;
+    int b = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    if (!a.offsets) pdl_wait();                   // (y may be memory that the kernel before still reads)
+    for (int t = cluster_id; t < num_tiles; t += clusters) {
+      const MtTile m = tile_of(t);
+      const int feature = m.feature + quarter * 32 + lane, n_out = a.N >> kGated;
+      const float factor = a.w_factors[(size_t)m.expert * a.N + min(feature, a.N - 1)];
+      if (ok && !mbar_wait_warp(acc_full_bar(b), acc_phase)) {
+        if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00E3);
+        ok = false;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+      const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + b * NT;
+      auto row_factor = [&](int c, float& x, float& pair) {
+        const int row = m.first + min(c, m.rows - 1);
+        x = a.x.factors[row];
+        pair = a.row_scale ? a.row_scale[bs_pair(a.order, row, a.M)] : 1.f;
+      };
+      if (splits == 1) {
+#pragma unroll 1
+        for (int q = 0; q < m.rows; q += 32) {
+          float x_factor, pair_factor;
+          row_factor(q + lane, x_factor, pair_factor);
+#pragma unroll 1
+          for (int c = q; c < min(q + 32, m.rows); c += 8) {
+            uint32_t v[8];
+            tmem_ld8(acc + c, v);
+            asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+            float s[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              s[j] = ms_scaled(__uint_as_float(v[j]), factor, __shfl_sync(0xffffffffu, x_factor, (c + j) & 31), __shfl_sync(0xffffffffu, pair_factor, (c + j) & 31));
+            if (!ok) continue;
+            if constexpr (kGated) {
+              // a pair of lanes has gate and up of an output: the even one finishes the even rows, the odd one the odd rows
+#pragma unroll
+              for (int j = 0; j < 8; j += 2) {
+                const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? s[j] : s[j + 1], 1);
+                const int row = c + j + (lane & 1);
+                const float out = lane & 1 ? mt_act<ACT>(other, s[j + 1], a) : mt_act<ACT>(s[j], other, a);
+                if (row < m.rows && feature >> 1 < n_out) y[(size_t)(m.first + row) * ldy + (feature >> 1)] = from_f32<TO>(out);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (c + j < m.rows && feature < n_out) y[(size_t)(m.first + c + j) * ldy + feature] = from_f32<TO>(mt_act<ACT>(s[j], 0.f, a));
+            }
+          }
+        }
+      }
+      // Block r of a cluster finishes features r * per .. of the tile.
+      const int log_splits = 31 - __clz(splits), per = 128 >> log_splits, stride = per + 4;
+      if (splits > 1) {
+        const int in = quarter * 32 + lane, owner = in >> (7 - log_splits);
+        const uint32_t dst = map_to_cta(smem_u32(red + (size_t)rank * NT * stride + (in & (per - 1))), owner), bar = map_to_cta(red_bar, owner);
+        if (et == 0) mbar_expect_tx(red_bar, 128 * 4 * ((m.rows + 7) & ~7));      // (the stores themselves count on the owner's barrier: no fence, no arrivals)
+#pragma unroll 1
+        for (int c = 0; c < m.rows; c += 8) {
+          uint32_t v[8];
+          tmem_ld8(acc + c, v);
+          asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+          for (int j = 0; j < 8; ++j) st_async_f32(dst + (c + j) * stride * 4, __uint_as_float(v[j]), bar);
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty_bar(b));
+      if (++b == 2) { b = 0; acc_phase ^= 1; }
+      if (splits > 1) {      // (a cluster has one tile: its sums' place is used once)
+        if (!mbar_wait_cluster(red_bar, 0)) {
+          if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00E5);
+          ok = false;
+        }
+        const int outs = per >> kGated, o = et & (outs - 1), f = rank * per + (o << kGated), out = (m.feature + f) >> kGated;
+        if (!ok || out >= n_out) continue;
+        const float g_factor = a.w_factors[(size_t)m.expert * a.N + m.feature + f], u_factor = kGated ? a.w_factors[(size_t)m.expert * a.N + m.feature + f + 1] : 0.f;
+        for (int c = et / outs; c < m.rows; c += 128 / outs) {
+          const float* from = red + (size_t)c * stride + (o << kGated);
+          float g = from[0], u = from[kGated];
+          for (int r = 1; r < splits; ++r) {
+            from += NT * stride;
+            g += from[0];
+            u += from[kGated];
+          }
+          float x_factor, pair_factor;
+          row_factor(c, x_factor, pair_factor);
+          g = ms_scaled(g, g_factor, x_factor, pair_factor);
+          u = ms_scaled(u, u_factor, x_factor, pair_factor);
+          y[(size_t)(m.first + c) * ldy + out] = from_f32<TO>(mt_act<ACT>(g, u, a));
+        }
+      }
+    }
+  }
+  __syncwarp();
+  if (splits > 1) {
+    cluster_sync_all();                           // every block has sent its sums, also one that gave up waiting for others',
+    if (warp == 0) mbar_wait_warp(red_bar, 0);    // and none leaves before what was sent to it has come
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
+  }
+}
+
+template <int NT> static uint32_t mt_smem(int stages, int splits, int experts) {
+  return 1024u + stages * MtShape<NT>::kStage + kMtBarBytes + 4 * (mt_red_floats<NT>(splits) + 2 * (experts + 1));
+}
+
+// The blocks that share a tile's steps: 8, 4 or 2 where there is room for them beside the other tiles' and the steps are enough to pay for the exchange.
+static int mt_splits(int64_t tiles, int steps, int blocks) {
+  if (tiles * 8 <= blocks && steps >= 32) return 8;
+  if (tiles * 4 <= blocks && steps >= 4) return 4;
+  return tiles * 2 <= blocks && steps >= 4 ? 2 : 1;
+}
+
+// How a product runs: blocks in the grid, those that share a tile, steps of a block at most, stages of its ring.
+struct MtPlan { int grid, splits, steps, stages; };
+template <int NT> static int mt_plan(int M, int N, int steps, int experts, MtPlan& p) {      // experts: 0 for one matrix
+  using S = MtShape<NT>;
+  constexpr int kBlocks = 148 * S::kPerSm;
+  const int64_t row_tiles = experts ? M / NT + (M < experts ? M : experts) : ceil_div(M, NT), tiles = row_tiles * ceil_div(N, 128);
+  p.splits = experts ? 1 : mt_splits(tiles, steps, kBlocks);
+  if (tiles * p.splits > 0x7fffffff) return TIB_E_SIZE;
+  p.grid = (int)(p.splits > 1 ? tiles * p.splits : tiles < kBlocks ? tiles : kBlocks);
+  const int64_t most = (int64_t)ceil_div(steps, p.splits) * ceil_div64(tiles * p.splits, p.grid);
+  p.steps = (int)(most < 0x7fffffff ? most : 0x7fffffff);
+  p.stages = 1;
+  while (p.stages < S::kStages && p.stages < p.steps && mt_smem<NT>(p.stages + 1, p.splits, experts) <= (S::kPerSm > 1 ? 113u * 1024 : (uint32_t)kMostSmem)) ++p.stages;
+  return TIB_OK;
+}
+// Rows of a tile: 32 where all rows are one tile, else 128 (the tiles of their scales).
+static int mt_tile_rows(int M) { return M <= 32 ? 32 : 128; }
+
+template <int NT, int ACT, typename TO>
+static int launch_mt(const CUtensorMap& map_w, const CUtensorMap& map_x, MsArgs& a, void* y, int64_t ldy, cudaStream_t stream) {
+  const int experts = a.offsets ? a.experts : 0;
+  MtPlan plan;
+  const int rc = mt_plan<NT>(a.M, a.N, a.steps, experts, plan);
+  if (rc != TIB_OK) return rc;
+  a.stages = plan.stages;
+  auto kern = microscaled_tcgen05_kernel<NT, ACT, TO>;
+  static bool allowed[64];      // (by device: the attribute belongs to its context)
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess && !(device < 64 && allowed[device])) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
+  if (e != cudaSuccess) return (int)e;
+  if (device < 64) allowed[device] = true;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kMtThreads);
+  cfg.dynamicSmemBytes = mt_smem<NT>(plan.stages, plan.splits, experts);
+  cfg.stream = stream;
+  cfg.gridDim = dim3((unsigned)plan.grid);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)plan.splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // (see launch_dependent in common.cuh)
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent_launch_flag() ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, kern, map_w, map_x, (const MsArgs)a, (TO*)y, ldy);
+  if (e != cudaSuccess) return (int)e;
+  TIB_LAUNCH_CHECK();
+  return TIB_OK;
+}
+
+template <int NT, typename TO>
+static int launch_mt_act(int act, const CUtensorMap& map_w, const CUtensorMap& map_x, MsArgs& a, void* y, int64_t ldy, cudaStream_t stream) {
+  switch (act) {
+    case MOE_ACT_NONE: return launch_mt<NT, MOE_ACT_NONE, TO>(map_w, map_x, a, y, ldy, stream);
+    case MOE_ACT_RELU2: return launch_mt<NT, MOE_ACT_RELU2, TO>(map_w, map_x, a, y, ldy, stream);
+    case MOE_ACT_SILU: return launch_mt<NT, MOE_ACT_SILU, TO>(map_w, map_x, a, y, ldy, stream);
+    case MOE_ACT_GELU: return launch_mt<NT, MOE_ACT_GELU, TO>(map_w, map_x, a, y, ldy, stream);
+    case MOE_ACT_GLU_CLAMP: return launch_mt<NT, MOE_ACT_GLU_CLAMP, TO>(map_w, map_x, a, y, ldy, stream);
+    default: return launch_mt<NT, MOE_ACT_SWIGLU, TO>(map_w, map_x, a, y, ldy, stream);
+  }
+}
+
+}  // namespace tib
+
+using namespace tib;
+
+// See tib_microscaled_product, which checks the arguments: rows as codes, scales and factors.
+TIB_API int tib_microscaled_tcgen05(const void* codes, const void* scales, const float* factors, const void* w, const void* w_scales, const float* w_factors, void* y,
+                                    int y_dtype, int64_t ldy, int M, int N, int K, const int* offsets, const int* order, int experts, int act, float limit,
+                                    float alpha, const float* row_scale, int* error_word, cudaStream_t stream) {
+  if (experts > kMtMaxExperts || (int64_t)experts * ceil_div(N, 128) * ms_steps(K) > (0x7fffffff >> 7)) return TIB_E_SIZE;
+  MsArgs a;
+  a.x = MsRows{(const unsigned char*)codes, (const unsigned char*)scales, factors};
+  a.w = (const unsigned char*)w; a.w_scales = (const unsigned char*)w_scales; a.w_factors = w_factors;
+  a.M = M; a.N = N; a.steps = ms_steps(K); a.stages = 0; a.offsets = offsets; a.order = order; a.experts = experts;
+  a.limit = limit; a.alpha = alpha; a.row_scale = row_scale; a.error_word = error_word;
+  CUtensorMap map_w, map_x;
+  int rc = bs_make_map(&map_w, w, (int64_t)experts * ceil_div(N, 128) * a.steps * 128, kMsStepBytes, 128);
+  if (rc == TIB_OK) rc = bs_make_map(&map_x, codes, M, (int64_t)a.steps * kMsStepBytes, 32);
+  if (rc != TIB_OK) return rc;
+#define TIB_MT_GO(NT) \
+  return y_dtype == TIB_BF16 ? launch_mt_act<NT, __nv_bfloat16>(act, map_w, map_x, a, y, ldy, stream) : launch_mt_act<NT, float>(act, map_w, map_x, a, y, ldy, stream)
+  if (mt_tile_rows(M) == 32) TIB_MT_GO(32);
+  TIB_MT_GO(128);
+#undef TIB_MT_GO
+}
