@@ -172,7 +172,8 @@ def check(y, x, matrices, act="none"):
 
 
 PLAIN = [(1, 4096, 4096), (1, 16, 8), (1, 1, 1), (2, 255, 129), (3, 257, 1), (8, 4096, 640), (8, 512, 28672), (16, 1000, 1302), (17, 2048, 300), (33, 300, 77), (64, 4096, 512),
-         (128, 520, 1400), (129, 256, 130), (200, 1000, 257), (333, 1000, 1302), (600, 4096, 1024), (1000, 272, 2304), (2100, 600, 500)]
+         (128, 520, 1400), (129, 256, 130), (200, 1000, 257), (333, 1000, 1302), (600, 4096, 1024), (1000, 272, 2304), (2100, 600, 500),
+         (2100, 600, 2500), (600, 4096, 4096), (129, 300, 9601), (1000, 272, 2561), (3000, 1100, 4000)]
 
 
 @pytest.mark.parametrize("out", [BF16, F32])
@@ -188,7 +189,7 @@ def test_products(m, k, n, out):
     assert torch.equal(gemm.linear(quantize_rows(x), weight, out_dtype=out), y)
 
 
-@pytest.mark.parametrize("m, k, n", [(1, 4096, 1024), (8, 512, 700), (20, 1000, 333), (130, 600, 129), (500, 1100, 1000), (2000, 512, 2304)])
+@pytest.mark.parametrize("m, k, n", [(1, 4096, 1024), (8, 512, 700), (20, 1000, 333), (130, 600, 129), (500, 1100, 1000), (2000, 512, 2304), (333, 1400, 4001)])
 def test_gated_products(m, k, n):
     need_gpu()
     gate, up = random_matrix(n, k, m + n, DEV, 1e-4), random_matrix(n, k, m + n + 1, DEV, 2.3e-4)
@@ -203,7 +204,8 @@ def test_gated_products(m, k, n):
 
 @pytest.mark.parametrize("act", ["none", "relu2", "silu", "gelu", "swiglu", "glu_clamp"])
 @pytest.mark.parametrize("counts, k, n, top", [([1, 0, 3, 0, 4], 520, 300, 2), ([0, 0, 1], 256, 40, 1), ([130, 5, 0, 129, 128, 1, 255], 300, 200, 3), ([16] * 60, 512, 96, 4),
-                                               ([700, 0, 900, 3], 1000, 257, 1)])
+                                               ([700, 0, 900, 3], 1000, 257, 1),
+                                               ([257, 0, 256, 1, 600, 130], 1600, 520, 2)])
 def test_products_of_experts(counts, k, n, top, act):
     need_gpu()
     experts, pairs = len(counts), sum(counts)

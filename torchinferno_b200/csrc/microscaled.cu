@@ -180,8 +180,13 @@ TIB_API int tib_microscaled_product(const void* x, int x_dtype, int64_t ldx, int
     const int rc = tib_microscaled_rows(x, x_dtype, ldx, x_rows, codes, scales, factors, M, K, offsets, order, experts, top, x_by_pair, stream);
     if (rc != TIB_OK) return rc;
   }
-  return tib_microscaled_tcgen05(codes, scales, factors, w, w_scales, w_factors, y, y_dtype, ldy, M, N, K, offsets, order, experts, act, limit, alpha, row_scale,
-                                 error_word, stream);
+  MsArgs a;
+  a.x = MsRows{(const unsigned char*)codes, (const unsigned char*)scales, factors};
+  a.w = (const unsigned char*)w; a.w_scales = (const unsigned char*)w_scales; a.w_factors = w_factors;
+  a.M = M; a.N = N; a.steps = ms_steps(K); a.stages = 0; a.offsets = offsets; a.order = order; a.experts = experts;
+  a.limit = limit; a.alpha = alpha; a.row_scale = row_scale; a.error_word = error_word;
+  if (ms_on_pairs_of_sms(M, N, offsets ? experts : 0)) return ms_product_2cta(a, act, y, y_dtype, ldy, stream);
+  return ms_product_tcgen05(a, act, y, y_dtype, ldy, stream);
 }
 
 TIB_PACKED(tib_microscaled_rows)

@@ -142,12 +142,9 @@ struct MsArgs {
 // output itself does.
 __device__ __forceinline__ float ms_scaled(float sum, float w_factor, float x_factor, float row_scale) { return sum * w_factor * x_factor * row_scale; }
 
-}  // namespace tib
+// Products of rows that are there as codes (microscaled_tcgen05.cu, microscaled_2cta.cu), with arguments that tib_microscaled_product has checked.
+bool ms_on_pairs_of_sms(int M, int N, int experts);
+int ms_product_2cta(const MsArgs& a, int act, void* y, int y_dtype, int64_t ldy, cudaStream_t stream);
+int ms_product_tcgen05(MsArgs& a, int act, void* y, int y_dtype, int64_t ldy, cudaStream_t stream);
 
-extern "C" {
-int tib_microscaled_rows(const void* x, int x_dtype, int64_t ldx, int x_rows, void* codes, void* scales, float* factors, int rows, int K, const int* offsets,
-                         const int* order, int experts, int top, int x_by_pair, cudaStream_t stream);
-int tib_microscaled_tcgen05(const void* codes, const void* scales, const float* factors, const void* w, const void* w_scales, const float* w_factors, void* y,
-                            int y_dtype, int64_t ldy, int M, int N, int K, const int* offsets, const int* order, int experts, int act, float limit, float alpha,
-                            const float* row_scale, int* error_word, cudaStream_t stream);
-}
+}  // namespace tib

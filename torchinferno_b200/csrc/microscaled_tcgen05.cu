@@ -400,23 +400,15 @@ static int launch_mt_act(int act, const CUtensorMap& map_w, const CUtensorMap& m
 
 using namespace tib;
 
-// See tib_microscaled_product, which checks the arguments: rows as codes, scales and factors.
-TIB_API int tib_microscaled_tcgen05(const void* codes, const void* scales, const float* factors, const void* w, const void* w_scales, const float* w_factors, void* y,
-                                    int y_dtype, int64_t ldy, int M, int N, int K, const int* offsets, const int* order, int experts, int act, float limit,
-                                    float alpha, const float* row_scale, int* error_word, cudaStream_t stream) {
-  if (experts > kMtMaxExperts || (int64_t)experts * ceil_div(N, 128) * ms_steps(K) > (0x7fffffff >> 7)) return TIB_E_SIZE;
-  MsArgs a;
-  a.x = MsRows{(const unsigned char*)codes, (const unsigned char*)scales, factors};
-  a.w = (const unsigned char*)w; a.w_scales = (const unsigned char*)w_scales; a.w_factors = w_factors;
-  a.M = M; a.N = N; a.steps = ms_steps(K); a.stages = 0; a.offsets = offsets; a.order = order; a.experts = experts;
-  a.limit = limit; a.alpha = alpha; a.row_scale = row_scale; a.error_word = error_word;
+int tib::ms_product_tcgen05(MsArgs& a, int act, void* y, int y_dtype, int64_t ldy, cudaStream_t stream) {
+  if (a.experts > kMtMaxExperts || (int64_t)a.experts * ceil_div(a.N, 128) * a.steps > (0x7fffffff >> 7)) return TIB_E_SIZE;
   CUtensorMap map_w, map_x;
-  int rc = bs_make_map(&map_w, w, (int64_t)experts * ceil_div(N, 128) * a.steps * 128, kMsStepBytes, 128);
-  if (rc == TIB_OK) rc = bs_make_map(&map_x, codes, M, (int64_t)a.steps * kMsStepBytes, 32);
+  int rc = bs_make_map(&map_w, a.w, (int64_t)a.experts * ceil_div(a.N, 128) * a.steps * 128, kMsStepBytes, 128);
+  if (rc == TIB_OK) rc = bs_make_map(&map_x, a.x.codes, a.M, (int64_t)a.steps * kMsStepBytes, 32);
   if (rc != TIB_OK) return rc;
 #define TIB_MT_GO(NT) \
   return y_dtype == TIB_BF16 ? launch_mt_act<NT, __nv_bfloat16>(act, map_w, map_x, a, y, ldy, stream) : launch_mt_act<NT, float>(act, map_w, map_x, a, y, ldy, stream)
-  if (mt_tile_rows(M) == 32) TIB_MT_GO(32);
+  if (mt_tile_rows(a.M) == 32) TIB_MT_GO(32);
   TIB_MT_GO(128);
 #undef TIB_MT_GO
 }
