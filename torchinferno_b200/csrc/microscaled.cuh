@@ -87,29 +87,28 @@ __device__ __forceinline__ float2 ms_numbers2(uint32_t byte) {
 // D fp32 in tensor memory (+)= the product of a chunk's 64 columns: A and B e2m1 in shared memory, K-major (descriptors by their lower halves), each
 // row's four e4m3 scales in tensor memory.  The instruction descriptor but for N and M: both types e2m1, unsigned e4m3 scales.
 constexpr uint32_t kMsIdesc = (1u << 7) | (1u << 10);
+// By one elected thread, in a branch of its own: predicated by lane, as the products of other kernels are, a copy took 45 cycles of the warp that issues it and an
+// MMA 64, and sixteen of them a step were what bound it (8,192 rows 8,192 -> 28,672: 1,118 us, in a branch 674).
 template <int CTAS>
-__device__ __forceinline__ void ms_umma(uint32_t leader, uint32_t tmem_d, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t a_scales, uint32_t b_scales,
-                                        uint32_t accumulate) {
+__device__ __forceinline__ void ms_umma(uint32_t tmem_d, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t a_scales, uint32_t b_scales, uint32_t accumulate) {
   static_assert(CTAS == 1 || CTAS == 2, "blocks of a tile");
   if constexpr (CTAS == 1)
-    asm volatile("{\n.reg .pred p, q;\n.reg .b64 a, b;\nmov.b64 a, {%1, %8};\nmov.b64 b, {%2, %8};\nsetp.ne.b32 p, %6, 0;\nsetp.ne.b32 q, %7, 0;\n"
-                 "@q tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], a, b, %3, [%4], [%5], p;\n}\n"
-                 ::"r"(tmem_d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate), "r"(leader), "r"(kUmmaDescHigh) : "memory");
+    asm volatile("{\n.reg .pred p;\n.reg .b64 a, b;\nmov.b64 a, {%1, %7};\nmov.b64 b, {%2, %7};\nsetp.ne.b32 p, %6, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], a, b, %3, [%4], [%5], p;\n}\n"
+                 ::"r"(tmem_d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate), "r"(kUmmaDescHigh) : "memory");
   else
-    asm volatile("{\n.reg .pred p, q;\n.reg .b64 a, b;\nmov.b64 a, {%1, %8};\nmov.b64 b, {%2, %8};\nsetp.ne.b32 p, %6, 0;\nsetp.ne.b32 q, %7, 0;\n"
-                 "@q tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], a, b, %3, [%4], [%5], p;\n}\n"
-                 ::"r"(tmem_d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate), "r"(leader), "r"(kUmmaDescHigh) : "memory");
+    asm volatile("{\n.reg .pred p;\n.reg .b64 a, b;\nmov.b64 a, {%1, %7};\nmov.b64 b, {%2, %7};\nsetp.ne.b32 p, %6, 0;\n"
+                 "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], a, b, %3, [%4], [%5], p;\n}\n"
+                 ::"r"(tmem_d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate), "r"(kUmmaDescHigh) : "memory");
 }
 // A chunk's scales (512 bytes of shared memory: 32 rows of 16) to four columns of tensor memory, once for each of its four groups of lanes.  The descriptor: no
 // swizzle, groups of eight rows 128 bytes apart.
-template <int CTAS> __device__ __forceinline__ void ms_copy_scales(uint32_t leader, uint32_t tmem, uint32_t smem) {
+template <int CTAS> __device__ __forceinline__ void ms_copy_scales(uint32_t tmem, uint32_t smem) {
   const uint32_t low = (smem & 0x3FFFF) >> 4, high = (128u >> 4) | (1u << 14);
   if constexpr (CTAS == 1)
-    asm volatile("{\n.reg .pred q;\n.reg .b64 s;\nmov.b64 s, {%1, %2};\nsetp.ne.b32 q, %3, 0;\n@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], s;\n}\n"
-                 ::"r"(tmem), "r"(low), "r"(high), "r"(leader) : "memory");
+    asm volatile("{\n.reg .b64 s;\nmov.b64 s, {%1, %2};\ntcgen05.cp.cta_group::1.32x128b.warpx4 [%0], s;\n}\n" ::"r"(tmem), "r"(low), "r"(high) : "memory");
   else
-    asm volatile("{\n.reg .pred q;\n.reg .b64 s;\nmov.b64 s, {%1, %2};\nsetp.ne.b32 q, %3, 0;\n@q tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], s;\n}\n"
-                 ::"r"(tmem), "r"(low), "r"(high), "r"(leader) : "memory");
+    asm volatile("{\n.reg .b64 s;\nmov.b64 s, {%1, %2};\ntcgen05.cp.cta_group::2.32x128b.warpx4 [%0], s;\n}\n" ::"r"(tmem), "r"(low), "r"(high) : "memory");
 }
 // Bytes side by side in memory to shared memory (both 16-byte aligned, a multiple of 16), counted on a barrier.
 __device__ __forceinline__ void ms_bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {

@@ -254,16 +254,17 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
           asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
           const uint32_t stage = base + s * kM2Stage, scales = stage + 2 * kM2Half, columns = tmem_base + kM2ScaleCols + 48 * s;
           const uint32_t x_src = umma_low_k128(stage), w_src = x_src + (kM2Half >> 4);
+          if (leader) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            ms_copy_scales<2>(leader, columns + 4 * k, scales + kMsChunkBytes * k);
-            ms_copy_scales<2>(leader, columns + 16 + 8 * k, scales + kMsStepScales + kMsChunkBytes * k);
-            ms_copy_scales<2>(leader, columns + 20 + 8 * k, scales + 2 * kMsStepScales + kMsChunkBytes * k);
+            for (int k = 0; k < 4; ++k) {
+              ms_copy_scales<2>(columns + 4 * k, scales + kMsChunkBytes * k);
+              ms_copy_scales<2>(columns + 16 + 8 * k, scales + kMsStepScales + kMsChunkBytes * k);
+              ms_copy_scales<2>(columns + 20 + 8 * k, scales + 2 * kMsStepScales + kMsChunkBytes * k);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) ms_umma<2>(tmem_base, x_src + 2 * k, w_src + 2 * k, kM2Idesc, columns + 4 * k, columns + 16 + 8 * k, step != 0 || k != 0);
+            pair_commit_both(empty_bar(s));      // the stage is free in both blocks once these MMAs have read it
           }
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            ms_umma<2>(leader, tmem_base, x_src + 2 * k, w_src + 2 * k, kM2Idesc, columns + 4 * k, columns + 16 + 8 * k, step != 0 || k != 0);
-          if (leader) pair_commit_both(empty_bar(s));      // the stage is free in both blocks once these MMAs have read it
           __syncwarp();
           if (++s == kM2Stages) { s = 0; phase ^= 1; }
         }

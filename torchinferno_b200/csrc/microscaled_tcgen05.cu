@@ -198,12 +198,14 @@ microscaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         const uint32_t stage = base + s * S::kStage, scales = stage + kMtWBytes + NT * kMsStepBytes;
         const uint32_t w_src = umma_low_k128(stage), x_src = w_src + (kMtWBytes >> 4), columns = tmem_base + S::kScaleCols + 32 * s;
+        if (leader) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) ms_copy_scales<1>(leader, columns + 4 * k, scales + kMsChunkBytes * k);      // (four of w, four of the rows)
+          for (int k = 0; k < 8; ++k) ms_copy_scales<1>(columns + 4 * k, scales + kMsChunkBytes * k);      // (four of w, four of the rows)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          ms_umma<1>(leader, tmem_base + b * NT, w_src + 2 * k, x_src + 2 * k, idesc, columns + 4 * k, columns + 16 + 4 * k, step != step0 || k != 0);
-        if (leader) umma_commit(empty_bar(s));
+          for (int k = 0; k < 4; ++k)
+            ms_umma<1>(tmem_base + b * NT, w_src + 2 * k, x_src + 2 * k, idesc, columns + 4 * k, columns + 16 + 4 * k, step != step0 || k != 0);
+          umma_commit(empty_bar(s));
+        }
         __syncwarp();
         if (++s == a.stages) { s = 0; phase ^= 1; }
       }
