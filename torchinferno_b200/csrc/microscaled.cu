@@ -19,13 +19,13 @@ constexpr int kMsHeld = 4;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
 microscaled_rows_kernel(const T* __restrict__ x, int64_t ldx, int x_rows, unsigned char* __restrict__ codes, unsigned char* __restrict__ scales,
-                        float* __restrict__ factors, int rows, int K, int steps, const int* __restrict__ offsets, const int* __restrict__ order,
+                        float* __restrict__ factors, int rows, int K, int steps, int groups, const int* __restrict__ offsets, const int* __restrict__ order,
                         int experts, int top, int x_by_pair) {
   pdl_wait();
   pdl_trigger();
   __shared__ uint32_t scratch[32];
   const int row = blockIdx.x, runs = steps * (kMsStep / kMsRun);
-  int from = row, tile = row >> 7, at = row & 127;
+  int from = row, tile = row >> 7, group = row >> 3, at = row;      // (at: from the first row of the expert)
   if (offsets) {
     if (row >= bs_offset(offsets, experts, rows)) return;
     int lo = 0, hi = experts;      // offsets[lo] <= row < offsets[hi]
@@ -35,8 +35,9 @@ microscaled_rows_kernel(const T* __restrict__ x, int64_t ldx, int x_rows, unsign
     }
     const int first = bs_offset(offsets, lo, rows);
     if (row < first) return;       // (rows ahead of the first expert's are none's)
-    tile = ms_first_tile(first, lo) + ((row - first) >> 7);
-    at = (row - first) & 127;
+    at = row - first;
+    tile = ms_first_tile(first, lo) + (at >> 7);
+    group = ms_first_group(first, lo) + (at >> 3);
     if (x_by_pair) from = min(bs_pair(order, row, rows) / top, x_rows - 1);
   }
   const T* src = x + (size_t)from * ldx;
@@ -57,8 +58,8 @@ microscaled_rows_kernel(const T* __restrict__ x, int64_t ldx, int x_rows, unsign
   float r, inverse;
   ms_row_scale(ms_block_max(largest, scratch), r, inverse);
   if (threadIdx.x == 0) factors[row] = r;
-  unsigned char* codes_row = codes + (size_t)row * steps * kMsStepBytes;
-  unsigned char* scales_row = scales + (size_t)tile * steps * kMsStepScales + ms_scale_at(at);
+  unsigned char* codes_row = codes + (size_t)group * kMsGroupBytes;
+  unsigned char* scales_row = scales + (size_t)tile * steps * kMsStepScales + ms_scale_at(at & 127);
   auto finish = [&](int run, const uint4 (&raw)[sizeof(T)]) {      // (whole quarters of a warp: runs and block sizes are multiples of 16)
     if (run >= runs) return;
     const float t = __uint_as_float(bs_largest16<T>(raw)) * inverse;
@@ -69,7 +70,7 @@ microscaled_rows_kernel(const T* __restrict__ x, int64_t ldx, int x_rows, unsign
 #pragma unroll
     for (int j = 0; j < 8; ++j) lo[j] = v[j], hi[j] = v[8 + j];
     const uint2 c = scale == 0 ? make_uint2(0, 0) : make_uint2(ms_codes8<T>(lo, inverse, reciprocal), ms_codes8<T>(hi, inverse, reciprocal));
-    *reinterpret_cast<uint2*>(codes_row + run * (kMsRun / 2)) = c;
+    *reinterpret_cast<uint2*>(codes_row + (size_t)(run >> 4) * groups * kMsGroupBytes + ms_code_at(at & 7, (run & 15) * (kMsRun / 2))) = c;
     const uint32_t mask = 0xfu << (threadIdx.x & 28), base = threadIdx.x & 28;
     uint32_t four = 0;
 #pragma unroll
@@ -95,7 +96,7 @@ microscaled_widen_kernel(MsRows x, TO* __restrict__ out, int64_t ldo, int rows, 
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const int row = (int)(i / runs), run = (int)(i - (int64_t)row * runs);
   if (row >= rows) return;
-  const uint2 c = *reinterpret_cast<const uint2*>(x.codes + ((size_t)row * steps * kMsStepBytes + run * (kMsRun / 2)));
+  const uint2 c = *reinterpret_cast<const uint2*>(x.codes + ((size_t)(run >> 4) * x.groups + (row >> 3)) * kMsGroupBytes + ms_code_at(row & 7, (run & 15) * (kMsRun / 2)));
   const float s = ms_scale_value(x.scales[((size_t)(row >> 7) * steps * 4 + (run >> 2)) * kMsChunkBytes + ms_scale_at(row & 127) + (run & 3)]), r = x.factors[row];
   float v[16];
 #pragma unroll
@@ -135,7 +136,7 @@ TIB_API int tib_microscaled_rows(const void* x, int x_dtype, int64_t ldx, int x_
   const bool vec = ((uintptr_t)x & 15) == 0 && (ldx * (x_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
 #define TIB_MS_ROWS_GO(T, VEC)                                                                                                                           \
   TIB_LAUNCH_DEPENDENT((microscaled_rows_kernel<T, VEC>), (unsigned)rows, threads, 0, stream, (const T*)x, ldx, x_rows, (unsigned char*)codes,              \
-                       (unsigned char*)scales, factors, rows, K, steps, offsets, order, experts, top, x_by_pair)
+                       (unsigned char*)scales, factors, rows, K, steps, ms_groups(rows, offsets ? experts : 0), offsets, order, experts, top, x_by_pair)
   if (x_dtype == TIB_BF16) {
     if (vec) TIB_MS_ROWS_GO(__nv_bfloat16, true);
     else TIB_MS_ROWS_GO(__nv_bfloat16, false);
@@ -156,7 +157,7 @@ TIB_API int tib_microscaled_widen(const void* codes, const void* scales, const f
   if (((uintptr_t)codes | (uintptr_t)scales) & 15) return TIB_E_ALIGN;
   const int64_t grid = ceil_div64((int64_t)rows * ceil_div(K, kMsRun), 256);
   if (grid > 0x7fffffff) return TIB_E_SIZE;
-  const MsRows r{(const unsigned char*)codes, (const unsigned char*)scales, factors};
+  const MsRows r{(const unsigned char*)codes, (const unsigned char*)scales, factors, ms_groups(rows, 0)};
   const int wide = ((uintptr_t)out & 15) == 0 && (ldo * (out_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
   if (out_dtype == TIB_BF16) TIB_LAUNCH_DEPENDENT(microscaled_widen_kernel<__nv_bfloat16>, (unsigned)grid, 256, 0, stream, r, (__nv_bfloat16*)out, ldo, rows, K, ms_steps(K), wide);
   else TIB_LAUNCH_DEPENDENT(microscaled_widen_kernel<float>, (unsigned)grid, 256, 0, stream, r, (float*)out, ldo, rows, K, ms_steps(K), wide);
@@ -181,7 +182,7 @@ TIB_API int tib_microscaled_product(const void* x, int x_dtype, int64_t ldx, int
     if (rc != TIB_OK) return rc;
   }
   MsArgs a;
-  a.x = MsRows{(const unsigned char*)codes, (const unsigned char*)scales, factors};
+  a.x = MsRows{(const unsigned char*)codes, (const unsigned char*)scales, factors, ms_groups(M, offsets ? experts : 0)};
   a.w = (const unsigned char*)w; a.w_scales = (const unsigned char*)w_scales; a.w_factors = w_factors;
   a.M = M; a.N = N; a.steps = ms_steps(K); a.stages = 0; a.offsets = offsets; a.order = order; a.experts = experts;
   a.limit = limit; a.alpha = alpha; a.row_scale = row_scale; a.error_word = error_word;

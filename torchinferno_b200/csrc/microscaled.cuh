@@ -3,13 +3,16 @@
 // A code is an e2m1 number (a sign, two bits of exponent, one of mantissa: 0, 1/2, 1, 3/2, 2, 3, 4, 6), two in a byte, the even column in the lower half.
 // Sixteen columns have one e4m3 scale (never negative).  A matrix [N, K] has one fp32 factor, held for each of its rows; rows x [M, K] have a power
 // of two each.  Columns are padded with zeros to whole steps of 256 (128 bytes of codes, the row of the 128-byte swizzle; four MMAs of 64 columns).
-//   codes of a matrix   [tiles of 128 rows][steps][128][128 bytes]: a step's 16 KB lie side by side in memory
-//   codes of rows       [M][steps][128 bytes]
+// Codes lie as the MMA reads them from shared memory, eight rows' 128 bytes of a step side by side, the 16-byte piece p of row i at p ^ (i % 8) (the 128-byte
+// swizzle), so that plain copies bring them.
+//   codes of a matrix   [tiles of 128 rows][steps][16 groups of 8 rows][1024 bytes]: a step's 16 KB of a tile are one copy
+//   codes of rows       [steps][groups of 8 rows][1024 bytes]: a step of neighbouring rows is one copy
 //   scales of both      [tiles of 128 rows][steps][4 chunks of 64 columns][512 bytes], row i of a tile at (i % 32) * 16 + (i / 32) * 4, a byte for each run of
 //                       16 columns: a chunk is what one tcgen05.cp of 32 x 128 bits brings to tensor memory, where lane i % 32 of column i / 32 then
 //                       holds the four scales of row i
-// The tiles of rows sorted by expert begin with the experts' first rows: expert e, whose rows begin at o_e, has the scales' tiles from
-// ceil(o_e / 128) + e on.  (o_e + n_e = o_(e + 1), so these end before the next expert's begin; all are fewer than ceil(M / 128) + experts.)
+// The groups (and the scales' tiles) of rows sorted by expert begin with the experts' first rows: expert e, whose rows begin at o_e, has those from
+// ceil(o_e / 8) + e (ceil(o_e / 128) + e) on.  (o_e + n_e = o_(e + 1), so these end before the next expert's begin; all are fewer than ceil(M / 8) +
+// experts.)
 #pragma once
 
 #include "block_scaled.cuh"
@@ -18,9 +21,14 @@
 namespace tib {
 
 constexpr int kMsRun = 16, kMsStep = 256, kMsStepBytes = 128, kMsChunkBytes = 512, kMsStepScales = 4 * kMsChunkBytes, kMsTileRows = 128;
+constexpr int kMsGroup = 8, kMsGroupBytes = kMsGroup * kMsStepBytes;
 
 static inline int ms_steps(int K) { return ceil_div(K, kMsStep); }
 __host__ __device__ __forceinline__ int ms_first_tile(int first_row, int expert) { return ((first_row + kMsTileRows - 1) >> 7) + expert; }
+__host__ __device__ __forceinline__ int ms_first_group(int first_row, int expert) { return ((first_row + kMsGroup - 1) >> 3) + expert; }
+static inline int ms_groups(int M, int experts) { return ceil_div(M, kMsGroup) + experts; }      // (experts: 0 for rows that are not sorted)
+// the place of byte b (0 .. 127) of a step of row i of a group, in the group
+__host__ __device__ __forceinline__ int ms_code_at(int i, int b) { return (i << 7) + ((((b >> 4) ^ i) << 4) | (b & 15)); }
 // the place of row i of a tile's four scales of a chunk
 __host__ __device__ __forceinline__ int ms_scale_at(int i) { return ((i & 31) << 4) + ((i >> 5) << 2); }
 
@@ -117,9 +125,10 @@ __device__ __forceinline__ void ms_bulk_load(uint32_t dst, const void* src, uint
 
 // The rows of a product: x as codes.
 struct MsRows {
-  const unsigned char* codes;      // [M, steps * 128]
+  const unsigned char* codes;      // [steps, groups, 1024]
   const unsigned char* scales;     // [tiles, steps, 2048]
   const float* factors;            // [M]
+  int groups;
 };
 
 // A product's arguments.

@@ -17,13 +17,13 @@ namespace tib {
 
 constexpr int kM2Stages = 5, kM2Threads = 384;
 constexpr uint32_t kM2Half = kMsTileRows * kMsStepBytes, kM2Stage = 2 * kM2Half + 3 * kMsStepScales;      // x, w, scales of x, of w's two tiles
-constexpr uint32_t kM2Smem = kM2Stages * kM2Stage + 1024 /* alignment */ + 256 /* barriers */ + 8 * 4096 /* outputs */;
+constexpr uint32_t kM2Smem = kM2Stages * kM2Stage + 1024 /* alignment */ + 256 /* barriers */ + 8 * 4096 /* outputs */ + 2 * 1024 /* factors */;
 constexpr int kM2MaxExperts = (kMostSmem - (int)kM2Smem) / 8 - 1;      // (two numbers each in what is left of shared memory)
 constexpr uint32_t kM2Idesc = kMsIdesc | ((256u >> 3) << 17) | ((256u >> 4) << 24);      // N = 256, M = 256 over the pair
 constexpr uint32_t kM2ScaleCols = 256;      // where the stages' scales begin in tensor memory: 16 columns of x's, 32 of w's each
 static_assert(kM2ScaleCols + 48 * kM2Stages <= 512, "tensor memory");
 
-struct M2Tile { int expert, first, rows, scale_tile, n_tile; };      // rows first .. first + rows - 1 of x (at most 256), features n_tile * 256 ..
+struct M2Tile { int expert, first, rows, group, scale_tile, n_tile; };      // rows first .. first + rows - 1 of x (at most 256), features n_tile * 256 ..
 
 // Persistent: pair p walks the tiles t = p, p + pairs, ...  Of one matrix, tile t is row tile t % m_tiles of feature tile t / m_tiles, so pairs that run
 // together share slices of w; of rows sorted by expert, feature tiles run fastest.
@@ -44,7 +44,8 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
   const uint32_t rank = cluster_rank();                    // 0: the even block of the pair, which issues the MMAs
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int n_tiles = (a.N + 255) >> 8;
-  int* tiles_before = reinterpret_cast<int*>(smem_raw + (bars - smem_u32(smem_raw)) + 256 + 8 * 4096);      // [experts + 1] where rows are sorted, and
+  float* tile_factors = reinterpret_cast<float*>(smem_raw + (bars - smem_u32(smem_raw)) + 256 + 8 * 4096);  // [2][256] the features', of two tiles in turn
+  int* tiles_before = reinterpret_cast<int*>(tile_factors + 512);                                           // [experts + 1] where rows are sorted, and
   int* first_row = tiles_before + a.experts + 1;                                                            // [experts + 1] their offsets
 
   if (threadIdx.x == 0) {
@@ -91,6 +92,7 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
       m.first = (t - m.n_tile * m_tiles) * 256;
       m.rows = min(256, a.M - m.first);
       m.scale_tile = m.first >> 7;
+      m.group = m.first >> 3;
       return m;
     }
     const int row_tile = t / n_tiles;
@@ -105,24 +107,27 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
     m.first = first_row[lo] + j * 256;
     m.rows = min(256, first_row[lo + 1] - m.first);
     m.scale_tile = ms_first_tile(first_row[lo], lo) + 2 * j;
+    m.group = ms_first_group(first_row[lo], lo) + 32 * j;
     return m;
   };
 
   if (warp >= 4) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;\n");
-    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const int quarter = warp & 3, half = (warp - 4) >> 2, et = threadIdx.x - 128;
     uint32_t acc_phase = 0;
-    for (int t = pair; t < num_tiles; t += pairs) {
+    bool ok = true;
+    for (int t = pair; t < num_tiles; t += pairs, acc_phase ^= 1) {
       const M2Tile m = tile_of(t);
       const int in_tile = (int)rank * 128 + quarter * 32 + lane, row = m.first + in_tile, last = m.first + m.rows;      // (rows from `last` on are not stored)
       const int col0 = m.n_tile * 256 + half * 128;
       const float x_factor = a.x.factors[min(row, last - 1)], pair_factor = a.row_scale ? a.row_scale[bs_pair(a.order, min(row, last - 1), a.M)] : 1.f;
-      const float* w_factors = a.w_factors + (size_t)m.expert * a.N;
-      if (!mbar_wait_warp(acc_full_bar, acc_phase)) {
+      tile_factors[acc_phase * 256 + et] = a.w_factors[(size_t)m.expert * a.N + min(m.n_tile * 256 + et, a.N - 1)];
+      asm volatile("bar.sync 1, 256;\n" ::: "memory");      // (the last tile but one is finished: its factors have been read)
+      if (ok && !mbar_wait_warp(acc_full_bar, acc_phase)) {
         if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00F3);
-        break;
+        ok = false;
       }
-      acc_phase ^= 1;
+      if (!ok) continue;
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
       uint32_t v[4][32];
       const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128;
@@ -133,6 +138,20 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
       __syncwarp();
       // (what this orders is the reading of tensor memory, which tcgen05.fence has ordered: no fence of the cluster)
       if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(map_to_cta(acc_empty_bar, 0)) : "memory");
+      f32x2 sum[64];
+      const f32x2 x_factor2 = f2_pack(x_factor, x_factor);
+      const ulonglong2* factors2 = reinterpret_cast<const ulonglong2*>(tile_factors + acc_phase * 256 + half * 128);
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) {      // (see ms_scaled)
+        const ulonglong2 f = factors2[c >> 1];
+        sum[c] = f2_mul(f2_mul(f2_pack(__uint_as_float(v[c >> 4][2 * c & 31]), __uint_as_float(v[c >> 4][(2 * c & 31) + 1])), f.x), x_factor2);
+        sum[c + 1] = f2_mul(f2_mul(f2_pack(__uint_as_float(v[c >> 4][(2 * c & 31) + 2]), __uint_as_float(v[c >> 4][(2 * c & 31) + 3])), f.y), x_factor2);
+      }
+      if (a.row_scale) {
+        const f32x2 pair_factor2 = f2_pack(pair_factor, pair_factor);
+#pragma unroll
+        for (int c = 0; c < 64; ++c) sum[c] = f2_mul(sum[c], pair_factor2);
+      }
       // A row's outputs lie in one thread: a warp's 32 rows cross its 4 KB of shared memory, 128 bytes of each at a time (16-byte pieces, swizzled by row),
       // and leave as whole lines.
       constexpr int kOut = kGated ? 64 : 128, kVec = 16 / sizeof(TO), kTurn = 8 * kVec;      // outputs of a thread, a piece, a turn
@@ -146,10 +165,10 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
           float y[kVec];
 #pragma unroll
           for (int j = 0; j < kVec; ++j) {
-            const int c = (turn * kTurn + p * kVec + j) << kGated;
-            auto scaled = [&](int i) { return ms_scaled(__uint_as_float(v[i >> 5][i & 31]), w_factors[min(col0 + i, a.N - 1)], x_factor, pair_factor); };
-            if constexpr (kGated) y[j] = bs_gated<ACT>(scaled(c), scaled(c + 1), a.limit, a.alpha);
-            else y[j] = bs_act<ACT>(scaled(c));
+            const int c = turn * kTurn + p * kVec + j;
+            float lo, hi;
+            f2_unpack(sum[kGated ? c : c >> 1], lo, hi);
+            y[j] = kGated ? bs_gated<ACT>(lo, hi, a.limit, a.alpha) : bs_act<ACT>(c & 1 ? hi : lo);
           }
           uint4 w;
           if constexpr (sizeof(TO) == 2) {
@@ -202,7 +221,7 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
       bool ok = true;
       for (int t = pair; t < num_tiles && ok; t += pairs) {
         const M2Tile m = tile_of(t);
-        const int m0 = m.first + (int)rank * 128;          // (behind the tile's rows come others', which are not stored, or zeros)
+        const int group = m.group + (int)rank * 16;        // (behind the tile's rows come others', which are not stored, or zeros)
         const int blocks = (a.N + 127) >> 7;
         // (a pair's second tile of features may lie behind the matrix: it reads the last one instead, which is not stored)
         auto w_at = [&](int tile) { return (m.expert * blocks + min(tile, blocks - 1)) * a.steps; };
@@ -216,8 +235,8 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
           if (leader) {
             if (rank == 0) mbar_expect_tx(full_bar(s), 2 * kM2Stage);
             const uint32_t bar0 = map_to_cta(full_bar(s), 0), stage = base + s * kM2Stage, scales = stage + 2 * kM2Half;
-            pair_tma_load(stage, &map_x, step * kMsStepBytes, m0, bar0);
-            pair_tma_load(stage + kM2Half, &map_w, 0, (w0 + step) << 7, bar0);
+            pair_tma_load(stage, &map_x, 0, step * a.x.groups + group, bar0);
+            pair_tma_load(stage + kM2Half, &map_w, 0, (w0 + step) << 4, bar0);
             pair_tma_load(scales, &map_xs, 0, ((m.scale_tile + (int)rank) * a.steps + step) << 2, bar0);
             pair_tma_load(scales + kMsStepScales, &map_ws, 0, (s0 + step) << 2, bar0);
             pair_tma_load(scales + 2 * kMsStepScales, &map_ws, 0, (s1 + step) << 2, bar0);
@@ -282,13 +301,13 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
   }
 }
 
-// Scales as chunks of 512 bytes, read four at a time.
-static int m2_scales_map(CUtensorMap* map, const void* ptr, int64_t tiles, int steps) {
+// Pieces of so many bytes (at most 1024) side by side in memory, read so many at a time.
+static int m2_map(CUtensorMap* map, const void* ptr, int64_t pieces, int bytes, int at_a_time) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return TIB_E_ARG;
-  const cuuint64_t dims[2] = {kMsChunkBytes / 4, (cuuint64_t)(tiles * steps * 4)};
-  const cuuint64_t strides[1] = {kMsChunkBytes};
-  const cuuint32_t box[2] = {kMsChunkBytes / 4, 4};
+  const cuuint64_t dims[2] = {(cuuint64_t)bytes / 4, (cuuint64_t)pieces};
+  const cuuint64_t strides[1] = {(cuuint64_t)bytes};
+  const cuuint32_t box[2] = {(cuuint32_t)bytes / 4, (cuuint32_t)at_a_time};
   const cuuint32_t elem[2] = {1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -327,14 +346,13 @@ bool tib::ms_on_pairs_of_sms(int M, int N, int experts) {
 }
 
 int tib::ms_product_2cta(const MsArgs& a, int act, void* out, int out_dtype, int64_t ldo, cudaStream_t stream) {
-  if ((int64_t)a.experts * ceil_div(a.N, 128) * a.steps > (0x7fffffff >> 7)) return TIB_E_SIZE;
-  const int64_t tiles = ceil_div(a.M, 128) + (a.offsets ? a.experts : 0);
-  if (tiles * a.steps > (0x7fffffff >> 2)) return TIB_E_SIZE;
+  const int64_t w_steps = (int64_t)a.experts * ceil_div(a.N, 128) * a.steps, x_tiles = ceil_div(a.M, 128) + (a.offsets ? a.experts : 0);
+  if (w_steps > (0x7fffffff >> 4) || (int64_t)a.x.groups * a.steps > 0x7fffffff || x_tiles * a.steps > (0x7fffffff >> 2)) return TIB_E_SIZE;
   CUtensorMap maps[4];
-  int rc = bs_make_map(&maps[0], a.x.codes, a.M, (int64_t)a.steps * kMsStepBytes, 128);
-  if (rc == TIB_OK) rc = bs_make_map(&maps[1], a.w, (int64_t)a.experts * ceil_div(a.N, 128) * a.steps * 128, kMsStepBytes, 128);
-  if (rc == TIB_OK) rc = m2_scales_map(&maps[2], a.x.scales, tiles, a.steps);
-  if (rc == TIB_OK) rc = m2_scales_map(&maps[3], a.w_scales, (int64_t)a.experts * ceil_div(a.N, 128), a.steps);
+  int rc = m2_map(&maps[0], a.x.codes, (int64_t)a.x.groups * a.steps, kMsGroupBytes, 16);
+  if (rc == TIB_OK) rc = m2_map(&maps[1], a.w, w_steps * 16, kMsGroupBytes, 16);
+  if (rc == TIB_OK) rc = m2_map(&maps[2], a.x.scales, x_tiles * a.steps * 4, kMsChunkBytes, 4);
+  if (rc == TIB_OK) rc = m2_map(&maps[3], a.w_scales, w_steps * 4, kMsChunkBytes, 4);
   if (rc != TIB_OK) return rc;
 #define TIB_M2_GO(ACT) \
   case ACT: return out_dtype == TIB_BF16 ? launch_m2<ACT, __nv_bfloat16>(maps, a, out, ldo, stream) : launch_m2<ACT, float>(maps, a, out, ldo, stream)

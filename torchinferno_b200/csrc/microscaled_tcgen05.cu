@@ -5,7 +5,7 @@
 // only, and the accumulator, which stays in tensor memory for the whole sum, is the transposed output (TMEM lane = feature, column = row).  A step of the loop
 // is 256 columns: the 128-byte row of the swizzle, eight copies of scales (512 bytes each) to tensor memory, four MMAs.  The scales of a stage of the
 // ring have columns of their own, so that they are free when the stage is.
-//   warp 0       producer: 16 KB of codes of w a step and 2 KB of its scales, one run of memory each; the rows' codes in boxes of 32 rows, their scales
+//   warp 0       producer: four copies a step, each of bytes that lie side by side: 16 KB of codes of w, 2 KB of its scales, the rows' codes and scales
 //   warp 1       copies scales and issues tcgen05.mma; owns the TMEM allocation
 //   the next 4   epilogue: eight rows at a time, a lane a feature, so that a warp writes 32 outputs of a row side by side; two accumulators take turns
 // A matrix of few tiles is split by steps over a cluster of up to eight blocks, whose sums meet in distributed shared memory, added in the order of the
@@ -26,7 +26,7 @@ template <int NT> struct MtShape {
 // of the sums of a shared tile: (a column's 128 / splits sums and four more, so that those that a warp writes at a time fall on all banks)
 template <int NT> __host__ __device__ constexpr int mt_red_floats(int splits) { return splits > 1 ? NT * (128 + 4 * splits) : 0; }
 
-struct MtTile { int expert, first, rows, scale_tile, feature; };
+struct MtTile { int expert, first, rows, group, scale_tile, feature; };
 
 // An output (of a gated unit: from its gate g and up u).
 template <int ACT> __device__ __forceinline__ float mt_act(float g, float u, const MsArgs& a) {
@@ -36,8 +36,7 @@ template <int ACT> __device__ __forceinline__ float mt_act(float g, float u, con
 
 template <int NT, int ACT, typename TO>
 __global__ void __launch_bounds__(kMtThreads, MtShape<NT>::kPerSm)
-microscaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ MsArgs a, TO* __restrict__ y,
-                           int64_t ldy) {
+microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y, int64_t ldy) {
   using S = MtShape<NT>;
   constexpr int kGated = moe_act_gated(ACT) ? 1 : 0;
   const int splits = (int)cluster_size(), rank = (int)cluster_rank();
@@ -60,10 +59,6 @@ microscaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
   const int cluster_id = blockIdx.x / splits, clusters = gridDim.x / splits;
   const int step0 = (int)((int64_t)a.steps * rank / splits), step1 = (int)((int64_t)a.steps * (rank + 1) / splits);
   if (warp == 0) {
-    if (lane == 0) {
-      asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map_w) : "memory");
-      asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map_x) : "memory");
-    }
     if (lane < a.stages) {
       mbar_init(full_bar(lane), 1);
       mbar_init(empty_bar(lane), 1);
@@ -113,7 +108,7 @@ microscaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
     MtTile m;
     int begin = 0, n = a.M, j = row_tile;
     m.expert = 0;
-    m.scale_tile = 0;
+    m.scale_tile = m.group = 0;
     if (a.offsets) {
       int lo = 0, hi = a.experts;                 // tiles_before[lo] <= row_tile < tiles_before[hi]
       while (hi - lo > 1) {
@@ -125,9 +120,11 @@ microscaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
       j = row_tile - tiles_before[lo];
       m.expert = lo;
       m.scale_tile = ms_first_tile(begin, lo);
+      m.group = ms_first_group(begin, lo);
     }
     m.first = begin + j * NT;
     m.rows = min(NT, n - j * NT);
+    m.group += j * (NT / kMsGroup);
     m.scale_tile += j * NT >> 7;                  // (tiles of fewer than 128 rows: the launch sees to it that there is one)
     m.feature = (t - row_tile * f_tiles) << 7;
     return m;
@@ -138,11 +135,12 @@ microscaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
     int ahead = 0, it = 0, s = 0;
     uint32_t phase = 1;
     bool ok = true;
+    auto rows_bytes = [&](const MtTile& m) { return (uint32_t)((m.rows + kMsGroup - 1) / kMsGroup) * kMsGroupBytes; };
     auto ask_w = [&](const MtTile& m, int step, int s) {
       const uint32_t stage = base + s * S::kStage;
       const int block = (m.expert * f_tiles + (m.feature >> 7)) * a.steps + step;
-      mbar_expect_tx(full_bar(s), kMtWBytes + 2 * kMsStepScales + ((m.rows + 31) >> 5) * 32 * kMsStepBytes);
-      tma_load_2d(stage, &map_w, 0, block << 7, full_bar(s));
+      mbar_expect_tx(full_bar(s), kMtWBytes + 2 * kMsStepScales + rows_bytes(m));
+      ms_bulk_load(stage, a.w + (size_t)block * kMtWBytes, kMtWBytes, full_bar(s));
       ms_bulk_load(stage + kMtWBytes + NT * kMsStepBytes, a.w_scales + (size_t)block * kMsStepScales, kMsStepScales, full_bar(s));
     };
     if (!a.offsets) {
@@ -167,9 +165,7 @@ microscaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
         }
         if (leader) {
           const uint32_t rows_at = base + s * S::kStage + kMtWBytes;
-#pragma unroll
-          for (int i = 0; i < NT / 32; ++i)       // (the last box may reach into the next tile's rows, or past the last: such columns are never stored)
-            if (32 * i < m.rows) tma_load_2d(rows_at + i * 32 * kMsStepBytes, &map_x, step * kMsStepBytes, m.first + 32 * i, full_bar(s));
+          ms_bulk_load(rows_at, a.x.codes + ((size_t)step * a.x.groups + m.group) * kMsGroupBytes, rows_bytes(m), full_bar(s));
           ms_bulk_load(rows_at + NT * kMsStepBytes + kMsStepScales, a.x.scales + ((size_t)m.scale_tile * a.steps + step) * kMsStepScales, kMsStepScales, full_bar(s));
         }
         __syncwarp();
@@ -353,7 +349,7 @@ template <int NT> static int mt_plan(int M, int N, int steps, int experts, MtPla
 static int mt_tile_rows(int M) { return M <= 32 ? 32 : 128; }
 
 template <int NT, int ACT, typename TO>
-static int launch_mt(const CUtensorMap& map_w, const CUtensorMap& map_x, MsArgs& a, void* y, int64_t ldy, cudaStream_t stream) {
+static int launch_mt(MsArgs& a, void* y, int64_t ldy, cudaStream_t stream) {
   const int experts = a.offsets ? a.experts : 0;
   MtPlan plan;
   const int rc = mt_plan<NT>(a.M, a.N, a.steps, experts, plan);
@@ -380,21 +376,21 @@ static int launch_mt(const CUtensorMap& map_w, const CUtensorMap& map_x, MsArgs&
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = dependent_launch_flag() ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kern, map_w, map_x, (const MsArgs)a, (TO*)y, ldy);
+  e = cudaLaunchKernelEx(&cfg, kern, (const MsArgs)a, (TO*)y, ldy);
   if (e != cudaSuccess) return (int)e;
   TIB_LAUNCH_CHECK();
   return TIB_OK;
 }
 
 template <int NT, typename TO>
-static int launch_mt_act(int act, const CUtensorMap& map_w, const CUtensorMap& map_x, MsArgs& a, void* y, int64_t ldy, cudaStream_t stream) {
+static int launch_mt_act(int act, MsArgs& a, void* y, int64_t ldy, cudaStream_t stream) {
   switch (act) {
-    case MOE_ACT_NONE: return launch_mt<NT, MOE_ACT_NONE, TO>(map_w, map_x, a, y, ldy, stream);
-    case MOE_ACT_RELU2: return launch_mt<NT, MOE_ACT_RELU2, TO>(map_w, map_x, a, y, ldy, stream);
-    case MOE_ACT_SILU: return launch_mt<NT, MOE_ACT_SILU, TO>(map_w, map_x, a, y, ldy, stream);
-    case MOE_ACT_GELU: return launch_mt<NT, MOE_ACT_GELU, TO>(map_w, map_x, a, y, ldy, stream);
-    case MOE_ACT_GLU_CLAMP: return launch_mt<NT, MOE_ACT_GLU_CLAMP, TO>(map_w, map_x, a, y, ldy, stream);
-    default: return launch_mt<NT, MOE_ACT_SWIGLU, TO>(map_w, map_x, a, y, ldy, stream);
+    case MOE_ACT_NONE: return launch_mt<NT, MOE_ACT_NONE, TO>(a, y, ldy, stream);
+    case MOE_ACT_RELU2: return launch_mt<NT, MOE_ACT_RELU2, TO>(a, y, ldy, stream);
+    case MOE_ACT_SILU: return launch_mt<NT, MOE_ACT_SILU, TO>(a, y, ldy, stream);
+    case MOE_ACT_GELU: return launch_mt<NT, MOE_ACT_GELU, TO>(a, y, ldy, stream);
+    case MOE_ACT_GLU_CLAMP: return launch_mt<NT, MOE_ACT_GLU_CLAMP, TO>(a, y, ldy, stream);
+    default: return launch_mt<NT, MOE_ACT_SWIGLU, TO>(a, y, ldy, stream);
   }
 }
 
@@ -403,13 +399,9 @@ static int launch_mt_act(int act, const CUtensorMap& map_w, const CUtensorMap& m
 using namespace tib;
 
 int tib::ms_product_tcgen05(MsArgs& a, int act, void* y, int y_dtype, int64_t ldy, cudaStream_t stream) {
-  if (a.experts > kMtMaxExperts || (int64_t)a.experts * ceil_div(a.N, 128) * a.steps > (0x7fffffff >> 7)) return TIB_E_SIZE;
-  CUtensorMap map_w, map_x;
-  int rc = bs_make_map(&map_w, a.w, (int64_t)a.experts * ceil_div(a.N, 128) * a.steps * 128, kMsStepBytes, 128);
-  if (rc == TIB_OK) rc = bs_make_map(&map_x, a.x.codes, a.M, (int64_t)a.steps * kMsStepBytes, 32);
-  if (rc != TIB_OK) return rc;
+  if (a.experts > kMtMaxExperts || (int64_t)a.experts * ceil_div(a.N, 128) * a.steps > 0x7fffffff) return TIB_E_SIZE;
 #define TIB_MT_GO(NT) \
-  return y_dtype == TIB_BF16 ? launch_mt_act<NT, __nv_bfloat16>(act, map_w, map_x, a, y, ldy, stream) : launch_mt_act<NT, float>(act, map_w, map_x, a, y, ldy, stream)
+  return y_dtype == TIB_BF16 ? launch_mt_act<NT, __nv_bfloat16>(act, a, y, ldy, stream) : launch_mt_act<NT, float>(act, a, y, ldy, stream)
   if (mt_tile_rows(a.M) == 32) TIB_MT_GO(32);
   TIB_MT_GO(128);
 #undef TIB_MT_GO

@@ -14,12 +14,13 @@ struct QnArgs {
   const int* rows;             // or null: every row
   const float* weight;
   void* out;                   // the normed rows [n_out, hidden], or null
-  unsigned char* codes;        // 4 bits: [n_out, steps * 128]; 8 bits: [n_out, runs * 128]
+  unsigned char* codes;        // 4 bits: [steps, groups, 1024]; 8 bits: [n_out, runs * 128]
   unsigned char* scales;       // of 4 bits
   float* factors;              // 4 bits: [n_out]; 8 bits: the scales [runs, lds]
   int64_t lds;
   int hidden;
   float eps;
+  int groups;
 };
 
 // Eight numbers to eight 8-bit codes
@@ -55,7 +56,7 @@ __device__ __forceinline__ void qn_codes8(const QnArgs& a, int row, int g, const
     four |= __shfl_xor_sync(0xffffffffu, four, 2);
     four |= __shfl_xor_sync(0xffffffffu, four, 4);
     if (g >= steps * (kMsStep / 8)) return;
-    *reinterpret_cast<uint32_t*>(a.codes + (size_t)row * steps * kMsStepBytes + g * 4) = c;
+    *reinterpret_cast<uint32_t*>(a.codes + ((size_t)(g >> 5) * a.groups + (row >> 3)) * kMsGroupBytes + ms_code_at(row & 7, (g & 31) * 4)) = c;
     if ((g & 7) == 0)
       *reinterpret_cast<uint32_t*>(a.scales + ((size_t)(row >> 7) * steps * 4 + (g >> 3)) * kMsChunkBytes + ms_scale_at(row & 127)) = four;
     if (g == 0) a.factors[row] = r;
@@ -187,7 +188,7 @@ TIB_API int tib_quantized_norm(const void* delta, const float* residual, float* 
   if (dtype != TIB_BF16 && dtype != TIB_F32) return TIB_E_DTYPE;
   if (bytes && lds < n_out) return TIB_E_SIZE;
   if (((uintptr_t)codes | (uintptr_t)scales) & 15) return TIB_E_ALIGN;
-  const QnArgs a{delta, residual, sum, rows, weight, out, (unsigned char*)codes, (unsigned char*)scales, factors, lds, hidden, eps};
+  const QnArgs a{delta, residual, sum, rows, weight, out, (unsigned char*)codes, (unsigned char*)scales, factors, lds, hidden, eps, ms_groups(n_out, 0)};
   if (dtype == TIB_BF16 && hidden % 8 == 0 && hidden <= 8192 &&
       (((uintptr_t)residual | (uintptr_t)sum | (uintptr_t)weight | (uintptr_t)out | (uintptr_t)delta) & 15) == 0) {
     const int threads = (hidden / 8 + 31) / 32 * 32;

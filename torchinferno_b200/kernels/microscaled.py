@@ -25,6 +25,7 @@ from torchinferno_b200.kernels import ops
 RUN = 16                # columns of a scale
 STEP = 256              # columns are padded to whole steps
 TILE = 128              # rows of a tile of scales
+GROUP = 8               # rows whose codes lie together
 SCALE_DTYPE = torch.float8_e4m3fn
 VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 BORDERS = (0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)       # (on a border the even code is taken: the one above 0.75, 1.75 and 3.5)
@@ -102,7 +103,7 @@ def quantize_matrix(matrix: torch.Tensor) -> MicroscaledMatrix:
 def _buffer(like: torch.Tensor, rows: int, columns: int, experts: int = 0) -> tuple[torch.Tensor, int, int]:
     """(room for the codes, scales and factors of so many rows, where in it the scales begin, where the factors); see csrc/microscaled.cuh."""
     steps = _count(columns, STEP)
-    codes, scales = rows * steps * (STEP // 2), (_count(rows, TILE) + experts) * steps * (TILE * STEP // RUN)
+    codes, scales = (_count(rows, GROUP) + experts) * steps * (GROUP * STEP // 2), (_count(rows, TILE) + experts) * steps * (TILE * STEP // RUN)
     return like.new_empty(codes + scales + 4 * rows, dtype=torch.uint8), codes, codes + scales
 
 
@@ -155,7 +156,7 @@ def add_rmsnorm(delta: torch.Tensor | None, residual: torch.Tensor, weight: torc
 
 # ------------------------------------------------------------------------------------------------ weights
 class Tiles:
-    """Matrices of one size as the kernels read them: ``codes`` [matrices, tiles of 128 rows, steps of 256 columns, 128, 128 bytes], ``scales``
+    """Matrices of one size as the kernels read them: ``codes`` [matrices, tiles of 128 rows, steps of 256 columns, 128, 128 bytes (pieces of 16 swizzled)], ``scales``
     [matrices, tiles, steps, 2048 bytes] and ``factors`` [matrices, N]; ``paired``: the matrices' rows are (gate i, up i)."""
     __slots__ = ("codes", "scales", "factors", "count", "features", "columns", "paired", "codes_at", "scales_at", "factors_at", "device_index")
 
@@ -190,10 +191,12 @@ def _laid_out(stacks: Sequence[Sequence[MicroscaledMatrix]], paired: bool) -> Ti
         codes[:, :, columns // 2] &= 15
     if int(scales.max()) > 0x7e:
         raise ValueError("the scales of a 4-bit matrix must be numbers, and none of them negative")
-    codes = codes.view(len(stacks), tiles, TILE, steps, STEP // 2).transpose(2, 3).contiguous()
+    # (piece p of 16 bytes of a step of row i: to piece p ^ (i % 8))
+    pieces = torch.arange(8, device=device) ^ (torch.arange(TILE, device=device) % 8)[:, None]
+    codes = codes.view(len(stacks), tiles, TILE, steps, 8, 16).transpose(2, 3)[:, :, :, torch.arange(TILE, device=device)[:, None], pieces].contiguous()
     # (row 32 a + b of a tile, run 4 c + d of a step: to [c][b][a][d])
     scales = scales.view(len(stacks), tiles, 4, 32, steps, 4, 4).permute(0, 1, 4, 5, 3, 2, 6).contiguous()
-    return Tiles(codes, scales.view(len(stacks), tiles, steps, -1), factors, columns, paired)
+    return Tiles(codes.view(len(stacks), tiles, steps, TILE, -1), scales.view(len(stacks), tiles, steps, -1), factors, columns, paired)
 
 
 def _product(x: "torch.Tensor | MicroscaledRows", tiles: Tiles, y: torch.Tensor, act: str, limit: float, alpha: float, offsets: int, order: int, top: int,
