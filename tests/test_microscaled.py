@@ -61,7 +61,8 @@ def test_views_of_a_weight():
     weight = MicroscaledWeight(random_matrix(300, 40, 1))
     view = weight.rows(128, 290)
     assert view.out_features == 162 and view.tiles.features == 162 and view.tiles.codes.shape[1] == 2
-    assert view.tiles.codes_at == weight.tiles.codes[:, 1].data_ptr() and view.tiles.factors_at == weight.tiles.factors[:, 128:].data_ptr()
+    tiles = weight.tiles
+    assert view.tiles.numbers[:3] == (tiles.codes[:, 1].data_ptr(), tiles.scales[:, 1].data_ptr(), tiles.factors[:, 128:].data_ptr())
     with pytest.raises(ValueError, match="inside a tile"):
         weight.rows(64, 128)
     for start, stop in ((0, 301), (5, 5), (-1, 3)):

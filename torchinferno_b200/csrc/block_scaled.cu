@@ -34,13 +34,11 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__
 // The numbers that codes stand for: a thread takes sixteen.
 template <typename TO>
 __global__ void __launch_bounds__(256)
-widen_rows_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const float* __restrict__ scales, int64_t lds, TO* __restrict__ out, int64_t ldo, int rows, int K, int wide) {
+widen_rows_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const float* __restrict__ scales, int64_t lds, TO* __restrict__ out, int64_t ldo, int K, int per_row, int wide) {
   pdl_wait();
   pdl_trigger();
-  const int parts = (K + 15) >> 4;
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int row = (int)(i / parts), col = (int)(i - (int64_t)row * parts) << 4;
-  if (row >= rows) return;
+  const int row = blockIdx.x / per_row, col = ((blockIdx.x - row * per_row) * blockDim.x + threadIdx.x) << 4;
+  if (col >= K) return;
   const uint4 c = *reinterpret_cast<const uint4*>(codes + (size_t)row * ldc + col);
   const uint32_t w[4] = {c.x, c.y, c.z, c.w};
   const float s = scales[(size_t)(col >> 7) * lds + row];
@@ -101,11 +99,12 @@ TIB_API int tib_widen_rows(const void* codes, int64_t ldc, const float* scales, 
   if (out_dtype != TIB_BF16 && out_dtype != TIB_F32) return TIB_E_DTYPE;
   if (ldc < (int64_t)ceil_div(K, kBlk) * kBlk || lds < rows) return TIB_E_SIZE;
   if (((uintptr_t)codes & 15) || ldc % 16) return TIB_E_ALIGN;
-  const int64_t grid = ceil_div64((int64_t)rows * ceil_div(K, 16), 256);
+  const int parts = ceil_div(K, 16), threads = parts >= 256 ? 256 : (parts + 31) / 32 * 32, per_row = ceil_div(parts, threads);
+  const int64_t grid = (int64_t)rows * per_row;
   if (grid > 0x7fffffff) return TIB_E_SIZE;
   const int wide = ((uintptr_t)out & 15) == 0 && (ldo * (out_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
-  if (out_dtype == TIB_BF16) TIB_LAUNCH_DEPENDENT(widen_rows_kernel<__nv_bfloat16>, (unsigned)grid, 256, 0, stream, (const uint8_t*)codes, ldc, scales, lds, (__nv_bfloat16*)out, ldo, rows, K, wide);
-  else TIB_LAUNCH_DEPENDENT(widen_rows_kernel<float>, (unsigned)grid, 256, 0, stream, (const uint8_t*)codes, ldc, scales, lds, (float*)out, ldo, rows, K, wide);
+  if (out_dtype == TIB_BF16) TIB_LAUNCH_DEPENDENT(widen_rows_kernel<__nv_bfloat16>, (unsigned)grid, threads, 0, stream, (const uint8_t*)codes, ldc, scales, lds, (__nv_bfloat16*)out, ldo, K, per_row, wide);
+  else TIB_LAUNCH_DEPENDENT(widen_rows_kernel<float>, (unsigned)grid, threads, 0, stream, (const uint8_t*)codes, ldc, scales, lds, (float*)out, ldo, K, per_row, wide);
   return TIB_OK;
 }
 

@@ -13,11 +13,10 @@ __device__ __forceinline__ uint32_t ms_block_max(uint32_t v, uint32_t* scratch) 
   return __reduce_max_sync(0xffffffffu, lane < warps ? scratch[lane] : 0u);
 }
 
-// A block takes a row, a thread runs of 16 columns of it, up to kMsHeld of which it keeps: the row's largest number has to be known before the
-// first code is.  (Wider rows are read again, from the L2.)
-constexpr int kMsHeld = 4;
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256)
+// A block takes a row, a thread runs of 16 columns of it, HELD of which it keeps: the row's largest number has to be known before the first code is.  (Wider rows
+// are read again, from the L2.)  What is held decides how many blocks an SM has, and these what is on its way.
+template <typename T, bool VEC, int HELD>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? (HELD == 1 ? 5 : HELD == 2 ? 4 : 2) : HELD == 1 ? 6 : HELD == 2 ? 5 : 4)
 microscaled_rows_kernel(const T* __restrict__ x, int64_t ldx, int x_rows, unsigned char* __restrict__ codes, unsigned char* __restrict__ scales,
                         float* __restrict__ factors, int rows, int K, int steps, int groups, const int* __restrict__ offsets, const int* __restrict__ order,
                         int experts, int top, int x_by_pair) {
@@ -41,16 +40,16 @@ microscaled_rows_kernel(const T* __restrict__ x, int64_t ldx, int x_rows, unsign
     if (x_by_pair) from = min(bs_pair(order, row, rows) / top, x_rows - 1);
   }
   const T* src = x + (size_t)from * ldx;
-  uint4 held[kMsHeld][sizeof(T)];
+  uint4 held[HELD][sizeof(T)];
   uint32_t largest = 0;
 #pragma unroll
-  for (int i = 0; i < kMsHeld; ++i) {
+  for (int i = 0; i < HELD; ++i) {
     const int run = threadIdx.x + i * blockDim.x;
     bs_ask16<T, VEC>(src + run * kMsRun, run < runs ? K - run * kMsRun : 0, held[i]);
   }
 #pragma unroll
-  for (int i = 0; i < kMsHeld; ++i) largest = max(largest, bs_largest16<T>(held[i]));
-  for (int run = threadIdx.x + kMsHeld * blockDim.x; run < runs; run += blockDim.x) {
+  for (int i = 0; i < HELD; ++i) largest = max(largest, bs_largest16<T>(held[i]));
+  for (int run = threadIdx.x + HELD * blockDim.x; run < runs; run += blockDim.x) {
     uint4 raw[sizeof(T)];
     bs_ask16<T, VEC>(src + run * kMsRun, K - run * kMsRun, raw);
     largest = max(largest, bs_largest16<T>(raw));
@@ -78,8 +77,8 @@ microscaled_rows_kernel(const T* __restrict__ x, int64_t ldx, int x_rows, unsign
     if ((threadIdx.x & 3) == 0) *reinterpret_cast<uint32_t*>(scales_row + (size_t)(run >> 2) * kMsChunkBytes) = four;
   };
 #pragma unroll
-  for (int i = 0; i < kMsHeld; ++i) finish(threadIdx.x + i * blockDim.x, held[i]);
-  for (int run = threadIdx.x + kMsHeld * blockDim.x; run < runs; run += blockDim.x) {
+  for (int i = 0; i < HELD; ++i) finish(threadIdx.x + i * blockDim.x, held[i]);
+  for (int run = threadIdx.x + HELD * blockDim.x; run < runs; run += blockDim.x) {
     uint4 raw[sizeof(T)];
     bs_ask16<T, VEC>(src + run * kMsRun, K - run * kMsRun, raw);
     finish(run, raw);
@@ -89,13 +88,11 @@ microscaled_rows_kernel(const T* __restrict__ x, int64_t ldx, int x_rows, unsign
 // The numbers that quantised rows stand for: a thread takes a run.
 template <typename TO>
 __global__ void __launch_bounds__(256)
-microscaled_widen_kernel(MsRows x, TO* __restrict__ out, int64_t ldo, int rows, int K, int steps, int wide) {
+microscaled_widen_kernel(MsRows x, TO* __restrict__ out, int64_t ldo, int K, int steps, int per_row, int wide) {
   pdl_wait();
   pdl_trigger();
-  const int runs = (K + kMsRun - 1) / kMsRun;
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int row = (int)(i / runs), run = (int)(i - (int64_t)row * runs);
-  if (row >= rows) return;
+  const int row = blockIdx.x / per_row, run = (blockIdx.x - row * per_row) * blockDim.x + threadIdx.x;
+  if (run * kMsRun >= K) return;
   const uint2 c = *reinterpret_cast<const uint2*>(x.codes + ((size_t)(run >> 4) * x.groups + (row >> 3)) * kMsGroupBytes + ms_code_at(row & 7, (run & 15) * (kMsRun / 2)));
   const float s = ms_scale_value(x.scales[((size_t)(row >> 7) * steps * 4 + (run >> 2)) * kMsChunkBytes + ms_scale_at(row & 127) + (run & 3)]), r = x.factors[row];
   float v[16];
@@ -132,11 +129,18 @@ TIB_API int tib_microscaled_rows(const void* x, int x_dtype, int64_t ldx, int x_
   if ((offsets && x_by_pair) ? !order : x_rows < rows) return TIB_E_ARG;
   if (x_dtype != TIB_BF16 && x_dtype != TIB_F32) return TIB_E_DTYPE;
   if (((uintptr_t)codes | (uintptr_t)scales) & 15) return TIB_E_ALIGN;
-  const int steps = ms_steps(K), runs = steps * (kMsStep / kMsRun), threads = runs >= 256 ? 256 : (runs + 31) / 32 * 32;
+  const int steps = ms_steps(K), runs = steps * (kMsStep / kMsRun), held = runs <= 256 ? 1 : runs <= 512 ? 2 : 4;
+  const int threads = runs >= 256 * held ? 256 : (ceil_div(runs, held) + 31) / 32 * 32;
   const bool vec = ((uintptr_t)x & 15) == 0 && (ldx * (x_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
-#define TIB_MS_ROWS_GO(T, VEC)                                                                                                                           \
-  TIB_LAUNCH_DEPENDENT((microscaled_rows_kernel<T, VEC>), (unsigned)rows, threads, 0, stream, (const T*)x, ldx, x_rows, (unsigned char*)codes,              \
+#define TIB_MS_ROWS_HELD(T, VEC, HELD)                                                                                                                      \
+  TIB_LAUNCH_DEPENDENT((microscaled_rows_kernel<T, VEC, HELD>), (unsigned)rows, threads, 0, stream, (const T*)x, ldx, x_rows, (unsigned char*)codes,          \
                        (unsigned char*)scales, factors, rows, K, steps, ms_groups(rows, offsets ? experts : 0), offsets, order, experts, top, x_by_pair)
+#define TIB_MS_ROWS_GO(T, VEC)                        \
+  do {                                                \
+    if (held == 1) TIB_MS_ROWS_HELD(T, VEC, 1);       \
+    else if (held == 2) TIB_MS_ROWS_HELD(T, VEC, 2);  \
+    else TIB_MS_ROWS_HELD(T, VEC, 4);                 \
+  } while (0)
   if (x_dtype == TIB_BF16) {
     if (vec) TIB_MS_ROWS_GO(__nv_bfloat16, true);
     else TIB_MS_ROWS_GO(__nv_bfloat16, false);
@@ -145,6 +149,7 @@ TIB_API int tib_microscaled_rows(const void* x, int x_dtype, int64_t ldx, int x_
     else TIB_MS_ROWS_GO(float, false);
   }
 #undef TIB_MS_ROWS_GO
+#undef TIB_MS_ROWS_HELD
   return TIB_OK;
 }
 
@@ -155,22 +160,23 @@ TIB_API int tib_microscaled_widen(const void* codes, const void* scales, const f
   if (!codes || !scales || !factors || !out || rows < 0 || K < 1) return TIB_E_ARG;
   if (out_dtype != TIB_BF16 && out_dtype != TIB_F32) return TIB_E_DTYPE;
   if (((uintptr_t)codes | (uintptr_t)scales) & 15) return TIB_E_ALIGN;
-  const int64_t grid = ceil_div64((int64_t)rows * ceil_div(K, kMsRun), 256);
+  const int runs = ceil_div(K, kMsRun), threads = runs >= 256 ? 256 : (runs + 31) / 32 * 32, per_row = ceil_div(runs, threads);
+  const int64_t grid = (int64_t)rows * per_row;
   if (grid > 0x7fffffff) return TIB_E_SIZE;
   const MsRows r{(const unsigned char*)codes, (const unsigned char*)scales, factors, ms_groups(rows, 0)};
   const int wide = ((uintptr_t)out & 15) == 0 && (ldo * (out_dtype == TIB_BF16 ? 2 : 4)) % 16 == 0;
-  if (out_dtype == TIB_BF16) TIB_LAUNCH_DEPENDENT(microscaled_widen_kernel<__nv_bfloat16>, (unsigned)grid, 256, 0, stream, r, (__nv_bfloat16*)out, ldo, rows, K, ms_steps(K), wide);
-  else TIB_LAUNCH_DEPENDENT(microscaled_widen_kernel<float>, (unsigned)grid, 256, 0, stream, r, (float*)out, ldo, rows, K, ms_steps(K), wide);
+  if (out_dtype == TIB_BF16) TIB_LAUNCH_DEPENDENT(microscaled_widen_kernel<__nv_bfloat16>, (unsigned)grid, threads, 0, stream, r, (__nv_bfloat16*)out, ldo, K, ms_steps(K), per_row, wide);
+  else TIB_LAUNCH_DEPENDENT(microscaled_widen_kernel<float>, (unsigned)grid, threads, 0, stream, r, (float*)out, ldo, K, ms_steps(K), per_row, wide);
   return TIB_OK;
 }
 
 // A product as its callers see it: y [M, N] (or [M, N / 2] of a gated activation) in y_dtype, row stride ldy.  codes, scales, factors: where the quantised rows
 // are, or (`make`) are put first, from rows x [x_rows, K].  w: codes, scales and factors [experts, N] of the matrices (`pairs`: of (gate, up) row pairs).
 // offsets [experts + 1], order [M], top, x_by_pair: rows sorted by expert as tib_moe_expert_product takes them; offsets null: one matrix for all rows.
-TIB_API int tib_microscaled_product(const void* x, int x_dtype, int64_t ldx, int x_rows, void* codes, void* scales, float* factors, int make, const void* w,
-                                    const void* w_scales, const float* w_factors, int pairs, void* y, int y_dtype, int64_t ldy, int M, int N, int K,
-                                    const int* offsets, const int* order, int experts, int top, int x_by_pair, int act, float limit, float alpha,
-                                    const float* row_scale, int* error_word, cudaStream_t stream) {
+TIB_API int tib_microscaled_product(const void* w, const void* w_scales, const float* w_factors, int pairs, int N, int K, int experts, const void* x, int x_dtype,
+                                    int64_t ldx, int x_rows, void* codes, void* scales, float* factors, int make, void* y, int y_dtype, int64_t ldy, int M,
+                                    const int* offsets, const int* order, int top, int x_by_pair, int act, float limit, float alpha, const float* row_scale,
+                                    int* error_word, cudaStream_t stream) {
   if (M == 0 || N == 0) return TIB_OK;
   if (!codes || !scales || !factors || !w || !w_scales || !w_factors || !y || M < 0 || N < 0 || K < 1 || experts < 1 || top < 1) return TIB_E_ARG;
   if ((offsets && !order) || (row_scale && !order)) return TIB_E_ARG;

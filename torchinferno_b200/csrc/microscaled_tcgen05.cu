@@ -52,7 +52,8 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
   static_assert(8 * (2 * kMtMaxStages + 5) + 8 <= kMtBarBytes, "the barriers' share of shared memory");
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem_gen + (tmem_slot - base));
   float* red = reinterpret_cast<float*>(smem_gen + (bars - base) + kMtBarBytes);         // [splits][NT][128 / splits + 4] sums
-  int* tiles_before = reinterpret_cast<int*>(red + mt_red_floats<NT>(splits));           // [experts + 1] where rows are sorted, and
+  float* tile_factors = red + mt_red_floats<NT>(splits);                                 // [2][NT][2] the rows' and their pairs', of two tiles in turn
+  int* tiles_before = reinterpret_cast<int*>(tile_factors + 4 * NT);                     // [experts + 1] where rows are sorted, and
   int* first_row = tiles_before + a.experts + 1;                                         // [experts + 1] their offsets
 
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -219,46 +220,41 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
       const MtTile m = tile_of(t);
       const int feature = m.feature + quarter * 32 + lane, n_out = a.N >> kGated;
       const float factor = a.w_factors[(size_t)m.expert * a.N + min(feature, a.N - 1)];
+      float2* factors = reinterpret_cast<float2*>(tile_factors) + b * NT;
+      if (et < m.rows) factors[et] = make_float2(a.x.factors[m.first + et], a.row_scale ? a.row_scale[bs_pair(a.order, m.first + et, a.M)] : 1.f);
+      asm volatile("bar.sync 1, 128;\n" ::: "memory");      // (the last tile but one is finished: its factors have been read)
       if (ok && !mbar_wait_warp(acc_full_bar(b), acc_phase)) {
         if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00E3);
         ok = false;
       }
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
       const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + b * NT;
-      auto row_factor = [&](int c, float& x, float& pair) {
-        const int row = m.first + min(c, m.rows - 1);
-        x = a.x.factors[row];
-        pair = a.row_scale ? a.row_scale[bs_pair(a.order, row, a.M)] : 1.f;
-      };
       if (splits == 1) {
 #pragma unroll 1
-        for (int q = 0; q < m.rows; q += 32) {
-          float x_factor, pair_factor;
-          row_factor(q + lane, x_factor, pair_factor);
-#pragma unroll 1
-          for (int c = q; c < min(q + 32, m.rows); c += 8) {
-            uint32_t v[8];
-            tmem_ld8(acc + c, v);
-            asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-            float s[8];
+        for (int c = 0; c < m.rows; c += 8) {
+          uint32_t v[8];
+          tmem_ld8(acc + c, v);
+          asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+          float s[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float2 f = factors[min(c + j, m.rows - 1)];
+            s[j] = ms_scaled(__uint_as_float(v[j]), factor, f.x, f.y);
+          }
+          if (!ok) continue;
+          if constexpr (kGated) {
+            // a pair of lanes has gate and up of an output: the even one finishes the even rows, the odd one the odd rows
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+              const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? s[j] : s[j + 1], 1);
+              const int row = c + j + (lane & 1);
+              const float out = lane & 1 ? mt_act<ACT>(other, s[j + 1], a) : mt_act<ACT>(s[j], other, a);
+              if (row < m.rows && feature >> 1 < n_out) y[(size_t)(m.first + row) * ldy + (feature >> 1)] = from_f32<TO>(out);
+            }
+          } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              s[j] = ms_scaled(__uint_as_float(v[j]), factor, __shfl_sync(0xffffffffu, x_factor, (c + j) & 31), __shfl_sync(0xffffffffu, pair_factor, (c + j) & 31));
-            if (!ok) continue;
-            if constexpr (kGated) {
-              // a pair of lanes has gate and up of an output: the even one finishes the even rows, the odd one the odd rows
-#pragma unroll
-              for (int j = 0; j < 8; j += 2) {
-                const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? s[j] : s[j + 1], 1);
-                const int row = c + j + (lane & 1);
-                const float out = lane & 1 ? mt_act<ACT>(other, s[j + 1], a) : mt_act<ACT>(s[j], other, a);
-                if (row < m.rows && feature >> 1 < n_out) y[(size_t)(m.first + row) * ldy + (feature >> 1)] = from_f32<TO>(out);
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (c + j < m.rows && feature < n_out) y[(size_t)(m.first + c + j) * ldy + feature] = from_f32<TO>(mt_act<ACT>(s[j], 0.f, a));
-            }
+              if (c + j < m.rows && feature < n_out) y[(size_t)(m.first + c + j) * ldy + feature] = from_f32<TO>(mt_act<ACT>(s[j], 0.f, a));
           }
         }
       }
@@ -286,21 +282,22 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
           if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00E5);
           ok = false;
         }
-        const int outs = per >> kGated, o = et & (outs - 1), f = rank * per + (o << kGated), out = (m.feature + f) >> kGated;
+        const int outs = per >> kGated, o = et & (outs - 1), f = rank * per + (o << kGated), out = (m.feature + f) >> kGated;      // (f: in the tile)
         if (!ok || out >= n_out) continue;
         const float g_factor = a.w_factors[(size_t)m.expert * a.N + m.feature + f], u_factor = kGated ? a.w_factors[(size_t)m.expert * a.N + m.feature + f + 1] : 0.f;
+#pragma unroll 4
         for (int c = et / outs; c < m.rows; c += 128 / outs) {
           const float* from = red + (size_t)c * stride + (o << kGated);
           float g = from[0], u = from[kGated];
-          for (int r = 1; r < splits; ++r) {
-            from += NT * stride;
-            g += from[0];
-            u += from[kGated];
-          }
-          float x_factor, pair_factor;
-          row_factor(c, x_factor, pair_factor);
-          g = ms_scaled(g, g_factor, x_factor, pair_factor);
-          u = ms_scaled(u, u_factor, x_factor, pair_factor);
+#pragma unroll
+          for (int r = 1; r < 8; ++r)
+            if (r < splits) {
+              g += from[r * NT * stride];
+              u += from[r * NT * stride + kGated];
+            }
+          const float2 f = factors[c];
+          g = ms_scaled(g, g_factor, f.x, f.y);
+          u = ms_scaled(u, u_factor, f.x, f.y);
           y[(size_t)(m.first + c) * ldy + out] = from_f32<TO>(mt_act<ACT>(g, u, a));
         }
       }
@@ -320,7 +317,7 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
 }
 
 template <int NT> static uint32_t mt_smem(int stages, int splits, int experts) {
-  return 1024u + stages * MtShape<NT>::kStage + kMtBarBytes + 4 * (mt_red_floats<NT>(splits) + 2 * (experts + 1));
+  return 1024u + stages * MtShape<NT>::kStage + kMtBarBytes + 4 * (mt_red_floats<NT>(splits) + 4 * NT + 2 * (experts + 1));
 }
 
 // The blocks that share a tile's steps: 8, 4 or 2 where there is room for them beside the other tiles' and the steps are enough to pay for the exchange.

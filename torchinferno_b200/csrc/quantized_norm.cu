@@ -127,7 +127,61 @@ quantized_norm_bf16x8_kernel(const QnArgs a) {
   qn_codes8<__nv_bfloat16, BYTES>(a, orow, threadIdx.x, v, r, inverse, (a.hidden + kMsStep - 1) / kMsStep);
 }
 
-// Any width, either type: the sums in add_rmsnorm_kernel's order (columns in turn), the codes eight columns a thread.
+// Any width up to 8 * 1024, either type: the sums in add_rmsnorm_kernel's order (columns in turn, so many a thread that 8 hold them), the codes eight columns a
+// thread: in between the normed row crosses shared memory.
+constexpr int kQnHeld = 8, kQnWidth = 8 * 1024;
+template <typename T, bool BYTES>
+__global__ void __launch_bounds__(1024)
+quantized_norm_held_kernel(const QnArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  extern __shared__ float normed_row[];      // [hidden rounded up to 256]
+  __shared__ float scratch[33];
+  __shared__ uint32_t scratch_max[32];
+  const int orow = blockIdx.x, srow = a.rows ? a.rows[orow] : orow;
+  const size_t at = (size_t)srow * a.hidden;
+  const T* delta = static_cast<const T*>(a.delta);
+  float h[kQnHeld];
+#pragma unroll
+  for (int i = 0; i < kQnHeld; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+    h[i] = c < a.hidden ? a.residual[at + c] : 0.f;
+    if (delta && c < a.hidden) h[i] += to_f32(delta[at + c]);
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < kQnHeld; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+    if (c >= a.hidden) break;
+    if (a.sum) a.sum[at + c] = h[i];
+    ss += h[i] * h[i];
+  }
+  const float total = block_sum(ss, scratch);
+  const float inv = rsqrtf(total / (float)a.hidden + a.eps);
+  const int steps = (a.hidden + kMsStep - 1) / kMsStep, eights = steps * (kMsStep / 8);
+  uint32_t largest = 0;
+#pragma unroll
+  for (int i = 0; i < kQnHeld; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+    if (c >= a.hidden) break;
+    const T y = from_f32<T>(h[i] * inv * a.weight[c]);
+    if (a.out) static_cast<T*>(a.out)[(size_t)orow * a.hidden + c] = y;
+    normed_row[c] = to_f32(y);
+    largest = max(largest, __float_as_uint(normed_row[c]) & 0x7fffffffu);
+  }
+  for (int c = a.hidden + threadIdx.x; c < steps * kMsStep; c += blockDim.x) normed_row[c] = 0.f;
+  float r = 1.f, inverse = 1.f;
+  if constexpr (BYTES) __syncthreads();
+  else ms_row_scale(qn_block_max(largest, scratch_max), r, inverse);      // (a barrier of the block)
+  for (int g = threadIdx.x; g < eights; g += blockDim.x) {                // (whole warps: both are multiples of 32)
+    float v[8];
+    const float4 lo = reinterpret_cast<const float4*>(normed_row)[2 * g], hi = reinterpret_cast<const float4*>(normed_row)[2 * g + 1];
+    v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+    qn_codes8<T, BYTES>(a, orow, g, v, r, inverse, steps);
+  }
+}
+
+// Wider rows: the same, with the row read again for its norm and for its codes.
 template <typename T, bool BYTES>
 __global__ void quantized_norm_kernel(const QnArgs a) {
   pdl_wait();
@@ -197,7 +251,12 @@ TIB_API int tib_quantized_norm(const void* delta, const float* residual, float* 
     return TIB_OK;
   }
   const int threads = norm_threads(hidden);
-#define TIB_QN_GO(T, BYTES) TIB_LAUNCH_DEPENDENT((quantized_norm_kernel<T, BYTES>), n_out, threads, 0, stream, a)
+  const size_t smem = (size_t)ceil_div(hidden, kMsStep) * kMsStep * sizeof(float);
+#define TIB_QN_GO(T, BYTES)                                                                                                  \
+  do {                                                                                                                       \
+    if (hidden <= kQnWidth) TIB_LAUNCH_DEPENDENT((quantized_norm_held_kernel<T, BYTES>), n_out, threads, smem, stream, a);   \
+    else TIB_LAUNCH_DEPENDENT((quantized_norm_kernel<T, BYTES>), n_out, threads, 0, stream, a);                              \
+  } while (0)
   if (dtype == TIB_BF16) {
     if (bytes) TIB_QN_GO(__nv_bfloat16, true);
     else TIB_QN_GO(__nv_bfloat16, false);

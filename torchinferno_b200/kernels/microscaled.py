@@ -15,6 +15,7 @@ There is no backward pass: this is an inference engine's weight format.
 """
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 from typing import Sequence
 
@@ -100,11 +101,13 @@ def quantize_matrix(matrix: torch.Tensor) -> MicroscaledMatrix:
 
 
 # ------------------------------------------------------------------------------------------------ rows
-def _buffer(like: torch.Tensor, rows: int, columns: int, experts: int = 0) -> tuple[torch.Tensor, int, int]:
-    """(room for the codes, scales and factors of so many rows, where in it the scales begin, where the factors); see csrc/microscaled.cuh."""
+@functools.lru_cache(maxsize=4096)
+def _sizes(rows: int, columns: int, experts: int) -> tuple[int, int, int]:
+    """(where in a buffer for so many rows' codes, scales and factors the scales begin, where the factors, its bytes); see csrc/microscaled.cuh.  (experts: 0 for
+    rows that are not sorted.)"""
     steps = _count(columns, STEP)
     codes, scales = (_count(rows, GROUP) + experts) * steps * (GROUP * STEP // 2), (_count(rows, TILE) + experts) * steps * (TILE * STEP // RUN)
-    return like.new_empty(codes + scales + 4 * rows, dtype=torch.uint8), codes, codes + scales
+    return codes, codes + scales, codes + scales + 4 * rows
 
 
 class MicroscaledRows:
@@ -112,8 +115,9 @@ class MicroscaledRows:
     __slots__ = ("buffer", "shape", "dtype", "codes_at", "scales_at", "factors_at")
 
     def __init__(self, like: torch.Tensor, rows: int, columns: int, dtype: torch.dtype) -> None:
-        self.buffer, scales, factors = _buffer(like, rows, columns)
-        self.shape, self.dtype, self.codes_at = torch.Size((rows, columns)), dtype, self.buffer.data_ptr()
+        scales, factors, size = _sizes(rows, columns, 0)
+        self.buffer = buffer = like.new_empty(size, dtype=torch.uint8)
+        self.shape, self.dtype, self.codes_at = torch.Size((rows, columns)), dtype, buffer.data_ptr()
         self.scales_at, self.factors_at = self.codes_at + scales, self.codes_at + factors
 
     @property
@@ -136,8 +140,8 @@ class MicroscaledRows:
 
 def quantize_rows(x: torch.Tensor) -> MicroscaledRows:
     """The rows ``x`` [M, K] (bfloat16 or float32, any row stride) in 4 bits; see the module's text."""
-    ops.need_rows(x, None, None, "quantize_rows")
-    rows = MicroscaledRows(x, *x.shape, x.dtype)
+    count = ops.need_rows(x, None, None, "quantize_rows")
+    rows = MicroscaledRows(x, count, x.shape[1], x.dtype)
     ops.microscaled_rows(x, rows.codes_at, rows.scales_at, rows.factors_at)
     return rows
 
@@ -158,11 +162,13 @@ def add_rmsnorm(delta: torch.Tensor | None, residual: torch.Tensor, weight: torc
 class Tiles:
     """Matrices of one size as the kernels read them: ``codes`` [matrices, tiles of 128 rows, steps of 256 columns, 128, 128 bytes (pieces of 16 swizzled)], ``scales``
     [matrices, tiles, steps, 2048 bytes] and ``factors`` [matrices, N]; ``paired``: the matrices' rows are (gate i, up i)."""
-    __slots__ = ("codes", "scales", "factors", "count", "features", "columns", "paired", "codes_at", "scales_at", "factors_at", "device_index")
+    __slots__ = ("codes", "scales", "factors", "count", "features", "columns", "paired", "device_index", "numbers")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, factors: torch.Tensor, columns: int, paired: bool) -> None:
         self.codes, self.scales, self.factors, self.count, self.features, self.columns, self.paired = codes, scales, factors, codes.shape[0], factors.shape[1], columns, paired
-        self.codes_at, self.scales_at, self.factors_at, self.device_index = codes.data_ptr(), scales.data_ptr(), factors.data_ptr(), codes.get_device()
+        self.device_index = codes.get_device()
+        # (what a product is told of them)
+        self.numbers = (codes.data_ptr(), scales.data_ptr(), factors.data_ptr(), int(paired), self.features, columns, self.count)
 
 
 def _laid_out(stacks: Sequence[Sequence[MicroscaledMatrix]], paired: bool) -> Tiles:
@@ -202,21 +208,13 @@ def _laid_out(stacks: Sequence[Sequence[MicroscaledMatrix]], paired: bool) -> Ti
 def _product(x: "torch.Tensor | MicroscaledRows", tiles: Tiles, y: torch.Tensor, act: str, limit: float, alpha: float, offsets: int, order: int, top: int,
              x_by_pair: bool, row_scale: torch.Tensor | None, error_word: torch.Tensor | None) -> None:
     if isinstance(x, MicroscaledRows):
-        ops.microscaled_product(None, x.codes_at, x.scales_at, x.factors_at, tiles, y, act, limit, alpha, offsets, order, top, x_by_pair, row_scale, error_word)
-        return
-    held, scales, factors = _buffer(x, len(y), tiles.columns, tiles.count if offsets else 0)
-    at = held.data_ptr()
-    ops.microscaled_product(x, at, at + scales, at + factors, tiles, y, act, limit, alpha, offsets, order, top, x_by_pair, row_scale, error_word)
-
-
-def _output(x: "torch.Tensor | MicroscaledRows", out: torch.Tensor | None, width: int, dtype: torch.dtype) -> torch.Tensor:
-    if dtype not in _OUT_DTYPES:
-        raise ops.KernelError(f"linear: unsupported output dtype {dtype}")
-    if out is None or out.dtype != dtype:
-        return torch.empty((len(x), width), dtype=dtype, device=x.device)
-    if out.shape != (len(x), width) or (out.stride(1) != 1 and width > 1) or out.get_device() != x.get_device():
-        raise ops.KernelError(f"linear: out is {tuple(out.shape)} on {out.device}, wanted {(len(x), width)} with unit inner stride on {x.device}")
-    return out
+        x, rows = None, (x.codes_at, x.scales_at, x.factors_at)
+    else:
+        scales, factors, size = _sizes(y.shape[0], tiles.columns, tiles.count if offsets else 0)
+        held = x.new_empty(size, dtype=torch.uint8)
+        at = held.data_ptr()
+        rows = (at, at + scales, at + factors)
+    ops.microscaled_product(tiles.numbers, x, rows, y, act, limit, alpha, offsets, order, top, x_by_pair, row_scale, error_word)
 
 
 class MicroscaledWeight:
@@ -244,7 +242,7 @@ class MicroscaledWeight:
         return self.tiles.codes.device
 
     def address(self) -> int:
-        return self.tiles.codes_at
+        return self.tiles.numbers[0]
 
     def nbytes(self) -> int:
         return self.tiles.codes.numel() + self.tiles.scales.numel() + 4 * self.tiles.factors.numel()
@@ -265,11 +263,17 @@ class MicroscaledWeight:
              error_word: torch.Tensor | None) -> torch.Tensor:
         if not isinstance(x, (torch.Tensor, MicroscaledRows)):
             raise ops.KernelError(f"linear: a 4-bit weight takes a tensor or MicroscaledRows, not {type(x).__name__}")
-        ops.need_rows(x, self.in_features, self.tiles.device_index, "linear")
-        y = _output(x, out, width, x.dtype if out_dtype is None else out_dtype)
-        if len(x):
-            _product(x, self.tiles, y, act, 0.0, 0.0, 0, 0, 1, False, None, error_word)
-        return y
+        rows = ops.need_rows(x, self.in_features, self.tiles.device_index, "linear")
+        dtype = x.dtype if out_dtype is None else out_dtype
+        if dtype not in _OUT_DTYPES:
+            raise ops.KernelError(f"linear: unsupported output dtype {dtype}")
+        if out is None or out.dtype != dtype:
+            out = (x if isinstance(x, torch.Tensor) else x.buffer).new_empty((rows, width), dtype=dtype)
+        elif out.shape != (rows, width) or (out.stride(1) != 1 and width > 1) or out.get_device() != x.get_device():
+            raise ops.KernelError(f"linear: out is {tuple(out.shape)} on {out.device}, wanted {(rows, width)} with unit inner stride on {x.device}")
+        if rows:
+            _product(x, self.tiles, out, act, 0.0, 0.0, 0, 0, 1, False, None, error_word)
+        return out
 
     def product(self, x: "torch.Tensor | MicroscaledRows", *, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
                 error_word: torch.Tensor | None = None) -> torch.Tensor:
@@ -301,7 +305,7 @@ class MicroscaledExperts:
         return self.tiles.codes.device
 
     def address(self) -> int:
-        return self.tiles.codes_at
+        return self.tiles.numbers[0]
 
     def nbytes(self) -> int:
         return self.tiles.codes.numel() + self.tiles.scales.numel() + 4 * self.tiles.factors.numel()

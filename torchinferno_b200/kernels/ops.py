@@ -1329,24 +1329,27 @@ def block_scaled_product(x: torch.Tensor | None, codes: int, make: bool, blocks,
 def microscaled_rows(x: torch.Tensor, codes: int, scales: int, factors: int) -> None:
     """Codes, scales and factors of the rows ``x``, to these addresses."""
     rows, columns = x.shape
-    _check("microscaled_rows", lib().tib_microscaled_rows(*_rows_at(x), codes, scales, factors, rows, columns, 0, 0, 1, 1, False, _stream()))
+    _check("microscaled_rows", _library.tib_microscaled_rows(x.data_ptr(), _code(x.dtype), x.stride(0), rows, codes, scales, factors, rows, columns, 0, 0, 1, 1, 0, _stream()))
 
 
 def microscaled_widen(codes: int, scales: int, factors: int, out: torch.Tensor) -> None:
     """The numbers that codes, scales and factors at these addresses stand for."""
     rows, columns = out.shape
-    _check("microscaled_widen", lib().tib_microscaled_widen(codes, scales, factors, out.data_ptr(), _code(out.dtype), out.stride(0), rows, columns, _stream()))
+    _check("microscaled_widen", _library.tib_microscaled_widen(codes, scales, factors, out.data_ptr(), _code(out.dtype), columns, rows, columns, _stream()))
 
 
-def microscaled_product(x: torch.Tensor | None, codes: int, scales: int, factors: int, tiles, y: torch.Tensor, act: str, limit: float, alpha: float, offsets: int,
-                        order: int, top: int, x_by_pair: bool, row_scale: torch.Tensor | None, error_word: torch.Tensor | None) -> None:
-    """Rows times matrices of 4-bit codes (a microscaled.Tiles), into ``y``: the rows at these addresses, where those of ``x`` are put first (None: they
-    are there).  ``offsets`` / ``order``: addresses of what sorts the rows of ``y`` by expert as in :func:`moe_expert_product`, or 0."""
-    if x is not None:
+def microscaled_product(weight: tuple, x: torch.Tensor | None, rows: tuple, y: torch.Tensor, act: str, limit: float, alpha: float, offsets: int, order: int,
+                        top: int, x_by_pair: bool, row_scale: torch.Tensor | None, error_word: torch.Tensor | None) -> None:
+    """Rows times matrices of 4-bit codes, into ``y``.  ``weight``: a microscaled.Tiles' numbers.  ``rows``: addresses of the rows' codes, scales and factors, where
+    those of ``x`` are put first (None: they are there).  ``offsets`` / ``order``: addresses of what sorts the rows of ``y`` by expert as in
+    :func:`moe_expert_product`, or 0."""
+    if x is None:
+        source = (0, BF16, 0, 0)
+    else:
+        source = (x.data_ptr(), _code(x.dtype), x.stride(0), x.shape[0])
         _counter["launches"] += 1
-    _check("microscaled_product", lib().tib_microscaled_product(
-        *_rows_at(x), codes, scales, factors, x is not None, tiles.codes_at, tiles.scales_at, tiles.factors_at, tiles.paired, y.data_ptr(), _code(y.dtype), y.stride(0),
-        len(y), tiles.features, tiles.columns, offsets, order, tiles.count, top, x_by_pair, MOE_ACT[act], limit, alpha,
+    _check("microscaled_product", _library.tib_microscaled_product(
+        *weight, *source, *rows, x is not None, y.data_ptr(), _code(y.dtype), y.stride(0), y.shape[0], offsets, order, top, x_by_pair, MOE_ACT[act], limit, alpha,
         0 if row_scale is None else row_scale.data_ptr(), 0 if error_word is None else error_word.data_ptr(), _stream()))
 
 
@@ -1362,24 +1365,34 @@ def quantized_norm(delta: torch.Tensor | None, residual: torch.Tensor, weight: t
                    out: torch.Tensor | None, new_residual: torch.Tensor | None, in_bytes: bool, count: int, codes: int, scales: int, factors: int, lds: int) -> None:
     """:func:`add_rmsnorm` whose ``count`` rows go, as codes and scales, to these addresses: ``in_bytes`` as :func:`quantize_rows` leaves them (``factors``: the scales), else
     as :func:`microscaled_rows` does."""
-    _need(residual, "residual", torch.float32), _need(weight, "weight", torch.float32)
-    if residual.dim() != 2 or not residual.shape[1] or weight.numel() != residual.shape[1]:
-        raise KernelError(f"add_rmsnorm: residual {tuple(residual.shape)} / weight {tuple(weight.shape)} do not fit")
-    device = residual.get_device()
+    shape, device = residual.shape, residual.get_device()
+    if len(shape) != 2 or not shape[1] or weight.numel() != shape[1]:
+        raise KernelError(f"add_rmsnorm: residual {tuple(shape)} / weight {tuple(weight.shape)} do not fit")
+    _need_on(residual, "residual", torch.float32, shape, device), _need_on(weight, "weight", torch.float32, weight.shape, device)
     if device != torch._C._cuda_getDevice():
         raise KernelError(f"add_rmsnorm: the residual is on cuda:{device}, the current device is cuda:{torch._C._cuda_getDevice()}")
-    if rows is not None and new_residual is not None:
-        raise KernelError("add_rmsnorm: with rows the residual is left as it is")
-    for name, t, kind, shape in (("delta", delta, dtype, residual.shape), ("rows", rows, torch.int32, (count,)), ("weight", weight, torch.float32, weight.shape),
-                                 ("out", out, dtype, (count, residual.shape[1])), ("new_residual", new_residual, torch.float32, residual.shape)):
-        if t is None:
-            continue
-        _need(t, name, kind)
-        if t.get_device() != device or t.shape != shape:
-            raise KernelError(f"add_rmsnorm: {name} is {tuple(t.shape)} on {t.device}, wanted {tuple(shape)} on {residual.device}")
-    kept = new_residual if new_residual is not None else residual if delta is not None and rows is None else None
-    _check("add_rmsnorm", lib().tib_quantized_norm(_ptr(delta), _ptr(residual), _ptr(kept), _ptr(rows), _ptr(weight), _ptr(out), in_bytes, codes, scales, factors, lds, count,
-                                                   residual.shape[1], eps, _code(dtype), _stream()))
+    if delta is not None:
+        _need_on(delta, "delta", dtype, shape, device)
+    if rows is not None:
+        _need_on(rows, "rows", torch.int32, (count,), device)
+        if new_residual is not None:
+            raise KernelError("add_rmsnorm: with rows the residual is left as it is")
+    if out is not None:
+        _need_on(out, "out", dtype, (count, shape[1]), device)
+    kept = residual if delta is not None and rows is None else None
+    if new_residual is not None:
+        kept = new_residual
+        _need_on(kept, "new_residual", torch.float32, shape, device)
+    _check("add_rmsnorm", _library.tib_quantized_norm(
+        0 if delta is None else delta.data_ptr(), residual.data_ptr(), 0 if kept is None else kept.data_ptr(), 0 if rows is None else rows.data_ptr(), weight.data_ptr(),
+        0 if out is None else out.data_ptr(), in_bytes, codes, scales, factors, lds, count, shape[1], eps, _code(dtype), _stream()))
+
+
+def _need_on(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: int) -> None:
+    if t.dtype is dtype and t.is_contiguous() and t.get_device() == device >= 0 and t.shape == shape:
+        return
+    _need(t, name, dtype)
+    raise KernelError(f"add_rmsnorm: {name} is {tuple(t.shape)} on {t.device}, wanted {tuple(shape)} on cuda:{device}")
 
 
 def glu_clamp(gate_up: torch.Tensor, out: torch.Tensor, limit: float, alpha: float) -> torch.Tensor:
