@@ -47,8 +47,9 @@ microscaled_rows_kernel(const T* __restrict__ x, int64_t ldx, int x_rows, unsign
     const int run = threadIdx.x + i * blockDim.x;
     bs_ask16<T, VEC>(src + run * kMsRun, run < runs ? K - run * kMsRun : 0, held[i]);
   }
+  uint32_t run_largest[HELD];
 #pragma unroll
-  for (int i = 0; i < HELD; ++i) largest = max(largest, bs_largest16<T>(held[i]));
+  for (int i = 0; i < HELD; ++i) largest = max(largest, run_largest[i] = bs_largest16<T>(held[i]));
   for (int run = threadIdx.x + HELD * blockDim.x; run < runs; run += blockDim.x) {
     uint4 raw[sizeof(T)];
     bs_ask16<T, VEC>(src + run * kMsRun, K - run * kMsRun, raw);
@@ -59,9 +60,9 @@ microscaled_rows_kernel(const T* __restrict__ x, int64_t ldx, int x_rows, unsign
   if (threadIdx.x == 0) factors[row] = r;
   unsigned char* codes_row = codes + (size_t)group * kMsGroupBytes;
   unsigned char* scales_row = scales + (size_t)tile * steps * kMsStepScales + ms_scale_at(at & 127);
-  auto finish = [&](int run, const uint4 (&raw)[sizeof(T)]) {      // (whole quarters of a warp: runs and block sizes are multiples of 16)
+  auto finish = [&](int run, const uint4 (&raw)[sizeof(T)], uint32_t run_largest) {      // (whole quarters of a warp: runs and block sizes are multiples of 16)
     if (run >= runs) return;
-    const float t = __uint_as_float(bs_largest16<T>(raw)) * inverse;
+    const float t = __uint_as_float(run_largest) * inverse;
     const uint32_t scale = inverse == 0.f ? 0u : ms_run_scale<T>(t);
     const float reciprocal = ms_reciprocal(ms_scale_value(scale));
     float v[16], lo[8], hi[8];
@@ -77,11 +78,11 @@ microscaled_rows_kernel(const T* __restrict__ x, int64_t ldx, int x_rows, unsign
     if ((threadIdx.x & 3) == 0) *reinterpret_cast<uint32_t*>(scales_row + (size_t)(run >> 2) * kMsChunkBytes) = four;
   };
 #pragma unroll
-  for (int i = 0; i < HELD; ++i) finish(threadIdx.x + i * blockDim.x, held[i]);
+  for (int i = 0; i < HELD; ++i) finish(threadIdx.x + i * blockDim.x, held[i], run_largest[i]);
   for (int run = threadIdx.x + HELD * blockDim.x; run < runs; run += blockDim.x) {
     uint4 raw[sizeof(T)];
     bs_ask16<T, VEC>(src + run * kMsRun, K - run * kMsRun, raw);
-    finish(run, raw);
+    finish(run, raw, bs_largest16<T>(raw));
   }
 }
 

@@ -71,18 +71,29 @@ __device__ __forceinline__ float ms_reciprocal(float s) {      // 0 for 0
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
   return s == 0.f ? 0.f : r;
 }
-// Eight numbers times `inverse` (a power of two) and `reciprocal` to eight codes, the first in the lowest four bits.
-template <typename T> __device__ __forceinline__ uint32_t ms_codes8(const float (&v)[8], float inverse, float reciprocal) {
-  const f32x2 inverse2 = f2_pack(inverse, inverse), reciprocal2 = f2_pack(reciprocal, reciprocal);
-  uint32_t codes = 0;
+// Eight numbers times `inverse` (a power of two) and `reciprocal` to eight codes, the first in the lowest four bits.  (The two factors are one where their product
+// is a normal number: but for rows whose largest number is under 2^-97.)
+template <typename T> __device__ __forceinline__ uint32_t ms_codes8(const float (&numbers)[8], float inverse, float reciprocal) {
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = ms_odd12<T>(numbers[j]);
+  if (inverse > 0x1p108f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= 0x1p32f;
+    inverse *= 0x1p-32f;
+  }
+  const f32x2 factor = f2_pack(inverse * reciprocal, inverse * reciprocal);
+  float q[8];
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {
-    float a, b;
-    f2_unpack(f2_mul(f2_mul(f2_pack(ms_odd12<T>(v[j]), ms_odd12<T>(v[j + 1])), inverse2), reciprocal2), a, b);
-    uint32_t c;
-    asm("{\n.reg .b8 b;\ncvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\ncvt.u32.u8 %0, b;\n}\n" : "=r"(c) : "f"(ms_round16(b)), "f"(ms_round16(a)));
-    codes |= c << (4 * j);
+    f2_unpack(f2_mul(f2_pack(v[j], v[j + 1]), factor), q[j], q[j + 1]);
+    q[j] = ms_round16(q[j]);
+    q[j + 1] = ms_round16(q[j + 1]);
   }
+  uint32_t codes;
+  asm("{\n.reg .b8 a, b, c, d;\ncvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\ncvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\ncvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\nmov.b32 %0, {a, b, c, d};\n}\n"
+      : "=r"(codes) : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
   return codes;
 }
 // two codes (a byte) to two floats

@@ -7,18 +7,20 @@
 // ring have columns of their own, so that they are free when the stage is.
 //   warp 0       producer: four copies a step, each of bytes that lie side by side: 16 KB of codes of w, 2 KB of its scales, the rows' codes and scales
 //   warp 1       copies scales and issues tcgen05.mma; owns the TMEM allocation
-//   the next 4   epilogue: eight rows at a time, a lane a feature, so that a warp writes 32 outputs of a row side by side; two accumulators take turns
+//   the next 4 or 8   epilogue: some rows at a time, a lane a feature, so that a warp writes 32 outputs of a row side by side; two accumulators take turns
 // A matrix of few tiles is split by steps over a cluster of up to eight blocks, whose sums meet in distributed shared memory, added in the order of the
 // steps.  Every wait is bounded and reports in error_word.
 #include "microscaled.cuh"
 
 namespace tib {
 
-constexpr int kMtMaxExperts = 1024, kMtMaxStages = 8, kMtThreads = 192;
+constexpr int kMtMaxExperts = 1024, kMtMaxStages = 8;
 constexpr uint32_t kMtWBytes = kMsTileRows * kMsStepBytes, kMtBarBytes = 256;
 
 template <int NT> struct MtShape {
   static constexpr int kPerSm = NT <= 32 ? 2 : 1;                                // blocks of an SM
+  static constexpr int kStorers = NT >= 128 ? 8 : 4, kThreads = 64 + 32 * kStorers, kCols = NT / (kStorers / 4);      // (columns of a storer)
+  static constexpr int kTurn = NT >= 128 ? 16 : 8;                               // columns that it takes at a time
   static constexpr uint32_t kTmemCols = 512 / kPerSm, kScaleCols = 2 * NT;       // two accumulators, then 32 columns of scales a stage
   static constexpr int kStages = (kTmemCols - kScaleCols) / 32 < kMtMaxStages ? (kTmemCols - kScaleCols) / 32 : kMtMaxStages;
   static constexpr uint32_t kStage = kMtWBytes + NT * kMsStepBytes + 2 * kMsStepScales;
@@ -35,7 +37,7 @@ template <int ACT> __device__ __forceinline__ float mt_act(float g, float u, con
 }
 
 template <int NT, int ACT, typename TO>
-__global__ void __launch_bounds__(kMtThreads, MtShape<NT>::kPerSm)
+__global__ void __launch_bounds__(MtShape<NT>::kThreads, MtShape<NT>::kPerSm)
 microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y, int64_t ldy) {
   using S = MtShape<NT>;
   constexpr int kGated = moe_act_gated(ACT) ? 1 : 0;
@@ -66,7 +68,7 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
     }
     if (lane < 2) {
       mbar_init(acc_full_bar(lane), 1);
-      mbar_init(acc_empty_bar(lane), 4);
+      mbar_init(acc_empty_bar(lane), S::kStorers);
     }
     if (lane == 0) mbar_init(red_bar, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -211,7 +213,7 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
       if (++b == 2) { b = 0; acc_phase ^= 1; }
     }
   } else {
-    const int quarter = warp & 3, et = threadIdx.x - 64;
+    const int quarter = warp & 3, et = threadIdx.x - 64, c0 = ((warp - 2) >> 2) * S::kCols;
     int b = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
@@ -222,30 +224,46 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
       const float factor = a.w_factors[(size_t)m.expert * a.N + min(feature, a.N - 1)];
       float2* factors = reinterpret_cast<float2*>(tile_factors) + b * NT;
       if (et < m.rows) factors[et] = make_float2(a.x.factors[m.first + et], a.row_scale ? a.row_scale[bs_pair(a.order, m.first + et, a.M)] : 1.f);
-      asm volatile("bar.sync 1, 128;\n" ::: "memory");      // (the last tile but one is finished: its factors have been read)
+      asm volatile("bar.sync 1, %0;\n" ::"r"(32 * S::kStorers) : "memory");      // (the last tile but one is finished: its factors have been read)
       if (ok && !mbar_wait_warp(acc_full_bar(b), acc_phase)) {
         if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00E3);
         ok = false;
       }
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
       const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + b * NT;
-      if (splits == 1) {
+      const int c1 = min(c0 + S::kCols, m.rows);
+      // (a turn's columns are on their way while those before are finished)
+      auto columns = [&](auto&& finish) {
+        uint32_t v[2][S::kTurn];
+        auto ask = [&](int i, int c) {
+          if constexpr (S::kTurn == 16) tmem_ld16(acc + c, v[i]);
+          else tmem_ld8(acc + c, v[i]);
+        };
+        if (c0 < c1) ask(0, c0);
 #pragma unroll 1
-        for (int c = 0; c < m.rows; c += 8) {
-          uint32_t v[8];
-          tmem_ld8(acc + c, v);
-          asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-          float s[8];
+        for (int c = c0; c < c1; c += 2 * S::kTurn) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
+          for (int i = 0; i < 2; ++i) {
+            if (c + i * S::kTurn >= c1) break;
+            asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+            if (c + (i + 1) * S::kTurn < c1) ask(i ^ 1, c + (i + 1) * S::kTurn);
+            finish(c + i * S::kTurn, v[i]);
+          }
+        }
+      };
+      if (splits == 1)
+        columns([&](int c, const uint32_t (&v)[S::kTurn]) {
+          float s[S::kTurn];
+#pragma unroll
+          for (int j = 0; j < S::kTurn; ++j) {
             const float2 f = factors[min(c + j, m.rows - 1)];
             s[j] = ms_scaled(__uint_as_float(v[j]), factor, f.x, f.y);
           }
-          if (!ok) continue;
+          if (!ok) return;
           if constexpr (kGated) {
             // a pair of lanes has gate and up of an output: the even one finishes the even rows, the odd one the odd rows
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) {
+            for (int j = 0; j < S::kTurn; j += 2) {
               const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? s[j] : s[j + 1], 1);
               const int row = c + j + (lane & 1);
               const float out = lane & 1 ? mt_act<ACT>(other, s[j + 1], a) : mt_act<ACT>(s[j], other, a);
@@ -253,25 +271,22 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
             }
           } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < S::kTurn; ++j)
               if (c + j < m.rows && feature < n_out) y[(size_t)(m.first + c + j) * ldy + feature] = from_f32<TO>(mt_act<ACT>(s[j], 0.f, a));
           }
-        }
-      }
+        });
       // Block r of a cluster finishes features r * per .. of the tile.
       const int log_splits = 31 - __clz(splits), per = 128 >> log_splits, stride = per + 4;
       if (splits > 1) {
         const int in = quarter * 32 + lane, owner = in >> (7 - log_splits);
         const uint32_t dst = map_to_cta(smem_u32(red + (size_t)rank * NT * stride + (in & (per - 1))), owner), bar = map_to_cta(red_bar, owner);
-        if (et == 0) mbar_expect_tx(red_bar, 128 * 4 * ((m.rows + 7) & ~7));      // (the stores themselves count on the owner's barrier: no fence, no arrivals)
-#pragma unroll 1
-        for (int c = 0; c < m.rows; c += 8) {
-          uint32_t v[8];
-          tmem_ld8(acc + c, v);
-          asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+        const int sent = (m.rows + 7) & ~7;
+        if (et == 0) mbar_expect_tx(red_bar, 128 * 4 * sent);      // (the stores themselves count on the owner's barrier: no fence, no arrivals)
+        columns([&](int c, const uint32_t (&v)[S::kTurn]) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) st_async_f32(dst + (c + j) * stride * 4, __uint_as_float(v[j]), bar);
-        }
+          for (int j = 0; j < S::kTurn; ++j)
+            if (j < 8 || c + j < sent) st_async_f32(dst + (c + j) * stride * 4, __uint_as_float(v[j]), bar);
+        });
       }
       asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
       __syncwarp();
@@ -286,7 +301,7 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
         if (!ok || out >= n_out) continue;
         const float g_factor = a.w_factors[(size_t)m.expert * a.N + m.feature + f], u_factor = kGated ? a.w_factors[(size_t)m.expert * a.N + m.feature + f + 1] : 0.f;
 #pragma unroll 4
-        for (int c = et / outs; c < m.rows; c += 128 / outs) {
+        for (int c = et / outs; c < m.rows; c += 32 * S::kStorers / outs) {
           const float* from = red + (size_t)c * stride + (o << kGated);
           float g = from[0], u = from[kGated];
 #pragma unroll
@@ -360,7 +375,7 @@ static int launch_mt(MsArgs& a, void* y, int64_t ldy, cudaStream_t stream) {
   if (e != cudaSuccess) return (int)e;
   if (device < 64) allowed[device] = true;
   cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(kMtThreads);
+  cfg.blockDim = dim3(MtShape<NT>::kThreads);
   cfg.dynamicSmemBytes = mt_smem<NT>(plan.stages, plan.splits, experts);
   cfg.stream = stream;
   cfg.gridDim = dim3((unsigned)plan.grid);
