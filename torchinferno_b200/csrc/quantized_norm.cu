@@ -7,6 +7,8 @@
 
 namespace tib {
 
+constexpr int kQnHeld = 8, kQnWidth = 8 * 1024;      // columns of a thread of those that norm a row, of a row that a block keeps
+
 struct QnArgs {
   const void* delta;           // [rows, hidden] in the rows' type, or null
   const float* residual;
@@ -127,9 +129,78 @@ quantized_norm_bf16x8_kernel(const QnArgs a) {
   qn_codes8<__nv_bfloat16, BYTES>(a, orow, threadIdx.x, v, r, inverse, (a.hidden + kMsStep - 1) / kMsStep);
 }
 
+// 32-bit rows of a multiple of four columns, up to 8 * 1024: four columns a load.  The sums are those of `virtuals` threads that each add up every virtuals-th column
+// (add_rmsnorm_kernel's), of which a thread is four neighbours: what is a shuffle over 1 and 2 lanes there is an addition here, what is one over 4, 8 and 16 one
+// over 1, 2 and 4.  A quarter of the threads a row is four times as many rows on an SM.
+template <bool BYTES, int HELD>
+__global__ void __launch_bounds__(256, HELD <= 4 ? 5 : 3)
+quantized_norm_f32x4_kernel(const QnArgs a, int virtuals) {
+  pdl_wait();
+  pdl_trigger();
+  extern __shared__ float normed_row[];      // [hidden rounded up to 256]
+  __shared__ float scratch[32];
+  __shared__ uint32_t scratch_max[32];
+  const int orow = blockIdx.x, srow = a.rows ? a.rows[orow] : orow, lane = threadIdx.x & 31;
+  const size_t at = (size_t)srow * a.hidden;
+  const float* delta = static_cast<const float*>(a.delta);
+  const int c0 = threadIdx.x * 4 < virtuals ? threadIdx.x * 4 : a.hidden;      // (threads beyond have no column)
+  float4 h[HELD], d[HELD];
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) {
+    const int c = c0 + i * virtuals;
+    h[i] = d[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (c < a.hidden) {
+      h[i] = *reinterpret_cast<const float4*>(a.residual + at + c);
+      if (delta) d[i] = *reinterpret_cast<const float4*>(delta + at + c);
+    }
+  }
+  float4 ss = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) {
+    const int c = c0 + i * virtuals;
+    if (c >= a.hidden) break;
+    if (delta) h[i] = make_float4(h[i].x + d[i].x, h[i].y + d[i].y, h[i].z + d[i].z, h[i].w + d[i].w);
+    if (a.sum) *reinterpret_cast<float4*>(a.sum + at + c) = h[i];
+    ss.x += h[i].x * h[i].x; ss.y += h[i].y * h[i].y; ss.z += h[i].z * h[i].z; ss.w += h[i].w * h[i].w;
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) {
+    ss.x += __shfl_xor_sync(0xffffffffu, ss.x, o);
+    ss.y += __shfl_xor_sync(0xffffffffu, ss.y, o);
+    ss.z += __shfl_xor_sync(0xffffffffu, ss.z, o);
+    ss.w += __shfl_xor_sync(0xffffffffu, ss.w, o);
+  }
+  const float part = (ss.x + ss.z) + (ss.y + ss.w);
+  if ((threadIdx.x & 7) == 0 && threadIdx.x * 4 < virtuals) scratch[threadIdx.x >> 3] = part;
+  __syncthreads();
+  const float total = warp_sum(lane < virtuals >> 5 ? scratch[lane] : 0.f);
+  const float inv = rsqrtf(total / (float)a.hidden + a.eps);
+  const int steps = (a.hidden + kMsStep - 1) / kMsStep, eights = steps * (kMsStep / 8);
+  uint32_t largest = 0;
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) {
+    const int c = c0 + i * virtuals;
+    if (c >= a.hidden) break;
+    const float4 w = *reinterpret_cast<const float4*>(a.weight + c);
+    const float4 y = make_float4(h[i].x * inv * w.x, h[i].y * inv * w.y, h[i].z * inv * w.z, h[i].w * inv * w.w);
+    if (a.out) *reinterpret_cast<float4*>(static_cast<float*>(a.out) + (size_t)orow * a.hidden + c) = y;
+    *reinterpret_cast<float4*>(normed_row + c) = y;
+    largest = max(max(max(largest, __float_as_uint(y.x) & 0x7fffffffu), max(__float_as_uint(y.y) & 0x7fffffffu, __float_as_uint(y.z) & 0x7fffffffu)), __float_as_uint(y.w) & 0x7fffffffu);
+  }
+  for (int c = a.hidden + threadIdx.x; c < steps * kMsStep; c += blockDim.x) normed_row[c] = 0.f;
+  float r = 1.f, inverse = 1.f;
+  if constexpr (BYTES) __syncthreads();
+  else ms_row_scale(qn_block_max(largest, scratch_max), r, inverse);      // (a barrier of the block)
+  for (int g = threadIdx.x; g < eights; g += blockDim.x) {                // (whole warps: both are multiples of 32)
+    float v[8];
+    const float4 lo = reinterpret_cast<const float4*>(normed_row)[2 * g], hi = reinterpret_cast<const float4*>(normed_row)[2 * g + 1];
+    v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+    qn_codes8<float, BYTES>(a, orow, g, v, r, inverse, steps);
+  }
+}
+
 // Any width up to 8 * 1024, either type: the sums in add_rmsnorm_kernel's order (columns in turn, so many a thread that 8 hold them), the codes eight columns a
 // thread: in between the normed row crosses shared memory.
-constexpr int kQnHeld = 8, kQnWidth = 8 * 1024;
 template <typename T, bool BYTES>
 __global__ void __launch_bounds__(1024)
 quantized_norm_held_kernel(const QnArgs a) {
@@ -252,6 +323,20 @@ TIB_API int tib_quantized_norm(const void* delta, const float* residual, float* 
   }
   const int threads = norm_threads(hidden);
   const size_t smem = (size_t)ceil_div(hidden, kMsStep) * kMsStep * sizeof(float);
+  if (dtype == TIB_F32 && hidden % 4 == 0 && hidden <= kQnWidth &&
+      (((uintptr_t)residual | (uintptr_t)sum | (uintptr_t)weight | (uintptr_t)out | (uintptr_t)delta) & 15) == 0) {
+    const int quarter = (threads / 4 + 31) / 32 * 32;
+#define TIB_QN_X4(BYTES, HELD) TIB_LAUNCH_DEPENDENT((quantized_norm_f32x4_kernel<BYTES, HELD>), n_out, quarter, smem, stream, a, threads)
+    if (hidden <= 4 * threads) {
+      if (bytes) TIB_QN_X4(true, 4);
+      else TIB_QN_X4(false, 4);
+    } else {
+      if (bytes) TIB_QN_X4(true, 8);
+      else TIB_QN_X4(false, 8);
+    }
+#undef TIB_QN_X4
+    return TIB_OK;
+  }
 #define TIB_QN_GO(T, BYTES)                                                                                                  \
   do {                                                                                                                       \
     if (hidden <= kQnWidth) TIB_LAUNCH_DEPENDENT((quantized_norm_held_kernel<T, BYTES>), n_out, threads, smem, stream, a);   \
