@@ -193,7 +193,7 @@ TIB_API int tib_microscaled_product(const void* w, const void* w_scales, const f
   a.w = (const unsigned char*)w; a.w_scales = (const unsigned char*)w_scales; a.w_factors = w_factors;
   a.M = M; a.N = N; a.steps = ms_steps(K); a.stages = 0; a.offsets = offsets; a.order = order; a.experts = experts;
   a.limit = limit; a.alpha = alpha; a.row_scale = row_scale; a.error_word = error_word;
-  if (ms_on_pairs_of_sms(M, N, offsets ? experts : 0)) return ms_product_2cta(a, act, y, y_dtype, ldy, stream);
+  if (ms_on_pairs_of_sms(M, N, a.steps, offsets ? experts : 0)) return ms_product_2cta(a, act, y, y_dtype, ldy, stream);
   return ms_product_tcgen05(a, act, y, y_dtype, ldy, stream);
 }
 

@@ -162,7 +162,7 @@ struct MsArgs {
 __device__ __forceinline__ float ms_scaled(float sum, float w_factor, float x_factor, float row_scale) { return sum * w_factor * x_factor * row_scale; }
 
 // Products of rows that are there as codes (microscaled_tcgen05.cu, microscaled_2cta.cu), with arguments that tib_microscaled_product has checked.
-bool ms_on_pairs_of_sms(int M, int N, int experts);
+bool ms_on_pairs_of_sms(int M, int N, int steps, int experts);
 int ms_product_2cta(const MsArgs& a, int act, void* y, int y_dtype, int64_t ldy, cudaStream_t stream);
 int ms_product_tcgen05(MsArgs& a, int act, void* y, int y_dtype, int64_t ldy, cudaStream_t stream);
 

@@ -339,10 +339,16 @@ static int launch_m2(const CUtensorMap (&maps)[4], const MsArgs& a, void* out, i
 
 using namespace tib;
 
-// Whether a product runs here (experts: 0 for one matrix).
-bool tib::ms_on_pairs_of_sms(int M, int N, int experts) {
-  if (experts) return M >= (int64_t)experts * 100 && experts <= kM2MaxExperts;
-  return M > 128 && (int64_t)ceil_div(M, 128) * ceil_div(N, 128) > 148;
+// Whether a product runs here (experts: 0 for one matrix).  Of one matrix: more than one tile of 128 rows, and enough tiles of 128 x 128 to keep pairs of SMs busy, the more
+// the longer they are.  (us, tiles of 128 / pairs: 4,096 -> 28,672 128 rows 16.9 / 19.5, 192 rows 25.8 / 20.0; 300 rows 2,048 -> 4,096 7.9 / 8.0; 1,024 rows
+// 1,024 -> 1,024 10.1 / 7.2; 4,096 -> 4,096 256 rows 10.6 / 10.3, 512 rows 10.8 / 10.4, 768 rows 15.3 / 11.0; 200 rows 2,048 -> 1,302 6.8 / 10.1; 512 rows 8,192 ->
+// 4,096 15.0 / 15.1; 14,336 -> 4,096 256 rows 16.7 / 22.3, 512 rows 21.5 / 22.7.)  Of rows by expert: from 16 an expert on, on average.  (32 experts 2,048 -> 1,024 with
+// their rows' codes, 4 choices a token: 64 tokens 14.3 / 17.0, 128 18.0 / 17.7, 256 19.4 / 18.4, 1,024 28.6 / 24.3, 2,048 44.4 / 34.0; gated 64 22.8 / 22.2, 128 27.1 / 24.3, 512
+// 39.5 / 28.3; 8 experts 1,024 -> 1,024 16 rows an expert 9.6 / 10.3.)
+constexpr int kM2ExpertRows = 16;
+bool tib::ms_on_pairs_of_sms(int M, int N, int steps, int experts) {
+  if (experts) return M >= (int64_t)experts * kM2ExpertRows && experts <= kM2MaxExperts;
+  return M > 128 && (int64_t)ceil_div(M, 128) * ceil_div(N, 128) >= (steps <= 16 ? 64 : steps <= 32 ? 128 : 149);
 }
 
 int tib::ms_product_2cta(const MsArgs& a, int act, void* out, int out_dtype, int64_t ldo, cudaStream_t stream) {

@@ -335,11 +335,15 @@ template <int NT> static uint32_t mt_smem(int stages, int splits, int experts) {
   return 1024u + stages * MtShape<NT>::kStage + kMtBarBytes + 4 * (mt_red_floats<NT>(splits) + 4 * NT + 2 * (experts + 1));
 }
 
-// The blocks that share a tile's steps: 8, 4 or 2 where there is room for them beside the other tiles' and the steps are enough to pay for the exchange.
-static int mt_splits(int64_t tiles, int steps, int blocks) {
-  if (tiles * 8 <= blocks && steps >= 32) return 8;
-  if (tiles * 4 <= blocks && steps >= 4) return 4;
-  return tiles * 2 <= blocks && steps >= 4 ? 2 : 1;
+// The blocks that share a tile's steps, where there is room for them beside the other tiles': 8, 4 or 2 if they are enough to pay for the exchange; of tiles of 128 rows, whose
+// exchange is four times as long, at most 4, and none of few steps.  (us by 1 / 2 / 4 / 8 blocks a tile: 8 rows 512 -> 1,024 2.8 / 3.2 / 3.3 / 3.3, 1,024 -> 1,024 3.2 /
+// 3.4 / 3.3 / 3.3, 2,048 -> 2,048 4.3 / 4.0 / 3.8 / 3.7, 4,096 -> 2,048 6.7 / 5.7 / 4.8 / 4.0, 4,096 -> 4,096 6.9 / 6.1 / 5.3 / 5.8, 4,096 -> 6,144 7.1 / 6.5 / 5.9 /
+// 9.4, 14,336 -> 4,096 17.8 / 13.3 / 9.5 / 9.3; 64 rows 1,024 -> 1,302 6.2 / 5.2 / 4.5 / 5.8, 4,096 -> 4,096 9.0 / 7.5 / 7.0 / 17.5; 128 rows 4,096 -> 2,048
+// 9.6 / 9.1 / 7.2 / 15.1; 333 rows 1,024 -> 1,302 6.8 / 7.6 / 7.4 / 20.9.)
+static int mt_splits(int64_t tiles, int steps, int M, int blocks) {
+  if (M > 32) return steps < (M <= 64 ? 4 : 8) ? 1 : tiles * 4 <= blocks ? 4 : tiles * 2 <= blocks ? 2 : 1;
+  if (tiles * 8 <= (steps >= 32 ? blocks : blocks / 2) && steps >= 8) return 8;
+  return steps < 4 ? 1 : tiles * 4 <= blocks ? 4 : tiles * 2 <= blocks ? 2 : 1;
 }
 
 // How a product runs: blocks in the grid, those that share a tile, steps of a block at most, stages of its ring.
@@ -348,7 +352,7 @@ template <int NT> static int mt_plan(int M, int N, int steps, int experts, MtPla
   using S = MtShape<NT>;
   constexpr int kBlocks = 148 * S::kPerSm;
   const int64_t row_tiles = experts ? M / NT + (M < experts ? M : experts) : ceil_div(M, NT), tiles = row_tiles * ceil_div(N, 128);
-  p.splits = experts ? 1 : mt_splits(tiles, steps, kBlocks);
+  p.splits = experts ? 1 : mt_splits(tiles, steps, M, kBlocks);
   if (tiles * p.splits > 0x7fffffff) return TIB_E_SIZE;
   p.grid = (int)(p.splits > 1 ? tiles * p.splits : tiles < kBlocks ? tiles : kBlocks);
   const int64_t most = (int64_t)ceil_div(steps, p.splits) * ceil_div64(tiles * p.splits, p.grid);
@@ -357,7 +361,8 @@ template <int NT> static int mt_plan(int M, int N, int steps, int experts, MtPla
   while (p.stages < S::kStages && p.stages < p.steps && mt_smem<NT>(p.stages + 1, p.splits, experts) <= (S::kPerSm > 1 ? 113u * 1024 : (uint32_t)kMostSmem)) ++p.stages;
   return TIB_OK;
 }
-// Rows of a tile: 32 where all rows are one tile, else 128 (the tiles of their scales).
+// Rows of a tile: 32 where all rows are one tile, else 128 (the tiles of their scales).  A tile's time is that of its weights: 8, 32, 33, 64 and 128 rows
+// 4,096 -> 28,672 take 12.3, 13.9, 14.3, 15.8 and 16.9 us.
 static int mt_tile_rows(int M) { return M <= 32 ? 32 : 128; }
 
 template <int NT, int ACT, typename TO>
