@@ -242,3 +242,372 @@ def test_rows_behind_the_last_expert_are_left_alone():
     x, y = rows(8, 300, 1), torch.full((8, 70), 3.0, device=DEV)
     ops.moe_expert_product(x, weight, y, offsets, order, 1, x_by_pair=False)
     assert (y[5:] == 3.0).all() and not (y[:5] == 3.0).any()
+
+
+# ------------------------------------------------------------------------------------------------ every way through the kernels
+def plan(rows, columns, features, experts=0):
+    """The library's own account of how such a product runs."""
+    import ctypes
+    found = (ctypes.c_int * 4)()
+    assert ops.lib().tib_microscaled_plan(rows, features, columns, experts, ctypes.addressof(found)) == 0
+    return tuple(found)
+
+
+def device_matrix(n, k, seed, factor=1e-3):
+    """A large matrix, made on the device."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    codes = torch.randint(0, 256, (n, (k + 1) // 2), generator=g, device=DEV, dtype=torch.uint8)
+    scales = (4.0 * torch.randn(n, -(-k // 16), generator=g, device=DEV).exp()).clamp(max=448.0)
+    return MicroscaledMatrix(codes, scales.to(torch.float8_e4m3fn), torch.tensor(factor, device=DEV), k)
+
+
+# (rows, columns, features, (rows of a tile, blocks that share it, steps of a block, stages of its ring)): rings that wrap and that do not, features that are no whole
+# tiles, columns that are no whole steps, more tiles than blocks among them.
+WAYS = [(8, 4096, 4096, (32, 4, 4, 3)), (8, 600, 38530, (32, 1, 6, 4)), (20, 2500, 19200, (32, 1, 10, 4)), (3, 8320, 4000, (32, 8, 5, 3)), (8, 900, 300, (32, 4, 1, 1)),
+        (8, 2300, 16000, (32, 2, 5, 3)), (64, 1100, 500, (128, 4, 2, 2)), (50, 8320, 9001, (128, 2, 17, 4)), (100, 2500, 19200, (128, 1, 20, 6)), (300, 8192, 1024, (128, 4, 8, 4)),
+        (333, 1000, 1302, (128, 1, 4, 4)), (1000, 300, 20000, (256, 1, 10, 5)), (700, 2600, 4001, (256, 1, 11, 5)), (2000, 128, 5000, (256, 1, 3, 5))]
+
+
+@pytest.mark.parametrize("m, k, n, way", WAYS)
+def test_every_way_of_a_product(m, k, n, way):
+    """Within the bound, with no wait run out, and the same bits again."""
+    need_gpu()
+    assert plan(m, k, n) == way
+    matrix, x = device_matrix(n, k, m), rows(m, k, n)
+    weight = MicroscaledWeight(matrix)
+    for out in (BF16, F32):
+        word = torch.zeros(1, dtype=torch.int32, device=DEV)
+        y = weight.product(x, out_dtype=out, error_word=word)
+        check(y, x, [matrix])
+        assert torch.equal(y, weight.product(x, out_dtype=out, error_word=word)) and int(word) == 0
+
+
+@pytest.mark.parametrize("m, k, n", [(8, 4096, 2400), (5, 8320, 250), (20, 2500, 9603), (50, 8320, 4501), (100, 2500, 9601), (700, 2600, 2001)])
+def test_every_way_of_a_gated_product(m, k, n):
+    need_gpu()
+    gate, up, x = device_matrix(n, k, m, 2e-5), device_matrix(n, k, m + 1, 3e-5), rows(m, k, n, spread=0.3)
+    weight = MicroscaledWeight(gate, up, epilogue="swiglu")
+    for out in (BF16, F32):
+        word = torch.zeros(1, dtype=torch.int32, device=DEV)
+        y = weight.swiglu(x, out_dtype=out, error_word=word)
+        check(y, x, [gate, up], "swiglu")
+        assert torch.equal(y, weight.swiglu(x, out_dtype=out)) and int(word) == 0
+
+
+@pytest.mark.parametrize("pairs, experts, k, n, way", [(30, 32, 2100, 2050, (32, 1, 18, 4)), (250, 32, 2100, 2050, (128, 1, 36, 6)), (3000, 240, 1100, 200, (128, 1, 20, 6)),
+                                                       (2400, 6, 1200, 2001, (256, 1, 10, 5)), (3600, 200, 300, 130, (256, 1, 6, 5)), (1500, 1024, 300, 70, (128, 1, 14, 5))])
+def test_every_way_of_experts(pairs, experts, k, n, way):
+    need_gpu()
+    assert plan(pairs, k, n, experts) == way
+    matrices = [device_matrix(n, k, e) for e in range(experts)]
+    weight = MicroscaledExperts(matrices)
+    g = torch.Generator().manual_seed(pairs)
+    ids = (torch.rand(pairs, generator=g) ** 2 * experts).long()
+    order = torch.sort(ids, stable=True).indices
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), torch.bincount(ids, minlength=experts).cumsum(0)]).to(torch.int32).to(DEV)
+    x, word = rows(pairs // 2, k, n, spread=0.5), torch.zeros(1, dtype=torch.int32, device=DEV)
+    y = torch.empty(pairs, n, device=DEV)
+    ops.moe_expert_product(x, weight, y, offsets, order.to(torch.int32).to(DEV), 2, x_by_pair=True, error_word=word)
+    again = torch.empty_like(y)
+    ops.moe_expert_product(x, weight, again, offsets, order.to(torch.int32).to(DEV), 2, x_by_pair=True, error_word=word)
+    assert torch.equal(y, again) and int(word) == 0
+    for e in range(experts):
+        at = slice(int(offsets[e]), int(offsets[e + 1]))
+        if at.start < at.stop and (experts < 100 or e % 17 == 0):
+            check(y[at], x[order[at].to(DEV) // 2], [matrices[e]])
+
+
+# ------------------------------------------------------------------------------------------------ what callers do
+def test_32_bit_rows_and_several_matrices():
+    need_gpu()
+    q, k, v = random_matrix(256, 300, 1, DEV, 1e-3), random_matrix(64, 300, 2, DEV, 0.7), random_matrix(70, 300, 3, DEV, 3e-6)
+    weight = MicroscaledWeight(q, k, v)
+    for m in (1, 40, 700):
+        x = rows(m, 300, m, F32)
+        y = gemm.linear(x, weight)
+        assert y.dtype == F32
+        for at, matrix in ((slice(0, 256), q), (slice(256, 320), k), (slice(320, 390), v)):
+            check(y[:, at], x, [matrix])
+        assert torch.equal(gemm.linear(x, weight.rows(0, 256)), y[:, :256]) and torch.equal(gemm.linear(x, weight.rows(256, 390)), y[:, 256:])
+
+
+@pytest.mark.parametrize("m", [3, 130, 300])
+def test_strided_rows_and_outputs(m):
+    need_gpu()
+    matrix = random_matrix(390, 601, 1, DEV)
+    weight, wide = MicroscaledWeight(matrix), rows(2 * m, 1500, 3)
+    for x in (wide[:m, 8:609], wide[:m, 3:604], wide[::2, 1:602], wide[:1, :601].expand(m, 601)):
+        want = gemm.linear(x.contiguous(), weight)
+        check(want, x, [matrix])
+        assert torch.equal(gemm.linear(x, weight), want)
+        for room in (torch.full((m, 500), 9.0, dtype=BF16, device=DEV), torch.full((m + 1, 397), 9.0, dtype=BF16, device=DEV)[1:]):
+            out = room[:, 3:393]
+            assert gemm.linear(x, weight, out=out).data_ptr() == out.data_ptr() and torch.equal(out, want)
+            assert (room[:, :3] == 9.0).all() and (room[:, 393:] == 9.0).all()
+
+
+@pytest.mark.parametrize("m", [5, 100, 700])
+def test_rows_that_are_not_finite_show(m):
+    need_gpu()
+    gate, up = random_matrix(200, 500, 1, DEV, 1e-4), random_matrix(200, 500, 2, DEV, 1e-4)
+    x = rows(m, 500, 3, spread=0.3)
+    x[1], x[2, 7], x[3, 499], x[m - 1, 250] = 0, float("nan"), float("inf"), -float("inf")
+    fine = [i for i in range(m) if i not in (2, 3, m - 1)]
+    for call, matrices, act in ((lambda: gemm.linear(x, MicroscaledWeight(gate)), [gate], "none"),
+                                (lambda: gemm.linear_swiglu(x, MicroscaledWeight(gate, up, epilogue="swiglu")), [gate, up], "swiglu")):
+        y = call()
+        assert y[[2, 3, m - 1]].isnan().all() and not y[1].any()
+        check(y[fine], x[fine], matrices, act)
+    for act in ("relu2", "silu", "gelu"):
+        y = torch.empty(m, 200, dtype=BF16, device=DEV)
+        ops.moe_expert_product(x, MicroscaledExperts([gate]), y, torch.tensor([0, m], dtype=torch.int32, device=DEV), torch.arange(m, dtype=torch.int32, device=DEV), 1,
+                               x_by_pair=False, act=act)
+        assert y[[2, 3, m - 1]].isnan().all() and not y[fine].isnan().any()
+
+
+def test_sizes_at_the_ends_of_the_range():
+    """Rows of the least and of the largest numbers, factors of both kinds: sums are scaled in turn, so only outputs that are beyond 32 bits are lost."""
+    need_gpu()
+    for size, factor in ((1e-37, 1e25), (2e38, 1e-30), (1e-30, 1e30), (3e38, 1e-38)):
+        for m in (2, 300):
+            x = (rows(m, 300, 5, F32, spread=0.1).clamp(-1, 1) * size)
+            matrix = random_matrix(260, 300, 6, DEV, factor)
+            check(gemm.linear(x, MicroscaledWeight(matrix)), x, [matrix])
+
+
+@pytest.mark.parametrize("m", [1, 8, 64, 100, 300])
+def test_a_row_does_not_depend_on_the_others(m):
+    need_gpu()
+    weight, x = MicroscaledWeight(random_matrix(390, 1100, 3, DEV)), rows(m, 1100, 2)
+    first = gemm.linear(x, weight)
+    assert torch.equal(first, gemm.linear(x, weight))
+    assert torch.equal(torch.roll(first, 1, 0), gemm.linear(torch.roll(x, 1, 0), weight))
+    quiet = x.clone()
+    quiet[1:] *= 1e-20
+    assert torch.equal(first[0], gemm.linear(quiet, weight)[0])
+
+
+def a_layer(seed):
+    gate, up, down = random_matrix(260, 400, seed, DEV, 1e-4), random_matrix(260, 400, seed + 1, DEV, 1e-4), random_matrix(400, 260, seed + 2, DEV, 1e-3)
+    norm = 1 + 0.1 * torch.randn(400, generator=torch.Generator().manual_seed(seed)).to(DEV)
+    return norm, MicroscaledWeight(gate, up, epilogue="swiglu"), MicroscaledWeight(down), (gate, up, down)
+
+
+@pytest.mark.parametrize("m", [1, 8, 40, 300, 700])
+def test_a_feed_forward_from_its_norm_on(m):
+    """residual + delta, the norm's rows in 4 bits, gate and up, down: each step against its definition on what the step before left."""
+    need_gpu()
+    norm, gated, down, matrices = a_layer(5)
+    delta, residual = rows(m, 400, m, spread=0.3), 2.0 * rows(m, 400, m + 1, F32, spread=0.2)
+    want, normed = residual.clone(), torch.empty(m, 400, dtype=BF16, device=DEV)
+    ops.add_rmsnorm(delta, want, norm, 1e-5, normed)
+    made = microscaled.add_rmsnorm(delta, residual, norm, 1e-5)
+    assert torch.equal(residual, want) and same(made.widened(F32), rows64(normed))
+    inner = gemm.linear_swiglu(made, gated)
+    check(inner, normed, matrices[:2], "swiglu")
+    assert torch.equal(inner, gemm.linear_swiglu(normed, gated))
+    y = gemm.linear(inner, down)
+    check(y, inner, matrices[2:])
+    # the part that a model has, as a layer calls it
+    from torchinferno_b200.parts.base import PartSpec, ResidualStream, build_part
+    part = build_part("feed_forward", PartSpec("swiglu", {"hidden_size": 400, "intermediate_size": 260}), dtype=BF16, device=torch.device(DEV))
+    part.bind(dict(zip(part.names, matrices)))
+    rms = build_part("norm", PartSpec("rmsnorm", {"width": 400, "eps": 1e-5}), dtype=BF16, device=torch.device(DEV))
+    rms.bind({"weight": norm})
+    stream = ResidualStream(2.0 * rows(m, 400, m + 1, F32, spread=0.2), BF16)
+    stream.add(delta)
+    read = stream.normed(rms, form=part.rows_form(m))
+    assert isinstance(read, microscaled.MicroscaledRows) and stream.pending is None and torch.equal(stream.residual, want)
+    assert torch.equal(part.forward(read, None), y)
+
+
+@pytest.mark.parametrize("m", [3, 8, 9, 100, 700])
+def test_8_bit_products_take_the_rows_of_a_norm(m):
+    """Codes made by the norm or by the product's own kernel are the same, so where the same kernel multiplies them (from nine rows on) the outputs are too."""
+    need_gpu()
+    g = torch.Generator().manual_seed(m)
+    matrices = [block_scaled.quantize_matrix(torch.randn(n, 400, generator=g).to(DEV) / 20) for n in (256, 100, 36)]
+    delta, residual, norm = rows(m, 400, m, spread=0.3), rows(m, 400, m + 1, F32), torch.ones(400, device=DEV)
+    normed = torch.empty(m, 400, dtype=BF16, device=DEV)
+    made = block_scaled.add_rmsnorm(delta, residual, norm, 1e-5, out=normed)
+    for weight, product in ((block_scaled.BlockScaledWeight(*matrices), gemm.linear),
+                            (block_scaled.BlockScaledWeight(matrices[0], matrices[0], epilogue="swiglu"), gemm.linear_swiglu)):
+        y, plain = product(made, weight), product(normed, weight)
+        assert y.dtype == BF16 and (torch.equal(y, plain) if m > block_scaled.FEW_ROWS else torch.allclose(y.float(), plain.float(), rtol=2.0 ** -7, atol=1e-4))
+        assert torch.equal(product(made, weight, out_dtype=F32).to(BF16), y)
+
+
+@pytest.mark.parametrize("m", [3, 100, 700])
+def test_captured_and_on_two_streams(m):
+    need_gpu()
+    norm, gated, down, _ = a_layer(11)
+    inputs = [rows(m, 400, i, spread=0.3) for i in range(4)]
+    residual = rows(m, 400, 9, F32)
+
+    def pass_of(x):
+        new = torch.empty_like(residual)
+        return gemm.linear(gemm.linear_swiglu(microscaled.add_rmsnorm(x, residual, norm, 1e-5, new_residual=new), gated), down), new
+    want = [pass_of(x) for x in inputs]
+    torch.cuda.synchronize()
+    graphs, statics = [], []
+    for i in range(2):                         # (two captured passes, replayed side by side: they share nothing but the weights)
+        x = inputs[i].clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = pass_of(x)
+        graphs.append(graph), statics.append((x, y))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for turn in range(8):
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                statics[i][0].copy_(inputs[(turn + i) % 4])
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(statics[i][1], want[(turn + i) % 4]))
+    outs = []
+    for turn in range(6):
+        with torch.cuda.stream(streams[turn % 2]):
+            outs.append(pass_of(inputs[turn % 4]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y[0], want[turn % 4][0]) for turn, y in enumerate(outs))
+
+
+def test_refusals():
+    need_gpu()
+    weight, x = MicroscaledWeight(random_matrix(100, 200, 1, DEV)), rows(4, 200, 1)
+    gated = MicroscaledWeight(random_matrix(100, 200, 1, DEV), random_matrix(100, 200, 2, DEV), epilogue="swiglu")
+    residual, ones = torch.zeros(4, 200, device=DEV), torch.ones(200, device=DEV)
+    for call in (lambda: gemm.linear(x[:, :199], weight), lambda: gemm.linear(x.half(), weight), lambda: gemm.linear(x, weight, out_dtype=torch.float16),
+                 lambda: gemm.linear(x.t().contiguous().t(), weight), lambda: gemm.linear(x[0], weight), lambda: gemm.linear_swiglu(x, weight),
+                 lambda: gemm.linear(x, weight, out=torch.empty(4, 99, dtype=BF16, device=DEV)), lambda: gemm.linear_swiglu(x.cpu(), gated),
+                 lambda: gemm.linear(x, weight, out=torch.empty(100, 4, dtype=BF16, device=DEV).t()),
+                 lambda: gemm.linear(x, MicroscaledWeight(random_matrix(100, 200, 1))), lambda: quantize_rows(x.half()), lambda: quantize_rows(x[0]),
+                 lambda: quantize_rows(x).widened(torch.float16), lambda: quantize_rows(x[:, :0]),
+                 lambda: gemm.linear(quantize_rows(x[:, :199]), weight), lambda: gemm.linear(quantize_rows(x), x),
+                 lambda: microscaled.add_rmsnorm(x, residual[:3], ones, 1e-5), lambda: microscaled.add_rmsnorm(x, residual, ones[:199], 1e-5),
+                 lambda: microscaled.add_rmsnorm(x, residual.to(BF16), ones, 1e-5), lambda: microscaled.add_rmsnorm(x, residual, ones, 1e-5, dtype=F32),
+                 lambda: microscaled.add_rmsnorm(x, residual, ones, 1e-5, out=torch.empty(4, 200, device=DEV)),
+                 lambda: microscaled.add_rmsnorm(x, residual, ones, 1e-5, new_residual=torch.empty(4, 199, device=DEV)),
+                 lambda: microscaled.add_rmsnorm(x, residual, ones, 1e-5, rows=torch.zeros(2, dtype=torch.int64, device=DEV)),
+                 lambda: microscaled.add_rmsnorm(x, residual, ones, 1e-5, rows=torch.zeros(2, dtype=torch.int32, device=DEV), new_residual=residual.clone()),
+                 lambda: block_scaled.add_rmsnorm(x.t().contiguous().t(), residual, ones, 1e-5)):
+        with pytest.raises(ops.KernelError):
+            call()
+    assert not residual.any()
+    assert gemm.linear(x[:0], weight).shape == (0, 100) and gemm.linear(quantize_rows(x[:0]), weight).shape == (0, 100)
+    assert len(microscaled.add_rmsnorm(x[:0], residual[:0], ones, 1e-5)) == 0
+
+
+def test_expert_refusals():
+    need_gpu()
+    weight = MicroscaledExperts([random_matrix(40, 100, e, DEV) for e in range(3)])
+    offsets, order = torch.tensor([0, 2, 2, 4], dtype=torch.int32, device=DEV), torch.arange(4, dtype=torch.int32, device=DEV)
+    x, y = rows(4, 100, 1), torch.empty(4, 40, device=DEV)
+
+    def call(x=x, y=y, offsets=offsets, order=order, top=1, **options):
+        return ops.moe_expert_product(x, weight, y, offsets, order, top, **{"x_by_pair": False, **options})
+    call()
+    for bad in (dict(x=rows(4, 99, 1)), dict(x=rows(3, 100, 1)), dict(y=y[:, :39]), dict(offsets=offsets[:3]), dict(offsets=offsets.long()), dict(order=order.long()), dict(top=0),
+                dict(act="swiglu"), dict(act="tanh"), dict(row_scale=torch.ones(3, device=DEV)), dict(row_scale=torch.ones(4, dtype=BF16, device=DEV)),
+                dict(x=quantize_rows(x)), dict(x=x.cpu()), dict(y=y.half()), dict(y=torch.empty(40, 4, device=DEV).t()), dict(x=rows(1, 100, 1), top=3, x_by_pair=True)):
+        with pytest.raises(ops.KernelError):
+            call(**bad)
+
+
+# ------------------------------------------------------------------------------------------------ models
+NVFP4 = {"quant_method": "modelopt", "quant_algo": "NVFP4"}
+
+
+def _engine(folder, dtype, **options):
+    from torchinferno_b200.config.engine_config import EngineConfig
+    from torchinferno_b200.engine.engine import InferenceEngine
+    return InferenceEngine.from_config(EngineConfig(model=str(folder), dtype=dtype, **options))
+
+
+def _generate(engine, prompts, tokens):
+    from torchinferno_b200.engine.types import GenerateRequest, SamplingConfig
+    return [list(o.token_ids) for o in engine.generate_many([GenerateRequest(f"g{i}", prompt_token_ids=p, sampling=SamplingConfig(tokens))
+                                                             for i, p in enumerate(prompts)])]
+
+
+@pytest.mark.parametrize("name", ["B", "D"])
+def test_a_model_in_codes(tmp_path, name):
+    """In float32 the engine gives the tokens of the numbers the codes stand for; in bfloat16 every decode step is captured, gives the same tokens as
+    uncaptured ones and run ahead or not, and its logits point where the float32 engine's do."""
+    need_gpu()
+    import numpy as np
+    import plain_llama
+    from conftest import TINY
+    from gpu_common import requests_for
+    from replay_util import InProcessReplayer, gather, trace_tail_decode
+    from torchinferno_b200.weights.random_init import write_random_model
+    config, seed = TINY[name]
+    folder = write_random_model({**config, "quantization_config": NVFP4}, tmp_path, seed)
+    cfg, stored = plain_llama.read_model_folder(folder)
+    beside = {n + suffix for n in stored for suffix in ("_scale", "_scale_2") if n + "_scale_2" in stored}
+    widened = {n: w if n + "_scale_2" not in stored else MicroscaledMatrix(w.to(torch.uint8), stored[n + "_scale"].to(torch.float8_e4m3fn),
+                                                                           stored[n + "_scale_2"].float()).widened().double()
+               for n, w in stored.items() if n not in beside}
+    wanted = requests_for(config, seed, [9, 21, 3, 14])
+    prompts = list(wanted.values())
+    with _engine(folder, "float32", page_size=16, max_batch_size=4) as engine:
+        assert _generate(engine, prompts, 8) == [plain_llama.generate_greedy(cfg, widened, p, 8) for p in prompts]
+    outs = []
+    for ahead in (True, False):
+        with _engine(folder, "bfloat16", page_size=16, max_batch_size=4, async_scheduling=ahead) as engine:
+            outs.append(_generate(engine, prompts, 12))
+            assert engine.runner.counters["graph_steps"] > 0
+    assert outs[0] == outs[1]
+    rows_by_dtype = {}
+    for dtype in ("float32", "bfloat16"):
+        steps, index = trace_tail_decode(wanted, 3)
+        rows_by_dtype[dtype] = gather(InProcessReplayer(folder, dtype, 512).run(steps), index)
+    # A number of a row is off by at most half the distance of two codes, which is a quarter of the lower one or less from 1 on: by 0.25 / sqrt(3) / 1.5 = 0.1 of it in the mean
+    # (the lower ends of the codes' intervals are off most), and so is a product.  A layer adds what four products behind one another make: gate, up and down
+    # 0.1 sqrt(3) x 1.5 (the activation's slope) = 0.26, projections in and out of attention 0.14 twice over for the softmax = 0.28; three layers:
+    # 0.38 sqrt(3) = 0.66 of the logits at the most, a cosine of 1 - 0.66^2 / 2 = 0.78.
+    pairs = [tuple(np.asarray(rows_by_dtype[d][k][0], dtype=np.float64) for d in ("float32", "bfloat16")) for k in rows_by_dtype["float32"]]
+    assert len(pairs) == 4 * 4 - 1      # (one prompt is shorter than its decoded tail)
+    cosines = [float((a * b).sum() / np.sqrt((a * a).sum() * (b * b).sum())) for a, b in pairs]
+    assert min(cosines) >= 0.78, min(cosines)
+
+
+@pytest.mark.parametrize("module, name", [("giforax_configs", "GA"), ("vofidra_configs", "VA"), ("zipedra_configs", "ZA"), ("tadalorn_configs", "TB")])
+def test_designs_with_experts_in_codes(tmp_path, module, name):
+    """Their experts are bound in codes and a random model generates: prompts in portions beside decode steps, the same tokens twice."""
+    need_gpu()
+    import importlib
+    from torchinferno_b200.weights.random_init import write_random_model
+    config, seed = importlib.import_module(module).CONFIGS[name]
+    folder = write_random_model({**config, "quantization_config": NVFP4}, tmp_path, seed)
+    g = torch.Generator().manual_seed(seed)
+    prompts = [torch.randint(0, config["vocab"], (n,), generator=g).tolist() for n in (11, 30, 2)]
+    outs = []
+    for _ in range(2):
+        with _engine(folder, "bfloat16", page_size=16, max_batch_size=4, prefill_chunk_size=16) as engine:
+            assert any(type(getattr(b.feed_forward, "up_weight", None)).__name__ == "MicroscaledExperts" for b in engine.runner.model.blocks
+                       if getattr(b, "feed_forward", None) is not None)
+            outs.append(_generate(engine, prompts, 6))
+    assert outs[0] == outs[1] and all(len(o) == 6 for o in outs[0])
+
+
+def test_a_layer_reads_its_norms_rows_in_8_bits_as_before(tmp_path, monkeypatch):
+    """A model in 8-bit blocks: the same tokens whether its norms leave codes or its products make them."""
+    need_gpu()
+    from conftest import TINY
+    from torchinferno_b200.parts import attention, mlp
+    from torchinferno_b200.weights.random_init import write_random_model
+    config, seed = TINY["B"]
+    folder = write_random_model({**config, "quantization_config": {"quant_method": "fp8", "weight_block_size": [128, 128]}}, tmp_path, seed)
+    g = torch.Generator().manual_seed(seed)
+    prompts = [torch.randint(0, config["vocab_size"], (n,), generator=g).tolist() for n in (11, 30, 200)]
+    outs = []
+    for fused in (True, False):
+        if not fused:
+            for module in (attention, mlp):
+                monkeypatch.setattr(module, "rows_form", lambda weight, count: None)
+        with _engine(folder, "bfloat16", page_size=16, max_batch_size=4) as engine:
+            outs.append(_generate(engine, prompts, 8))
+    assert outs[0] == outs[1]

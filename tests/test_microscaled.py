@@ -134,3 +134,138 @@ def test_calls_that_are_refused_without_a_gpu():
     for product in (gemm.linear, gemm.linear_swiglu):
         with pytest.raises(ops.KernelError, match="quantised rows are for quantised weights"):
             product(eight_rows, gemm.LinearWeight(torch.ones(4, 32), few_rows_tcgen05=False))
+
+
+# ------------------------------------------------------------------------------------------------ checkpoints
+NVFP4 = {"quant_method": "modelopt", "quant_algo": "NVFP4", "ignore": ["lm_head"],
+         "config_groups": {"group_0": {"weights": {"num_bits": 4, "type": "float", "group_size": 16}, "targets": ["Linear"]}}}
+
+
+def test_quantization_config():
+    from torchinferno_b200.config.model_config import ConfigError
+    from torchinferno_b200.config.quantization import BlockQuantization, MicroscaledQuantization, quantization_of
+    assert quantization_of({}) is None and quantization_of({"quantization_config": None}) is None
+    assert quantization_of({"quantization_config": {"quant_method": "modelopt", "quant_algo": "FP8"}}) is None
+    assert isinstance(quantization_of({"quantization_config": {"quant_method": "fp8", "weight_block_size": [128, 128]}}), BlockQuantization)
+    q = quantization_of({"quantization_config": {**NVFP4, "ignore": ["lm_head", "model.layers.1.mlp", "model.layers.2*", "o_proj"]}})
+    assert isinstance(q, MicroscaledQuantization)
+    assert [q.converts(n) for n in ("lm_head.weight", "model.layers.1.mlp.up_proj.weight", "model.layers.11.mlp.up_proj.weight", "model.layers.2.mlp.up_proj.weight",
+                                    "model.layers.0.self_attn.o_proj.weight", "model.layers.0.self_attn.q_proj.weight")] == [False, False, True, False, False, True]
+    for bad in ({**NVFP4, "config_groups": {"g": {"weights": {"group_size": 32}}}}, {**NVFP4, "group_size": 32}, {**NVFP4, "ignore": "lm_head"}, {**NVFP4, "ignore": [1]},
+                {**NVFP4, "config_groups": [1]}):
+        with pytest.raises(ConfigError):
+            quantization_of({"quantization_config": bad})
+
+
+def _folder(tmp_path, config, drop=(), **changes):
+    """A random model folder with these tensors changed or left out, and its tensors as they were."""
+    from safetensors.torch import load_file, save_file
+    from torchinferno_b200.weights.random_init import write_random_model
+    write_random_model(config, tmp_path, seed=0)
+    tensors = {k: v.clone() for k, v in load_file(str(tmp_path / "model.safetensors")).items()}
+    save_file({k: v for k, v in {**tensors, **changes}.items() if k not in drop}, str(tmp_path / "model.safetensors"))
+    return tensors
+
+
+def test_a_checkpoint_of_codes_is_bound_in_codes(tmp_path):
+    from conftest import TINY_B
+    from torchinferno_b200.kernels.gemm import LinearWeight
+    from torchinferno_b200.kernels.microscaled import MicroscaledRows
+    from torchinferno_b200.weights.loader import load_weights
+    from torchinferno_b200.weights.random_init import build_model, init_random_weights
+    config = {**TINY_B, "quantization_config": {**NVFP4, "ignore": ["model.layers.2.self_attn*"]}}
+    name = "model.layers.0.mlp.down_proj.weight"
+    tensors = _folder(tmp_path, config, **{"model.layers.0.mlp.down_proj.input_scale": torch.tensor(0.01)})
+    model = build_model(config, dtype=torch.bfloat16, device="cpu")
+    report = load_weights(model, tmp_path)
+    assert report["stored_dtypes"] == ["bfloat16", "uint8"] and report["ignored"] == ["model.layers.0.mlp.down_proj.input_scale"]
+    assert tensors[name].shape == (192, 256) and tensors[name + "_scale"].shape == (192, 32) and tensors[name + "_scale_2"].shape == ()
+    block = model.blocks[0]
+    down = block.feed_forward.down_weight
+    assert isinstance(down, MicroscaledWeight) and down.in_features == 512 and down.out_features == 192
+    want = MicroscaledWeight(MicroscaledMatrix(tensors[name], tensors[name + "_scale"], tensors[name + "_scale_2"])).tiles
+    assert torch.equal(down.tiles.codes, want.codes) and torch.equal(down.tiles.scales, want.scales) and torch.equal(down.tiles.factors, want.factors)
+    assert isinstance(block.mixer.qkv_weight, MicroscaledWeight) and block.feed_forward.gate_up_weight.tiles.paired
+    assert isinstance(model.blocks[2].mixer.qkv_weight, LinearWeight) and isinstance(model.blocks[2].feed_forward.down_weight, MicroscaledWeight)
+    # the norms ahead of 4-bit products leave rows of codes
+    assert [b.mixer.rows_form(1) for b in model.blocks] == [MicroscaledRows, MicroscaledRows, None] and block.feed_forward.rows_form(4) is MicroscaledRows
+    from torchinferno_b200.kernels import native_block
+    assert native_block.block_weights(block) is None
+    plain = build_model(TINY_B, dtype=torch.bfloat16, device="cpu")
+    init_random_weights(plain, 0)
+    assert model.weight_bytes() < plain.weight_bytes()
+    same = build_model(config, dtype=torch.bfloat16, device="cpu")
+    init_random_weights(same, 0, config=config)
+    assert torch.equal(same.blocks[0].feed_forward.down_weight.tiles.codes, down.tiles.codes)
+    # in 32 bits the numbers they stand for
+    wide = build_model(config, dtype=torch.float32, device="cpu")
+    load_weights(wide, tmp_path)
+    assert torch.equal(wide.blocks[0].feed_forward.down_weight.tensor, MicroscaledMatrix(tensors[name], tensors[name + "_scale"], tensors[name + "_scale_2"]).widened())
+
+
+UP = "model.layers.0.mlp.up_proj.weight"
+
+
+@pytest.mark.parametrize("changes, drop, message", [
+    ({UP + "_scale": torch.ones(512, 11).to(torch.float8_e4m3fn)}, (), r"_scale: file \[512, 11\] vs \[512, 12\]"),
+    ({UP + "_scale": torch.ones(512, 12)}, (), "_scale: stored as F32"),
+    ({UP + "_scale_2": torch.ones(2)}, (), r"_scale_2: file \[2\]"),
+    ({UP + "_scale_2": torch.ones((), dtype=torch.bfloat16)}, (), "_scale_2: stored as BF16"),
+    ({UP: torch.zeros(512, 95, dtype=torch.uint8)}, (), r"up_proj.weight: file \[512, 95\]"),
+    ({UP: torch.zeros(512, 192, dtype=torch.bfloat16)}, (), "up_proj.weight: "),
+    ({}, (UP + "_scale",), "_scale_2"),
+    ({}, (UP + "_scale", UP + "_scale_2"), r"up_proj.weight: file \[512, 96\]"),
+    ({"model.norm.weight_scale": torch.ones(1)}, (), "unexpected"),
+    ({"model.norm.input_scale": torch.ones(1)}, (), "unexpected")])
+def test_checkpoints_that_do_not_fit_are_refused(tmp_path, changes, drop, message):
+    from conftest import TINY_B
+    from torchinferno_b200.weights.loader import WeightError, load_weights
+    from torchinferno_b200.weights.random_init import build_model
+    config = {**TINY_B, "quantization_config": NVFP4}
+    _folder(tmp_path, config, drop, **changes)
+    for dtype in (torch.bfloat16, torch.float32):
+        with pytest.raises(WeightError, match=message):
+            load_weights(build_model(config, dtype=dtype, device="cpu"), tmp_path)
+
+
+def test_codes_of_another_form_are_refused(tmp_path):
+    """Scales that are no numbers, and a config.json that names another run of columns."""
+    import json
+    from conftest import TINY_B
+    from torchinferno_b200.weights.loader import WeightError, load_weights
+    from torchinferno_b200.weights.random_init import build_model, init_random_weights
+    config = {**TINY_B, "quantization_config": NVFP4}
+    _folder(tmp_path, config, **{UP + "_scale": torch.full((512, 12), -1.0).to(torch.float8_e4m3fn)})
+    with pytest.raises(ValueError, match="none of them negative"):
+        load_weights(build_model(config, dtype=torch.bfloat16, device="cpu"), tmp_path)
+    _folder(tmp_path, config)
+    other = {**config, "quantization_config": {**NVFP4, "group_size": 32}}
+    (tmp_path / "config.json").write_text(json.dumps(other))
+    with pytest.raises(WeightError, match="4-bit codes, but quantization_config"):
+        load_weights(build_model(config, dtype=torch.bfloat16, device="cpu"), tmp_path)
+    model = build_model(other, dtype=torch.bfloat16, device="cpu")
+    init_random_weights(model, 0, config=other)      # (random weights are of the model's own type then)
+    assert model.blocks[0].feed_forward.down_weight.dtype == torch.bfloat16
+
+
+def test_fused_projections_are_stored_alike(tmp_path):
+    from conftest import TINY_B
+    from torchinferno_b200.weights.loader import load_weights
+    from torchinferno_b200.weights.random_init import build_model
+    config = {**TINY_B, "quantization_config": {**NVFP4, "ignore": ["k_proj"]}}
+    _folder(tmp_path, config)
+    with pytest.raises(ValueError, match="all be stored in 4-bit codes, or none"):
+        load_weights(build_model(config, dtype=torch.bfloat16, device="cpu"), tmp_path)
+
+
+def test_experts_are_bound_in_codes():
+    from giforax_configs import GA
+    from torchinferno_b200.weights.random_init import build_model, init_random_weights
+    config = {**GA, "quantization_config": NVFP4}
+    model = build_model(config, dtype=torch.bfloat16, device="cpu")
+    init_random_weights(model, 1, config=config)
+    moes = [b.feed_forward for b in model.blocks if type(b.feed_forward).__name__ == "RoutedExperts"]
+    assert moes
+    for moe in moes:
+        assert isinstance(moe.up_weight, MicroscaledExperts) and moe.up_weight.paired == moe.glu and moe.up_weight.experts == moe.experts
+        assert isinstance(moe.down_weight, MicroscaledExperts) and moe.router_weight.dtype == torch.float32 and moe.rows_form(3) is None

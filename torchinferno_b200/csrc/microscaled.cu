@@ -197,6 +197,15 @@ TIB_API int tib_microscaled_product(const void* w, const void* w_scales, const f
   return ms_product_tcgen05(a, act, y, y_dtype, ldy, stream);
 }
 
+// How a product of M rows with one matrix (experts 0) or sorted by expert runs: {rows of a tile at most (256: on pairs of SMs), blocks that share a tile, steps of a block at
+// most, stages of its ring}.
+TIB_API int tib_microscaled_plan(int M, int N, int K, int experts, int* plan) {
+  if (!plan || M < 1 || N < 1 || K < 1 || experts < 0) return TIB_E_ARG;
+  const int steps = ms_steps(K);
+  return ms_on_pairs_of_sms(M, N, steps, experts) ? ms_plan_2cta(M, N, steps, experts, plan) : ms_plan_tcgen05(M, N, steps, experts, plan);
+}
+
 TIB_PACKED(tib_microscaled_rows)
 TIB_PACKED(tib_microscaled_widen)
 TIB_PACKED(tib_microscaled_product)
+TIB_PACKED(tib_microscaled_plan)

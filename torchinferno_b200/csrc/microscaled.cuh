@@ -164,6 +164,9 @@ __device__ __forceinline__ float ms_scaled(float sum, float w_factor, float x_fa
 // Products of rows that are there as codes (microscaled_tcgen05.cu, microscaled_2cta.cu), with arguments that tib_microscaled_product has checked.
 bool ms_on_pairs_of_sms(int M, int N, int steps, int experts);
 int ms_product_2cta(const MsArgs& a, int act, void* y, int y_dtype, int64_t ldy, cudaStream_t stream);
+// How a product runs there: {rows of a tile at most, blocks that share a tile, steps of a block at most, stages of its ring}.
+int ms_plan_2cta(int M, int N, int steps, int experts, int* plan);
+int ms_plan_tcgen05(int M, int N, int steps, int experts, int* plan);
 int ms_product_tcgen05(MsArgs& a, int act, void* y, int y_dtype, int64_t ldy, cudaStream_t stream);
 
 }  // namespace tib

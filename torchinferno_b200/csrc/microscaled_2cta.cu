@@ -373,3 +373,9 @@ int tib::ms_product_2cta(const MsArgs& a, int act, void* out, int out_dtype, int
 #undef TIB_M2_GO
   return TIB_E_SIZE;
 }
+
+int tib::ms_plan_2cta(int M, int N, int steps, int experts, int* plan) {
+  const int64_t tiles = m2_tiles(M, N, experts), most = steps * ceil_div64(tiles, tiles < 74 ? tiles : 74);
+  plan[0] = 256; plan[1] = 1; plan[2] = (int)(most < 0x7fffffff ? most : 0x7fffffff); plan[3] = kM2Stages;
+  return TIB_OK;
+}

@@ -423,3 +423,11 @@ int tib::ms_product_tcgen05(MsArgs& a, int act, void* y, int y_dtype, int64_t ld
   TIB_MT_GO(128);
 #undef TIB_MT_GO
 }
+
+int tib::ms_plan_tcgen05(int M, int N, int steps, int experts, int* plan) {
+  MtPlan p;
+  plan[0] = mt_tile_rows(M);
+  const int rc = plan[0] == 32 ? mt_plan<32>(M, N, steps, experts, p) : mt_plan<128>(M, N, steps, experts, p);
+  plan[1] = p.splits; plan[2] = p.steps; plan[3] = p.stages;
+  return rc;
+}

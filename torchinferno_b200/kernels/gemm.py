@@ -13,7 +13,7 @@ import weakref
 
 import torch
 
-from torchinferno_b200.kernels import ops
+from torchinferno_b200.kernels import block_scaled, microscaled, ops
 from torchinferno_b200.kernels.block_scaled import BlockScaledExperts, BlockScaledMatrix, BlockScaledRows, BlockScaledWeight
 from torchinferno_b200.kernels.microscaled import MicroscaledExperts, MicroscaledMatrix, MicroscaledRows, MicroscaledWeight
 
@@ -179,6 +179,19 @@ def expert_matrices(matrices: "list[Matrix]", ups: "list[Matrix] | None" = None)
     if kind is not None:
         return _EXPERTS[kind](matrices, ups)
     return torch.stack(matrices if ups is None else [row_pairs(g, u) for g, u in zip(matrices, ups)]).contiguous()
+
+
+def rows_form(weight: "LinearWeight | QuantizedWeight | None", count: int) -> type | None:
+    """The form of quantised rows in which a norm should leave ``count`` rows for a product with ``weight``; None: a tensor.  (8-bit products of few rows
+    quantise them in their own kernel.)"""
+    if isinstance(weight, MicroscaledWeight):
+        return MicroscaledRows
+    return BlockScaledRows if isinstance(weight, BlockScaledWeight) and count > block_scaled.FEW_ROWS else None
+
+
+def add_rmsnorm(form: type, delta: torch.Tensor | None, residual: torch.Tensor, weight: torch.Tensor, eps: float, **options) -> Rows:
+    """:func:`ops.add_rmsnorm` whose rows leave in this form (see :func:`block_scaled.add_rmsnorm` and :func:`microscaled.add_rmsnorm`)."""
+    return (microscaled if form is MicroscaledRows else block_scaled).add_rmsnorm(delta, residual, weight, eps, **options)
 
 
 def linear(x: Rows, weight: "torch.Tensor | LinearWeight | QuantizedWeight", *, out_dtype: torch.dtype | None = None,

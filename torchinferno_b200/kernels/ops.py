@@ -1281,14 +1281,19 @@ def need_expert_product(x: torch.Tensor, y: torch.Tensor, offsets: torch.Tensor,
     rows = need_rows(x, columns, here, "moe_expert_product")
     if y.shape != (pairs, width) or offsets.numel() != experts + 1 or top < 1 or (pairs % top or rows < pairs // top if x_by_pair else rows < pairs):
         raise KernelError("moe_expert_product: shapes do not fit")
-    for name, t, dtype in (("offsets", offsets, torch.int32), ("order", order, torch.int32), ("row_scale", row_scale, torch.float32)):
-        if t is not None and (t.dtype != dtype or t.get_device() != here or not t.is_contiguous()):
-            raise KernelError(f"moe_expert_product: {name} must be contiguous {dtype} on cuda:{here}, not {t.dtype} on {t.device}")
+    _need_plain(offsets, "offsets", torch.int32, here), _need_plain(order, "order", torch.int32, here)
+    if row_scale is not None:
+        _need_plain(row_scale, "row_scale", torch.float32, here)
+        if row_scale.numel() != pairs:
+            raise KernelError("moe_expert_product: row_scale must hold one factor per pair")
     if y.get_device() != here or (y.stride(1) != 1 and width > 1):
         raise KernelError(f"moe_expert_product: y must be rows with unit inner stride on cuda:{here}")
-    if row_scale is not None and row_scale.numel() != pairs:
-        raise KernelError("moe_expert_product: row_scale must hold one factor per pair")
     return pairs
+
+
+def _need_plain(t: torch.Tensor, name: str, dtype: torch.dtype, here: int) -> None:
+    if t.dtype is not dtype or t.get_device() != here or not t.is_contiguous():
+        raise KernelError(f"moe_expert_product: {name} must be contiguous {dtype} on cuda:{here}, not {t.dtype} on {t.device}")
 
 
 # ---------------------------------------------------------------------------
@@ -1329,13 +1334,13 @@ def block_scaled_product(x: torch.Tensor | None, codes: int, make: bool, blocks,
 def microscaled_rows(x: torch.Tensor, codes: int, scales: int, factors: int) -> None:
     """Codes, scales and factors of the rows ``x``, to these addresses."""
     rows, columns = x.shape
-    _check("microscaled_rows", _library.tib_microscaled_rows(x.data_ptr(), _code(x.dtype), x.stride(0), rows, codes, scales, factors, rows, columns, 0, 0, 1, 1, 0, _stream()))
+    _check("microscaled_rows", lib().tib_microscaled_rows(x.data_ptr(), _code(x.dtype), x.stride(0), rows, codes, scales, factors, rows, columns, 0, 0, 1, 1, 0, _stream()))
 
 
 def microscaled_widen(codes: int, scales: int, factors: int, out: torch.Tensor) -> None:
     """The numbers that codes, scales and factors at these addresses stand for."""
     rows, columns = out.shape
-    _check("microscaled_widen", _library.tib_microscaled_widen(codes, scales, factors, out.data_ptr(), _code(out.dtype), columns, rows, columns, _stream()))
+    _check("microscaled_widen", lib().tib_microscaled_widen(codes, scales, factors, out.data_ptr(), _code(out.dtype), columns, rows, columns, _stream()))
 
 
 def microscaled_product(weight: tuple, x: torch.Tensor | None, rows: tuple, y: torch.Tensor, act: str, limit: float, alpha: float, offsets: int, order: int,
@@ -1348,7 +1353,7 @@ def microscaled_product(weight: tuple, x: torch.Tensor | None, rows: tuple, y: t
     else:
         source = (x.data_ptr(), _code(x.dtype), x.stride(0), x.shape[0])
         _counter["launches"] += 1
-    _check("microscaled_product", _library.tib_microscaled_product(
+    _check("microscaled_product", lib().tib_microscaled_product(
         *weight, *source, *rows, x is not None, y.data_ptr(), _code(y.dtype), y.stride(0), y.shape[0], offsets, order, top, x_by_pair, MOE_ACT[act], limit, alpha,
         0 if row_scale is None else row_scale.data_ptr(), 0 if error_word is None else error_word.data_ptr(), _stream()))
 
@@ -1383,7 +1388,7 @@ def quantized_norm(delta: torch.Tensor | None, residual: torch.Tensor, weight: t
     if new_residual is not None:
         kept = new_residual
         _need_on(kept, "new_residual", torch.float32, shape, device)
-    _check("add_rmsnorm", _library.tib_quantized_norm(
+    _check("add_rmsnorm", lib().tib_quantized_norm(
         0 if delta is None else delta.data_ptr(), residual.data_ptr(), 0 if kept is None else kept.data_ptr(), 0 if rows is None else rows.data_ptr(), weight.data_ptr(),
         0 if out is None else out.data_ptr(), in_bytes, codes, scales, factors, lds, count, shape[1], eps, _code(dtype), _stream()))
 

@@ -14,6 +14,7 @@ import torch
 
 from torchinferno_b200.kernels import gemm, ops
 from torchinferno_b200.kernels.block_scaled import BlockScaledExperts, BlockScaledWeight
+from torchinferno_b200.kernels.microscaled import MicroscaledExperts, MicroscaledWeight
 from torchinferno_b200.kernels.gemm import linear
 from torchinferno_b200.models.spec import ModelSpec, StageCall
 from torchinferno_b200.parts.base import (Block, CacheSpec, KVBinding, LayerContext, ResidualStream,
@@ -114,7 +115,7 @@ class CausalLM:
         for _, part in self._owned_parts():
             for key, value in vars(part).items():
                 if key.endswith("weight"):
-                    if isinstance(value, (BlockScaledWeight, BlockScaledExperts)):
+                    if isinstance(value, (BlockScaledWeight, BlockScaledExperts, MicroscaledWeight, MicroscaledExperts)):
                         seen[value.address()] = value.nbytes()
                     else:
                         note(getattr(value, "tensor", value) if not isinstance(value, torch.Tensor) else value)

@@ -19,8 +19,7 @@ from typing import Mapping
 import torch
 
 from torchinferno_b200.kernels import attention as attention_kernels
-from torchinferno_b200.kernels.block_scaled import BlockScaledWeight
-from torchinferno_b200.kernels.gemm import LinearWeight, linear, projection
+from torchinferno_b200.kernels.gemm import LinearWeight, QuantizedWeight, linear, projection, rows_form
 from torchinferno_b200.parts.base import (CacheSpec, LayerContext, Mixer, PartSpec, WeightSpec,
                                           build_part, register_part)
 
@@ -41,8 +40,8 @@ class GQAAttention(Mixer):
         if not isinstance(position, PartSpec):
             position = PartSpec(**position)
         self.position = build_part("position", position, dtype=dtype, device=device)
-        self.qkv_weight: LinearWeight | BlockScaledWeight | None = None
-        self.o_weight: LinearWeight | BlockScaledWeight | None = None
+        self.qkv_weight: LinearWeight | QuantizedWeight | None = None
+        self.o_weight: LinearWeight | QuantizedWeight | None = None
 
     def weight_specs(self) -> list[WeightSpec]:
         q, k, v, o = self.names
@@ -56,6 +55,9 @@ class GQAAttention(Mixer):
 
     def cache_spec(self) -> CacheSpec:
         return CacheSpec(self.kv_heads, self.head_dim, self.window)
+
+    def rows_form(self, count: int) -> type | None:
+        return rows_form(self.qkv_weight, count)
 
     def forward(self, x: torch.Tensor, ctx: LayerContext) -> torch.Tensor:
         if ctx.kv is None:

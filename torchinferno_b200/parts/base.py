@@ -51,7 +51,9 @@ class WeightSpec:
     free_dims: tuple[int, ...] = ()   # dimensions whose size the file decides (``shape`` holds what random weights get);
                                       # the part reads the size off the tensor it is bound to
     block_scaled: bool = False        # may be stored as e4m3 codes with a 32-bit scale for each block of 128 x 128 (a tensor named
-                                      # name + "_scale_inv"); in bfloat16 the part is then bound to a kernels.block_scaled.BlockScaledMatrix
+                                      # name + "_scale_inv"); in bfloat16 the part is then bound to a kernels.block_scaled.BlockScaledMatrix.  Or as 4-bit
+                                      # codes with a scale for each 16 columns and a factor (name + "_scale", name + "_scale_2"): a
+                                      # kernels.microscaled.MicroscaledMatrix
 
 
 @dataclass(frozen=True)
@@ -187,9 +189,14 @@ class ResidualStream:
             self.pending_write = None
         return out
 
-    def normed(self, norm: "Norm", rows: torch.Tensor | None = None) -> torch.Tensor:
+    def normed(self, norm: "Norm", rows: torch.Tensor | None = None, form: type | None = None):
+        """The normed rows: a tensor, or quantised rows in this form where the norm can leave them so."""
         if self.streams is not None:
             return self.read_streams(None, norm, rows)
+        if form is not None and rows is None and norm.quantizes:
+            made = norm.quantized_forward(form, self.pending, self.residual, self.dtype)
+            self.pending = None
+            return made
         n = self.residual.shape[0] if rows is None else rows.numel()
         out = torch.empty((n, self.residual.shape[1]), dtype=self.dtype, device=self.residual.device)
         if self.pending is None:
@@ -247,6 +254,12 @@ class Part:
 
 
 class Norm(Part):
+    quantizes = False        # whether quantized_forward is there
+
+    def quantized_forward(self, form: type, delta: torch.Tensor | None, residual: torch.Tensor, dtype: torch.dtype):
+        """:meth:`add_forward` (or :meth:`forward` without a delta) whose rows, rounded to ``dtype``, leave quantised."""
+        raise NotImplementedError
+
     def forward(self, residual: torch.Tensor, out: torch.Tensor, rows: torch.Tensor | None = None) -> torch.Tensor:
         raise NotImplementedError
 
@@ -278,11 +291,19 @@ class Mixer(Part):
     def state_spec(self) -> StateSpec | None:
         return None
 
+    def rows_form(self, count: int) -> type | None:
+        """The form of quantised rows in which this part wants ``count`` normed rows (see :func:`gemm.rows_form`); None: a tensor."""
+        return None
+
     def forward(self, x: torch.Tensor, ctx: LayerContext) -> torch.Tensor:
         raise NotImplementedError
 
 
 class FeedForward(Part):
+    def rows_form(self, count: int) -> type | None:
+        """As of a mixer."""
+        return None
+
     def forward(self, x: torch.Tensor, ctx: LayerContext) -> torch.Tensor:
         raise NotImplementedError
 

@@ -72,8 +72,10 @@ class PreNormBlock(Block):
     def capturable(self) -> bool:
         return all(stage.capturable for _, stage in self._input_stages())
 
-    def _read(self, stream: ResidualStream, norm, stage, ctx: LayerContext, state_off: int) -> torch.Tensor:
-        return stream.normed(norm) if stage is None else stage.forward(stream, norm, ctx, state_off)
+    def _read(self, stream: ResidualStream, norm, stage, part, ctx: LayerContext, state_off: int):
+        if stage is not None:
+            return stage.forward(stream, norm, ctx, state_off)
+        return stream.normed(norm, form=part.rows_form(stream.residual.shape[0]))
 
     def forward(self, stream: ResidualStream, ctx: LayerContext) -> None:
         if self._native is _UNKNOWN or self._native_generation != gemm.generation():
@@ -86,11 +88,11 @@ class PreNormBlock(Block):
             window = self.mixer.window if self.mixer.window is not None else ctx.kv.window
             native_block.run_block(self._native, stream, ctx, window)
             return
-        stream.add(self.mixer.forward(self._read(stream, self.mixer_norm, self.mixer_input, ctx, 0), ctx))
+        stream.add(self.mixer.forward(self._read(stream, self.mixer_norm, self.mixer_input, self.mixer, ctx, 0), ctx))
         if self.feed_forward is not None:
             behind = 0 if self.mixer_input is None else self.mixer_input.state_floats()
             stream.add(self.feed_forward.forward(
-                self._read(stream, self.feed_forward_norm, self.feed_forward_input, ctx, behind), ctx))
+                self._read(stream, self.feed_forward_norm, self.feed_forward_input, self.feed_forward, ctx, behind), ctx))
 
 
 register_part("block", "prenorm", PreNormBlock)

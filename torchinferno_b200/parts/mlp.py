@@ -15,8 +15,7 @@ from typing import Mapping
 import torch
 
 from torchinferno_b200.kernels import ops
-from torchinferno_b200.kernels.block_scaled import BlockScaledWeight
-from torchinferno_b200.kernels.gemm import LinearWeight, gated_projection, linear, linear_swiglu, projection
+from torchinferno_b200.kernels.gemm import LinearWeight, QuantizedWeight, gated_projection, linear, linear_swiglu, projection, rows_form
 from torchinferno_b200.parts.base import FeedForward, LayerContext, WeightSpec, register_part
 
 
@@ -27,8 +26,8 @@ class SwiGLUFeedForward(FeedForward):
         super().__init__(dtype=dtype, device=device)
         self.hidden_size, self.intermediate_size = hidden_size, intermediate_size
         self.names = (gate_name, up_name, down_name)
-        self.gate_up_weight: LinearWeight | BlockScaledWeight | None = None
-        self.down_weight: LinearWeight | BlockScaledWeight | None = None
+        self.gate_up_weight: LinearWeight | QuantizedWeight | None = None
+        self.down_weight: LinearWeight | QuantizedWeight | None = None
 
     def weight_specs(self) -> list[WeightSpec]:
         g, u, d = self.names
@@ -39,6 +38,9 @@ class SwiGLUFeedForward(FeedForward):
     def bind(self, weights: Mapping[str, torch.Tensor]) -> None:
         g, u, d = self.names
         self.gate_up_weight, self.down_weight = gated_projection(weights[g], weights[u]), projection(weights[d])
+
+    def rows_form(self, count: int) -> type | None:
+        return rows_form(self.gate_up_weight, count)
 
     def forward(self, x: torch.Tensor, ctx: LayerContext) -> torch.Tensor:
         return linear(linear_swiglu(x, self.gate_up_weight), self.down_weight)
@@ -57,8 +59,8 @@ class DenseFeedForward(FeedForward):
             raise ValueError(f"unknown activation {activation!r}; known: ['relu2']")
         self.hidden_size, self.intermediate_size, self.activation = hidden_size, intermediate_size, activation
         self.names = (up_name, down_name)
-        self.up_weight: LinearWeight | BlockScaledWeight | None = None
-        self.down_weight: LinearWeight | BlockScaledWeight | None = None
+        self.up_weight: LinearWeight | QuantizedWeight | None = None
+        self.down_weight: LinearWeight | QuantizedWeight | None = None
 
     def weight_specs(self) -> list[WeightSpec]:
         u, d = self.names
@@ -68,6 +70,9 @@ class DenseFeedForward(FeedForward):
     def bind(self, weights: Mapping[str, torch.Tensor]) -> None:
         u, d = self.names
         self.up_weight, self.down_weight = projection(weights[u]), projection(weights[d])
+
+    def rows_form(self, count: int) -> type | None:
+        return rows_form(self.up_weight, count)
 
     def forward(self, x: torch.Tensor, ctx: LayerContext) -> torch.Tensor:
         hidden = linear(x, self.up_weight)

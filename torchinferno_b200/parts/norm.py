@@ -13,11 +13,13 @@ from typing import Mapping
 
 import torch
 
-from torchinferno_b200.kernels import ops
+from torchinferno_b200.kernels import gemm, ops
 from torchinferno_b200.parts.base import Norm, WeightSpec, register_part
 
 
 class RMSNorm(Norm):
+    quantizes = True
+
     def __init__(self, *, width: int, eps: float, weight_name: str = "weight", weight_offset: float = 0.0,
                  dtype: torch.dtype, device: torch.device) -> None:
         super().__init__(dtype=dtype, device=device)
@@ -38,6 +40,9 @@ class RMSNorm(Norm):
 
     def add_forward(self, delta, residual, out, rows=None):
         return ops.add_rmsnorm(delta, residual, self.weight, self.eps, out, rows)
+
+    def quantized_forward(self, form, delta, residual, dtype):
+        return gemm.add_rmsnorm(form, delta, residual, self.weight, self.eps, dtype=dtype)
 
     def forward_rows(self, x: torch.Tensor) -> torch.Tensor:
         """Norm rows held in the activation type (not the residual stream)."""

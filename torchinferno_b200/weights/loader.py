@@ -14,9 +14,10 @@ widened to fp32 (lossless); integer tables become int32.  When the engine
 computes in float32 every floating tensor is widened to fp32.  A matrix that its
 part takes in 8-bit blocks (``WeightSpec.block_scaled``) and that is stored as e4m3
 codes with a tensor of scales beside it (its name and ``_scale_inv``) stays so in
-bfloat16, and is widened to the numbers it stands for in float32.  Codes without their
-scales are refused, and so are those of a folder whose ``quantization_config`` names
-another form of 8-bit weights (config/quantization.py).
+bfloat16, and is widened to the numbers it stands for in float32; so does one stored as
+4-bit codes with tensors of scales (its name and ``_scale``) and a factor (``_scale_2``)
+beside it.  Codes without their scales are refused, and so are those of a folder whose
+``quantization_config`` names another form (config/quantization.py).
 """
 from __future__ import annotations
 
@@ -27,8 +28,10 @@ from typing import Iterable
 import torch
 
 from torchinferno_b200.config.model_config import ConfigError
-from torchinferno_b200.config.quantization import SCALE_SUFFIX, BlockQuantization
+from torchinferno_b200.config.quantization import (CODE_FACTOR_SUFFIX, CODE_SCALE_SUFFIX, SCALE_SUFFIX, BlockQuantization, MicroscaledQuantization,
+                                                   measured_scale_of_rows)
 from torchinferno_b200.kernels.block_scaled import BlockScaledMatrix, blocks
+from torchinferno_b200.kernels.microscaled import RUN, MicroscaledMatrix
 
 SINGLE_FILE = "model.safetensors"
 INDEX_FILE = "model.safetensors.index.json"
@@ -101,8 +104,11 @@ def load_weights(model, folder: str | Path) -> dict[str, object]:
         missing = [n for n, ws in expected.items() if n not in files and not ws.optional]
         scales = {n + SCALE_SUFFIX: n for n, ws in expected.items() if ws.block_scaled and n in files}
         in_blocks = {n for s, n in scales.items() if s in files}
-        ignored = sorted(n for n in files if n not in expected and n.endswith(IGNORED_SUFFIXES))
-        unexpected = [n for n in files if n not in expected and n not in ignored and scales.get(n) not in in_blocks]
+        in_codes = {n for n, ws in expected.items() if ws.block_scaled and n in files and n + CODE_SCALE_SUFFIX in files and n + CODE_FACTOR_SUFFIX in files}
+        beside_codes = {n + suffix for n in in_codes for suffix in (CODE_SCALE_SUFFIX, CODE_FACTOR_SUFFIX)}
+        not_needed = {measured_scale_of_rows(n) for n in in_codes}
+        ignored = sorted(n for n in files if n not in expected and (n.endswith(IGNORED_SUFFIXES) or n in not_needed))
+        unexpected = [n for n in files if n not in expected and n not in ignored and scales.get(n) not in in_blocks and n not in beside_codes]
         # a head that the model ties to its embedding is not read even if the file stores a copy
         unused = set(model.unused_optional_tensors()) if hasattr(model, "unused_optional_tensors") else set()
         wrong: list[str] = []
@@ -111,6 +117,9 @@ def load_weights(model, folder: str | Path) -> dict[str, object]:
                 continue
             view = handle_of(files[name]).get_slice(name)
             shape = tuple(view.get_shape())
+            if name in in_codes:
+                wrong += _wrong_codes(name, ws.shape, *(handle_of(files[n]).get_slice(n) for n in (name, name + CODE_SCALE_SUFFIX, name + CODE_FACTOR_SUFFIX)))
+                continue
             free = getattr(ws, "free_dims", ())
             if len(shape) != len(ws.shape) or any(a != b for d, (a, b) in enumerate(zip(shape, ws.shape)) if d not in free):
                 wrong.append(f"{name}: file {list(shape)} vs model {list(ws.shape)}")
@@ -126,6 +135,8 @@ def load_weights(model, folder: str | Path) -> dict[str, object]:
                     wrong.append(f"{name + SCALE_SUFFIX}: stored as {beside.get_dtype()}, scales are floating-point numbers")
             elif dtype.startswith("F8") and name not in unused:      # (codes stand for nothing without their scales)
                 wrong.append(f"{name}: stored as {dtype} without {name + SCALE_SUFFIX}" if ws.block_scaled else f"{name}: stored as {dtype}, which the model does not take")
+            elif dtype == "U8" and ws.block_scaled:
+                wrong.append(f"{name}: stored as {dtype} without {name + CODE_SCALE_SUFFIX} and {name + CODE_FACTOR_SUFFIX}")
         if missing or unexpected or wrong:
             parts = [f"checkpoint {folder} does not fit the model ({model.spec.architecture}):"]
             if missing:
@@ -136,11 +147,14 @@ def load_weights(model, folder: str | Path) -> dict[str, object]:
                 parts.append(f"  wrong shape ({len(wrong)}): " + "; ".join(sorted(wrong)[:12])
                              + (f"; ... (+{len(wrong) - 12} more)" if len(wrong) > 12 else ""))
             raise WeightError("\n".join(parts))
-        if in_blocks and (Path(folder) / CONFIG_FILE).is_file():
-            try:
-                BlockQuantization.from_config(json.loads((Path(folder) / CONFIG_FILE).read_text()))
-            except ConfigError as exc:
-                raise WeightError(f"checkpoint {folder} holds 8-bit blocks, but {exc}") from None
+        if (in_blocks or in_codes) and (Path(folder) / CONFIG_FILE).is_file():
+            said = json.loads((Path(folder) / CONFIG_FILE).read_text())
+            for held, form, what in ((in_blocks, BlockQuantization, "8-bit blocks"), (in_codes, MicroscaledQuantization, "4-bit codes")):
+                try:
+                    if held:
+                        form.from_config(said)
+                except ConfigError as exc:
+                    raise WeightError(f"checkpoint {folder} holds {what}, but {exc}") from None
         tensors: dict[str, torch.Tensor] = {}
         stored: dict[str, str] = {}
         for name, ws in expected.items():
@@ -150,6 +164,10 @@ def load_weights(model, folder: str | Path) -> dict[str, object]:
             stored[name] = str(tensor.dtype).replace("torch.", "")
             if name in in_blocks:
                 matrix = BlockScaledMatrix(tensor.contiguous(), handle_of(files[name + SCALE_SUFFIX]).get_tensor(name + SCALE_SUFFIX).to(torch.float32).contiguous())
+                tensors[name] = place_blocks(matrix, model.dtype, model.device)
+            elif name in in_codes:
+                beside, factor = (handle_of(files[name + suffix]).get_tensor(name + suffix) for suffix in (CODE_SCALE_SUFFIX, CODE_FACTOR_SUFFIX))
+                matrix = MicroscaledMatrix(tensor.contiguous(), beside.contiguous(), factor.to(torch.float32).reshape(()), ws.shape[1])
                 tensors[name] = place_blocks(matrix, model.dtype, model.device)
             else:
                 tensors[name] = place(tensor, ws.role, model.dtype, model.device)
@@ -162,8 +180,18 @@ def load_weights(model, folder: str | Path) -> dict[str, object]:
             "not_read": sorted(unused & set(files))}
 
 
-def place_blocks(matrix: BlockScaledMatrix, compute_dtype: torch.dtype, device: torch.device) -> "BlockScaledMatrix | torch.Tensor":
-    """The same for a matrix in 8-bit blocks."""
+def _wrong_codes(name: str, wanted: tuple[int, ...], codes, scales, factor) -> list[str]:
+    """What does not fit of a matrix of 4-bit codes and the tensors beside it (slices of the file)."""
+    n, k = wanted
+    found = {name: codes, name + CODE_SCALE_SUFFIX: scales, name + CODE_FACTOR_SUFFIX: factor}
+    shapes = {name: [[n, -(-k // 2)]], name + CODE_SCALE_SUFFIX: [[n, -(-k // RUN)]], name + CODE_FACTOR_SUFFIX: [[], [1]]}
+    kinds = {name: "U8", name + CODE_SCALE_SUFFIX: "F8_E4M3", name + CODE_FACTOR_SUFFIX: "F32"}
+    wrong = [f"{t}: file {list(view.get_shape())} vs {shapes[t][0]} of a 4-bit {list(wanted)}" for t, view in found.items() if list(view.get_shape()) not in shapes[t]]
+    return wrong + [f"{t}: stored as {view.get_dtype()}, of a matrix of 4-bit codes it is {kinds[t]}" for t, view in found.items() if str(view.get_dtype()) != kinds[t]]
+
+
+def place_blocks(matrix: "BlockScaledMatrix | MicroscaledMatrix", compute_dtype: torch.dtype, device: torch.device) -> "BlockScaledMatrix | MicroscaledMatrix | torch.Tensor":
+    """The same for a matrix in 8-bit blocks or 4-bit codes."""
     matrix = matrix.to(device)
     return matrix.widened(torch.float32) if compute_dtype == torch.float32 else matrix
 

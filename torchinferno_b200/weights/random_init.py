@@ -7,8 +7,8 @@ The reference has no such mode; its tests build an eager model under
 ``torch.manual_seed`` and write it out to load it back
 (tests/test_model_variants.py:319-354 in the reference project).
 
-With ``quantization_config`` in config.json (config/quantization.py) the matrices it covers are quantised to 8-bit blocks; where it names
-a form that is not read, random weights are of the model's own type, as without it.
+With ``quantization_config`` in config.json (config/quantization.py) the matrices it covers are quantised, to 8-bit blocks or 4-bit codes; where it
+names a form that is not read, random weights are of the model's own type, as without it.
 """
 from __future__ import annotations
 
@@ -20,9 +20,9 @@ from typing import Any, Mapping
 import torch
 
 from torchinferno_b200.config.model_config import ConfigError
-from torchinferno_b200.config.quantization import SCALE_SUFFIX, BlockQuantization
+from torchinferno_b200.config.quantization import CODE_FACTOR_SUFFIX, CODE_SCALE_SUFFIX, SCALE_SUFFIX, BlockQuantization, MicroscaledQuantization, quantization_of
 from torchinferno_b200.config.registry import resolve_architecture
-from torchinferno_b200.kernels.block_scaled import quantize_matrix
+from torchinferno_b200.kernels import block_scaled, microscaled
 from torchinferno_b200.weights.loader import SINGLE_FILE, place, place_blocks
 
 
@@ -58,17 +58,19 @@ def build_model(config: Mapping[str, Any], *, dtype: torch.dtype, device: torch.
     return CausalLM(entry.build(typed), dtype=dtype, device=device)
 
 
-def _quantization(config: Mapping[str, Any]) -> BlockQuantization | None:
-    """What config.json has stored in 8-bit blocks.  (A form of 8-bit weights that is not read concerns files, and their loader: a random model has none.)"""
+def _quantization(config: Mapping[str, Any]) -> "BlockQuantization | MicroscaledQuantization | None":
+    """What config.json has stored in 8-bit blocks or 4-bit codes.  (A form that is not read concerns files, and their loader: a random model has none.)"""
     try:
-        return BlockQuantization.from_config(config)
+        return quantization_of(config)
     except ConfigError:
         return None
 
 
-def _in_blocks(quantization: BlockQuantization | None, spec) -> bool:
-    """Whether config.json has this tensor stored in 8-bit blocks."""
-    return spec.block_scaled and quantization is not None and quantization.converts(spec.name)
+def _quantized(quantization: "BlockQuantization | MicroscaledQuantization | None", spec, tensor) -> "block_scaled.BlockScaledMatrix | microscaled.MicroscaledMatrix | None":
+    """The tensor that ``tensor()`` makes, as config.json has it stored; None where it is stored as it is."""
+    if not spec.block_scaled or quantization is None or not quantization.converts(spec.name):
+        return None
+    return (block_scaled if isinstance(quantization, BlockQuantization) else microscaled).quantize_matrix(tensor())
 
 
 def write_random_model(config: Mapping[str, Any], folder: str | Path, seed: int,
@@ -85,9 +87,12 @@ def write_random_model(config: Mapping[str, Any], folder: str | Path, seed: int,
     for name, spec in model.expected_tensors().items():
         if spec.optional:
             continue  # e.g. a head tied to the embedding is not stored
-        if _in_blocks(quantization, spec):
-            matrix = quantize_matrix(random_tensor(spec, seed))
+        matrix = _quantized(quantization, spec, lambda: random_tensor(spec, seed))
+        if isinstance(matrix, block_scaled.BlockScaledMatrix):
             tensors[name], tensors[name + SCALE_SUFFIX] = matrix.codes, matrix.scales
+            continue
+        if matrix is not None:
+            tensors[name], tensors[name + CODE_SCALE_SUFFIX], tensors[name + CODE_FACTOR_SUFFIX] = matrix.codes, matrix.scales, matrix.factor
             continue
         tensors[name] = random_tensor(spec, seed, dtype=dtype).contiguous()
     (folder / "config.json").write_text(json.dumps(config, indent=1) + "\n")
@@ -97,14 +102,15 @@ def write_random_model(config: Mapping[str, Any], folder: str | Path, seed: int,
 
 def init_random_weights(model, seed: int, storage_dtype: torch.dtype = torch.bfloat16, config: Mapping[str, Any] | None = None) -> None:
     """Bind seeded random weights generated on the model's device (nothing touches the disk).  ``config``: the config.json whose
-    ``quantization_config`` says which matrices are stored in 8-bit blocks (None: none)."""
+    ``quantization_config`` says which matrices are stored in 8-bit blocks or 4-bit codes (None: none)."""
     quantization = None if config is None else _quantization(config)
     tensors = {}
     for name, spec in model.expected_tensors().items():
         if spec.optional:
             continue
-        if _in_blocks(quantization, spec):
-            tensors[name] = place_blocks(quantize_matrix(random_tensor(spec, seed, device=model.device)), model.dtype, model.device)
+        matrix = _quantized(quantization, spec, lambda: random_tensor(spec, seed, device=model.device))
+        if matrix is not None:
+            tensors[name] = place_blocks(matrix, model.dtype, model.device)
             continue
         raw = random_tensor(spec, seed, device=model.device, dtype=storage_dtype)
         tensors[name] = place(raw, spec.role, model.dtype, model.device)
