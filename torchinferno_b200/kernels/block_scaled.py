@@ -110,7 +110,7 @@ class BlockScaledRows:
     __slots__ = ("buffer", "shape", "dtype", "codes_at", "scales_at", "lds")
 
     def __init__(self, like: torch.Tensor, rows: int, columns: int, dtype: torch.dtype) -> None:
-        self.buffer = _code_buffer(like, rows, columns)
+        self.buffer = ops.new_bytes(like, blocks(columns) * (rows * BLOCK + 4 * ((rows + 3) & ~3)))
         self.shape, self.dtype, self.lds, self.codes_at = torch.Size((rows, columns)), dtype, (rows + 3) & ~3, self.buffer.data_ptr()
         self.scales_at = self.codes_at + blocks(columns) * BLOCK * rows
 
@@ -132,7 +132,11 @@ class BlockScaledRows:
 
     def widened(self, dtype: torch.dtype | None = None) -> torch.Tensor:
         """The numbers the rows stand for, in ``dtype`` (bfloat16 or float32; left out: the rows' own)."""
-        out = self.buffer.new_empty(self.shape, dtype=self.dtype if dtype is None else dtype)
+        dtype = self.dtype if dtype is None else dtype
+        rows = ops.need_rows(self, None, None, "widened")
+        if dtype not in _OUT_DTYPES:
+            raise ops.KernelError(f"widened: unsupported dtype {dtype}")
+        out = ops.new_rows(self.buffer, rows, self.shape[1], dtype)
         ops.widen_rows(self.codes_at, self.scales_at, self.lds, out)
         return out
 

@@ -102,12 +102,12 @@ def quantize_matrix(matrix: torch.Tensor) -> MicroscaledMatrix:
 
 # ------------------------------------------------------------------------------------------------ rows
 @functools.lru_cache(maxsize=4096)
-def _sizes(rows: int, columns: int, experts: int) -> tuple[int, int, int]:
-    """(where in a buffer for so many rows' codes, scales and factors the scales begin, where the factors, its bytes); see csrc/microscaled.cuh.  (experts: 0 for
-    rows that are not sorted.)"""
+def _sizes(rows: int, columns: int, experts: int) -> tuple[int, int, int, torch.Size]:
+    """(where in a buffer for so many rows' codes, scales and factors the scales begin, where the factors, its bytes, the rows' shape); see
+    csrc/microscaled.cuh.  (experts: 0 for rows that are not sorted.)"""
     steps = _count(columns, STEP)
     codes, scales = (_count(rows, GROUP) + experts) * steps * (GROUP * STEP // 2), (_count(rows, TILE) + experts) * steps * (TILE * STEP // RUN)
-    return codes, codes + scales, codes + scales + 4 * rows
+    return codes, codes + scales, codes + scales + 4 * rows, torch.Size((rows, columns))
 
 
 class MicroscaledRows:
@@ -115,10 +115,10 @@ class MicroscaledRows:
     __slots__ = ("buffer", "shape", "dtype", "codes_at", "scales_at", "factors_at")
 
     def __init__(self, like: torch.Tensor, rows: int, columns: int, dtype: torch.dtype) -> None:
-        scales, factors, size = _sizes(rows, columns, 0)
-        self.buffer = buffer = like.new_empty(size, dtype=torch.uint8)
-        self.shape, self.dtype, self.codes_at = torch.Size((rows, columns)), dtype, buffer.data_ptr()
-        self.scales_at, self.factors_at = self.codes_at + scales, self.codes_at + factors
+        scales, factors, size, self.shape = _sizes(rows, columns, 0)
+        self.buffer = buffer = ops.new_bytes(like, size)
+        self.dtype, self.codes_at = dtype, (at := buffer.data_ptr())
+        self.scales_at, self.factors_at = at + scales, at + factors
 
     @property
     def device(self) -> torch.device:
@@ -132,9 +132,13 @@ class MicroscaledRows:
 
     def widened(self, dtype: torch.dtype | None = None) -> torch.Tensor:
         """The numbers the rows stand for, in ``dtype`` (bfloat16, which holds them all but where they underflow, or float32; left out: the rows' own)."""
+        rows, columns = self.shape
         dtype = self.dtype if dtype is None else dtype
-        out = self.buffer.new_empty(self.shape, dtype=dtype)
-        ops.microscaled_widen(self.codes_at, self.scales_at, self.factors_at, out)
+        ops.need_rows(self, None, None, "widened")
+        if dtype not in _OUT_DTYPES:
+            raise ops.KernelError(f"widened: unsupported dtype {dtype}")
+        out = ops.new_rows(self.buffer, rows, columns, dtype)
+        ops.microscaled_widen(self.codes_at, self.scales_at, self.factors_at, out, rows, columns)
         return out
 
 
@@ -210,8 +214,8 @@ def _product(x: "torch.Tensor | MicroscaledRows", tiles: Tiles, y: torch.Tensor,
     if isinstance(x, MicroscaledRows):
         x, rows = None, (x.codes_at, x.scales_at, x.factors_at)
     else:
-        scales, factors, size = _sizes(y.shape[0], tiles.columns, tiles.count if offsets else 0)
-        held = x.new_empty(size, dtype=torch.uint8)
+        scales, factors, size, _ = _sizes(y.shape[0], tiles.columns, tiles.count if offsets else 0)
+        held = ops.new_bytes(x, size)
         at = held.data_ptr()
         rows = (at, at + scales, at + factors)
     ops.microscaled_product(tiles.numbers, x, rows, y, act, limit, alpha, offsets, order, top, x_by_pair, row_scale, error_word)
@@ -268,7 +272,7 @@ class MicroscaledWeight:
         if dtype not in _OUT_DTYPES:
             raise ops.KernelError(f"linear: unsupported output dtype {dtype}")
         if out is None or out.dtype != dtype:
-            out = (x if isinstance(x, torch.Tensor) else x.buffer).new_empty((rows, width), dtype=dtype)
+            out = ops.new_rows(x if isinstance(x, torch.Tensor) else x.buffer, rows, width, dtype)
         elif out.shape != (rows, width) or (out.stride(1) != 1 and width > 1) or out.get_device() != x.get_device():
             raise ops.KernelError(f"linear: out is {tuple(out.shape)} on {out.device}, wanted {(rows, width)} with unit inner stride on {x.device}")
         if rows:
