@@ -46,8 +46,9 @@ __device__ __forceinline__ void ms_row_scale(uint32_t largest, float& r, float& 
 
 // Quotients are made with an approximate reciprocal and still rounded as the exact quotient is.  A border between two codes (or two scales) times the divisor has at
 // most seven significant bits, so a number of up to twelve is either on the border or off by 2^-12 of it, far more than the 2^-22 that the
-// product with the reciprocal is off by: rounded to 16 bits, it is on the border if and only if the exact quotient is.  A bf16 has eight bits; a 32-bit number
-// is first cut to twelve, the last of them set where any that was cut off is (which leaves it on the same side of every number of fewer bits).
+// product with the reciprocal is off by: rounded to 16 bits, or to multiples of 2^-16 (a border of codes is 1/4 or more), it is on the border if and only if the exact
+// quotient is.  A bf16 has eight bits; a 32-bit number is first cut to twelve, the last of them set where any that was cut off is (which leaves it on the same side of
+// every number of fewer bits).
 template <typename T> __device__ __forceinline__ float ms_odd12(float v) {
   if constexpr (sizeof(T) == 2) return v;
   const uint32_t b = __float_as_uint(v);
@@ -82,14 +83,11 @@ template <typename T> __device__ __forceinline__ uint32_t ms_codes8(const float 
     for (int j = 0; j < 8; ++j) v[j] *= 0x1p32f;
     inverse *= 0x1p-32f;
   }
-  const f32x2 factor = f2_pack(inverse * reciprocal, inverse * reciprocal);
+  // (192 + q is a multiple of 2^-16; a quotient is at most 9, where a scale of 1.5 * 2^-9 was rounded to 2^-9)
+  const f32x2 factor = f2_pack(inverse * reciprocal, inverse * reciprocal), up = f2_pack(192.f, 192.f), down = f2_pack(-192.f, -192.f), one = f2_pack(1.f, 1.f);
   float q[8];
 #pragma unroll
-  for (int j = 0; j < 8; j += 2) {
-    f2_unpack(f2_mul(f2_pack(v[j], v[j + 1]), factor), q[j], q[j + 1]);
-    q[j] = ms_round16(q[j]);
-    q[j + 1] = ms_round16(q[j + 1]);
-  }
+  for (int j = 0; j < 8; j += 2) f2_unpack(f2_fma(f2_fma(f2_pack(v[j], v[j + 1]), factor, up), one, down), q[j], q[j + 1]);
   uint32_t codes;
   asm("{\n.reg .b8 a, b, c, d;\ncvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\ncvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\ncvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n"
       "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\nmov.b32 %0, {a, b, c, d};\n}\n"
