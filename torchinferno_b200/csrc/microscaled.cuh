@@ -146,7 +146,7 @@ struct MsArgs {
   const unsigned char* w;          // codes of the matrices
   const unsigned char* w_scales;
   const float* w_factors;          // [experts, N]
-  int M, N, steps, stages;
+  int M, N, steps, stages, tmem_cols;
   const int* offsets;              // [experts + 1] of rows sorted by expert, or null: one matrix
   const int* order;
   int experts;

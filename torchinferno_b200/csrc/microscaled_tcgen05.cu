@@ -12,6 +12,8 @@
 // steps.  Every wait is bounded and reports in error_word.
 #include "microscaled.cuh"
 
+#include <algorithm>
+
 namespace tib {
 
 constexpr int kMtMaxExperts = 1024, kMtMaxStages = 8;
@@ -21,8 +23,10 @@ template <int NT> struct MtShape {
   static constexpr int kPerSm = NT <= 32 ? 2 : 1;                                // blocks of an SM
   static constexpr int kStorers = NT >= 128 ? 8 : 4, kThreads = 64 + 32 * kStorers, kCols = NT / (kStorers / 4);      // (columns of a storer)
   static constexpr int kTurn = NT >= 128 ? 16 : 8;                               // columns that it takes at a time
-  static constexpr uint32_t kTmemCols = 512 / kPerSm, kScaleCols = 2 * NT;       // two accumulators, then 32 columns of scales a stage
-  static constexpr int kStages = (kTmemCols - kScaleCols) / 32 < kMtMaxStages ? (kTmemCols - kScaleCols) / 32 : kMtMaxStages;
+  // Tensor memory: accumulators (two; one of a shared tile, which is a block's only one), then 32 columns of scales a stage.
+  static constexpr uint32_t tmem_cols(int splits) { return (splits > 1 ? 256 : 512) / kPerSm; }
+  __host__ __device__ static constexpr uint32_t scale_cols(int splits) { return splits > 1 ? NT : 2 * NT; }
+  static constexpr int stages(int splits) { return (tmem_cols(splits) - scale_cols(splits)) / 32 < kMtMaxStages ? (tmem_cols(splits) - scale_cols(splits)) / 32 : kMtMaxStages; }
   static constexpr uint32_t kStage = kMtWBytes + NT * kMsStepBytes + 2 * kMsStepScales;
 };
 // of the sums of a shared tile: (a column's 128 / splits sums and four more, so that those that a warp writes at a time fall on all banks)
@@ -74,7 +78,7 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tmem_slot), "r"(S::kTmemCols) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tmem_slot), "r"(a.tmem_cols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
   if (a.offsets) {
@@ -196,7 +200,7 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
         }
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         const uint32_t stage = base + s * S::kStage, scales = stage + kMtWBytes + NT * kMsStepBytes;
-        const uint32_t w_src = umma_low_k128(stage), x_src = w_src + (kMtWBytes >> 4), columns = tmem_base + S::kScaleCols + 32 * s;
+        const uint32_t w_src = umma_low_k128(stage), x_src = w_src + (kMtWBytes >> 4), columns = tmem_base + S::scale_cols(splits) + 32 * s;
         if (leader) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) ms_copy_scales<1>(columns + 4 * k, scales + kMsChunkBytes * k);      // (four of w, four of the rows)
@@ -327,7 +331,7 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
   __syncthreads();
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(a.tmem_cols) : "memory");
   }
 }
 
@@ -358,7 +362,7 @@ template <int NT> static int mt_plan(int M, int N, int steps, int experts, MtPla
   const int64_t most = (int64_t)ceil_div(steps, p.splits) * ceil_div64(tiles * p.splits, p.grid);
   p.steps = (int)(most < 0x7fffffff ? most : 0x7fffffff);
   p.stages = 1;
-  while (p.stages < S::kStages && p.stages < p.steps && mt_smem<NT>(p.stages + 1, p.splits, experts) <= (S::kPerSm > 1 ? 113u * 1024 : (uint32_t)kMostSmem)) ++p.stages;
+  while (p.stages < S::stages(p.splits) && p.stages < p.steps && mt_smem<NT>(p.stages + 1, p.splits, experts) <= (S::kPerSm > 1 ? 113u * 1024 : (uint32_t)kMostSmem)) ++p.stages;
   return TIB_OK;
 }
 // Rows of a tile: 32 where all rows are one tile, else 128 (the tiles of their scales).  A tile's time is that of its weights: 8, 32, 33, 64 and 128 rows
@@ -372,6 +376,7 @@ static int launch_mt(MsArgs& a, void* y, int64_t ldy, cudaStream_t stream) {
   const int rc = mt_plan<NT>(a.M, a.N, a.steps, experts, plan);
   if (rc != TIB_OK) return rc;
   a.stages = plan.stages;
+  a.tmem_cols = (int)MtShape<NT>::tmem_cols(plan.splits);
   auto kern = microscaled_tcgen05_kernel<NT, ACT, TO>;
   static bool allowed[64];      // (by device: the attribute belongs to its context)
   int device = 0;
@@ -382,6 +387,9 @@ static int launch_mt(MsArgs& a, void* y, int64_t ldy, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(MtShape<NT>::kThreads);
   cfg.dynamicSmemBytes = mt_smem<NT>(plan.stages, plan.splits, experts);
+  // Blocks that wait for others of their cluster must not wait for tensor memory that a block of another such cluster holds while it waits for one that cannot have it here
+  // (two streams' calls): a shared tile's block takes as large a share of an SM's shared memory (228 KB, 1 KB of it for each block itself) as of its 512 columns.
+  if (plan.splits > 1) cfg.dynamicSmemBytes = std::max(cfg.dynamicSmemBytes, (size_t)a.tmem_cols * (228 * 1024 / 512) - 1024);
   cfg.stream = stream;
   cfg.gridDim = dim3((unsigned)plan.grid);
   cudaLaunchAttribute attr[2];

@@ -22,8 +22,11 @@ struct QnArgs {
   int64_t lds;
   int hidden;
   float eps;
-  int groups;
+  int groups, n_rows;          // n_rows: of the residual
 };
+
+// The row of the residual that row `orow` is (an index is kept within what there is)
+__device__ __forceinline__ int qn_row(const QnArgs& a, int orow) { return a.rows ? min(max(a.rows[orow], 0), a.n_rows - 1) : orow; }
 
 // Eight numbers to eight 8-bit codes
 __device__ __forceinline__ uint2 qn_bytes8(const float (&v)[8], float inverse) {
@@ -82,7 +85,7 @@ quantized_norm_bf16x8_kernel(const QnArgs a) {
   pdl_trigger();
   __shared__ float scratch[33];
   __shared__ uint32_t scratch_max[32];
-  const int orow = blockIdx.x, srow = a.rows ? a.rows[orow] : orow, c = threadIdx.x * 8;
+  const int orow = blockIdx.x, srow = qn_row(a, orow), c = threadIdx.x * 8;
   const bool active = c < a.hidden;
   float h[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   float ss = 0.f;
@@ -140,7 +143,7 @@ quantized_norm_f32x4_kernel(const QnArgs a, int virtuals) {
   extern __shared__ float normed_row[];      // [hidden rounded up to 256]
   __shared__ float scratch[32];
   __shared__ uint32_t scratch_max[32];
-  const int orow = blockIdx.x, srow = a.rows ? a.rows[orow] : orow, lane = threadIdx.x & 31;
+  const int orow = blockIdx.x, srow = qn_row(a, orow), lane = threadIdx.x & 31;
   const size_t at = (size_t)srow * a.hidden;
   const float* delta = static_cast<const float*>(a.delta);
   const int c0 = threadIdx.x * 4 < virtuals ? threadIdx.x * 4 : a.hidden;      // (threads beyond have no column)
@@ -209,7 +212,7 @@ quantized_norm_held_kernel(const QnArgs a) {
   extern __shared__ float normed_row[];      // [hidden rounded up to 256]
   __shared__ float scratch[33];
   __shared__ uint32_t scratch_max[32];
-  const int orow = blockIdx.x, srow = a.rows ? a.rows[orow] : orow;
+  const int orow = blockIdx.x, srow = qn_row(a, orow);
   const size_t at = (size_t)srow * a.hidden;
   const T* delta = static_cast<const T*>(a.delta);
   float h[kQnHeld];
@@ -259,7 +262,7 @@ __global__ void quantized_norm_kernel(const QnArgs a) {
   pdl_trigger();
   __shared__ float scratch[33];
   __shared__ uint32_t scratch_max[32];
-  const int orow = blockIdx.x, srow = a.rows ? a.rows[orow] : orow;
+  const int orow = blockIdx.x, srow = qn_row(a, orow);
   const float* res = a.residual + (size_t)srow * a.hidden;
   const T* delta = a.delta ? static_cast<const T*>(a.delta) + (size_t)srow * a.hidden : nullptr;
   // (h is added up anew where it is needed: residual and sum may be the same memory, where each thread reads and writes the columns of its own)
@@ -303,17 +306,17 @@ __global__ void quantized_norm_kernel(const QnArgs a) {
 
 using namespace tib;
 
-// residual [rows, hidden] fp32, delta [rows, hidden] in dtype or null; sum [rows, hidden] fp32 takes residual + delta (it may be residual itself; null: it is not kept, and
+// residual [n_rows, hidden] fp32, delta [n_rows, hidden] in dtype or null; sum [n_rows, hidden] fp32 takes residual + delta (it may be residual itself; null: it is not kept, and
 // with `rows`, indices of the n_out rows to norm, it has to be null).  bytes 0: codes, scales, factors as tib_microscaled_rows leaves them, 1: codes
 // [n_out, runs * 128] and factors = scales [runs, lds] as tib_quantize_rows does.  out: the normed rows in dtype, or null.
 TIB_API int tib_quantized_norm(const void* delta, const float* residual, float* sum, const int* rows, const float* weight, void* out, int bytes, void* codes,
-                               void* scales, float* factors, int64_t lds, int n_out, int hidden, float eps, int dtype, cudaStream_t stream) {
+                               void* scales, float* factors, int64_t lds, int n_out, int n_rows, int hidden, float eps, int dtype, cudaStream_t stream) {
   if (n_out == 0) return TIB_OK;
-  if (!residual || !weight || !codes || !factors || (!bytes && !scales) || n_out < 0 || hidden < 1 || (rows && sum)) return TIB_E_ARG;
+  if (!residual || !weight || !codes || !factors || (!bytes && !scales) || n_out < 0 || n_rows < 1 || (!rows && n_out > n_rows) || hidden < 1 || (rows && sum)) return TIB_E_ARG;
   if (dtype != TIB_BF16 && dtype != TIB_F32) return TIB_E_DTYPE;
   if (bytes && lds < n_out) return TIB_E_SIZE;
   if (((uintptr_t)codes | (uintptr_t)scales) & 15) return TIB_E_ALIGN;
-  const QnArgs a{delta, residual, sum, rows, weight, out, (unsigned char*)codes, (unsigned char*)scales, factors, lds, hidden, eps, ms_groups(n_out, 0)};
+  const QnArgs a{delta, residual, sum, rows, weight, out, (unsigned char*)codes, (unsigned char*)scales, factors, lds, hidden, eps, ms_groups(n_out, 0), n_rows};
   if (dtype == TIB_BF16 && hidden % 8 == 0 && hidden <= 8192 &&
       (((uintptr_t)residual | (uintptr_t)sum | (uintptr_t)weight | (uintptr_t)out | (uintptr_t)delta) & 15) == 0) {
     const int threads = (hidden / 8 + 31) / 32 * 32;

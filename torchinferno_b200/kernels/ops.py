@@ -1414,7 +1414,7 @@ def quantized_norm(delta: torch.Tensor | None, residual: torch.Tensor, weight: t
         _need_on(kept, "new_residual", torch.float32, shape, device)
     _check("add_rmsnorm", lib().tib_quantized_norm(
         0 if delta is None else delta.data_ptr(), residual.data_ptr(), 0 if kept is None else kept.data_ptr(), 0 if rows is None else rows.data_ptr(), weight.data_ptr(),
-        0 if out is None else out.data_ptr(), in_bytes, codes, scales, factors, lds, count, shape[1], eps, _code(dtype), _stream()))
+        0 if out is None else out.data_ptr(), in_bytes, codes, scales, factors, lds, count, shape[0], shape[1], eps, _code(dtype), _stream()))
 
 
 def _need_on(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: int) -> None:
