@@ -20,8 +20,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? (HELD == 1 ? 5 : HELD ==
 microscaled_rows_kernel(const T* __restrict__ x, int64_t ldx, int x_rows, unsigned char* __restrict__ codes, unsigned char* __restrict__ scales,
                         float* __restrict__ factors, int rows, int K, int steps, int groups, const int* __restrict__ offsets, const int* __restrict__ order,
                         int experts, int top, int x_by_pair) {
+  pdl_trigger();      // (a product behind this kernel asks for its weights while the kernel before is still at work)
   pdl_wait();
-  pdl_trigger();
   __shared__ uint32_t scratch[32];
   const int row = blockIdx.x, runs = steps * (kMsStep / kMsRun);
   int from = row, tile = row >> 7, group = row >> 3, at = row;      // (at: from the first row of the expert)
@@ -86,7 +86,8 @@ microscaled_rows_kernel(const T* __restrict__ x, int64_t ldx, int x_rows, unsign
   }
 }
 
-// The numbers that quantised rows stand for: a thread takes a run.
+// The numbers that quantised rows stand for: a thread takes a run.  (s r, four bits and at least 2^-135, is exact.)  8,192 x 14,336: 55 us, 5.5 TB/s; half a run a thread takes
+// 72 us, two runs 57.
 template <typename TO>
 __global__ void __launch_bounds__(256)
 microscaled_widen_kernel(MsRows x, TO* __restrict__ out, int64_t ldo, int K, int steps, int per_row, int wide) {
@@ -95,13 +96,13 @@ microscaled_widen_kernel(MsRows x, TO* __restrict__ out, int64_t ldo, int K, int
   const int row = blockIdx.x / per_row, run = (blockIdx.x - row * per_row) * blockDim.x + threadIdx.x;
   if (run * kMsRun >= K) return;
   const uint2 c = *reinterpret_cast<const uint2*>(x.codes + ((size_t)(run >> 4) * x.groups + (row >> 3)) * kMsGroupBytes + ms_code_at(row & 7, (run & 15) * (kMsRun / 2)));
-  const float s = ms_scale_value(x.scales[((size_t)(row >> 7) * steps * 4 + (run >> 2)) * kMsChunkBytes + ms_scale_at(row & 127) + (run & 3)]), r = x.factors[row];
+  const float factor = ms_scale_value(x.scales[((size_t)(row >> 7) * steps * 4 + (run >> 2)) * kMsChunkBytes + ms_scale_at(row & 127) + (run & 3)]) * x.factors[row];
   float v[16];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float2 p = ms_numbers2(((j < 4 ? c.x : c.y) >> (8 * (j & 3))) & 0xffu);
-    v[2 * j] = p.x * s * r;
-    v[2 * j + 1] = p.y * s * r;
+    v[2 * j] = p.x * factor;
+    v[2 * j + 1] = p.y * factor;
   }
   TO* dst = out + (size_t)row * ldo + run * kMsRun;
   TO w[16];

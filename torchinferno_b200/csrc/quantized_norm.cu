@@ -81,8 +81,8 @@ __device__ __forceinline__ uint32_t qn_block_max(uint32_t v, uint32_t* scratch) 
 template <bool BYTES>
 __global__ void __launch_bounds__(1024)
 quantized_norm_bf16x8_kernel(const QnArgs a) {
+  pdl_trigger();      // (see microscaled_rows_kernel)
   pdl_wait();
-  pdl_trigger();
   __shared__ float scratch[33];
   __shared__ uint32_t scratch_max[32];
   const int orow = blockIdx.x, srow = qn_row(a, orow), c = threadIdx.x * 8;
@@ -138,8 +138,8 @@ quantized_norm_bf16x8_kernel(const QnArgs a) {
 template <bool BYTES, int HELD>
 __global__ void __launch_bounds__(256, HELD <= 4 ? 5 : 3)
 quantized_norm_f32x4_kernel(const QnArgs a, int virtuals) {
+  pdl_trigger();      // (see microscaled_rows_kernel)
   pdl_wait();
-  pdl_trigger();
   extern __shared__ float normed_row[];      // [hidden rounded up to 256]
   __shared__ float scratch[32];
   __shared__ uint32_t scratch_max[32];
@@ -207,8 +207,8 @@ quantized_norm_f32x4_kernel(const QnArgs a, int virtuals) {
 template <typename T, bool BYTES>
 __global__ void __launch_bounds__(1024)
 quantized_norm_held_kernel(const QnArgs a) {
+  pdl_trigger();      // (see microscaled_rows_kernel)
   pdl_wait();
-  pdl_trigger();
   extern __shared__ float normed_row[];      // [hidden rounded up to 256]
   __shared__ float scratch[33];
   __shared__ uint32_t scratch_max[32];
@@ -258,8 +258,8 @@ quantized_norm_held_kernel(const QnArgs a) {
 // Wider rows: the same, with the row read again for its norm and for its codes.
 template <typename T, bool BYTES>
 __global__ void quantized_norm_kernel(const QnArgs a) {
+  pdl_trigger();      // (see microscaled_rows_kernel)
   pdl_wait();
-  pdl_trigger();
   __shared__ float scratch[33];
   __shared__ uint32_t scratch_max[32];
   const int orow = blockIdx.x, srow = qn_row(a, orow);

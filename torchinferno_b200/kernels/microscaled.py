@@ -199,13 +199,14 @@ def _laid_out(stacks: Sequence[Sequence[MicroscaledMatrix]], paired: bool) -> Ti
             first += m.shape[0]
     if columns % 2:      # (the half byte behind the last column)
         codes[:, :, columns // 2] &= 15
-    if int(scales.max()) > 0x7e:
-        raise ValueError("the scales of a 4-bit matrix must be numbers, and none of them negative")
     # (piece p of 16 bytes of a step of row i: to piece p ^ (i % 8))
     pieces = torch.arange(8, device=device) ^ (torch.arange(TILE, device=device) % 8)[:, None]
     codes = codes.view(len(stacks), tiles, TILE, steps, 8, 16).transpose(2, 3)[:, :, :, torch.arange(TILE, device=device)[:, None], pieces].contiguous()
     # (row 32 a + b of a tile, run 4 c + d of a step: to [c][b][a][d])
     scales = scales.view(len(stacks), tiles, 4, 32, steps, 4, 4).permute(0, 1, 4, 5, 3, 2, 6).contiguous()
+    # (The products ask for their weights ahead of the kernels before them in the stream: this waits until all of the above is there.)
+    if int(scales.max()) > 0x7e:
+        raise ValueError("the scales of a 4-bit matrix must be numbers, and none of them negative")
     return Tiles(codes.view(len(stacks), tiles, steps, TILE, -1), scales.view(len(stacks), tiles, steps, -1), factors, columns, paired)
 
 
