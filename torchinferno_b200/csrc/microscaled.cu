@@ -15,6 +15,8 @@ __device__ __forceinline__ uint32_t ms_block_max(uint32_t v, uint32_t* scratch) 
 
 // A block takes a row, a thread runs of 16 columns of it, HELD of which it keeps: the row's largest number has to be known before the first code is.  (Wider rows
 // are read again, from the L2.)  What is held decides how many blocks an SM has, and these what is on its way.
+// What bounds it: its instructions (74 % of the issue slots are used) and memory alike: 8,192 x 14,336 bf16 55 us, 5.4 TB/s; 8,192 x 4,096 17.7 us, in 32 bits 25.8.  (Tried: blocks
+// that stay and ask for their next row ahead of this one's codes, 86 and 28 us, of half as many threads an SM.)
 template <typename T, bool VEC, int HELD>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 ? (HELD == 1 ? 5 : HELD == 2 ? 4 : 2) : HELD == 1 ? 6 : HELD == 2 ? 5 : 4)
 microscaled_rows_kernel(const T* __restrict__ x, int64_t ldx, int x_rows, unsigned char* __restrict__ codes, unsigned char* __restrict__ scales,

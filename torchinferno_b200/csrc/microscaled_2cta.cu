@@ -9,6 +9,11 @@
 //   warp 0       TMA producer into a ring of five stages      warp 1 (of the even block)   copies scales and issues the MMAs; either owns its block's TMEM
 //   warps 4..11  epilogue, 32 rows x 128 features each: read into registers at once, so that the next tile's MMAs may begin, then finished.  These take registers
 //                that the first four warps give up (168 a thread at launch, 40 + 2 x 232 after)
+// What bounds it: the step, and behind the last of a tile its reading.  8,192 rows -> 28,672: 153, 368 and 663 us at 1,024, 4,096 and 8,192 columns, so 0.37 us a step of
+// 256 (some 690 cycles, where the MMAs take 512) and 1.6 us a tile beside them.  Without the copies from memory a step takes 0.31 us (the MMAs read 32 KB of shared memory a step,
+// the scales' copies 6, and 38 KB are written: 76 KB for a port of 128 bytes a cycle are 594), and without the outputs a tile costs 0.3 us: those are 64 KB a block through
+// the same paths.  The gated product of 8,192 rows 4,096 -> 2 x 14,336 takes 0.34 ms, 5,600 TFLOP/s, 0.36 with its rows' codes, in a row under the power limit 0.42.  (What
+// took it there from 0.62 ms: see ms_umma; the features' factors read from shared memory in place of global, 0.38 to 0.37.)
 // Every wait is bounded and reports in error_word; no block leaves before its partner is done and what was sent to it has come; every copy lands in the block that
 // issued it.
 #include "microscaled.cuh"
