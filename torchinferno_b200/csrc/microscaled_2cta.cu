@@ -9,11 +9,12 @@
 //   warp 0       TMA producer into a ring of five stages      warp 1 (of the even block)   copies scales and issues the MMAs; either owns its block's TMEM
 //   warps 4..11  epilogue, 32 rows x 128 features each: read into registers at once, so that the next tile's MMAs may begin, then finished.  These take registers
 //                that the first four warps give up (168 a thread at launch, 40 + 2 x 232 after)
-// What bounds it: the step, and behind the last of a tile its reading.  8,192 rows -> 28,672: 153, 368 and 663 us at 1,024, 4,096 and 8,192 columns, so 0.37 us a step of
+// What bounds it: the step, and behind the last of a tile its reading.  8,192 rows -> 28,672: 146, 368 and 663 us at 1,024, 4,096 and 8,192 columns, so 0.37 us a step of
 // 256 (some 690 cycles, where the MMAs take 512) and 1.6 us a tile beside them.  Without the copies from memory a step takes 0.31 us (the MMAs read 32 KB of shared memory a step,
 // the scales' copies 6, and 38 KB are written: 76 KB for a port of 128 bytes a cycle are 594), and without the outputs a tile costs 0.3 us: those are 64 KB a block through
 // the same paths.  The gated product of 8,192 rows 4,096 -> 2 x 14,336 takes 0.34 ms, 5,600 TFLOP/s, 0.36 with its rows' codes, in a row under the power limit 0.42.  (What
-// took it there from 0.62 ms: see ms_umma; the features' factors read from shared memory in place of global, 0.38 to 0.37.)
+// took it there from 0.62 ms: see ms_umma; the features' factors read from shared memory in place of global, 0.38 to 0.37; a tile's factors asked for a tile ahead, at 1,024
+// columns 154 to 146.)
 // Every wait is bounded and reports in error_word; no block leaves before its partner is done and what was sent to it has come; every copy lands in the block that
 // issued it.
 #include "microscaled.cuh"
@@ -121,12 +122,23 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
     const int quarter = warp & 3, half = (warp - 4) >> 2, et = threadIdx.x - 128;
     uint32_t acc_phase = 0;
     bool ok = true;
+    // A tile's factors (of a feature, of this thread's row and of its pair) are asked for while the tile before is finished.
+    float w_factor = 0.f, x_factor = 0.f, pair_factor = 1.f;
+    auto ask = [&](const M2Tile& m) {
+      const int row = min(m.first + (int)rank * 128 + quarter * 32 + lane, m.first + m.rows - 1);
+      w_factor = a.w_factors[(size_t)m.expert * a.N + min(m.n_tile * 256 + et, a.N - 1)];
+      x_factor = a.x.factors[row];
+      if (a.row_scale) pair_factor = a.row_scale[bs_pair(a.order, row, a.M)];
+    };
+    M2Tile next = {};
+    if (pair < num_tiles) ask(next = tile_of(pair));
     for (int t = pair; t < num_tiles; t += pairs, acc_phase ^= 1) {
-      const M2Tile m = tile_of(t);
+      const M2Tile m = next;
       const int in_tile = (int)rank * 128 + quarter * 32 + lane, row = m.first + in_tile, last = m.first + m.rows;      // (rows from `last` on are not stored)
       const int col0 = m.n_tile * 256 + half * 128;
-      const float x_factor = a.x.factors[min(row, last - 1)], pair_factor = a.row_scale ? a.row_scale[bs_pair(a.order, min(row, last - 1), a.M)] : 1.f;
-      tile_factors[acc_phase * 256 + et] = a.w_factors[(size_t)m.expert * a.N + min(m.n_tile * 256 + et, a.N - 1)];
+      tile_factors[acc_phase * 256 + et] = w_factor;
+      const f32x2 x_factor2 = f2_pack(x_factor, x_factor), pair_factor2 = f2_pack(pair_factor, pair_factor);
+      if (t + pairs < num_tiles) ask(next = tile_of(t + pairs));
       asm volatile("bar.sync 1, 256;\n" ::: "memory");      // (the last tile but one is finished: its factors have been read)
       if (ok && !mbar_wait_warp(acc_full_bar, acc_phase)) {
         if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00F3);
@@ -144,7 +156,6 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
       // (what this orders is the reading of tensor memory, which tcgen05.fence has ordered: no fence of the cluster)
       if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(map_to_cta(acc_empty_bar, 0)) : "memory");
       f32x2 sum[64];
-      const f32x2 x_factor2 = f2_pack(x_factor, x_factor);
       const ulonglong2* factors2 = reinterpret_cast<const ulonglong2*>(tile_factors + acc_phase * 256 + half * 128);
 #pragma unroll
       for (int c = 0; c < 64; c += 2) {      // (see ms_scaled)
@@ -153,7 +164,6 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
         sum[c + 1] = f2_mul(f2_mul(f2_pack(__uint_as_float(v[c >> 4][(2 * c & 31) + 2]), __uint_as_float(v[c >> 4][(2 * c & 31) + 3])), f.y), x_factor2);
       }
       if (a.row_scale) {
-        const f32x2 pair_factor2 = f2_pack(pair_factor, pair_factor);
 #pragma unroll
         for (int c = 0; c < 64; ++c) sum[c] = f2_mul(sum[c], pair_factor2);
       }
