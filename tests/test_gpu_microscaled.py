@@ -492,6 +492,7 @@ def test_refusals():
                  lambda: microscaled.add_rmsnorm(x, residual, ones, 1e-5, new_residual=torch.empty(4, 199, device=DEV)),
                  lambda: microscaled.add_rmsnorm(x, residual, ones, 1e-5, rows=torch.zeros(2, dtype=torch.int64, device=DEV)),
                  lambda: microscaled.add_rmsnorm(x, residual, ones, 1e-5, rows=torch.zeros(2, dtype=torch.int32, device=DEV), new_residual=residual.clone()),
+                 lambda: microscaled.add_rmsnorm(x, residual, ones, 1e-5, out=x), lambda: microscaled.add_rmsnorm(None, residual, ones, 1e-5, dtype=F32, out=residual),
                  lambda: block_scaled.add_rmsnorm(x.t().contiguous().t(), residual, ones, 1e-5)):
         with pytest.raises(ops.KernelError):
             call()

@@ -1408,6 +1408,8 @@ def quantized_norm(delta: torch.Tensor | None, residual: torch.Tensor, weight: t
             raise KernelError("add_rmsnorm: with rows the residual is left as it is")
     if out is not None:
         _need_on(out, "out", dtype, (count, shape[1]), device)
+        if count and out.data_ptr() in [t.data_ptr() for t in (delta, residual, new_residual) if t is not None]:
+            raise KernelError("add_rmsnorm: out is not the memory of another operand (a row is read again after its normed form is written)")
     kept = residual if delta is not None and rows is None else None
     if new_residual is not None:
         kept = new_residual
