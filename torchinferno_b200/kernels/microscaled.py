@@ -189,14 +189,14 @@ def _laid_out(stacks: Sequence[Sequence[MicroscaledMatrix]], paired: bool) -> Ti
     codes = torch.zeros((len(stacks), tiles * TILE, steps * (STEP // 2)), dtype=torch.uint8, device=device)
     scales = torch.zeros((len(stacks), tiles * TILE, steps * (STEP // RUN)), dtype=torch.uint8, device=device)
     factors = torch.empty((len(stacks), features), dtype=torch.float32, device=device)
-    for i, stack in enumerate(stacks):
-        first = 0
-        for j, m in enumerate(stack):
-            at = slice(j, features, 2) if paired else slice(first, first + m.shape[0])
-            codes[i, at, :m.codes.shape[1]] = m.codes
-            scales[i, at, :m.scales.shape[1]] = m.scales.view(torch.uint8)
-            factors[i, at] = m.factor.reshape(())
-            first += m.shape[0]
+    first = 0
+    for j, height in enumerate(heights):      # (all stacks' j-th matrices at once)
+        at = slice(j, features, 2) if paired else slice(first, first + height)
+        part = [stack[j] for stack in stacks]
+        codes[:, at, :part[0].codes.shape[1]] = torch.stack([m.codes for m in part]) if len(part) > 1 else part[0].codes
+        scales[:, at, :part[0].scales.shape[1]] = torch.stack([m.scales.view(torch.uint8) for m in part]) if len(part) > 1 else part[0].scales.view(torch.uint8)
+        factors[:, at] = torch.stack([m.factor.reshape(1) for m in part])
+        first += height
     if columns % 2:      # (the half byte behind the last column)
         codes[:, :, columns // 2] &= 15
     # (piece p of 16 bytes of a step of row i: to piece p ^ (i % 8))

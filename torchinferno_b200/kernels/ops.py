@@ -105,7 +105,7 @@ def _current_device() -> int:
 
 
 # (the allocation alone, on the current device: 0.9 us where new_empty takes 1.5 to 2.4, the calls below allocating twice each)
-_empty_strided_cuda = getattr(torch._C._dynamo.guards, "_empty_strided_cuda", None)
+_empty_strided_cuda = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
 
 
 def new_bytes(like: torch.Tensor, size: int) -> torch.Tensor:
