@@ -612,3 +612,30 @@ def test_a_layer_reads_its_norms_rows_in_8_bits_as_before(tmp_path, monkeypatch)
         with _engine(folder, "bfloat16", page_size=16, max_batch_size=4) as engine:
             outs.append(_generate(engine, prompts, 8))
     assert outs[0] == outs[1]
+
+
+@pytest.mark.parametrize("form", [NVFP4, {"quant_method": "fp8", "weight_block_size": [128, 128]}])
+def test_kernels_let_in_early_change_nothing(form):
+    """Prompts in portions and captured decode steps give the same tokens whether a kernel is placed while the one ahead of it is at work or not."""
+    need_gpu()
+    from conftest import TINY_D
+    from torchinferno_b200.engine.batch import StepEntry
+    from torchinferno_b200.engine.factory import make_runner, random_model
+    config = {**TINY_D, "quantization_config": form}
+    outs = []
+    with torch.inference_mode():
+        model = random_model(config, seed=0, dtype="bfloat16")
+        prompts = torch.randint(0, config["vocab_size"], (12, 90), generator=torch.Generator().manual_seed(1)).tolist()
+        for early in (True, False):
+            before = ops.set_dependent_launch(early)
+            try:
+                runner = make_runner(model, page_size=16, max_tokens=12 * 320, max_requests=12, max_request_tokens=300)
+                ids = [f"r{i}" for i in range(12)]
+                for at in (0, 40):
+                    logits = runner.step([StepEntry(i, p[at:at + 50 if at else 40], [49] if at else []) for i, p in zip(ids, prompts)])
+                first = logits.argmax(1).tolist()
+                outs.append((first, runner.decode_loop(ids, first, 150, temperature=[0.0] * 12, seeds=list(range(12))).cpu().clone()))
+                runner.end(ids)
+            finally:
+                ops.set_dependent_launch(before)
+    assert outs[0][0] == outs[1][0] and torch.equal(outs[0][1], outs[1][1])

@@ -269,3 +269,26 @@ def test_experts_are_bound_in_codes():
     for moe in moes:
         assert isinstance(moe.up_weight, MicroscaledExperts) and moe.up_weight.paired == moe.glu and moe.up_weight.experts == moe.experts
         assert isinstance(moe.down_weight, MicroscaledExperts) and moe.router_weight.dtype == torch.float32 and moe.rows_form(3) is None
+
+
+def test_what_the_library_refuses():
+    """Refused by their arguments alone, before anything is launched: null pointers, sizes, types, alignment, and activations that do not fit."""
+    lib = ops.lib()
+    at = 1 << 20      # (an address that nothing reads)
+    rows = dict(x=at, x_dtype=1, ldx=64, x_rows=4, codes=at, scales=at, factors=at, rows=4, K=64, offsets=0, order=0, experts=1, top=1, x_by_pair=0, stream=0)
+    for wrong, status in ((dict(x=0), -5), (dict(codes=0), -5), (dict(K=0), -5), (dict(rows=-1), -5), (dict(x_rows=3), -5), (dict(x_dtype=2), -1), (dict(codes=at + 8), -3),
+                          (dict(scales=at + 4), -3), (dict(offsets=at, x_by_pair=1), -5), (dict(top=0), -5), (dict(rows=0, x=0), 0)):
+        assert lib.tib_microscaled_rows(*{**rows, **wrong}.values()) == status, wrong
+    widen = dict(codes=at, scales=at, factors=at, out=at, out_dtype=1, ldo=64, rows=4, K=64, stream=0)
+    for wrong, status in ((dict(out=0), -5), (dict(K=0), -5), (dict(out_dtype=7), -1), (dict(codes=at + 1), -3), (dict(rows=0), 0)):
+        assert lib.tib_microscaled_widen(*{**widen, **wrong}.values()) == status, wrong
+    product = dict(w=at, w_scales=at, w_factors=at, pairs=0, N=8, K=64, experts=1, x=0, x_dtype=1, ldx=0, x_rows=0, codes=at, scales=at, factors=at, make=0, y=at, y_dtype=1, ldy=8,
+                   M=4, offsets=0, order=0, top=1, x_by_pair=0, act=0, limit=0.0, alpha=0.0, row_scale=0, error_word=0, stream=0)
+    for wrong, status in ((dict(w=0), -5), (dict(y=0), -5), (dict(codes=0), -5), (dict(K=0), -5), (dict(M=-1), -5), (dict(experts=0), -5), (dict(make=1), -5), (dict(offsets=at), -5),
+                          (dict(row_scale=at), -5), (dict(act=9), -2), (dict(act=4), -2), (dict(pairs=1, N=7), -2), (dict(y_dtype=2), -1), (dict(w=at + 8), -3),
+                          (dict(offsets=at, order=at, experts=2000), -2), (dict(N=1 << 30, K=1 << 20), -2), (dict(M=0), 0), (dict(N=0), 0)):
+        assert lib.tib_microscaled_product(*{**product, **wrong}.values()) == status, wrong
+    norm = dict(delta=0, residual=at, sum=0, rows=0, weight=at, out=0, bytes=0, codes=at, scales=at, factors=at, lds=0, n_out=4, n_rows=4, hidden=64, eps=1e-5, dtype=1, stream=0)
+    for wrong, status in ((dict(residual=0), -5), (dict(weight=0), -5), (dict(scales=0), -5), (dict(rows=at, sum=at), -5), (dict(n_out=5), -5), (dict(hidden=0), -5),
+                          (dict(dtype=3), -1), (dict(bytes=1, lds=3), -2), (dict(codes=at + 4), -3), (dict(n_out=0), 0)):
+        assert lib.tib_quantized_norm(*{**norm, **wrong}.values()) == status, wrong
