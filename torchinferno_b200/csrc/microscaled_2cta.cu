@@ -6,7 +6,7 @@
 // slice, and gets rows r * 128 .. of the accumulator, which needs the scales of its own rows and of all 256 features.  A step is 256 columns: the 128-byte
 // row of the swizzle, twelve copies of scales to tensor memory, four MMAs.  The accumulator (256 columns) stays in tensor memory for the whole sum; beside it
 // every stage of the ring has 48 columns for its scales.
-//   warp 0       TMA producer into a ring of five stages      warp 1 (of the even block)   copies scales and issues the MMAs; either owns its block's TMEM
+//   warp 0       TMA producer into a ring of five stages, the first weights ahead of the end of the kernel before      warp 1 (of the even block)   copies scales and issues the MMAs; either owns its block's TMEM
 //   warps 4..11  epilogue, 32 rows x 128 features each: read into registers at once, so that the next tile's MMAs may begin, then finished.  These take registers
 //                that the first four warps give up (168 a thread at launch, 40 + 2 x 232 after)
 // What bounds it: the step, and behind the last of a tile its reading.  8,192 rows -> 28,672: 146, 368 and 663 us at 1,024, 4,096 and 8,192 columns, so 0.37 us a step of
@@ -67,7 +67,7 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tmem_slot), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
   }
-  pdl_wait();
+  if (a.offsets) pdl_wait();                               // (of one matrix, each warp waits where it first needs what the kernel ahead leaves)
   if (a.offsets && warp == 0) {                            // the experts' row tiles, summed
     int before = 0;
     for (int e0 = 0; e0 < a.experts; e0 += 32) {
@@ -131,6 +131,7 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
       if (a.row_scale) pair_factor = a.row_scale[bs_pair(a.order, row, a.M)];
     };
     M2Tile next = {};
+    if (!a.offsets) pdl_wait();
     if (pair < num_tiles) ask(next = tile_of(pair));
     for (int t = pair; t < num_tiles; t += pairs, acc_phase ^= 1) {
       const M2Tile m = next;
@@ -231,30 +232,46 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;\n");
     if (warp == 0) {
       const uint32_t leader = umma_leader();
-      int s = 0;
+      int ahead = 0, it = 0, s = 0;
       uint32_t phase = 1;
       bool ok = true;
+      const int blocks = (a.N + 127) >> 7;
+      // (a pair's second tile of features may lie behind the matrix: it reads the last one instead, which is not stored)
+      auto w_at = [&](const M2Tile& m, int half) { return (m.expert * blocks + min(m.n_tile * 2 + half, blocks - 1)) * a.steps; };
+      // (a step's five copies; x's last two by themselves where the weights' are on their way already)
+      auto ask = [&](int w0, int s0, int s1, int xs0, int group, int step, int s, bool w, bool x) {
+        if (w && rank == 0) mbar_expect_tx(full_bar(s), 2 * kM2Stage);
+        const uint32_t bar0 = map_to_cta(full_bar(s), 0), stage = base + s * kM2Stage, scales = stage + 2 * kM2Half;
+        if (x) pair_tma_load(stage, &map_x, 0, step * a.x.groups + group, bar0);
+        if (w) pair_tma_load(stage + kM2Half, &map_w, 0, (w0 + step) << 4, bar0);
+        if (x) pair_tma_load(scales, &map_xs, 0, (xs0 + step) << 2, bar0);
+        if (w) {
+          pair_tma_load(scales + kMsStepScales, &map_ws, 0, (s0 + step) << 2, bar0);
+          pair_tma_load(scales + 2 * kMsStepScales, &map_ws, 0, (s1 + step) << 2, bar0);
+        }
+      };
+      if (!a.offsets) {      // the first weights: they do not wait for the kernel ahead
+        for (int t = pair; t < num_tiles && ahead < kM2Stages; t += pairs) {
+          const M2Tile m = tile_of(t);
+          for (int step = 0; step < a.steps && ahead < kM2Stages; ++step, ++ahead)
+            if (leader) ask(w_at(m, (int)rank), w_at(m, 0), w_at(m, 1), 0, 0, step, ahead, true, false);
+        }
+        pdl_wait();
+      }
       for (int t = pair; t < num_tiles && ok; t += pairs) {
         const M2Tile m = tile_of(t);
+        const int w0 = w_at(m, (int)rank), s0 = w_at(m, 0), s1 = w_at(m, 1), xs0 = (m.scale_tile + (int)rank) * a.steps;
         const int group = m.group + (int)rank * 16;        // (behind the tile's rows come others', which are not stored, or zeros)
-        const int blocks = (a.N + 127) >> 7;
-        // (a pair's second tile of features may lie behind the matrix: it reads the last one instead, which is not stored)
-        auto w_at = [&](int tile) { return (m.expert * blocks + min(tile, blocks - 1)) * a.steps; };
-        const int w0 = w_at(m.n_tile * 2 + (int)rank), s0 = w_at(m.n_tile * 2), s1 = w_at(m.n_tile * 2 + 1);
-        for (int step = 0; step < a.steps; ++step) {
-          if (!mbar_wait_warp(empty_bar(s), phase)) {
-            if (a.error_word && leader) atomicExch(a.error_word, 0x7C00F1);
-            ok = false;
-            break;
-          }
-          if (leader) {
-            if (rank == 0) mbar_expect_tx(full_bar(s), 2 * kM2Stage);
-            const uint32_t bar0 = map_to_cta(full_bar(s), 0), stage = base + s * kM2Stage, scales = stage + 2 * kM2Half;
-            pair_tma_load(stage, &map_x, 0, step * a.x.groups + group, bar0);
-            pair_tma_load(stage + kM2Half, &map_w, 0, (w0 + step) << 4, bar0);
-            pair_tma_load(scales, &map_xs, 0, ((m.scale_tile + (int)rank) * a.steps + step) << 2, bar0);
-            pair_tma_load(scales + kMsStepScales, &map_ws, 0, (s0 + step) << 2, bar0);
-            pair_tma_load(scales + 2 * kMsStepScales, &map_ws, 0, (s1 + step) << 2, bar0);
+        for (int step = 0; step < a.steps; ++step, ++it) {
+          if (it < ahead) {
+            if (leader) ask(w0, s0, s1, xs0, group, step, s, false, true);
+          } else {
+            if (!mbar_wait_warp(empty_bar(s), phase)) {
+              if (a.error_word && leader) atomicExch(a.error_word, 0x7C00F1);
+              ok = false;
+              break;
+            }
+            if (leader) ask(w0, s0, s1, xs0, group, step, s, true, true);
           }
           __syncwarp();
           if (++s == kM2Stages) { s = 0; phase ^= 1; }
@@ -270,6 +287,7 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
       }
     } else if (warp == 1 && rank == 0) {
       const uint32_t leader = umma_leader();
+      if (!a.offsets) pdl_wait();      // (the bounded waits begin when the kernel ahead is over)
       int s = 0;
       uint32_t phase = 0, acc_phase = 1;
       bool ok = true;
