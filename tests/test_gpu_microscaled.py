@@ -106,7 +106,8 @@ def test_widened_rows_in_both_types():
 
 # ------------------------------------------------------------------------------------------------ norms that leave quantised rows
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("m, k", [(1, 1), (8, 4096), (3, 520), (130, 1000), (5, 2055), (2, 9000), (7, 8192), (1, 264)])
+@pytest.mark.parametrize("m, k", [(1, 1), (8, 4096), (3, 520), (130, 1000), (5, 2055), (2, 9000), (7, 8192), (1, 264), (3, 1004), (9, 4100), (2, 8196), (300, 10240), (5, 16384), (2, 9002),
+                                  (2, 16388)])
 def test_a_norm_leaves_the_codes_of_its_rows(m, k, dtype):
     need_gpu()
     g = torch.Generator().manual_seed(m + k)

@@ -6,12 +6,13 @@
 // It lets the kernel behind it in before it waits for the one ahead.  That is as good for whoever waits: a kernel is over only when the one ahead of it is.  What kernels behind it read
 // before they wait (weights, positions, older pages of the cache) was there before the step's first kernels, which wait before they let anybody in.
 // What bounds it: memory.  8,192 x 4,096 bf16: 61.7 us for 354 MB (5.7 TB/s; tib_add_rmsnorm, whose rows leave in bf16, takes 60.9, and codes made behind it 17.7 more), in 32 bits
-// 69 us for 421 MB; eight rows 3.1 us, where tib_add_rmsnorm takes 2.5 and the codes 2.
+// 69 us for 421 MB; eight rows 2.9 us, where tib_add_rmsnorm takes 2.5 and the codes 2.
 #include "microscaled.cuh"
 
 namespace tib {
 
 constexpr int kQnHeld = 8, kQnWidth = 8 * 1024;      // columns of a thread of those that norm a row, of a row that a block keeps
+constexpr int kQnFoursWidth = 16 * 1024;             // the same of a row read four columns a load
 
 struct QnArgs {
   const void* delta;           // [rows, hidden] in the rows' type, or null
@@ -148,12 +149,30 @@ quantized_norm_bf16x8_kernel(const QnArgs a) {
   qn_codes8<__nv_bfloat16, BYTES>(a, orow, threadIdx.x, v, r, inverse, (a.hidden + kMsStep - 1) / kMsStep);
 }
 
-// 32-bit rows of a multiple of four columns, up to 8 * 1024: four columns a load.  The sums are those of `virtuals` threads that each add up every virtuals-th column
+// Four neighbours of a row, in 32 bits and back (rounded: what comes back is what was stored).
+__device__ __forceinline__ float4 qn_load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 qn_load4(const __nv_bfloat16* p) {
+  const uint2 raw = *reinterpret_cast<const uint2*>(p);
+  return make_float4(__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u), __uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u));
+}
+__device__ __forceinline__ float4 qn_store4(float* p, float4 v) {
+  if (p) *reinterpret_cast<float4*>(p) = v;
+  return v;
+}
+__device__ __forceinline__ float4 qn_store4(__nv_bfloat16* p, float4 v) {
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+  if (p) *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  return make_float4(__low2float(lo), __high2float(lo), __low2float(hi), __high2float(hi));
+}
+
+// Rows of a multiple of four columns, up to 16 * 1024: four columns a load.  The sums are those of `virtuals` threads that each add up every virtuals-th column
 // (add_rmsnorm_kernel's), of which a thread is four neighbours: what is a shuffle over 1 and 2 lanes there is an addition here, what is one over 4, 8 and 16 one
-// over 1, 2 and 4.  A quarter of the threads a row is four times as many rows on an SM.
-template <bool BYTES, int HELD>
-__global__ void __launch_bounds__(256, HELD <= 4 ? 5 : 3)
-quantized_norm_f32x4_kernel(const QnArgs a, int virtuals) {
+// over 1, 2 and 4.  A quarter of the threads a row is four times as many rows on an SM.  Of long rows eight loads a thread are asked for at a time: all 16 ahead of
+// the first sum take more registers than two blocks an SM leave (2,048 rows of 16,384 in bf16: 89 us, so 106; quantized_norm_kernel takes 179).
+// 8 rows of 14,336 in bf16 take 7.7 us (12.4 there; the norm and the codes by two kernels 9.8).
+template <typename T, bool BYTES, int HELD>
+__global__ void __launch_bounds__(256, HELD <= 4 ? 5 : HELD <= 8 ? 3 : 2)
+quantized_norm_x4_kernel(const QnArgs a, int virtuals) {
   pdl_trigger();      // (see microscaled_rows_kernel)
   pdl_wait();
   extern __shared__ float normed_row[];      // [hidden rounded up to 256]
@@ -161,26 +180,32 @@ quantized_norm_f32x4_kernel(const QnArgs a, int virtuals) {
   __shared__ uint32_t scratch_max[32];
   const int orow = blockIdx.x, srow = qn_row(a, orow), lane = threadIdx.x & 31;
   const size_t at = (size_t)srow * a.hidden;
-  const float* delta = static_cast<const float*>(a.delta);
+  const T* delta = static_cast<const T*>(a.delta);
+  T* out = a.out ? static_cast<T*>(a.out) + (size_t)orow * a.hidden : nullptr;
   const int c0 = threadIdx.x * 4 < virtuals ? threadIdx.x * 4 : a.hidden;      // (threads beyond have no column)
-  float4 h[HELD], d[HELD];
+  constexpr int ASKED = HELD < 8 ? HELD : 8;      // (at a time: registers)
+  float4 h[HELD], ss = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < HELD; ++i) {
-    const int c = c0 + i * virtuals;
-    h[i] = d[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (c < a.hidden) {
-      h[i] = *reinterpret_cast<const float4*>(a.residual + at + c);
-      if (delta) d[i] = *reinterpret_cast<const float4*>(delta + at + c);
+  for (int first = 0; first < HELD; first += ASKED) {
+    float4 d[ASKED];
+#pragma unroll
+    for (int i = 0; i < ASKED; ++i) {
+      const int c = c0 + (first + i) * virtuals;
+      h[first + i] = d[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c < a.hidden) {
+        h[first + i] = qn_load4(a.residual + at + c);
+        if (delta) d[i] = qn_load4(delta + at + c);
+      }
     }
-  }
-  float4 ss = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < HELD; ++i) {
-    const int c = c0 + i * virtuals;
-    if (c >= a.hidden) break;
-    if (delta) h[i] = make_float4(h[i].x + d[i].x, h[i].y + d[i].y, h[i].z + d[i].z, h[i].w + d[i].w);
-    if (a.sum) *reinterpret_cast<float4*>(a.sum + at + c) = h[i];
-    ss.x += h[i].x * h[i].x; ss.y += h[i].y * h[i].y; ss.z += h[i].z * h[i].z; ss.w += h[i].w * h[i].w;
+    for (int i = 0; i < ASKED; ++i) {
+      const int c = c0 + (first + i) * virtuals;
+      float4& v = h[first + i];
+      if (c >= a.hidden) break;
+      if (delta) v = make_float4(v.x + d[i].x, v.y + d[i].y, v.z + d[i].z, v.w + d[i].w);
+      if (a.sum) *reinterpret_cast<float4*>(a.sum + at + c) = v;
+      ss.x += v.x * v.x; ss.y += v.y * v.y; ss.z += v.z * v.z; ss.w += v.w * v.w;
+    }
   }
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) {
@@ -201,8 +226,7 @@ quantized_norm_f32x4_kernel(const QnArgs a, int virtuals) {
     const int c = c0 + i * virtuals;
     if (c >= a.hidden) break;
     const float4 w = *reinterpret_cast<const float4*>(a.weight + c);
-    const float4 y = make_float4(h[i].x * inv * w.x, h[i].y * inv * w.y, h[i].z * inv * w.z, h[i].w * inv * w.w);
-    if (a.out) *reinterpret_cast<float4*>(static_cast<float*>(a.out) + (size_t)orow * a.hidden + c) = y;
+    const float4 y = qn_store4(out ? out + c : nullptr, make_float4(h[i].x * inv * w.x, h[i].y * inv * w.y, h[i].z * inv * w.z, h[i].w * inv * w.w));
     *reinterpret_cast<float4*>(normed_row + c) = y;
     largest = max(max(max(largest, __float_as_uint(y.x) & 0x7fffffffu), max(__float_as_uint(y.y) & 0x7fffffffu, __float_as_uint(y.z) & 0x7fffffffu)), __float_as_uint(y.w) & 0x7fffffffu);
   }
@@ -214,11 +238,11 @@ quantized_norm_f32x4_kernel(const QnArgs a, int virtuals) {
     float v[8];
     const float4 lo = reinterpret_cast<const float4*>(normed_row)[2 * g], hi = reinterpret_cast<const float4*>(normed_row)[2 * g + 1];
     v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
-    qn_codes8<float, BYTES>(a, orow, g, v, r, inverse, steps);
+    qn_codes8<T, BYTES>(a, orow, g, v, r, inverse, steps);
   }
 }
 
-// Any width up to 8 * 1024, either type: the sums in add_rmsnorm_kernel's order (columns in turn, so many a thread that 8 hold them), the codes eight columns a
+// Any other width up to 8 * 1024, either type: the sums in add_rmsnorm_kernel's order (columns in turn, so many a thread that 8 hold them), the codes eight columns a
 // thread: in between the normed row crosses shared memory.
 template <typename T, bool BYTES>
 __global__ void __launch_bounds__(1024)
@@ -342,17 +366,31 @@ TIB_API int tib_quantized_norm(const void* delta, const float* residual, float* 
   }
   const int threads = norm_threads(hidden);
   const size_t smem = (size_t)ceil_div(hidden, kMsStep) * kMsStep * sizeof(float);
-  if (dtype == TIB_F32 && hidden % 4 == 0 && hidden <= kQnWidth &&
-      (((uintptr_t)residual | (uintptr_t)sum | (uintptr_t)weight | (uintptr_t)out | (uintptr_t)delta) & 15) == 0) {
-    const int quarter = (threads / 4 + 31) / 32 * 32;
-#define TIB_QN_X4(BYTES, HELD) TIB_LAUNCH_DEPENDENT((quantized_norm_f32x4_kernel<BYTES, HELD>), n_out, quarter, smem, stream, a, threads)
-    if (hidden <= 4 * threads) {
-      if (bytes) TIB_QN_X4(true, 4);
-      else TIB_QN_X4(false, 4);
+  if (hidden % 4 == 0 && hidden <= kQnFoursWidth && (((uintptr_t)residual | (uintptr_t)sum | (uintptr_t)weight | (uintptr_t)out | (uintptr_t)delta) & 15) == 0) {
+    const int quarter = (threads / 4 + 31) / 32 * 32, held = ceil_div(hidden, threads);      // (at most 16: threads is hidden / 4 or 1,024)
+#define TIB_QN_X4(T, BYTES, HELD)                                                                                                          \
+  do {                                                                                                                                     \
+    auto kern = quantized_norm_x4_kernel<T, BYTES, HELD>;                                                                                  \
+    if (smem > 48 * 1024) {                                                                                                                \
+      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kQnFoursWidth * (int)sizeof(float));    \
+      if (e != cudaSuccess) return (int)e;                                                                                                 \
+    }                                                                                                                                      \
+    TIB_LAUNCH_DEPENDENT(kern, n_out, quarter, smem, stream, a, threads);                                                                  \
+  } while (0)
+#define TIB_QN_X4_HELD(T, BYTES)                 \
+  do {                                           \
+    if (held <= 4) TIB_QN_X4(T, BYTES, 4);       \
+    else if (held <= 8) TIB_QN_X4(T, BYTES, 8);  \
+    else TIB_QN_X4(T, BYTES, 16);                \
+  } while (0)
+    if (dtype == TIB_BF16) {
+      if (bytes) TIB_QN_X4_HELD(__nv_bfloat16, true);
+      else TIB_QN_X4_HELD(__nv_bfloat16, false);
     } else {
-      if (bytes) TIB_QN_X4(true, 8);
-      else TIB_QN_X4(false, 8);
+      if (bytes) TIB_QN_X4_HELD(float, true);
+      else TIB_QN_X4_HELD(float, false);
     }
+#undef TIB_QN_X4_HELD
 #undef TIB_QN_X4
     return TIB_OK;
   }
