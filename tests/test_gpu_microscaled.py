@@ -262,6 +262,67 @@ def device_matrix(n, k, seed, factor=1e-3):
     return MicroscaledMatrix(codes, scales.to(torch.float8_e4m3fn), torch.tensor(factor, device=DEV), k)
 
 
+# Up to eight short rows (8,192 columns in all, of each row a multiple of eight) whose codes the product's kernel makes: rings that wrap, shared tiles, the last run and step in part.
+MADE = [(1, 8, 1), (1, 8192, 1000), (1, 4096, 28672), (2, 4096, 640), (2, 3304, 36000), (3, 2048, 2048), (4, 1992, 130), (5, 1024, 30000), (7, 264, 300), (8, 1024, 1024), (8, 1000, 37000),
+        (8, 16, 128)]
+
+
+@pytest.mark.parametrize("m, k, n", MADE)
+def test_rows_that_the_product_quantises(m, k, n):
+    """One launch, and the bits of rows that were quantised before."""
+    need_gpu()
+    assert ops.microscaled_makes(m, n, k)
+    matrix, x = device_matrix(n, k, m), rows(m, k, n)
+    weight, strided = MicroscaledWeight(matrix), torch.zeros(m, k + 8, dtype=BF16, device=DEV)[:, :k]
+    for out in (BF16, F32):
+        word, before = torch.zeros(1, dtype=torch.int32, device=DEV), ops.launch_count()
+        y = weight.product(x, out_dtype=out, error_word=word)
+        assert ops.launch_count() == before + 1
+        check(y, x, [matrix])
+        assert torch.equal(y, weight.product(quantize_rows(x), out_dtype=out)) and int(word) == 0
+        assert torch.equal(y, weight.product(strided.copy_(x), out_dtype=out))
+    if n % 2 == 0:
+        gated = MicroscaledWeight(*(MicroscaledMatrix(matrix.codes[i::2].contiguous(), matrix.scales[i::2].contiguous(), matrix.factor) for i in (0, 1)), epilogue="swiglu")
+        assert torch.equal(gated.swiglu(x), gated.swiglu(quantize_rows(x)))
+
+
+def test_rows_that_the_product_quantises_hold_anything():
+    """Zeros, subnormal numbers, the largest, an infinity and a NaN, each a row of its own: as they are quantised before."""
+    need_gpu()
+    x = rows(8, 1000, 3)
+    x[0], x[1], x[2], x[3, 7], x[4, 999], x[5, 0], x[6, 500] = 0, 1e-39, x[2] * 1e-30, float("inf"), float("nan"), 3e38, -float("inf")
+    weight = MicroscaledWeight(device_matrix(700, 1000, 1))
+    y, want = weight.product(x, out_dtype=F32), weight.product(quantize_rows(x), out_dtype=F32)
+    assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y.nan_to_num(), want.nan_to_num())
+    assert y[[3, 4, 6]].isnan().all() and not y[[0, 1, 2, 5, 7]].isnan().any() and not y[0].any()
+
+
+def test_where_the_product_does_not_quantise():
+    """More rows or columns than a round of loads takes, columns or strides that are no multiples of eight, more tiles than blocks; an output that lies over the rows."""
+    need_gpu()
+    assert not any(ops.microscaled_makes(*sizes) for sizes in ((9, 512, 512), (8, 512, 1032), (3, 512, 2056), (2, 512, 4104), (1, 512, 8200), (1, 512, 1001), (1, 300 * 128, 512)))
+    weight, x = MicroscaledWeight(random_matrix(512, 512, 1, DEV)), rows(8, 512, 1)
+    want = gemm.linear(x, weight)
+    apart, shifted = torch.zeros(8, 513, dtype=BF16, device=DEV)[:, :512], torch.zeros(8 * 512 + 1, dtype=BF16, device=DEV)[1:].view(8, 512)
+    for other in (apart, shifted):
+        before = ops.launch_count()
+        assert torch.equal(gemm.linear(other.copy_(x), weight), want) and ops.launch_count() == before + 2
+    assert torch.equal(gemm.linear(apart.copy_(x), weight, out=apart), want)
+    # (right behind the rows, or ahead of them, is not over them)
+    gated = MicroscaledWeight(random_matrix(256, 512, 2, DEV), random_matrix(256, 512, 3, DEV), epilogue="swiglu")
+    for made, act, width in ((weight, "none", 512), (gated, "swiglu", 256)):
+        for first in (False, True):
+            whole = torch.zeros(8 * (512 + width), dtype=BF16, device=DEV)
+            at = 8 * width if first else 0
+            near, y = whole[at:at + 8 * 512].view(8, 512), (whole[:at] if first else whole[8 * 512:]).view(8, width)
+            ops.microscaled_product(made.tiles.numbers, near.copy_(x), (0, 0, 0), y, act, 0.0, 0.0, 0, 0, 1, False, None, None)
+            assert torch.equal(near, x) and torch.equal(y, made.swiglu(x) if act == "swiglu" else want)
+    over = x.clone()
+    with pytest.raises(ops.KernelError):
+        ops.microscaled_product(weight.tiles.numbers, over, (0, 0, 0), over, "none", 0.0, 0.0, 0, 0, 1, False, None, None)
+    assert torch.equal(over, x) and torch.equal(gemm.linear(over, weight, out=over), want)
+
+
 # (rows, columns, features, (rows of a tile, blocks that share it, steps of a block, stages of its ring)): rings that wrap and that do not, features that are no whole
 # tiles, columns that are no whole steps, more tiles than blocks among them.
 WAYS = [(8, 4096, 4096, (32, 4, 4, 3)), (8, 600, 38530, (32, 1, 6, 4)), (20, 2500, 19200, (32, 1, 10, 4)), (3, 8320, 4000, (32, 8, 5, 3)), (8, 900, 300, (32, 4, 1, 1)),

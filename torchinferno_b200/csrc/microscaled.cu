@@ -64,14 +64,8 @@ microscaled_rows_kernel(const T* __restrict__ x, int64_t ldx, int x_rows, unsign
   unsigned char* scales_row = scales + (size_t)tile * steps * kMsStepScales + ms_scale_at(at & 127);
   auto finish = [&](int run, const uint4 (&raw)[sizeof(T)], uint32_t run_largest) {      // (whole quarters of a warp: runs and block sizes are multiples of 16)
     if (run >= runs) return;
-    const float t = __uint_as_float(run_largest) * inverse;
-    const uint32_t scale = inverse == 0.f ? 0u : ms_run_scale<T>(t);
-    const float reciprocal = ms_reciprocal(ms_scale_value(scale));
-    float v[16], lo[8], hi[8];
-    bs_floats16<T>(raw, v);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) lo[j] = v[j], hi[j] = v[8 + j];
-    const uint2 c = scale == 0 ? make_uint2(0, 0) : make_uint2(ms_codes8<T>(lo, inverse, reciprocal), ms_codes8<T>(hi, inverse, reciprocal));
+    uint32_t scale;
+    const uint2 c = ms_run_codes<T>(raw, run_largest, inverse, scale);
     *reinterpret_cast<uint2*>(codes_row + (size_t)(run >> 4) * groups * kMsGroupBytes + ms_code_at(at & 7, (run & 15) * (kMsRun / 2))) = c;
     const uint32_t mask = 0xfu << (threadIdx.x & 28), base = threadIdx.x & 28;
     uint32_t four = 0;
@@ -183,12 +177,20 @@ TIB_API int tib_microscaled_product(const void* w, const void* w_scales, const f
                                     const int* offsets, const int* order, int top, int x_by_pair, int act, float limit, float alpha, const float* row_scale,
                                     int* error_word, cudaStream_t stream) {
   if (M == 0 || N == 0) return TIB_OK;
-  if (!codes || !scales || !factors || !w || !w_scales || !w_factors || !y || M < 0 || N < 0 || K < 1 || experts < 1 || top < 1) return TIB_E_ARG;
+  const bool made_inside = make && !codes;
+  if ((!made_inside && (!codes || !scales || !factors)) || !w || !w_scales || !w_factors || !y || M < 0 || N < 0 || K < 1 || experts < 1 || top < 1) return TIB_E_ARG;
   if ((offsets && !order) || (row_scale && !order)) return TIB_E_ARG;
   if (act < MOE_ACT_NONE || act > MOE_ACT_GELU || (moe_act_gated(act) && !pairs) || (pairs && N % 2)) return TIB_E_SIZE;
   if (y_dtype != TIB_BF16 && y_dtype != TIB_F32) return TIB_E_DTYPE;
   if (((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)w | (uintptr_t)w_scales) & 15) return TIB_E_ALIGN;
-  if (make) {
+  if (made_inside) {      // (every block reads the rows while others write y)
+    if (!x || offsets || M > x_rows || !ms_makes_rows(M, N, K)) return TIB_E_ARG;
+    if (x_dtype != TIB_BF16) return TIB_E_DTYPE;
+    if (((uintptr_t)x & 15) || ldx % 8) return TIB_E_ALIGN;
+    const char *from = (const char*)x, *to = (const char*)y;
+    const int width = moe_act_gated(act) ? N / 2 : N;
+    if (from < to + ((int64_t)(M - 1) * ldy + width) * (y_dtype == TIB_BF16 ? 2 : 4) && to < from + ((int64_t)(M - 1) * ldx + K) * 2) return TIB_E_ARG;
+  } else if (make) {
     const int rc = tib_microscaled_rows(x, x_dtype, ldx, x_rows, codes, scales, factors, M, K, offsets, order, experts, top, x_by_pair, stream);
     if (rc != TIB_OK) return rc;
   }
@@ -197,7 +199,8 @@ TIB_API int tib_microscaled_product(const void* w, const void* w_scales, const f
   a.w = (const unsigned char*)w; a.w_scales = (const unsigned char*)w_scales; a.w_factors = w_factors;
   a.M = M; a.N = N; a.steps = ms_steps(K); a.stages = a.tmem_cols = 0; a.offsets = offsets; a.order = order; a.experts = experts;
   a.limit = limit; a.alpha = alpha; a.row_scale = row_scale; a.error_word = error_word;
-  if (ms_on_pairs_of_sms(M, N, a.steps, offsets ? experts : 0)) return ms_product_2cta(a, act, y, y_dtype, ldy, stream);
+  a.made = made_inside ? (const __nv_bfloat16*)x : nullptr; a.ld_made = ldx; a.K = K;
+  if (!made_inside && ms_on_pairs_of_sms(M, N, a.steps, offsets ? experts : 0)) return ms_product_2cta(a, act, y, y_dtype, ldy, stream);
   return ms_product_tcgen05(a, act, y, y_dtype, ldy, stream);
 }
 
@@ -209,7 +212,15 @@ TIB_API int tib_microscaled_plan(int M, int N, int K, int experts, int* plan) {
   return ms_on_pairs_of_sms(M, N, steps, experts) ? ms_plan_2cta(M, N, steps, experts, plan) : ms_plan_tcgen05(M, N, steps, experts, plan);
 }
 
+// Whether tib_microscaled_product makes the codes of M rows of 16-bit numbers (16-byte aligned, as is a row's stride) for one matrix without room for them (codes null).
+TIB_API int tib_microscaled_makes(int M, int N, int K, int* answer) {
+  if (!answer || M < 1 || N < 1 || K < 1) return TIB_E_ARG;
+  *answer = ms_makes_rows(M, N, K);
+  return TIB_OK;
+}
+
 TIB_PACKED(tib_microscaled_rows)
+TIB_PACKED(tib_microscaled_makes)
 TIB_PACKED(tib_microscaled_widen)
 TIB_PACKED(tib_microscaled_product)
 TIB_PACKED(tib_microscaled_plan)

@@ -94,6 +94,17 @@ template <typename T> __device__ __forceinline__ uint32_t ms_codes8(const float 
       : "=r"(codes) : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
   return codes;
 }
+// A run's codes and (into `scale`) its scale.  inverse: of the row's factor, 0 where the row holds no finite sum.
+template <typename T> __device__ __forceinline__ uint2 ms_run_codes(const uint4 (&raw)[sizeof(T)], uint32_t run_largest, float inverse, uint32_t& scale) {
+  const float t = __uint_as_float(run_largest) * inverse;
+  scale = inverse == 0.f ? 0u : ms_run_scale<T>(t);
+  const float reciprocal = ms_reciprocal(ms_scale_value(scale));
+  float v[16], lo[8], hi[8];
+  bs_floats16<T>(raw, v);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) lo[j] = v[j], hi[j] = v[8 + j];
+  return scale == 0 ? make_uint2(0, 0) : make_uint2(ms_codes8<T>(lo, inverse, reciprocal), ms_codes8<T>(hi, inverse, reciprocal));
+}
 // two codes (a byte) to two floats
 __device__ __forceinline__ float2 ms_numbers2(uint32_t byte) {
   uint32_t h;
@@ -153,6 +164,9 @@ struct MsArgs {
   float limit, alpha;              // of the clamped gated unit
   const float* row_scale;          // [M] by pair, or null
   int* error_word;
+  const __nv_bfloat16* made;       // the rows themselves where the product's kernel makes their codes (then `x` is empty), or null
+  int64_t ld_made;
+  int K;
 };
 
 // An output from its sum(s): times the matrix's factor, the row's (a power of two) and the pair's, in turn, so that nothing leaves the range of 32 bits but what the
@@ -165,6 +179,8 @@ int ms_product_2cta(const MsArgs& a, int act, void* y, int y_dtype, int64_t ldy,
 // How a product runs there: {rows of a tile at most, blocks that share a tile, steps of a block at most, stages of its ring}.
 int ms_plan_2cta(int M, int N, int steps, int experts, int* plan);
 int ms_plan_tcgen05(int M, int N, int steps, int experts, int* plan);
+// Whether the kernel of a product with one matrix may make the codes of its rows itself.
+bool ms_makes_rows(int M, int N, int K);
 int ms_product_tcgen05(MsArgs& a, int act, void* y, int y_dtype, int64_t ldy, cudaStream_t stream);
 
 }  // namespace tib

@@ -7,7 +7,8 @@
 // ring have columns of their own, so that they are free when the stage is.
 //   warp 0       producer: four copies a step, each of bytes that lie side by side: 16 KB of codes of w, 2 KB of its scales, the rows' codes and scales
 //   warp 1       copies scales and issues tcgen05.mma; owns the TMEM allocation
-//   the next 4 or 8   epilogue: some rows at a time, a lane a feature, so that a warp writes 32 outputs of a row side by side; two accumulators take turns
+//   the next 4 or 8   epilogue: some rows at a time, a lane a feature, so that a warp writes 32 outputs of a row side by side; two accumulators take turns.  Of up to eight short
+//                rows (ms_makes_rows) they first make the codes, straight into the ring, where no kernel has made them before
 // A matrix of few tiles is split by steps over a cluster of up to eight blocks, whose sums meet in distributed shared memory, added in the order of the
 // steps.
 // What bounds it, at few rows: memory.  8 rows 4,096 -> 28,672: 12.3 us for 66 MB (5.4 TB/s, 84 % of the measured copy bandwidth; without the copies 7.1); 14,336 -> 4,096 9.2 us
@@ -36,6 +37,9 @@ template <int NT> struct MtShape {
 // of the sums of a shared tile: (a column's 128 / splits sums and four more, so that those that a warp writes at a time fall on all banks)
 template <int NT> __host__ __device__ constexpr int mt_red_floats(int splits) { return splits > 1 ? NT * (128 + 4 * splits) : 0; }
 
+// (the binary logarithm of) how many of eight loads are of the same of M rows.
+__host__ __device__ constexpr int mt_more_loads(int M) { return M > 4 ? 0 : M > 2 ? 1 : 4 - M; }
+
 struct MtTile { int expert, first, rows, group, scale_tile, feature; };
 
 // An output (of a gated unit: from its gate g and up u).
@@ -44,7 +48,9 @@ template <int ACT> __device__ __forceinline__ float mt_act(float g, float u, con
   else return bs_act<ACT>(g);
 }
 
-template <int NT, int ACT, typename TO>
+// MAKE: up to eight rows, short ones, whose codes the finishing warps, idle till then, put into the ring themselves: a thread a run of a step.  Every block looks for the rows' largest
+// numbers first.
+template <int NT, int ACT, typename TO, bool MAKE>
 __global__ void __launch_bounds__(MtShape<NT>::kThreads, MtShape<NT>::kPerSm)
 microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y, int64_t ldy) {
   using S = MtShape<NT>;
@@ -71,7 +77,7 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
   const int step0 = (int)((int64_t)a.steps * rank / splits), step1 = (int)((int64_t)a.steps * (rank + 1) / splits);
   if (warp == 0) {
     if (lane < a.stages) {
-      mbar_init(full_bar(lane), 1);
+      mbar_init(full_bar(lane), MAKE ? 1 + S::kStorers : 1);
       mbar_init(empty_bar(lane), 1);
     }
     if (lane < 2) {
@@ -150,7 +156,7 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
     auto ask_w = [&](const MtTile& m, int step, int s) {
       const uint32_t stage = base + s * S::kStage;
       const int block = (m.expert * f_tiles + (m.feature >> 7)) * a.steps + step;
-      mbar_expect_tx(full_bar(s), kMtWBytes + 2 * kMsStepScales + rows_bytes(m));
+      mbar_expect_tx(full_bar(s), MAKE ? kMtWBytes + kMsStepScales : kMtWBytes + 2 * kMsStepScales + rows_bytes(m));
       ms_bulk_load(stage, a.w + (size_t)block * kMtWBytes, kMtWBytes, full_bar(s));
       ms_bulk_load(stage + kMtWBytes + NT * kMsStepBytes, a.w_scales + (size_t)block * kMsStepScales, kMsStepScales, full_bar(s));
     };
@@ -174,7 +180,7 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
           if (leader) ask_w(m, step, s);
           __syncwarp();
         }
-        if (leader) {
+        if (!MAKE && leader) {
           const uint32_t rows_at = base + s * S::kStage + kMtWBytes;
           ms_bulk_load(rows_at, a.x.codes + ((size_t)step * a.x.groups + m.group) * kMsGroupBytes, rows_bytes(m), full_bar(s));
           ms_bulk_load(rows_at + NT * kMsStepBytes + kMsStepScales, a.x.scales + ((size_t)m.scale_tile * a.steps + step) * kMsStepScales, kMsStepScales, full_bar(s));
@@ -226,13 +232,69 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
     uint32_t acc_phase = 0;
     bool ok = true;
     if (!a.offsets) pdl_wait();                   // (y may be memory that the kernel before still reads)
+    const int own_row = et >> 4, own_run = et & 15;      // (of a step of eight rows)
+    float r = 1.f, inverse = 1.f;
+    int ring = 0;
+    uint32_t ring_phase = 1;
+    if constexpr (MAKE) {
+      static_assert(NT == 32 && S::kStorers == 4, "eight rows of 16 runs are a thread's each");
+      uint32_t* found = reinterpret_cast<uint32_t*>(tile_factors) + 32;      // [4 warps][8] (behind the eight rows' factors)
+      // Eight loads of eight numbers a thread, all on their way at once; of fewer rows several of a row: load i is of row i >> more.
+      const int more = mt_more_loads(a.M), mask = (1 << more) - 1;
+      uint4 raw[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = i >> more, at = (et + (i & mask) * 128) * 8;
+        raw[i] = row < a.M && at < a.K ? *reinterpret_cast<const uint4*>(a.made + row * a.ld_made + at) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t two = __vmaxu2(__vmaxu2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu), __vmaxu2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu));
+        const uint32_t most = __reduce_max_sync(0xffffffffu, max(two << 16, two & 0xffff0000u));
+        if (lane == 0) found[(warp - 2) * 8 + i] = most;
+      }
+      asm volatile("bar.sync 1, %0;\n" ::"r"(32 * S::kStorers) : "memory");
+      if (own_row < a.M) {
+        uint32_t most = 0;
+        for (int i = own_row << more; i <= (own_row << more | mask); ++i) most = max(most, max(max(found[i], found[8 + i]), max(found[16 + i], found[24 + i])));
+        ms_row_scale(most, r, inverse);
+      }
+    }
     for (int t = cluster_id; t < num_tiles; t += clusters) {
       const MtTile m = tile_of(t);
       const int feature = m.feature + quarter * 32 + lane, n_out = a.N >> kGated;
       const float factor = a.w_factors[(size_t)m.expert * a.N + min(feature, a.N - 1)];
       float2* factors = reinterpret_cast<float2*>(tile_factors) + b * NT;
-      if (et < m.rows) factors[et] = make_float2(a.x.factors[m.first + et], a.row_scale ? a.row_scale[bs_pair(a.order, m.first + et, a.M)] : 1.f);
+      if constexpr (MAKE) {
+        if (own_run == 0 && own_row < m.rows) factors[own_row] = make_float2(r, 1.f);
+      } else if (et < m.rows) factors[et] = make_float2(a.x.factors[m.first + et], a.row_scale ? a.row_scale[bs_pair(a.order, m.first + et, a.M)] : 1.f);
       asm volatile("bar.sync 1, %0;\n" ::"r"(32 * S::kStorers) : "memory");      // (the last tile but one is finished: its factors have been read)
+      if constexpr (MAKE) {
+        const __nv_bfloat16* src = a.made + own_row * a.ld_made;
+        for (int step = step0; step < step1 && ok; ++step) {
+          if (!mbar_wait_warp(empty_bar(ring), ring_phase)) {
+            if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00E6);
+            ok = false;
+            break;
+          }
+          if (own_row < a.M) {
+            const int run = step * (kMsStep / kMsRun) + own_run;
+            unsigned char* rows_at = smem_gen + ring * S::kStage + kMtWBytes;
+            uint4 raw[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              raw[i] = run * kMsRun + 8 * i < a.K ? *reinterpret_cast<const uint4*>(src + run * kMsRun + 8 * i) : make_uint4(0, 0, 0, 0);
+            uint32_t scale;
+            const uint2 codes = ms_run_codes<__nv_bfloat16>(raw, bs_largest16<__nv_bfloat16>(raw), inverse, scale);
+            *reinterpret_cast<uint2*>(rows_at + ms_code_at(own_row, own_run * (kMsRun / 2))) = codes;
+            rows_at[NT * kMsStepBytes + kMsStepScales + (own_run >> 2) * kMsChunkBytes + ms_scale_at(own_row) + (own_run & 3)] = (unsigned char)scale;
+          }
+          asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full_bar(ring));
+          if (++ring == a.stages) { ring = 0; ring_phase ^= 1; }
+        }
+      }
       if (ok && !mbar_wait_warp(acc_full_bar(b), acc_phase)) {
         if (a.error_word && lane == 0) atomicExch(a.error_word, 0x7C00E3);
         ok = false;
@@ -373,7 +435,7 @@ template <int NT> static int mt_plan(int M, int N, int steps, int experts, MtPla
 // 4,096 -> 28,672 take 12.3, 13.9, 14.3, 15.8 and 16.9 us.
 static int mt_tile_rows(int M) { return M <= 32 ? 32 : 128; }
 
-template <int NT, int ACT, typename TO>
+template <int NT, int ACT, typename TO, bool MAKE>
 static int launch_mt(MsArgs& a, void* y, int64_t ldy, cudaStream_t stream) {
   const int experts = a.offsets ? a.experts : 0;
   MtPlan plan;
@@ -381,7 +443,7 @@ static int launch_mt(MsArgs& a, void* y, int64_t ldy, cudaStream_t stream) {
   if (rc != TIB_OK) return rc;
   a.stages = plan.stages;
   a.tmem_cols = (int)MtShape<NT>::tmem_cols(plan.splits);
-  auto kern = microscaled_tcgen05_kernel<NT, ACT, TO>;
+  auto kern = microscaled_tcgen05_kernel<NT, ACT, TO, MAKE>;
   static bool allowed[64];      // (by device: the attribute belongs to its context)
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
@@ -411,15 +473,15 @@ static int launch_mt(MsArgs& a, void* y, int64_t ldy, cudaStream_t stream) {
   return TIB_OK;
 }
 
-template <int NT, typename TO>
+template <int NT, typename TO, bool MAKE>
 static int launch_mt_act(int act, MsArgs& a, void* y, int64_t ldy, cudaStream_t stream) {
   switch (act) {
-    case MOE_ACT_NONE: return launch_mt<NT, MOE_ACT_NONE, TO>(a, y, ldy, stream);
-    case MOE_ACT_RELU2: return launch_mt<NT, MOE_ACT_RELU2, TO>(a, y, ldy, stream);
-    case MOE_ACT_SILU: return launch_mt<NT, MOE_ACT_SILU, TO>(a, y, ldy, stream);
-    case MOE_ACT_GELU: return launch_mt<NT, MOE_ACT_GELU, TO>(a, y, ldy, stream);
-    case MOE_ACT_GLU_CLAMP: return launch_mt<NT, MOE_ACT_GLU_CLAMP, TO>(a, y, ldy, stream);
-    default: return launch_mt<NT, MOE_ACT_SWIGLU, TO>(a, y, ldy, stream);
+    case MOE_ACT_NONE: return launch_mt<NT, MOE_ACT_NONE, TO, MAKE>(a, y, ldy, stream);
+    case MOE_ACT_RELU2: return launch_mt<NT, MOE_ACT_RELU2, TO, MAKE>(a, y, ldy, stream);
+    case MOE_ACT_SILU: return launch_mt<NT, MOE_ACT_SILU, TO, MAKE>(a, y, ldy, stream);
+    case MOE_ACT_GELU: return launch_mt<NT, MOE_ACT_GELU, TO, MAKE>(a, y, ldy, stream);
+    case MOE_ACT_GLU_CLAMP: return launch_mt<NT, MOE_ACT_GLU_CLAMP, TO, MAKE>(a, y, ldy, stream);
+    default: return launch_mt<NT, MOE_ACT_SWIGLU, TO, MAKE>(a, y, ldy, stream);
   }
 }
 
@@ -427,12 +489,21 @@ static int launch_mt_act(int act, MsArgs& a, void* y, int64_t ldy, cudaStream_t 
 
 using namespace tib;
 
+// Where a block's threads find the rows' largest numbers with one round of loads, and have a tile each.  (One kernel / two, us on the device: 1 row 1,024 -> 1,024 3.5 / 4.4, 8 rows
+// 3.8 / 4.7; 4 rows 2,048 -> 2,048 4.3 / 4.9; 2 rows 4,096 -> 4,096 6.5 / 6.5; 1 row 4,096 -> 28,672 14.6 / 14.5, 2 rows 15.2 / 14.8; 1 row 8,192 -> 8,192 10.4 / 10.2; where calls
+// are bound by the host 8.5 / 12.1 each.  With more rounds every block's reading of all rows shows: 4 rows 4,096 -> 4,096 8.0 / 6.6, 1 row 14,336 -> 4,096 11.2 / 10.5.)
+bool tib::ms_makes_rows(int M, int N, int K) {
+  MtPlan p;
+  return M <= 8 && K % 8 == 0 && K <= 1024 << mt_more_loads(M) && mt_plan<32>(M, N, ms_steps(K), 0, p) == TIB_OK && p.grid == ceil_div(N, 128) * p.splits;
+}
+
 int tib::ms_product_tcgen05(MsArgs& a, int act, void* y, int y_dtype, int64_t ldy, cudaStream_t stream) {
   if (a.experts > kMtMaxExperts || (int64_t)a.experts * ceil_div(a.N, 128) * a.steps > 0x7fffffff) return TIB_E_SIZE;
-#define TIB_MT_GO(NT) \
-  return y_dtype == TIB_BF16 ? launch_mt_act<NT, __nv_bfloat16>(act, a, y, ldy, stream) : launch_mt_act<NT, float>(act, a, y, ldy, stream)
-  if (mt_tile_rows(a.M) == 32) TIB_MT_GO(32);
-  TIB_MT_GO(128);
+#define TIB_MT_GO(NT, MAKE) \
+  return y_dtype == TIB_BF16 ? launch_mt_act<NT, __nv_bfloat16, MAKE>(act, a, y, ldy, stream) : launch_mt_act<NT, float, MAKE>(act, a, y, ldy, stream)
+  if (a.made) TIB_MT_GO(32, true);
+  if (mt_tile_rows(a.M) == 32) TIB_MT_GO(32, false);
+  TIB_MT_GO(128, false);
 #undef TIB_MT_GO
 }
 

@@ -110,6 +110,9 @@ def _sizes(rows: int, columns: int, experts: int) -> tuple[int, int, int, torch.
     return codes, codes + scales, codes + scales + 4 * rows, torch.Size((rows, columns))
 
 
+_makes = functools.lru_cache(maxsize=4096)(ops.microscaled_makes)
+
+
 class MicroscaledRows:
     """Quantised rows [rows, columns], as the kernels read them.  ``dtype``: the type of what they were made from."""
     __slots__ = ("buffer", "shape", "dtype", "codes_at", "scales_at", "factors_at")
@@ -210,10 +213,17 @@ def _laid_out(stacks: Sequence[Sequence[MicroscaledMatrix]], paired: bool) -> Ti
     return Tiles(codes.view(len(stacks), tiles, steps, TILE, -1), scales.view(len(stacks), tiles, steps, -1), factors, columns, paired)
 
 
+_NO_ROWS = (0, 0, 0)
+
+
 def _product(x: "torch.Tensor | MicroscaledRows", tiles: Tiles, y: torch.Tensor, act: str, limit: float, alpha: float, offsets: int, order: int, top: int,
-             x_by_pair: bool, row_scale: torch.Tensor | None, error_word: torch.Tensor | None) -> None:
+             x_by_pair: bool, row_scale: torch.Tensor | None, error_word: torch.Tensor | None, fresh: bool = False) -> None:
+    # (fresh: y is memory that x is not)
     if isinstance(x, MicroscaledRows):
         x, rows = None, (x.codes_at, x.scales_at, x.factors_at)
+    elif (fresh and y.shape[0] <= GROUP and x.dtype is torch.bfloat16 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 and
+          _makes(y.shape[0], tiles.features, tiles.columns)):
+        rows = _NO_ROWS
     else:
         scales, factors, size, _ = _sizes(y.shape[0], tiles.columns, tiles.count if offsets else 0)
         held = ops.new_bytes(x, size)
@@ -272,12 +282,13 @@ class MicroscaledWeight:
         dtype = x.dtype if out_dtype is None else out_dtype
         if dtype not in _OUT_DTYPES:
             raise ops.KernelError(f"linear: unsupported output dtype {dtype}")
-        if out is None or out.dtype != dtype:
+        fresh = out is None or out.dtype != dtype
+        if fresh:
             out = ops.new_rows(x if isinstance(x, torch.Tensor) else x.buffer, rows, width, dtype)
         elif out.shape != (rows, width) or (out.stride(1) != 1 and width > 1) or out.get_device() != x.get_device():
             raise ops.KernelError(f"linear: out is {tuple(out.shape)} on {out.device}, wanted {(rows, width)} with unit inner stride on {x.device}")
         if rows:
-            _product(x, self.tiles, out, act, 0.0, 0.0, 0, 0, 1, False, None, error_word)
+            _product(x, self.tiles, out, act, 0.0, 0.0, 0, 0, 1, False, None, error_word, fresh)
         return out
 
     def product(self, x: "torch.Tensor | MicroscaledRows", *, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,

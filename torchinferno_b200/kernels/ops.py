@@ -1370,16 +1370,25 @@ def microscaled_widen(codes: int, scales: int, factors: int, out: torch.Tensor, 
 def microscaled_product(weight: tuple, x: torch.Tensor | None, rows: tuple, y: torch.Tensor, act: str, limit: float, alpha: float, offsets: int, order: int,
                         top: int, x_by_pair: bool, row_scale: torch.Tensor | None, error_word: torch.Tensor | None) -> None:
     """Rows times matrices of 4-bit codes, into ``y``.  ``weight``: a microscaled.Tiles' numbers.  ``rows``: addresses of the rows' codes, scales and factors, where
-    those of ``x`` are put first (None: they are there).  ``offsets`` / ``order``: addresses of what sorts the rows of ``y`` by expert as in
-    :func:`moe_expert_product`, or 0."""
+    those of ``x`` are put first (None: they are there); zeros where the product's kernel makes them itself (:func:`microscaled_makes`).  ``offsets`` / ``order``: addresses
+    of what sorts the rows of ``y`` by expert as in :func:`moe_expert_product`, or 0."""
     if x is None:
         source = (0, BF16, 0, 0)
     else:
         source = (x.data_ptr(), _code(x.dtype), x.stride(0), x.shape[0])
-        _counter["launches"] += 1
+        if rows[0]:
+            _counter["launches"] += 1
     _check("microscaled_product", lib().tib_microscaled_product(
         *weight, *source, *rows, x is not None, y.data_ptr(), _code(y.dtype), y.stride(0), y.shape[0], offsets, order, top, x_by_pair, MOE_ACT[act], limit, alpha,
         0 if row_scale is None else row_scale.data_ptr(), 0 if error_word is None else error_word.data_ptr(), _stream()))
+
+
+def microscaled_makes(rows: int, features: int, columns: int) -> bool:
+    """Whether a product with one matrix makes the codes of so many rows (bfloat16, on 16 bytes as their stride) in its own kernel.  The rows may not lie where ``y`` does."""
+    answer = ctypes.c_int()
+    _check("microscaled_makes", lib().tib_microscaled_makes(rows, features, columns, ctypes.addressof(answer)))
+    count_launches(-1)
+    return bool(answer.value)
 
 
 def quantized_norm_type(delta: torch.Tensor | None, dtype: torch.dtype | None) -> torch.dtype:
