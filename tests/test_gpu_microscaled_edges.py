@@ -1,0 +1,64 @@
+"""4-bit rows, norms that leave quantised rows and their products where 32-bit numbers end and where the kernels change, against the definition in 64 bits."""
+import pytest
+import torch
+
+from gpu_common import need_gpu
+from microscaled_oracle import random_matrix, rows64
+from test_gpu_microscaled import check, rows, same, same_rows
+from torchinferno_b200.kernels import gemm, microscaled, ops
+from torchinferno_b200.kernels.microscaled import MicroscaledWeight, quantize_rows
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+# ------------------------------------------------------------------------------------------------ subnormal numbers
+def subnormal(m, k, power, seed):
+    """Gaussian numbers of this size, most of them subnormal."""
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(m, k, generator=g, dtype=torch.float64) * 2.0 ** power).to(F32).to(DEV)
+
+
+@pytest.mark.parametrize("power", [-147, -140, -137, -134, -131, -128, -126, -124, -118])
+@pytest.mark.parametrize("m, k", [(70, 400), (3, 1003), (1, 17000)])
+def test_rows_of_subnormal_numbers(m, k, power):
+    need_gpu()
+    same_rows(subnormal(m, k, power, m - power))
+
+
+def test_subnormal_numbers_beside_the_borders_of_codes():
+    """Runs with each of the scales that are odd or even multiples of 2^-9, in rows whose factor is 2^-126: a code is a number of units of 2^-149."""
+    need_gpu()
+    runs = []
+    for m in range(1, 16):
+        unit = m << 14                                                       # m 2^-9 2^-126
+        near = [int(b * unit) + off for b in (0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)
+                for off in (-4097, -4096, -2049, -2048, -2047, -700, -1, 0, 1, 700, 2047, 2048, 4096)]
+        near = [min(n, 6 * unit) for n in near] + [0] * (-len(near) % 15)
+        for first in range(0, len(near), 15):
+            runs.append([6 * unit] + near[first:first + 15])
+    bits = torch.tensor(runs, dtype=torch.int32)
+    sign = torch.where(torch.arange(16) % 3 == 1, -1.0, 1.0)
+    x = bits.view(F32) * sign
+    same_rows(x.to(DEV))
+    same_rows(x.reshape(1, -1).to(DEV))                                      # (one row: the scales are of every size)
+    one = torch.zeros(2, 16, dtype=torch.int32)
+    one[:, 0], one[0, 1], one[1, 1] = 6 << 14, 0x1909, 0x262a
+    assert quantize_rows(one.view(F32).to(DEV)).widened(F32)[:, 1].tolist() == [2.0 ** -136, 2.0 ** -136]
+
+
+@pytest.mark.parametrize("m, k", [(4, 520), (3, 1003), (2, 9002), (2, 10240)])
+def test_a_norm_of_subnormal_rows(m, k):
+    need_gpu()
+    residual, weight = rows(m, k, 3, F32, spread=0.3), subnormal(1, k, -131, k)[0]
+    out = torch.empty(m, k, device=DEV)
+    made = microscaled.add_rmsnorm(None, residual, weight, 1e-5, dtype=F32, out=out)
+    assert (out.abs() < 2.0 ** -126).any() and same(made.widened(F32), rows64(out))
+
+
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_products_of_subnormal_rows(m):
+    need_gpu()
+    x, matrix = subnormal(m, 300, -130, m), random_matrix(260, 300, 6, DEV, 1e30)
+    check(gemm.linear(x, MicroscaledWeight(matrix)), x, [matrix])

@@ -73,16 +73,19 @@ __device__ __forceinline__ float ms_reciprocal(float s) {      // 0 for 0
   return s == 0.f ? 0.f : r;
 }
 // Eight numbers times `inverse` (a power of two) and `reciprocal` to eight codes, the first in the lowest four bits.  (The two factors are one where their product
-// is a normal number: but for rows whose largest number is under 2^-97.)
+// is a normal number: but for rows whose largest number is under 2^-97, of which the numbers are multiplied by 2^32 first, so that none near a border is
+// subnormal.  In other rows r is 2^-108 or more and the least scale 2^-9: a subnormal number is less than 2^-9 of that, and its code 0, cut or not.)
 template <typename T> __device__ __forceinline__ uint32_t ms_codes8(const float (&numbers)[8], float inverse, float reciprocal) {
   float v[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = ms_odd12<T>(numbers[j]);
+  for (int j = 0; j < 8; ++j) v[j] = numbers[j];
   if (inverse > 0x1p108f) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= 0x1p32f;
     inverse *= 0x1p-32f;
   }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = ms_odd12<T>(v[j]);
   // (192 + q is a multiple of 2^-16; a quotient is at most 9, where a scale of 1.5 * 2^-9 was rounded to 2^-9)
   const f32x2 factor = f2_pack(inverse * reciprocal, inverse * reciprocal), up = f2_pack(192.f, 192.f), down = f2_pack(-192.f, -192.f), one = f2_pack(1.f, 1.f);
   float q[8];
