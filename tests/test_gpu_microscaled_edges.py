@@ -5,7 +5,7 @@ import torch
 from gpu_common import need_gpu
 from microscaled_oracle import random_matrix, rows64
 from test_gpu_microscaled import check, rows, same, same_rows
-from torchinferno_b200.kernels import gemm, microscaled, ops
+from torchinferno_b200.kernels import block_scaled, gemm, microscaled, ops
 from torchinferno_b200.kernels.microscaled import MicroscaledWeight, quantize_rows
 
 pytestmark = pytest.mark.gpu
@@ -62,3 +62,31 @@ def test_products_of_subnormal_rows(m):
     need_gpu()
     x, matrix = subnormal(m, 300, -130, m), random_matrix(260, 300, 6, DEV, 1e30)
     check(gemm.linear(x, MicroscaledWeight(matrix)), x, [matrix])
+
+
+# ------------------------------------------------------------------------------------------------ norms whose row nearly fills, fills and overfills 48 KB of shared memory
+WIDTHS = (8196, 12028, 12032, 12036, 12160, 12284, 12288, 12292, 16384)
+
+
+def every_width():
+    """Every kernel of norms of this width, the narrower rows first (what a wider row asks for would serve them too)."""
+    for k in WIDTHS:
+        for dtype in (BF16, F32):
+            delta, residual, weight = rows(3, k, k, dtype), rows(3, k, k + 1, F32, spread=0.3), 1 + 0.1 * rows(1, k, k + 2, F32, spread=0.1)[0]
+            want = torch.empty(3, k, dtype=dtype, device=DEV)
+            ops.add_rmsnorm(delta, residual.clone(), weight, 1e-5, want)
+            assert torch.equal(microscaled.add_rmsnorm(delta, residual.clone(), weight, 1e-5).widened(F32), quantize_rows(want).widened(F32)), (k, dtype)
+            made, (codes, scales) = block_scaled.add_rmsnorm(delta, residual.clone(), weight, 1e-5), block_scaled.quantize_rows(want)
+            assert torch.equal(made.parts()[0].view(torch.uint8), codes.view(torch.uint8)) and torch.equal(made.parts()[1], scales), (k, dtype)
+
+
+def test_norms_about_48_kb_of_shared_memory():
+    """In a process of its own, whose kernels no wider row has met."""
+    need_gpu()
+    import subprocess
+    import sys
+    from pathlib import Path
+    here = Path(__file__).resolve().parent
+    code = f"import sys; sys.path[:0] = [{str(here)!r}, {str(here.parent)!r}]; import test_gpu_microscaled_edges as t; t.every_width(); print('every width')"
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "every width" in done.stdout, done.stdout[-2000:] + done.stderr[-3000:]

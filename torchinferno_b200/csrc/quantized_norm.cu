@@ -342,6 +342,19 @@ __global__ void quantized_norm_kernel(const QnArgs a) {
   }
 }
 
+// Rows of more than 8,192 columns, whose 32 to 64 KB beside a kernel's own arrays are more than the 48 KB that it has without asking: asked for once a device (the
+// attribute belongs to its context), whatever a row's width.
+template <typename T, bool BYTES>
+static int qn_allow_smem(void (*kern)(const QnArgs, int)) {
+  static bool allowed[64];
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess && !(device < 64 && allowed[device])) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kQnFoursWidth * (int)sizeof(float));
+  if (e != cudaSuccess) return (int)e;
+  if (device < 64) allowed[device] = true;
+  return TIB_OK;
+}
+
 }  // namespace tib
 
 using namespace tib;
@@ -371,9 +384,9 @@ TIB_API int tib_quantized_norm(const void* delta, const float* residual, float* 
 #define TIB_QN_X4(T, BYTES, HELD)                                                                                                          \
   do {                                                                                                                                     \
     auto kern = quantized_norm_x4_kernel<T, BYTES, HELD>;                                                                                  \
-    if (smem > 48 * 1024) {                                                                                                                \
-      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kQnFoursWidth * (int)sizeof(float));    \
-      if (e != cudaSuccess) return (int)e;                                                                                                 \
+    if (HELD == 16) {                                                                                                                      \
+      const int rc = qn_allow_smem<T, BYTES>(kern);                                                                                        \
+      if (rc != TIB_OK) return rc;                                                                                                         \
     }                                                                                                                                      \
     TIB_LAUNCH_DEPENDENT(kern, n_out, quarter, smem, stream, a, threads);                                                                  \
   } while (0)
