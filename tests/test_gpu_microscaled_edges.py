@@ -3,10 +3,10 @@ import pytest
 import torch
 
 from gpu_common import need_gpu
-from microscaled_oracle import random_matrix, rows64
+from microscaled_oracle import matrix64, random_matrix, rows64
 from test_gpu_microscaled import check, rows, same, same_rows
 from torchinferno_b200.kernels import block_scaled, gemm, microscaled, ops
-from torchinferno_b200.kernels.microscaled import MicroscaledWeight, quantize_rows
+from torchinferno_b200.kernels.microscaled import MicroscaledExperts, MicroscaledMatrix, MicroscaledWeight, quantize_rows
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -90,3 +90,74 @@ def test_norms_about_48_kb_of_shared_memory():
     code = f"import sys; sys.path[:0] = [{str(here)!r}, {str(here.parent)!r}]; import test_gpu_microscaled_edges as t; t.every_width(); print('every width')"
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "every width" in done.stdout, done.stdout[-2000:] + done.stderr[-3000:]
+
+
+# ------------------------------------------------------------------------------------------------ factors at the ends of the range
+def check_numbers(y, sums, slack):
+    """y against sums in 64 bits that are off by ``slack`` at most, two multiplications and one rounding (check's text), and, of numbers at the lower end, by two steps
+    of 2^-149: beyond the largest number y is infinite."""
+    half, largest = torch.finfo(y.dtype).eps / 2, torch.finfo(y.dtype).max
+    bound = slack + sums.abs() * (half + 2.0 ** -22) + 2.0 ** (-149 if y.dtype == F32 else -133) * 2
+    beyond = sums.abs() - bound > largest * (1 + half)
+    assert (y[beyond].double() == torch.copysign(torch.full_like(sums, float("inf")), sums)[beyond]).all()
+    near = sums.abs() + bound < largest
+    assert y[near].isfinite().all() and ((y.double() - sums).abs() <= bound)[near].all()
+    return near
+
+
+def sums_of(x, matrix):
+    wide, w = rows64(x), matrix64(matrix)
+    return wide @ w.t(), wide.abs() @ w.abs().t() * (x.shape[1] + 4) * 2.0 ** -24
+
+
+# (the size of a row's largest numbers, the matrix's factor): products of factor and sum, or of row and sum, that are no 32-bit numbers, where the output is one
+ENDS = [(2e-24, 1e33), (1e-30, 1e36), (3e-36, 3e38), (1e-38, 3e38), (1e-42, 3e38), (1e30, 1e-39), (1e36, 1e-43), (3e38, 2e-45), (3e38, 1e-38), (1.0, 3e38), (1.0, 1e-45), (3e38, 3e38),
+        (1e-40, 1e-40)]
+
+
+@pytest.mark.parametrize("size, factor", ENDS)
+@pytest.mark.parametrize("m, k, n", [(1, 1000, 260), (8, 1000, 700), (3, 8320, 130), (40, 520, 260), (300, 300, 260), (700, 600, 4001)])
+def test_products_at_the_ends_of_the_range(m, k, n, size, factor):
+    """Rows that the product quantises, tiles of 32 and 128 rows, shared and not, and pairs of SMs."""
+    need_gpu()
+    matrix = random_matrix(n, k, n, DEV, factor)
+    x = (rows(m, k, 5, F32, spread=0.1).clamp(-1, 1).double() * size).to(F32)
+    weight = MicroscaledWeight(matrix)
+    check_numbers(gemm.linear(x, weight), *sums_of(x, matrix))
+    x = x.to(BF16)
+    check_numbers(gemm.linear(x, weight, out_dtype=F32), *sums_of(x, matrix))
+
+
+@pytest.mark.parametrize("m", [2, 40, 300])
+def test_the_smallest_sums(m):
+    """Two codes of 1/2 and two scales of 2^-9 make a sum of 2^-20: with the least normal factor no normal number, with the rows' it is one."""
+    need_gpu()
+    factor = 1.7 * 2.0 ** -126
+    codes = torch.zeros(260, 16, dtype=torch.uint8)
+    codes[:, 8] = torch.arange(260) % 16 << 4                                 # (column 17)
+    scales = torch.zeros(260, 2)
+    scales[:, 1] = torch.arange(1, 261) % 9 * 2.0 ** -9
+    matrix = MicroscaledMatrix(codes.to(DEV), scales.to(torch.float8_e4m3fn).to(DEV), torch.tensor(factor, device=DEV))
+    x = torch.zeros(m, 32, device=DEV)
+    x[:, 0], x[:, 16], x[:, 17] = 2688.0, 4 * 2.0 ** -9, 0.5 * 2.0 ** -9
+    x *= (2.0 ** (torch.arange(m, device=DEV) % 110))[:, None]
+    for dtype in (F32, BF16):
+        y = gemm.linear(x.to(dtype), MicroscaledWeight(matrix), out_dtype=F32)
+        sums, slack = sums_of(x, matrix)
+        assert (sums != 0).any() and check_numbers(y, sums, slack * 0).all()      # (one product each: no sum is rounded)
+
+
+@pytest.mark.parametrize("m", [20, 300, 900])
+@pytest.mark.parametrize("size, factor, scale", [(1e-30, 1e36, 1e-15), (3e36, 1e-30, 1e-15), (1e30, 1e12, 1e-10), (1e-30, 1e-22, 1e15), (1.0, 1e-3, 0.0), (1.0, 1e-3, -0.75), (3e38, 1e30, 1e-18),
+                                                 (1e-38, 1e-15, 5e17)])
+def test_factors_of_pairs_at_the_ends_of_the_range(m, size, factor, scale):
+    need_gpu()
+    matrix = random_matrix(300, 520, m, DEV, factor)
+    x = (rows(m, 520, 5, F32, spread=0.1).clamp(-1, 1).double() * size).to(F32)
+    row_scale = scale * (1 + 0.5 * torch.rand(m, generator=torch.Generator().manual_seed(m))).to(DEV)
+    order = torch.randperm(m, generator=torch.Generator().manual_seed(m)).to(torch.int32).to(DEV)
+    y = torch.empty(m, 300, device=DEV)
+    ops.moe_expert_product(x, MicroscaledExperts([matrix]), y, torch.tensor([0, m], dtype=torch.int32, device=DEV), order, 1, x_by_pair=False, row_scale=row_scale)
+    sums, slack = sums_of(x, matrix)
+    each = row_scale.double()[order.long()][:, None]
+    check_numbers(y, sums * each, slack * each.abs())

@@ -48,7 +48,7 @@ __device__ __forceinline__ void ms_row_scale(uint32_t largest, float& r, float& 
 // most seven significant bits, so a number of up to twelve is either on the border or off by 2^-12 of it, far more than the 2^-22 that the
 // product with the reciprocal is off by: rounded to 16 bits, or to multiples of 2^-16 (a border of codes is 1/4 or more), it is on the border if and only if the exact
 // quotient is.  A bf16 has eight bits; a 32-bit number is first cut to twelve, the last of them set where any that was cut off is (which leaves it on the same side of
-// every number of fewer bits).
+// every number of fewer bits).  That holds for normal numbers: a subnormal one that may be near a border is multiplied by 2^32 before it is cut (ms_codes8).
 template <typename T> __device__ __forceinline__ float ms_odd12(float v) {
   if constexpr (sizeof(T) == 2) return v;
   const uint32_t b = __float_as_uint(v);
@@ -172,9 +172,22 @@ struct MsArgs {
   int K;
 };
 
-// An output from its sum(s): times the matrix's factor, the row's (a power of two) and the pair's, in turn, so that nothing leaves the range of 32 bits but what the
-// output itself does.
-__device__ __forceinline__ float ms_scaled(float sum, float w_factor, float x_factor, float row_scale) { return sum * w_factor * x_factor * row_scale; }
+// What a row's sums are multiplied by ahead of the matrix's factor f and behind it: y = sum * f * r * q, r the row's power of two (or NaN) and q its pair's factor (1 where it has
+// none).  A sum is 0 or from 2^-20 (two codes of 1/2, two scales of 2^-9) to under 2^56 in size.  With q = m 2^e, 1 <= m < 2, what comes first is the power of two 2^e r, kept
+// within 2^-106 .. 2^70, where it leaves every sum a normal number, and exact; what it was kept from comes last, with m.  So if the product with f is too large, so is y
+// (what is left is at least 1), and if that is too small to be a normal number, y is, too (what is left is less than 2): whatever f and r are, and q from 2^-60 to 2^60 in
+// size or 0, nothing leaves the range of 32 bits but what the output itself does.
+__device__ __forceinline__ float2 ms_row_factors(float r, float q) {
+  if (!(r < INFINITY && fabsf(q) < INFINITY) || q == 0.f) return make_float2(q == 0.f ? 0.f : 1.f, r * q);
+  int e = (int)(__float_as_uint(r) >> 23) - 2 * 127;
+  if (fabsf(q) < 0x1p-126f) q *= 0x1p24f, e -= 24;
+  const uint32_t bits = __float_as_uint(q);
+  e += (int)((bits >> 23) & 0xffu);
+  const int first = min(max(e, -106), 70), last = min(max(e - first, -126), 127);
+  return make_float2(__uint_as_float((uint32_t)(first + 127) << 23), __uint_as_float((bits & 0x807fffffu) | 0x3f800000u) * __uint_as_float((uint32_t)(last + 127) << 23));
+}
+// An output from its sum: see ms_row_factors.
+__device__ __forceinline__ float ms_scaled(float sum, float w_factor, float2 row) { return sum * row.x * w_factor * row.y; }
 
 // Products of rows that are there as codes (microscaled_tcgen05.cu, microscaled_2cta.cu), with arguments that tib_microscaled_product has checked.
 bool ms_on_pairs_of_sms(int M, int N, int steps, int experts);

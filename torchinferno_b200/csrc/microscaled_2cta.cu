@@ -138,7 +138,8 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
       const int in_tile = (int)rank * 128 + quarter * 32 + lane, row = m.first + in_tile, last = m.first + m.rows;      // (rows from `last` on are not stored)
       const int col0 = m.n_tile * 256 + half * 128;
       tile_factors[acc_phase * 256 + et] = w_factor;
-      const f32x2 x_factor2 = f2_pack(x_factor, x_factor), pair_factor2 = f2_pack(pair_factor, pair_factor);
+      const float2 of_row = ms_row_factors(x_factor, pair_factor);
+      const f32x2 ahead2 = f2_pack(of_row.x, of_row.x), behind2 = f2_pack(of_row.y, of_row.y);
       if (t + pairs < num_tiles) ask(next = tile_of(t + pairs));
       asm volatile("bar.sync 1, 256;\n" ::: "memory");      // (the last tile but one is finished: its factors have been read)
       if (ok && !mbar_wait_warp(acc_full_bar, acc_phase)) {
@@ -161,12 +162,12 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
 #pragma unroll
       for (int c = 0; c < 64; c += 2) {      // (see ms_scaled)
         const ulonglong2 f = factors2[c >> 1];
-        sum[c] = f2_mul(f2_mul(f2_pack(__uint_as_float(v[c >> 4][2 * c & 31]), __uint_as_float(v[c >> 4][(2 * c & 31) + 1])), f.x), x_factor2);
-        sum[c + 1] = f2_mul(f2_mul(f2_pack(__uint_as_float(v[c >> 4][(2 * c & 31) + 2]), __uint_as_float(v[c >> 4][(2 * c & 31) + 3])), f.y), x_factor2);
+        sum[c] = f2_mul(f2_mul(f2_pack(__uint_as_float(v[c >> 4][2 * c & 31]), __uint_as_float(v[c >> 4][(2 * c & 31) + 1])), ahead2), f.x);
+        sum[c + 1] = f2_mul(f2_mul(f2_pack(__uint_as_float(v[c >> 4][(2 * c & 31) + 2]), __uint_as_float(v[c >> 4][(2 * c & 31) + 3])), ahead2), f.y);
       }
-      if (a.row_scale) {
+      if (__any_sync(0xffffffffu, of_row.y != 1.f)) {      // (a pair's factor, or a row at the ends of the range)
 #pragma unroll
-        for (int c = 0; c < 64; ++c) sum[c] = f2_mul(sum[c], pair_factor2);
+        for (int c = 0; c < 64; ++c) sum[c] = f2_mul(sum[c], behind2);
       }
       // A row's outputs lie in one thread: a warp's 32 rows cross its 4 KB of shared memory, 128 bytes of each at a time (16-byte pieces, swizzled by row),
       // and leave as whole lines.

@@ -68,7 +68,7 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
   static_assert(8 * (2 * kMtMaxStages + 5) + 8 <= kMtBarBytes, "the barriers' share of shared memory");
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem_gen + (tmem_slot - base));
   float* red = reinterpret_cast<float*>(smem_gen + (bars - base) + kMtBarBytes);         // [splits][NT][128 / splits + 4] sums
-  float* tile_factors = red + mt_red_floats<NT>(splits);                                 // [2][NT][2] the rows' and their pairs', of two tiles in turn
+  float* tile_factors = red + mt_red_floats<NT>(splits);                                 // [2][NT][2] what a row's sums are multiplied by (ms_row_factors), of two tiles in turn
   int* tiles_before = reinterpret_cast<int*>(tile_factors + 4 * NT);                     // [experts + 1] where rows are sorted, and
   int* first_row = tiles_before + a.experts + 1;                                         // [experts + 1] their offsets
 
@@ -266,8 +266,8 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
       const float factor = a.w_factors[(size_t)m.expert * a.N + min(feature, a.N - 1)];
       float2* factors = reinterpret_cast<float2*>(tile_factors) + b * NT;
       if constexpr (MAKE) {
-        if (own_run == 0 && own_row < m.rows) factors[own_row] = make_float2(r, 1.f);
-      } else if (et < m.rows) factors[et] = make_float2(a.x.factors[m.first + et], a.row_scale ? a.row_scale[bs_pair(a.order, m.first + et, a.M)] : 1.f);
+        if (own_run == 0 && own_row < m.rows) factors[own_row] = ms_row_factors(r, 1.f);
+      } else if (et < m.rows) factors[et] = ms_row_factors(a.x.factors[m.first + et], a.row_scale ? a.row_scale[bs_pair(a.order, m.first + et, a.M)] : 1.f);
       asm volatile("bar.sync 1, %0;\n" ::"r"(32 * S::kStorers) : "memory");      // (the last tile but one is finished: its factors have been read)
       if constexpr (MAKE) {
         const __nv_bfloat16* src = a.made + own_row * a.ld_made;
@@ -326,8 +326,7 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
           float s[S::kTurn];
 #pragma unroll
           for (int j = 0; j < S::kTurn; ++j) {
-            const float2 f = factors[min(c + j, m.rows - 1)];
-            s[j] = ms_scaled(__uint_as_float(v[j]), factor, f.x, f.y);
+            s[j] = ms_scaled(__uint_as_float(v[j]), factor, factors[min(c + j, m.rows - 1)]);
           }
           if (!ok) return;
           if constexpr (kGated) {
@@ -381,8 +380,8 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
               u += from[r * NT * stride + kGated];
             }
           const float2 f = factors[c];
-          g = ms_scaled(g, g_factor, f.x, f.y);
-          u = ms_scaled(u, u_factor, f.x, f.y);
+          g = ms_scaled(g, g_factor, f);
+          u = ms_scaled(u, u_factor, f);
           y[(size_t)(m.first + c) * ldy + out] = from_f32<TO>(mt_act<ACT>(g, u, a));
         }
       }
