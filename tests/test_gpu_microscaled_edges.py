@@ -161,3 +161,34 @@ def test_factors_of_pairs_at_the_ends_of_the_range(m, size, factor, scale):
     sums, slack = sums_of(x, matrix)
     each = row_scale.double()[order.long()][:, None]
     check_numbers(y, sums * each, slack * each.abs())
+
+
+# ------------------------------------------------------------------------------------------------ blocks of several kernels on an SM
+def test_short_products_of_every_kind_side_by_side():
+    """4-bit, 8-bit and bf16 products with rings of one stage to full ones, tiles shared by clusters and not, behind one another in a stream and on three streams at once:
+    the bits of each by itself."""
+    need_gpu()
+    g = torch.Generator().manual_seed(3)
+    sizes = [(256, 512), (256, 2048), (512, 1024), (1024, 300 * 8), (2048, 1024), (768, 4096)]
+    weights = []
+    for i, (k, n) in enumerate(sizes):
+        dense = torch.randn(n, k, generator=g).to(DEV) / k ** 0.5
+        weights.append((k, MicroscaledWeight(random_matrix(n, k, i, DEV, 1e-5))))
+        weights.append((k, gemm.LinearWeight(dense.to(BF16), few_rows_tcgen05=True)))
+        weights.append((k, block_scaled.BlockScaledWeight(block_scaled.quantize_matrix(dense))))
+    inputs = {(m, k): rows(m, k, m + k, spread=0.2) for m in (3, 40, 64, 100) for k in {k for k, _ in sizes}}
+    calls = [(m, k, w) for m in (3, 40, 64, 100) for k, w in weights if m <= 64 or not isinstance(w, gemm.LinearWeight)]      # (bf16 above 64 rows: the library's)
+    g = torch.Generator().manual_seed(4)
+    want = {}
+    for i, (m, k, w) in enumerate(calls):
+        want[i] = gemm.linear(inputs[m, k], w)
+        torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for turn in range(6):
+        order, outs = torch.randperm(len(calls), generator=g).tolist(), []
+        for j, i in enumerate(order):
+            m, k, w = calls[i]
+            with torch.cuda.stream(streams[j % 3 if turn % 2 else 0]):
+                outs.append((i, gemm.linear(inputs[m, k], w)))
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want[i]) for i, y in outs)

@@ -26,6 +26,7 @@ namespace tib {
 constexpr int kB2Stages = 6, kB2Threads = 384;
 constexpr uint32_t kB2Half = 128 * kBlk, kB2Stage = 2 * kB2Half;
 constexpr uint32_t kB2Smem = kB2Stages * kB2Stage + 1024 /* alignment */ + 256 /* barriers */ + 8 * 4096 /* outputs */;
+static_assert(kB2Smem >= tmem_share_smem(512), "see smem_for_tmem");
 constexpr int kB2MaxExperts = (kMostSmem - (int)kB2Smem) / 8 - 1;      // (two numbers each in what is left of shared memory)
 // D fp32, A and B e4m3, both K-major, N = 256, M = 256 over the pair
 constexpr uint32_t kB2Idesc = (1u << 4) | ((256u >> 3) << 17) | ((256u >> 4) << 24);

@@ -279,10 +279,10 @@ block_scaled_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __g
       if (lane == 0) tiles_before[0] = 0, first_row[a.experts] = bs_offset(a.offsets, a.experts, a.M);
     }
   }
-  pdl_trigger();
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+  pdl_trigger();      // (tensor memory is this block's by now: a block of the kernel behind it cannot take it first)
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot_ptr, 0);
   if (splits > 1) cluster_sync_all();             // every block of the cluster runs and has its barriers
 
@@ -682,8 +682,8 @@ static int bs_tile_rows(int rows, int features, int runs) {
   return rows <= 64 || ceil_div(rows, 64) * f_tiles <= 148 ? 64 : 128;
 }
 
-// How a product runs: blocks in the grid, those that share a tile, steps of a block at most, stages of its ring.
-struct BsPlan { int grid, splits, steps, stages; };
+// How a product runs: blocks in the grid, those that share a tile, steps of a block at most, stages of its ring, shared memory.
+struct BsPlan { int grid, splits, steps, stages; uint32_t smem; };
 template <int NT, bool CODES> static int bs_plan(int M, int N, int runs, int experts, BsPlan& p) {      // experts: 0 for one matrix
   using S = BsShape<NT, CODES>;
   constexpr int kBlocks = 148 * S::kPerSm;
@@ -696,6 +696,7 @@ template <int NT, bool CODES> static int bs_plan(int M, int N, int runs, int exp
   p.steps = (int)(steps < 0x7fffffff ? steps : 0x7fffffff);
   p.stages = 1;
   while (p.stages < kBsMaxStages && p.stages < p.steps && bs_smem<NT>(p.stages + 1, p.splits, experts) <= (S::kPerSm > 1 ? 113u * 1024 : (uint32_t)kMostSmem)) ++p.stages;
+  p.smem = smem_for_tmem(bs_smem<NT>(p.stages, p.splits, experts), S::kTmemCols);
   // (A wait by parity tells a stage's last use from the one before only while a helper's step before implies the latter is over: with no more helpers
   // than stages, or every stage used once.)
   return !CODES && p.stages < S::kHelpers && p.stages < p.steps ? TIB_E_SMEM : TIB_OK;
@@ -723,7 +724,7 @@ static int launch_block_scaled(const CUtensorMap& map_w, const CUtensorMap& map_
   if (device < 64) allowed[device] = true;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(BsShape<NT, kCodes>::kThreads);
-  cfg.dynamicSmemBytes = bs_smem<NT>(plan.stages, plan.splits, experts);
+  cfg.dynamicSmemBytes = plan.smem;
   cfg.stream = stream;
   cfg.gridDim = dim3((unsigned)plan.grid);
   cudaLaunchAttribute attr[2];
@@ -793,14 +794,31 @@ TIB_API int tib_block_scaled_tcgen05(const void* x, int x_dtype, int64_t ldx, in
 #undef TIB_BS_GO
 }
 
-// How a product of M rows (codes, or not) with one matrix (experts 0) or sorted by expert runs here: {rows of a tile at most, blocks that share a tile, steps of a
-// block at most, stages of its ring}.
-TIB_API int tib_block_scaled_tcgen05_plan(int codes, int M, int N, int K, int experts, int* plan) {
-  if (!plan || M < 1 || N < 1 || K < 1 || experts < 0 || experts > kBsMaxExperts) return TIB_E_ARG;
-  const int runs = ceil_div(K, kBlk), nt = codes ? bs_code_rows(M, N, runs, experts) : 16;
+template <int NT, bool CODES> static int bs_room(int M, int N, int runs, int experts, int* plan, int* room) {
   BsPlan p;
-  const int rc = nt == 16 ? bs_plan<16, false>(M, N, runs, experts, p) : nt == 32 ? bs_plan<32, true>(M, N, runs, experts, p)
-               : nt == 64 ? bs_plan<64, true>(M, N, runs, experts, p) : bs_plan<128, true>(M, N, runs, experts, p);
-  plan[0] = nt; plan[1] = p.splits; plan[2] = p.steps; plan[3] = p.stages;
+  const int rc = bs_plan<NT, CODES>(M, N, runs, experts, p);
+  if (plan) plan[0] = NT, plan[1] = p.splits, plan[2] = p.steps, plan[3] = p.stages;
+  if (room) room[0] = (int)BsShape<NT, CODES>::kTmemCols, room[1] = (int)p.smem;
   return rc;
 }
+static int bs_plan_of(int codes, int M, int N, int K, int experts, int* plan, int* room) {
+  if (M < 1 || N < 1 || K < 1 || experts < 0 || experts > kBsMaxExperts) return TIB_E_ARG;
+  const int runs = ceil_div(K, kBlk);
+  switch (codes ? bs_code_rows(M, N, runs, experts) : 16) {
+    case 16: return bs_room<16, false>(M, N, runs, experts, plan, room);
+    case 32: return bs_room<32, true>(M, N, runs, experts, plan, room);
+    case 64: return bs_room<64, true>(M, N, runs, experts, plan, room);
+    default: return bs_room<128, true>(M, N, runs, experts, plan, room);
+  }
+}
+
+// How a product of M rows (codes, or not) with one matrix (experts 0) or sorted by expert runs here: {rows of a tile at most, blocks that share a tile, steps of a
+// block at most, stages of its ring}; and what a block of it takes of an SM: {columns of tensor memory (of 512), bytes of shared memory} (smem_for_tmem).
+TIB_API int tib_block_scaled_tcgen05_plan(int codes, int M, int N, int K, int experts, int* plan) {
+  return plan ? bs_plan_of(codes, M, N, K, experts, plan, nullptr) : TIB_E_ARG;
+}
+TIB_API int tib_block_scaled_tcgen05_room(int codes, int M, int N, int K, int experts, int* room) {
+  return room ? bs_plan_of(codes, M, N, K, experts, nullptr, room) : TIB_E_ARG;
+}
+
+TIB_PACKED(tib_block_scaled_tcgen05_room)

@@ -197,7 +197,7 @@ TIB_API int tib_microscaled_product(const void* w, const void* w_scales, const f
   MsArgs a;
   a.x = MsRows{(const unsigned char*)codes, (const unsigned char*)scales, factors, ms_groups(M, offsets ? experts : 0)};
   a.w = (const unsigned char*)w; a.w_scales = (const unsigned char*)w_scales; a.w_factors = w_factors;
-  a.M = M; a.N = N; a.steps = ms_steps(K); a.stages = a.tmem_cols = 0; a.offsets = offsets; a.order = order; a.experts = experts;
+  a.M = M; a.N = N; a.steps = ms_steps(K); a.stages = a.tmem_cols = a.scale_cols = 0; a.offsets = offsets; a.order = order; a.experts = experts;
   a.limit = limit; a.alpha = alpha; a.row_scale = row_scale; a.error_word = error_word;
   a.made = made_inside ? (const __nv_bfloat16*)x : nullptr; a.ld_made = ldx; a.K = K;
   if (!made_inside && ms_on_pairs_of_sms(M, N, a.steps, offsets ? experts : 0)) return ms_product_2cta(a, act, y, y_dtype, ldy, stream);
@@ -212,6 +212,12 @@ TIB_API int tib_microscaled_plan(int M, int N, int K, int experts, int* plan) {
   return ms_on_pairs_of_sms(M, N, steps, experts) ? ms_plan_2cta(M, N, steps, experts, plan) : ms_plan_tcgen05(M, N, steps, experts, plan);
 }
 
+// What a block of such a product takes of an SM: {columns of tensor memory (of 512), bytes of shared memory} (smem_for_tmem).
+TIB_API int tib_microscaled_room(int M, int N, int K, int experts, int* room) {
+  if (!room || M < 1 || N < 1 || K < 1 || experts < 0) return TIB_E_ARG;
+  return ms_on_pairs_of_sms(M, N, ms_steps(K), experts) ? ms_room_2cta(experts, room) : ms_room_tcgen05(M, N, ms_steps(K), experts, room);
+}
+
 // Whether tib_microscaled_product makes the codes of M rows of 16-bit numbers (16-byte aligned, as is a row's stride) for one matrix without room for them (codes null).
 TIB_API int tib_microscaled_makes(int M, int N, int K, int* answer) {
   if (!answer || M < 1 || N < 1 || K < 1) return TIB_E_ARG;
@@ -224,3 +230,4 @@ TIB_PACKED(tib_microscaled_makes)
 TIB_PACKED(tib_microscaled_widen)
 TIB_PACKED(tib_microscaled_product)
 TIB_PACKED(tib_microscaled_plan)
+TIB_PACKED(tib_microscaled_room)

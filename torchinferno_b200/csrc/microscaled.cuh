@@ -160,7 +160,7 @@ struct MsArgs {
   const unsigned char* w;          // codes of the matrices
   const unsigned char* w_scales;
   const float* w_factors;          // [experts, N]
-  int M, N, steps, stages, tmem_cols;
+  int M, N, steps, stages, tmem_cols, scale_cols;
   const int* offsets;              // [experts + 1] of rows sorted by expert, or null: one matrix
   const int* order;
   int experts;
@@ -195,6 +195,9 @@ int ms_product_2cta(const MsArgs& a, int act, void* y, int y_dtype, int64_t ldy,
 // How a product runs there: {rows of a tile at most, blocks that share a tile, steps of a block at most, stages of its ring}.
 int ms_plan_2cta(int M, int N, int steps, int experts, int* plan);
 int ms_plan_tcgen05(int M, int N, int steps, int experts, int* plan);
+// What a block of it takes: {columns of tensor memory, bytes of shared memory}.
+int ms_room_2cta(int experts, int* room);
+int ms_room_tcgen05(int M, int N, int steps, int experts, int* room);
 // Whether the kernel of a product with one matrix may make the codes of its rows itself.
 bool ms_makes_rows(int M, int N, int K);
 int ms_product_tcgen05(MsArgs& a, int act, void* y, int y_dtype, int64_t ldy, cudaStream_t stream);

@@ -348,6 +348,9 @@ static int m2_map(CUtensorMap* map, const void* ptr, int64_t pieces, int bytes, 
   return r == CUDA_SUCCESS ? TIB_OK : TIB_E_ARG;
 }
 
+static_assert(kM2Smem >= tmem_share_smem(512), "see smem_for_tmem");
+static uint32_t m2_smem(int experts) { return kM2Smem + (experts ? 8 * (experts + 1) : 0); }
+
 static int64_t m2_tiles(int M, int N, int experts) {      // at most; experts: 0 for one matrix
   return (int64_t)(experts ? M / 256 + (M < experts ? M : experts) : ceil_div(M, 256)) * ceil_div(N, 256);
 }
@@ -364,7 +367,7 @@ static int launch_m2(const CUtensorMap (&maps)[4], const MsArgs& a, void* out, i
   const int64_t tiles = m2_tiles(a.M, a.N, a.offsets ? a.experts : 0);
   if (tiles > 0x7fffffff) return TIB_E_SIZE;
   const int wide = ((uintptr_t)out & 15) == 0 && (ldo * sizeof(TO)) % 16 == 0;
-  TIB_LAUNCH_DEPENDENT(kern, 2 * (int)(tiles < 74 ? tiles : 74), kM2Threads, kM2Smem + (a.offsets ? 8 * (a.experts + 1) : 0), stream, maps[0], maps[1], maps[2], maps[3], a,
+  TIB_LAUNCH_DEPENDENT(kern, 2 * (int)(tiles < 74 ? tiles : 74), kM2Threads, m2_smem(a.offsets ? a.experts : 0), stream, maps[0], maps[1], maps[2], maps[3], a,
                        (TO*)out, ldo, wide);
   return TIB_OK;
 }
@@ -411,5 +414,10 @@ int tib::ms_product_2cta(const MsArgs& a, int act, void* out, int out_dtype, int
 int tib::ms_plan_2cta(int M, int N, int steps, int experts, int* plan) {
   const int64_t tiles = m2_tiles(M, N, experts), most = steps * ceil_div64(tiles, tiles < 74 ? tiles : 74);
   plan[0] = 256; plan[1] = 1; plan[2] = (int)(most < 0x7fffffff ? most : 0x7fffffff); plan[3] = kM2Stages;
+  return TIB_OK;
+}
+
+int tib::ms_room_2cta(int experts, int* room) {
+  room[0] = 512; room[1] = (int)m2_smem(experts);
   return TIB_OK;
 }

@@ -17,8 +17,6 @@
 // have their next columns on their way, 22.5 with four that wait for each eight of them, 12.8 without.  Every wait is bounded and reports in error_word.
 #include "microscaled.cuh"
 
-#include <algorithm>
-
 namespace tib {
 
 constexpr int kMtMaxExperts = 1024, kMtMaxStages = 8;
@@ -28,9 +26,9 @@ template <int NT> struct MtShape {
   static constexpr int kPerSm = NT <= 32 ? 2 : 1;                                // blocks of an SM
   static constexpr int kStorers = NT >= 128 ? 8 : 4, kThreads = 64 + 32 * kStorers, kCols = NT / (kStorers / 4);      // (columns of a storer)
   static constexpr int kTurn = NT >= 128 ? 16 : 8;                               // columns that it takes at a time
-  // Tensor memory: accumulators (two; one of a shared tile, which is a block's only one), then 32 columns of scales a stage.
+  // Tensor memory: accumulators (two; one where a block has one tile, as it has of shared ones), then 32 columns of scales a stage.  At most:
   static constexpr uint32_t tmem_cols(int splits) { return (splits > 1 ? 256 : 512) / kPerSm; }
-  __host__ __device__ static constexpr uint32_t scale_cols(int splits) { return splits > 1 ? NT : 2 * NT; }
+  static constexpr uint32_t scale_cols(int splits) { return splits > 1 ? NT : 2 * NT; }
   static constexpr int stages(int splits) { return (tmem_cols(splits) - scale_cols(splits)) / 32 < kMtMaxStages ? (tmem_cols(splits) - scale_cols(splits)) / 32 : kMtMaxStages; }
   static constexpr uint32_t kStage = kMtWBytes + NT * kMsStepBytes + 2 * kMsStepScales;
 };
@@ -210,7 +208,7 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
         }
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         const uint32_t stage = base + s * S::kStage, scales = stage + kMtWBytes + NT * kMsStepBytes;
-        const uint32_t w_src = umma_low_k128(stage), x_src = w_src + (kMtWBytes >> 4), columns = tmem_base + S::scale_cols(splits) + 32 * s;
+        const uint32_t w_src = umma_low_k128(stage), x_src = w_src + (kMtWBytes >> 4), columns = tmem_base + a.scale_cols + 32 * s;
         if (leader) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) ms_copy_scales<1>(columns + 4 * k, scales + kMsChunkBytes * k);      // (four of w, four of the rows)
@@ -415,8 +413,9 @@ static int mt_splits(int64_t tiles, int steps, int M, int blocks) {
   return steps < 4 ? 1 : tiles * 4 <= blocks ? 4 : tiles * 2 <= blocks ? 2 : 1;
 }
 
-// How a product runs: blocks in the grid, those that share a tile, steps of a block at most, stages of its ring.
-struct MtPlan { int grid, splits, steps, stages; };
+// How a product runs: blocks in the grid, those that share a tile, steps of a block at most, stages of its ring; where its scales begin in tensor memory, and what a
+// block takes of that and of shared memory.
+struct MtPlan { int grid, splits, steps, stages, scale_cols; uint32_t tmem_cols, smem; };
 template <int NT> static int mt_plan(int M, int N, int steps, int experts, MtPlan& p) {      // experts: 0 for one matrix
   using S = MtShape<NT>;
   constexpr int kBlocks = 148 * S::kPerSm;
@@ -428,6 +427,10 @@ template <int NT> static int mt_plan(int M, int N, int steps, int experts, MtPla
   p.steps = (int)(most < 0x7fffffff ? most : 0x7fffffff);
   p.stages = 1;
   while (p.stages < S::stages(p.splits) && p.stages < p.steps && mt_smem<NT>(p.stages + 1, p.splits, experts) <= (S::kPerSm > 1 ? 113u * 1024 : (uint32_t)kMostSmem)) ++p.stages;
+  p.scale_cols = (p.grid == tiles * p.splits ? 1 : 2) * NT;
+  p.tmem_cols = p.splits > 1 ? 128 : 32;      // (in clusters: see smem_for_tmem)
+  while (p.tmem_cols < (uint32_t)(p.scale_cols + 32 * p.stages)) p.tmem_cols *= 2;
+  p.smem = smem_for_tmem(mt_smem<NT>(p.stages, p.splits, experts), p.tmem_cols);
   return TIB_OK;
 }
 // Rows of a tile: 32 where all rows are one tile, else 128 (the tiles of their scales).  A tile's time is that of its weights: 8, 32, 33, 64 and 128 rows
@@ -441,7 +444,8 @@ static int launch_mt(MsArgs& a, void* y, int64_t ldy, cudaStream_t stream) {
   const int rc = mt_plan<NT>(a.M, a.N, a.steps, experts, plan);
   if (rc != TIB_OK) return rc;
   a.stages = plan.stages;
-  a.tmem_cols = (int)MtShape<NT>::tmem_cols(plan.splits);
+  a.tmem_cols = (int)plan.tmem_cols;
+  a.scale_cols = plan.scale_cols;
   auto kern = microscaled_tcgen05_kernel<NT, ACT, TO, MAKE>;
   static bool allowed[64];      // (by device: the attribute belongs to its context)
   int device = 0;
@@ -451,10 +455,7 @@ static int launch_mt(MsArgs& a, void* y, int64_t ldy, cudaStream_t stream) {
   if (device < 64) allowed[device] = true;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(MtShape<NT>::kThreads);
-  cfg.dynamicSmemBytes = mt_smem<NT>(plan.stages, plan.splits, experts);
-  // Blocks that wait for others of their cluster must not wait for tensor memory that a block of another such cluster holds while it waits for one that cannot have it here
-  // (two streams' calls): a shared tile's block takes as large a share of an SM's shared memory (228 KB, 1 KB of it for each block itself) as of its 512 columns.
-  if (plan.splits > 1) cfg.dynamicSmemBytes = std::max(cfg.dynamicSmemBytes, (size_t)a.tmem_cols * (228 * 1024 / 512) - 1024);
+  cfg.dynamicSmemBytes = plan.smem;
   cfg.stream = stream;
   cfg.gridDim = dim3((unsigned)plan.grid);
   cudaLaunchAttribute attr[2];
@@ -492,7 +493,7 @@ using namespace tib;
 // 3.8 / 4.7; 4 rows 2,048 -> 2,048 4.3 / 4.9; 2 rows 4,096 -> 4,096 6.5 / 6.5; 1 row 4,096 -> 28,672 14.6 / 14.5, 2 rows 15.2 / 14.8; 1 row 8,192 -> 8,192 10.4 / 10.2; where calls
 // are bound by the host 8.5 / 12.1 each.  With more rounds every block's reading of all rows shows: 4 rows 4,096 -> 4,096 8.0 / 6.6, 1 row 14,336 -> 4,096 11.2 / 10.5.)
 bool tib::ms_makes_rows(int M, int N, int K) {
-  MtPlan p;
+  MtPlan p{};
   return M <= 8 && K % 8 == 0 && K <= 1024 << mt_more_loads(M) && mt_plan<32>(M, N, ms_steps(K), 0, p) == TIB_OK && p.grid == ceil_div(N, 128) * p.splits;
 }
 
@@ -506,10 +507,18 @@ int tib::ms_product_tcgen05(MsArgs& a, int act, void* y, int y_dtype, int64_t ld
 #undef TIB_MT_GO
 }
 
+static int mt_plan_of(int M, int N, int steps, int experts, MtPlan& p) {
+  return mt_tile_rows(M) == 32 ? mt_plan<32>(M, N, steps, experts, p) : mt_plan<128>(M, N, steps, experts, p);
+}
 int tib::ms_plan_tcgen05(int M, int N, int steps, int experts, int* plan) {
-  MtPlan p;
-  plan[0] = mt_tile_rows(M);
-  const int rc = plan[0] == 32 ? mt_plan<32>(M, N, steps, experts, p) : mt_plan<128>(M, N, steps, experts, p);
-  plan[1] = p.splits; plan[2] = p.steps; plan[3] = p.stages;
+  MtPlan p{};
+  const int rc = mt_plan_of(M, N, steps, experts, p);
+  plan[0] = mt_tile_rows(M); plan[1] = p.splits; plan[2] = p.steps; plan[3] = p.stages;
+  return rc;
+}
+int tib::ms_room_tcgen05(int M, int N, int steps, int experts, int* room) {
+  MtPlan p{};
+  const int rc = mt_plan_of(M, N, steps, experts, p);
+  room[0] = (int)p.tmem_cols; room[1] = (int)p.smem;
   return rc;
 }

@@ -9,6 +9,15 @@ namespace tib {
 
 constexpr uint32_t kWaitLimit = 1u << 22;
 
+// Tensor memory (512 columns an SM) is waited for in the hardware, in no order and without a limit.  Two blocks that wait for each other would wait for good: blocks of two
+// clusters, each with columns that a partner of the other's lacks, or a block without columns and one of a later kernel that was let in early, took them and waits for the
+// former's kernel to end.  So a block takes as large a share of an SM's shared memory (228 KB, 1 KB of it for each block itself) as of its columns: blocks that are on an SM
+// together then all find theirs.  (Of 256 columns and more, 28 columns' share less: two such blocks leave 25 KB, less than any kernel with columns takes, but room for the
+// small kernels behind them.)  The products of 4-bit and 8-bit weights see to it by these; bf16 products in clusters take that much and more, but on pairs of SMs 512 columns
+// and 199 KB: a block of another cluster takes more than the 29 KB beside it.
+constexpr uint32_t tmem_share_smem(uint32_t columns) { return (columns - (columns >= 256 ? 28 : 0)) * (228 * 1024 / 512) - 1024; }
+static inline uint32_t smem_for_tmem(uint32_t smem, uint32_t columns) { return smem > tmem_share_smem(columns) ? smem : tmem_share_smem(columns); }
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
