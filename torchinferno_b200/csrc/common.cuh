@@ -183,8 +183,14 @@ __device__ __forceinline__ float block_sum(float v, float* scratch) {
 // kernel wrote (or writes anything an earlier kernel reads).  pdl_wait() returns once every kernel
 // before it has completed and its writes are visible; in a kernel launched the ordinary way it
 // returns at once.  pdl_trigger() lets the kernel after this one be placed early in the same way.
-// Every kernel of this library that is launched this way waits first thing, so completion is
-// transitive along the stream.  The switch is process-wide (tib_set_dependent_launch).
+// A grid is over only when all its threads are, some of which wait in every kernel launched this way: completion is transitive along the stream.
+// What may be read ahead of pdl_wait().  Most kernels wait first thing and then call pdl_trigger().  Some trigger ahead of their wait: the norms and rows that leave codes
+// (quantized_norm.cu, microscaled.cu), which do nothing before it, and those that also read before it: the bf16 products of few rows (gemm_decode.cu, gemm_tcgen05.cu), 4-bit and
+// 8-bit products (weights) and the decode attention (slots, positions, the block table, pages up to the newest token's tile).  A chain of these may have
+// its last kernel at work while the one ahead of the chain still writes.  So whatever a kernel reads before it waits has to be written ahead of
+// a kernel that waits and then triggers: the embedding stands between a step's records, positions and tokens and its first norm, and a page is read so
+// in the step behind the one that wrote it at the earliest.  (Weights come from copies and from torch's kernels, which let nobody in before their end.)
+// The switch is process-wide (tib_set_dependent_launch).
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
 

@@ -3,8 +3,8 @@
 //     h = residual + delta (32 bits; kept as the next residual),  v = h / sqrt(mean(h^2) + eps) * weight, rounded to the rows' type,  codes and scales of v
 // A block takes a row.  The sums run in tib_add_rmsnorm's order and the codes are made of what it writes, so that codes, scales and residual are bit for
 // bit those of the three steps one by one.
-// It lets the kernel behind it in before it waits for the one ahead.  That is as good for whoever waits: a kernel is over only when the one ahead of it is.  What kernels behind it read
-// before they wait (weights, positions, older pages of the cache) was there before the step's first kernels, which wait before they let anybody in.
+// It lets the kernel behind it in before it waits for the one ahead.  That is as good for whoever waits: a kernel is over only when the one ahead of it is.  (What kernels
+// behind it may read before they wait: see launch_dependent.)
 // What bounds it: memory.  8,192 x 4,096 bf16: 61.7 us for 354 MB (5.7 TB/s; tib_add_rmsnorm, whose rows leave in bf16, takes 60.9, and codes made behind it 17.7 more), in 32 bits
 // 69 us for 421 MB; eight rows 2.9 us, where tib_add_rmsnorm takes 2.5 and the codes 2.
 #include "microscaled.cuh"
