@@ -53,3 +53,36 @@ def test_no_room_for_no_product(sizes):
     for status in (ops.lib().tib_microscaled_room(m, n, k, e, ctypes.addressof(found)), ops.lib().tib_block_scaled_tcgen05_room(1, m, n, k, e, ctypes.addressof(found)),
                    ops.lib().tib_microscaled_room(8, 8, 8, 0, 0), ops.lib().tib_block_scaled_tcgen05_room(1, 8, 8, 8, 0, 0)):
         assert status < 0
+
+
+# ------------------------------------------------------------------------------------------------ checkpoints
+def folder_of(tmp_path, said, **more):
+    """A random model folder in 4-bit codes whose config.json says this, with these tensors beside its own."""
+    import json
+    from conftest import TINY_B
+    from safetensors.torch import load_file, save_file
+    from torchinferno_b200.weights.random_init import build_model, write_random_model
+    write_random_model({**TINY_B, "quantization_config": {"quant_method": "modelopt", "quant_algo": "NVFP4"}}, tmp_path, seed=0)
+    config = {**TINY_B} if said is None else {**TINY_B, "quantization_config": said}
+    (tmp_path / "config.json").write_text(json.dumps(config))
+    tensors = {k: v.clone() for k, v in load_file(str(tmp_path / "model.safetensors")).items()}
+    save_file({**tensors, **more}, str(tmp_path / "model.safetensors"))
+    return build_model(config, dtype=torch.bfloat16, device="cpu")
+
+
+@pytest.mark.parametrize("said, form", [({"quant_method": "modelopt", "quant_algo": "FP8"}, "'FP8'"), ({"quant_method": "modelopt", "quant_algo": "W4A16_AWQ"}, "'W4A16_AWQ'"),
+                                        ({"quant_algo": "MIXED_PRECISION"}, "'MIXED_PRECISION'"), ({"quant_method": "fp8", "weight_block_size": [128, 128]}, "'fp8'"),
+                                        ({"quant_method": "awq", "bits": 4}, "'awq'")])
+def test_codes_of_a_folder_that_names_another_form_are_refused(tmp_path, said, form):
+    from torchinferno_b200.weights.loader import WeightError, load_weights
+    with pytest.raises(WeightError, match=f"4-bit codes, but quantization_config names {form}"):
+        load_weights(folder_of(tmp_path, said), tmp_path)
+
+
+@pytest.mark.parametrize("said", [None, {}, {"quant_algo": "nvfp4"}, {"quant_method": "modelopt"}, {"quant_method": "modelopt_fp4"}, {"quant_method": "modelopt", "quant_algo": "NVFP4", "group_size": 16}])
+def test_codes_of_a_folder_that_names_them_or_nothing_are_read(tmp_path, said):
+    from torchinferno_b200.kernels.microscaled import MicroscaledWeight
+    from torchinferno_b200.weights.loader import load_weights
+    model = folder_of(tmp_path, said)
+    load_weights(model, tmp_path)
+    assert isinstance(model.blocks[0].feed_forward.down_weight, MicroscaledWeight)

@@ -89,6 +89,15 @@ class MicroscaledQuantization:
         return not any(f".{module}." in f".{name}." or fnmatchcase(name, module) or fnmatchcase(name.rpartition(".")[0], module) for module in self.ignored)
 
 
+def check_codes(config: Mapping[str, Any]) -> None:
+    """Raises ConfigError where config.json says of a folder that holds 4-bit codes that they are of another form.  (One that says nothing of them is taken by its tensors.)"""
+    data = _settings(config)
+    algo, method = (str(data.get(key) or "") for key in ("quant_algo", "quant_method"))
+    if algo.upper() not in ("", "NVFP4") or (not algo and method and not method.lower().startswith("modelopt")):
+        raise ConfigError(f"quantization_config names {algo or method!r} (codes with a scale for each 16 columns are 'NVFP4')")
+    MicroscaledQuantization.from_config(config)
+
+
 def quantization_of(config: Mapping[str, Any]) -> "BlockQuantization | MicroscaledQuantization | None":
     """The form of quantised weights that config.json names, if it is one that is read."""
     return BlockQuantization.from_config(config) or MicroscaledQuantization.from_config(config)

@@ -17,7 +17,7 @@ codes with a tensor of scales beside it (its name and ``_scale_inv``) stays so i
 bfloat16, and is widened to the numbers it stands for in float32; so does one stored as
 4-bit codes with tensors of scales (its name and ``_scale``) and a factor (``_scale_2``)
 beside it.  Codes without their scales are refused, and so are those of a folder whose
-``quantization_config`` names another form (config/quantization.py).
+``quantization_config`` names other blocks, or another form of 4-bit codes (config/quantization.py).
 """
 from __future__ import annotations
 
@@ -28,7 +28,7 @@ from typing import Iterable
 import torch
 
 from torchinferno_b200.config.model_config import ConfigError
-from torchinferno_b200.config.quantization import (CODE_FACTOR_SUFFIX, CODE_SCALE_SUFFIX, SCALE_SUFFIX, BlockQuantization, MicroscaledQuantization,
+from torchinferno_b200.config.quantization import (CODE_FACTOR_SUFFIX, CODE_SCALE_SUFFIX, SCALE_SUFFIX, BlockQuantization, check_codes,
                                                    measured_scale_of_rows)
 from torchinferno_b200.kernels.block_scaled import BlockScaledMatrix, blocks
 from torchinferno_b200.kernels.microscaled import RUN, MicroscaledMatrix
@@ -149,10 +149,10 @@ def load_weights(model, folder: str | Path) -> dict[str, object]:
             raise WeightError("\n".join(parts))
         if (in_blocks or in_codes) and (Path(folder) / CONFIG_FILE).is_file():
             said = json.loads((Path(folder) / CONFIG_FILE).read_text())
-            for held, form, what in ((in_blocks, BlockQuantization, "8-bit blocks"), (in_codes, MicroscaledQuantization, "4-bit codes")):
+            for held, check, what in ((in_blocks, BlockQuantization.from_config, "8-bit blocks"), (in_codes, check_codes, "4-bit codes")):
                 try:
                     if held:
-                        form.from_config(said)
+                        check(said)
                 except ConfigError as exc:
                     raise WeightError(f"checkpoint {folder} holds {what}, but {exc}") from None
         tensors: dict[str, torch.Tensor] = {}
