@@ -86,3 +86,32 @@ def test_codes_of_a_folder_that_names_them_or_nothing_are_read(tmp_path, said):
     model = folder_of(tmp_path, said)
     load_weights(model, tmp_path)
     assert isinstance(model.blocks[0].feed_forward.down_weight, MicroscaledWeight)
+
+
+CACHE_SCALES = {f"model.layers.{i}.self_attn.{p}_proj.{p}_scale": torch.tensor(0.05 * (i + 1)) for i in range(2) for p in "kv"}
+
+
+def test_scales_of_an_8_bit_cache_are_left_aside(tmp_path):
+    from torchinferno_b200.kernels.microscaled import MicroscaledWeight
+    from torchinferno_b200.weights.loader import load_weights
+    said = {"quant_method": "modelopt", "quant_algo": "NVFP4", "kv_cache_scheme": {"dynamic": False, "num_bits": 8, "type": "float"}}
+    model = folder_of(tmp_path, said, **CACHE_SCALES, **{"model.layers.0.self_attn.k_proj.input_scale": torch.tensor(0.1)})
+    report = load_weights(model, tmp_path)
+    assert report["ignored"] == sorted([*CACHE_SCALES, "model.layers.0.self_attn.k_proj.input_scale"])
+    plain = folder_of(tmp_path, said)
+    load_weights(plain, tmp_path)
+    assert isinstance(model.blocks[0].mixer.qkv_weight, MicroscaledWeight)
+    assert torch.equal(model.blocks[0].mixer.qkv_weight.tiles.codes, plain.blocks[0].mixer.qkv_weight.tiles.codes)
+
+
+def test_scales_of_a_cache_beside_other_tensors_are_not_known(tmp_path):
+    from conftest import TINY_B
+    from safetensors.torch import load_file, save_file
+    from torchinferno_b200.weights.loader import WeightError, load_weights
+    from torchinferno_b200.weights.random_init import build_model, write_random_model
+    with pytest.raises(WeightError, match="unexpected"):
+        load_weights(folder_of(tmp_path, None, **{"model.norm.k_scale": torch.ones(1)}), tmp_path)
+    write_random_model(TINY_B, tmp_path, seed=0)      # (a folder without codes)
+    save_file({**load_file(str(tmp_path / "model.safetensors")), **CACHE_SCALES}, str(tmp_path / "model.safetensors"))
+    with pytest.raises(WeightError, match="unexpected"):
+        load_weights(build_model(TINY_B, dtype=torch.bfloat16, device="cpu"), tmp_path)

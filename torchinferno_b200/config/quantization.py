@@ -4,7 +4,8 @@ Two forms are read.  ``"quant_method": "fp8"`` with a scale for each block of 12
 codes, its scales are the 32-bit tensor ``name + "_scale_inv"``, and activations are quantised as they come (``"activation_scheme": "dynamic"``).
 The rows' scales are powers of two (kernels/block_scaled.py), whether or not the file says so (``scale_fmt``).
 ``"quant_algo": "NVFP4"``: a matrix ``name`` is e2m1 codes, two in a byte, with an e4m3 scale for each 16 columns (``name + "_scale"``) and one 32-bit factor
-(``name + "_scale_2"``); the rows' scales are their own (kernels/microscaled.py), so the measured ones that such files hold (``input_scale``) are not read.
+(``name + "_scale_2"``); the rows' scales are their own (kernels/microscaled.py), so the measured ones that such files hold (``input_scale``), and those of an
+8-bit cache (``k_scale``, ``v_scale``), are not read.
 Which of a model's matrices may be stored so is up to its parts (``WeightSpec.block_scaled``); which of them are is seen from the file.
 Other methods are left to the loader, which refuses tensors that the model does not know; a file with 8-bit blocks or 4-bit codes is checked against its form, and random
 models leave any other aside.
@@ -24,6 +25,12 @@ CODE_SCALE_SUFFIX, CODE_FACTOR_SUFFIX = "_scale", "_scale_2"
 def measured_scale_of_rows(name: str) -> str | None:
     """The tensor that files in 4 bits hold beside the matrix ``name`` for the rows it meets, which is not read."""
     return name.removesuffix("weight") + "input_scale" if name.endswith(".weight") else None
+
+
+def scales_of_a_cache(name: str) -> tuple[str, ...]:
+    """The tensors that files in 4 bits which were made for a key and value cache in 8 bits hold beside the projection ``name``.  They concern such a cache alone, and
+    are not read: the cache here has the model's own type."""
+    return tuple(name.removesuffix("weight") + suffix for suffix in ("k_scale", "v_scale")) if name.endswith(".weight") else ()
 
 
 def _settings(config: Mapping[str, Any]) -> Mapping[str, Any]:

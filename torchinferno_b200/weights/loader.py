@@ -29,7 +29,7 @@ import torch
 
 from torchinferno_b200.config.model_config import ConfigError
 from torchinferno_b200.config.quantization import (CODE_FACTOR_SUFFIX, CODE_SCALE_SUFFIX, SCALE_SUFFIX, BlockQuantization, check_codes,
-                                                   measured_scale_of_rows)
+                                                   measured_scale_of_rows, scales_of_a_cache)
 from torchinferno_b200.kernels.block_scaled import BlockScaledMatrix, blocks
 from torchinferno_b200.kernels.microscaled import RUN, MicroscaledMatrix
 
@@ -107,6 +107,8 @@ def load_weights(model, folder: str | Path) -> dict[str, object]:
         in_codes = {n for n, ws in expected.items() if ws.block_scaled and n in files and n + CODE_SCALE_SUFFIX in files and n + CODE_FACTOR_SUFFIX in files}
         beside_codes = {n + suffix for n in in_codes for suffix in (CODE_SCALE_SUFFIX, CODE_FACTOR_SUFFIX)}
         not_needed = {measured_scale_of_rows(n) for n in in_codes}
+        if in_codes:      # (whichever of the matrices are in codes)
+            not_needed.update(scale for n, ws in expected.items() if ws.block_scaled for scale in scales_of_a_cache(n))
         ignored = sorted(n for n in files if n not in expected and (n.endswith(IGNORED_SUFFIXES) or n in not_needed))
         unexpected = [n for n in files if n not in expected and n not in ignored and scales.get(n) not in in_blocks and n not in beside_codes]
         # a head that the model ties to its embedding is not read even if the file stores a copy
