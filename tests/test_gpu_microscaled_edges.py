@@ -192,3 +192,12 @@ def test_short_products_of_every_kind_side_by_side():
                 outs.append((i, gemm.linear(inputs[m, k], w)))
         torch.cuda.synchronize()
         assert all(torch.equal(y, want[i]) for i, y in outs)
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-30, 1e30])
+def test_a_matrix_is_quantised_alike_on_the_host_and_on_the_device(size):
+    need_gpu()
+    w = torch.randn(5000, 3601, generator=torch.Generator().manual_seed(1)) * size
+    for made in (w, w.to(BF16)):
+        here, there = microscaled.quantize_matrix(made), microscaled.quantize_matrix(made.to(DEV)).to("cpu")
+        assert torch.equal(here.codes, there.codes) and torch.equal(here.scales.view(torch.uint8), there.scales.view(torch.uint8)) and here.factor == there.factor

@@ -5,7 +5,9 @@ import random
 import pytest
 import torch
 
+from microscaled_oracle import CODES, SCALES
 from torchinferno_b200.kernels import ops
+from torchinferno_b200.kernels.microscaled import quantize_matrix
 
 
 def room(rows, columns, features, experts=0, bits=4, codes=1):
@@ -115,3 +117,54 @@ def test_scales_of_a_cache_beside_other_tensors_are_not_known(tmp_path):
     save_file({**load_file(str(tmp_path / "model.safetensors")), **CACHE_SCALES}, str(tmp_path / "model.safetensors"))
     with pytest.raises(WeightError, match="unexpected"):
         load_weights(build_model(TINY_B, dtype=torch.bfloat16, device="cpu"), tmp_path)
+
+
+# ------------------------------------------------------------------------------------------------ matrices
+def check_nearest(matrix, made):
+    """Every scale and every code is the nearest one, of two as near the even one: compared by products that are exact in 64 bits."""
+    n, k = matrix.shape
+    w, f = matrix.double(), made.factor.double()
+    table = torch.tensor(SCALES, dtype=torch.float64)
+    runs = torch.nn.functional.pad(w.abs(), (0, -k % 16)).view(n, -1, 16).amax(2)
+    index = torch.searchsorted(table, made.scales.double())
+    assert torch.equal(table[index], made.scales.double())
+    even = index % 2 == 0
+    below, above = (table[(index - 1).clamp(min=0)] + table[index]) / 2 * 6 * f, (table[(index + 1).clamp(max=len(SCALES) - 1)] + table[index]) / 2 * 6 * f
+    assert ((index == 0) | (runs > below) | ((runs == below) & even)).all() and ((index == len(SCALES) - 1) | (runs < above) | ((runs == above) & even)).all()
+    halves = torch.stack([made.codes % 16, made.codes // 16], 2).view(n, -1)[:, :k].long()
+    code, codes = halves % 8, torch.tensor(CODES, dtype=torch.float64)
+    unit = made.scales.double()[:, torch.arange(k) // 16] * f
+    low, high = (codes[(code - 1).clamp(min=0)] + codes[code]) / 2 * unit, (codes[(code + 1).clamp(max=7)] + codes[code]) / 2 * unit
+    size, even = torch.where(unit == 0, 0.0, w.abs()), code % 2 == 0
+    assert ((code == 0) | (size > low) | ((size == low) & even)).all() and ((code == 7) | (size < high) | ((size == high) & even)).all()
+    assert torch.equal(halves > 7, (w < 0) & (code > 0)) and not (code[unit == 0]).any()
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_a_matrix_gets_the_nearest_scales_and_codes(seed):
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randn(1200, 1003, generator=g) * torch.randn(1200, 1, generator=g).exp()
+    check_nearest(w, quantize_matrix(w))
+    check_nearest(w.bfloat16(), quantize_matrix(w.bfloat16()))
+
+
+@pytest.mark.parametrize("largest", [2688.0, 1.0, 0.1, 3.7e-3, 2688 * 1.2345678e-5, 3e38, 1e-30])
+def test_numbers_of_a_matrix_beside_every_border(largest):
+    """For the factor that this largest number gives: numbers on and next to each border of codes, under each scale, and runs' largest ones beside the borders of scales."""
+    f = (torch.tensor(largest) / 2688.0).double()
+    rows = []
+    for s in SCALES[1::3] + [448.0]:
+        top, near = (6 * s * f).float(), []
+        for border in (0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0):
+            b = (border * s * f).float()
+            near += [torch.nextafter(b, torch.tensor(0.0)), b, torch.nextafter(b, torch.tensor(3e38))]
+        rows += [torch.stack([top] + near[:15]), torch.stack([top] + near[6:])]
+    for low, high in zip(SCALES[:-1], SCALES[1:]):
+        b = ((low + high) / 2 * 6 * f).float()
+        rows += [torch.cat([v[None], torch.zeros(15)]) for v in (torch.nextafter(b, torch.tensor(0.0)), b, torch.nextafter(b, torch.tensor(3e38)))]
+    rows.append(torch.cat([torch.tensor([largest]), torch.zeros(15)]))
+    w = torch.stack(rows).clamp(max=largest)
+    made = quantize_matrix(w)
+    assert made.factor == torch.tensor(largest) / 2688.0
+    check_nearest(w, made)
+    assert torch.equal(quantize_matrix(-w).scales.view(torch.uint8), made.scales.view(torch.uint8))

@@ -82,22 +82,38 @@ class MicroscaledMatrix:
         return (signed[halves.long()] * scales * self.factor.reshape(())).to(dtype)
 
 
+def _nearest_scales(v: torch.Tensor) -> torch.Tensor:
+    """The e4m3 numbers nearest to ``v`` (64 bits, none negative), ties to even, at most 448."""
+    steps = torch.tensor([2.0 ** (binade - 3) for binade in range(-6, 9)], dtype=v.dtype, device=v.device)
+    step = steps[(torch.frexp(v).exponent.long() - 1).clamp(-6, 8) + 6]
+    return (torch.round(v / step) * step).clamp(max=448.0).to(torch.float32).to(SCALE_DTYPE)
+
+
 def quantize_matrix(matrix: torch.Tensor) -> MicroscaledMatrix:
-    """The 4-bit form of ``matrix`` [N, K]: f = (its largest absolute value) / 2688, S = e4m3(a run's largest / (6 f)), codes the nearest ones."""
+    """The 4-bit form of ``matrix`` [N, K]: f = (its largest absolute value) / 2688, S = e4m3(a run's largest / (6 f)), codes the nearest ones; ties to even.
+
+    Quotients are taken in 64 bits, of products that are exact there: a quotient that is not on a border, a number of few bits, is off it by 2^-32 of it or more."""
     if matrix.dim() != 2 or 0 in matrix.shape:
         raise ValueError(f"quantize_matrix takes a non-empty matrix, got {tuple(matrix.shape)}")
     n, k = matrix.shape
-    runs = torch.nn.functional.pad(matrix.to(torch.float32), (0, -k % RUN)).view(n, -1, RUN)
-    factor = (runs.abs().amax() / LARGEST).clamp(min=torch.finfo(torch.float32).tiny)
-    scales = (runs.abs().amax(2) / 6.0 / factor).clamp(max=448.0).to(SCALE_DTYPE)
-    wide = scales.to(torch.float32)[..., None]
-    v = torch.where(wide == 0, 0.0, runs / torch.where(wide == 0, 1.0, wide) / factor).view(n, -1)
-    size = v.abs()
-    codes = torch.zeros_like(v, dtype=torch.uint8)
-    for i, border in enumerate(BORDERS):
-        codes += size >= border if i % 2 else size > border
-    codes += 8 * ((v < 0) & (codes > 0)).to(torch.uint8)
-    return MicroscaledMatrix((codes[:, 0::2] | (codes[:, 1::2] << 4))[:, :_count(k, 2)].contiguous(), scales.contiguous(), factor, k)
+    largest = matrix.abs().amax().to(torch.float32)
+    factor = (largest / torch.full_like(largest, LARGEST)).clamp(min=torch.finfo(torch.float32).tiny)      # (a number of Python's would be a product with its inverse on a GPU)
+    codes = torch.empty((n, _count(k, 2)), dtype=torch.uint8, device=matrix.device)
+    scales = torch.empty((n, _count(k, RUN)), dtype=SCALE_DTYPE, device=matrix.device)
+    wide_factor, rows = factor.to(torch.float64), max(1, (1 << 24) // k)
+    for first in range(0, n, rows):
+        at = slice(first, first + rows)
+        runs = torch.nn.functional.pad(matrix[at].to(torch.float64), (0, -k % RUN)).view(-1, scales.shape[1], RUN)
+        scales[at] = _nearest_scales(runs.abs().amax(2) / (6.0 * wide_factor))
+        wide = scales[at].to(torch.float64)[..., None]
+        size = torch.where(wide == 0, 0.0, runs.abs() / torch.where(wide == 0, 1.0, wide * wide_factor))
+        part = torch.zeros(runs.shape, dtype=torch.uint8, device=matrix.device)
+        for i, border in enumerate(BORDERS):
+            part += size >= border if i % 2 else size > border
+        part += 8 * ((runs < 0) & (part > 0)).to(torch.uint8)
+        part = part.view(len(part), -1)
+        codes[at] = (part[:, 0::2] | (part[:, 1::2] << 4))[:, :codes.shape[1]]
+    return MicroscaledMatrix(codes, scales, factor, k)
 
 
 # ------------------------------------------------------------------------------------------------ rows
