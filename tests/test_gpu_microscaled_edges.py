@@ -4,7 +4,7 @@ import torch
 
 from gpu_common import need_gpu
 from microscaled_oracle import matrix64, random_matrix, rows64
-from test_gpu_microscaled import check, rows, same, same_rows
+from test_gpu_microscaled import act64, check, rows, same, same_rows
 from torchinferno_b200.kernels import block_scaled, gemm, microscaled, ops
 from torchinferno_b200.kernels.microscaled import MicroscaledExperts, MicroscaledMatrix, MicroscaledWeight, quantize_rows
 
@@ -201,3 +201,42 @@ def test_a_matrix_is_quantised_alike_on_the_host_and_on_the_device(size):
     for made in (w, w.to(BF16)):
         here, there = microscaled.quantize_matrix(made), microscaled.quantize_matrix(made.to(DEV)).to("cpu")
         assert torch.equal(here.codes, there.codes) and torch.equal(here.scales.view(torch.uint8), there.scales.view(torch.uint8)) and here.factor == there.factor
+
+
+# ------------------------------------------------------------------------------------------------ pairs' factors and activations
+def check_scaled(y, x, matrices, act, scale):
+    """As check, of sums that are multiplied by a factor each row has ahead of the activation: one more product, 2^-24 of a sum."""
+    half = torch.finfo(y.dtype).eps / 2
+    wide, k, scale = rows64(x), x.shape[1], scale.double()[:, None]
+    ws = [matrix64(m) for m in matrices]
+    sums = [wide @ w.t() * scale for w in ws]
+    slack = [wide.abs() @ w.abs().t() * scale.abs() * (k + 5) * 2.0 ** -24 for w in ws]
+    want = act64(act, sums)
+    bound = {"none": lambda: slack[0], "silu": lambda: 1.13 * slack[0], "gelu": lambda: 1.13 * slack[0], "relu2": lambda: 2 * sums[0].abs() * slack[0] + slack[0] ** 2,
+             "swiglu": lambda: 1.13 * slack[0] * (sums[1].abs() + slack[1]) + sums[0].abs() * slack[1], "glu_clamp": lambda: 1.7 * slack[0] * 8.0 + 7.0 * slack[1]}[act]()
+    bound = bound + want.abs() * (half + 2.0 ** -20) + (0 if act == "none" else 2.0 ** -20 * sums[0].abs().clamp(max=1.0))
+    bad = (y.double() - want).abs() > bound
+    assert not bad.any(), (int(bad.sum()), float(((y.double() - want).abs() / bound).max()))
+
+
+@pytest.mark.parametrize("act", ["none", "relu2", "silu", "gelu", "swiglu", "glu_clamp"])
+@pytest.mark.parametrize("counts, top", [([1, 0, 3, 0, 4], 2), ([30, 5, 0, 29, 28, 1, 27], 4), ([700, 0, 901, 3], 4), ([257, 0, 256, 1, 600, 130], 2)])
+def test_pairs_factors_multiply_the_sums_ahead_of_every_activation(counts, top, act):
+    """Factors of both signs and of sizes from 2^-8 to 2^3, the pair's and not the row's."""
+    need_gpu()
+    k, n, experts, pairs = 520, 260, len(counts), sum(counts)
+    gates = [random_matrix(n, k, 7 * e, DEV, 1e-4 * (1 + e % 3)) for e in range(experts)]
+    ups = [random_matrix(n, k, 7 * e + 1, DEV, 1e-4) for e in range(experts)] if act in ops.MOE_GATED else None
+    weight = MicroscaledExperts(gates, ups)
+    offsets = torch.tensor([0] + counts).cumsum(0).to(torch.int32).to(DEV)
+    g = torch.Generator().manual_seed(pairs)
+    order = torch.randperm(pairs, generator=g).to(torch.int32).to(DEV)
+    scale = (torch.randn(pairs, generator=g).sign() * 2.0 ** (11 * torch.rand(pairs, generator=g) - 8)).to(DEV)
+    for by_pair, out in ((True, F32), (False, BF16)):
+        x = rows(pairs // top if by_pair else pairs, k, pairs, spread=0.5)
+        y = torch.empty(pairs, n, dtype=out, device=DEV)
+        ops.moe_expert_product(x, weight, y, offsets, order, top, x_by_pair=by_pair, act=act, limit=7.0, alpha=1.702, row_scale=scale)
+        for e in range(experts):
+            at = slice(int(offsets[e]), int(offsets[e + 1]))
+            if at.start < at.stop:
+                check_scaled(y[at], x[order[at].long() // top] if by_pair else x[at], [gates[e]] + ([ups[e]] if ups else []), act, scale[order[at].long()])
