@@ -240,3 +240,42 @@ def test_pairs_factors_multiply_the_sums_ahead_of_every_activation(counts, top, 
             at = slice(int(offsets[e]), int(offsets[e + 1]))
             if at.start < at.stop:
                 check_scaled(y[at], x[order[at].long() // top] if by_pair else x[at], [gates[e]] + ([ups[e]] if ups else []), act, scale[order[at].long()])
+
+
+# ------------------------------------------------------------------------------------------------ operands of a norm that share memory
+def test_operands_of_a_norm_that_overlap_are_refused():
+    """Blocks write rows of what others still read: refused, and nothing is written.  Side by side in one piece of memory, or the same rows, is fine."""
+    need_gpu()
+    m, k = 40, 520
+    weight = torch.ones(k, device=DEV)
+    for dtype in (F32, BF16):
+        size = m * k * (4 if dtype == F32 else 2)
+        room = torch.zeros(8 * m * k, dtype=torch.float32, device=DEV)
+        pieces = room.view(torch.uint8)
+        at = lambda first, t, shape=(m, k): pieces[first:first + shape[0] * shape[1] * (2 if t == BF16 else 4)].view(t).view(shape)      # noqa: E731
+        residual = at(0, F32)
+        residual.copy_(rows(m, k, 1, F32, spread=0.2))
+        delta = at(m * k * 4, dtype)
+        delta.copy_(rows(m, k, 2, dtype, spread=0.2))
+        kept = room.clone()
+        end = m * k * 4 + size
+        for form in (microscaled, block_scaled):
+            for bad in (dict(out=at(m * k * 4 - 1024, dtype)), dict(out=at(end - 1024, dtype)), dict(out=at(512, dtype)), dict(out=at(0, dtype)), dict(out=at(m * k * 4, dtype)),
+                        dict(new_residual=at(k * 4, F32)), dict(new_residual=at(end - 16, F32)), dict(new_residual=at(end, F32), out=at(end + 64, dtype)),
+                        *([dict(new_residual=at(m * k * 4, F32))] if dtype == BF16 else [])):
+                with pytest.raises(ops.KernelError, match="memory"):
+                    form.add_rmsnorm(delta, residual, weight, 1e-5, **bad)
+            torch.cuda.synchronize()
+            assert torch.equal(room, kept)
+            want, new = residual.clone(), residual.float() + delta.float()
+            normed = torch.empty_like(delta)
+            ops.add_rmsnorm(delta, want, weight, 1e-5, normed)
+            made = form.add_rmsnorm(delta, residual, weight, 1e-5, new_residual=at(end, F32), out=at(end + m * k * 4, dtype))
+            assert torch.equal(at(end, F32), new) and torch.equal(at(end + m * k * 4, dtype), normed) and torch.equal(residual, kept[:m * k].view(m, k))
+            same_place = form.add_rmsnorm(delta, residual, weight, 1e-5, new_residual=residual)
+            assert torch.equal(residual, new) and torch.equal(same_place.widened(F32), made.widened(F32))
+            residual.copy_(kept[:m * k].view(m, k))
+            if dtype == F32:      # (the sum takes the place of delta)
+                form.add_rmsnorm(delta, residual, weight, 1e-5, new_residual=delta)
+                assert torch.equal(delta, new)
+            room.copy_(kept)

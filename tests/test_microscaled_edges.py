@@ -168,3 +168,13 @@ def test_numbers_of_a_matrix_beside_every_border(largest):
     assert made.factor == torch.tensor(largest) / 2688.0
     check_nearest(w, made)
     assert torch.equal(quantize_matrix(-w).scales.view(torch.uint8), made.scales.view(torch.uint8))
+
+
+def test_operands_of_a_norm_that_overlap_are_refused():
+    """By their addresses alone: 4 rows of 64 columns, 1,024 bytes in 32 bits and 512 in bf16."""
+    lib, at = ops.lib(), 1 << 20      # (an address that nothing reads)
+    norm = dict(delta=at + 4096, residual=at, sum=at + 8192, rows=0, weight=at + 12288, out=at + 16384, bytes=0, codes=at + 65536, scales=at + 131072, factors=at + 196608, lds=0, n_out=4,
+                n_rows=4, hidden=64, eps=1e-5, dtype=1, stream=0)
+    for wrong in (dict(sum=at + 16), dict(sum=at - 1008), dict(sum=at + 4096), dict(sum=at + 4096 - 1008, dtype=0), dict(sum=at + 12288 + 240), dict(out=at + 1008), dict(out=at - 496), dict(out=at),
+                  dict(out=at + 4096 + 496), dict(out=at + 8192 + 512), dict(out=at + 12288 - 496), dict(sum=at, delta=at + 256, out=0)):
+        assert lib.tib_quantized_norm(*{**norm, **wrong}.values()) == -8, wrong

@@ -33,6 +33,7 @@ enum TibError : int {
   TIB_E_ARG = -5,        // null pointer or inconsistent arguments
   TIB_E_WAIT = -6,       // a bounded device-side wait ran out
   TIB_E_SCRATCH = -7,    // needs more scratch than the library's built-in array holds
+  TIB_E_OVERLAP = -8,    // operands share memory that they may not share
 };
 
 // The fixed-size record every live request has on the device, one row of int32 words per request slot.

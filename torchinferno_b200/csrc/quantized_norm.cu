@@ -359,9 +359,9 @@ static int qn_allow_smem(void (*kern)(const QnArgs, int)) {
 
 using namespace tib;
 
-// residual [n_rows, hidden] fp32, delta [n_rows, hidden] in dtype or null; sum [n_rows, hidden] fp32 takes residual + delta (it may be residual itself; null: it is not kept, and
+// residual [n_rows, hidden] fp32, delta [n_rows, hidden] in dtype or null; sum [n_rows, hidden] fp32 takes residual + delta (it may be residual itself, or an fp32 delta; null: it is not kept, and
 // with `rows`, indices of the n_out rows to norm, it has to be null).  bytes 0: codes, scales, factors as tib_microscaled_rows leaves them, 1: codes
-// [n_out, runs * 128] and factors = scales [runs, lds] as tib_quantize_rows does.  out: the normed rows in dtype, or null.
+// [n_out, runs * 128] and factors = scales [runs, lds] as tib_quantize_rows does.  out: the normed rows in dtype, or null, memory of its own.
 TIB_API int tib_quantized_norm(const void* delta, const float* residual, float* sum, const int* rows, const float* weight, void* out, int bytes, void* codes,
                                void* scales, float* factors, int64_t lds, int n_out, int n_rows, int hidden, float eps, int dtype, cudaStream_t stream) {
   if (n_out == 0) return TIB_OK;
@@ -369,6 +369,13 @@ TIB_API int tib_quantized_norm(const void* delta, const float* residual, float* 
   if (dtype != TIB_BF16 && dtype != TIB_F32) return TIB_E_DTYPE;
   if (bytes && lds < n_out) return TIB_E_SIZE;
   if (((uintptr_t)codes | (uintptr_t)scales) & 15) return TIB_E_ALIGN;
+  // (a block writes its row's sum and normed form while others read theirs)
+  const int64_t size = dtype == TIB_BF16 ? 2 : 4, numbers = (int64_t)n_rows * hidden, normed = (int64_t)n_out * hidden;
+  auto share = [](const void* p, int64_t p_bytes, const void* q, int64_t q_bytes) { return p && q && (const char*)p < (const char*)q + q_bytes && (const char*)q < (const char*)p + p_bytes; };
+  if ((sum != residual && share(sum, 4 * numbers, residual, 4 * numbers)) || (!(sum == delta && size == 4) && share(sum, 4 * numbers, delta, size * numbers)) ||
+      share(sum, 4 * numbers, weight, (int64_t)4 * hidden) || share(out, size * normed, residual, 4 * numbers) || share(out, size * normed, delta, size * numbers) ||
+      share(out, size * normed, sum, 4 * numbers) || share(out, size * normed, weight, (int64_t)4 * hidden))
+    return TIB_E_OVERLAP;
   const QnArgs a{delta, residual, sum, rows, weight, out, (unsigned char*)codes, (unsigned char*)scales, factors, lds, hidden, eps, ms_groups(n_out, 0), n_rows};
   if (dtype == TIB_BF16 && hidden % 8 == 0 && hidden <= 8192 &&
       (((uintptr_t)residual | (uintptr_t)sum | (uintptr_t)weight | (uintptr_t)out | (uintptr_t)delta) & 15) == 0) {

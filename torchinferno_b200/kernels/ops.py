@@ -26,6 +26,7 @@ _ERRORS = {
     -5: "null pointer or inconsistent arguments",
     -6: "the device-side wait limit was reached (kernel gave up)",
     -7: "needs more scratch than the library's built-in array holds",
+    -8: "operands share memory that they may not share",
 }
 
 
@@ -1402,7 +1403,7 @@ def quantized_norm_type(delta: torch.Tensor | None, dtype: torch.dtype | None) -
 def quantized_norm(delta: torch.Tensor | None, residual: torch.Tensor, weight: torch.Tensor, eps: float, dtype: torch.dtype, rows: torch.Tensor | None,
                    out: torch.Tensor | None, new_residual: torch.Tensor | None, in_bytes: bool, count: int, codes: int, scales: int, factors: int, lds: int) -> None:
     """:func:`add_rmsnorm` whose ``count`` rows go, as codes and scales, to these addresses: ``in_bytes`` as :func:`quantize_rows` leaves them (``factors``: the scales), else
-    as :func:`microscaled_rows` does."""
+    as :func:`microscaled_rows` does.  ``out`` is memory of its own; ``new_residual``, too, or the residual's (or a float32 delta's), row for row."""
     shape, device = residual.shape, residual.get_device()
     if len(shape) != 2 or not shape[1] or weight.numel() != shape[1]:
         raise KernelError(f"add_rmsnorm: residual {tuple(shape)} / weight {tuple(weight.shape)} do not fit")
@@ -1417,8 +1418,6 @@ def quantized_norm(delta: torch.Tensor | None, residual: torch.Tensor, weight: t
             raise KernelError("add_rmsnorm: with rows the residual is left as it is")
     if out is not None:
         _need_on(out, "out", dtype, (count, shape[1]), device)
-        if count and out.data_ptr() in [t.data_ptr() for t in (delta, residual, new_residual) if t is not None]:
-            raise KernelError("add_rmsnorm: out is not the memory of another operand (a row is read again after its normed form is written)")
     kept = residual if delta is not None and rows is None else None
     if new_residual is not None:
         kept = new_residual
