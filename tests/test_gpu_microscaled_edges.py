@@ -279,3 +279,31 @@ def test_operands_of_a_norm_that_overlap_are_refused():
                 form.add_rmsnorm(delta, residual, weight, 1e-5, new_residual=delta)
                 assert torch.equal(delta, new)
             room.copy_(kept)
+
+
+@pytest.mark.parametrize("m", [1, 8, 30, 200])
+def test_far_factors_of_gated_weights_experts_and_views(m):
+    """Matrices with far factors beside others: every output of each."""
+    need_gpu()
+    k, size = 520, 2.0 ** -60
+    x = (rows(m, k, 5, F32, spread=0.1).clamp(-1, 1).double() * size).to(F32)
+    matrices = [random_matrix(128, k, 1, DEV, 1e15), random_matrix(260, k, 2, DEV, 1e36), random_matrix(70, k, 3, DEV, 2e-20), random_matrix(130, k, 4, DEV, 1e-45)]
+    weight = MicroscaledWeight(*matrices)
+    y, first = gemm.linear(x, weight), 0
+    for matrix in matrices:
+        check_numbers(y[:, first:first + matrix.shape[0]], *sums_of(x, matrix))
+        first += matrix.shape[0]
+    assert torch.equal(gemm.linear(x, weight.rows(128, 458)), y[:, 128:458])
+    word = torch.zeros(1, dtype=torch.int32, device=DEV)
+    assert torch.equal(weight.product(quantize_rows(x), error_word=word), y) and int(word) == 0
+    gate, up = random_matrix(200, k, 7, DEV, 2.0 ** 55), random_matrix(200, k, 8, DEV, 2.0 ** 80)      # (sums about 1 and 2^25)
+    x = x * 2.0 ** -18
+    check(gemm.linear_swiglu(x, MicroscaledWeight(gate, up, epilogue="swiglu")), x, [gate, up], "swiglu")
+    experts = MicroscaledExperts([matrices[1], random_matrix(260, k, 9, DEV, 1e18), random_matrix(260, k, 10, DEV, 1e-38)])
+    offsets = torch.tensor([0, m // 3, m // 2, m], dtype=torch.int32, device=DEV)
+    out, order = torch.empty(m, 260, device=DEV), torch.arange(m, dtype=torch.int32, device=DEV)
+    ops.moe_expert_product(x, experts, out, offsets, order, 1, x_by_pair=False)
+    for e, matrix in enumerate([matrices[1], random_matrix(260, k, 9, DEV, 1e18), random_matrix(260, k, 10, DEV, 1e-38)]):
+        at = slice(int(offsets[e]), int(offsets[e + 1]))
+        if at.start < at.stop:
+            check_numbers(out[at], *sums_of(x[at], matrix))

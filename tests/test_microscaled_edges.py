@@ -5,9 +5,9 @@ import random
 import pytest
 import torch
 
-from microscaled_oracle import CODES, SCALES
+from microscaled_oracle import CODES, SCALES, random_matrix
 from torchinferno_b200.kernels import ops
-from torchinferno_b200.kernels.microscaled import quantize_matrix
+from torchinferno_b200.kernels.microscaled import MicroscaledExperts, MicroscaledMatrix, MicroscaledWeight, quantize_matrix
 
 
 def room(rows, columns, features, experts=0, bits=4, codes=1):
@@ -45,7 +45,7 @@ def test_blocks_that_fit_an_sm_together_find_their_columns():
             assert columns in (32, 64, 128, 256, 512) and smem <= 227 * 1024, (m, k, n, e, bits)
             assert smem + 1024 >= (columns - (28 if columns >= 256 else 0)) * 228 * 1024 // 512, (m, k, n, e, bits, columns, smem)
             assert e or shared(m, k, n, bits, codes) == 1 or smem + 1024 > 30 * 1024      # (in clusters: beside 512 columns and 199 KB)
-    assert {(4, 64), (4, 128), (4, 256), (4, 512), (8, 64), (8, 128), (8, 256), (8, 512)} <= seen and least > 56 * 228 * 1024 // 512
+    assert {(4, 128), (4, 256), (4, 512), (8, 64), (8, 128), (8, 256), (8, 512)} <= seen and least > 56 * 228 * 1024 // 512
 
 
 @pytest.mark.parametrize("sizes", [(0, 8, 8, 0), (8, 0, 8, 0), (8, 8, 0, 0), (8, 8, 8, -1)])
@@ -178,3 +178,37 @@ def test_operands_of_a_norm_that_overlap_are_refused():
     for wrong in (dict(sum=at + 16), dict(sum=at - 1008), dict(sum=at + 4096), dict(sum=at + 4096 - 1008, dtype=0), dict(sum=at + 12288 + 240), dict(out=at + 1008), dict(out=at - 496), dict(out=at),
                   dict(out=at + 4096 + 496), dict(out=at + 8192 + 512), dict(out=at + 12288 - 496), dict(sum=at, delta=at + 256, out=0)):
         assert lib.tib_quantized_norm(*{**norm, **wrong}.values()) == -8, wrong
+
+
+# ------------------------------------------------------------------------------------------------ factors that are far from 1
+def with_factor(n, factor, zeros=False):
+    matrix = random_matrix(n, 32, n, factor=1.0)
+    return MicroscaledMatrix(matrix.codes, torch.zeros_like(matrix.scales) if zeros else matrix.scales, torch.tensor(factor))
+
+
+def test_which_weights_have_far_factors():
+    """Those whose factor is outside 2^-100 .. 2^70 where it matters: not a matrix of zeros', whatever its factor."""
+    tiny, least, most = 1e-38, 2.0 ** -100, 2.0 ** 70
+    for factors, far in (((1e-3,), False), ((least,), False), ((most,), False), ((least * 0.999,), True), ((most * 1.001,), True), ((0.0,), False), ((-1e25,), True), ((1e-3, tiny), True),
+                         ((tiny, 1e-3), True), ((3e38,), True)):
+        weight = MicroscaledWeight(*(with_factor(140, f) for f in factors))
+        assert weight.tiles.far is far and weight.tiles.numbers[3] == 2 * far and weight.rows(128, 140).tiles.numbers[3] == 2 * far
+        gated = MicroscaledWeight(with_factor(6, 1e-3), with_factor(6, factors[-1]), epilogue="swiglu")
+        assert gated.tiles.numbers[3] == 1 + 2 * (not least <= abs(factors[-1]) <= most and factors[-1] != 0)
+    assert not MicroscaledWeight(with_factor(3, tiny, zeros=True), with_factor(5, 1.0)).tiles.far and not MicroscaledWeight(quantize_matrix(torch.zeros(4, 32))).tiles.far
+    experts = [with_factor(4, 1e-3) for _ in range(300)]
+    assert not MicroscaledExperts(experts).tiles.far
+    experts[200] = with_factor(4, tiny)
+    with pytest.raises(ValueError, match="more than 223 experts"):
+        MicroscaledExperts(experts)
+    assert MicroscaledExperts(experts[78:]).tiles.far and not MicroscaledExperts(experts[:200] + [with_factor(4, tiny, zeros=True)] + experts[201:]).tiles.far
+
+
+def test_products_with_far_factors_are_told_so():
+    """2 of `pairs`: no product that quantises its rows itself, and no more experts than pairs of SMs take."""
+    lib, at = ops.lib(), 1 << 20
+    product = dict(w=at, w_scales=at, w_factors=at, pairs=2, N=8, K=64, experts=1, x=at, x_dtype=1, ldx=64, x_rows=4, codes=0, scales=0, factors=0, make=1, y=at + 65536, y_dtype=1, ldy=8,
+                   M=4, offsets=0, order=0, top=1, x_by_pair=0, act=0, limit=0.0, alpha=0.0, row_scale=0, error_word=0, stream=0)
+    for wrong, status in ((dict(), -5), (dict(codes=at, scales=at, factors=at, make=0, act=4), -2), (dict(codes=at, scales=at, factors=at, make=0, pairs=3, N=7), -2),
+                          (dict(codes=at, scales=at, factors=at, make=0, offsets=at, order=at, experts=224), -2)):
+        assert lib.tib_microscaled_product(*{**product, **wrong}.values()) == status, wrong

@@ -170,7 +170,8 @@ TIB_API int tib_microscaled_widen(const void* codes, const void* scales, const f
 }
 
 // A product as its callers see it: y [M, N] (or [M, N / 2] of a gated activation) in y_dtype, row stride ldy.  codes, scales, factors: where the quantised rows
-// are, or (`make`) are put first, from rows x [x_rows, K].  w: codes, scales and factors [experts, N] of the matrices (`pairs`: of (gate, up) row pairs).
+// are, or (`make`) are put first, from rows x [x_rows, K].  w: codes, scales and factors [experts, N] of the matrices (`pairs`: 1 of (gate, up) row pairs; 2 more where a factor that
+// matters is outside 2^-100 .. 2^70: these run on pairs of SMs).
 // offsets [experts + 1], order [M], top, x_by_pair: rows sorted by expert as tib_moe_expert_product takes them; offsets null: one matrix for all rows.
 TIB_API int tib_microscaled_product(const void* w, const void* w_scales, const float* w_factors, int pairs, int N, int K, int experts, const void* x, int x_dtype,
                                     int64_t ldx, int x_rows, void* codes, void* scales, float* factors, int make, void* y, int y_dtype, int64_t ldy, int M,
@@ -180,11 +181,12 @@ TIB_API int tib_microscaled_product(const void* w, const void* w_scales, const f
   const bool made_inside = make && !codes;
   if ((!made_inside && (!codes || !scales || !factors)) || !w || !w_scales || !w_factors || !y || M < 0 || N < 0 || K < 1 || experts < 1 || top < 1) return TIB_E_ARG;
   if ((offsets && !order) || (row_scale && !order)) return TIB_E_ARG;
-  if (act < MOE_ACT_NONE || act > MOE_ACT_GELU || (moe_act_gated(act) && !pairs) || (pairs && N % 2)) return TIB_E_SIZE;
+  if (act < MOE_ACT_NONE || act > MOE_ACT_GELU || (moe_act_gated(act) && !(pairs & 1)) || ((pairs & 1) && N % 2)) return TIB_E_SIZE;
+  const bool far = pairs & 2;
   if (y_dtype != TIB_BF16 && y_dtype != TIB_F32) return TIB_E_DTYPE;
   if (((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)w | (uintptr_t)w_scales) & 15) return TIB_E_ALIGN;
   if (made_inside) {      // (every block reads the rows while others write y)
-    if (!x || offsets || M > x_rows || !ms_makes_rows(M, N, K)) return TIB_E_ARG;
+    if (!x || offsets || far || M > x_rows || !ms_makes_rows(M, N, K)) return TIB_E_ARG;
     if (x_dtype != TIB_BF16) return TIB_E_DTYPE;
     if (((uintptr_t)x & 15) || ldx % 8) return TIB_E_ALIGN;
     const char *from = (const char*)x, *to = (const char*)y;
@@ -197,10 +199,10 @@ TIB_API int tib_microscaled_product(const void* w, const void* w_scales, const f
   MsArgs a;
   a.x = MsRows{(const unsigned char*)codes, (const unsigned char*)scales, factors, ms_groups(M, offsets ? experts : 0)};
   a.w = (const unsigned char*)w; a.w_scales = (const unsigned char*)w_scales; a.w_factors = w_factors;
-  a.M = M; a.N = N; a.steps = ms_steps(K); a.stages = a.tmem_cols = a.scale_cols = 0; a.offsets = offsets; a.order = order; a.experts = experts;
+  a.M = M; a.N = N; a.steps = ms_steps(K); a.stages = a.tmem_cols = 0; a.offsets = offsets; a.order = order; a.experts = experts;
   a.limit = limit; a.alpha = alpha; a.row_scale = row_scale; a.error_word = error_word;
   a.made = made_inside ? (const __nv_bfloat16*)x : nullptr; a.ld_made = ldx; a.K = K;
-  if (!made_inside && ms_on_pairs_of_sms(M, N, a.steps, offsets ? experts : 0)) return ms_product_2cta(a, act, y, y_dtype, ldy, stream);
+  if (!made_inside && (far || ms_on_pairs_of_sms(M, N, a.steps, offsets ? experts : 0))) return ms_product_2cta(a, act, y, y_dtype, ldy, stream);
   return ms_product_tcgen05(a, act, y, y_dtype, ldy, stream);
 }
 

@@ -160,7 +160,7 @@ struct MsArgs {
   const unsigned char* w;          // codes of the matrices
   const unsigned char* w_scales;
   const float* w_factors;          // [experts, N]
-  int M, N, steps, stages, tmem_cols, scale_cols;
+  int M, N, steps, stages, tmem_cols;
   const int* offsets;              // [experts + 1] of rows sorted by expert, or null: one matrix
   const int* order;
   int experts;
@@ -172,11 +172,25 @@ struct MsArgs {
   int K;
 };
 
-// What a row's sums are multiplied by ahead of the matrix's factor f and behind it: y = sum * f * r * q, r the row's power of two (or NaN) and q its pair's factor (1 where it has
-// none).  A sum is 0 or from 2^-20 (two codes of 1/2, two scales of 2^-9) to under 2^56 in size.  With q = m 2^e, 1 <= m < 2, what comes first is the power of two 2^e r, kept
-// within 2^-106 .. 2^70, where it leaves every sum a normal number, and exact; what it was kept from comes last, with m.  So if the product with f is too large, so is y
-// (what is left is at least 1), and if that is too small to be a normal number, y is, too (what is left is less than 2): whatever f and r are, and q from 2^-60 to 2^60 in
-// size or 0, nothing leaves the range of 32 bits but what the output itself does.
+// An output is sum * f * r * q: the matrix's factor f, the row's power of two r (or NaN) and its pair's factor q (1 where it has none).  A sum is 0 or from 2^-20 (two codes
+// of 1/2, two scales of 2^-9) to under 2^56 in size.  The kernels take the products in an order in which nothing leaves the range of 32 bits but what the output itself does,
+// for q from 2^-50 to 2^50 in size or 0 and
+//   f from 2^-100 to 2^70 (or 0), which leaves every sum a normal number: f first, then what ms_row_scales gives.  (In the fewest steps: microscaled_tcgen05.cu.  With what
+//   follows in their place 8 rows 1,024 -> 1,024 took 4.2 us for 3.95, with a branch for other factors as much.)
+//   any f: what ms_row_factors gives, ahead of f and behind it (microscaled_2cta.cu, where it costs nothing; matrices with other factors run there whatever their rows are).
+// r q is a power of two more or less where it is a normal number, and comes after f as one.  Where it is too small, or too large, so is q alone, and the product with r
+// alone leaves the range only where the one with both does.
+__device__ __forceinline__ float2 ms_row_scales(float r, float q) {
+  const float both = r * q;
+  return (fabsf(both) >= 0x1p-126f && fabsf(both) < INFINITY) || q == 0.f ? make_float2(both, 1.f) : make_float2(r, q);
+}
+// With q = m 2^e, 1 <= m < 2, what comes ahead of f is the power of two 2^e r, kept within 2^-106 .. 2^70, where it leaves every sum a normal number, and exact; what it was kept
+// from comes behind f, with m.  So if the product with f is too large, so is the output (what is left is at least 1), and if that is too small to be a normal number, the
+// output is, too (what is left is less than 2).
+__device__ __forceinline__ float2 ms_row_factors(float r) {      // (q = 1; a NaN is behind)
+  const float first = fminf(fmaxf(r, 0x1p-106f), 0x1p70f);
+  return make_float2(first, first == r ? 1.f : r * (r > 1.f ? 0x1p-70f : 0x1p106f));
+}
 __device__ __forceinline__ float2 ms_row_factors(float r, float q) {
   if (!(r < INFINITY && fabsf(q) < INFINITY) || q == 0.f) return make_float2(q == 0.f ? 0.f : 1.f, r * q);
   int e = (int)(__float_as_uint(r) >> 23) - 2 * 127;
@@ -186,8 +200,6 @@ __device__ __forceinline__ float2 ms_row_factors(float r, float q) {
   const int first = min(max(e, -106), 70), last = min(max(e - first, -126), 127);
   return make_float2(__uint_as_float((uint32_t)(first + 127) << 23), __uint_as_float((bits & 0x807fffffu) | 0x3f800000u) * __uint_as_float((uint32_t)(last + 127) << 23));
 }
-// An output from its sum: see ms_row_factors.
-__device__ __forceinline__ float ms_scaled(float sum, float w_factor, float2 row) { return sum * row.x * w_factor * row.y; }
 
 // Products of rows that are there as codes (microscaled_tcgen05.cu, microscaled_2cta.cu), with arguments that tib_microscaled_product has checked.
 bool ms_on_pairs_of_sms(int M, int N, int steps, int experts);

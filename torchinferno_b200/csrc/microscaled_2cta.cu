@@ -138,7 +138,7 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
       const int in_tile = (int)rank * 128 + quarter * 32 + lane, row = m.first + in_tile, last = m.first + m.rows;      // (rows from `last` on are not stored)
       const int col0 = m.n_tile * 256 + half * 128;
       tile_factors[acc_phase * 256 + et] = w_factor;
-      const float2 of_row = ms_row_factors(x_factor, pair_factor);
+      const float2 of_row = a.row_scale ? ms_row_factors(x_factor, pair_factor) : ms_row_factors(x_factor);
       const f32x2 ahead2 = f2_pack(of_row.x, of_row.x), behind2 = f2_pack(of_row.y, of_row.y);
       if (t + pairs < num_tiles) ask(next = tile_of(t + pairs));
       asm volatile("bar.sync 1, 256;\n" ::: "memory");      // (the last tile but one is finished: its factors have been read)
@@ -160,7 +160,7 @@ microscaled_2cta_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
       f32x2 sum[64];
       const ulonglong2* factors2 = reinterpret_cast<const ulonglong2*>(tile_factors + acc_phase * 256 + half * 128);
 #pragma unroll
-      for (int c = 0; c < 64; c += 2) {      // (see ms_scaled)
+      for (int c = 0; c < 64; c += 2) {      // (by the row: see ms_row_factors)
         const ulonglong2 f = factors2[c >> 1];
         sum[c] = f2_mul(f2_mul(f2_pack(__uint_as_float(v[c >> 4][2 * c & 31]), __uint_as_float(v[c >> 4][(2 * c & 31) + 1])), ahead2), f.x);
         sum[c + 1] = f2_mul(f2_mul(f2_pack(__uint_as_float(v[c >> 4][(2 * c & 31) + 2]), __uint_as_float(v[c >> 4][(2 * c & 31) + 3])), ahead2), f.y);
@@ -389,6 +389,7 @@ bool tib::ms_on_pairs_of_sms(int M, int N, int steps, int experts) {
 }
 
 int tib::ms_product_2cta(const MsArgs& a, int act, void* out, int out_dtype, int64_t ldo, cudaStream_t stream) {
+  if (a.offsets && a.experts > kM2MaxExperts) return TIB_E_SIZE;
   const int64_t w_steps = (int64_t)a.experts * ceil_div(a.N, 128) * a.steps, x_tiles = ceil_div(a.M, 128) + (a.offsets ? a.experts : 0);
   if (w_steps > (0x7fffffff >> 4) || (int64_t)a.x.groups * a.steps > 0x7fffffff || x_tiles * a.steps > (0x7fffffff >> 2)) return TIB_E_SIZE;
   CUtensorMap maps[4];

@@ -14,7 +14,8 @@
 // What bounds it, at few rows: memory.  8 rows 4,096 -> 28,672: 12.3 us for 66 MB (5.4 TB/s, 84 % of the measured copy bandwidth; without the copies 7.1); 14,336 -> 4,096 9.2 us
 // for 33 MB, 4,096 -> 4,096 5.1 us for 9.4 MB, of which some 3.5 are the start, the exchange and the end.  With the kernel that makes the rows' codes ahead of it, whose time
 // the first copies of weights fill, 14.5, 10.3 and 6.4 us.  In tiles of 128 rows the finishing of 128 x 128 outputs: 128 rows 4,096 -> 28,672 16.8 us with eight warps that
-// have their next columns on their way, 22.5 with four that wait for each eight of them, 12.8 without.  Every wait is bounded and reports in error_word.
+// have their next columns on their way, 22.5 with four that wait for each eight of them, 12.8 without; and their number: 224 tiles are a round of 148 SMs and one half
+// empty.  Every wait is bounded and reports in error_word.
 #include "microscaled.cuh"
 
 namespace tib {
@@ -26,9 +27,9 @@ template <int NT> struct MtShape {
   static constexpr int kPerSm = NT <= 32 ? 2 : 1;                                // blocks of an SM
   static constexpr int kStorers = NT >= 128 ? 8 : 4, kThreads = 64 + 32 * kStorers, kCols = NT / (kStorers / 4);      // (columns of a storer)
   static constexpr int kTurn = NT >= 128 ? 16 : 8;                               // columns that it takes at a time
-  // Tensor memory: accumulators (two; one where a block has one tile, as it has of shared ones), then 32 columns of scales a stage.  At most:
+  // Tensor memory: accumulators (two; one of a shared tile, which is a block's only one), then 32 columns of scales a stage.  At most:
   static constexpr uint32_t tmem_cols(int splits) { return (splits > 1 ? 256 : 512) / kPerSm; }
-  static constexpr uint32_t scale_cols(int splits) { return splits > 1 ? NT : 2 * NT; }
+  __host__ __device__ static constexpr uint32_t scale_cols(int splits) { return splits > 1 ? NT : 2 * NT; }
   static constexpr int stages(int splits) { return (tmem_cols(splits) - scale_cols(splits)) / 32 < kMtMaxStages ? (tmem_cols(splits) - scale_cols(splits)) / 32 : kMtMaxStages; }
   static constexpr uint32_t kStage = kMtWBytes + NT * kMsStepBytes + 2 * kMsStepScales;
 };
@@ -66,7 +67,7 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
   static_assert(8 * (2 * kMtMaxStages + 5) + 8 <= kMtBarBytes, "the barriers' share of shared memory");
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem_gen + (tmem_slot - base));
   float* red = reinterpret_cast<float*>(smem_gen + (bars - base) + kMtBarBytes);         // [splits][NT][128 / splits + 4] sums
-  float* tile_factors = red + mt_red_floats<NT>(splits);                                 // [2][NT][2] what a row's sums are multiplied by (ms_row_factors), of two tiles in turn
+  float* tile_factors = red + mt_red_floats<NT>(splits);                                 // [2][NT][2] what a row's sums are multiplied by (ms_row_scales), of two tiles in turn
   int* tiles_before = reinterpret_cast<int*>(tile_factors + 4 * NT);                     // [experts + 1] where rows are sorted, and
   int* first_row = tiles_before + a.experts + 1;                                         // [experts + 1] their offsets
 
@@ -208,7 +209,7 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
         }
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         const uint32_t stage = base + s * S::kStage, scales = stage + kMtWBytes + NT * kMsStepBytes;
-        const uint32_t w_src = umma_low_k128(stage), x_src = w_src + (kMtWBytes >> 4), columns = tmem_base + a.scale_cols + 32 * s;
+        const uint32_t w_src = umma_low_k128(stage), x_src = w_src + (kMtWBytes >> 4), columns = tmem_base + S::scale_cols(splits) + 32 * s;
         if (leader) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) ms_copy_scales<1>(columns + 4 * k, scales + kMsChunkBytes * k);      // (four of w, four of the rows)
@@ -264,8 +265,11 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
       const float factor = a.w_factors[(size_t)m.expert * a.N + min(feature, a.N - 1)];
       float2* factors = reinterpret_cast<float2*>(tile_factors) + b * NT;
       if constexpr (MAKE) {
-        if (own_run == 0 && own_row < m.rows) factors[own_row] = ms_row_factors(r, 1.f);
-      } else if (et < m.rows) factors[et] = ms_row_factors(a.x.factors[m.first + et], a.row_scale ? a.row_scale[bs_pair(a.order, m.first + et, a.M)] : 1.f);
+        if (own_run == 0 && own_row < m.rows) factors[own_row] = make_float2(r, 1.f);
+      } else if (et < m.rows) {
+        factors[et] = make_float2(a.x.factors[m.first + et], 1.f);
+        if (a.row_scale) factors[et] = ms_row_scales(a.x.factors[m.first + et], a.row_scale[bs_pair(a.order, m.first + et, a.M)]);
+      }
       asm volatile("bar.sync 1, %0;\n" ::"r"(32 * S::kStorers) : "memory");      // (the last tile but one is finished: its factors have been read)
       if constexpr (MAKE) {
         const __nv_bfloat16* src = a.made + own_row * a.ld_made;
@@ -324,7 +328,8 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
           float s[S::kTurn];
 #pragma unroll
           for (int j = 0; j < S::kTurn; ++j) {
-            s[j] = ms_scaled(__uint_as_float(v[j]), factor, factors[min(c + j, m.rows - 1)]);
+            const float2 f = factors[min(c + j, m.rows - 1)];
+            s[j] = __uint_as_float(v[j]) * factor * f.x * f.y;
           }
           if (!ok) return;
           if constexpr (kGated) {
@@ -378,8 +383,8 @@ microscaled_tcgen05_kernel(const __grid_constant__ MsArgs a, TO* __restrict__ y,
               u += from[r * NT * stride + kGated];
             }
           const float2 f = factors[c];
-          g = ms_scaled(g, g_factor, f);
-          u = ms_scaled(u, u_factor, f);
+          g = g * g_factor * f.x * f.y;
+          u = u * u_factor * f.x * f.y;
           y[(size_t)(m.first + c) * ldy + out] = from_f32<TO>(mt_act<ACT>(g, u, a));
         }
       }
@@ -413,9 +418,8 @@ static int mt_splits(int64_t tiles, int steps, int M, int blocks) {
   return steps < 4 ? 1 : tiles * 4 <= blocks ? 4 : tiles * 2 <= blocks ? 2 : 1;
 }
 
-// How a product runs: blocks in the grid, those that share a tile, steps of a block at most, stages of its ring; where its scales begin in tensor memory, and what a
-// block takes of that and of shared memory.
-struct MtPlan { int grid, splits, steps, stages, scale_cols; uint32_t tmem_cols, smem; };
+// How a product runs: blocks in the grid, those that share a tile, steps of a block at most, stages of its ring; what a block takes of tensor memory and of shared memory.
+struct MtPlan { int grid, splits, steps, stages; uint32_t tmem_cols, smem; };
 template <int NT> static int mt_plan(int M, int N, int steps, int experts, MtPlan& p) {      // experts: 0 for one matrix
   using S = MtShape<NT>;
   constexpr int kBlocks = 148 * S::kPerSm;
@@ -427,9 +431,8 @@ template <int NT> static int mt_plan(int M, int N, int steps, int experts, MtPla
   p.steps = (int)(most < 0x7fffffff ? most : 0x7fffffff);
   p.stages = 1;
   while (p.stages < S::stages(p.splits) && p.stages < p.steps && mt_smem<NT>(p.stages + 1, p.splits, experts) <= (S::kPerSm > 1 ? 113u * 1024 : (uint32_t)kMostSmem)) ++p.stages;
-  p.scale_cols = (p.grid == tiles * p.splits ? 1 : 2) * NT;
   p.tmem_cols = p.splits > 1 ? 128 : 32;      // (in clusters: see smem_for_tmem)
-  while (p.tmem_cols < (uint32_t)(p.scale_cols + 32 * p.stages)) p.tmem_cols *= 2;
+  while (p.tmem_cols < S::scale_cols(p.splits) + 32 * p.stages) p.tmem_cols *= 2;
   p.smem = smem_for_tmem(mt_smem<NT>(p.stages, p.splits, experts), p.tmem_cols);
   return TIB_OK;
 }
@@ -445,7 +448,6 @@ static int launch_mt(MsArgs& a, void* y, int64_t ldy, cudaStream_t stream) {
   if (rc != TIB_OK) return rc;
   a.stages = plan.stages;
   a.tmem_cols = (int)plan.tmem_cols;
-  a.scale_cols = plan.scale_cols;
   auto kern = microscaled_tcgen05_kernel<NT, ACT, TO, MAKE>;
   static bool allowed[64];      // (by device: the attribute belongs to its context)
   int device = 0;

@@ -342,8 +342,8 @@ __global__ void quantized_norm_kernel(const QnArgs a) {
   }
 }
 
-// Rows of more than 8,192 columns, whose 32 to 64 KB beside a kernel's own arrays are more than the 48 KB that it has without asking: asked for once a device (the
-// attribute belongs to its context), whatever a row's width.
+// Rows of more than 8,192 columns take 33 to 64 KB, and the kernel's own arrays beside them: above the 48 KB that it has without asking from 12,036 columns on.  It asks once a
+// device (the attribute belongs to its context), whatever the row's width.
 template <typename T, bool BYTES>
 static int qn_allow_smem(void (*kern)(const QnArgs, int)) {
   static bool allowed[64];

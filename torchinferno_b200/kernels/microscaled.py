@@ -8,7 +8,8 @@ code(n, k) * S[n, k // 16] * f.  The rows x [M, K] of a product are quantised on
     s = a_b / (6 r) rounded to e4m3        codes = x / (s r) rounded to e2m1, at most 6 (0 where s is 0)
     y[m, n] = r[m] f sum over b of s[m, b] S[n, b] (sum over run b of code_x[m, k] code_w[n, k])
 
-All rounding is to nearest, ties to even, of the exact quotient: codes are the same on any machine.  Sums have 32 bits, y is rounded once.  A row
+All rounding is to nearest, ties to even, of the exact quotient: codes are the same on any machine.  Sums have 32 bits, y is rounded once, and whatever f and r
+are it is lost only where it is beyond 32 bits itself (with a factor for each pair too, :func:`ops.moe_expert_product`, from 2^-50 to 2^50 in size or 0).  A row
 that holds an infinity or a NaN makes its whole output row NaN.  A row's codes are its own: they do not depend on the rows beside it.
 
 There is no backward pass: this is an inference engine's weight format.
@@ -31,6 +32,8 @@ SCALE_DTYPE = torch.float8_e4m3fn
 VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 BORDERS = (0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)       # (on a border the even code is taken: the one above 0.75, 1.75 and 3.5)
 LARGEST = 6.0 * 448.0
+ORDINARY = (2.0 ** -100, 2.0 ** 70)      # factors of matrices that every kernel takes; others' products run on pairs of SMs,
+FAR_EXPERTS = 223                        # which take so many experts
 _OUT_DTYPES = (torch.bfloat16, torch.float32)
 
 
@@ -184,14 +187,15 @@ def add_rmsnorm(delta: torch.Tensor | None, residual: torch.Tensor, weight: torc
 # ------------------------------------------------------------------------------------------------ weights
 class Tiles:
     """Matrices of one size as the kernels read them: ``codes`` [matrices, tiles of 128 rows, steps of 256 columns, 128, 128 bytes (pieces of 16 swizzled)], ``scales``
-    [matrices, tiles, steps, 2048 bytes] and ``factors`` [matrices, N]; ``paired``: the matrices' rows are (gate i, up i)."""
-    __slots__ = ("codes", "scales", "factors", "count", "features", "columns", "paired", "device_index", "numbers")
+    [matrices, tiles, steps, 2048 bytes] and ``factors`` [matrices, N]; ``paired``: the matrices' rows are (gate i, up i); ``far``: a factor
+    is outside ``ORDINARY`` (csrc/microscaled.cuh)."""
+    __slots__ = ("codes", "scales", "factors", "count", "features", "columns", "paired", "far", "device_index", "numbers")
 
-    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, factors: torch.Tensor, columns: int, paired: bool) -> None:
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, factors: torch.Tensor, columns: int, paired: bool, far: bool) -> None:
         self.codes, self.scales, self.factors, self.count, self.features, self.columns, self.paired = codes, scales, factors, codes.shape[0], factors.shape[1], columns, paired
-        self.device_index = codes.get_device()
+        self.far, self.device_index = far, codes.get_device()
         # (what a product is told of them)
-        self.numbers = (codes.data_ptr(), scales.data_ptr(), factors.data_ptr(), int(paired), self.features, columns, self.count)
+        self.numbers = (codes.data_ptr(), scales.data_ptr(), factors.data_ptr(), int(paired) + 2 * far, self.features, columns, self.count)
 
 
 def _laid_out(stacks: Sequence[Sequence[MicroscaledMatrix]], paired: bool) -> Tiles:
@@ -208,13 +212,15 @@ def _laid_out(stacks: Sequence[Sequence[MicroscaledMatrix]], paired: bool) -> Ti
     codes = torch.zeros((len(stacks), tiles * TILE, steps * (STEP // 2)), dtype=torch.uint8, device=device)
     scales = torch.zeros((len(stacks), tiles * TILE, steps * (STEP // RUN)), dtype=torch.uint8, device=device)
     factors = torch.empty((len(stacks), features), dtype=torch.float32, device=device)
-    first = 0
+    first, checks = 0, []
     for j, height in enumerate(heights):      # (all stacks' j-th matrices at once)
         at = slice(j, features, 2) if paired else slice(first, first + height)
         part = [stack[j] for stack in stacks]
         codes[:, at, :part[0].codes.shape[1]] = torch.stack([m.codes for m in part]) if len(part) > 1 else part[0].codes
         scales[:, at, :part[0].scales.shape[1]] = torch.stack([m.scales.view(torch.uint8) for m in part]) if len(part) > 1 else part[0].scales.view(torch.uint8)
-        factors[:, at] = torch.stack([m.factor.reshape(1) for m in part])
+        factors[:, at] = of_part = torch.stack([m.factor.reshape(1) for m in part])
+        # (whether a factor is far: not that of a matrix of zeros)
+        checks.append(((of_part.abs() < ORDINARY[0]) | (of_part.abs() > ORDINARY[1]))[:, 0] & of_part.isfinite()[:, 0] & (of_part != 0)[:, 0] & scales[:, at].flatten(1).any(1))
         first += height
     if columns % 2:      # (the half byte behind the last column)
         codes[:, :, columns // 2] &= 15
@@ -224,9 +230,12 @@ def _laid_out(stacks: Sequence[Sequence[MicroscaledMatrix]], paired: bool) -> Ti
     # (row 32 a + b of a tile, run 4 c + d of a step: to [c][b][a][d])
     scales = scales.view(len(stacks), tiles, 4, 32, steps, 4, 4).permute(0, 1, 4, 5, 3, 2, 6).contiguous()
     # (The products ask for their weights ahead of the kernels before them in the stream: this waits until all of the above is there.)
-    if int(scales.max()) > 0x7e:
+    largest, far = torch.stack([scales.max().to(torch.int64), torch.stack(checks).any().to(torch.int64)]).tolist()
+    if largest > 0x7e:
         raise ValueError("the scales of a 4-bit matrix must be numbers, and none of them negative")
-    return Tiles(codes.view(len(stacks), tiles, steps, TILE, -1), scales.view(len(stacks), tiles, steps, -1), factors, columns, paired)
+    if far and len(stacks) > FAR_EXPERTS:
+        raise ValueError(f"factors of 4-bit matrices outside {ORDINARY[0]:g} .. {ORDINARY[1]:g} are not taken of more than {FAR_EXPERTS} experts")
+    return Tiles(codes.view(len(stacks), tiles, steps, TILE, -1), scales.view(len(stacks), tiles, steps, -1), factors, columns, paired, bool(far))
 
 
 _NO_ROWS = (0, 0, 0)
@@ -237,7 +246,7 @@ def _product(x: "torch.Tensor | MicroscaledRows", tiles: Tiles, y: torch.Tensor,
     # (fresh: y is memory that x is not)
     if isinstance(x, MicroscaledRows):
         x, rows = None, (x.codes_at, x.scales_at, x.factors_at)
-    elif (fresh and y.shape[0] <= GROUP and x.dtype is torch.bfloat16 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 and
+    elif (fresh and not tiles.far and y.shape[0] <= GROUP and x.dtype is torch.bfloat16 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 and
           _makes(y.shape[0], tiles.features, tiles.columns)):
         rows = _NO_ROWS
     else:
@@ -287,7 +296,7 @@ class MicroscaledWeight:
         view = object.__new__(MicroscaledWeight)
         view.epilogue, view.in_features, view.out_features = "none", self.in_features, stop - start
         at = slice(start // TILE, _count(stop, TILE))
-        view.tiles = Tiles(self.tiles.codes[:, at], self.tiles.scales[:, at], self.tiles.factors[:, start:stop], self.in_features, False)
+        view.tiles = Tiles(self.tiles.codes[:, at], self.tiles.scales[:, at], self.tiles.factors[:, start:stop], self.in_features, False, self.tiles.far)
         return view
 
     def _run(self, x: "torch.Tensor | MicroscaledRows", act: str, width: int, out_dtype: torch.dtype | None, out: torch.Tensor | None,

@@ -1215,8 +1215,9 @@ def moe_expert_product(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor, offset
     ``x_by_pair``: the source of sorted row s is token order[s] // top, else row s itself.  ``act="glu_clamp"``: the rows
     of ``w`` are (gate i, up i) pairs and y has N / 2 columns: g * sigmoid(alpha g) * (u + 1) with g = min(g, limit),
     u = clamp(u, -limit, limit); ``act="swiglu"``: silu(g) * u over the same pairs.  ``row_scale``: one fp32 factor per
-    (token, choice) pair, or None.  ``w`` may also be a :class:`~torchinferno_b200.kernels.block_scaled.BlockScaledExperts`."""
-    if not isinstance(w, torch.Tensor):      # (experts in 8-bit blocks: block_scaled.BlockScaledExperts)
+    (token, choice) pair, or None.  ``w`` may also be a :class:`~torchinferno_b200.kernels.block_scaled.BlockScaledExperts` or a
+    :class:`~torchinferno_b200.kernels.microscaled.MicroscaledExperts`, whose rows are quantised on the way."""
+    if not isinstance(w, torch.Tensor):      # (experts in 8-bit blocks or 4-bit codes)
         return w.product(x, y, offsets, order, top, x_by_pair=x_by_pair, act=act, limit=limit, alpha=alpha, row_scale=row_scale,
                          error_word=error_word)
     _rows_of(x, "x"), _need(w, "w"), _rows_of(y, "y")
