@@ -17,6 +17,7 @@ There is no backward pass: this is an inference engine's weight format.
 from __future__ import annotations
 
 import functools
+import math
 from dataclasses import dataclass
 from typing import Sequence
 
@@ -212,15 +213,14 @@ def _laid_out(stacks: Sequence[Sequence[MicroscaledMatrix]], paired: bool) -> Ti
     codes = torch.zeros((len(stacks), tiles * TILE, steps * (STEP // 2)), dtype=torch.uint8, device=device)
     scales = torch.zeros((len(stacks), tiles * TILE, steps * (STEP // RUN)), dtype=torch.uint8, device=device)
     factors = torch.empty((len(stacks), features), dtype=torch.float32, device=device)
-    first, checks = 0, []
+    first, found = 0, []
     for j, height in enumerate(heights):      # (all stacks' j-th matrices at once)
         at = slice(j, features, 2) if paired else slice(first, first + height)
         part = [stack[j] for stack in stacks]
         codes[:, at, :part[0].codes.shape[1]] = torch.stack([m.codes for m in part]) if len(part) > 1 else part[0].codes
         scales[:, at, :part[0].scales.shape[1]] = torch.stack([m.scales.view(torch.uint8) for m in part]) if len(part) > 1 else part[0].scales.view(torch.uint8)
         factors[:, at] = of_part = torch.stack([m.factor.reshape(1) for m in part])
-        # (whether a factor is far: not that of a matrix of zeros)
-        checks.append(((of_part.abs() < ORDINARY[0]) | (of_part.abs() > ORDINARY[1]))[:, 0] & of_part.isfinite()[:, 0] & (of_part != 0)[:, 0] & scales[:, at].flatten(1).any(1))
+        found.append(of_part.view(-1))
         first += height
     if columns % 2:      # (the half byte behind the last column)
         codes[:, :, columns // 2] &= 15
@@ -230,12 +230,14 @@ def _laid_out(stacks: Sequence[Sequence[MicroscaledMatrix]], paired: bool) -> Ti
     # (row 32 a + b of a tile, run 4 c + d of a step: to [c][b][a][d])
     scales = scales.view(len(stacks), tiles, 4, 32, steps, 4, 4).permute(0, 1, 4, 5, 3, 2, 6).contiguous()
     # (The products ask for their weights ahead of the kernels before them in the stream: this waits until all of the above is there.)
-    largest, far = torch.stack([scales.max().to(torch.int64), torch.stack(checks).any().to(torch.int64)]).tolist()
+    *values, largest = torch.cat([*found, scales.max().to(torch.float32).view(1)]).tolist()
     if largest > 0x7e:
         raise ValueError("the scales of a 4-bit matrix must be numbers, and none of them negative")
+    ordered = [stack[j] for j in range(len(heights)) for stack in stacks]      # (a factor is far where it matters: not that of a matrix of zeros)
+    far = any(not ORDINARY[0] <= abs(f) <= ORDINARY[1] and f != 0 and math.isfinite(f) and bool(m.scales.view(torch.uint8).any()) for f, m in zip(values, ordered))
     if far and len(stacks) > FAR_EXPERTS:
         raise ValueError(f"factors of 4-bit matrices outside {ORDINARY[0]:g} .. {ORDINARY[1]:g} are not taken of more than {FAR_EXPERTS} experts")
-    return Tiles(codes.view(len(stacks), tiles, steps, TILE, -1), scales.view(len(stacks), tiles, steps, -1), factors, columns, paired, bool(far))
+    return Tiles(codes.view(len(stacks), tiles, steps, TILE, -1), scales.view(len(stacks), tiles, steps, -1), factors, columns, paired, far)
 
 
 _NO_ROWS = (0, 0, 0)
