@@ -206,7 +206,7 @@ TIB_API int tib_microscaled_product(const void* w, const void* w_scales, const f
   return ms_product_tcgen05(a, act, y, y_dtype, ldy, stream);
 }
 
-// How a product of M rows with one matrix (experts 0) or sorted by expert runs: {rows of a tile at most (256: on pairs of SMs), blocks that share a tile, steps of a block at
+// How a product of M rows with one matrix (experts 0) or sorted by expert runs where its factors are ordinary: {rows of a tile at most (256: on pairs of SMs), blocks that share a tile, steps of a block at
 // most, stages of its ring}.
 TIB_API int tib_microscaled_plan(int M, int N, int K, int experts, int* plan) {
   if (!plan || M < 1 || N < 1 || K < 1 || experts < 0) return TIB_E_ARG;

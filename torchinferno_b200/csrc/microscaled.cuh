@@ -178,8 +178,8 @@ struct MsArgs {
 //   f from 2^-100 to 2^70 (or 0), which leaves every sum a normal number: f first, then what ms_row_scales gives.  (In the fewest steps: microscaled_tcgen05.cu.  With what
 //   follows in their place 8 rows 1,024 -> 1,024 took 4.2 us for 3.95, with a branch for other factors as much.)
 //   any f: what ms_row_factors gives, ahead of f and behind it (microscaled_2cta.cu, where it costs nothing; matrices with other factors run there whatever their rows are).
-// r q is a power of two more or less where it is a normal number, and comes after f as one.  Where it is too small, or too large, so is q alone, and the product with r
-// alone leaves the range only where the one with both does.
+// Behind an ordinary f: r q, exact where it is a normal number.  Where it is too small for one, q is less than 1 (r is 2^-126 or more), and where it is too large, more
+// (r is 2^117 or less): then r comes first, and what leaves the range with it does so with both.
 __device__ __forceinline__ float2 ms_row_scales(float r, float q) {
   const float both = r * q;
   return (fabsf(both) >= 0x1p-126f && fabsf(both) < INFINITY) || q == 0.f ? make_float2(both, 1.f) : make_float2(r, q);

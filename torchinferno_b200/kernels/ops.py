@@ -1388,8 +1388,8 @@ def microscaled_product(weight: tuple, x: torch.Tensor | None, rows: tuple, y: t
 def microscaled_makes(rows: int, features: int, columns: int) -> bool:
     """Whether a product with one matrix makes the codes of so many rows (bfloat16, on 16 bytes as their stride) in its own kernel.  The rows may not lie where ``y`` does."""
     answer = ctypes.c_int()
-    _check("microscaled_makes", lib().tib_microscaled_makes(rows, features, columns, ctypes.addressof(answer)))
-    count_launches(-1)
+    if lib().tib_microscaled_makes(rows, features, columns, ctypes.addressof(answer)):
+        raise KernelError(f"microscaled_makes: no product of {rows} rows with {features} features of {columns} columns")
     return bool(answer.value)
 
 
