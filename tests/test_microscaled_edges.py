@@ -180,6 +180,15 @@ def test_operands_of_a_norm_that_overlap_are_refused():
         assert lib.tib_quantized_norm(*{**norm, **wrong}.values()) == -8, wrong
 
 
+def test_a_parameter_is_quantised_as_its_numbers():
+    g = torch.Generator().manual_seed(1)
+    w = torch.randn(40, 33, generator=g)
+    for given in (torch.nn.Parameter(w.clone()), w.double(), w.t().contiguous().t()):
+        made, want = quantize_matrix(given), quantize_matrix(w)
+        assert torch.equal(made.codes, want.codes) and torch.equal(made.scales.view(torch.uint8), want.scales.view(torch.uint8)) and made.factor == want.factor
+        assert not made.factor.requires_grad and not made.scales.requires_grad and MicroscaledWeight(made).tiles.numbers[3] == 0
+
+
 # ------------------------------------------------------------------------------------------------ factors that are far from 1
 def with_factor(n, factor, zeros=False):
     matrix = random_matrix(n, 32, n, factor=1.0)

@@ -100,6 +100,7 @@ def quantize_matrix(matrix: torch.Tensor) -> MicroscaledMatrix:
     if matrix.dim() != 2 or 0 in matrix.shape:
         raise ValueError(f"quantize_matrix takes a non-empty matrix, got {tuple(matrix.shape)}")
     n, k = matrix.shape
+    matrix = matrix.detach()
     largest = matrix.abs().amax().to(torch.float32)
     factor = (largest / torch.full_like(largest, LARGEST)).clamp(min=torch.finfo(torch.float32).tiny)      # (a number of Python's would be a product with its inverse on a GPU)
     codes = torch.empty((n, _count(k, 2)), dtype=torch.uint8, device=matrix.device)
